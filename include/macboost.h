@@ -79,6 +79,10 @@ typedef struct mbk_context mbk_context;
 
 /* One device + one stream.  Replaces MetalEngine.init (MetalEngine.swift:43-65). */
 int mbk_context_create(int32_t device, mbk_context **out, char **err);
+/* No counterpart in the reference: a context whose calls queue on the caller's
+ * stream (a hipStream_t of `device`; NULL: its default stream), in order with the
+ * caller's own work there.  The stream must outlive the context. */
+int mbk_context_create_on(int32_t device, void *stream, mbk_context **out, char **err);
 void mbk_context_destroy(mbk_context *ctx);
 int mbk_device_alloc(mbk_context *ctx, size_t bytes, void **out, char **err);
 void mbk_device_free(mbk_context *ctx, void *ptr);
@@ -275,6 +279,92 @@ int mbk_treeshap(mbk_context *ctx, const int32_t *feature, const float *threshol
                  const uint32_t *mask, int32_t num_trees, int32_t nodes_per_tree,
                  float base_score, int32_t data_bins, const float *x, int64_t rows, int32_t cols,
                  float *out, char **err);
+
+/* ---- a loss over many classes.  No counterpart in the reference, whose softmax
+ * objective keeps every class's score and grows a tree for each (3..128 classes).
+ * With more, a model boosts dim outputs h and scores class v by h . w[v] + bias[v];
+ * these calls give each row's loss and what the next boosting round and the
+ * next w need, without keeping the rows x classes scores:
+ *   z = h . w[v] + bias[v],  lse = log sum_v exp z
+ *   loss = weight * (lse - z of the row's label)
+ *   g[v] = weight * (exp(z - lse) - [v is the label])
+ *   dh = sum_v g[v] w[v],  dw[v] = sum over rows g[v] h,  dbias[v] = sum over rows g[v]
+ * All arrays are device memory.  h: [rows] rows of dim elements, h_stride
+ * apart; w: [classes], w_stride apart; dh and dw lie as h and w do, are of the same
+ * type and may be NULL, as may dbias [classes]; what lies between their rows
+ * stays as it is.  labels, weights (NULL: 1), loss and lse: [rows]; bias: [classes] or
+ * NULL.  Outputs must not overlap inputs.
+ * A row whose label is outside [0, classes) or whose weight is 0 is left out: its
+ * loss and dh are 0, and what its h holds reaches nothing but its own lse.  A class
+ * whose bias is -INFINITY is not offered: what its w holds reaches nothing, its dw
+ * and dbias are 0.  With no class offered every lse is -INFINITY and every row is out.
+ * Other h, w and bias must be finite for finite results.  Sums are f32; bf16 operands
+ * are multiplied exactly, with g rounded to bf16 for dh, dw and dbias, f32 operands to 22
+ * bits.  The results do not depend on the call, bit for bit.
+ * To boost output j with them: mbk_quantize with objective 0, preds = dh's column j
+ * and labels of 0. */
+enum { MBK_F32 = 0, MBK_BF16 = 1 };
+typedef struct {
+    int64_t rows;                /* 0..2^31-256 */
+    int64_t classes;             /* 1..2^31-256 */
+    int32_t dim;                 /* 1..2^20 */
+    int32_t type;                /* of h, w, dh, dw: MBK_F32 or MBK_BF16 */
+    int64_t h_stride, w_stride;  /* elements from row to row, >= dim */
+} mbk_xent_shape;
+int mbk_xent(mbk_context *ctx, const mbk_xent_shape *shape, const void *h, const void *w,
+             const float *bias, const int32_t *labels, const float *weights, float *loss,
+             float *lse, char **err);
+int mbk_xent_grad(mbk_context *ctx, const mbk_xent_shape *shape, const void *h, const void *w,
+                  const float *bias, const int32_t *labels, const float *weights, float *loss,
+                  float *lse, void *dh, void *dw, float *dbias, char **err);
+
+/* ---- rows sorted by expert and back.  No counterpart in the reference.  A model of
+ * several boosters (one a segment, or the k best of a gate) sends each row to k of
+ * them; a booster predicts, explains or trains on its rows as one matrix, and the rows
+ * get the weighted sum of their boosters' outputs.  All arrays are device memory.
+ *
+ * mbk_expert_sort: assignment a = row * k + j goes to expert[a]; ids outside
+ * [0, experts) are dropped.  Expert e's assignments get the slots
+ * offsets[e] .. offsets[e+1], in ascending order of a; source[slot] = a, slot[a] = its
+ * slot or -1, and source is -1 behind the last slot taken.
+ * mbk_expert_gather: sorted[slot] = x[row].
+ * mbk_expert_combine: out[row] = sum over j, ascending, of weights[row][j] *
+ * sorted[slot[row][j]], a dropped one adding nothing (0 with none left); weights NULL:
+ * 1, which also is mbk_expert_gather's gradient.
+ * mbk_expert_combine_grad: d_sorted[slot[row][j]] = weights[row][j] * dout[row] and
+ * d_weights[row][j] = dout[row] . sorted[slot[row][j]], 0 for a dropped one.
+ * Sums are f32, rounded once.  What lies behind the last slot taken in sorted and
+ * d_sorted is neither read nor written. */
+typedef struct {
+    int64_t rows;
+    int32_t k;                   /* rows * k at most 2^31-256 */
+    int32_t experts;             /* 1..8192 */
+    const int32_t *expert;       /* [rows][k] */
+    int32_t *offsets;            /* [experts + 1], written by mbk_expert_sort, */
+    int32_t *source;             /* [rows * k]     read by the others */
+    int32_t *slot;               /* [rows][k] */
+} mbk_expert_plan;
+/* A matrix of the rows, x, out or dout: element (row, f) at
+ * data[row * row_stride + f * col_stride].  The sorted matrix that goes with it is of
+ * the same type, [rows * k] rows of cols elements, or with blocked != 0 each expert's
+ * rows as one feature-major block [cols][n], n = offsets[e+1] - offsets[e], at element
+ * cols * offsets[e]: what mbk_predict_forest, mbk_treeshap and mbk_fit take, and
+ * mbk_predict_forest's outputs one after another give. */
+typedef struct {
+    void *data;
+    int64_t row_stride, col_stride;
+    int32_t cols;
+    int32_t type;                /* MBK_F32 or MBK_BF16 */
+    int32_t blocked;
+} mbk_expert_matrix;
+int mbk_expert_sort(mbk_context *ctx, const mbk_expert_plan *plan, char **err);
+int mbk_expert_gather(mbk_context *ctx, const mbk_expert_plan *plan, const mbk_expert_matrix *x,
+                      void *sorted, char **err);
+int mbk_expert_combine(mbk_context *ctx, const mbk_expert_plan *plan, const void *sorted,
+                       const float *weights, const mbk_expert_matrix *out, char **err);
+int mbk_expert_combine_grad(mbk_context *ctx, const mbk_expert_plan *plan,
+                            const mbk_expert_matrix *dout, const void *sorted,
+                            const float *weights, void *d_sorted, float *d_weights, char **err);
 
 /* fitImpl (Booster.swift:445-1701) over raw features already in device
  * memory: x is read as x[i*cols + f] when row_major != 0, else x[f*rows + i];

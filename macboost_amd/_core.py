@@ -66,6 +66,29 @@ class MbkTreeOut(ctypes.Structure):
     _fields_ = [("split", _P), ("leaf", _P), ("gain", _P), ("cover", _P), ("mask", _P)]
 
 
+class MbkXentShape(ctypes.Structure):
+    """mbk_xent_shape (include/macboost.h)."""
+    _fields_ = [("rows", ctypes.c_int64), ("classes", ctypes.c_int64), ("dim", ctypes.c_int32),
+                ("type", ctypes.c_int32), ("h_stride", ctypes.c_int64),
+                ("w_stride", ctypes.c_int64)]
+
+
+class MbkExpertPlan(ctypes.Structure):
+    """mbk_expert_plan: device pointers of a sort by expert."""
+    _fields_ = [("rows", ctypes.c_int64), ("k", ctypes.c_int32), ("experts", ctypes.c_int32),
+                ("expert", _P), ("offsets", _P), ("source", _P), ("slot", _P)]
+
+
+class MbkExpertMatrix(ctypes.Structure):
+    """mbk_expert_matrix: the rows' matrix and the layout of the sorted one."""
+    _fields_ = [("data", _P), ("row_stride", ctypes.c_int64), ("col_stride", ctypes.c_int64),
+                ("cols", ctypes.c_int32), ("type", ctypes.c_int32), ("blocked", ctypes.c_int32)]
+
+
+F32, BF16 = 0, 1         # MBK_F32, MBK_BF16
+_XENT_P = ctypes.POINTER(MbkXentShape)
+_PLAN_P = ctypes.POINTER(MbkExpertPlan)
+_MATRIX_P = ctypes.POINTER(MbkExpertMatrix)
 _SHAPE_P = ctypes.POINTER(MbkTreeShape)
 _SPLIT_P = ctypes.POINTER(MbkSplitParams)
 
@@ -110,6 +133,8 @@ def _configure(l):
     # kernel seam
     l.mbk_context_create.restype = ctypes.c_int
     l.mbk_context_create.argtypes = [ctypes.c_int32, ctypes.POINTER(_P), _c_char_pp]
+    l.mbk_context_create_on.restype = ctypes.c_int
+    l.mbk_context_create_on.argtypes = [ctypes.c_int32, _P, ctypes.POINTER(_P), _c_char_pp]
     l.mbk_context_destroy.restype = None
     l.mbk_context_destroy.argtypes = [_P]
     l.mbk_device_alloc.restype = ctypes.c_int
@@ -149,7 +174,13 @@ def _configure(l):
                                ctypes.c_int64, _P, _P, _P, MbkTreeOut, _P, _c_char_pp]),
             ("mbk_treeshap", [_P, _P, _P, _P, _P, _P, _P, ctypes.c_int32, ctypes.c_int32,
                               ctypes.c_float, ctypes.c_int32, _P, ctypes.c_int64, ctypes.c_int32,
-                              _P, _c_char_pp])):
+                              _P, _c_char_pp]),
+            ("mbk_xent", [_P, _XENT_P, _P, _P, _P, _P, _P, _P, _P, _c_char_pp]),
+            ("mbk_xent_grad", [_P, _XENT_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _c_char_pp]),
+            ("mbk_expert_sort", [_P, _PLAN_P, _c_char_pp]),
+            ("mbk_expert_gather", [_P, _PLAN_P, _MATRIX_P, _P, _c_char_pp]),
+            ("mbk_expert_combine", [_P, _PLAN_P, _P, _P, _MATRIX_P, _c_char_pp]),
+            ("mbk_expert_combine_grad", [_P, _PLAN_P, _MATRIX_P, _P, _P, _P, _P, _c_char_pp])):
         getattr(l, name).restype = ctypes.c_int
         getattr(l, name).argtypes = args
     l.mbk_fit.restype = ctypes.c_void_p
@@ -227,11 +258,12 @@ EXPORTED = (
     "macboost_feature_importance", "macboost_predict_contrib", "macboost_save", "macboost_load",
     "macboost_num_trees", "macboost_num_features", "macboost_best_iteration",
     "macboost_warnings", "macboost_free", "macboost_free_string",
-    "mbk_context_create", "mbk_context_destroy", "mbk_device_alloc", "mbk_device_free",
+    "mbk_context_create", "mbk_context_create_on", "mbk_context_destroy", "mbk_device_alloc", "mbk_device_free",
     "mbk_copy_to_device", "mbk_copy_to_host", "mbk_synchronize", "mbk_quantile_edges", "mbk_bin_data", "mbk_quantize",
     "mbk_node_hist_split", "mbk_predict_forest", "mbk_fit", "mbk_tree_begin", "mbk_hist_build",
     "mbk_hist_subtract", "mbk_find_splits", "mbk_decide_level", "mbk_route", "mbk_final_leaves",
-    "mbk_grow_tree", "mbk_treeshap", "mbk_node_hist_split_noalloc",
+    "mbk_xent", "mbk_xent_grad", "mbk_expert_sort", "mbk_expert_gather", "mbk_expert_combine",
+    "mbk_expert_combine_grad", "mbk_grow_tree", "mbk_treeshap", "mbk_node_hist_split_noalloc",
     "mbx_trainer_create", "mbx_trainer_grow", "mbx_trainer_profile", "mbx_trainer_hist_stats",
     "mbx_trainer_level_stats", "mbx_trainer_setup_seconds", "mbx_trainer_booster", "mbx_trainer_free", "mbx_friedman",
     "mbx_version", "mbx_dataset_make", "mbx_dataset_save", "mbx_dataset_load",
@@ -543,12 +575,19 @@ class Trainer:
 
 
 class Context:
-    """Kernel seam (mbk_*): one device, one stream, device buffers."""
+    """Kernel seam (mbk_*): one device, one stream, device buffers.  With stream
+    (a hipStream_t as an integer; 0 is the device's default stream) its calls
+    queue on that stream, which must outlive the context."""
 
-    def __init__(self, device: int = 0):
+    def __init__(self, device: int = 0, stream: int | None = None):
         self.ptr = _P()
         err = ctypes.c_char_p()
-        if lib().mbk_context_create(device, ctypes.byref(self.ptr), ctypes.byref(err)) != 0:
+        if stream is None:
+            rc = lib().mbk_context_create(device, ctypes.byref(self.ptr), ctypes.byref(err))
+        else:
+            rc = lib().mbk_context_create_on(device, stream, ctypes.byref(self.ptr),
+                                             ctypes.byref(err))
+        if rc != 0:
             raise MacBoostError(_take_error(err))
         self._bufs = []
 

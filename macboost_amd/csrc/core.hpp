@@ -24,6 +24,11 @@ namespace mb {
 // The device and stream of a kernel-seam context (seam.cpp).
 int context_device(const mbk_context *ctx);
 hipStream_t context_stream(const mbk_context *ctx);
+int context_cus(const mbk_context *ctx);
+// `bytes` of the context's scratch for the operators of ops.cpp, with its device
+// current: one block that grows.  A block that a captured graph may replay on is kept
+// until the context ends, and growing under capture is refused.
+char *context_scratch(mbk_context *ctx, size_t bytes);
 
 // A named range on the ROCm tracer's marker timeline (rocprofv3
 // --marker-trace) around one phase of host work; free when no tool listens.
@@ -107,7 +112,9 @@ struct Device {
     hipStream_t stream = nullptr;
     hipStream_t copy_stream = nullptr;   // host uploads that overlap work on `stream`
     int num_cus = 0;
+    bool borrowed = false;               // `stream` is a caller's
     explicit Device(int device_id);
+    Device(int device_id, hipStream_t caller_stream);
     ~Device();
     Device(const Device &) = delete;
     Device &operator=(const Device &) = delete;
@@ -167,7 +174,6 @@ struct DevBuf {
     }
     void alloc(size_t count) {
         release();
-        n = count;
         if (!count) return;
         if (pooled) {
             ptr = static_cast<T *>(pool_alloc(count * sizeof(T), &device));
@@ -176,6 +182,7 @@ struct DevBuf {
             MB_HIP(malloc_or_trim(&p, count * sizeof(T)));
             ptr = static_cast<T *>(p);
         }
+        n = count;                   // not before: a failed call leaves the buffer empty
     }
     void release() {
         if (ptr) {
@@ -186,6 +193,18 @@ struct DevBuf {
         n = 0;
     }
     size_t bytes() const { return n * sizeof(T); }
+};
+
+// The calling thread's current device, put back when it goes out of scope.
+struct OnDevice {
+    int before = 0;
+    explicit OnDevice(int id) {
+        MB_HIP(hipGetDevice(&before));
+        if (before != id) MB_HIP(hipSetDevice(id));
+    }
+    ~OnDevice() { (void)hipSetDevice(before); }
+    OnDevice(const OnDevice &) = delete;
+    OnDevice &operator=(const OnDevice &) = delete;
 };
 
 // Waits for a stream when it goes out of scope: declared after pooled buffers

@@ -69,6 +69,10 @@ struct Scratch {
     DevBuf<uint32_t> forest_features, forest_mark;
     DevBuf<mbk::PredNode> nodes;
     std::mutex nodes_mu;             // listing, packing and walk queued together
+    // the operators of ops.cpp (context_scratch)
+    DevBuf<char> ops;
+    std::vector<DevBuf<char>> ops_before;            // outgrown, but in a captured graph
+    bool ops_captured = false;
 };
 
 }  // namespace
@@ -204,6 +208,25 @@ mbk::LevelArgs level_args(int32_t d, bool terminal) {
     return mbk::LevelArgs{d, (uint32_t)((1u << d) - 1), 1u << d, terminal ? 1u : 0u};
 }
 
+mbk_context *make_context(std::unique_ptr<mb::Device> dev) {
+    auto c = std::make_unique<mbk_context>();
+    c->dev = std::move(dev);
+    Scratch &sc = c->scratch;
+    sc.forest_features.pooled = sc.forest_mark.pooled = sc.nodes.pooled = true;
+    sc.forest_features.alloc(mbk::PRED_INFO_WORDS);
+    sc.forest_mark.alloc(mbk::PRED_MARK_WORDS);
+    sc.nodes.alloc(PREDICT_NODES);
+    MB_HIP(hipMemsetAsync(sc.forest_mark.ptr, 0, sc.forest_mark.bytes(), c->dev->stream));
+    return c.release();
+}
+
+// `device`, if there is one.
+int device_or_throw(int device) {
+    int n = 0;
+    if (hipGetDeviceCount(&n) != hipSuccess || n <= device) throw mb::Error("No HIP GPU available");
+    return device;
+}
+
 // The histogram item list of a level must have fit the scratch: the
 // planning kernels report an overflow in the control block.
 void check_overflow(mbk_context *ctx) {
@@ -219,21 +242,46 @@ void check_overflow(mbk_context *ctx) {
 namespace mb {
 int context_device(const mbk_context *ctx) { return ctx->dev->id; }
 hipStream_t context_stream(const mbk_context *ctx) { return ctx->dev->stream; }
+int context_cus(const mbk_context *ctx) { return ctx->dev->num_cus; }
+
+char *context_scratch(mbk_context *ctx, size_t bytes) {
+    Scratch &sc = ctx->scratch;
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    MB_HIP(hipStreamIsCapturing(ctx->dev->stream, &st));
+    const bool capturing = st != hipStreamCaptureStatusNone;
+    if (sc.ops.n < bytes) {
+        need(!capturing, "the context's scratch must grow, which a captured call cannot do: "
+                         "make a call of the same sizes before the capture");
+        if (sc.ops_captured) sc.ops_before.push_back(std::move(sc.ops));
+        sc.ops_captured = false;
+        sc.ops.alloc(bytes + bytes / 8);
+    }
+    sc.ops_captured |= capturing;
+    return sc.ops.ptr;
+}
 }  // namespace mb
 
 extern "C" {
 
 int mbk_context_create(int32_t device, mbk_context **out, char **err) {
     return guarded(err, [&]() -> int {
-        auto c = std::make_unique<mbk_context>();
-        c->dev = std::make_unique<mb::Device>(device);
-        Scratch &sc = c->scratch;
-        sc.forest_features.pooled = sc.forest_mark.pooled = sc.nodes.pooled = true;
-        sc.forest_features.alloc(mbk::PRED_INFO_WORDS);
-        sc.forest_mark.alloc(mbk::PRED_MARK_WORDS);
-        sc.nodes.alloc(PREDICT_NODES);
-        MB_HIP(hipMemsetAsync(sc.forest_mark.ptr, 0, sc.forest_mark.bytes(), c->dev->stream));
-        *out = c.release();
+        *out = make_context(std::make_unique<mb::Device>(device));
+        return 0;
+    }, -1);
+}
+
+int mbk_context_create_on(int32_t device, void *stream, mbk_context **out, char **err) {
+    return guarded(err, [&]() -> int {
+        need(out != nullptr, "null argument");
+        need(device >= 0, "device must be >= 0");
+        mb::OnDevice here(device_or_throw(device));
+        hipStream_t s = static_cast<hipStream_t>(stream);
+        if (s) {
+            hipDevice_t of = device;
+            MB_HIP(hipStreamGetDevice(s, &of));
+            need(of == device, "the stream belongs to another device");
+        }
+        *out = make_context(std::make_unique<mb::Device>(device, s));
         return 0;
     }, -1);
 }

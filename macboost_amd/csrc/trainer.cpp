@@ -259,28 +259,41 @@ void pool_trim() {
     for (const CachedBlock &b : all) (void)hipFree(b.p);
 }
 
-Device::Device(int device_id) : id(device_id) {
+// The CU count, looked up once per device (a properties query costs ~1 ms).
+static int cu_count(int device_id) {
+    static std::mutex mu;
+    static int cus[64] = {};
+    std::lock_guard<std::mutex> lock(mu);
+    if (device_id < 64 && cus[device_id]) return cus[device_id];
+    int n = 0;
+    MB_HIP(hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, device_id));
+    if (device_id < 64) cus[device_id] = n;
+    return n;
+}
+
+// Makes a device current, if there is one.
+static void use_device(int device_id) {
     int n = 0;
     if (hipGetDeviceCount(&n) != hipSuccess || n <= device_id)
         throw Error("No HIP GPU available");
     MB_HIP(hipSetDevice(device_id));
+}
+
+Device::Device(int device_id) : id(device_id) {
+    use_device(device_id);
     MB_HIP(hipStreamCreateWithFlags(&stream, hipStreamNonBlocking));
     MB_HIP(hipStreamCreateWithFlags(&copy_stream, hipStreamNonBlocking));
-    // the CU count, looked up once per device (a properties query costs ~1 ms)
-    static std::mutex mu;
-    static int cus[64] = {};
-    std::lock_guard<std::mutex> lock(mu);
-    if (device_id >= 64 || !cus[device_id]) {
-        int n = 0;
-        MB_HIP(hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, device_id));
-        if (device_id >= 64) { num_cus = n; return; }
-        cus[device_id] = n;
-    }
-    num_cus = cus[device_id];
+    num_cus = cu_count(device_id);
+}
+
+Device::Device(int device_id, hipStream_t caller_stream)
+    : id(device_id), stream(caller_stream), borrowed(true) {
+    use_device(device_id);
+    num_cus = cu_count(device_id);
 }
 
 Device::~Device() {
-    if (stream) (void)hipStreamDestroy(stream);
+    if (stream && !borrowed) (void)hipStreamDestroy(stream);
     if (copy_stream) (void)hipStreamDestroy(copy_stream);
 }
 
