@@ -28,72 +28,19 @@
 
 #include "mbk.h"
 #include "ops.h"
+#include "xent.hpp"
 
 namespace mbk {
 
 namespace {
 
-typedef __attribute__((ext_vector_type(4))) unsigned int u32x4;       // 8 operands
-typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
-typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
-typedef __attribute__((ext_vector_type(4))) short i16x4;
-typedef __attribute__((ext_vector_type(16))) float f32x16;
-typedef unsigned short u16;
-
-constexpr float LOG2E = 1.44269504088896341f;
 constexpr int TILE = 128;                // rows and columns of a workgroup's product
 constexpr int LD_PAD = 128;              // operands' rows are padded to it
 constexpr float G_SCALE = 32768.0f;      // f32: |G / w| <= 1 as f16 terms
 
-// ---- control words -----------------------------------------------------------
-struct Ctl {
-    uint32_t w_max, hg_max;              // bits of the largest |W|, |w h| that is finite
-    uint32_t open;                       // a class is offered
-};
-
-__global__ void k_xent_init(Ctl *ctl) {
+__global__ void k_xent_init(XentCtl *ctl) {
     ctl->w_max = ctl->hg_max = ctl->open = 0;
 }
-
-__device__ __forceinline__ uint32_t finite_bits(float x) {
-    const uint32_t b = __float_as_uint(fabsf(x));
-    return b < 0x7F800000u ? b : 0u;
-}
-// The exponent that brings a maximum below 2^14 (0 for a maximum of 0).
-__device__ __forceinline__ int scale_exp(uint32_t max_bits) {
-    if (!max_bits) return 0;
-    const int s = 13 - ilogbf(__uint_as_float(max_bits));
-    return min(126, max(-126, s));
-}
-__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o, 64));
-    return v;
-}
-
-__device__ __forceinline__ u16 bits_of(__bf16 v) { return __builtin_bit_cast(u16, v); }
-__device__ __forceinline__ u16 bits_of(_Float16 v) { return __builtin_bit_cast(u16, v); }
-
-// x 2^s in two f16 terms.
-__device__ __forceinline__ void split_f16(float x, u16 &hi, u16 &lo) {
-    const _Float16 h = (_Float16)x;
-    hi = bits_of(h);
-    lo = bits_of((_Float16)(x - (float)h));
-}
-
-// ---- packing -------------------------------------------------------------------
-// What the kernels read: operands in rows of ld 16-bit elements, zeros behind the
-// sizes, P planes of them.
-struct Pack {
-    int64_t n, v, n_pad, v_pad;
-    int32_t d, ld;
-    Ctl *ctl;
-    u16 *h, *hg, *w;                     // planes of n_pad * ld, v_pad * ld
-    float *bias;                         // [v_pad], -inf: not offered
-    float *row_scale;                    // [n_pad], f32: 2^-s of h's row
-    int32_t *label;                      // [n_pad], -1: out
-    float *weight;                       // [n_pad], 0: out
-};
 
 template <typename T> __device__ __forceinline__ float load_f32(const void *p, int64_t i) {
     return (float)static_cast<const T *>(p)[i];
@@ -101,7 +48,7 @@ template <typename T> __device__ __forceinline__ float load_f32(const void *p, i
 
 // Classes: the padded bias, whether any is offered, the largest |W|.
 template <typename T>
-__global__ __launch_bounds__(256) void k_xent_classes(Pack k, const void *w, int64_t stride,
+__global__ __launch_bounds__(256) void k_xent_classes(XentPack k, const void *w, int64_t stride,
                                                       const float *__restrict__ bias) {
     const int lane = threadIdx.x & 63;
     const int64_t v = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -120,7 +67,7 @@ __global__ __launch_bounds__(256) void k_xent_classes(Pack k, const void *w, int
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void k_xent_pack_w(Pack k, const void *w, int64_t stride) {
+__global__ __launch_bounds__(256) void k_xent_pack_w(XentPack k, const void *w, int64_t stride) {
     const int lane = threadIdx.x & 63;
     const int64_t v = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (v >= k.v_pad) return;
@@ -142,7 +89,7 @@ __global__ __launch_bounds__(256) void k_xent_pack_w(Pack k, const void *w, int6
 
 // Rows: label and weight (-1 and 0 where the row is out), h scaled by row.
 template <typename T>
-__global__ __launch_bounds__(256) void k_xent_rows(Pack k, const void *h, int64_t stride,
+__global__ __launch_bounds__(256) void k_xent_rows(XentPack k, const void *h, int64_t stride,
                                                    const int32_t *__restrict__ labels,
                                                    const float *__restrict__ weights) {
     const int lane = threadIdx.x & 63;
@@ -185,7 +132,7 @@ __global__ __launch_bounds__(256) void k_xent_rows(Pack k, const void *h, int64_
 // h as dW's product takes it: rows that are out are zeros; f32: times the row's
 // weight, with one scale for all rows (they are summed over).
 template <typename T>
-__global__ __launch_bounds__(256) void k_xent_pack_hg(Pack k, const void *h, int64_t stride) {
+__global__ __launch_bounds__(256) void k_xent_pack_hg(XentPack k, const void *h, int64_t stride) {
     const int lane = threadIdx.x & 63;
     const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (i >= k.n_pad) return;
@@ -220,21 +167,6 @@ struct Operand {
     const u16 *p;
     int64_t plane, ld;
 };
-
-template <int P>
-__device__ __forceinline__ f32x16 mma(const u32x4 (&a)[P], const u32x4 (&b)[P], f32x16 c) {
-    if constexpr (P == 1) {
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a[0]),
-                                                       __builtin_bit_cast(bf16x8, b[0]), c, 0, 0,
-                                                       0);
-    } else {
-        const f16x8 a0 = __builtin_bit_cast(f16x8, a[0]), a1 = __builtin_bit_cast(f16x8, a[1]);
-        const f16x8 b0 = __builtin_bit_cast(f16x8, b[0]), b1 = __builtin_bit_cast(f16x8, b[1]);
-        c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a1, b0, c, 0, 0, 0);
-        c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a0, b1, c, 0, 0, 0);
-        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a0, b0, c, 0, 0, 0);
-    }
-}
 
 // Bytes of 16-byte chunk c of row r in LDS.  A read of the matrix instruction's
 // operand takes one chunk of 8 rows at a time (KC) or 32 bytes of 4 rows: the chunks
@@ -371,7 +303,7 @@ __device__ __forceinline__ int block_row(int r) {
 // row: the maximum and sum stay in registers over the classes of a split, and only
 // two lanes and two wavefronts have parts of a row.  part[2 * split + half][row].
 template <int P>
-__global__ __launch_bounds__(256) void k_xent_stats(Pack k, int64_t class_tiles, int32_t splits,
+__global__ __launch_bounds__(256) void k_xent_stats(XentPack k, int64_t class_tiles, int32_t splits,
                                                     float2 *__restrict__ part,
                                                     float *__restrict__ z_label) {
     extern __shared__ char lds[];
@@ -434,7 +366,7 @@ __global__ __launch_bounds__(256) void k_xent_stats(Pack k, int64_t class_tiles,
 }
 
 // The parts of a row joined, in order: lse and loss.
-__global__ __launch_bounds__(256) void k_xent_join(Pack k, int32_t parts,
+__global__ __launch_bounds__(256) void k_xent_join(XentPack k, int32_t parts,
                                                    const float2 *__restrict__ part,
                                                    const float *__restrict__ z_label,
                                                    float *__restrict__ lse_pad,
@@ -460,7 +392,7 @@ __global__ __launch_bounds__(256) void k_xent_join(Pack k, int32_t parts,
 // ---- pass 2: G of a piece ------------------------------------------------------------
 // g[v - v0][i - r0], rows of rows_pad; f32: G / w in two f16 terms times 2^15.
 template <int P>
-__global__ __launch_bounds__(256) void k_xent_g(Pack k, int64_t v0, int64_t r0, int64_t rows_pad,
+__global__ __launch_bounds__(256) void k_xent_g(XentPack k, int64_t v0, int64_t r0, int64_t rows_pad,
                                                 int64_t plane, int32_t row_tiles,
                                                 const float *__restrict__ lse,
                                                 u16 *__restrict__ g) {
@@ -506,6 +438,7 @@ __global__ __launch_bounds__(256) void k_xent_g(Pack k, int64_t v0, int64_t r0, 
 struct Out {
     float *acc;                  // [m][ld]
     bool first, last;
+    const float *bias;           // dW: rows of bias -inf are 0
     void *out;
     int64_t rows, stride;        // of the output; its columns are d
 };
@@ -518,6 +451,7 @@ __device__ __forceinline__ void put(const Out &o, int32_t d, int32_t ld, int64_t
     if (!o.last) {
         *acc = v;
     } else if (m < o.rows && n < d) {
+        if (o.bias && o.bias[m] == -INFINITY) v = 0.0f;
         if constexpr (P == 1) static_cast<__bf16 *>(o.out)[m * o.stride + n] = (__bf16)v;
         else static_cast<float *>(o.out)[m * o.stride + n] = v * scale;
     }
@@ -525,7 +459,7 @@ __device__ __forceinline__ void put(const Out &o, int32_t d, int32_t ld, int64_t
 
 // dh[i][j] += sum over the piece's v of g[v][i] W[v][j].
 template <int P>
-__global__ __launch_bounds__(256) void k_xent_dh(Pack k, int64_t v0, int64_t classes_pad,
+__global__ __launch_bounds__(256) void k_xent_dh(XentPack k, int64_t v0, int64_t classes_pad,
                                                  int64_t r0, int64_t rows_pad, int64_t plane,
                                                  int32_t row_tiles, const u16 *__restrict__ g,
                                                  Out o) {
@@ -553,7 +487,7 @@ __global__ __launch_bounds__(256) void k_xent_dh(Pack k, int64_t v0, int64_t cla
 
 // dW[v][j] += sum over the rows of g[v][i] hg[i][j].
 template <int P>
-__global__ __launch_bounds__(256) void k_xent_dw(Pack k, int64_t v0, int64_t r0, int64_t rows_pad,
+__global__ __launch_bounds__(256) void k_xent_dw(XentPack k, int64_t v0, int64_t r0, int64_t rows_pad,
                                                  int64_t plane, int32_t class_tiles,
                                                  const u16 *__restrict__ g, Out o) {
     extern __shared__ char lds[];
@@ -577,7 +511,7 @@ __global__ __launch_bounds__(256) void k_xent_dw(Pack k, int64_t v0, int64_t r0,
 
 // db[v] += sum over the rows of G, one wavefront a class.
 template <int P>
-__global__ __launch_bounds__(256) void k_xent_db(Pack k, int64_t v0, int64_t classes, int64_t r0,
+__global__ __launch_bounds__(256) void k_xent_db(XentPack k, int64_t v0, int64_t classes, int64_t r0,
                                                  int64_t rows_pad, int64_t plane,
                                                  const u16 *__restrict__ g, bool first,
                                                  float *__restrict__ db) {
@@ -599,6 +533,7 @@ __global__ __launch_bounds__(256) void k_xent_db(Pack k, int64_t v0, int64_t cla
     for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
     if (lane == 0) {
         if (P == 2) sum *= 1.0f / G_SCALE;
+        if (k.bias[v0 + c] == -INFINITY) sum = 0.0f;
         db[v0 + c] = first ? sum : db[v0 + c] + sum;
     }
 }
@@ -646,7 +581,7 @@ Plan plan_of(const XentCall &c) {
         at += (bytes + 255) / 256 * 256;
         return here;
     };
-    p.ctl = take(sizeof(Ctl));
+    p.ctl = take(sizeof(XentCtl));
     p.h = take((size_t)2 * p.P * p.n_pad * p.ld);
     p.w = take((size_t)2 * p.P * p.v_pad * p.ld);
     p.bias = take((size_t)4 * p.v_pad);
@@ -668,14 +603,14 @@ Plan plan_of(const XentCall &c) {
 
 template <int P, typename T>
 hipError_t run(hipStream_t s, const XentCall &c, const Plan &p, char *m) {
-    Pack k{};
+    XentPack k{};
     k.n = c.rows;
     k.v = c.classes;
     k.n_pad = p.n_pad;
     k.v_pad = p.v_pad;
     k.d = c.dim;
     k.ld = (int32_t)p.ld;
-    k.ctl = reinterpret_cast<Ctl *>(m + p.ctl);
+    k.ctl = reinterpret_cast<XentCtl *>(m + p.ctl);
     k.h = reinterpret_cast<u16 *>(m + p.h);
     k.hg = reinterpret_cast<u16 *>(m + p.hg);
     k.w = reinterpret_cast<u16 *>(m + p.w);
@@ -720,13 +655,13 @@ hipError_t run(hipStream_t s, const XentCall &c, const Plan &p, char *m) {
                                plane, rt, lse, g);
             if (c.dh) {
                 const Out o{reinterpret_cast<float *>(m + p.dh_acc), v0 == 0, v0 + nv == k.v_pad,
-                            c.dh, k.n, c.h_stride};
+                            nullptr, c.dh, k.n, c.h_stride};
                 hipLaunchKernelGGL((k_xent_dh<P>), dim3((uint32_t)rt * cols), b, LDS, s, k, v0, nv,
                                    r0, nr, plane, rt, g, o);
             }
             if (c.dw) {
                 const Out o{reinterpret_cast<float *>(m + p.dw_acc), r0 == 0, r0 + nr == k.n_pad,
-                            c.dw, k.v, c.w_stride};
+                            k.bias, c.dw, k.v, c.w_stride};
                 hipLaunchKernelGGL((k_xent_dw<P>), dim3((uint32_t)vt * cols), b, LDS, s, k, v0, r0,
                                    nr, plane, vt, g, o);
             }
@@ -741,9 +676,13 @@ hipError_t run(hipStream_t s, const XentCall &c, const Plan &p, char *m) {
 
 }  // namespace
 
-size_t xent_scratch(const XentCall &c) { return c.rows ? plan_of(c).end : 0; }
+size_t xent_scratch(const XentCall &c) {
+    if (!c.rows) return 0;
+    return c.dim <= XENT_FUSED_DIM ? xent_fused_scratch(c) : plan_of(c).end;
+}
 
 hipError_t launch_xent(hipStream_t s, const XentCall &c, char *scratch) {
+    if (c.rows && c.dim <= XENT_FUSED_DIM) return launch_xent_fused(s, c, scratch);
     if (c.rows) {
         const Plan p = plan_of(c);
         return c.bf16 ? run<1, __bf16>(s, c, p, scratch) : run<2, float>(s, c, p, scratch);

@@ -1,0 +1,709 @@
+// kernels_xent_fused.hip — the many-class loss for few outputs (dim <= 128): a
+// workgroup keeps 128 rows of one operand in registers and streams the other through
+// LDS, so neither the scores nor G ever leave the registers.
+//
+//   rows pass:    X = 128 rows of h, Y = the classes of a split.  S' = Y X' gives a lane
+//                 scores of one row: running maximum, sum, and O' += Y' P' with
+//                 P = exp(S - maximum).  The splits' parts of a row are joined into lse,
+//                 loss and dh = w (O / sum - W_label).
+//   classes pass: X = 128 classes, Y = the rows of a split.  P = exp(S - lse) less the
+//                 label's 1, times the row's weight; O' += Y' P' is dW, parts summed in
+//                 order.
+//
+// Both products of a tile read the same LDS rows: the first along them, the second
+// across (ds_read_tr16_b64).  S' comes out with a lane's values 8 (r / 4) + 4 half +
+// r % 4 of Y; the second product's sum over Y may take them in any order, so the
+// lane's own registers, rounded, are its operand, and the read across picks Y's
+// rows in that order: no value moves between lanes.
+//
+// f32 operands are two f16 terms (kernels_xent.hip says why); exponents are of 2, with
+// log2 e in the scale of S.
+#include <algorithm>
+
+#include "mbk.h"
+#include "xent.hpp"
+
+namespace mbk {
+
+namespace {
+
+constexpr int XB = 128;                  // X rows of a workgroup, 32 a wavefront
+constexpr int TY = 64;                   // Y rows of a tile
+constexpr float LN2 = 0.69314718055994531f;
+// p = 2^(z - maximum) is kept times 2^13, and the maximum may lag by 2^2, so that p as
+// f16 terms is at most 2^15 and keeps steps of 2^-38.
+constexpr float P_EXP = 13.0f, LAG = 2.0f;
+
+// Elements of a packed row for KS slabs of 16.
+__host__ __device__ constexpr int row_ld(int ks) { return ks <= 2 ? 32 : ks <= 4 ? 64 : 128; }
+
+struct Fused {
+    int64_t n, v, n_pad, v_pad;
+    int32_t d;
+    XentCtl *ctl;
+    u16 *h, *w;                          // planes of n_pad * ld, v_pad * ld
+    float *bias2;                        // [v_pad] bias log2 e, -inf: not offered
+    // of the rows, [n_pad]:
+    float *sc;                           // log2 e times the scale of a score
+    int32_t *exp;                        // f32: h is packed times 2^exp
+    int32_t *label;                      // -1: out, -2: out and not finite
+    float *weight;                       // 0: out
+    float *c2;                           // lse log2 e, +inf: out
+    float *wq;                           // weight as the classes pass multiplies with it
+};
+
+// Values beyond this in a row that is out count as not finite: times a finite W
+// they could still overflow.
+constexpr uint32_t HUGE_BITS = 0x5D800000u;          // 2^60
+
+__global__ void k_fused_init(XentCtl *ctl) {
+    ctl->w_max = ctl->hg_max = ctl->open = 0;
+}
+
+template <typename T> __device__ __forceinline__ float load_f32(const void *p, int64_t i) {
+    return (float)static_cast<const T *>(p)[i];
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void k_fused_classes(Fused k, const void *w, int64_t stride,
+                                                       const float *__restrict__ bias) {
+    const int lane = threadIdx.x & 63;
+    const int64_t v = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (v >= k.v_pad) return;
+    const float b = v < k.v ? (bias ? bias[v] : 0.0f) : -INFINITY;
+    const bool open = b != -INFINITY;
+    if (lane == 0) {
+        k.bias2[v] = b * LOG2E;
+        if (open) k.ctl->open = 1u;
+    }
+    if (sizeof(T) == 2 || !open) return;
+    uint32_t m = 0;
+    for (int32_t f = lane; f < k.d; f += 64) m = max(m, finite_bits(load_f32<T>(w, v * stride + f)));
+    m = wave_max(m);
+    if (lane == 0) atomicMax(&k.ctl->w_max, m);
+}
+
+// One wavefront a packed row, of W and then of h.
+template <typename T>
+__global__ __launch_bounds__(256) void k_fused_pack(Fused k, int32_t ld, const void *w,
+                                                    int64_t w_stride, const void *h,
+                                                    int64_t h_stride,
+                                                    const int32_t *__restrict__ labels,
+                                                    const float *__restrict__ weights) {
+    const int lane = threadIdx.x & 63;
+    int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const bool of_w = i < k.v_pad;
+    if (!of_w) i -= k.v_pad;
+    if (!of_w && i >= k.n_pad) return;
+    const int sw = sizeof(T) == 4 ? scale_exp(k.ctl->w_max) : 0;
+    const void *src = of_w ? w : h;
+    const int64_t at = i * (of_w ? w_stride : h_stride);
+    bool in = of_w ? i < k.v && k.bias2[i] != -INFINITY : i < k.n;
+    float x[2];
+    uint32_t m = 0;
+    bool finite = true;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        const int f = lane + 64 * q;
+        x[q] = in && f < k.d ? load_f32<T>(src, at + f) : 0.0f;
+        const uint32_t b = __float_as_uint(fabsf(x[q]));
+        finite = finite && b < HUGE_BITS;
+        m = max(m, finite_bits(x[q]));
+    }
+    int s = sw;
+    if (!of_w) {
+        int32_t y = i < k.n ? labels[i] : -1;
+        float wt = i < k.n ? (weights ? weights[i] : 1.0f) : 0.0f;
+        if (y < 0 || y >= k.v || wt == 0.0f || !k.ctl->open) {
+            wt = 0.0f;
+            y = -1;
+            if (__ballot(!finite)) {
+                y = -2;
+                x[0] = x[1] = 0.0f;
+                m = 0;
+            }
+        }
+        if (sizeof(T) == 4) {
+            m = wave_max(m);
+            s = scale_exp(m);
+        }
+        if (lane == 0) {
+            k.label[i] = y;
+            k.weight[i] = wt;
+            k.exp[i] = s;
+            k.sc[i] = sizeof(T) == 4 ? ldexpf(LOG2E, -(s + sw)) : LOG2E;
+            if (sizeof(T) == 4 && wt != 0.0f)
+                atomicMax(&k.ctl->hg_max, finite_bits(wt * __uint_as_float(m)));
+        }
+    }
+    u16 *row = (of_w ? k.w : k.h) + i * ld;
+    const int64_t plane = (of_w ? k.v_pad : k.n_pad) * ld;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        const int f = lane + 64 * q;
+        if (f >= ld) break;
+        if (sizeof(T) == 2) {
+            row[f] = bits_of((__bf16)x[q]);
+        } else {
+            u16 hi, lo;
+            split_f16(ldexpf(x[q], s), hi, lo);
+            row[f] = hi;
+            row[plane + f] = lo;
+        }
+    }
+}
+
+// ---- a tile in LDS -----------------------------------------------------------------
+// TY rows of LD elements a plane, the 16-byte chunks of a row permuted by the row so
+// that the 8 rows x 1 chunk of an operand's read and the 4 rows x 2 chunks of a read
+// across both fall on different banks.
+template <int LD> __device__ __forceinline__ int chunk_xor(int row) {
+    if constexpr (LD == 32) return ((row >> 1) & 1) * 2 + ((row >> 2) & 1);
+    else return (row & 3) * 2 + ((row >> 2) & 1);
+}
+template <int P, int LD> constexpr int TILE_BYTES = P * TY * LD * 2;
+
+typedef __attribute__((address_space(3))) void lds_void;
+typedef const __attribute__((address_space(1))) void global_void;
+
+// The copies that this wavefront has started are in LDS; a barrier alone does not wait
+// for them.
+__device__ __forceinline__ void copies_done() { __builtin_amdgcn_s_waitcnt(0x0F70); }
+
+// Starts the copies of a tile's operand; the LDS side is linear, so the source is
+// read in the permuted order.
+template <int P, int LD>
+__device__ __forceinline__ void load_tile(const u16 *src, int64_t plane, char *lds, int wave) {
+    constexpr int ROW = LD * 2, PLANE = TY * ROW;
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+#pragma unroll
+        for (int q = 0; q < PLANE / 4096; ++q) {
+            const int at = (q * 4 + wave) * 1024, o = at + lane * 16;
+            const int row = o / ROW, chunk = (o % ROW / 16) ^ chunk_xor<LD>(row);
+            __builtin_amdgcn_global_load_lds(
+                (global_void *)(src + p * plane + row * LD + chunk * 8),
+                (lds_void *)(lds + p * PLANE + at), 16, 0, 0);
+        }
+}
+
+template <int P, int LD>
+__device__ __forceinline__ void along(const char *lds, int row, int slab, u32x4 (&f)[P]) {
+    const int lane = threadIdx.x & 63, r = row + (lane & 31);
+    const int chunk = (slab * 2 + (lane >> 5)) ^ chunk_xor<LD>(r);
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+        f[p] = *reinterpret_cast<const u32x4 *>(lds + p * (TY * LD * 2) + r * (LD * 2) + chunk * 16);
+}
+
+template <int P, int LD>
+__device__ __forceinline__ void across(const char *lds, int row, int col, u32x4 (&f)[P]) {
+    typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
+    const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
+    const int c = col + (g & 1) * 16 + (i & 3) * 4;
+    const int r = row + (g >> 1) * 4 + (i >> 2);
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+        union {
+            i16x4 h[2];
+            u32x4 v;
+        } u;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const int rr = r + 8 * t, chunk = (c >> 3) ^ chunk_xor<LD>(rr);
+            u.h[t] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (lds_i16x4 *)(lds + p * (TY * LD * 2) + rr * (LD * 2) + chunk * 16 + (c & 7) * 2));
+        }
+        f[p] = u.v;
+    }
+}
+
+// Eight values as the second product's operand.
+template <int P> __device__ __forceinline__ void pack8(const float (&x)[8], u32x4 (&f)[P]) {
+    if constexpr (P == 1) {
+        bf16x8 v;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = (__bf16)x[e];
+        f[0] = __builtin_bit_cast(u32x4, v);
+    } else {
+        f16x8 hi, lo;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            hi[e] = (_Float16)x[e];
+            lo[e] = (_Float16)(x[e] - (float)hi[e]);
+        }
+        f[0] = __builtin_bit_cast(u32x4, hi);
+        f[1] = __builtin_bit_cast(u32x4, lo);
+    }
+}
+
+__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 64); }
+
+// ---- rows pass ----------------------------------------------------------------------
+// part_o[split][row][ld], part_ms[split][row] = (reference, sum): sum and O are of
+// 2^(z - reference).
+template <int P, int KS, bool GRAD>
+__global__ __launch_bounds__(256, 2) void k_fused_rows(Fused k, int32_t splits,
+                                                       float *__restrict__ part_o,
+                                                       float2 *__restrict__ part_ms) {
+    constexpr int LD = row_ld(KS), JT = (KS + 1) / 2;
+    constexpr int BUF = TILE_BYTES<P, LD> + TY * 4;
+    extern __shared__ char lds[];
+    const int lane = threadIdx.x & 63, half = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t x0 = (int64_t)(blockIdx.x / splits) * XB;
+    const int32_t split = blockIdx.x % splits;
+    const int64_t tiles = k.v_pad / TY, first = tiles * split / splits,
+                  last = tiles * (split + 1) / splits;
+    const int64_t row = x0 + wave * 32 + (lane & 31);
+    u32x4 x[KS][P];
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+            x[s][p] = *reinterpret_cast<const u32x4 *>(k.h + p * k.n_pad * LD + row * LD + s * 16 +
+                                                       half * 8);
+    const float sc = P == 1 ? LOG2E : k.sc[row];
+    float ref = 0.0f, top = -INFINITY, sum = 0.0f;
+    f32x16 o[GRAD ? JT : 1];
+#pragma unroll
+    for (int j = 0; j < (GRAD ? JT : 1); ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[j][r] = 0.0f;
+
+    auto load = [&](int64_t t, int buf) {
+        char *to = lds + buf * BUF;
+        load_tile<P, LD>(k.w + t * TY * LD, k.v_pad * LD, to, wave);
+        if (wave == 0)
+            __builtin_amdgcn_global_load_lds((global_void *)(k.bias2 + t * TY + lane),
+                                             (lds_void *)(to + TILE_BYTES<P, LD>), 4, 0, 0);
+    };
+    if (first < last) load(first, 0);
+    for (int64_t t = first; t < last; ++t) {
+        const int buf = (t - first) & 1;
+        copies_done();
+        __syncthreads();                 // the tile is there; the other one is read
+        if (t + 1 < last) load(t + 1, buf ^ 1);
+        const char *tile = lds + buf * BUF;
+        const float *bias = reinterpret_cast<const float *>(tile + TILE_BYTES<P, LD>);
+#pragma unroll
+        for (int y = 0; y < TY; y += 32) {
+            f32x16 s;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = 0.0f;
+#pragma unroll
+            for (int q = 0; q < KS; ++q) {
+                u32x4 a[P];
+                along<P, LD>(tile, y, q, a);
+                s = mma<P>(a, x[q], s);
+            }
+            float m = -INFINITY;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s[r] = __builtin_fmaf(s[r], sc, bias[y + (r >> 2) * 8 + half * 4 + (r & 3)]);
+                m = fmaxf(m, s[r]);
+            }
+            // a new maximum: what was summed so far is brought to it
+            if (__any(m > top + LAG)) {
+                const float now = fmaxf(top, fmaxf(m, other_half(m)));
+                if (now > top) {
+                    const float to = now - P_EXP;
+                    const float scale = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ref - to);
+                    sum *= scale;
+                    if constexpr (GRAD)
+#pragma unroll
+                        for (int j = 0; j < JT; ++j)
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) o[j][r] *= scale;
+                    ref = to;
+                    top = now;
+                }
+            }
+            float p[2][8], part[2] = {0.0f, 0.0f};
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                p[r >> 3][r & 7] = __builtin_amdgcn_exp2f(s[r] - ref);
+                part[r & 1] += p[r >> 3][r & 7];
+            }
+            sum += part[0] + part[1];
+            if constexpr (GRAD) {
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    u32x4 b[P];
+                    pack8<P>(p[q], b);
+#pragma unroll
+                    for (int j = 0; j < JT; ++j) {
+                        u32x4 a[P];
+                        across<P, LD>(tile, y + q * 16, j * 32, a);
+                        o[j] = mma<P>(a, b, o[j]);
+                    }
+                }
+            }
+        }
+    }
+    sum += other_half(sum);
+    const int64_t at = split * k.n_pad + row;
+    if (half == 0) part_ms[at] = make_float2(top == -INFINITY ? -INFINITY : ref, sum);
+    if constexpr (GRAD) {
+        float *out = part_o + at * LD;
+#pragma unroll
+        for (int j = 0; j < JT; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                *reinterpret_cast<float4 *>(out + j * 32 + q * 8 + half * 4) =
+                    make_float4(o[j][q * 4], o[j][q * 4 + 1], o[j][q * 4 + 2], o[j][q * 4 + 3]);
+    }
+}
+
+// The splits of a row joined, one wavefront a row; its label's score is summed in f32
+// from h and W themselves.
+template <typename T, bool GRAD>
+__global__ __launch_bounds__(256) void k_fused_join_rows(
+    Fused k, XentCall c, int32_t splits, int32_t ld, const float *__restrict__ part_o,
+    const float2 *__restrict__ part_ms) {
+    const int lane = threadIdx.x & 63;
+    const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (i >= k.n_pad) return;
+    float ref = -INFINITY;
+    for (int s = 0; s < splits; ++s) ref = fmaxf(ref, part_ms[s * k.n_pad + i].x);
+    const bool none = ref == -INFINITY;
+    float sum = 0.0f, o[2] = {0.0f, 0.0f};
+    for (int s = 0; s < splits; ++s) {
+        const float2 ms = part_ms[s * k.n_pad + i];
+        const float scale = none ? 1.0f : __builtin_amdgcn_exp2f(ms.x - ref);
+        sum += ms.y * scale;
+        if constexpr (GRAD)
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+                if (lane + 64 * q < k.d)
+                    o[q] += part_o[(s * k.n_pad + i) * ld + lane + 64 * q] * scale;
+    }
+    const int32_t y = k.label[i];
+    // a sum that is not a number is one with no reference, too
+    const float l2 = none && sum == 0.0f ? -INFINITY : (none ? 0.0f : ref) + log2f(sum);
+    const float lse = y == -2 ? NAN : l2 * LN2;
+    const float wt = k.weight[i];
+    const bool open = y >= 0 && k.bias2[y] != -INFINITY;
+    float wy[2] = {0.0f, 0.0f}, dot = 0.0f;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        const int f = lane + 64 * q;
+        if (open && f < k.d) {
+            wy[q] = load_f32<T>(c.w, y * c.w_stride + f);
+            dot += wy[q] * load_f32<T>(c.h, i * c.h_stride + f);
+        }
+    }
+#pragma unroll
+    for (int m = 32; m > 0; m >>= 1) dot += __shfl_xor(dot, m, 64);
+    if (lane == 0) {
+        if (i < k.n) {
+            const float z = open ? dot + (c.bias ? c.bias[y] : 0.0f) : -INFINITY;
+            c.lse[i] = lse;
+            c.loss[i] = y < 0 ? 0.0f : wt * (lse - z);
+        }
+        if constexpr (GRAD) {
+            k.c2[i] = y < 0 ? INFINITY : l2;
+            if (sizeof(T) == 2) {
+                k.wq[i] = wt;
+            } else {
+                // weight 2^-exp and the power of two that brings the largest below 2^15
+                const uint32_t m = k.ctl->hg_max;
+                const int up = m ? min(126, max(-126, 27 - ilogbf(__uint_as_float(m)))) : 0;
+                const float q = ldexpf(wt, up - k.exp[i]);
+                k.wq[i] = fminf(fmaxf(q, -60000.0f), 60000.0f);
+            }
+        }
+    }
+    if constexpr (GRAD) {
+        if (!c.dh || i >= k.n) return;
+        const float scale = sizeof(T) == 4 ? ldexpf(1.0f, -scale_exp(k.ctl->w_max)) : 1.0f;
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            const int f = lane + 64 * q;
+            if (f >= k.d) break;
+            const float g = y < 0 ? 0.0f : wt * (o[q] * scale / sum - wy[q]);
+            static_cast<T *>(c.dh)[i * c.h_stride + f] = (T)g;
+        }
+    }
+}
+
+// ---- classes pass ---------------------------------------------------------------------
+// part[split][class][ld] of dW, part_db[split][class]
+template <int P, int KS>
+__global__ __launch_bounds__(256, 2) void k_fused_classes_pass(Fused k, int32_t splits,
+                                                               float *__restrict__ part,
+                                                               float *__restrict__ part_db) {
+    constexpr int LD = row_ld(KS), JT = (KS + 1) / 2;
+    constexpr int ROWS_AT = TILE_BYTES<P, LD>;           // sc, c2, wq, label, weight
+    constexpr int BUF = ROWS_AT + 5 * TY * 4;
+    extern __shared__ char lds[];
+    const int lane = threadIdx.x & 63, half = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t x0 = (int64_t)(blockIdx.x / splits) * XB + wave * 32;
+    const int32_t split = blockIdx.x % splits;
+    const int64_t tiles = k.n_pad / TY, first = tiles * split / splits,
+                  last = tiles * (split + 1) / splits;
+    const int64_t v = x0 + (lane & 31);
+    u32x4 x[KS][P];
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+            x[s][p] = *reinterpret_cast<const u32x4 *>(k.w + p * k.v_pad * LD + v * LD + s * 16 +
+                                                       half * 8);
+    const float b2 = k.bias2[v];
+    float db = 0.0f;
+    f32x16 o[JT];
+#pragma unroll
+    for (int j = 0; j < JT; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[j][r] = 0.0f;
+
+    auto load = [&](int64_t t, int buf) {
+        char *to = lds + buf * BUF;
+        load_tile<P, LD>(k.h + t * TY * LD, k.n_pad * LD, to, wave);
+        const void *rows[5] = {k.sc, k.c2, k.wq, k.label, k.weight};
+#pragma unroll
+        for (int q = 0; q < 5; ++q)
+            if (wave == (q & 3))
+                __builtin_amdgcn_global_load_lds(
+                    (global_void *)(static_cast<const float *>(rows[q]) + t * TY + lane),
+                    (lds_void *)(to + ROWS_AT + q * TY * 4), 4, 0, 0);
+    };
+    if (first < last) load(first, 0);
+    for (int64_t t = first; t < last; ++t) {
+        const int buf = (t - first) & 1;
+        copies_done();
+        __syncthreads();
+        if (t + 1 < last) load(t + 1, buf ^ 1);
+        const char *tile = lds + buf * BUF;
+        const float *sc = reinterpret_cast<const float *>(tile + ROWS_AT), *c2 = sc + TY,
+                    *wq = sc + 2 * TY, *weight = sc + 4 * TY;
+        const int32_t *label = reinterpret_cast<const int32_t *>(sc + 3 * TY);
+#pragma unroll
+        for (int y = 0; y < TY; y += 32) {
+            f32x16 s;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = 0.0f;
+#pragma unroll
+            for (int q = 0; q < KS; ++q) {
+                u32x4 a[P];
+                along<P, LD>(tile, y, q, a);
+                s = mma<P>(a, x[q], s);
+            }
+            const int64_t mine = label[y + (lane & 31)] - x0;
+            const bool hot = __any(mine >= 0 && mine < 32);
+            float p[2][8];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int i = y + (r >> 2) * 8 + half * 4 + (r & 3);
+                float e = __builtin_amdgcn_exp2f(
+                    __builtin_fmaf(s[r], P == 1 ? LOG2E : sc[i], b2 - c2[i]));
+                p[r >> 3][r & 7] = e;
+            }
+            if (hot)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (label[y + (r >> 2) * 8 + half * 4 + (r & 3)] == v) p[r >> 3][r & 7] -= 1.0f;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int i = y + (r >> 2) * 8 + half * 4 + (r & 3);
+                if (part_db) db = __builtin_fmaf(p[r >> 3][r & 7], weight[i], db);
+                p[r >> 3][r & 7] *= wq[i];
+            }
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                u32x4 b[P];
+                pack8<P>(p[q], b);
+#pragma unroll
+                for (int j = 0; j < JT; ++j) {
+                    u32x4 a[P];
+                    across<P, LD>(tile, y + q * 16, j * 32, a);
+                    o[j] = mma<P>(a, b, o[j]);
+                }
+            }
+        }
+    }
+    const int64_t at = split * k.v_pad + v;
+    if (part_db) {
+        db += other_half(db);
+        if (half == 0) part_db[at] = db;
+    }
+    float *out = part + at * LD;
+#pragma unroll
+    for (int j = 0; j < JT; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<float4 *>(out + j * 32 + q * 8 + half * 4) =
+                make_float4(o[j][q * 4], o[j][q * 4 + 1], o[j][q * 4 + 2], o[j][q * 4 + 3]);
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void k_fused_join_classes(Fused k, XentCall c, int32_t splits,
+                                                            int32_t ld,
+                                                            const float *__restrict__ part,
+                                                            const float *__restrict__ part_db) {
+    const int lane = threadIdx.x & 63;
+    const int64_t v = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (v >= k.v) return;
+    const bool open = k.bias2[v] != -INFINITY;
+    float scale = 1.0f;
+    if (sizeof(T) == 4) {
+        const uint32_t m = k.ctl->hg_max;
+        scale = ldexpf(1.0f, -(m ? min(126, max(-126, 27 - ilogbf(__uint_as_float(m)))) : 0));
+    }
+    if (c.dw)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            const int f = lane + 64 * q;
+            if (f >= k.d) break;
+            float sum = 0.0f;
+            for (int s = 0; s < splits; ++s) sum += part[(s * k.v_pad + v) * ld + f];
+            static_cast<T *>(c.dw)[v * c.w_stride + f] = (T)(open ? sum * scale : 0.0f);
+        }
+    if (c.dbias && lane == 0) {
+        float sum = 0.0f;
+        for (int s = 0; s < splits; ++s) sum += part_db[s * k.v_pad + v];
+        c.dbias[v] = open ? sum : 0.0f;
+    }
+}
+
+// ---- the call ---------------------------------------------------------------------------
+int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
+uint32_t blocks(int64_t x, int64_t per) { return (uint32_t)((x + per - 1) / per); }
+
+// Workgroups for `blocks` X blocks over `tiles` Y tiles: two run on a CU at once, and
+// the last round of them should be full.  At least 4 tiles a split.
+int32_t pick_splits(int64_t x_blocks, int64_t tiles, int num_cus) {
+    const int64_t slots = 2 * (int64_t)num_cus;
+    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(tiles / 4, 64));
+    int64_t best = 1;
+    double cost = 1e30;
+    for (int64_t s = 1; s <= most; ++s) {
+        // rounds of workgroups times a workgroup's tiles, and its start and end
+        const double c = (double)((x_blocks * s + slots - 1) / slots) *
+                         ((double)((tiles + s - 1) / s) + 3.0);
+        if (c < cost) {
+            cost = c;
+            best = s;
+        }
+    }
+    return (int32_t)best;
+}
+
+struct Plan {
+    int P, ks;
+    int64_t n_pad, v_pad, ld;
+    int32_t row_splits, class_splits;
+    size_t ctl, h, w, bias2, rows, part_ms, part, part_db, end;
+};
+
+Plan plan_of(const XentCall &c) {
+    Plan p{};
+    p.P = c.bf16 ? 1 : 2;
+    p.ks = c.dim <= 32 ? 2 : c.dim <= 64 ? 4 : 8;
+    p.ld = row_ld(p.ks);
+    p.n_pad = up(c.rows, XB);
+    p.v_pad = up(c.classes, XB);
+    p.row_splits = pick_splits(p.n_pad / XB, p.v_pad / TY, c.num_cus);
+    p.class_splits = pick_splits(p.v_pad / XB, p.n_pad / TY, c.num_cus);
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        const size_t here = at;
+        at += (bytes + 255) / 256 * 256;
+        return here;
+    };
+    p.ctl = take(sizeof(XentCtl));
+    p.h = take((size_t)2 * p.P * p.n_pad * p.ld);
+    p.w = take((size_t)2 * p.P * p.v_pad * p.ld);
+    p.bias2 = take((size_t)4 * p.v_pad);
+    p.rows = take((size_t)6 * 4 * p.n_pad);
+    p.part_ms = take((size_t)8 * p.row_splits * p.n_pad);
+    if (c.grad) {
+        p.part = take((size_t)4 * p.ld * std::max(p.row_splits * p.n_pad, p.class_splits * p.v_pad));
+        p.part_db = take((size_t)4 * p.class_splits * p.v_pad);
+    }
+    p.end = at;
+    return p;
+}
+
+template <int P, int KS, typename T>
+hipError_t run(hipStream_t s, const XentCall &c, const Plan &p, char *m) {
+    constexpr int LD = row_ld(KS);
+    Fused k{};
+    k.n = c.rows;
+    k.v = c.classes;
+    k.n_pad = p.n_pad;
+    k.v_pad = p.v_pad;
+    k.d = c.dim;
+    k.ctl = reinterpret_cast<XentCtl *>(m + p.ctl);
+    k.h = reinterpret_cast<u16 *>(m + p.h);
+    k.w = reinterpret_cast<u16 *>(m + p.w);
+    k.bias2 = reinterpret_cast<float *>(m + p.bias2);
+    float *rows = reinterpret_cast<float *>(m + p.rows);
+    k.sc = rows;
+    k.exp = reinterpret_cast<int32_t *>(rows + p.n_pad);
+    k.label = reinterpret_cast<int32_t *>(rows + 2 * p.n_pad);
+    k.weight = rows + 3 * p.n_pad;
+    k.c2 = rows + 4 * p.n_pad;
+    k.wq = rows + 5 * p.n_pad;
+    float2 *part_ms = reinterpret_cast<float2 *>(m + p.part_ms);
+    float *part = reinterpret_cast<float *>(m + p.part);
+    float *part_db = reinterpret_cast<float *>(m + p.part_db);
+    const dim3 b(256);
+    const size_t lds_rows = 2 * (TILE_BYTES<P, LD> + TY * 4);
+    const size_t lds_classes = 2 * (TILE_BYTES<P, LD> + 5 * TY * 4);
+    const void *big[] = {reinterpret_cast<const void *>(k_fused_rows<P, KS, true>),
+                         reinterpret_cast<const void *>(k_fused_rows<P, KS, false>),
+                         reinterpret_cast<const void *>(k_fused_classes_pass<P, KS>)};
+    for (const void *f : big) {
+        const hipError_t e = allow_all_lds(f);
+        if (e != hipSuccess) return e;
+    }
+    hipLaunchKernelGGL(k_fused_init, dim3(1), dim3(1), 0, s, k.ctl);
+    hipLaunchKernelGGL((k_fused_classes<T>), dim3(blocks(k.v_pad, 4)), b, 0, s, k, c.w, c.w_stride,
+                       c.bias);
+    hipLaunchKernelGGL((k_fused_pack<T>), dim3(blocks(k.v_pad + k.n_pad, 4)), b, 0, s, k, LD, c.w,
+                       c.w_stride, c.h, c.h_stride, c.labels, c.weights);
+    const dim3 gr((uint32_t)(k.n_pad / XB * p.row_splits)), gj(blocks(k.n_pad, 4));
+    if (!c.grad) {
+        hipLaunchKernelGGL((k_fused_rows<P, KS, false>), gr, b, lds_rows, s, k, p.row_splits,
+                           static_cast<float *>(nullptr), part_ms);
+        hipLaunchKernelGGL((k_fused_join_rows<T, false>), gj, b, 0, s, k, c, p.row_splits, LD, part,
+                           part_ms);
+        return hipGetLastError();
+    }
+    hipLaunchKernelGGL((k_fused_rows<P, KS, true>), gr, b, lds_rows, s, k, p.row_splits, part,
+                       part_ms);
+    hipLaunchKernelGGL((k_fused_join_rows<T, true>), gj, b, 0, s, k, c, p.row_splits, LD, part,
+                       part_ms);
+    if (c.dw || c.dbias) {
+        hipLaunchKernelGGL((k_fused_classes_pass<P, KS>),
+                           dim3((uint32_t)(k.v_pad / XB * p.class_splits)), b, lds_classes, s, k,
+                           p.class_splits, part, c.dbias ? part_db : nullptr);
+        hipLaunchKernelGGL((k_fused_join_classes<T>), dim3(blocks(k.v, 4)), b, 0, s, k, c,
+                           p.class_splits, LD, part, part_db);
+    }
+    return hipGetLastError();
+}
+
+template <int P, typename T>
+hipError_t run_dim(hipStream_t s, const XentCall &c, const Plan &p, char *m) {
+    switch (p.ks) {
+    case 2: return run<P, 2, T>(s, c, p, m);
+    case 4: return run<P, 4, T>(s, c, p, m);
+    default: return run<P, 8, T>(s, c, p, m);
+    }
+}
+
+}  // namespace
+
+size_t xent_fused_scratch(const XentCall &c) { return plan_of(c).end; }
+
+hipError_t launch_xent_fused(hipStream_t s, const XentCall &c, char *scratch) {
+    const Plan p = plan_of(c);
+    return c.bf16 ? run_dim<1, __bf16>(s, c, p, scratch) : run_dim<2, float>(s, c, p, scratch);
+}
+
+}  // namespace mbk

@@ -1,0 +1,86 @@
+// xent.hpp — what the kernels of the many-class loss share: the packed operands and
+// the matrix instruction on them.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "ops.h"
+
+namespace mbk {
+
+typedef __attribute__((ext_vector_type(4))) unsigned int u32x4;       // 8 operands
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+typedef __attribute__((ext_vector_type(4))) short i16x4;
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef unsigned short u16;
+
+constexpr float LOG2E = 1.44269504088896341f;
+
+// ---- control words -----------------------------------------------------------
+struct XentCtl {
+    uint32_t w_max, hg_max;              // bits of the largest |W|, |w h| that is finite
+    uint32_t open;                       // a class is offered
+};
+
+__device__ __forceinline__ uint32_t finite_bits(float x) {
+    const uint32_t b = __float_as_uint(fabsf(x));
+    return b < 0x7F800000u ? b : 0u;
+}
+// The exponent that brings a maximum below 2^14 (0 for a maximum of 0).
+__device__ __forceinline__ int scale_exp(uint32_t max_bits) {
+    if (!max_bits) return 0;
+    const int s = 13 - ilogbf(__uint_as_float(max_bits));
+    return min(126, max(-126, s));
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o, 64));
+    return v;
+}
+
+__device__ __forceinline__ u16 bits_of(__bf16 v) { return __builtin_bit_cast(u16, v); }
+__device__ __forceinline__ u16 bits_of(_Float16 v) { return __builtin_bit_cast(u16, v); }
+
+// x 2^s in two f16 terms.
+__device__ __forceinline__ void split_f16(float x, u16 &hi, u16 &lo) {
+    const _Float16 h = (_Float16)x;
+    hi = bits_of(h);
+    lo = bits_of((_Float16)(x - (float)h));
+}
+
+// What the kernels read: operands in rows of ld 16-bit elements, zeros behind the
+// sizes, P planes of them.
+struct XentPack {
+    int64_t n, v, n_pad, v_pad;
+    int32_t d, ld;
+    XentCtl *ctl;
+    u16 *h, *hg, *w;                     // planes of n_pad * ld, v_pad * ld
+    float *bias;                         // [v_pad], -inf: not offered
+    float *row_scale;                    // [n_pad], f32: 2^-s of h's row
+    int32_t *label;                      // [n_pad], -1: out
+    float *weight;                       // [n_pad], 0: out
+};
+
+template <int P>
+__device__ __forceinline__ f32x16 mma(const u32x4 (&a)[P], const u32x4 (&b)[P], f32x16 c) {
+    if constexpr (P == 1) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a[0]),
+                                                       __builtin_bit_cast(bf16x8, b[0]), c, 0, 0,
+                                                       0);
+    } else {
+        const f16x8 a0 = __builtin_bit_cast(f16x8, a[0]), a1 = __builtin_bit_cast(f16x8, a[1]);
+        const f16x8 b0 = __builtin_bit_cast(f16x8, b[0]), b1 = __builtin_bit_cast(f16x8, b[1]);
+        c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a1, b0, c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a0, b1, c, 0, 0, 0);
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a0, b0, c, 0, 0, 0);
+    }
+}
+
+// The kernels of up to XENT_FUSED_DIM outputs (kernels_xent_fused.hip): scores, their
+// exponentials and the product with them in one pass for dh and one for dW.
+constexpr int XENT_FUSED_DIM = 128;
+size_t xent_fused_scratch(const XentCall &c);
+hipError_t launch_xent_fused(hipStream_t s, const XentCall &c, char *scratch);
+
+}  // namespace mbk

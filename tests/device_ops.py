@@ -141,9 +141,13 @@ def xent_reference(h, w, labels, kind, bias=None, weights=None):
         rel = np.where(closed, 0, ez) + elz[:, None] + (3 * dist + 8) * u
         half = HALF["bf16"] if kind == "bf16" else 2.0 ** -22
         eg = np.abs(wl)[:, None] * (p * rel + np.abs(p - hot) * half + 2.0 ** -38)
-        eg[~live] = 0
-        eg[:, closed] = 0
-        g[:, closed] = 0
+        # f16 terms of G times the row's weight share one scale, that of the largest row
+        rows = np.abs(hl).max(1) if d else np.zeros(n)
+        with_scale = 0.0 if kind == "bf16" else 2.0 ** -37 * (np.abs(wl) * rows).max(initial=0)
+        ew = eg + np.where(rows > 0, with_scale / np.where(rows > 0, rows, 1), 0)[:, None]
+        for e in (eg, ew, g):
+            e[~live] = 0
+            e[:, closed] = 0
 
         def product(left, right, e_left, e_right, terms):
             return (e_left @ np.abs(right) + np.abs(left) @ e_right
@@ -152,7 +156,7 @@ def xent_reference(h, w, labels, kind, bias=None, weights=None):
         none_w, none_h = np.zeros_like(w), np.zeros_like(hl)
         for name, value, err in (
                 ("dh", g @ w, product(g, w, eg, none_w, v)),
-                ("dw", g.T @ hl, product(g.T, hl, eg.T, none_h, n)),
+                ("dw", g.T @ hl, product(g.T, hl, ew.T, none_h, n)),
                 ("db", g.sum(0), eg.sum(0) + np.abs(g).sum(0) * (n + 4) * u)):
             step = HALF[kind] if name != "db" else u
             out[name] = (value, err + (np.abs(value) + err) * step + 1e-37)

@@ -125,6 +125,7 @@ def test_xent_label_not_offered(ctx, kind, d):
         r[name], want[name] = r[name][keep], tuple(t[keep] for t in want[name])
     D.check(r, want, ("loss", "lse", "dh"))
     assert np.isfinite(r["dw"]).all()
+    assert np.all(r["dw"][7] == 0) and r["db"][7] == 0
 
 
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
