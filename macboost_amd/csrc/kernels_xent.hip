@@ -57,13 +57,13 @@ __global__ __launch_bounds__(256) void k_xent_classes(XentPack k, const void *w,
     const bool open = b != -INFINITY;
     if (lane == 0) {
         k.bias[v] = b;
-        if (open) k.ctl->open = 1u;
+        if (open && !k.ctl->open) k.ctl->open = 1u;
     }
     if (sizeof(T) == 2 || !open) return;
     uint32_t m = 0;
     for (int32_t f = lane; f < k.d; f += 64) m = max(m, finite_bits(load_f32<T>(w, v * stride + f)));
     m = wave_max(m);
-    if (lane == 0) atomicMax(&k.ctl->w_max, m);
+    if (lane == 0) raise(&k.ctl->w_max, m);
 }
 
 template <typename T>
@@ -108,7 +108,7 @@ __global__ __launch_bounds__(256) void k_xent_rows(XentPack k, const void *h, in
         s = scale_exp(m);
         if (lane == 0) {
             k.row_scale[i] = ldexpf(1.0f, -s);
-            if (wt != 0.0f) atomicMax(&k.ctl->hg_max, finite_bits(wt * __uint_as_float(m)));
+            if (wt != 0.0f) raise(&k.ctl->hg_max, finite_bits(wt * __uint_as_float(m)));
         }
     }
     if (lane == 0) {

@@ -56,6 +56,11 @@ struct Fused {
 // they could still overflow.
 constexpr uint32_t HUGE_BITS = 0x5D800000u;          // 2^60
 
+// The exponent of the classes pass's weights, for the largest |w h|.
+__device__ __forceinline__ int wq_exp(uint32_t hg_max) {
+    return hg_max ? min(126, max(-126, 27 - ilogbf(__uint_as_float(hg_max)))) : 0;
+}
+
 __global__ void k_fused_init(XentCtl *ctl) {
     ctl->w_max = ctl->hg_max = ctl->open = 0;
 }
@@ -74,13 +79,13 @@ __global__ __launch_bounds__(256) void k_fused_classes(Fused k, const void *w, i
     const bool open = b != -INFINITY;
     if (lane == 0) {
         k.bias2[v] = b * LOG2E;
-        if (open) k.ctl->open = 1u;
+        if (open && !k.ctl->open) k.ctl->open = 1u;
     }
     if (sizeof(T) == 2 || !open) return;
     uint32_t m = 0;
     for (int32_t f = lane; f < k.d; f += 64) m = max(m, finite_bits(load_f32<T>(w, v * stride + f)));
     m = wave_max(m);
-    if (lane == 0) atomicMax(&k.ctl->w_max, m);
+    if (lane == 0) raise(&k.ctl->w_max, m);
 }
 
 // One wavefront a packed row, of W and then of h.
@@ -133,7 +138,7 @@ __global__ __launch_bounds__(256) void k_fused_pack(Fused k, int32_t ld, const v
             k.exp[i] = s;
             k.sc[i] = sizeof(T) == 4 ? ldexpf(LOG2E, -(s + sw)) : LOG2E;
             if (sizeof(T) == 4 && wt != 0.0f)
-                atomicMax(&k.ctl->hg_max, finite_bits(wt * __uint_as_float(m)));
+                raise(&k.ctl->hg_max, finite_bits(wt * __uint_as_float(m)));
         }
     }
     u16 *row = (of_w ? k.w : k.h) + i * ld;
@@ -197,27 +202,7 @@ __device__ __forceinline__ void along(const char *lds, int row, int slab, u32x4 
         f[p] = *reinterpret_cast<const u32x4 *>(lds + p * (TY * LD * 2) + r * (LD * 2) + chunk * 16);
 }
 
-template <int P, int LD>
-__device__ __forceinline__ void across(const char *lds, int row, int col, u32x4 (&f)[P]) {
-    typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
-    const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
-    const int c = col + (g & 1) * 16 + (i & 3) * 4;
-    const int r = row + (g >> 1) * 4 + (i >> 2);
-#pragma unroll
-    for (int p = 0; p < P; ++p) {
-        union {
-            i16x4 h[2];
-            u32x4 v;
-        } u;
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const int rr = r + 8 * t, chunk = (c >> 3) ^ chunk_xor<LD>(rr);
-            u.h[t] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (lds_i16x4 *)(lds + p * (TY * LD * 2) + rr * (LD * 2) + chunk * 16 + (c & 7) * 2));
-        }
-        f[p] = u.v;
-    }
-}
+typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
 
 // Eight values as the second product's operand.
 template <int P> __device__ __forceinline__ void pack8(const float (&x)[8], u32x4 (&f)[P]) {
@@ -227,16 +212,136 @@ template <int P> __device__ __forceinline__ void pack8(const float (&x)[8], u32x
         for (int e = 0; e < 8; ++e) v[e] = (__bf16)x[e];
         f[0] = __builtin_bit_cast(u32x4, v);
     } else {
-        f16x8 hi, lo;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            hi[e] = (_Float16)x[e];
-            lo[e] = (_Float16)(x[e] - (float)hi[e]);
+        for (int e = 0; e < 8; e += 2) {
+            const f16x2 hi = {(_Float16)x[e], (_Float16)x[e + 1]};
+            const uint32_t h = __builtin_bit_cast(uint32_t, hi);
+            float r0, r1;                // x - hi in one instruction each
+            asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r0) : "v"(h), "v"(x[e]));
+            asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
+                : "=v"(r1) : "v"(h), "v"(x[e + 1]));
+            const f16x2 lo = {(_Float16)r0, (_Float16)r1};
+            f[0][e / 2] = h;
+            f[1][e / 2] = __builtin_bit_cast(uint32_t, lo);
         }
-        f[0] = __builtin_bit_cast(u32x4, hi);
-        f[1] = __builtin_bit_cast(u32x4, lo);
     }
 }
+
+// The reads across, for the columns of two blocks of 32 (one with LD == 32): lane l gets
+// column l % 32 of the block and rows 4 (l / 32) + 0..3 and 8 + that.  They wait for
+// themselves: the compiler would have the builtin wait for the copies of the next
+// tile too, which no read here depends on.
+__device__ __forceinline__ uint32_t lds_address(const char *p) {
+    return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char *)p;
+}
+template <int LD> __device__ __forceinline__ int across_at() {
+    const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
+    const int r = (g >> 1) * 4 + (i >> 2), c = (g & 1) * 16 + (i & 3) * 4;
+    return r * (LD * 2) + ((c >> 3) ^ chunk_xor<LD>(r)) * 16 + (c & 7) * 2;
+}
+typedef __attribute__((ext_vector_type(2))) unsigned int u32x2;
+#define TR(dst, addr, off) "ds_read_b64_tr_b16 " dst ", " addr " offset:" off "\n\t"
+template <int P, int LD, int ROW, int COL>
+__device__ __forceinline__ void across(uint32_t at, u32x4 (&f)[2][P]) {
+    constexpr int R = LD * 2, O = ROW * R + COL * 2, PLANE = TY * R;
+    const uint32_t at1 = at ^ 64;                // the other block of the pair
+    u32x2 x[2][P][2];
+    if constexpr (LD == 32 && P == 1) {
+        asm volatile(TR("%0", "%2", "%3") TR("%1", "%2", "%4") "s_waitcnt lgkmcnt(0)"
+                     : "=&v"(x[0][0][0]), "=&v"(x[0][0][1])
+                     : "v"(at), "n"(O), "n"(O + 8 * R)
+                     : "memory");
+    } else if constexpr (LD == 32) {
+        asm volatile(TR("%0", "%4", "%5") TR("%1", "%4", "%6") TR("%2", "%4", "%7")
+                     TR("%3", "%4", "%8") "s_waitcnt lgkmcnt(0)"
+                     : "=&v"(x[0][0][0]), "=&v"(x[0][0][1]), "=&v"(x[0][1][0]), "=&v"(x[0][1][1])
+                     : "v"(at), "n"(O), "n"(O + 8 * R), "n"(PLANE + O), "n"(PLANE + O + 8 * R)
+                     : "memory");
+    } else if constexpr (P == 1) {
+        asm volatile(TR("%0", "%4", "%6") TR("%1", "%4", "%7") TR("%2", "%5", "%6")
+                     TR("%3", "%5", "%7") "s_waitcnt lgkmcnt(0)"
+                     : "=&v"(x[0][0][0]), "=&v"(x[0][0][1]), "=&v"(x[1][0][0]), "=&v"(x[1][0][1])
+                     : "v"(at), "v"(at1), "n"(O), "n"(O + 8 * R)
+                     : "memory");
+    } else {
+        asm volatile(TR("%0", "%8", "%10") TR("%1", "%8", "%11") TR("%2", "%8", "%12")
+                     TR("%3", "%8", "%13") TR("%4", "%9", "%10") TR("%5", "%9", "%11")
+                     TR("%6", "%9", "%12") TR("%7", "%9", "%13") "s_waitcnt lgkmcnt(0)"
+                     : "=&v"(x[0][0][0]), "=&v"(x[0][0][1]), "=&v"(x[0][1][0]), "=&v"(x[0][1][1]),
+                       "=&v"(x[1][0][0]), "=&v"(x[1][0][1]), "=&v"(x[1][1][0]), "=&v"(x[1][1][1])
+                     : "v"(at), "v"(at1), "n"(O), "n"(O + 8 * R), "n"(PLANE + O),
+                       "n"(PLANE + O + 8 * R)
+                     : "memory");
+    }
+#pragma unroll
+    for (int j = 0; j < (LD == 32 ? 1 : 2); ++j)
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+            f[j][p] = u32x4{x[j][p][0][0], x[j][p][0][1], x[j][p][1][0], x[j][p][1][1]};
+}
+#undef TR
+
+// O' += Y' P' for the 32 rows of Y from row Y on, P in p.
+template <int P, int KS, int Y>
+__device__ __forceinline__ void second_product(uint32_t at, const float (&p)[2][8],
+                                               f32x16 (&o)[(KS + 1) / 2]) {
+    constexpr int LD = row_ld(KS), JT = (KS + 1) / 2;
+    u32x4 b[2][P];
+    pack8<P>(p[0], b[0]);
+    pack8<P>(p[1], b[1]);
+    u32x4 a[2][P];
+    across<P, LD, Y, 0>(at, a);
+    o[0] = mma<P>(a[0], b[0], o[0]);
+    if constexpr (JT > 1) o[1] = mma<P>(a[1], b[0], o[1]);
+    if constexpr (JT > 2) {
+        across<P, LD, Y, 64>(at, a);
+        o[2] = mma<P>(a[0], b[0], o[2]);
+        if constexpr (JT > 3) o[3] = mma<P>(a[1], b[0], o[3]);
+    }
+    across<P, LD, Y + 16, 0>(at, a);
+    o[0] = mma<P>(a[0], b[1], o[0]);
+    if constexpr (JT > 1) o[1] = mma<P>(a[1], b[1], o[1]);
+    if constexpr (JT > 2) {
+        across<P, LD, Y + 16, 64>(at, a);
+        o[2] = mma<P>(a[0], b[1], o[2]);
+        if constexpr (JT > 3) o[3] = mma<P>(a[1], b[1], o[3]);
+    }
+}
+
+// S' of the 32 rows of Y from row y on: all of the operand is asked for first.
+template <int P, int KS>
+__device__ __forceinline__ f32x16 first_product(const char *tile, int y, const u32x4 (&x)[KS][P]) {
+    constexpr int LD = row_ld(KS), STEP = KS < 4 ? KS : 4;
+    f32x16 s;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = 0.0f;
+#pragma unroll
+    for (int q0 = 0; q0 < KS; q0 += STEP) {
+        u32x4 a[STEP][P];
+#pragma unroll
+        for (int q = 0; q < STEP; ++q)
+            if (q0 + q < KS) along<P, LD>(tile, y, q0 + q, a[q]);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int q = 0; q < STEP; ++q)
+            if (q0 + q < KS) s = mma<P>(a[q], x[q0 + q], s);
+    }
+    return s;
+}
+// The values of 16 rows of Y that go with a lane's registers of S'.
+template <typename V> __device__ __forceinline__ void of_rows(const V *rows, int y, V (&out)[16]) {
+    typedef __attribute__((ext_vector_type(4))) V V4;
+    const V *from = rows + y + ((threadIdx.x & 63) >> 5) * 4;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const V4 v = *reinterpret_cast<const V4 *>(from + 8 * q);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) out[q * 4 + e] = v[e];
+    }
+}
+template <int Y> struct At {
+    static constexpr int value = Y;
+};
 
 __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 64); }
 
@@ -287,21 +392,16 @@ __global__ __launch_bounds__(256, 2) void k_fused_rows(Fused k, int32_t splits,
         if (t + 1 < last) load(t + 1, buf ^ 1);
         const char *tile = lds + buf * BUF;
         const float *bias = reinterpret_cast<const float *>(tile + TILE_BYTES<P, LD>);
-#pragma unroll
-        for (int y = 0; y < TY; y += 32) {
-            f32x16 s;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = 0.0f;
-#pragma unroll
-            for (int q = 0; q < KS; ++q) {
-                u32x4 a[P];
-                along<P, LD>(tile, y, q, a);
-                s = mma<P>(a, x[q], s);
-            }
+        const uint32_t at = lds_address(tile) + across_at<LD>();
+        auto block = [&](auto where) {
+            constexpr int y = decltype(where)::value;
+            float b2[16];
+            of_rows(bias, y, b2);
+            f32x16 s = first_product<P, KS>(tile, y, x);
             float m = -INFINITY;
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                s[r] = __builtin_fmaf(s[r], sc, bias[y + (r >> 2) * 8 + half * 4 + (r & 3)]);
+                s[r] = __builtin_fmaf(s[r], sc, b2[r]);
                 m = fmaxf(m, s[r]);
             }
             // a new maximum: what was summed so far is brought to it
@@ -327,20 +427,10 @@ __global__ __launch_bounds__(256, 2) void k_fused_rows(Fused k, int32_t splits,
                 part[r & 1] += p[r >> 3][r & 7];
             }
             sum += part[0] + part[1];
-            if constexpr (GRAD) {
-#pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    u32x4 b[P];
-                    pack8<P>(p[q], b);
-#pragma unroll
-                    for (int j = 0; j < JT; ++j) {
-                        u32x4 a[P];
-                        across<P, LD>(tile, y + q * 16, j * 32, a);
-                        o[j] = mma<P>(a, b, o[j]);
-                    }
-                }
-            }
-        }
+            if constexpr (GRAD) second_product<P, KS, y>(at, p, o);
+        };
+        block(At<0>{});
+        block(At<32>{});
     }
     sum += other_half(sum);
     const int64_t at = split * k.n_pad + row;
@@ -356,48 +446,49 @@ __global__ __launch_bounds__(256, 2) void k_fused_rows(Fused k, int32_t splits,
     }
 }
 
-// The splits of a row joined, one wavefront a row; its label's score is summed in f32
+// The splits of a row joined, LD / 4 lanes a row; its label's score is summed in f32
 // from h and W themselves.
-template <typename T, bool GRAD>
-__global__ __launch_bounds__(256) void k_fused_join_rows(
-    Fused k, XentCall c, int32_t splits, int32_t ld, const float *__restrict__ part_o,
-    const float2 *__restrict__ part_ms) {
-    const int lane = threadIdx.x & 63;
-    const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (i >= k.n_pad) return;
+template <typename T, int LD, bool GRAD>
+__global__ __launch_bounds__(256) void k_fused_join_rows(Fused k, XentCall c, int32_t splits,
+                                                         const float *__restrict__ part_o,
+                                                         const float2 *__restrict__ part_ms) {
+    constexpr int LANES = LD / 4;
+    const int64_t i = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+    const int f = threadIdx.x % LANES * 4;
+    const int32_t y = k.label[i];
+    const bool open = y >= 0 && k.bias2[y] != -INFINITY;
+    float wy[4] = {0.0f, 0.0f, 0.0f, 0.0f}, dot = 0.0f;
+    if (open)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (f + e < k.d) {
+                wy[e] = load_f32<T>(c.w, y * c.w_stride + f + e);
+                dot += wy[e] * load_f32<T>(c.h, i * c.h_stride + f + e);
+            }
+#pragma unroll
+    for (int m = LANES / 2; m > 0; m >>= 1) dot += __shfl_xor(dot, m, 64);
     float ref = -INFINITY;
     for (int s = 0; s < splits; ++s) ref = fmaxf(ref, part_ms[s * k.n_pad + i].x);
     const bool none = ref == -INFINITY;
-    float sum = 0.0f, o[2] = {0.0f, 0.0f};
+    float sum = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int s = 0; s < splits; ++s) {
         const float2 ms = part_ms[s * k.n_pad + i];
         const float scale = none ? 1.0f : __builtin_amdgcn_exp2f(ms.x - ref);
         sum += ms.y * scale;
-        if constexpr (GRAD)
-#pragma unroll
-            for (int q = 0; q < 2; ++q)
-                if (lane + 64 * q < k.d)
-                    o[q] += part_o[(s * k.n_pad + i) * ld + lane + 64 * q] * scale;
-    }
-    const int32_t y = k.label[i];
-    // a sum that is not a number is one with no reference, too
-    const float l2 = none && sum == 0.0f ? -INFINITY : (none ? 0.0f : ref) + log2f(sum);
-    const float lse = y == -2 ? NAN : l2 * LN2;
-    const float wt = k.weight[i];
-    const bool open = y >= 0 && k.bias2[y] != -INFINITY;
-    float wy[2] = {0.0f, 0.0f}, dot = 0.0f;
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-        const int f = lane + 64 * q;
-        if (open && f < k.d) {
-            wy[q] = load_f32<T>(c.w, y * c.w_stride + f);
-            dot += wy[q] * load_f32<T>(c.h, i * c.h_stride + f);
+        if constexpr (GRAD) {
+            const float4 p = *reinterpret_cast<const float4 *>(part_o + (s * k.n_pad + i) * LD + f);
+            o[0] += p.x * scale;
+            o[1] += p.y * scale;
+            o[2] += p.z * scale;
+            o[3] += p.w * scale;
         }
     }
-#pragma unroll
-    for (int m = 32; m > 0; m >>= 1) dot += __shfl_xor(dot, m, 64);
-    if (lane == 0) {
+    // a sum that is not a number is one with no reference, too
+    const float l2 = none && sum == 0.0f ? -INFINITY : (none ? 0.0f : ref) + log2f(sum);
+    const float wt = k.weight[i];
+    if (f == 0) {
         if (i < k.n) {
+            const float lse = y == -2 ? NAN : l2 * LN2;
             const float z = open ? dot + (c.bias ? c.bias[y] : 0.0f) : -INFINITY;
             c.lse[i] = lse;
             c.loss[i] = y < 0 ? 0.0f : wt * (lse - z);
@@ -408,9 +499,7 @@ __global__ __launch_bounds__(256) void k_fused_join_rows(
                 k.wq[i] = wt;
             } else {
                 // weight 2^-exp and the power of two that brings the largest below 2^15
-                const uint32_t m = k.ctl->hg_max;
-                const int up = m ? min(126, max(-126, 27 - ilogbf(__uint_as_float(m)))) : 0;
-                const float q = ldexpf(wt, up - k.exp[i]);
+                const float q = ldexpf(wt, wq_exp(k.ctl->hg_max) - k.exp[i]);
                 k.wq[i] = fminf(fmaxf(q, -60000.0f), 60000.0f);
             }
         }
@@ -419,12 +508,11 @@ __global__ __launch_bounds__(256) void k_fused_join_rows(
         if (!c.dh || i >= k.n) return;
         const float scale = sizeof(T) == 4 ? ldexpf(1.0f, -scale_exp(k.ctl->w_max)) : 1.0f;
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-            const int f = lane + 64 * q;
-            if (f >= k.d) break;
-            const float g = y < 0 ? 0.0f : wt * (o[q] * scale / sum - wy[q]);
-            static_cast<T *>(c.dh)[i * c.h_stride + f] = (T)g;
-        }
+        for (int e = 0; e < 4; ++e)
+            if (f + e < k.d) {
+                const float g = y < 0 ? 0.0f : wt * (o[e] * scale / sum - wy[e]);
+                static_cast<T *>(c.dh)[i * c.h_stride + f + e] = (T)g;
+            }
     }
 }
 
@@ -481,49 +569,38 @@ __global__ __launch_bounds__(256, 2) void k_fused_classes_pass(Fused k, int32_t 
         const float *sc = reinterpret_cast<const float *>(tile + ROWS_AT), *c2 = sc + TY,
                     *wq = sc + 2 * TY, *weight = sc + 4 * TY;
         const int32_t *label = reinterpret_cast<const int32_t *>(sc + 3 * TY);
-#pragma unroll
-        for (int y = 0; y < TY; y += 32) {
-            f32x16 s;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = 0.0f;
-#pragma unroll
-            for (int q = 0; q < KS; ++q) {
-                u32x4 a[P];
-                along<P, LD>(tile, y, q, a);
-                s = mma<P>(a, x[q], s);
-            }
+        const uint32_t at = lds_address(tile) + across_at<LD>();
+        auto block = [&](auto where) {
+            constexpr int y = decltype(where)::value;
             const int64_t mine = label[y + (lane & 31)] - x0;
             const bool hot = __any(mine >= 0 && mine < 32);
-            float p[2][8];
+            f32x16 s = first_product<P, KS>(tile, y, x);
+            float p[2][8], of[16], of2[16];
+            of_rows(c2, y, of);
+            if (P == 2) of_rows(sc, y, of2);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int i = y + (r >> 2) * 8 + half * 4 + (r & 3);
-                float e = __builtin_amdgcn_exp2f(
-                    __builtin_fmaf(s[r], P == 1 ? LOG2E : sc[i], b2 - c2[i]));
-                p[r >> 3][r & 7] = e;
-            }
-            if (hot)
+            for (int r = 0; r < 16; ++r)
+                p[r >> 3][r & 7] = __builtin_amdgcn_exp2f(
+                    __builtin_fmaf(s[r], P == 1 ? LOG2E : of2[r], b2 - of[r]));
+            if (hot) {
+                int32_t l[16];
+                of_rows(label, y, l);
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
-                    if (label[y + (r >> 2) * 8 + half * 4 + (r & 3)] == v) p[r >> 3][r & 7] -= 1.0f;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int i = y + (r >> 2) * 8 + half * 4 + (r & 3);
-                if (part_db) db = __builtin_fmaf(p[r >> 3][r & 7], weight[i], db);
-                p[r >> 3][r & 7] *= wq[i];
+                    if (l[r] == v) p[r >> 3][r & 7] -= 1.0f;
             }
+            if (part_db) {
+                of_rows(weight, y, of);
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                u32x4 b[P];
-                pack8<P>(p[q], b);
-#pragma unroll
-                for (int j = 0; j < JT; ++j) {
-                    u32x4 a[P];
-                    across<P, LD>(tile, y + q * 16, j * 32, a);
-                    o[j] = mma<P>(a, b, o[j]);
-                }
+                for (int r = 0; r < 16; ++r) db = __builtin_fmaf(p[r >> 3][r & 7], of[r], db);
             }
-        }
+            of_rows(wq, y, of);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) p[r >> 3][r & 7] *= of[r];
+            second_product<P, KS, y>(at, p, o);
+        };
+        block(At<0>{});
+        block(At<32>{});
     }
     const int64_t at = split * k.v_pad + v;
     if (part_db) {
@@ -550,8 +627,7 @@ __global__ __launch_bounds__(256) void k_fused_join_classes(Fused k, XentCall c,
     const bool open = k.bias2[v] != -INFINITY;
     float scale = 1.0f;
     if (sizeof(T) == 4) {
-        const uint32_t m = k.ctl->hg_max;
-        scale = ldexpf(1.0f, -(m ? min(126, max(-126, 27 - ilogbf(__uint_as_float(m)))) : 0));
+        scale = ldexpf(1.0f, -wq_exp(k.ctl->hg_max));
     }
     if (c.dw)
 #pragma unroll
@@ -559,6 +635,7 @@ __global__ __launch_bounds__(256) void k_fused_join_classes(Fused k, XentCall c,
             const int f = lane + 64 * q;
             if (f >= k.d) break;
             float sum = 0.0f;
+#pragma unroll 8
             for (int s = 0; s < splits; ++s) sum += part[(s * k.v_pad + v) * ld + f];
             static_cast<T *>(c.dw)[v * c.w_stride + f] = (T)(open ? sum * scale : 0.0f);
         }
@@ -666,17 +743,17 @@ hipError_t run(hipStream_t s, const XentCall &c, const Plan &p, char *m) {
                        c.bias);
     hipLaunchKernelGGL((k_fused_pack<T>), dim3(blocks(k.v_pad + k.n_pad, 4)), b, 0, s, k, LD, c.w,
                        c.w_stride, c.h, c.h_stride, c.labels, c.weights);
-    const dim3 gr((uint32_t)(k.n_pad / XB * p.row_splits)), gj(blocks(k.n_pad, 4));
+    const dim3 gr((uint32_t)(k.n_pad / XB * p.row_splits)), gj(blocks(k.n_pad, 1024 / LD));
     if (!c.grad) {
         hipLaunchKernelGGL((k_fused_rows<P, KS, false>), gr, b, lds_rows, s, k, p.row_splits,
                            static_cast<float *>(nullptr), part_ms);
-        hipLaunchKernelGGL((k_fused_join_rows<T, false>), gj, b, 0, s, k, c, p.row_splits, LD, part,
+        hipLaunchKernelGGL((k_fused_join_rows<T, LD, false>), gj, b, 0, s, k, c, p.row_splits, part,
                            part_ms);
         return hipGetLastError();
     }
     hipLaunchKernelGGL((k_fused_rows<P, KS, true>), gr, b, lds_rows, s, k, p.row_splits, part,
                        part_ms);
-    hipLaunchKernelGGL((k_fused_join_rows<T, true>), gj, b, 0, s, k, c, p.row_splits, LD, part,
+    hipLaunchKernelGGL((k_fused_join_rows<T, LD, true>), gj, b, 0, s, k, c, p.row_splits, part,
                        part_ms);
     if (c.dw || c.dbias) {
         hipLaunchKernelGGL((k_fused_classes_pass<P, KS>),

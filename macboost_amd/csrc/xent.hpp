@@ -39,6 +39,11 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
     return v;
 }
 
+// *max = max(*max, v): most calls find it there already, and leave the line alone.
+__device__ __forceinline__ void raise(uint32_t *max, uint32_t v) {
+    if (v > __atomic_load_n(max, __ATOMIC_RELAXED)) atomicMax(max, v);
+}
+
 __device__ __forceinline__ u16 bits_of(__bf16 v) { return __builtin_bit_cast(u16, v); }
 __device__ __forceinline__ u16 bits_of(_Float16 v) { return __builtin_bit_cast(u16, v); }
 
