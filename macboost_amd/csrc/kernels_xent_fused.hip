@@ -27,6 +27,8 @@ namespace mbk {
 
 namespace {
 
+typedef __attribute__((ext_vector_type(4))) unsigned short u16x4;
+
 constexpr int XB = 128;                  // X rows of a workgroup, 32 a wavefront
 constexpr int TY = 64;                   // Y rows of a tile
 constexpr float LN2 = 0.69314718055994531f;
@@ -69,102 +71,123 @@ template <typename T> __device__ __forceinline__ float load_f32(const void *p, i
     return (float)static_cast<const T *>(p)[i];
 }
 
+// Up to four elements of a row from f on, zeros behind the row.
 template <typename T>
-__global__ __launch_bounds__(256) void k_fused_classes(Fused k, const void *w, int64_t stride,
-                                                       const float *__restrict__ bias) {
-    const int lane = threadIdx.x & 63;
-    const int64_t v = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (v >= k.v_pad) return;
-    const float b = v < k.v ? (bias ? bias[v] : 0.0f) : -INFINITY;
-    const bool open = b != -INFINITY;
-    if (lane == 0) {
-        k.bias2[v] = b * LOG2E;
-        if (open && !k.ctl->open) k.ctl->open = 1u;
-    }
-    if (sizeof(T) == 2 || !open) return;
-    uint32_t m = 0;
-    for (int32_t f = lane; f < k.d; f += 64) m = max(m, finite_bits(load_f32<T>(w, v * stride + f)));
-    m = wave_max(m);
-    if (lane == 0) raise(&k.ctl->w_max, m);
+__device__ __forceinline__ void load4(const void *p, int64_t row, int f, int d, float (&x)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = f + e < d ? load_f32<T>(p, row + f + e) : 0.0f;
+}
+__device__ __forceinline__ uint32_t finite_max(const float (&x)[4]) {
+    return max(max(finite_bits(x[0]), finite_bits(x[1])), max(finite_bits(x[2]), finite_bits(x[3])));
+}
+// The workgroup's largest goes to *max: few atomics on one word.
+__device__ __forceinline__ void raise_by_block(uint32_t *max, uint32_t v) {
+    __shared__ uint32_t most[4];
+    v = wave_max(v);
+    if ((threadIdx.x & 63) == 0) most[threadIdx.x >> 6] = v;
+    __syncthreads();
+    if (threadIdx.x == 0) raise(max, ::max(::max(most[0], most[1]), ::max(most[2], most[3])));
 }
 
-// One wavefront a packed row, of W and then of h.
-template <typename T>
-__global__ __launch_bounds__(256) void k_fused_pack(Fused k, int32_t ld, const void *w,
-                                                    int64_t w_stride, const void *h,
-                                                    int64_t h_stride,
+// LD / 4 lanes a row in the kernels that prepare and join, and a grid that goes over
+// the rows in turns.
+template <typename T, int LD>
+__global__ __launch_bounds__(256) void k_fused_classes(Fused k, const void *w, int64_t stride,
+                                                       const float *__restrict__ bias) {
+    constexpr int LANES = LD / 4, ROWS = 256 / LANES;
+    const int f = threadIdx.x % LANES * 4;
+    uint32_t m = 0;
+    bool any = false;
+    for (int64_t v = (int64_t)blockIdx.x * ROWS + threadIdx.x / LANES; v < k.v_pad;
+         v += (int64_t)gridDim.x * ROWS) {
+        const float b = v < k.v ? (bias ? bias[v] : 0.0f) : -INFINITY;
+        const bool open = b != -INFINITY;
+        any = any || open;
+        if (f == 0) k.bias2[v] = b * LOG2E;
+        if (sizeof(T) == 2 || !open) continue;
+        float x[4];
+        load4<T>(w, v * stride, f, k.d, x);
+        m = max(m, finite_max(x));
+    }
+    if (any && !k.ctl->open) k.ctl->open = 1u;
+    if (sizeof(T) == 4) raise_by_block(&k.ctl->w_max, m);
+}
+
+// The packed rows of W and then of h.
+template <typename T, int LD>
+__global__ __launch_bounds__(256) void k_fused_pack(Fused k, const void *w, int64_t w_stride,
+                                                    const void *h, int64_t h_stride,
                                                     const int32_t *__restrict__ labels,
                                                     const float *__restrict__ weights) {
-    const int lane = threadIdx.x & 63;
-    int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const bool of_w = i < k.v_pad;
-    if (!of_w) i -= k.v_pad;
-    if (!of_w && i >= k.n_pad) return;
+    constexpr int LANES = LD / 4, ROWS = 256 / LANES;
+    const int f = threadIdx.x % LANES * 4;
     const int sw = sizeof(T) == 4 ? scale_exp(k.ctl->w_max) : 0;
-    const void *src = of_w ? w : h;
-    const int64_t at = i * (of_w ? w_stride : h_stride);
-    bool in = of_w ? i < k.v && k.bias2[i] != -INFINITY : i < k.n;
-    float x[2];
-    uint32_t m = 0;
-    bool finite = true;
+    const bool any = k.ctl->open;
+    uint32_t hg = 0;
+    for (int64_t at = (int64_t)blockIdx.x * ROWS + threadIdx.x / LANES; at < k.v_pad + k.n_pad;
+         at += (int64_t)gridDim.x * ROWS) {
+        const bool of_w = at < k.v_pad;
+        const int64_t i = of_w ? at : at - k.v_pad;
+        float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        int s = sw;
+        if (of_w) {
+            if (k.bias2[i] != -INFINITY) load4<T>(w, i * w_stride, f, k.d, x);
+        } else {
+            if (i < k.n) load4<T>(h, i * h_stride, f, k.d, x);
+            int32_t y = i < k.n ? labels[i] : -1;
+            float wt = i < k.n ? (weights ? weights[i] : 1.0f) : 0.0f;
+            uint32_t m = finite_max(x);
+            uint32_t most = m;                   // of all values, finite or not
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-        const int f = lane + 64 * q;
-        x[q] = in && f < k.d ? load_f32<T>(src, at + f) : 0.0f;
-        const uint32_t b = __float_as_uint(fabsf(x[q]));
-        finite = finite && b < HUGE_BITS;
-        m = max(m, finite_bits(x[q]));
-    }
-    int s = sw;
-    if (!of_w) {
-        int32_t y = i < k.n ? labels[i] : -1;
-        float wt = i < k.n ? (weights ? weights[i] : 1.0f) : 0.0f;
-        if (y < 0 || y >= k.v || wt == 0.0f || !k.ctl->open) {
-            wt = 0.0f;
-            y = -1;
-            if (__ballot(!finite)) {
-                y = -2;
-                x[0] = x[1] = 0.0f;
-                m = 0;
+            for (int e = 0; e < 4; ++e) most = max(most, __float_as_uint(fabsf(x[e])));
+#pragma unroll
+            for (int o = LANES / 2; o > 0; o >>= 1) {
+                m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
+                most = max(most, (uint32_t)__shfl_xor((int)most, o, 64));
+            }
+            if (y < 0 || y >= k.v || wt == 0.0f || !any) {
+                wt = 0.0f;
+                y = -1;
+                if (most >= HUGE_BITS) {
+                    y = -2;
+                    m = 0;
+                    x[0] = x[1] = x[2] = x[3] = 0.0f;
+                }
+            }
+            if (sizeof(T) == 4) s = scale_exp(m);
+            if (f == 0) {
+                k.label[i] = y;
+                k.weight[i] = wt;
+                k.exp[i] = s;
+                k.sc[i] = sizeof(T) == 4 ? ldexpf(LOG2E, -(s + sw)) : LOG2E;
+                if (wt != 0.0f) hg = max(hg, finite_bits(wt * __uint_as_float(m)));
             }
         }
-        if (sizeof(T) == 4) {
-            m = wave_max(m);
-            s = scale_exp(m);
-        }
-        if (lane == 0) {
-            k.label[i] = y;
-            k.weight[i] = wt;
-            k.exp[i] = s;
-            k.sc[i] = sizeof(T) == 4 ? ldexpf(LOG2E, -(s + sw)) : LOG2E;
-            if (sizeof(T) == 4 && wt != 0.0f)
-                raise(&k.ctl->hg_max, finite_bits(wt * __uint_as_float(m)));
-        }
-    }
-    u16 *row = (of_w ? k.w : k.h) + i * ld;
-    const int64_t plane = (of_w ? k.v_pad : k.n_pad) * ld;
+        u16 *row = (of_w ? k.w : k.h) + i * LD + f;
+        u16 hi[4], lo[4];
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-        const int f = lane + 64 * q;
-        if (f >= ld) break;
-        if (sizeof(T) == 2) {
-            row[f] = bits_of((__bf16)x[q]);
-        } else {
-            u16 hi, lo;
-            split_f16(ldexpf(x[q], s), hi, lo);
-            row[f] = hi;
-            row[plane + f] = lo;
+        for (int e = 0; e < 4; ++e) {
+            if (sizeof(T) == 2) hi[e] = bits_of((__bf16)x[e]);
+            else split_f16(ldexpf(x[e], s), hi[e], lo[e]);
         }
+        *reinterpret_cast<u16x4 *>(row) = u16x4{hi[0], hi[1], hi[2], hi[3]};
+        if (sizeof(T) == 4)
+            *reinterpret_cast<u16x4 *>(row + (of_w ? k.v_pad : k.n_pad) * LD) =
+                u16x4{lo[0], lo[1], lo[2], lo[3]};
     }
+    if (sizeof(T) == 4) raise_by_block(&k.ctl->hg_max, hg);
 }
 
 // ---- a tile in LDS -----------------------------------------------------------------
 // TY rows of LD elements a plane, the 16-byte chunks of a row permuted by the row so
-// that the 8 rows x 1 chunk of an operand's read and the 4 rows x 2 chunks of a read
-// across both fall on different banks.
+// that the 16 rows x 1 chunk of a read along and the 4 rows x 4 chunks of a read
+// across fall on all 64 banks.  Rows 8 apart differ in bit 1 alone, rows 16 apart not
+// at all.
 template <int LD> __device__ __forceinline__ int chunk_xor(int row) {
-    if constexpr (LD == 32) return ((row >> 1) & 1) * 2 + ((row >> 2) & 1);
-    else return (row & 3) * 2 + ((row >> 2) & 1);
+    const int low = (row >> 2) & 3;
+    if constexpr (LD == 32) return low;
+    else if constexpr (LD == 64) return ((row >> 1) & 1) * 4 + low;
+    else return (row & 3) * 4 + low;
 }
 template <int P, int LD> constexpr int TILE_BYTES = P * TY * LD * 2;
 
@@ -243,34 +266,35 @@ typedef __attribute__((ext_vector_type(2))) unsigned int u32x2;
 #define TR(dst, addr, off) "ds_read_b64_tr_b16 " dst ", " addr " offset:" off "\n\t"
 template <int P, int LD, int ROW, int COL>
 __device__ __forceinline__ void across(uint32_t at, u32x4 (&f)[2][P]) {
-    constexpr int R = LD * 2, O = ROW * R + COL * 2, PLANE = TY * R;
-    const uint32_t at1 = at ^ 64;                // the other block of the pair
+    constexpr int R = LD * 2, O = ROW * R, O8 = O + 8 * R, PLANE = TY * R;
+    // the block's columns, its rows 8 further, and both for the pair's other block
+    const uint32_t a0 = at ^ (COL * 2), a8 = a0 ^ 32, b0 = a0 ^ 64, b8 = a0 ^ 96;
     u32x2 x[2][P][2];
     if constexpr (LD == 32 && P == 1) {
-        asm volatile(TR("%0", "%2", "%3") TR("%1", "%2", "%4") "s_waitcnt lgkmcnt(0)"
+        asm volatile(TR("%0", "%2", "%4") TR("%1", "%3", "%5") "s_waitcnt lgkmcnt(0)"
                      : "=&v"(x[0][0][0]), "=&v"(x[0][0][1])
-                     : "v"(at), "n"(O), "n"(O + 8 * R)
+                     : "v"(a0), "v"(a8), "n"(O), "n"(O8)
                      : "memory");
     } else if constexpr (LD == 32) {
-        asm volatile(TR("%0", "%4", "%5") TR("%1", "%4", "%6") TR("%2", "%4", "%7")
-                     TR("%3", "%4", "%8") "s_waitcnt lgkmcnt(0)"
+        asm volatile(TR("%0", "%4", "%6") TR("%1", "%5", "%7") TR("%2", "%4", "%8")
+                     TR("%3", "%5", "%9") "s_waitcnt lgkmcnt(0)"
                      : "=&v"(x[0][0][0]), "=&v"(x[0][0][1]), "=&v"(x[0][1][0]), "=&v"(x[0][1][1])
-                     : "v"(at), "n"(O), "n"(O + 8 * R), "n"(PLANE + O), "n"(PLANE + O + 8 * R)
+                     : "v"(a0), "v"(a8), "n"(O), "n"(O8), "n"(PLANE + O), "n"(PLANE + O8)
                      : "memory");
     } else if constexpr (P == 1) {
-        asm volatile(TR("%0", "%4", "%6") TR("%1", "%4", "%7") TR("%2", "%5", "%6")
-                     TR("%3", "%5", "%7") "s_waitcnt lgkmcnt(0)"
+        asm volatile(TR("%0", "%4", "%8") TR("%1", "%5", "%9") TR("%2", "%6", "%8")
+                     TR("%3", "%7", "%9") "s_waitcnt lgkmcnt(0)"
                      : "=&v"(x[0][0][0]), "=&v"(x[0][0][1]), "=&v"(x[1][0][0]), "=&v"(x[1][0][1])
-                     : "v"(at), "v"(at1), "n"(O), "n"(O + 8 * R)
+                     : "v"(a0), "v"(a8), "v"(b0), "v"(b8), "n"(O), "n"(O8)
                      : "memory");
     } else {
-        asm volatile(TR("%0", "%8", "%10") TR("%1", "%8", "%11") TR("%2", "%8", "%12")
-                     TR("%3", "%8", "%13") TR("%4", "%9", "%10") TR("%5", "%9", "%11")
-                     TR("%6", "%9", "%12") TR("%7", "%9", "%13") "s_waitcnt lgkmcnt(0)"
+        asm volatile(TR("%0", "%8", "%12") TR("%1", "%9", "%13") TR("%2", "%8", "%14")
+                     TR("%3", "%9", "%15") TR("%4", "%10", "%12") TR("%5", "%11", "%13")
+                     TR("%6", "%10", "%14") TR("%7", "%11", "%15") "s_waitcnt lgkmcnt(0)"
                      : "=&v"(x[0][0][0]), "=&v"(x[0][0][1]), "=&v"(x[0][1][0]), "=&v"(x[0][1][1]),
                        "=&v"(x[1][0][0]), "=&v"(x[1][0][1]), "=&v"(x[1][1][0]), "=&v"(x[1][1][1])
-                     : "v"(at), "v"(at1), "n"(O), "n"(O + 8 * R), "n"(PLANE + O),
-                       "n"(PLANE + O + 8 * R)
+                     : "v"(a0), "v"(a8), "v"(b0), "v"(b8), "n"(O), "n"(O8), "n"(PLANE + O),
+                       "n"(PLANE + O8)
                      : "memory");
     }
 #pragma unroll
@@ -353,7 +377,7 @@ __global__ __launch_bounds__(256, 2) void k_fused_rows(Fused k, int32_t splits,
                                                        float *__restrict__ part_o,
                                                        float2 *__restrict__ part_ms) {
     constexpr int LD = row_ld(KS), JT = (KS + 1) / 2;
-    constexpr int BUF = TILE_BYTES<P, LD> + TY * 4;
+    constexpr int BUF = TILE_BYTES<P, LD> + TY * 4;      // a multiple of 256: see across
     extern __shared__ char lds[];
     const int lane = threadIdx.x & 63, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -393,6 +417,7 @@ __global__ __launch_bounds__(256, 2) void k_fused_rows(Fused k, int32_t splits,
         const char *tile = lds + buf * BUF;
         const float *bias = reinterpret_cast<const float *>(tile + TILE_BYTES<P, LD>);
         const uint32_t at = lds_address(tile) + across_at<LD>();
+        static_assert(BUF % 256 == 0, "reads across xor the low bits of the address");
         auto block = [&](auto where) {
             constexpr int y = decltype(where)::value;
             float b2[16];
@@ -570,6 +595,7 @@ __global__ __launch_bounds__(256, 2) void k_fused_classes_pass(Fused k, int32_t 
                     *wq = sc + 2 * TY, *weight = sc + 4 * TY;
         const int32_t *label = reinterpret_cast<const int32_t *>(sc + 3 * TY);
         const uint32_t at = lds_address(tile) + across_at<LD>();
+        static_assert(BUF % 256 == 0, "reads across xor the low bits of the address");
         auto block = [&](auto where) {
             constexpr int y = decltype(where)::value;
             const int64_t mine = label[y + (lane & 31)] - x0;
@@ -679,7 +705,7 @@ struct Plan {
 Plan plan_of(const XentCall &c) {
     Plan p{};
     p.P = c.bf16 ? 1 : 2;
-    p.ks = c.dim <= 32 ? 2 : c.dim <= 64 ? 4 : 8;
+    p.ks = (c.dim + 15) / 16;
     p.ld = row_ld(p.ks);
     p.n_pad = up(c.rows, XB);
     p.v_pad = up(c.classes, XB);
@@ -739,10 +765,12 @@ hipError_t run(hipStream_t s, const XentCall &c, const Plan &p, char *m) {
         if (e != hipSuccess) return e;
     }
     hipLaunchKernelGGL(k_fused_init, dim3(1), dim3(1), 0, s, k.ctl);
-    hipLaunchKernelGGL((k_fused_classes<T>), dim3(blocks(k.v_pad, 4)), b, 0, s, k, c.w, c.w_stride,
-                       c.bias);
-    hipLaunchKernelGGL((k_fused_pack<T>), dim3(blocks(k.v_pad + k.n_pad, 4)), b, 0, s, k, LD, c.w,
-                       c.w_stride, c.h, c.h_stride, c.labels, c.weights);
+    const auto grid = [&](int64_t rows) {
+        return dim3(std::min<uint32_t>(blocks(rows, 1024 / LD), 8 * (uint32_t)c.num_cus));
+    };
+    hipLaunchKernelGGL((k_fused_classes<T, LD>), grid(k.v_pad), b, 0, s, k, c.w, c.w_stride, c.bias);
+    hipLaunchKernelGGL((k_fused_pack<T, LD>), grid(k.v_pad + k.n_pad), b, 0, s, k, c.w, c.w_stride,
+                       c.h, c.h_stride, c.labels, c.weights);
     const dim3 gr((uint32_t)(k.n_pad / XB * p.row_splits)), gj(blocks(k.n_pad, 1024 / LD));
     if (!c.grad) {
         hipLaunchKernelGGL((k_fused_rows<P, KS, false>), gr, b, lds_rows, s, k, p.row_splits,
@@ -768,8 +796,13 @@ hipError_t run(hipStream_t s, const XentCall &c, const Plan &p, char *m) {
 template <int P, typename T>
 hipError_t run_dim(hipStream_t s, const XentCall &c, const Plan &p, char *m) {
     switch (p.ks) {
+    case 1: return run<P, 1, T>(s, c, p, m);
     case 2: return run<P, 2, T>(s, c, p, m);
+    case 3: return run<P, 3, T>(s, c, p, m);
     case 4: return run<P, 4, T>(s, c, p, m);
+    case 5: return run<P, 5, T>(s, c, p, m);
+    case 6: return run<P, 6, T>(s, c, p, m);
+    case 7: return run<P, 7, T>(s, c, p, m);
     default: return run<P, 8, T>(s, c, p, m);
     }
 }
