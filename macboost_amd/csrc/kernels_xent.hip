@@ -21,9 +21,10 @@
 // two that puts the largest element of h's row, or of all of W, below 2^14, so that
 // elements down to 2^-38 of it keep a step of their own.
 //
-// Rows that are out (label outside [0, V), weight 0, or no class offered) and classes
-// not offered (bias -inf) are packed as zeros wherever another row or class would
-// meet them, so what they hold reaches nothing.
+// Classes not offered (bias -inf) are packed as zeros, and so are rows that are out
+// (label outside [0, V), weight 0, or no class offered) and hold NaN, infinities or values
+// that could overflow: what they hold reaches nothing, and a finite row that is out is
+// multiplied by zeros.
 #include <algorithm>
 
 #include "mbk.h"
@@ -56,7 +57,7 @@ __global__ __launch_bounds__(256) void k_xent_classes(XentPack k, const void *w,
     const float b = v < k.v ? (bias ? bias[v] : 0.0f) : -INFINITY;
     const bool open = b != -INFINITY;
     if (lane == 0) {
-        k.bias[v] = b;
+        k.bias[v] = b * LOG2E;
         if (open && !k.ctl->open) k.ctl->open = 1u;
     }
     if (sizeof(T) == 2 || !open) return;
@@ -87,7 +88,8 @@ __global__ __launch_bounds__(256) void k_xent_pack_w(XentPack k, const void *w, 
     }
 }
 
-// Rows: label and weight (-1 and 0 where the row is out), h scaled by row.
+// Rows: label and weight (-1 and 0 where the row is out), h scaled by row.  A row that
+// is out and not finite is packed as zeros, its label -2.
 template <typename T>
 __global__ __launch_bounds__(256) void k_xent_rows(XentPack k, const void *h, int64_t stride,
                                                    const int32_t *__restrict__ labels,
@@ -97,27 +99,38 @@ __global__ __launch_bounds__(256) void k_xent_rows(XentPack k, const void *h, in
     if (i >= k.n_pad) return;
     int32_t y = i < k.n ? labels[i] : -1;
     float wt = i < k.n ? (weights ? weights[i] : 1.0f) : 0.0f;
-    if (y < 0 || y >= k.v || wt == 0.0f || !k.ctl->open) { y = -1; wt = 0.0f; }
+    const bool out = y < 0 || y >= k.v || wt == 0.0f || !k.ctl->open;
     int s = 0;
-    if (sizeof(T) == 4) {
-        uint32_t m = 0;
-        if (i < k.n)
-            for (int32_t f = lane; f < k.d; f += 64)
-                m = max(m, finite_bits(load_f32<T>(h, i * stride + f)));
-        m = wave_max(m);
-        s = scale_exp(m);
-        if (lane == 0) {
-            k.row_scale[i] = ldexpf(1.0f, -s);
-            if (wt != 0.0f) raise(&k.ctl->hg_max, finite_bits(wt * __uint_as_float(m)));
+    bool zeros = i >= k.n;
+    if (out) {
+        y = -1;
+        wt = 0.0f;
+    }
+    if ((out || sizeof(T) == 4) && i < k.n) {
+        uint32_t m = 0, most = 0;
+        for (int32_t f = lane; f < k.d; f += 64) {
+            const float x = load_f32<T>(h, i * stride + f);
+            m = max(m, finite_bits(x));
+            most = max(most, __float_as_uint(fabsf(x)));
         }
+        m = wave_max(m);
+        if (out && wave_max(most) >= XENT_HUGE) {
+            y = -2;
+            m = 0;
+            zeros = true;
+        }
+        if (sizeof(T) == 4) s = scale_exp(m);
+        if (sizeof(T) == 4 && lane == 0 && wt != 0.0f)
+            raise(&k.ctl->hg_max, finite_bits(wt * __uint_as_float(m)));
     }
     if (lane == 0) {
+        if (sizeof(T) == 4) k.row_scale[i] = ldexpf(LOG2E, -(s + scale_exp(k.ctl->w_max)));
         k.label[i] = y;
         k.weight[i] = wt;
     }
     u16 *row = k.h + i * k.ld;
     for (int32_t f = lane; f < k.ld; f += 64) {
-        const bool in = i < k.n && f < k.d;
+        const bool in = !zeros && f < k.d;
         if (sizeof(T) == 2) {
             row[f] = in ? static_cast<const u16 *>(h)[i * stride + f] : 0;
         } else {
@@ -129,27 +142,21 @@ __global__ __launch_bounds__(256) void k_xent_rows(XentPack k, const void *h, in
     }
 }
 
-// h as dW's product takes it: rows that are out are zeros; f32: times the row's
-// weight, with one scale for all rows (they are summed over).
-template <typename T>
-__global__ __launch_bounds__(256) void k_xent_pack_hg(XentPack k, const void *h, int64_t stride) {
+// f32: h as dW's product takes it, times the row's weight and with one scale for all
+// rows (they are summed over).
+__global__ __launch_bounds__(256) void k_xent_pack_hg(XentPack k, const float *h, int64_t stride) {
     const int lane = threadIdx.x & 63;
     const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (i >= k.n_pad) return;
     const bool live = k.label[i] >= 0;
     const float wt = k.weight[i];
-    const int s = sizeof(T) == 4 ? scale_exp(k.ctl->hg_max) : 0;
+    const int s = scale_exp(k.ctl->hg_max);
     u16 *row = k.hg + i * k.ld;
     for (int32_t f = lane; f < k.ld; f += 64) {
-        const bool in = live && f < k.d;
-        if (sizeof(T) == 2) {
-            row[f] = in ? static_cast<const u16 *>(h)[i * stride + f] : 0;
-        } else {
-            u16 hi, lo;
-            split_f16(in ? ldexpf(wt * load_f32<T>(h, i * stride + f), s) : 0.0f, hi, lo);
-            row[f] = hi;
-            row[k.n_pad * k.ld + f] = lo;
-        }
+        u16 hi, lo;
+        split_f16(live && f < k.d ? ldexpf(wt * h[i * stride + f], s) : 0.0f, hi, lo);
+        row[f] = hi;
+        row[k.n_pad * k.ld + f] = lo;
     }
 }
 
@@ -301,33 +308,38 @@ __device__ __forceinline__ int block_row(int r) {
 // ---- pass 1: each row's maximum and sum ---------------------------------------------
 // The product is W h' (classes down, rows across), so that a lane has scores of one
 // row: the maximum and sum stay in registers over the classes of a split, and only
-// two lanes and two wavefronts have parts of a row.  part[2 * split + half][row].
+// two lanes and two wavefronts have parts of a row.  part[2 * split + half][row]: the
+// maximum of z log2 e, and the sum of its powers of 2.
 template <int P>
-__global__ __launch_bounds__(256) void k_xent_stats(XentPack k, int64_t class_tiles, int32_t splits,
-                                                    float2 *__restrict__ part,
-                                                    float *__restrict__ z_label) {
+__global__ __launch_bounds__(256, 2) void k_xent_stats(XentPack k, int64_t class_tiles,
+                                                       int32_t splits,
+                                                       float2 *__restrict__ part) {
     extern __shared__ char lds[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t i0 = (int64_t)(blockIdx.x / splits) * TILE;
     const int32_t split = blockIdx.x % splits;
     const Operand a{k.w, k.v_pad * k.ld, k.ld}, b{k.h, k.n_pad * k.ld, k.ld};
     const int64_t steps = (k.d + BK<P> - 1) / BK<P>;
-    const float ws = P == 2 ? ldexpf(1.0f, -scale_exp(k.ctl->w_max)) : 1.0f;
-    float m[2], s[2], hs[2];
-    int32_t label[2];
+    float m[2], s[2], sc[2];
     int64_t row[2];
 #pragma unroll
     for (int y = 0; y < 2; ++y) {
         row[y] = i0 + (wave & 1) * 64 + y * 32 + (lane & 31);
         m[y] = -INFINITY;
         s[y] = 0.0f;
-        hs[y] = P == 2 ? k.row_scale[row[y]] : 1.0f;
-        label[y] = k.label[row[y]];
+        sc[y] = P == 2 ? k.row_scale[row[y]] : LOG2E;
     }
     for (int64_t t = split; t < class_tiles; t += splits) {
         f32x16 acc[2][2];
         clear(acc);
         tile_product<P, true, true>(a, b, t * TILE, i0, steps, lds, acc);
+        const float *bias = k.bias + t * TILE + (wave >> 1) * 64 + (lane >> 5) * 4;
+        float4 b2[2][4];
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                b2[x][q] = *reinterpret_cast<const float4 *>(bias + x * 32 + q * 8);
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
             float top = m[y];
@@ -335,101 +347,121 @@ __global__ __launch_bounds__(256) void k_xent_stats(XentPack k, int64_t class_ti
             for (int x = 0; x < 2; ++x)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    const int64_t v = t * TILE + (wave >> 1) * 64 + x * 32 + block_row(r);
-                    float z = acc[x][y][r];
-                    if (P == 2) z = z * hs[y] * ws;
-                    z += k.bias[v];
-                    acc[x][y][r] = z;
-                    top = fmaxf(top, z);
-                    if (v == label[y]) z_label[row[y]] = z;
+                    const float4 q = b2[x][r >> 2];
+                    const float b = (r & 3) == 0 ? q.x : (r & 3) == 1 ? q.y : (r & 3) == 2 ? q.z : q.w;
+                    acc[x][y][r] = __builtin_fmaf(acc[x][y][r], sc[y], b);
+                    top = fmaxf(top, acc[x][y][r]);
                 }
             const float ref = top == -INFINITY ? 0.0f : top;
-            float sum = s[y] * __builtin_amdgcn_exp2f((m[y] - ref) * LOG2E);
+            float sum[2] = {s[y] * __builtin_amdgcn_exp2f(m[y] - ref), 0.0f};
 #pragma unroll
             for (int x = 0; x < 2; ++x)
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
-                    sum += __builtin_amdgcn_exp2f((acc[x][y][r] - ref) * LOG2E);
+                    sum[r & 1] += __builtin_amdgcn_exp2f(acc[x][y][r] - ref);
             m[y] = top;
-            s[y] = sum;
+            s[y] = sum[0] + sum[1];
         }
     }
 #pragma unroll
     for (int y = 0; y < 2; ++y) {
         const float m2 = __shfl_xor(m[y], 32, 64), s2 = __shfl_xor(s[y], 32, 64);
         const float top = fmaxf(m[y], m2), ref = top == -INFINITY ? 0.0f : top;
-        const float sum = s[y] * __builtin_amdgcn_exp2f((m[y] - ref) * LOG2E) +
-                          s2 * __builtin_amdgcn_exp2f((m2 - ref) * LOG2E);
+        const float sum = s[y] * __builtin_amdgcn_exp2f(m[y] - ref) +
+                          s2 * __builtin_amdgcn_exp2f(m2 - ref);
         if (lane < 32)
             part[(2 * split + (wave >> 1)) * k.n_pad + row[y]] = make_float2(top, sum);
     }
 }
 
-// The parts of a row joined, in order: lse and loss.
-__global__ __launch_bounds__(256) void k_xent_join(XentPack k, int32_t parts,
+// The parts of a row joined, one wavefront a row: lse and loss.  The label's score is
+// summed in f32 from h and W themselves.
+template <typename T>
+__global__ __launch_bounds__(256) void k_xent_join(XentPack k, XentCall c, int32_t parts,
                                                    const float2 *__restrict__ part,
-                                                   const float *__restrict__ z_label,
-                                                   float *__restrict__ lse_pad,
-                                                   float *__restrict__ loss,
-                                                   float *__restrict__ lse) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+                                                   float *__restrict__ lse2) {
+    const int lane = threadIdx.x & 63;
+    const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (i >= k.n_pad) return;
-    float top = -INFINITY;
-    for (int p = 0; p < parts; ++p) top = fmaxf(top, part[p * k.n_pad + i].x);
-    const float ref = top == -INFINITY ? 0.0f : top;
-    float sum = 0.0f;
-    for (int p = 0; p < parts; ++p) {
-        const float2 c = part[p * k.n_pad + i];
-        sum += c.y * __builtin_amdgcn_exp2f((c.x - ref) * LOG2E);
+    float top = -INFINITY, sum = 0.0f;
+    for (int p = lane; p < parts; p += 64) {
+        const float2 q = part[p * k.n_pad + i];
+        const float now = fmaxf(top, q.x), ref = now == -INFINITY ? 0.0f : now;
+        sum = sum * __builtin_amdgcn_exp2f(top - ref) + q.y * __builtin_amdgcn_exp2f(q.x - ref);
+        top = now;
     }
-    const float l = ref + logf(sum);
-    lse_pad[i] = l;
+    const int32_t y = k.label[i];
+    const bool open = y >= 0 && k.bias[y] != -INFINITY;
+    float dot = 0.0f;
+    if (open)
+        for (int32_t f = lane; f < k.d; f += 64)
+            dot += load_f32<T>(c.h, i * c.h_stride + f) * load_f32<T>(c.w, y * c.w_stride + f);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        const float t2 = __shfl_xor(top, o, 64), s2 = __shfl_xor(sum, o, 64);
+        const float now = fmaxf(top, t2), ref = now == -INFINITY ? 0.0f : now;
+        sum = sum * __builtin_amdgcn_exp2f(top - ref) + s2 * __builtin_amdgcn_exp2f(t2 - ref);
+        top = now;
+        dot += __shfl_xor(dot, o, 64);
+    }
+    const float l2 = (top == -INFINITY ? 0.0f : top) + log2f(sum);
+    if (lane != 0) return;
+    lse2[i] = l2;
     if (i >= k.n) return;
-    lse[i] = l;
-    loss[i] = k.label[i] < 0 ? 0.0f : k.weight[i] * (l - z_label[i]);
+    const float lse = y == -2 ? NAN : l2 * LN2, z = open ? dot + (c.bias ? c.bias[y] : 0.0f) : -INFINITY;
+    c.lse[i] = lse;
+    c.loss[i] = y < 0 ? 0.0f : k.weight[i] * (lse - z);
 }
 
 // ---- pass 2: G of a piece ------------------------------------------------------------
 // g[v - v0][i - r0], rows of rows_pad; f32: G / w in two f16 terms times 2^15.
 template <int P>
-__global__ __launch_bounds__(256) void k_xent_g(XentPack k, int64_t v0, int64_t r0, int64_t rows_pad,
+__global__ __launch_bounds__(256, 2) void k_xent_g(XentPack k, int64_t v0, int64_t r0, int64_t rows_pad,
                                                 int64_t plane, int32_t row_tiles,
-                                                const float *__restrict__ lse,
+                                                const float *__restrict__ lse2,
                                                 u16 *__restrict__ g) {
     extern __shared__ char lds[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t i0 = r0 + (int64_t)(blockIdx.x % row_tiles) * TILE;
     const int64_t c0 = v0 + (int64_t)(blockIdx.x / row_tiles) * TILE;
     const Operand a{k.w, k.v_pad * k.ld, k.ld}, b{k.h, k.n_pad * k.ld, k.ld};
-    const float ws = P == 2 ? ldexpf(1.0f, -scale_exp(k.ctl->w_max)) : 1.0f;
     f32x16 acc[2][2];
     clear(acc);
     tile_product<P, true, true>(a, b, c0, i0, (k.d + BK<P> - 1) / BK<P>, lds, acc);
+    const int64_t c = c0 + (wave >> 1) * 64 + (lane >> 5) * 4;
 #pragma unroll
     for (int y = 0; y < 2; ++y) {
         const int64_t i = i0 + (wave & 1) * 64 + y * 32 + (lane & 31);
-        const float hs = P == 2 ? k.row_scale[i] : 1.0f, l = lse[i], wt = k.weight[i];
+        const float sc = P == 2 ? k.row_scale[i] : LOG2E;
         const int32_t label = k.label[i];
+        // a row that is out: 2^-inf
+        const float l = label < 0 ? INFINITY : lse2[i], wt = k.weight[i];
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
+        for (int x = 0; x < 2; ++x) {
+            const int64_t here = c + x * 32;
+            const int64_t mine = label - here;           // 8 q + e if the label is here
+            const bool hot = __any(mine >= 0 && mine < 32);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int64_t v = c0 + (wave >> 1) * 64 + x * 32 + block_row(r);
-                float z = acc[x][y][r];
-                if (P == 2) z = z * hs * ws;
-                float p = __builtin_amdgcn_exp2f((z + k.bias[v] - l) * LOG2E);
-                if (v == label) p -= 1.0f;
-                if (label < 0) p = 0.0f;
-                u16 *at = g + (v - v0) * rows_pad + (i - r0);
-                if constexpr (P == 1) {
-                    *at = bits_of((__bf16)(wt * p));
-                } else {
-                    u16 hi, lo;
-                    split_f16(p * G_SCALE, hi, lo);
-                    at[0] = hi;
-                    at[plane] = lo;
+            for (int q = 0; q < 4; ++q) {
+                const float4 b4 = *reinterpret_cast<const float4 *>(k.bias + here + q * 8);
+                const float b2[4] = {b4.x, b4.y, b4.z, b4.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float p = __builtin_amdgcn_exp2f(
+                        __builtin_fmaf(acc[x][y][q * 4 + e], sc, b2[e] - l));
+                    if (hot && mine == q * 8 + e) p -= 1.0f;
+                    u16 *at = g + (here + q * 8 + e - v0) * rows_pad + (i - r0);
+                    if constexpr (P == 1) {
+                        *at = bits_of((__bf16)(wt * p));
+                    } else {
+                        u16 hi, lo;
+                        split_f16(p * G_SCALE, hi, lo);
+                        at[0] = hi;
+                        at[plane] = lo;
+                    }
                 }
             }
+        }
     }
 }
 
@@ -459,7 +491,7 @@ __device__ __forceinline__ void put(const Out &o, int32_t d, int32_t ld, int64_t
 
 // dh[i][j] += sum over the piece's v of g[v][i] W[v][j].
 template <int P>
-__global__ __launch_bounds__(256) void k_xent_dh(XentPack k, int64_t v0, int64_t classes_pad,
+__global__ __launch_bounds__(256, 2) void k_xent_dh(XentPack k, int64_t v0, int64_t classes_pad,
                                                  int64_t r0, int64_t rows_pad, int64_t plane,
                                                  int32_t row_tiles, const u16 *__restrict__ g,
                                                  Out o) {
@@ -487,7 +519,7 @@ __global__ __launch_bounds__(256) void k_xent_dh(XentPack k, int64_t v0, int64_t
 
 // dW[v][j] += sum over the rows of g[v][i] hg[i][j].
 template <int P>
-__global__ __launch_bounds__(256) void k_xent_dw(XentPack k, int64_t v0, int64_t r0, int64_t rows_pad,
+__global__ __launch_bounds__(256, 2) void k_xent_dw(XentPack k, int64_t v0, int64_t r0, int64_t rows_pad,
                                                  int64_t plane, int32_t class_tiles,
                                                  const u16 *__restrict__ g, Out o) {
     extern __shared__ char lds[];
@@ -559,7 +591,7 @@ struct Plan {
     int P;
     int64_t n_pad, v_pad, ld, piece_rows, piece_classes;
     int32_t splits;
-    size_t ctl, h, hg, w, bias, scale, label, weight, lse, z_label, part, g, dh_acc, dw_acc, end;
+    size_t ctl, h, hg, w, bias, scale, label, weight, lse, part, g, dh_acc, dw_acc, end;
 };
 
 Plan plan_of(const XentCall &c) {
@@ -589,10 +621,9 @@ Plan plan_of(const XentCall &c) {
     p.label = take((size_t)4 * p.n_pad);
     p.weight = take((size_t)4 * p.n_pad);
     p.lse = take((size_t)4 * p.n_pad);
-    p.z_label = take((size_t)4 * p.n_pad);
     p.part = take((size_t)16 * p.splits * p.n_pad);
     if (c.grad) {
-        p.hg = take((size_t)2 * p.P * p.n_pad * p.ld);
+        p.hg = c.bf16 ? p.h : take((size_t)2 * p.P * p.n_pad * p.ld);
         p.g = take((size_t)2 * p.P * p.piece_rows * p.piece_classes);
         if (p.piece_classes < p.v_pad) p.dh_acc = take((size_t)4 * p.n_pad * p.ld);
         if (p.piece_rows < p.n_pad) p.dw_acc = take((size_t)4 * p.v_pad * p.ld);
@@ -619,7 +650,6 @@ hipError_t run(hipStream_t s, const XentCall &c, const Plan &p, char *m) {
     k.label = reinterpret_cast<int32_t *>(m + p.label);
     k.weight = reinterpret_cast<float *>(m + p.weight);
     float *lse = reinterpret_cast<float *>(m + p.lse);
-    float *z_label = reinterpret_cast<float *>(m + p.z_label);
     float2 *part = reinterpret_cast<float2 *>(m + p.part);
     const dim3 b(256);
     constexpr int LDS = LDS_TILES<P>;
@@ -638,11 +668,13 @@ hipError_t run(hipStream_t s, const XentCall &c, const Plan &p, char *m) {
     hipLaunchKernelGGL((k_xent_rows<T>), dim3(blocks(k.n_pad, 4)), b, 0, s, k, c.h, c.h_stride,
                        c.labels, c.weights);
     hipLaunchKernelGGL((k_xent_stats<P>), dim3((uint32_t)(k.n_pad / TILE * p.splits)), b, LDS, s, k,
-                       k.v_pad / TILE, p.splits, part, z_label);
-    hipLaunchKernelGGL(k_xent_join, dim3(blocks(k.n_pad, 256)), b, 0, s, k, 2 * p.splits, part,
-                       z_label, lse, c.loss, c.lse);
+                       k.v_pad / TILE, p.splits, part);
+    hipLaunchKernelGGL((k_xent_join<T>), dim3(blocks(k.n_pad, 4)), b, 0, s, k, c, 2 * p.splits,
+                       part, lse);
     if (!c.grad) return hipGetLastError();
-    hipLaunchKernelGGL((k_xent_pack_hg<T>), dim3(blocks(k.n_pad, 4)), b, 0, s, k, c.h, c.h_stride);
+    if constexpr (P == 2)
+        hipLaunchKernelGGL(k_xent_pack_hg, dim3(blocks(k.n_pad, 4)), b, 0, s, k,
+                           static_cast<const float *>(c.h), c.h_stride);
     u16 *g = reinterpret_cast<u16 *>(m + p.g);
     const int64_t plane = p.piece_rows * p.piece_classes;
     const uint32_t cols = (uint32_t)(p.ld / TILE);

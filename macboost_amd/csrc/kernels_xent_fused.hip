@@ -31,7 +31,6 @@ typedef __attribute__((ext_vector_type(4))) unsigned short u16x4;
 
 constexpr int XB = 128;                  // X rows of a workgroup, 32 a wavefront
 constexpr int TY = 64;                   // Y rows of a tile
-constexpr float LN2 = 0.69314718055994531f;
 // p = 2^(z - maximum) is kept times 2^13, and the maximum may lag by 2^2, so that p as
 // f16 terms is at most 2^15 and keeps steps of 2^-38.
 constexpr float P_EXP = 13.0f, LAG = 2.0f;
@@ -53,10 +52,6 @@ struct Fused {
     float *c2;                           // lse log2 e, +inf: out
     float *wq;                           // weight as the classes pass multiplies with it
 };
-
-// Values beyond this in a row that is out count as not finite: times a finite W
-// they could still overflow.
-constexpr uint32_t HUGE_BITS = 0x5D800000u;          // 2^60
 
 // The exponent of the classes pass's weights, for the largest |w h|.
 __device__ __forceinline__ int wq_exp(uint32_t hg_max) {
@@ -148,7 +143,7 @@ __global__ __launch_bounds__(256) void k_fused_pack(Fused k, const void *w, int6
             if (y < 0 || y >= k.v || wt == 0.0f || !any) {
                 wt = 0.0f;
                 y = -1;
-                if (most >= HUGE_BITS) {
+                if (most >= XENT_HUGE) {
                     y = -2;
                     m = 0;
                     x[0] = x[1] = x[2] = x[3] = 0.0f;
@@ -642,34 +637,56 @@ __global__ __launch_bounds__(256, 2) void k_fused_classes_pass(Fused k, int32_t 
                 make_float4(o[j][q * 4], o[j][q * 4 + 1], o[j][q * 4 + 2], o[j][q * 4 + 3]);
 }
 
-template <typename T>
+// LD / 4 lanes a class, and where there are many splits SPLIT_GROUPS of them, whose sums
+// are added in order.
+constexpr int SPLIT_GROUPS = 8;
+template <typename T, int LD, bool GROUPS>
 __global__ __launch_bounds__(256) void k_fused_join_classes(Fused k, XentCall c, int32_t splits,
-                                                            int32_t ld,
                                                             const float *__restrict__ part,
                                                             const float *__restrict__ part_db) {
-    const int lane = threadIdx.x & 63;
-    const int64_t v = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    constexpr int LANES = LD / 4, G = GROUPS ? SPLIT_GROUPS : 1, CLASSES = 256 / LANES / G;
+    __shared__ float4 sums[GROUPS ? 256 : 1];
+    __shared__ float dbs[GROUPS ? 256 : 1];
+    const int l = threadIdx.x % LANES, f = l * 4;
+    const int g = threadIdx.x / LANES % G;
+    const int64_t v = (int64_t)blockIdx.x * CLASSES + threadIdx.x / (LANES * G);
+    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float db = 0.0f;
+    if (v < k.v) {
+#pragma unroll 4
+        for (int s = g; s < splits; s += G) {
+            const float4 p = *reinterpret_cast<const float4 *>(part + (s * k.v_pad + v) * LD + f);
+            sum.x += p.x;
+            sum.y += p.y;
+            sum.z += p.z;
+            sum.w += p.w;
+            if (c.dbias && l == 0) db += part_db[s * k.v_pad + v];
+        }
+    }
+    if constexpr (GROUPS) {
+        sums[threadIdx.x] = sum;
+        dbs[threadIdx.x] = db;
+        __syncthreads();
+        if (g != 0) return;
+        for (int o = 1; o < G; ++o) {
+            const float4 p = sums[threadIdx.x + o * LANES];
+            sum.x += p.x;
+            sum.y += p.y;
+            sum.z += p.z;
+            sum.w += p.w;
+            db += dbs[threadIdx.x + o * LANES];
+        }
+    }
     if (v >= k.v) return;
     const bool open = k.bias2[v] != -INFINITY;
-    float scale = 1.0f;
-    if (sizeof(T) == 4) {
-        scale = ldexpf(1.0f, -wq_exp(k.ctl->hg_max));
-    }
+    const float scale = sizeof(T) == 4 ? ldexpf(1.0f, -wq_exp(k.ctl->hg_max)) : 1.0f;
+    const float x[4] = {sum.x, sum.y, sum.z, sum.w};
     if (c.dw)
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-            const int f = lane + 64 * q;
-            if (f >= k.d) break;
-            float sum = 0.0f;
-#pragma unroll 8
-            for (int s = 0; s < splits; ++s) sum += part[(s * k.v_pad + v) * ld + f];
-            static_cast<T *>(c.dw)[v * c.w_stride + f] = (T)(open ? sum * scale : 0.0f);
-        }
-    if (c.dbias && lane == 0) {
-        float sum = 0.0f;
-        for (int s = 0; s < splits; ++s) sum += part_db[s * k.v_pad + v];
-        c.dbias[v] = open ? sum : 0.0f;
-    }
+        for (int e = 0; e < 4; ++e)
+            if (f + e < k.d)
+                static_cast<T *>(c.dw)[v * c.w_stride + f + e] = (T)(open ? x[e] * scale : 0.0f);
+    if (c.dbias && l == 0) c.dbias[v] = open ? db : 0.0f;
 }
 
 // ---- the call ---------------------------------------------------------------------------
@@ -787,8 +804,13 @@ hipError_t run(hipStream_t s, const XentCall &c, const Plan &p, char *m) {
         hipLaunchKernelGGL((k_fused_classes_pass<P, KS>),
                            dim3((uint32_t)(k.v_pad / XB * p.class_splits)), b, lds_classes, s, k,
                            p.class_splits, part, c.dbias ? part_db : nullptr);
-        hipLaunchKernelGGL((k_fused_join_classes<T>), dim3(blocks(k.v, 4)), b, 0, s, k, c,
-                           p.class_splits, LD, part, part_db);
+        if (p.class_splits >= 2 * SPLIT_GROUPS)
+            hipLaunchKernelGGL((k_fused_join_classes<T, LD, true>),
+                               dim3(blocks(k.v, 1024 / LD / SPLIT_GROUPS)), b, 0, s, k, c,
+                               p.class_splits, part, part_db);
+        else
+            hipLaunchKernelGGL((k_fused_join_classes<T, LD, false>), dim3(blocks(k.v, 1024 / LD)),
+                               b, 0, s, k, c, p.class_splits, part, part_db);
     }
     return hipGetLastError();
 }

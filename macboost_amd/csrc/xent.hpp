@@ -16,6 +16,10 @@ typedef __attribute__((ext_vector_type(16))) float f32x16;
 typedef unsigned short u16;
 
 constexpr float LOG2E = 1.44269504088896341f;
+constexpr float LN2 = 0.69314718055994531f;
+// Values beyond this (2^60) in a row that is out count as not finite: times a finite W they
+// could still overflow.
+constexpr uint32_t XENT_HUGE = 0x5D800000u;
 
 // ---- control words -----------------------------------------------------------
 struct XentCtl {
@@ -61,9 +65,9 @@ struct XentPack {
     int32_t d, ld;
     XentCtl *ctl;
     u16 *h, *hg, *w;                     // planes of n_pad * ld, v_pad * ld
-    float *bias;                         // [v_pad], -inf: not offered
-    float *row_scale;                    // [n_pad], f32: 2^-s of h's row
-    int32_t *label;                      // [n_pad], -1: out
+    float *bias;                         // [v_pad] bias log2 e, -inf: not offered
+    float *row_scale;                    // [n_pad], f32: log2 e times the scale of a score
+    int32_t *label;                      // [n_pad], -1: out, -2: out and not finite
     float *weight;                       // [n_pad], 0: out
 };
 
