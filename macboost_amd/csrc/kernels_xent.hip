@@ -35,7 +35,6 @@ namespace mbk {
 
 namespace {
 
-constexpr int TILE = 128;                // rows and columns of a workgroup's product
 constexpr int LD_PAD = 128;              // operands' rows are padded to it
 constexpr float G_SCALE = 32768.0f;      // f32: |G / w| <= 1 as f16 terms
 
@@ -161,148 +160,197 @@ __global__ __launch_bounds__(256) void k_xent_pack_hg(XentPack k, const float *h
 }
 
 // ---- products --------------------------------------------------------------------
-// C[m][n] = sum_k A[m][k] B[n][k], a tile of 128 x 128 by 4 wavefronts of 64 x 64.
-// An operand lies with k contiguous (KC: element (m, k) at m * ld + k) or with m
-// contiguous (k * ld + m); the second kind is turned by the LDS reads
-// (ds_read_tr16_b64: 16 lanes read 4 rows of 16 elements, lane i gets column i).
+// C[m][n] = sum_k A[m][k] B[n][k].  An operand lies with k contiguous (KC: element (m, k)
+// at m * ld + k) or with m contiguous (k * ld + m); the second kind is turned by the LDS
+// reads (ds_read_tr16_b64: 16 lanes read 4 rows of 16 elements, lane i gets column i).
 // P == 1: bf16; P == 2: f16 in two planes, three products.
+//
+// A workgroup has a tile of 256 x 256 in eight wavefronts (Wide: 128 x 64 each) or of
+// 128 x 128 in four (Narrow: 64 x 64 each).  Steps of k are copied into LDS directly, one
+// step ahead, 64 of bf16 or 32 of the planes.
+template <int WM_, int WN_, int MT_, int NT_> struct Tiling {
+    static constexpr int WM = WM_, WN = WN_, MT = MT_, NT = NT_;     // wavefronts, blocks of 32
+    static constexpr int WAVES = WM * WN, T = WM * MT * 32;
+    static_assert(T == WN * NT * 32, "square tiles");
+};
+using Wide = Tiling<2, 4, 4, 2>;
+using Narrow = Tiling<2, 2, 2, 2>;
+
 template <int P> constexpr int BK = 64 / P;          // k of a step
-template <int P> constexpr int OP_BYTES = P * TILE * BK<P> * 2;
-template <int P> constexpr int LDS_TILES = 4 * OP_BYTES<P>;      // A and B, twice
+template <int P, class C> constexpr int OP_BYTES = P * C::T * BK<P> * 2;
+template <int P, class C> constexpr int LDS_TILES = 4 * OP_BYTES<P, C>;      // A and B, twice
 
 struct Operand {
     const u16 *p;
     int64_t plane, ld;
 };
 
-// Bytes of 16-byte chunk c of row r in LDS.  A read of the matrix instruction's
-// operand takes one chunk of 8 rows at a time (KC) or 32 bytes of 4 rows: the chunks
-// are permuted so that these fall on different banks.
-template <int P, bool KC> __device__ __forceinline__ int lds_at(int r, int c) {
-    if constexpr (KC) {
-        constexpr int CH = BK<P> / 8;
-        const int x = CH == 8 ? r & 7 : (r >> 1) & 3;
-        return (r * CH + (c ^ x)) * 16;
-    } else {
-        return (r * 16 + ((((c >> 1) ^ (r & 7)) << 1) | (c & 1))) * 16;
-    }
+// The chunks of 16 bytes of an LDS row are permuted by the row.  Rows of k (KC, 64 or 128
+// bytes): the 16 rows x 1 chunk of a read fall on all banks.  Rows of m: the 4 rows x 4
+// chunks of a read across do.
+template <int P, bool KC> __device__ __forceinline__ int chunk_xor(int row) {
+    if constexpr (!KC) return (row & 3) * 4;
+    else if constexpr (P == 1) return ((row >> 1) & 1) * 4 + ((row >> 2) & 3);
+    else return (row >> 2) & 3;
 }
 
-template <int P, bool KC> struct Stage {
-    static constexpr int NQ = BK<P> / 16;            // chunks a thread and plane
-    u32x4 r[P][NQ];
-    __device__ __forceinline__ void load(const Operand &o, int64_t m0, int64_t k0) {
-#pragma unroll
-        for (int p = 0; p < P; ++p)
-#pragma unroll
-            for (int q = 0; q < NQ; ++q) {
-                const int idx = threadIdx.x + 256 * q;
-                int64_t at;
-                if constexpr (KC) {
-                    constexpr int CH = BK<P> / 8;
-                    at = (m0 + idx / CH) * o.ld + k0 + idx % CH * 8;
-                } else {
-                    at = (k0 + idx / 16) * o.ld + m0 + idx % 16 * 8;
-                }
-                r[p][q] = *reinterpret_cast<const u32x4 *>(o.p + p * o.plane + at);
-            }
-    }
-    __device__ __forceinline__ void store(char *lds) const {
-        constexpr int CH = KC ? BK<P> / 8 : 16;
-#pragma unroll
-        for (int p = 0; p < P; ++p)
-#pragma unroll
-            for (int q = 0; q < NQ; ++q) {
-                const int idx = threadIdx.x + 256 * q;
-                *reinterpret_cast<u32x4 *>(lds + p * (TILE * BK<P> * 2) +
-                                           lds_at<P, KC>(idx / CH, idx % CH)) = r[p][q];
-            }
-    }
-};
-
-// The operand of the matrix instruction: lane l has element m0 + l % 32, k =
-// k0 + l / 32 * 8 .. + 7.
-template <int P, bool KC>
-__device__ __forceinline__ void fragment(const char *lds, int m0, int k0, u32x4 (&f)[P]) {
+// Starts the copies of a step of an operand from m0, k0 on.
+template <int P, bool KC, class C>
+__device__ __forceinline__ void copy_step(const Operand &o, int64_t m0, int64_t k0, char *lds,
+                                          int wave) {
+    constexpr int ROW = (KC ? BK<P> : C::T) * 2, PLANE = C::T * BK<P> * 2;
+    constexpr int ROWS = 1024 / ROW;                 // of a wavefront's copy
     const int lane = threadIdx.x & 63;
+    const int row = wave * ROWS + lane * 16 / ROW;
+    const int chunk = (lane * 16 % ROW / 16) ^ chunk_xor<P, KC>(row);
+    const uint32_t mine = (uint32_t)row * (uint32_t)o.ld * 2 + chunk * 16;
 #pragma unroll
     for (int p = 0; p < P; ++p) {
-        const char *plane = lds + p * (TILE * BK<P> * 2);
-        if constexpr (KC) {
-            f[p] = *reinterpret_cast<const u32x4 *>(
-                plane + lds_at<P, true>(m0 + (lane & 31), k0 / 8 + (lane >> 5)));
+        const char *from = reinterpret_cast<const char *>(o.p + p * o.plane +
+                                                          (KC ? m0 * o.ld + k0 : k0 * o.ld + m0));
+#pragma unroll
+        for (int q = 0; q < PLANE / 1024 / C::WAVES; ++q)
+            __builtin_amdgcn_global_load_lds(
+                (global_void *)(from + (int64_t)q * C::WAVES * ROWS * o.ld * 2 + mine),
+                (lds_void *)(lds + p * PLANE + (q * C::WAVES + wave) * 1024), 16, 0, 0);
+    }
+}
+
+// Operands of the matrix instruction, lane l with element m0 + l % 32 of a block and k =
+// 16 SLAB + l / 32 * 8 .. + 7, for N blocks of 32 from m0 on.
+template <int P, class C, int SLAB, int N>
+__device__ __forceinline__ void along(const char *lds, int m0, u32x4 (&f)[N][P]) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int t = 0; t < N; ++t) {
+        const int row = m0 + t * 32 + (lane & 31);
+        const int chunk = (SLAB * 2 + (lane >> 5)) ^ chunk_xor<P, true>(row);
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+            f[t][p] = *reinterpret_cast<const u32x4 *>(lds + p * (C::T * BK<P> * 2) +
+                                                       row * (BK<P> * 2) + chunk * 16);
+    }
+}
+// Across: m0 is a multiple of 32 N, so that the blocks differ in chunk bits alone.  The
+// reads wait for themselves: see kernels_xent_fused.hip.
+template <class C> __device__ __forceinline__ uint32_t across_at(int m0) {
+    const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
+    const int row = (g >> 1) * 8 + (i >> 2), m = m0 + (g & 1) * 16 + (i & 3) * 4;
+    return row * (C::T * 2) + ((m >> 3) ^ ((row & 3) * 4)) * 16 + (m & 7) * 2;
+}
+#define TR(dst, addr, off) "ds_read_b64_tr_b16 " dst ", " addr " offset:" off "\n\t"
+template <int P, class C, int SLAB, int N>
+__device__ __forceinline__ void across(uint32_t at, u32x4 (&f)[N][P]) {
+    constexpr int ROW = C::T * 2, O = SLAB * 16 * ROW, O4 = O + 4 * ROW, PLANE = C::T * BK<P> * 2;
+    u32x2 x[N][P][2];
+    const uint32_t a1 = at ^ 64, a2 = at ^ 128, a3 = at ^ 192;
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+        if constexpr (N == 2) {
+            asm volatile(TR("%0", "%4", "%6") TR("%1", "%4", "%7") TR("%2", "%5", "%6")
+                         TR("%3", "%5", "%7") "s_waitcnt lgkmcnt(0)"
+                         : "=&v"(x[0][p][0]), "=&v"(x[0][p][1]), "=&v"(x[1][p][0]),
+                           "=&v"(x[1][p][1])
+                         : "v"(at + p * PLANE), "v"(a1 + p * PLANE), "n"(O), "n"(O4)
+                         : "memory");
         } else {
-            typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
-            const int g = lane >> 4, i = lane & 15;
-            const int m = m0 + (g & 1) * 16 + (i & 3) * 4, k = k0 + (g >> 1) * 8 + (i >> 2);
-            union {
-                i16x4 h[2];
-                u32x4 v;
-            } u;
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-                u.h[t] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    (lds_i16x4 *)(plane + lds_at<P, false>(k + 4 * t, m / 8) + (m & 7) * 2));
-            f[p] = u.v;
+            asm volatile(TR("%0", "%8", "%12") TR("%1", "%8", "%13") TR("%2", "%9", "%12")
+                         TR("%3", "%9", "%13") TR("%4", "%10", "%12") TR("%5", "%10", "%13")
+                         TR("%6", "%11", "%12") TR("%7", "%11", "%13") "s_waitcnt lgkmcnt(0)"
+                         : "=&v"(x[0][p][0]), "=&v"(x[0][p][1]), "=&v"(x[1][p][0]),
+                           "=&v"(x[1][p][1]), "=&v"(x[2][p][0]), "=&v"(x[2][p][1]),
+                           "=&v"(x[3][p][0]), "=&v"(x[3][p][1])
+                         : "v"(at + p * PLANE), "v"(a1 + p * PLANE), "v"(a2 + p * PLANE),
+                           "v"(a3 + p * PLANE), "n"(O), "n"(O4)
+                         : "memory");
         }
     }
+#pragma unroll
+    for (int t = 0; t < N; ++t)
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+            f[t][p] = u32x4{x[t][p][0][0], x[t][p][0][1], x[t][p][1][0], x[t][p][1][1]};
 }
+#undef TR
 
-// Adds the product of steps [0, steps) into acc[mt][nt]: wavefront w has rows
-// (w >> 1) * 64 + mt * 32 and columns (w & 1) * 64 + nt * 32 of the tile.
-template <int P, bool AK, bool BKC>
-__device__ __forceinline__ void tile_product(const Operand &a, const Operand &b, int64_t m0,
-                                             int64_t n0, int64_t steps, char *lds,
-                                             f32x16 (&acc)[2][2]) {
-    const int wave = threadIdx.x >> 6;
-    Stage<P, AK> sa;
-    Stage<P, BKC> sb;
-    sa.load(a, m0, 0);
-    sb.load(b, n0, 0);
-    __syncthreads();                     // the last tile's reads
-    sa.store(lds);
-    sb.store(lds + OP_BYTES<P>);
-    __syncthreads();
-    for (int64_t t = 0; t < steps; ++t) {
-        const char *cur = lds + (t & 1) * 2 * OP_BYTES<P>;
-        char *nxt = lds + ((t + 1) & 1) * 2 * OP_BYTES<P>;
-        if (t + 1 < steps) {
-            sa.load(a, m0, (t + 1) * BK<P>);
-            sb.load(b, n0, (t + 1) * BK<P>);
-        }
+template <class C> using Acc = f32x16[C::MT][C::NT];
+template <class C> __device__ __forceinline__ void clear(Acc<C> &acc) {
 #pragma unroll
-        for (int k = 0; k < BK<P>; k += 16) {
-            u32x4 fa[2][P], fb[2][P];
+    for (int x = 0; x < C::MT; ++x)
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                fragment<P, AK>(cur, (wave >> 1) * 64 + x * 32, k, fa[x]);
-                fragment<P, BKC>(cur + OP_BYTES<P>, (wave & 1) * 64 + x * 32, k, fb[x]);
-            }
-#pragma unroll
-            for (int x = 0; x < 2; ++x)
-#pragma unroll
-                for (int y = 0; y < 2; ++y) acc[x][y] = mma<P>(fa[x], fb[y], acc[x][y]);
-        }
-        if (t + 1 < steps) {
-            sa.store(nxt);
-            sb.store(nxt + OP_BYTES<P>);
-        }
-        __syncthreads();
-    }
-}
-
-__device__ __forceinline__ void clear(f32x16 (&acc)[2][2]) {
-#pragma unroll
-    for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int y = 0; y < 2; ++y)
+        for (int y = 0; y < C::NT; ++y)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[x][y][r] = 0.0f;
 }
 
-// Row of register r in a 32 x 32 block; its column is lane % 32.
-__device__ __forceinline__ int block_row(int r) {
-    return (r >> 2) * 8 + ((threadIdx.x & 63) >> 5) * 4 + (r & 3);
+// The product over the steps [first, last) of k of a sequence of tiles: next(i, m0, n0)
+// gives tile i, done(i) takes its sums from acc.  The copies run ahead over the ends of
+// tiles.
+template <int P, bool AK, bool BKC, class C, class Next, class Done>
+__device__ __forceinline__ void products(const Operand &a, const Operand &b, int64_t tiles,
+                                         int64_t first, int64_t last, char *lds, Acc<C> &acc,
+                                         Next next, Done done) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave / C::WN * C::MT * 32, wn = wave % C::WN * C::NT * 32;
+    const uint32_t base = lds_address(lds);
+    const uint32_t a_at = AK ? 0 : across_at<C>(wm);
+    const uint32_t b_at = BKC ? 0 : across_at<C>(wn);
+    if (first >= last) {                 // a split without a step: no copy is left behind
+        clear<C>(acc);
+        return;
+    }
+    int64_t m0, n0;
+    next(0, m0, n0);
+    copy_step<P, AK, C>(a, m0, first * BK<P>, lds, wave);
+    copy_step<P, BKC, C>(b, n0, first * BK<P>, lds + OP_BYTES<P, C>, wave);
+    int buf = 0;
+    for (int64_t i = 0; i < tiles; ++i) {
+        clear<C>(acc);
+        for (int64_t t = first; t < last; ++t) {
+            copies_done();
+            __syncthreads();             // the step is there; the other buffer is read
+            const int cur = buf * 2 * OP_BYTES<P, C>, nxt = 2 * OP_BYTES<P, C> - cur;
+            buf ^= 1;
+            const bool end = t + 1 == last;
+            if (end && i + 1 < tiles) next(i + 1, m0, n0);
+            if (!end || i + 1 < tiles) {
+                const int64_t k0 = (end ? first : t + 1) * BK<P>;
+                copy_step<P, AK, C>(a, m0, k0, lds + nxt, wave);
+                copy_step<P, BKC, C>(b, n0, k0, lds + nxt + OP_BYTES<P, C>, wave);
+            }
+            const auto slab = [&](auto which) {
+                constexpr int S = decltype(which)::value;
+                u32x4 fa[C::MT][P], fb[C::NT][P];
+                if constexpr (AK) along<P, C, S>(lds + cur, wm, fa);
+                else across<P, C, S>(base + cur + a_at, fa);
+                if constexpr (BKC) along<P, C, S>(lds + cur + OP_BYTES<P, C>, wn, fb);
+                else across<P, C, S>(base + cur + OP_BYTES<P, C> + b_at, fb);
+#pragma unroll
+                for (int x = 0; x < C::MT; ++x)
+#pragma unroll
+                    for (int y = 0; y < C::NT; ++y) acc[x][y] = mma<P>(fa[x], fb[y], acc[x][y]);
+            };
+            slab(At<0>{});
+            slab(At<1>{});
+            if constexpr (BK<P> == 64) {
+                slab(At<2>{});
+                slab(At<3>{});
+            }
+        }
+        done(i);
+    }
+}
+
+// Workgroups go to the 8 XCDs in turn; each XCD gets a run of tiles, in groups of 8
+// rows of tiles, so that what its L2 holds is used by many.
+__device__ __forceinline__ void tile_of(uint32_t id, uint32_t total, uint32_t tiles_m,
+                                        uint32_t tiles_n, uint32_t &tm, uint32_t &tn) {
+    const uint32_t xcd = id & 7, per = total >> 3, more = total & 7;
+    const uint32_t at = xcd * per + min(xcd, more) + (id >> 3);
+    const uint32_t group = at / (8 * tiles_n), in = at % (8 * tiles_n);
+    const uint32_t rows = min(8u, tiles_m - group * 8);
+    tm = group * 8 + in % rows;
+    tn = in / rows;
 }
 
 // ---- pass 1: each row's maximum and sum ---------------------------------------------
@@ -310,67 +358,75 @@ __device__ __forceinline__ int block_row(int r) {
 // row: the maximum and sum stay in registers over the classes of a split, and only
 // two lanes and two wavefronts have parts of a row.  part[2 * split + half][row]: the
 // maximum of z log2 e, and the sum of its powers of 2.
-template <int P>
-__global__ __launch_bounds__(256, 2) void k_xent_stats(XentPack k, int64_t class_tiles,
-                                                       int32_t splits,
-                                                       float2 *__restrict__ part) {
+template <int P, class C>
+__global__ __launch_bounds__(C::WAVES * 64, 2) void k_xent_stats(XentPack k, int32_t row_tiles,
+                                                                 int32_t class_tiles,
+                                                                 int32_t splits,
+                                                                 float2 *__restrict__ part) {
     extern __shared__ char lds[];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t i0 = (int64_t)(blockIdx.x / splits) * TILE;
-    const int32_t split = blockIdx.x % splits;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    uint32_t row_tile, split;
+    tile_of(blockIdx.x, gridDim.x, row_tiles, splits, row_tile, split);
+    const int64_t i0 = (int64_t)row_tile * C::T;
     const Operand a{k.w, k.v_pad * k.ld, k.ld}, b{k.h, k.n_pad * k.ld, k.ld};
-    const int64_t steps = (k.d + BK<P> - 1) / BK<P>;
-    float m[2], s[2], sc[2];
-    int64_t row[2];
+    float m[C::NT], s[C::NT], sc[C::NT];
+    int64_t row[C::NT];
 #pragma unroll
-    for (int y = 0; y < 2; ++y) {
-        row[y] = i0 + (wave & 1) * 64 + y * 32 + (lane & 31);
+    for (int y = 0; y < C::NT; ++y) {
+        row[y] = i0 + wave % C::WN * C::NT * 32 + y * 32 + (lane & 31);
         m[y] = -INFINITY;
         s[y] = 0.0f;
         sc[y] = P == 2 ? k.row_scale[row[y]] : LOG2E;
     }
-    for (int64_t t = split; t < class_tiles; t += splits) {
-        f32x16 acc[2][2];
-        clear(acc);
-        tile_product<P, true, true>(a, b, t * TILE, i0, steps, lds, acc);
-        const float *bias = k.bias + t * TILE + (wave >> 1) * 64 + (lane >> 5) * 4;
-        float4 b2[2][4];
+    Acc<C> acc;
+    const auto next = [&](int64_t i, int64_t &m0, int64_t &n0) {
+        m0 = (split + i * splits) * C::T;
+        n0 = i0;
+    };
+    const auto done = [&](int64_t i) {
+        const float *bias = k.bias + (split + i * splits) * C::T + wave / C::WN * C::MT * 32 +
+                            (lane >> 5) * 4;
+        float top[C::NT];
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
+        for (int y = 0; y < C::NT; ++y) top[y] = m[y];
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-                b2[x][q] = *reinterpret_cast<const float4 *>(bias + x * 32 + q * 8);
+        for (int x = 0; x < C::MT; ++x)
 #pragma unroll
-        for (int y = 0; y < 2; ++y) {
-            float top = m[y];
+            for (int q = 0; q < 4; ++q) {
+                const f32x4 b2 = *reinterpret_cast<const f32x4 *>(bias + x * 32 + q * 8);
 #pragma unroll
-            for (int x = 0; x < 2; ++x)
+                for (int e = 0; e < 4; ++e)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const float4 q = b2[x][r >> 2];
-                    const float b = (r & 3) == 0 ? q.x : (r & 3) == 1 ? q.y : (r & 3) == 2 ? q.z : q.w;
-                    acc[x][y][r] = __builtin_fmaf(acc[x][y][r], sc[y], b);
-                    top = fmaxf(top, acc[x][y][r]);
-                }
-            const float ref = top == -INFINITY ? 0.0f : top;
+                    for (int y = 0; y < C::NT; ++y) {
+                        const float z = __builtin_fmaf(acc[x][y][q * 4 + e], sc[y], b2[e]);
+                        acc[x][y][q * 4 + e] = z;
+                        top[y] = fmaxf(top[y], z);
+                    }
+            }
+#pragma unroll
+        for (int y = 0; y < C::NT; ++y) {
+            const float ref = top[y] == -INFINITY ? 0.0f : top[y];
             float sum[2] = {s[y] * __builtin_amdgcn_exp2f(m[y] - ref), 0.0f};
 #pragma unroll
-            for (int x = 0; x < 2; ++x)
+            for (int x = 0; x < C::MT; ++x)
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
                     sum[r & 1] += __builtin_amdgcn_exp2f(acc[x][y][r] - ref);
-            m[y] = top;
+            m[y] = top[y];
             s[y] = sum[0] + sum[1];
         }
-    }
+    };
+    const int64_t tiles = (class_tiles - (int64_t)split + splits - 1) / splits;
+    products<P, true, true, C>(a, b, tiles, 0, (k.d + BK<P> - 1) / BK<P>, lds, acc, next, done);
 #pragma unroll
-    for (int y = 0; y < 2; ++y) {
+    for (int y = 0; y < C::NT; ++y) {
         const float m2 = __shfl_xor(m[y], 32, 64), s2 = __shfl_xor(s[y], 32, 64);
         const float top = fmaxf(m[y], m2), ref = top == -INFINITY ? 0.0f : top;
         const float sum = s[y] * __builtin_amdgcn_exp2f(m[y] - ref) +
                           s2 * __builtin_amdgcn_exp2f(m2 - ref);
         if (lane < 32)
-            part[(2 * split + (wave >> 1)) * k.n_pad + row[y]] = make_float2(top, sum);
+            part[(2 * split + wave / C::WN) * k.n_pad + row[y]] = make_float2(top, sum);
     }
 }
 
@@ -415,130 +471,147 @@ __global__ __launch_bounds__(256) void k_xent_join(XentPack k, XentCall c, int32
 
 // ---- pass 2: G of a piece ------------------------------------------------------------
 // g[v - v0][i - r0], rows of rows_pad; f32: G / w in two f16 terms times 2^15.
-template <int P>
-__global__ __launch_bounds__(256, 2) void k_xent_g(XentPack k, int64_t v0, int64_t r0, int64_t rows_pad,
-                                                int64_t plane, int32_t row_tiles,
-                                                const float *__restrict__ lse2,
-                                                u16 *__restrict__ g) {
+template <int P, class C>
+__global__ __launch_bounds__(C::WAVES * 64, 2) void k_xent_g(XentPack k, int64_t v0, int64_t r0,
+                                                             int64_t rows_pad, int64_t plane,
+                                                             int32_t class_tiles,
+                                                             int32_t row_tiles,
+                                                             const float *__restrict__ lse2,
+                                                             u16 *__restrict__ g) {
     extern __shared__ char lds[];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t i0 = r0 + (int64_t)(blockIdx.x % row_tiles) * TILE;
-    const int64_t c0 = v0 + (int64_t)(blockIdx.x / row_tiles) * TILE;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    uint32_t tm, tn;
+    tile_of(blockIdx.x, gridDim.x, class_tiles, row_tiles, tm, tn);
+    const int64_t i0 = r0 + (int64_t)tn * C::T, c0 = v0 + (int64_t)tm * C::T;
     const Operand a{k.w, k.v_pad * k.ld, k.ld}, b{k.h, k.n_pad * k.ld, k.ld};
-    f32x16 acc[2][2];
-    clear(acc);
-    tile_product<P, true, true>(a, b, c0, i0, (k.d + BK<P> - 1) / BK<P>, lds, acc);
-    const int64_t c = c0 + (wave >> 1) * 64 + (lane >> 5) * 4;
+    Acc<C> acc;
+    const auto next = [&](int64_t, int64_t &m0, int64_t &n0) {
+        m0 = c0;
+        n0 = i0;
+    };
+    products<P, true, true, C>(a, b, 1, 0, (k.d + BK<P> - 1) / BK<P>, lds, acc, next,
+                               [](int64_t) {});
+    const int64_t c = c0 + wave / C::WN * C::MT * 32 + (lane >> 5) * 4;
 #pragma unroll
-    for (int y = 0; y < 2; ++y) {
-        const int64_t i = i0 + (wave & 1) * 64 + y * 32 + (lane & 31);
+    for (int y = 0; y < C::NT; ++y) {
+        const int64_t i = i0 + wave % C::WN * C::NT * 32 + y * 32 + (lane & 31);
         const float sc = P == 2 ? k.row_scale[i] : LOG2E;
         const int32_t label = k.label[i];
         // a row that is out: 2^-inf
         const float l = label < 0 ? INFINITY : lse2[i], wt = k.weight[i];
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
+        for (int x = 0; x < C::MT; ++x) {
             const int64_t here = c + x * 32;
             const int64_t mine = label - here;           // 8 q + e if the label is here
             const bool hot = __any(mine >= 0 && mine < 32);
+            u16 *to = g + (here - v0) * rows_pad + (i - r0);
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                const float4 b4 = *reinterpret_cast<const float4 *>(k.bias + here + q * 8);
-                const float b2[4] = {b4.x, b4.y, b4.z, b4.w};
+                const f32x4 b2 = *reinterpret_cast<const f32x4 *>(k.bias + here + q * 8);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     float p = __builtin_amdgcn_exp2f(
                         __builtin_fmaf(acc[x][y][q * 4 + e], sc, b2[e] - l));
                     if (hot && mine == q * 8 + e) p -= 1.0f;
-                    u16 *at = g + (here + q * 8 + e - v0) * rows_pad + (i - r0);
                     if constexpr (P == 1) {
-                        *at = bits_of((__bf16)(wt * p));
+                        *to = bits_of((__bf16)(wt * p));
                     } else {
                         u16 hi, lo;
                         split_f16(p * G_SCALE, hi, lo);
-                        at[0] = hi;
-                        at[plane] = lo;
+                        to[0] = hi;
+                        to[plane] = lo;
                     }
+                    to += e < 3 ? rows_pad : 5 * rows_pad;
                 }
             }
         }
     }
 }
 
-// Where a product's tile goes: the f32 sums of the pieces so far, and, with the last
-// piece, the output.
+// Where a product over the pieces goes: the f32 sums so far, [split][m_pad][ld], and, with
+// the last piece and no splits, the output.
 struct Out {
-    float *acc;                  // [m][ld]
+    float *acc;
+    int64_t m_pad;
     bool first, last;
-    const float *bias;           // dW: rows of bias -inf are 0
+    int32_t splits;
     void *out;
-    int64_t rows, stride;        // of the output; its columns are d
+    int64_t rows, stride;        // of the output; its columns are k.d
+    bool classes;                // dW: rows whose bias is -inf are 0; dh: f32, times weight
 };
-
+template <int P> __device__ __forceinline__ float out_scale(const XentPack &k, bool classes) {
+    if (P == 1) return 1.0f;
+    return ldexpf(1.0f, -scale_exp(classes ? k.ctl->hg_max : k.ctl->w_max)) / G_SCALE;
+}
 template <int P>
-__device__ __forceinline__ void put(const Out &o, int32_t d, int32_t ld, int64_t m, int64_t n,
-                                    float v, float scale) {
-    float *acc = o.acc + m * ld + n;
-    if (!o.first) v += *acc;
-    if (!o.last) {
-        *acc = v;
-    } else if (m < o.rows && n < d) {
-        if (o.bias && o.bias[m] == -INFINITY) v = 0.0f;
-        if constexpr (P == 1) static_cast<__bf16 *>(o.out)[m * o.stride + n] = (__bf16)v;
-        else static_cast<float *>(o.out)[m * o.stride + n] = v * scale;
+__device__ __forceinline__ void put(const XentPack &k, const Out &o, int64_t m, int64_t n, float v,
+                                    float scale) {
+    if (m >= o.rows || n >= k.d) return;
+    if (o.classes) {
+        if (k.bias[m] == -INFINITY) v = 0.0f;
+    } else if (P == 2) {
+        scale *= k.weight[m];
     }
+    if constexpr (P == 1) static_cast<__bf16 *>(o.out)[m * o.stride + n] = (__bf16)v;
+    else static_cast<float *>(o.out)[m * o.stride + n] = v * scale;
 }
 
-// dh[i][j] += sum over the piece's v of g[v][i] W[v][j].
-template <int P>
-__global__ __launch_bounds__(256, 2) void k_xent_dh(XentPack k, int64_t v0, int64_t classes_pad,
-                                                 int64_t r0, int64_t rows_pad, int64_t plane,
-                                                 int32_t row_tiles, const u16 *__restrict__ g,
-                                                 Out o) {
+// The products with G: dh (A = G across, m the rows) and dW (A = G along, m the classes),
+// B = W or h across.  C's first row is m_first of the output.
+template <int P, bool AK, class C>
+__global__ __launch_bounds__(C::WAVES * 64, 2) void k_xent_product(XentPack k, Operand a,
+                                                                   Operand b, int32_t tiles_m,
+                                                                   int32_t tiles_n, int64_t steps,
+                                                                   int64_t m_first, Out o) {
     extern __shared__ char lds[];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t m0 = (int64_t)(blockIdx.x % row_tiles) * TILE;
-    const int64_t n0 = (int64_t)(blockIdx.x / row_tiles) * TILE;
-    const Operand a{g, plane, rows_pad}, b{k.w + v0 * k.ld, k.v_pad * k.ld, k.ld};
-    const float ws = P == 2 ? ldexpf(1.0f, -scale_exp(k.ctl->w_max)) / G_SCALE : 1.0f;
-    f32x16 acc[2][2];
-    clear(acc);
-    tile_product<P, false, false>(a, b, m0, n0, classes_pad / BK<P>, lds, acc);
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t per = tiles_m * tiles_n, split = blockIdx.x / per;
+    uint32_t tm, tn;
+    tile_of(blockIdx.x % per, per, tiles_m, tiles_n, tm, tn);
+    Acc<C> acc;
+    const auto next = [&](int64_t, int64_t &m0, int64_t &n0) {
+        m0 = (int64_t)tm * C::T;
+        n0 = (int64_t)tn * C::T;
+    };
+    products<P, AK, false, C>(a, b, 1, steps * split / o.splits, steps * (split + 1) / o.splits,
+                              lds, acc, next, [](int64_t) {});
+    const float scale = out_scale<P>(k, o.classes);
+    float *sums = o.acc + split * o.m_pad * k.ld;
 #pragma unroll
-    for (int x = 0; x < 2; ++x)
+    for (int x = 0; x < C::MT; ++x)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            const int64_t i = r0 + m0 + (wave >> 1) * 64 + x * 32 + block_row(r);
-            const float scale = P == 2 ? ws * k.weight[i] : 1.0f;
+            const int64_t m = m_first + (int64_t)tm * C::T + wave / C::WN * C::MT * 32 + x * 32 +
+                              (r >> 2) * 8 + (lane >> 5) * 4 + (r & 3);
 #pragma unroll
-            for (int y = 0; y < 2; ++y)
-                put<P>(o, k.d, k.ld, i, n0 + (wave & 1) * 64 + y * 32 + (lane & 31), acc[x][y][r],
-                       scale);
+            for (int y = 0; y < C::NT; ++y) {
+                const int64_t n = (int64_t)tn * C::T + wave % C::WN * C::NT * 32 + y * 32 +
+                                  (lane & 31);
+                float v = acc[x][y][r];
+                if (o.first && o.last && o.splits == 1) {
+                    put<P>(k, o, m, n, v, scale);
+                } else if (n < k.ld) {
+                    if (!o.first) v += sums[m * k.ld + n];
+                    if (o.last && o.splits == 1) put<P>(k, o, m, n, v, scale);
+                    else sums[m * k.ld + n] = v;
+                }
+            }
         }
 }
 
-// dW[v][j] += sum over the rows of g[v][i] hg[i][j].
+// The splits of a product added, in order, from row m_first of the output on.
 template <int P>
-__global__ __launch_bounds__(256, 2) void k_xent_dw(XentPack k, int64_t v0, int64_t r0, int64_t rows_pad,
-                                                 int64_t plane, int32_t class_tiles,
-                                                 const u16 *__restrict__ g, Out o) {
-    extern __shared__ char lds[];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t m0 = (int64_t)(blockIdx.x % class_tiles) * TILE;
-    const int64_t n0 = (int64_t)(blockIdx.x / class_tiles) * TILE;
-    const Operand a{g, plane, rows_pad}, b{k.hg + r0 * k.ld, k.n_pad * k.ld, k.ld};
-    const float scale = P == 2 ? ldexpf(1.0f, -scale_exp(k.ctl->hg_max)) / G_SCALE : 1.0f;
-    f32x16 acc[2][2];
-    clear(acc);
-    tile_product<P, true, false>(a, b, m0, n0, rows_pad / BK<P>, lds, acc);
-#pragma unroll
-    for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-#pragma unroll
-            for (int y = 0; y < 2; ++y)
-                put<P>(o, k.d, k.ld, v0 + m0 + (wave >> 1) * 64 + x * 32 + block_row(r),
-                       n0 + (wave & 1) * 64 + y * 32 + (lane & 31), acc[x][y][r], scale);
+__global__ __launch_bounds__(256) void k_xent_join_splits(XentPack k, int64_t m_first, Out o) {
+    const int64_t m = m_first + blockIdx.x;
+    const float scale = out_scale<P>(k, o.classes);
+    for (int32_t n = threadIdx.x; n < k.d; n += 256) {
+        float v = 0.0f;
+#pragma unroll 4
+        for (int s = 0; s < o.splits; ++s) v += o.acc[(s * o.m_pad + m) * k.ld + n];
+        put<P>(k, o, m, n, v, scale);
+    }
 }
 
 // db[v] += sum over the rows of G, one wavefront a class.
@@ -587,35 +660,63 @@ uint32_t blocks(int64_t x, int64_t per) { return (uint32_t)((x + per - 1) / per)
 constexpr int64_t PIECE_ROWS = 32768;
 constexpr int64_t PIECE_BYTES = (int64_t)256 << 20;
 
+// Wide tiles where they fill the chip.
+bool wide_tiles(int64_t m, int64_t n, int64_t splits, int num_cus) {
+    return up(m, 256) / 256 * (up(n, 256) / 256) * splits >= num_cus;
+}
+
+// How a product over k of m x n is cut.
+struct Cut {
+    bool wide;
+    int32_t tiles_m, tiles_n, splits;
+};
+Cut cut_of(bool wide, int64_t m, int64_t n, int64_t steps, int num_cus) {
+    // not with many columns of wide tiles wasted
+    wide = wide && up(n, 256) * 5 <= up(n, 128) * 6 &&
+           wide_tiles(m, n, std::max<int64_t>(1, steps / 16), num_cus);
+    const int64_t t = wide ? 256 : 128;
+    Cut c{wide, (int32_t)(m / t), (int32_t)(up(n, t) / t), 1};
+    const int64_t tiles = (int64_t)c.tiles_m * c.tiles_n, slots = (wide ? 1 : 2) * (int64_t)num_cus;
+    // too few tiles: k is split, 8 steps a workgroup at least
+    c.splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>({slots / tiles, steps / 8, 64}));
+    return c;
+}
+
 struct Plan {
     int P;
+    bool wide;
     int64_t n_pad, v_pad, ld, piece_rows, piece_classes;
     int32_t splits;
+    Cut dh, dw;                  // of whole pieces
     size_t ctl, h, hg, w, bias, scale, label, weight, lse, part, g, dh_acc, dw_acc, end;
 };
 
 Plan plan_of(const XentCall &c) {
     Plan p{};
     p.P = c.bf16 ? 1 : 2;
-    p.n_pad = up(c.rows, TILE);
-    p.v_pad = up(c.classes, TILE);
+    p.wide = c.rows > 128 && wide_tiles(c.rows, c.classes, 1, c.num_cus);
+    const int64_t t = p.wide ? 256 : 128, step = 64 / p.P;
+    p.n_pad = up(c.rows, t);
+    p.v_pad = up(c.classes, t);
     p.ld = up(c.dim, LD_PAD);
-    const int64_t row_tiles = p.n_pad / TILE, class_tiles = p.v_pad / TILE;
-    // three workgroups a CU, if there are as many tiles
+    const int64_t row_tiles = p.n_pad / t, class_tiles = p.v_pad / t;
+    // one wide workgroup a CU or two narrow ones
     p.splits = (int32_t)std::max<int64_t>(
-        1, std::min<int64_t>(class_tiles, (3 * (int64_t)c.num_cus + row_tiles - 1) / row_tiles));
+        1, std::min<int64_t>(class_tiles, (p.wide ? 1 : 2) * (int64_t)c.num_cus / row_tiles));
     p.piece_rows = std::min(p.n_pad, PIECE_ROWS);
     p.piece_classes = std::min(
-        p.v_pad, std::max<int64_t>(TILE, PIECE_BYTES / (2 * p.P * p.piece_rows) / TILE * TILE));
+        p.v_pad, std::max<int64_t>(t, PIECE_BYTES / (2 * p.P * p.piece_rows) / t * t));
     size_t at = 0;
     auto take = [&](size_t bytes) {
         const size_t here = at;
         at += (bytes + 255) / 256 * 256;
         return here;
     };
+    // a wide tile may read 128 elements past the last packed row
+    const size_t past = 512;
     p.ctl = take(sizeof(XentCtl));
-    p.h = take((size_t)2 * p.P * p.n_pad * p.ld);
-    p.w = take((size_t)2 * p.P * p.v_pad * p.ld);
+    p.h = take((size_t)2 * p.P * p.n_pad * p.ld + past);
+    p.w = take((size_t)2 * p.P * p.v_pad * p.ld + past);
     p.bias = take((size_t)4 * p.v_pad);
     p.scale = take((size_t)4 * p.n_pad);
     p.label = take((size_t)4 * p.n_pad);
@@ -623,13 +724,48 @@ Plan plan_of(const XentCall &c) {
     p.lse = take((size_t)4 * p.n_pad);
     p.part = take((size_t)16 * p.splits * p.n_pad);
     if (c.grad) {
-        p.hg = c.bf16 ? p.h : take((size_t)2 * p.P * p.n_pad * p.ld);
+        p.hg = c.bf16 ? p.h : take((size_t)2 * p.P * p.n_pad * p.ld + past);
         p.g = take((size_t)2 * p.P * p.piece_rows * p.piece_classes);
-        if (p.piece_classes < p.v_pad) p.dh_acc = take((size_t)4 * p.n_pad * p.ld);
-        if (p.piece_rows < p.n_pad) p.dw_acc = take((size_t)4 * p.v_pad * p.ld);
+        p.dh = cut_of(p.wide, p.piece_rows, c.dim, p.piece_classes / step, c.num_cus);
+        p.dw = cut_of(p.wide, p.piece_classes, c.dim, p.piece_rows / step, c.num_cus);
+        if (p.dh.splits > 1 || p.piece_classes < p.v_pad)
+            p.dh_acc = take((size_t)4 * p.dh.splits * p.n_pad * p.ld);
+        if (p.dw.splits > 1 || p.piece_rows < p.n_pad)
+            p.dw_acc = take((size_t)4 * p.dw.splits * p.v_pad * p.ld);
     }
     p.end = at;
     return p;
+}
+
+template <int P, bool AK>
+void launch_product(hipStream_t s, const XentPack &k, const Operand &a, const Operand &b, Cut cut,
+                    int64_t m, int64_t steps, int64_t m_first, Out o) {
+    cut.tiles_m = (int32_t)(m / (cut.wide ? 256 : 128));
+    o.splits = cut.splits;
+    const dim3 g((uint32_t)cut.tiles_m * cut.tiles_n * cut.splits);
+    if (cut.wide)
+        hipLaunchKernelGGL((k_xent_product<P, AK, Wide>), g, dim3(512), (LDS_TILES<P, Wide>), s, k,
+                           a, b, cut.tiles_m, cut.tiles_n, steps, m_first, o);
+    else
+        hipLaunchKernelGGL((k_xent_product<P, AK, Narrow>), g, dim3(256), (LDS_TILES<P, Narrow>), s,
+                           k, a, b, cut.tiles_m, cut.tiles_n, steps, m_first, o);
+    if (o.last && o.splits > 1 && m_first < o.rows)
+        hipLaunchKernelGGL((k_xent_join_splits<P>), dim3((uint32_t)std::min(m, o.rows - m_first)),
+                           dim3(256), 0, s, k, m_first, o);
+}
+
+template <int P, class C>
+void launch_stats(hipStream_t s, const XentPack &k, int32_t splits, float2 *part) {
+    const int32_t rt = (int32_t)(k.n_pad / C::T), vt = (int32_t)(k.v_pad / C::T);
+    hipLaunchKernelGGL((k_xent_stats<P, C>), dim3((uint32_t)rt * splits), dim3(C::WAVES * 64),
+                       (LDS_TILES<P, C>), s, k, rt, vt, splits, part);
+}
+template <int P, class C>
+void launch_g(hipStream_t s, const XentPack &k, int64_t v0, int64_t nv, int64_t r0, int64_t nr,
+              int64_t plane, const float *lse2, u16 *g) {
+    const int32_t rt = (int32_t)(nr / C::T), vt = (int32_t)(nv / C::T);
+    hipLaunchKernelGGL((k_xent_g<P, C>), dim3((uint32_t)rt * vt), dim3(C::WAVES * 64),
+                       (LDS_TILES<P, C>), s, k, v0, r0, nr, plane, vt, rt, lse2, g);
 }
 
 template <int P, typename T>
@@ -649,14 +785,17 @@ hipError_t run(hipStream_t s, const XentCall &c, const Plan &p, char *m) {
     k.row_scale = reinterpret_cast<float *>(m + p.scale);
     k.label = reinterpret_cast<int32_t *>(m + p.label);
     k.weight = reinterpret_cast<float *>(m + p.weight);
-    float *lse = reinterpret_cast<float *>(m + p.lse);
+    float *lse2 = reinterpret_cast<float *>(m + p.lse);
     float2 *part = reinterpret_cast<float2 *>(m + p.part);
     const dim3 b(256);
-    constexpr int LDS = LDS_TILES<P>;
-    const void *big[] = {reinterpret_cast<const void *>(k_xent_stats<P>),
-                         reinterpret_cast<const void *>(k_xent_g<P>),
-                         reinterpret_cast<const void *>(k_xent_dh<P>),
-                         reinterpret_cast<const void *>(k_xent_dw<P>)};
+    const void *big[] = {reinterpret_cast<const void *>(k_xent_stats<P, Wide>),
+                         reinterpret_cast<const void *>(k_xent_stats<P, Narrow>),
+                         reinterpret_cast<const void *>(k_xent_g<P, Wide>),
+                         reinterpret_cast<const void *>(k_xent_g<P, Narrow>),
+                         reinterpret_cast<const void *>(k_xent_product<P, true, Wide>),
+                         reinterpret_cast<const void *>(k_xent_product<P, true, Narrow>),
+                         reinterpret_cast<const void *>(k_xent_product<P, false, Wide>),
+                         reinterpret_cast<const void *>(k_xent_product<P, false, Narrow>)};
     for (const void *f : big) {
         const hipError_t e = allow_all_lds(f);
         if (e != hipSuccess) return e;
@@ -667,36 +806,33 @@ hipError_t run(hipStream_t s, const XentCall &c, const Plan &p, char *m) {
     hipLaunchKernelGGL((k_xent_pack_w<T>), dim3(blocks(k.v_pad, 4)), b, 0, s, k, c.w, c.w_stride);
     hipLaunchKernelGGL((k_xent_rows<T>), dim3(blocks(k.n_pad, 4)), b, 0, s, k, c.h, c.h_stride,
                        c.labels, c.weights);
-    hipLaunchKernelGGL((k_xent_stats<P>), dim3((uint32_t)(k.n_pad / TILE * p.splits)), b, LDS, s, k,
-                       k.v_pad / TILE, p.splits, part);
+    if (p.wide) launch_stats<P, Wide>(s, k, p.splits, part);
+    else launch_stats<P, Narrow>(s, k, p.splits, part);
     hipLaunchKernelGGL((k_xent_join<T>), dim3(blocks(k.n_pad, 4)), b, 0, s, k, c, 2 * p.splits,
-                       part, lse);
+                       part, lse2);
     if (!c.grad) return hipGetLastError();
     if constexpr (P == 2)
         hipLaunchKernelGGL(k_xent_pack_hg, dim3(blocks(k.n_pad, 4)), b, 0, s, k,
                            static_cast<const float *>(c.h), c.h_stride);
     u16 *g = reinterpret_cast<u16 *>(m + p.g);
-    const int64_t plane = p.piece_rows * p.piece_classes;
-    const uint32_t cols = (uint32_t)(p.ld / TILE);
+    const int64_t plane = p.piece_rows * p.piece_classes, step = BK<P>;
     for (int64_t v0 = 0; v0 < k.v_pad; v0 += p.piece_classes)
         for (int64_t r0 = 0; r0 < k.n_pad; r0 += p.piece_rows) {
             const int64_t nv = std::min(p.piece_classes, k.v_pad - v0);
             const int64_t nr = std::min(p.piece_rows, k.n_pad - r0);
-            const int32_t vt = (int32_t)(nv / TILE), rt = (int32_t)(nr / TILE);
-            hipLaunchKernelGGL((k_xent_g<P>), dim3((uint32_t)(vt * rt)), b, LDS, s, k, v0, r0, nr,
-                               plane, rt, lse, g);
-            if (c.dh) {
-                const Out o{reinterpret_cast<float *>(m + p.dh_acc), v0 == 0, v0 + nv == k.v_pad,
-                            nullptr, c.dh, k.n, c.h_stride};
-                hipLaunchKernelGGL((k_xent_dh<P>), dim3((uint32_t)rt * cols), b, LDS, s, k, v0, nv,
-                                   r0, nr, plane, rt, g, o);
-            }
-            if (c.dw) {
-                const Out o{reinterpret_cast<float *>(m + p.dw_acc), r0 == 0, r0 + nr == k.n_pad,
-                            k.bias, c.dw, k.v, c.w_stride};
-                hipLaunchKernelGGL((k_xent_dw<P>), dim3((uint32_t)vt * cols), b, LDS, s, k, v0, r0,
-                                   nr, plane, vt, g, o);
-            }
+            if (p.wide) launch_g<P, Wide>(s, k, v0, nv, r0, nr, plane, lse2, g);
+            else launch_g<P, Narrow>(s, k, v0, nv, r0, nr, plane, lse2, g);
+            const Operand ag{g, plane, nr};
+            if (c.dh)
+                launch_product<P, false>(
+                    s, k, ag, {k.w + v0 * k.ld, k.v_pad * k.ld, k.ld}, p.dh, nr, nv / step, r0,
+                    Out{reinterpret_cast<float *>(m + p.dh_acc), k.n_pad, v0 == 0,
+                        v0 + nv == k.v_pad, 1, c.dh, k.n, c.h_stride, false});
+            if (c.dw)
+                launch_product<P, true>(
+                    s, k, ag, {k.hg + r0 * k.ld, k.n_pad * k.ld, k.ld}, p.dw, nv, nr / step, v0,
+                    Out{reinterpret_cast<float *>(m + p.dw_acc), k.v_pad, r0 == 0,
+                        r0 + nr == k.n_pad, 1, c.dw, k.v, c.w_stride, true});
             if (c.dbias) {
                 const int64_t live = std::min(nv, k.v - v0);
                 hipLaunchKernelGGL((k_xent_db<P>), dim3(blocks(live, 4)), b, 0, s, k, v0, live, r0,

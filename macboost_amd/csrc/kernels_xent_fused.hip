@@ -186,13 +186,6 @@ template <int LD> __device__ __forceinline__ int chunk_xor(int row) {
 }
 template <int P, int LD> constexpr int TILE_BYTES = P * TY * LD * 2;
 
-typedef __attribute__((address_space(3))) void lds_void;
-typedef const __attribute__((address_space(1))) void global_void;
-
-// The copies that this wavefront has started are in LDS; a barrier alone does not wait
-// for them.
-__device__ __forceinline__ void copies_done() { __builtin_amdgcn_s_waitcnt(0x0F70); }
-
 // Starts the copies of a tile's operand; the LDS side is linear, so the source is
 // read in the permuted order.
 template <int P, int LD>
@@ -249,15 +242,11 @@ template <int P> __device__ __forceinline__ void pack8(const float (&x)[8], u32x
 // column l % 32 of the block and rows 4 (l / 32) + 0..3 and 8 + that.  They wait for
 // themselves: the compiler would have the builtin wait for the copies of the next
 // tile too, which no read here depends on.
-__device__ __forceinline__ uint32_t lds_address(const char *p) {
-    return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char *)p;
-}
 template <int LD> __device__ __forceinline__ int across_at() {
     const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
     const int r = (g >> 1) * 4 + (i >> 2), c = (g & 1) * 16 + (i & 3) * 4;
     return r * (LD * 2) + ((c >> 3) ^ chunk_xor<LD>(r)) * 16 + (c & 7) * 2;
 }
-typedef __attribute__((ext_vector_type(2))) unsigned int u32x2;
 #define TR(dst, addr, off) "ds_read_b64_tr_b16 " dst ", " addr " offset:" off "\n\t"
 template <int P, int LD, int ROW, int COL>
 __device__ __forceinline__ void across(uint32_t at, u32x4 (&f)[2][P]) {
@@ -358,10 +347,6 @@ template <typename V> __device__ __forceinline__ void of_rows(const V *rows, int
         for (int e = 0; e < 4; ++e) out[q * 4 + e] = v[e];
     }
 }
-template <int Y> struct At {
-    static constexpr int value = Y;
-};
-
 __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 64); }
 
 // ---- rows pass ----------------------------------------------------------------------

@@ -9,6 +9,8 @@
 namespace mbk {
 
 typedef __attribute__((ext_vector_type(4))) unsigned int u32x4;       // 8 operands
+typedef __attribute__((ext_vector_type(2))) unsigned int u32x2;
+typedef __attribute__((ext_vector_type(4))) float f32x4;
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 typedef __attribute__((ext_vector_type(4))) short i16x4;
@@ -85,6 +87,22 @@ __device__ __forceinline__ f32x16 mma(const u32x4 (&a)[P], const u32x4 (&b)[P], 
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(a0, b0, c, 0, 0, 0);
     }
 }
+
+// ---- copies from memory to LDS
+typedef __attribute__((address_space(3))) void lds_void;
+typedef const __attribute__((address_space(1))) void global_void;
+
+// The copies that this wavefront has started are in LDS; a barrier alone does not wait
+// for them.
+__device__ __forceinline__ void copies_done() { __builtin_amdgcn_s_waitcnt(0x0F70); }
+
+__device__ __forceinline__ uint32_t lds_address(const char *p) {
+    return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char *)p;
+}
+// A number that a generic lambda takes as a constant.
+template <int N> struct At {
+    static constexpr int value = N;
+};
 
 // The kernels of up to XENT_FUSED_DIM outputs (kernels_xent_fused.hip): scores, their
 // exponentials and the product with them in one pass for dh and one for dW.

@@ -49,6 +49,21 @@ def test_xent_sizes(ctx, kind, n, d, v):
     D.check(x.results(), want)
 
 
+@pytest.mark.parametrize("kind,n,d,v", [
+    ("f32", 2100, 200, 8200), ("bf16", 2100, 200, 8200),        # tiles that fill the chip
+    ("f32", 33000, 130, 200), ("bf16", 33000, 130, 200),        # rows in two pieces
+    ("f32", 20, 129, 525000),                                   # classes in two pieces
+    ("f32", 9000, 20, 700), ("bf16", 70, 100, 30000)])
+def test_xent_many_rows_or_classes(ctx, kind, n, d, v):
+    rng, h, w, y = _problem(n + v, n, d, v)
+    bias = rng.standard_normal(v).astype(np.float32)
+    weights = (rng.random(n) + 0.5).astype(np.float32)
+    y[::17] = -1
+    x = D.Xent(ctx, h, w, y, kind, bias, weights)
+    x.grad()
+    D.check(x.results(), D.xent_reference(h, w, y, kind, bias, weights))
+
+
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
 @pytest.mark.parametrize("h_pad,w_pad", [(0, 0), (8, 0), (0, 8), (1, 2)])
 def test_xent_strides_and_no_bias(ctx, kind, h_pad, w_pad):
