@@ -295,8 +295,8 @@ int mbk_treeshap(mbk_context *ctx, const int32_t *feature, const float *threshol
  * stays as it is.  labels, weights (NULL: 1), loss and lse: [rows]; bias: [classes] or
  * NULL.  Outputs must not overlap inputs.
  * A row whose label is outside [0, classes) or whose weight is 0 is left out: its
- * loss and dh are 0, and what its h holds reaches nothing but its own lse (NaN where
- * h holds NaN, infinities or values beyond 2^60).  A class
+ * loss and dh are 0, and what its h holds reaches nothing but its own lse (which may be
+ * NaN where h holds NaN, infinities or values beyond 2^60).  A class
  * whose bias is -INFINITY is not offered: what its w holds reaches nothing, its dw
  * and dbias are 0.  With no class offered every lse is -INFINITY and every row is out.
  * Other h, w and bias must be finite for finite results.  Sums are f32; bf16 operands

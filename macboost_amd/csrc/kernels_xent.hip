@@ -471,62 +471,73 @@ __global__ __launch_bounds__(256) void k_xent_join(XentPack k, XentCall c, int32
 
 // ---- pass 2: G of a piece ------------------------------------------------------------
 // g[v - v0][i - r0], rows of rows_pad; f32: G / w in two f16 terms times 2^15.
+// A workgroup has a tile of rows and every splits-th tile of classes.
 template <int P, class C>
 __global__ __launch_bounds__(C::WAVES * 64, 2) void k_xent_g(XentPack k, int64_t v0, int64_t r0,
                                                              int64_t rows_pad, int64_t plane,
-                                                             int32_t class_tiles,
                                                              int32_t row_tiles,
+                                                             int32_t class_tiles, int32_t splits,
                                                              const float *__restrict__ lse2,
                                                              u16 *__restrict__ g) {
     extern __shared__ char lds[];
-    const int lane = threadIdx.x & 63;
+    const int lane = threadIdx.x & 63, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    uint32_t tm, tn;
-    tile_of(blockIdx.x, gridDim.x, class_tiles, row_tiles, tm, tn);
-    const int64_t i0 = r0 + (int64_t)tn * C::T, c0 = v0 + (int64_t)tm * C::T;
+    uint32_t row_tile, split;
+    tile_of(blockIdx.x, gridDim.x, row_tiles, splits, row_tile, split);
+    const int64_t i0 = r0 + (int64_t)row_tile * C::T;
     const Operand a{k.w, k.v_pad * k.ld, k.ld}, b{k.h, k.n_pad * k.ld, k.ld};
-    Acc<C> acc;
-    const auto next = [&](int64_t, int64_t &m0, int64_t &n0) {
-        m0 = c0;
-        n0 = i0;
-    };
-    products<P, true, true, C>(a, b, 1, 0, (k.d + BK<P> - 1) / BK<P>, lds, acc, next,
-                               [](int64_t) {});
-    const int64_t c = c0 + wave / C::WN * C::MT * 32 + (lane >> 5) * 4;
+    const int64_t iw = i0 + wave % C::WN * C::NT * 32;
+    float sc[C::NT], l[C::NT], wt[C::NT];
+    int32_t label[C::NT];
 #pragma unroll
     for (int y = 0; y < C::NT; ++y) {
-        const int64_t i = i0 + wave % C::WN * C::NT * 32 + y * 32 + (lane & 31);
-        const float sc = P == 2 ? k.row_scale[i] : LOG2E;
-        const int32_t label = k.label[i];
-        // a row that is out: 2^-inf
-        const float l = label < 0 ? INFINITY : lse2[i], wt = k.weight[i];
+        const int64_t i = iw + y * 32 + (lane & 31);
+        sc[y] = P == 2 ? k.row_scale[i] : LOG2E;
+        label[y] = k.label[i];
+        l[y] = label[y] < 0 ? INFINITY : lse2[i];        // a row that is out: 2^-inf
+        wt[y] = P == 2 ? G_SCALE : k.weight[i];
+    }
+    const uint32_t mine = half * 4 * (uint32_t)rows_pad + (lane & 31);
+    Acc<C> acc;
+    const auto next = [&](int64_t i, int64_t &m0, int64_t &n0) {
+        m0 = v0 + (split + i * splits) * C::T;
+        n0 = i0;
+    };
+    const auto done = [&](int64_t i) {
+        const int64_t c0 = v0 + (split + i * splits) * C::T + wave / C::WN * C::MT * 32;
 #pragma unroll
-        for (int x = 0; x < C::MT; ++x) {
-            const int64_t here = c + x * 32;
-            const int64_t mine = label - here;           // 8 q + e if the label is here
-            const bool hot = __any(mine >= 0 && mine < 32);
-            u16 *to = g + (here - v0) * rows_pad + (i - r0);
+        for (int x = 0; x < C::MT; ++x)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const f32x4 b2 = *reinterpret_cast<const f32x4 *>(k.bias + here + q * 8);
+            for (int y = 0; y < C::NT; ++y) {
+                const int64_t c = c0 + x * 32;
+                const int64_t at = label[y] - c - half * 4;      // 8 q + e if the label is here
+                const bool hot = __any(at >= 0 && at < 32);
+                u16 *to = g + (c - v0) * rows_pad + (iw - r0) + y * 32;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float p = __builtin_amdgcn_exp2f(
-                        __builtin_fmaf(acc[x][y][q * 4 + e], sc, b2[e] - l));
-                    if (hot && mine == q * 8 + e) p -= 1.0f;
-                    if constexpr (P == 1) {
-                        *to = bits_of((__bf16)(wt * p));
-                    } else {
-                        u16 hi, lo;
-                        split_f16(p * G_SCALE, hi, lo);
-                        to[0] = hi;
-                        to[plane] = lo;
+                for (int q = 0; q < 4; ++q) {
+                    const f32x4 b2 =
+                        *reinterpret_cast<const f32x4 *>(k.bias + c + half * 4 + q * 8);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float p = __builtin_amdgcn_exp2f(
+                            __builtin_fmaf(acc[x][y][q * 4 + e], sc[y], b2[e] - l[y]));
+                        if (hot && at == q * 8 + e) p -= 1.0f;
+                        p *= wt[y];
+                        if constexpr (P == 1) {
+                            to[mine] = bits_of((__bf16)p);
+                        } else {
+                            u16 hi, lo;
+                            split_f16(p, hi, lo);
+                            to[mine] = hi;
+                            to[plane + mine] = lo;
+                        }
+                        to += e < 3 ? rows_pad : 5 * rows_pad;
                     }
-                    to += e < 3 ? rows_pad : 5 * rows_pad;
                 }
             }
-        }
-    }
+    };
+    const int64_t tiles = (class_tiles - (int64_t)split + splits - 1) / splits;
+    products<P, true, true, C>(a, b, tiles, 0, (k.d + BK<P> - 1) / BK<P>, lds, acc, next, done);
 }
 
 // Where a product over the pieces goes: the f32 sums so far, [split][m_pad][ld], and, with
@@ -656,9 +667,11 @@ __global__ __launch_bounds__(256) void k_xent_zero(T *out, int64_t rows, int32_t
 int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 uint32_t blocks(int64_t x, int64_t per) { return (uint32_t)((x + per - 1) / per); }
 
-// G of a piece: 32k rows and 256 MB at most (what the memory-side cache holds).
+// G of a piece: 32k rows and 512 MB at most.  16384 x 1024 x 65536 bf16 with gradients: 8.8
+// ms; with 256 MB, which the memory-side cache would hold, 9.3 (half the tiles of dW, so
+// that k is split), with 1 GB 8.7.
 constexpr int64_t PIECE_ROWS = 32768;
-constexpr int64_t PIECE_BYTES = (int64_t)256 << 20;
+constexpr int64_t PIECE_BYTES = (int64_t)512 << 20;
 
 // Wide tiles where they fill the chip.
 bool wide_tiles(int64_t m, int64_t n, int64_t splits, int num_cus) {
@@ -682,6 +695,12 @@ Cut cut_of(bool wide, int64_t m, int64_t n, int64_t steps, int num_cus) {
     return c;
 }
 
+// Workgroups that share a tile of rows: one wide workgroup a CU or two narrow ones.
+template <class C> int32_t splits_of(int64_t row_tiles, int64_t class_tiles, int num_cus) {
+    const int64_t slots = (C::T == 256 ? 1 : 2) * (int64_t)num_cus;
+    return (int32_t)std::max<int64_t>(1, std::min(class_tiles, slots / row_tiles));
+}
+
 struct Plan {
     int P;
     bool wide;
@@ -700,9 +719,8 @@ Plan plan_of(const XentCall &c) {
     p.v_pad = up(c.classes, t);
     p.ld = up(c.dim, LD_PAD);
     const int64_t row_tiles = p.n_pad / t, class_tiles = p.v_pad / t;
-    // one wide workgroup a CU or two narrow ones
-    p.splits = (int32_t)std::max<int64_t>(
-        1, std::min<int64_t>(class_tiles, (p.wide ? 1 : 2) * (int64_t)c.num_cus / row_tiles));
+    p.splits = p.wide ? splits_of<Wide>(row_tiles, class_tiles, c.num_cus)
+                      : splits_of<Narrow>(row_tiles, class_tiles, c.num_cus);
     p.piece_rows = std::min(p.n_pad, PIECE_ROWS);
     p.piece_classes = std::min(
         p.v_pad, std::max<int64_t>(t, PIECE_BYTES / (2 * p.P * p.piece_rows) / t * t));
@@ -762,10 +780,11 @@ void launch_stats(hipStream_t s, const XentPack &k, int32_t splits, float2 *part
 }
 template <int P, class C>
 void launch_g(hipStream_t s, const XentPack &k, int64_t v0, int64_t nv, int64_t r0, int64_t nr,
-              int64_t plane, const float *lse2, u16 *g) {
+              int64_t plane, int num_cus, const float *lse2, u16 *g) {
     const int32_t rt = (int32_t)(nr / C::T), vt = (int32_t)(nv / C::T);
-    hipLaunchKernelGGL((k_xent_g<P, C>), dim3((uint32_t)rt * vt), dim3(C::WAVES * 64),
-                       (LDS_TILES<P, C>), s, k, v0, r0, nr, plane, vt, rt, lse2, g);
+    const int32_t splits = splits_of<C>(rt, vt, num_cus);
+    hipLaunchKernelGGL((k_xent_g<P, C>), dim3((uint32_t)rt * splits), dim3(C::WAVES * 64),
+                       (LDS_TILES<P, C>), s, k, v0, r0, nr, plane, rt, vt, splits, lse2, g);
 }
 
 template <int P, typename T>
@@ -820,8 +839,8 @@ hipError_t run(hipStream_t s, const XentCall &c, const Plan &p, char *m) {
         for (int64_t r0 = 0; r0 < k.n_pad; r0 += p.piece_rows) {
             const int64_t nv = std::min(p.piece_classes, k.v_pad - v0);
             const int64_t nr = std::min(p.piece_rows, k.n_pad - r0);
-            if (p.wide) launch_g<P, Wide>(s, k, v0, nv, r0, nr, plane, lse2, g);
-            else launch_g<P, Narrow>(s, k, v0, nv, r0, nr, plane, lse2, g);
+            if (p.wide) launch_g<P, Wide>(s, k, v0, nv, r0, nr, plane, c.num_cus, lse2, g);
+            else launch_g<P, Narrow>(s, k, v0, nv, r0, nr, plane, c.num_cus, lse2, g);
             const Operand ag{g, plane, nr};
             if (c.dh)
                 launch_product<P, false>(
@@ -846,10 +865,12 @@ hipError_t run(hipStream_t s, const XentCall &c, const Plan &p, char *m) {
 
 size_t xent_scratch(const XentCall &c) {
     if (!c.rows) return 0;
+    if (xent_few(c)) return xent_few_scratch(c);
     return c.dim <= XENT_FUSED_DIM ? xent_fused_scratch(c) : plan_of(c).end;
 }
 
 hipError_t launch_xent(hipStream_t s, const XentCall &c, char *scratch) {
+    if (c.rows && xent_few(c)) return launch_xent_few(s, c, scratch);
     if (c.rows && c.dim <= XENT_FUSED_DIM) return launch_xent_fused(s, c, scratch);
     if (c.rows) {
         const Plan p = plan_of(c);

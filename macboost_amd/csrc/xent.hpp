@@ -110,4 +110,9 @@ constexpr int XENT_FUSED_DIM = 128;
 size_t xent_fused_scratch(const XentCall &c);
 hipError_t launch_xent_fused(hipStream_t s, const XentCall &c, char *scratch);
 
+// The loss of few rows (kernels_xent_few.hip), whose work is one reading of W.
+bool xent_few(const XentCall &c);
+size_t xent_few_scratch(const XentCall &c);
+hipError_t launch_xent_few(hipStream_t s, const XentCall &c, char *scratch);
+
 }  // namespace mbk

@@ -52,7 +52,7 @@ def test_xent_sizes(ctx, kind, n, d, v):
 @pytest.mark.parametrize("kind,n,d,v", [
     ("f32", 2100, 200, 8200), ("bf16", 2100, 200, 8200),        # tiles that fill the chip
     ("f32", 33000, 130, 200), ("bf16", 33000, 130, 200),        # rows in two pieces
-    ("f32", 20, 129, 525000),                                   # classes in two pieces
+    ("f32", 5, 129, 1048576 + 700),                             # classes in two pieces
     ("f32", 9000, 20, 700), ("bf16", 70, 100, 30000)])
 def test_xent_many_rows_or_classes(ctx, kind, n, d, v):
     rng, h, w, y = _problem(n + v, n, d, v)
@@ -62,6 +62,36 @@ def test_xent_many_rows_or_classes(ctx, kind, n, d, v):
     x = D.Xent(ctx, h, w, y, kind, bias, weights)
     x.grad()
     D.check(x.results(), D.xent_reference(h, w, y, kind, bias, weights))
+
+
+@pytest.mark.parametrize("kind,d", [("f32", 4), ("f32", 64), ("f32", 100), ("f32", 512),
+                                    ("bf16", 8), ("bf16", 64), ("bf16", 200), ("bf16", 1024)])
+@pytest.mark.parametrize("n,v", [(1, 1), (1, 1000), (3, 33), (16, 5000), (32, 70000), (32, 300)])
+def test_xent_loss_of_few_rows(ctx, kind, d, n, v):
+    rng, h, w, y = _problem(n + v + d, n, d, v)
+    bias = rng.standard_normal(v).astype(np.float32)
+    weights = (rng.random(n) + 0.5).astype(np.float32)
+    closed = rng.random(v) < 0.2
+    closed[0] = False
+    open_classes = np.flatnonzero(~closed)
+    y = open_classes[rng.integers(0, open_classes.size, n)].astype(np.int32)
+    bias[closed] = -np.inf
+    y[n // 2] = -1
+    weights[n // 3] = 0
+    want = D.xent_reference(h, w, y, kind, bias, weights)
+    w[closed] = np.nan                   # not read
+    h[n // 2] = np.inf
+    x = D.Xent(ctx, h, w, y, kind, bias, weights, h_pad=3, w_pad=8)
+    x.forward()
+    got = x.results(False)
+    keep = np.arange(n) != n // 2
+    got["lse"], want["lse"] = got["lse"][keep], tuple(t[keep] for t in want["lse"])
+    D.check(got, want, ("loss", "lse"))
+    # without bias and weights
+    _, h, w, y = _problem(n + v + d, n, d, v)
+    x = D.Xent(ctx, h, w, y, kind)
+    x.forward()
+    D.check(x.results(False), D.xent_reference(h, w, y, kind), ("loss", "lse"))
 
 
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
