@@ -24,9 +24,101 @@ __device__ __forceinline__ float to_f32(__bf16 v) { return (float)v; }
 // counts them by expert, the counts are summed over the wavefronts before it
 // and the experts below, and it then hands out slots in ascending order: every
 // step is ordered, so the sort is stable and needs no atomic on global memory.
-// Counters of one wavefront lie in LDS.
+// Counters of one wavefront lie in LDS.  Keys are loaded AHEAD at a time, since one at a
+// time waits for memory.
 // ---------------------------------------------------------------------------
 constexpr int SORT_WAVES = 4;
+constexpr int AHEAD = 8;
+
+// Workgroups go to the 8 XCDs in turn; each XCD gets a run of them, so that neighbours'
+// writes to one list meet in one L2.
+__device__ __forceinline__ uint32_t run_of(uint32_t id, uint32_t total) {
+    const uint32_t xcd = id & 7, per = total >> 3, more = total & 7;
+    return xcd * per + min(xcd, more) + (id >> 3);
+}
+
+// Keys [a, b) in their order, 64 at a time: take(first index, key), -1 behind the end.
+template <class Take>
+__device__ __forceinline__ void each_key(const int32_t *__restrict__ expert, int64_t a, int64_t b,
+                                         Take take) {
+    const int lane = threadIdx.x & 63;
+    int32_t ahead[AHEAD];
+    const auto load = [&](int64_t i0) {
+#pragma unroll
+        for (int q = 0; q < AHEAD; ++q) {
+            const int64_t i = i0 + q * 64 + lane;
+            ahead[q] = i < b ? expert[i] : -1;
+        }
+    };
+    if (a < b) load(a);
+    for (int64_t i0 = a; i0 < b; i0 += 64 * AHEAD) {
+        int32_t now[AHEAD];
+#pragma unroll
+        for (int q = 0; q < AHEAD; ++q) now[q] = ahead[q];
+        if (i0 + 64 * AHEAD < b) load(i0 + 64 * AHEAD);
+#pragma unroll
+        for (int q = 0; q < AHEAD; ++q)
+            if (i0 + q * 64 < b) take(i0 + q * 64, (uint32_t)now[q]);
+    }
+}
+
+__device__ __forceinline__ void count_keys(const int32_t *__restrict__ expert, int64_t a, int64_t b,
+                                           int32_t experts, uint32_t *count) {
+    each_key(expert, a, b, [&](int64_t, uint32_t e) {
+        if (e < (uint32_t)experts) atomicAdd(&count[e], 1u);
+    });
+}
+
+// next[e]: the slot that the wavefront's next assignment to e gets.
+__device__ __forceinline__ void place_keys(const int32_t *__restrict__ expert, int64_t a, int64_t b,
+                                           int32_t experts, int32_t key_bits, uint32_t *next,
+                                           int64_t kept_all, int32_t *__restrict__ source,
+                                           int32_t *__restrict__ slot) {
+    const int lane = threadIdx.x & 63;
+    each_key(expert, a, b, [&](int64_t i0, uint32_t e) {
+        const int64_t i = i0 + lane;
+        const bool kept = e < (uint32_t)experts;
+        uint64_t same = __ballot(kept);         // lanes with this lane's expert
+        for (int k = 0; k < key_bits; ++k) {
+            const uint64_t ones = __ballot((e >> k) & 1u);
+            same &= (e >> k) & 1u ? ones : ~ones;
+        }
+        const uint32_t rank = lanes_below(same);
+        uint32_t at = 0;
+        if (kept) at = next[e] + rank;
+        __builtin_amdgcn_wave_barrier();
+        if (kept && rank == 0) next[e] = at + (uint32_t)__popcll(same);
+        __builtin_amdgcn_wave_barrier();
+        if (kept) source[at] = (int32_t)i;
+        if (i < b) {
+            slot[i] = kept ? (int32_t)at : -1;
+            if (i >= kept_all) source[i] = -1;  // behind the last slot taken
+        }
+    });
+}
+
+// The sum of v over the threads before, and over all, of a workgroup of W wavefronts.
+template <int W>
+__device__ __forceinline__ uint32_t sum_before(uint32_t v, uint32_t *wave_sum, uint32_t &all) {
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    uint32_t x = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t y = __shfl_up(x, o, 64);
+        if (lane >= o) x += y;
+    }
+    if (lane == 63) wave_sum[wave] = x;
+    __syncthreads();
+    uint32_t before = 0;
+    all = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+        if (w < wave) before += wave_sum[w];
+        all += wave_sum[w];
+    }
+    __syncthreads();
+    return before + x - v;
+}
 
 // table[e * units + u]: assignments of wavefront u to expert e.
 __global__ __launch_bounds__(64 * SORT_WAVES) void k_expert_count(
@@ -35,41 +127,35 @@ __global__ __launch_bounds__(64 * SORT_WAVES) void k_expert_count(
     extern __shared__ uint32_t lds[];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     uint32_t *count = lds + (size_t)wave * experts;
-    const int32_t u = blockIdx.x * SORT_WAVES + wave;
+    const int32_t u = run_of(blockIdx.x, gridDim.x) * SORT_WAVES + wave;
     for (int e = lane; e < experts; e += 64) count[e] = 0;
     __syncthreads();
-    if (u < units) {
-        const int64_t a = u * per, b = min(slots, a + per);
-        for (int64_t i = a + lane; i < b; i += 64) {
-            const uint32_t e = (uint32_t)expert[i];
-            if (e < (uint32_t)experts) atomicAdd(&count[e], 1u);
-        }
-    }
+    if (u < units) count_keys(expert, u * per, min(slots, (u + 1) * per), experts, count);
     __syncthreads();
     if (u < units)
         for (int e = lane; e < experts; e += 64) table[(int64_t)e * units + u] = count[e];
 }
 
-// One wavefront per expert: its counts become sums over the wavefronts before,
-// total[e] their sum.
-__global__ __launch_bounds__(256) void k_expert_scan(uint32_t *__restrict__ table, int32_t experts,
-                                                     int32_t units, uint32_t *__restrict__ total) {
-    const int e = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (e >= experts) return;
-    uint32_t *row = table + (int64_t)e * units;
-    uint32_t sum = 0;
-    for (int u0 = 0; u0 < units; u0 += 64) {
-        const uint32_t c = u0 + lane < units ? row[u0 + lane] : 0;
-        uint32_t x = c;
+// A workgroup an expert: its counts become sums over the wavefronts before, total[e] their
+// sum.  Up to 8 wavefronts' counts a thread.
+constexpr int SCAN = 256, SCAN_EACH = 8;
+__global__ __launch_bounds__(SCAN) void k_expert_scan(uint32_t *__restrict__ table, int32_t units,
+                                                      uint32_t *__restrict__ total) {
+    __shared__ uint32_t wave_sum[SCAN / 64];
+    uint32_t *row = table + (int64_t)blockIdx.x * units;
+    const int u0 = threadIdx.x * SCAN_EACH;
+    uint32_t c[SCAN_EACH], sum = 0, all;
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const uint32_t y = __shfl_up(x, o, 64);
-            if (lane >= o) x += y;
-        }
-        if (u0 + lane < units) row[u0 + lane] = sum + x - c;
-        sum += __shfl(x, 63, 64);
+    for (int q = 0; q < SCAN_EACH; ++q) c[q] = u0 + q < units ? row[u0 + q] : 0;
+#pragma unroll
+    for (int q = 0; q < SCAN_EACH; ++q) sum += c[q];
+    uint32_t before = sum_before<SCAN / 64>(sum, wave_sum, all);
+#pragma unroll
+    for (int q = 0; q < SCAN_EACH; ++q) {
+        if (u0 + q < units) row[u0 + q] = before;
+        before += c[q];
     }
-    if (lane == 0) total[e] = sum;
+    if (threadIdx.x == 0) total[blockIdx.x] = all;
 }
 
 // offsets[e] = assignments to experts below e, by one workgroup.
@@ -77,27 +163,12 @@ __global__ __launch_bounds__(1024) void k_expert_offsets(const uint32_t *__restr
                                                          int32_t experts,
                                                          int32_t *__restrict__ offsets) {
     __shared__ uint32_t wave_sum[16];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    uint32_t before = 0;
+    uint32_t before = 0, all;
     for (int e0 = 0; e0 < experts; e0 += 1024) {
         const int e = e0 + threadIdx.x;
-        const uint32_t c = e < experts ? total[e] : 0;
-        uint32_t x = c;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const uint32_t y = __shfl_up(x, o, 64);
-            if (lane >= o) x += y;
-        }
-        if (lane == 63) wave_sum[wave] = x;
-        __syncthreads();
-        uint32_t below = 0, all = 0;
-        for (int w = 0; w < 16; ++w) {
-            if (w < wave) below += wave_sum[w];
-            all += wave_sum[w];
-        }
-        if (e < experts) offsets[e] = (int32_t)(before + below + x - c);
+        const uint32_t below = sum_before<16>(e < experts ? total[e] : 0, wave_sum, all);
+        if (e < experts) offsets[e] = (int32_t)(before + below);
         before += all;
-        __syncthreads();
     }
     if (threadIdx.x == 0) offsets[experts] = (int32_t)before;
 }
@@ -110,42 +181,63 @@ __global__ __launch_bounds__(64 * SORT_WAVES) void k_expert_place(
     extern __shared__ uint32_t lds[];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     uint32_t *next = lds + (size_t)wave * experts;
-    const int32_t u = blockIdx.x * SORT_WAVES + wave;
+    const int32_t u = run_of(blockIdx.x, gridDim.x) * SORT_WAVES + wave;
     if (u >= units) return;                     // no barrier below
     for (int e = lane; e < experts; e += 64)
         next[e] = (uint32_t)offsets[e] + table[(int64_t)e * units + u];
-    const int64_t a = u * per, b = min(slots, a + per);
-    for (int64_t i0 = a; i0 < b; i0 += 64) {
-        const int64_t i = i0 + lane;
-        const uint32_t e = i < b ? (uint32_t)expert[i] : 0xFFFFFFFFu;
-        const bool kept = e < (uint32_t)experts;
-        uint64_t same = __ballot(kept);         // lanes with this lane's expert
-        for (int k = 0; k < key_bits; ++k) {
-            const uint64_t ones = __ballot((e >> k) & 1u);
-            same &= (e >> k) & 1u ? ones : ~ones;
+    place_keys(expert, u * per, min(slots, (u + 1) * per), experts, key_bits, next,
+               offsets[experts], source, slot);
+}
+
+// Few assignments: the whole sort by one workgroup (1000 to 4 experts 13 us less than by
+// the four kernels above, whose launches are all there is).
+constexpr int SMALL_WAVES = 16;
+constexpr int64_t SMALL_SLOTS = 16384;
+constexpr int32_t SMALL_EXPERTS = 2048;
+__global__ __launch_bounds__(64 * SMALL_WAVES) void k_expert_sort_small(
+    const int32_t *__restrict__ expert, int64_t slots, int32_t experts, int32_t key_bits,
+    int64_t per, int32_t *__restrict__ offsets, int32_t *__restrict__ source,
+    int32_t *__restrict__ slot) {
+    extern __shared__ uint32_t lds[];
+    uint32_t *wave_sum = lds, *count = lds + SMALL_WAVES;        // [wave][expert]
+    const int wave = threadIdx.x >> 6;
+    for (int e = threadIdx.x; e < SMALL_WAVES * experts; e += 64 * SMALL_WAVES) count[e] = 0;
+    __syncthreads();
+    const int64_t a = min(slots, wave * per), b = min(slots, a + per);
+    count_keys(expert, a, b, experts, count + wave * experts);
+    __syncthreads();
+    uint32_t before = 0, all;
+    for (int e0 = 0; e0 < experts; e0 += 64 * SMALL_WAVES) {
+        const int e = e0 + threadIdx.x;
+        uint32_t sum = 0;
+        if (e < experts)
+            for (int w = 0; w < SMALL_WAVES; ++w) sum += count[w * experts + e];
+        uint32_t at = before + sum_before<SMALL_WAVES>(sum, wave_sum, all);
+        if (e < experts) {
+            offsets[e] = (int32_t)at;
+            for (int w = 0; w < SMALL_WAVES; ++w) {
+                const uint32_t c = count[w * experts + e];
+                count[w * experts + e] = at;
+                at += c;
+            }
         }
-        uint32_t at = 0;
-        if (kept) at = next[e] + lanes_below(same);
-        __builtin_amdgcn_wave_barrier();
-        if (kept && lanes_below(same) == 0) next[e] = at + (uint32_t)__popcll(same);
-        __builtin_amdgcn_wave_barrier();
-        if (kept) source[at] = (int32_t)i;
-        if (i < b) slot[i] = kept ? (int32_t)at : -1;
+        before += all;
     }
-    // the places behind the last kept assignment
-    const int64_t kept = offsets[experts];
-    for (int64_t i = a + lane; i < b; i += 64)
-        if (i >= kept) source[i] = -1;
+    if (threadIdx.x == 0) offsets[experts] = (int32_t)before;
+    __syncthreads();
+    place_keys(expert, a, b, experts, key_bits, count + wave * experts, before, source, slot);
 }
 
 struct SortShape {
     int64_t per;
     int32_t units;
 };
-// At least 1024 assignments a wavefront, at most 8 wavefronts a CU and 4M counters.
+// At least 1024 assignments a wavefront, at most 8 wavefronts a CU (a thread of the scan
+// takes eight) and 4M counters.
 SortShape sort_shape(const ExpertPlan &p, int num_cus) {
     const int64_t slots = p.rows * p.k;
-    int64_t units = std::min<int64_t>((slots + 1023) / 1024, 8 * (int64_t)num_cus);
+    int64_t units = std::min<int64_t>((slots + 1023) / 1024,
+                                      std::min<int64_t>(8 * (int64_t)num_cus, SCAN * SCAN_EACH));
     units = std::max<int64_t>(1, std::min<int64_t>(units, ((int64_t)4 << 20) / p.experts));
     const int64_t per = std::max<int64_t>(64, ((slots + units - 1) / units + 63) / 64 * 64);
     return {per, (int32_t)std::max<int64_t>(1, (slots + per - 1) / per)};
@@ -171,11 +263,219 @@ __device__ __forceinline__ Place place_of(const ExpertPlan &p, int64_t a, int32_
     return {(int64_t)first * cols + (s - first), p.offsets[e + 1] - first};
 }
 
-constexpr int TILE = 64;
+// ---- both matrices by rows: L lanes a row, B bytes a lane ----
+template <int B> struct Bytes;
+template <> struct Bytes<16> { typedef __attribute__((ext_vector_type(4))) uint32_t type; };
+template <> struct Bytes<4> { typedef uint32_t type; };
+template <> struct Bytes<2> { typedef uint16_t type; };
 
-// A tile of 64 rows x 64 columns at a time, 256 threads; XCOLS / SCOLS: the lanes of a
-// wavefront run along the columns of the rows' matrix / of the sorted matrix, else
-// along the rows; LDS turns the tile where the two differ.
+// Row and chunks of a lane: rows_of(256 / lanes a workgroup).
+struct RowLanes {
+    int64_t row;
+    int lane, lanes;
+};
+__device__ __forceinline__ RowLanes row_lanes(int log2_lanes) {
+    const int lanes = 1 << log2_lanes;
+    return {((int64_t)blockIdx.x << (8 - log2_lanes)) + (threadIdx.x >> log2_lanes),
+            (int)threadIdx.x & (lanes - 1), lanes};
+}
+
+// A row is read once and written to each of its slots.
+template <typename T, int B>
+__global__ __launch_bounds__(256) void k_expert_gather_rows(ExpertPlan p, ExpertMatrix x,
+                                                            int32_t chunks, int log2_lanes,
+                                                            T *__restrict__ sorted) {
+    typedef typename Bytes<B>::type V;
+    const RowLanes r = row_lanes(log2_lanes);
+    if (r.row >= p.rows) return;
+    const V *from = reinterpret_cast<const V *>(static_cast<const T *>(x.data) +
+                                                r.row * x.row_stride);
+    const int32_t *slots = p.slot + r.row * p.k;
+    for (int c = r.lane; c < chunks; c += 4 * r.lanes) {
+        V v[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            if (c + q * r.lanes < chunks) v[q] = from[c + q * r.lanes];
+        for (int j = 0; j < p.k; ++j) {
+            const int32_t s = slots[j];
+            if (s < 0) continue;
+            V *to = reinterpret_cast<V *>(sorted + (int64_t)s * x.cols);
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (c + q * r.lanes < chunks) to[c + q * r.lanes] = v[q];
+        }
+    }
+}
+
+template <typename T, int B>
+__global__ __launch_bounds__(256) void k_expert_combine_rows(ExpertPlan p,
+                                                             const T *__restrict__ sorted,
+                                                             const float *__restrict__ weights,
+                                                             ExpertMatrix out, int32_t chunks,
+                                                             int log2_lanes) {
+    typedef typename Bytes<B>::type V;
+    constexpr int E = B / sizeof(T);
+    const RowLanes r = row_lanes(log2_lanes);
+    if (r.row >= p.rows) return;
+    V *to = reinterpret_cast<V *>(static_cast<T *>(out.data) + r.row * out.row_stride);
+    for (int c = r.lane; c < chunks; c += 2 * r.lanes) {
+        float sum[2][E];
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+            for (int e = 0; e < E; ++e) sum[q][e] = 0.0f;
+        for (int j = 0; j < p.k; ++j) {
+            const int64_t a = r.row * p.k + j;
+            const int32_t s = p.slot[a];
+            if (s < 0) continue;
+            const float w = weights ? weights[a] : 1.0f;
+            const V *from = reinterpret_cast<const V *>(sorted + (int64_t)s * out.cols);
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                if (c + q * r.lanes >= chunks) break;
+                const V v = from[c + q * r.lanes];
+                T x[E];
+                __builtin_memcpy(x, &v, B);
+#pragma unroll
+                for (int e = 0; e < E; ++e) sum[q][e] += w * to_f32(x[e]);
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            if (c + q * r.lanes >= chunks) break;
+            T x[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) x[e] = (T)sum[q][e];
+            V v;
+            __builtin_memcpy(&v, x, B);
+            to[c + q * r.lanes] = v;
+        }
+    }
+}
+
+// A row's dot products are summed by its lanes, each over its own columns, and the lanes
+// added in a fixed order.
+template <typename T, int B>
+__global__ __launch_bounds__(256) void k_expert_combine_grad_rows(
+    ExpertPlan p, ExpertMatrix dout, const T *__restrict__ sorted,
+    const float *__restrict__ weights, T *__restrict__ d_sorted, float *__restrict__ d_weights,
+    int32_t chunks, int log2_lanes) {
+    typedef typename Bytes<B>::type V;
+    constexpr int E = B / sizeof(T);
+    const RowLanes r = row_lanes(log2_lanes);
+    if (r.row >= p.rows) return;
+    const V *from = reinterpret_cast<const V *>(static_cast<const T *>(dout.data) +
+                                                r.row * dout.row_stride);
+    for (int j = 0; j < p.k; ++j) {
+        const int64_t a = r.row * p.k + j;
+        const int32_t s = p.slot[a];
+        float dot = 0.0f;
+        if (s >= 0) {
+            const float w = weights ? weights[a] : 1.0f;
+            const V *y = reinterpret_cast<const V *>(sorted + (int64_t)s * dout.cols);
+            V *dy = reinterpret_cast<V *>(d_sorted + (int64_t)s * dout.cols);
+#pragma unroll 2
+            for (int c = r.lane; c < chunks; c += r.lanes) {
+                const V gv = from[c], yv = y[c];
+                T g[E], x[E];
+                __builtin_memcpy(g, &gv, B);
+                __builtin_memcpy(x, &yv, B);
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const float f = to_f32(g[e]);
+                    dot += f * to_f32(x[e]);
+                    x[e] = (T)(w * f);
+                }
+                V v;
+                __builtin_memcpy(&v, x, B);
+                dy[c] = v;
+            }
+        }
+        for (int o = r.lanes / 2; o > 0; o >>= 1) dot += __shfl_xor(dot, o, 64);
+        if (r.lane == 0) d_weights[a] = s < 0 ? 0.0f : dot;
+    }
+}
+
+// ---- feature-major to blocks: the assignments of a run of rows, in LDS in their order ----
+// An expert's assignments of consecutive rows have consecutive slots: with the run's values
+// of a column ordered by (expert, slot) in LDS, both sides of the copy are runs of
+// addresses.
+constexpr int RUN = 1024, RUN_COLS = 8, RUN_EXPERTS = 512;
+template <typename T>
+__global__ __launch_bounds__(256) void k_expert_gather_runs(ExpertPlan p, ExpertMatrix x,
+                                                            int32_t run_rows,
+                                                            T *__restrict__ sorted) {
+    __shared__ uint32_t first[RUN_EXPERTS], begin[RUN_EXPERTS], wave_sum[4];
+    __shared__ int64_t base[RUN];
+    __shared__ int32_t step[RUN];
+    __shared__ T tile[RUN_COLS][RUN];
+    const int64_t i0 = (int64_t)run_of(blockIdx.x, gridDim.x) * run_rows;
+    const int32_t rows = (int32_t)min((int64_t)run_rows, p.rows - i0), n = rows * p.k;
+    for (int e = threadIdx.x; e < RUN_EXPERTS; e += 256) {
+        first[e] = 0xFFFFFFFFu;
+        begin[e] = 0;
+    }
+    __syncthreads();
+    int32_t slot[RUN / 256], expert[RUN / 256];
+#pragma unroll
+    for (int q = 0; q < RUN / 256; ++q) {
+        const int a = threadIdx.x + 256 * q;
+        slot[q] = a < n ? p.slot[i0 * p.k + a] : -1;
+        expert[q] = slot[q] >= 0 ? p.expert[i0 * p.k + a] : 0;
+        if (slot[q] >= 0) {
+            atomicMin(&first[expert[q]], (uint32_t)slot[q]);
+            atomicAdd(&begin[expert[q]], 1u);
+        }
+    }
+    __syncthreads();
+    uint32_t taken;
+    {
+        const int e = threadIdx.x * 2;               // RUN_EXPERTS / 256 experts a thread
+        const uint32_t c0 = begin[e], c1 = begin[e + 1];
+        const uint32_t before = sum_before<4>(c0 + c1, wave_sum, taken);
+        begin[e] = before;
+        begin[e + 1] = before + c0;
+    }
+    __syncthreads();
+    int at[RUN / 256], row[RUN / 256];
+#pragma unroll
+    for (int q = 0; q < RUN / 256; ++q) {
+        at[q] = -1;
+        row[q] = (threadIdx.x + 256 * q) / p.k;
+        if (slot[q] < 0) continue;
+        const int32_t e = expert[q], o = p.offsets[e];
+        at[q] = (int)(begin[e] + ((uint32_t)slot[q] - first[e]));
+        base[at[q]] = (int64_t)o * x.cols + (slot[q] - o);
+        step[at[q]] = p.offsets[e + 1] - o;
+    }
+    const T *data = static_cast<const T *>(x.data) + i0 * x.row_stride;
+    for (int32_t f0 = blockIdx.y * RUN_COLS; f0 < x.cols; f0 += gridDim.y * RUN_COLS) {
+        const int cols = min(RUN_COLS, x.cols - f0);
+        __syncthreads();                             // base and step, the last columns' reads
+#pragma unroll
+        for (int q = 0; q < RUN / 256; ++q)
+            if (at[q] >= 0)
+#pragma unroll
+                for (int c = 0; c < RUN_COLS; ++c)
+                    if (c < cols)
+                        tile[c][at[q]] = data[row[q] * x.row_stride + (f0 + c) * x.col_stride];
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < RUN / 256; ++q) {
+            const int l = threadIdx.x + 256 * q;
+            if (l >= (int)taken) break;
+            T *to = sorted + base[l] + (int64_t)f0 * step[l];
+#pragma unroll
+            for (int c = 0; c < RUN_COLS; ++c)
+                if (c < cols) to[(int64_t)c * step[l]] = tile[c][l];
+        }
+    }
+}
+
+// ---- other layouts: a tile of 64 rows x 64 columns at a time, 256 threads ----
+// XCOLS / SCOLS: the lanes of a wavefront run along the columns of the rows' matrix / of
+// the sorted matrix, else along the rows; LDS turns the tile where the two differ.
+constexpr int TILE = 64;
 template <typename T, bool XCOLS, bool SCOLS>
 __global__ __launch_bounds__(256) void k_expert_gather(ExpertPlan p, ExpertMatrix x,
                                                        T *__restrict__ sorted) {
@@ -184,6 +484,7 @@ __global__ __launch_bounds__(256) void k_expert_gather(ExpertPlan p, ExpertMatri
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const T *data = static_cast<const T *>(x.data);
     for (int32_t f0 = blockIdx.y * TILE; f0 < x.cols; f0 += gridDim.y * TILE) {
+#pragma unroll 4
         for (int q = wave; q < TILE; q += 4) {
             const int64_t i = i0 + (XCOLS ? q : lane);
             const int32_t f = f0 + (XCOLS ? lane : q);
@@ -217,23 +518,42 @@ template <typename T, bool XCOLS, bool SCOLS>
 __global__ __launch_bounds__(256) void k_expert_combine(ExpertPlan p, const T *__restrict__ sorted,
                                                         const float *__restrict__ weights,
                                                         ExpertMatrix out) {
+    constexpr int Q = TILE / 4;
     __shared__ float tile[TILE][TILE + 1];
     const int64_t i0 = (int64_t)blockIdx.x * TILE;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     T *data = static_cast<T *>(out.data);
     for (int32_t f0 = blockIdx.y * TILE; f0 < out.cols; f0 += gridDim.y * TILE) {
-        for (int q = wave; q < TILE; q += 4) {
-            const int r = SCOLS ? q : lane, c = SCOLS ? lane : q;
-            if (i0 + r >= p.rows || f0 + c >= out.cols) continue;
-            float sum = 0.0f;
+        if (SCOLS) {
+#pragma unroll 2
+            for (int q = wave; q < TILE; q += 4) {
+                if (i0 + q >= p.rows || f0 + lane >= out.cols) continue;
+                float sum = 0.0f;
+                for (int j = 0; j < p.k; ++j) {
+                    const int64_t a = (i0 + q) * p.k + j;
+                    const Place at = place_of(p, a, out.cols, out.blocked);
+                    if (at.base < 0) continue;
+                    const float v = to_f32(sorted[at.base + (f0 + lane) * at.step]);
+                    sum += weights ? weights[a] * v : v;
+                }
+                tile[q][lane] = sum;
+            }
+        } else if (i0 + lane < p.rows) {
+            float sum[Q];
+#pragma unroll
+            for (int q = 0; q < Q; ++q) sum[q] = 0.0f;
             for (int j = 0; j < p.k; ++j) {
-                const int64_t a = (i0 + r) * p.k + j;
+                const int64_t a = (i0 + lane) * p.k + j;
                 const Place at = place_of(p, a, out.cols, out.blocked);
                 if (at.base < 0) continue;
-                const float v = to_f32(sorted[at.base + (f0 + c) * at.step]);
-                sum += weights ? weights[a] * v : v;
+                const float w = weights ? weights[a] : 1.0f;
+                const T *from = sorted + at.base + (f0 + wave) * at.step;
+#pragma unroll
+                for (int q = 0; q < Q; ++q)
+                    if (f0 + wave + 4 * q < out.cols) sum[q] += w * to_f32(from[4 * q * at.step]);
             }
-            tile[r][c] = sum;
+#pragma unroll
+            for (int q = 0; q < Q; ++q) tile[lane][wave + 4 * q] = sum[q];
         }
         __syncthreads();
         for (int q = wave; q < TILE; q += 4) {
@@ -252,44 +572,70 @@ template <typename T, bool XCOLS, bool SCOLS>
 __global__ __launch_bounds__(256) void k_expert_combine_grad(
     ExpertPlan p, ExpertMatrix dout, const T *__restrict__ sorted,
     const float *__restrict__ weights, T *__restrict__ d_sorted, float *__restrict__ d_weights) {
-    constexpr int ROWS = 16;
-    __shared__ T tile[ROWS][TILE + 2];
-    __shared__ float sums[ROWS][17];
-    const int64_t i0 = (int64_t)blockIdx.x * ROWS;
+    __shared__ T tile[TILE][TILE + 1];
+    __shared__ float sums[TILE][5];
+    const int64_t i0 = (int64_t)blockIdx.x * TILE;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const T *data = static_cast<const T *>(dout.data);
-    // 16 threads a row; along the rows the row is the thread's fast index
-    const int xr = XCOLS ? threadIdx.x >> 4 : threadIdx.x & 15;
-    const int xc = XCOLS ? threadIdx.x & 15 : threadIdx.x >> 4;
-    const int sr = SCOLS ? threadIdx.x >> 4 : threadIdx.x & 15;
-    const int sc = SCOLS ? threadIdx.x & 15 : threadIdx.x >> 4;
     for (int j = 0; j < p.k; ++j) {
-        const int64_t a = (i0 + sr) * p.k + j;
-        const bool row = i0 + sr < p.rows;
-        const Place at = row ? place_of(p, a, dout.cols, dout.blocked) : Place{-1, 0};
-        const float w = row && weights ? weights[a] : 1.0f;
-        float dot = 0.0f;
+        // SCOLS: the sums of rows wave + 4 q over this lane's columns; else of row lane
+        float dot[SCOLS ? TILE / 4 : 1];
+#pragma unroll
+        for (int q = 0; q < (SCOLS ? TILE / 4 : 1); ++q) dot[q] = 0.0f;
+        Place mine{-1, 0};
+        float w = 1.0f;
+        if (!SCOLS && i0 + lane < p.rows) {
+            mine = place_of(p, (i0 + lane) * p.k + j, dout.cols, dout.blocked);
+            if (weights) w = weights[(i0 + lane) * p.k + j];
+        }
         for (int32_t f0 = 0; f0 < dout.cols; f0 += TILE) {
             __syncthreads();
-            for (int c = xc; c < TILE; c += 16)
-                if (i0 + xr < p.rows && f0 + c < dout.cols)
-                    tile[xr][c] = data[(i0 + xr) * dout.row_stride + (f0 + c) * dout.col_stride];
+#pragma unroll 4
+            for (int q = wave; q < TILE; q += 4) {
+                const int r = XCOLS ? q : lane, c = XCOLS ? lane : q;
+                if (i0 + r < p.rows && f0 + c < dout.cols)
+                    tile[r][c] = data[(i0 + r) * dout.row_stride + (f0 + c) * dout.col_stride];
+            }
             __syncthreads();
-            if (at.base >= 0)
-                for (int c = sc; c < TILE && f0 + c < dout.cols; c += 16) {
-                    const float g = to_f32(tile[sr][c]);
-                    const int64_t k = at.base + (f0 + c) * at.step;
-                    dot += g * to_f32(sorted[k]);
+            if constexpr (SCOLS) {
+#pragma unroll
+                for (int q = 0; q < TILE / 4; ++q) {
+                    const int r = wave + 4 * q;
+                    if (i0 + r >= p.rows || f0 + lane >= dout.cols) continue;
+                    const int64_t a = (i0 + r) * p.k + j;
+                    const Place at = place_of(p, a, dout.cols, dout.blocked);
+                    if (at.base < 0) continue;
+                    const float g = to_f32(tile[r][lane]);
+                    const int64_t k = at.base + (f0 + lane) * at.step;
+                    dot[q] += g * to_f32(sorted[k]);
+                    d_sorted[k] = (T)((weights ? weights[a] : 1.0f) * g);
+                }
+            } else if (mine.base >= 0) {
+#pragma unroll 4
+                for (int q = wave; q < TILE; q += 4) {
+                    if (f0 + q >= dout.cols) break;
+                    const float g = to_f32(tile[lane][q]);
+                    const int64_t k = mine.base + (f0 + q) * mine.step;
+                    dot[0] += g * to_f32(sorted[k]);
                     d_sorted[k] = (T)(w * g);
                 }
+            }
         }
-        sums[sr][sc] = dot;
-        __syncthreads();
-        if (threadIdx.x < ROWS && i0 + threadIdx.x < p.rows) {
-            float s = 0.0f;
-            for (int c = 0; c < 16; ++c) s += sums[threadIdx.x][c];
-            d_weights[(i0 + threadIdx.x) * p.k + j] = s;
+        if constexpr (SCOLS) {
+#pragma unroll
+            for (int q = 0; q < TILE / 4; ++q) {
+                float s = dot[q];
+                for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+                if (lane == 0 && i0 + wave + 4 * q < p.rows)
+                    d_weights[(i0 + wave + 4 * q) * p.k + j] = s;
+            }
+        } else {
+            sums[lane][wave] = dot[0];
+            __syncthreads();
+            if (threadIdx.x < TILE && i0 + lane < p.rows)
+                d_weights[(i0 + lane) * p.k + j] =
+                    (sums[lane][0] + sums[lane][1]) + (sums[lane][2] + sums[lane][3]);
         }
-        __syncthreads();
     }
 }
 
@@ -300,16 +646,64 @@ dim3 tile_grid(int64_t rows, int32_t cols) {
                 (uint32_t)std::min<int32_t>((cols + TILE - 1) / TILE, 1024));
 }
 
+// Bytes a lane moves where both matrices lie by rows: 16 where everything is aligned to
+// it, else 4 or an element.
+int lane_bytes(const ExpertMatrix &x, int size, const void *a, const void *b) {
+    const uintptr_t all = reinterpret_cast<uintptr_t>(x.data) | reinterpret_cast<uintptr_t>(a) |
+                          reinterpret_cast<uintptr_t>(b) | (uintptr_t)(x.row_stride * size) |
+                          (uintptr_t)((int64_t)x.cols * size);
+    return all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : size;
+}
+struct RowShape {
+    int bytes, log2_lanes;
+    int32_t chunks;
+    uint32_t groups;
+};
+RowShape row_shape(const ExpertMatrix &x, int64_t rows, int size, const void *a, const void *b) {
+    RowShape r{lane_bytes(x, size, a, b), 0, 0, 0};
+    r.chunks = (int32_t)((int64_t)x.cols * size / r.bytes);
+    while (r.log2_lanes < 6 && (1 << r.log2_lanes) < r.chunks) ++r.log2_lanes;
+    const int64_t per = 256 >> r.log2_lanes;
+    r.groups = (uint32_t)((rows + per - 1) / per);
+    return r;
+}
+// By rows on both sides.
+bool by_rows(const ExpertMatrix &x) { return x.col_stride == 1 && !x.blocked; }
+
+#define BY_BYTES(kernel, ...)                                                                    \
+    do {                                                                                         \
+        if (r.bytes == 16)                                                                       \
+            hipLaunchKernelGGL((kernel<T, 16>), dim3(r.groups), dim3(256), 0, s, __VA_ARGS__);   \
+        else if (r.bytes == 4)                                                                   \
+            hipLaunchKernelGGL((kernel<T, 4>), dim3(r.groups), dim3(256), 0, s, __VA_ARGS__);    \
+        else if constexpr (sizeof(T) == 2)                                                       \
+            hipLaunchKernelGGL((kernel<T, 2>), dim3(r.groups), dim3(256), 0, s, __VA_ARGS__);    \
+    } while (0)
+#define BY_LAYOUT(kernel, grid, ...)                                                             \
+    do {                                                                                         \
+        const bool xc = along_columns(x), sc = !x.blocked;                                       \
+        if (xc && sc) hipLaunchKernelGGL((kernel<T, true, true>), grid, dim3(256), 0, s, __VA_ARGS__);  \
+        else if (xc) hipLaunchKernelGGL((kernel<T, true, false>), grid, dim3(256), 0, s, __VA_ARGS__);  \
+        else if (sc) hipLaunchKernelGGL((kernel<T, false, true>), grid, dim3(256), 0, s, __VA_ARGS__);  \
+        else hipLaunchKernelGGL((kernel<T, false, false>), grid, dim3(256), 0, s, __VA_ARGS__);  \
+    } while (0)
+
 template <typename T>
 hipError_t gather(hipStream_t s, const ExpertPlan &p, const ExpertMatrix &x, void *sorted) {
-    const dim3 g = tile_grid(p.rows, x.cols), b(256);
     T *out = static_cast<T *>(sorted);
-    if (along_columns(x)) {
-        if (x.blocked) hipLaunchKernelGGL((k_expert_gather<T, true, false>), g, b, 0, s, p, x, out);
-        else hipLaunchKernelGGL((k_expert_gather<T, true, true>), g, b, 0, s, p, x, out);
+    if (by_rows(x)) {
+        const RowShape r = row_shape(x, p.rows, sizeof(T), sorted, nullptr);
+        BY_BYTES(k_expert_gather_rows, p, x, r.chunks, r.log2_lanes, out);
+    } else if (x.blocked && !along_columns(x) && p.experts <= RUN_EXPERTS && p.k <= 16) {
+        const int32_t rows = RUN / p.k;
+        const uint32_t runs = (uint32_t)((p.rows + rows - 1) / rows);
+        const uint32_t cols = (uint32_t)((x.cols + RUN_COLS - 1) / RUN_COLS);
+        // few runs: their columns go to several workgroups
+        const uint32_t parts = std::max(1u, std::min({cols, 1024 / std::max(1u, runs), 65535u}));
+        hipLaunchKernelGGL((k_expert_gather_runs<T>), dim3(runs, parts), dim3(256), 0, s, p, x, rows,
+                           out);
     } else {
-        if (x.blocked) hipLaunchKernelGGL((k_expert_gather<T, false, false>), g, b, 0, s, p, x, out);
-        else hipLaunchKernelGGL((k_expert_gather<T, false, true>), g, b, 0, s, p, x, out);
+        BY_LAYOUT(k_expert_gather, tile_grid(p.rows, x.cols), p, x, out);
     }
     return hipGetLastError();
 }
@@ -317,14 +711,12 @@ hipError_t gather(hipStream_t s, const ExpertPlan &p, const ExpertMatrix &x, voi
 template <typename T>
 hipError_t combine(hipStream_t s, const ExpertPlan &p, const void *sorted, const float *w,
                    const ExpertMatrix &x) {
-    const dim3 g = tile_grid(p.rows, x.cols), b(256);
     const T *y = static_cast<const T *>(sorted);
-    if (along_columns(x)) {
-        if (x.blocked) hipLaunchKernelGGL((k_expert_combine<T, true, false>), g, b, 0, s, p, y, w, x);
-        else hipLaunchKernelGGL((k_expert_combine<T, true, true>), g, b, 0, s, p, y, w, x);
+    if (by_rows(x)) {
+        const RowShape r = row_shape(x, p.rows, sizeof(T), sorted, nullptr);
+        BY_BYTES(k_expert_combine_rows, p, y, w, x, r.chunks, r.log2_lanes);
     } else {
-        if (x.blocked) hipLaunchKernelGGL((k_expert_combine<T, false, false>), g, b, 0, s, p, y, w, x);
-        else hipLaunchKernelGGL((k_expert_combine<T, false, true>), g, b, 0, s, p, y, w, x);
+        BY_LAYOUT(k_expert_combine, tile_grid(p.rows, x.cols), p, y, w, x);
     }
     return hipGetLastError();
 }
@@ -332,26 +724,19 @@ hipError_t combine(hipStream_t s, const ExpertPlan &p, const void *sorted, const
 template <typename T>
 hipError_t combine_grad(hipStream_t s, const ExpertPlan &p, const ExpertMatrix &x,
                         const void *sorted, const float *w, void *d_sorted, float *d_weights) {
-    const dim3 g((uint32_t)((p.rows + 15) / 16)), b(256);
     const T *y = static_cast<const T *>(sorted);
     T *dy = static_cast<T *>(d_sorted);
-    if (along_columns(x)) {
-        if (x.blocked)
-            hipLaunchKernelGGL((k_expert_combine_grad<T, true, false>), g, b, 0, s, p, x, y, w, dy,
-                               d_weights);
-        else
-            hipLaunchKernelGGL((k_expert_combine_grad<T, true, true>), g, b, 0, s, p, x, y, w, dy,
-                               d_weights);
+    if (by_rows(x)) {
+        const RowShape r = row_shape(x, p.rows, sizeof(T), sorted, d_sorted);
+        BY_BYTES(k_expert_combine_grad_rows, p, x, y, w, dy, d_weights, r.chunks, r.log2_lanes);
     } else {
-        if (x.blocked)
-            hipLaunchKernelGGL((k_expert_combine_grad<T, false, false>), g, b, 0, s, p, x, y, w,
-                               dy, d_weights);
-        else
-            hipLaunchKernelGGL((k_expert_combine_grad<T, false, true>), g, b, 0, s, p, x, y, w, dy,
-                               d_weights);
+        BY_LAYOUT(k_expert_combine_grad, dim3((uint32_t)((p.rows + TILE - 1) / TILE)), p, x, y, w,
+                  dy, d_weights);
     }
     return hipGetLastError();
 }
+#undef BY_BYTES
+#undef BY_LAYOUT
 
 }  // namespace
 
@@ -367,15 +752,25 @@ hipError_t launch_expert_sort(hipStream_t s, const ExpertPlan &p, int num_cus, c
     uint32_t *total = table + (size_t)p.experts * sh.units;
     int bits = 0;
     while (bits < 31 && (1 << bits) < p.experts) ++bits;
+    for (const void *f : {reinterpret_cast<const void *>(k_expert_count),
+                          reinterpret_cast<const void *>(k_expert_place),
+                          reinterpret_cast<const void *>(k_expert_sort_small)}) {
+        const hipError_t e = allow_all_lds(f);
+        if (e != hipSuccess) return e;
+    }
+    if (slots <= SMALL_SLOTS && p.experts <= SMALL_EXPERTS) {
+        const int64_t per = ((slots + SMALL_WAVES - 1) / SMALL_WAVES + 63) / 64 * 64;
+        hipLaunchKernelGGL(k_expert_sort_small, dim3(1), dim3(64 * SMALL_WAVES),
+                           (size_t)SMALL_WAVES * (p.experts + 1) * sizeof(uint32_t), s, p.expert,
+                           slots, p.experts, bits, per, p.offsets, p.source, p.slot);
+        return hipGetLastError();
+    }
     const dim3 g((uint32_t)((sh.units + SORT_WAVES - 1) / SORT_WAVES)), b(64 * SORT_WAVES);
     const size_t lds = (size_t)SORT_WAVES * p.experts * sizeof(uint32_t);
-    hipError_t e = allow_all_lds(reinterpret_cast<const void *>(k_expert_count));
-    if (e == hipSuccess) e = allow_all_lds(reinterpret_cast<const void *>(k_expert_place));
-    if (e != hipSuccess) return e;
     hipLaunchKernelGGL(k_expert_count, g, b, lds, s, p.expert, slots, p.experts, sh.per, sh.units,
                        table);
-    hipLaunchKernelGGL(k_expert_scan, dim3((uint32_t)((p.experts + 3) / 4)), dim3(256), 0, s,
-                       table, p.experts, sh.units, total);
+    hipLaunchKernelGGL(k_expert_scan, dim3((uint32_t)p.experts), dim3(SCAN), 0, s, table, sh.units,
+                       total);
     hipLaunchKernelGGL(k_expert_offsets, dim3(1), dim3(1024), 0, s, total, p.experts, p.offsets);
     hipLaunchKernelGGL(k_expert_place, g, b, lds, s, p.expert, slots, p.experts, bits, sh.per,
                        sh.units, table, p.offsets, p.source, p.slot);
