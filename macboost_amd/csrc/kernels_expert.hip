@@ -69,11 +69,13 @@ __device__ __forceinline__ void count_keys(const int32_t *__restrict__ expert, i
     });
 }
 
-// next[e]: the slot that the wavefront's next assignment to e gets.
+// next[e]: the slot that the wavefront's next assignment to e gets.  Lanes with nothing to
+// write write to trash: with stores under a branch the loads ahead would wait for all
+// of them to be done.
 __device__ __forceinline__ void place_keys(const int32_t *__restrict__ expert, int64_t a, int64_t b,
                                            int32_t experts, int32_t key_bits, uint32_t *next,
-                                           int64_t kept_all, int32_t *__restrict__ source,
-                                           int32_t *__restrict__ slot) {
+                                           int32_t *__restrict__ source,
+                                           int32_t *__restrict__ slot, int32_t *trash) {
     const int lane = threadIdx.x & 63;
     each_key(expert, a, b, [&](int64_t i0, uint32_t e) {
         const int64_t i = i0 + lane;
@@ -89,12 +91,14 @@ __device__ __forceinline__ void place_keys(const int32_t *__restrict__ expert, i
         __builtin_amdgcn_wave_barrier();
         if (kept && rank == 0) next[e] = at + (uint32_t)__popcll(same);
         __builtin_amdgcn_wave_barrier();
-        if (kept) source[at] = (int32_t)i;
-        if (i < b) {
-            slot[i] = kept ? (int32_t)at : -1;
-            if (i >= kept_all) source[i] = -1;  // behind the last slot taken
-        }
+        *(kept ? source + at : trash) = (int32_t)i;
+        *(i < b ? slot + i : trash) = kept ? (int32_t)at : -1;
     });
+}
+// source of [a, b) behind the last slot taken.
+__device__ __forceinline__ void no_source(int64_t a, int64_t b, int64_t kept,
+                                          int32_t *__restrict__ source) {
+    for (int64_t i = max(a, kept) + (threadIdx.x & 63); i < b; i += 64) source[i] = -1;
 }
 
 // The sum of v over the threads before, and over all, of a workgroup of W wavefronts.
@@ -177,7 +181,7 @@ __global__ __launch_bounds__(64 * SORT_WAVES) void k_expert_place(
     const int32_t *__restrict__ expert, int64_t slots, int32_t experts, int32_t key_bits,
     int64_t per, int32_t units, const uint32_t *__restrict__ table,
     const int32_t *__restrict__ offsets, int32_t *__restrict__ source,
-    int32_t *__restrict__ slot) {
+    int32_t *__restrict__ slot, int32_t *trash) {
     extern __shared__ uint32_t lds[];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     uint32_t *next = lds + (size_t)wave * experts;
@@ -185,8 +189,9 @@ __global__ __launch_bounds__(64 * SORT_WAVES) void k_expert_place(
     if (u >= units) return;                     // no barrier below
     for (int e = lane; e < experts; e += 64)
         next[e] = (uint32_t)offsets[e] + table[(int64_t)e * units + u];
-    place_keys(expert, u * per, min(slots, (u + 1) * per), experts, key_bits, next,
-               offsets[experts], source, slot);
+    const int64_t a = u * per, b = min(slots, a + per);
+    place_keys(expert, a, b, experts, key_bits, next, source, slot, trash);
+    no_source(a, b, offsets[experts], source);
 }
 
 // Few assignments: the whole sort by one workgroup (1000 to 4 experts 13 us less than by
@@ -197,7 +202,7 @@ constexpr int32_t SMALL_EXPERTS = 2048;
 __global__ __launch_bounds__(64 * SMALL_WAVES) void k_expert_sort_small(
     const int32_t *__restrict__ expert, int64_t slots, int32_t experts, int32_t key_bits,
     int64_t per, int32_t *__restrict__ offsets, int32_t *__restrict__ source,
-    int32_t *__restrict__ slot) {
+    int32_t *__restrict__ slot, int32_t *trash) {
     extern __shared__ uint32_t lds[];
     uint32_t *wave_sum = lds, *count = lds + SMALL_WAVES;        // [wave][expert]
     const int wave = threadIdx.x >> 6;
@@ -225,7 +230,8 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void k_expert_sort_small(
     }
     if (threadIdx.x == 0) offsets[experts] = (int32_t)before;
     __syncthreads();
-    place_keys(expert, a, b, experts, key_bits, count + wave * experts, before, source, slot);
+    place_keys(expert, a, b, experts, key_bits, count + wave * experts, source, slot, trash);
+    no_source(a, b, before, source);
 }
 
 struct SortShape {
@@ -400,7 +406,7 @@ __global__ __launch_bounds__(256) void k_expert_combine_grad_rows(
 // An expert's assignments of consecutive rows have consecutive slots: with the run's values
 // of a column ordered by (expert, slot) in LDS, both sides of the copy are runs of
 // addresses.
-constexpr int RUN = 1024, RUN_COLS = 8, RUN_EXPERTS = 512;
+constexpr int RUN = 1024, RUN_COLS = 4, RUN_EXPERTS = 512;
 template <typename T>
 __global__ __launch_bounds__(256) void k_expert_gather_runs(ExpertPlan p, ExpertMatrix x,
                                                             int32_t run_rows,
@@ -448,18 +454,34 @@ __global__ __launch_bounds__(256) void k_expert_gather_runs(ExpertPlan p, Expert
         base[at[q]] = (int64_t)o * x.cols + (slot[q] - o);
         step[at[q]] = p.offsets[e + 1] - o;
     }
-    const T *data = static_cast<const T *>(x.data) + i0 * x.row_stride;
-    for (int32_t f0 = blockIdx.y * RUN_COLS; f0 < x.cols; f0 += gridDim.y * RUN_COLS) {
-        const int cols = min(RUN_COLS, x.cols - f0);
+    const T *from[RUN / 256];
+#pragma unroll
+    for (int q = 0; q < RUN / 256; ++q)
+        from[q] = static_cast<const T *>(x.data) + (i0 + (at[q] >= 0 ? row[q] : 0)) * x.row_stride;
+    T v[RUN / 256][RUN_COLS];
+    // the next columns are asked for before the last ones are stored: a load waits for
+    // every access before it
+    const auto load = [&](int32_t f0) {
+#pragma unroll
+        for (int c = 0; c < RUN_COLS; ++c) {
+            const int64_t f = (int64_t)min(f0 + c, x.cols - 1) * x.col_stride;
+#pragma unroll
+            for (int q = 0; q < RUN / 256; ++q) v[q][c] = from[q][f];
+        }
+    };
+    int32_t f0 = blockIdx.y * RUN_COLS;
+    if (f0 < x.cols) load(f0);
+    for (; f0 < x.cols; f0 += gridDim.y * RUN_COLS) {
         __syncthreads();                             // base and step, the last columns' reads
 #pragma unroll
         for (int q = 0; q < RUN / 256; ++q)
             if (at[q] >= 0)
 #pragma unroll
-                for (int c = 0; c < RUN_COLS; ++c)
-                    if (c < cols)
-                        tile[c][at[q]] = data[row[q] * x.row_stride + (f0 + c) * x.col_stride];
+                for (int c = 0; c < RUN_COLS; ++c) tile[c][at[q]] = v[q][c];
         __syncthreads();
+        const int32_t next = f0 + gridDim.y * RUN_COLS;
+        if (next < x.cols) load(next);
+        const int cols = min(RUN_COLS, x.cols - f0);
 #pragma unroll
         for (int q = 0; q < RUN / 256; ++q) {
             const int l = threadIdx.x + 256 * q;
@@ -742,7 +764,7 @@ hipError_t combine_grad(hipStream_t s, const ExpertPlan &p, const ExpertMatrix &
 
 size_t expert_scratch(const ExpertPlan &p, int num_cus) {
     const SortShape sh = sort_shape(p, num_cus);
-    return ((size_t)p.experts * sh.units + p.experts) * sizeof(uint32_t);
+    return ((size_t)p.experts * sh.units + p.experts + 1) * sizeof(uint32_t);
 }
 
 hipError_t launch_expert_sort(hipStream_t s, const ExpertPlan &p, int num_cus, char *scratch) {
@@ -750,6 +772,7 @@ hipError_t launch_expert_sort(hipStream_t s, const ExpertPlan &p, int num_cus, c
     const int64_t slots = p.rows * p.k;
     uint32_t *table = reinterpret_cast<uint32_t *>(scratch);
     uint32_t *total = table + (size_t)p.experts * sh.units;
+    int32_t *trash = reinterpret_cast<int32_t *>(total + p.experts);
     int bits = 0;
     while (bits < 31 && (1 << bits) < p.experts) ++bits;
     for (const void *f : {reinterpret_cast<const void *>(k_expert_count),
@@ -762,7 +785,7 @@ hipError_t launch_expert_sort(hipStream_t s, const ExpertPlan &p, int num_cus, c
         const int64_t per = ((slots + SMALL_WAVES - 1) / SMALL_WAVES + 63) / 64 * 64;
         hipLaunchKernelGGL(k_expert_sort_small, dim3(1), dim3(64 * SMALL_WAVES),
                            (size_t)SMALL_WAVES * (p.experts + 1) * sizeof(uint32_t), s, p.expert,
-                           slots, p.experts, bits, per, p.offsets, p.source, p.slot);
+                           slots, p.experts, bits, per, p.offsets, p.source, p.slot, trash);
         return hipGetLastError();
     }
     const dim3 g((uint32_t)((sh.units + SORT_WAVES - 1) / SORT_WAVES)), b(64 * SORT_WAVES);
@@ -773,7 +796,7 @@ hipError_t launch_expert_sort(hipStream_t s, const ExpertPlan &p, int num_cus, c
                        total);
     hipLaunchKernelGGL(k_expert_offsets, dim3(1), dim3(1024), 0, s, total, p.experts, p.offsets);
     hipLaunchKernelGGL(k_expert_place, g, b, lds, s, p.expert, slots, p.experts, bits, sh.per,
-                       sh.units, table, p.offsets, p.source, p.slot);
+                       sh.units, table, p.offsets, p.source, p.slot, trash);
     return hipGetLastError();
 }
 
