@@ -300,8 +300,9 @@ int mbk_treeshap(mbk_context *ctx, const int32_t *feature, const float *threshol
  * whose bias is -INFINITY is not offered: what its w holds reaches nothing, its dw
  * and dbias are 0.  With no class offered every lse is -INFINITY and every row is out.
  * Other h, w and bias must be finite for finite results.  Sums are f32; bf16 operands
- * are multiplied exactly, with g rounded to bf16 for dh, dw and dbias, f32 operands to 22
- * bits.  The results do not depend on the call, bit for bit.
+ * are multiplied as they are and g with 11 bits, f32 operands and g with 22 bits, where
+ * elements below 2^-38 of the largest of their row (h) or of all (w) count as 0.  The
+ * results do not depend on the call, bit for bit.
  * To boost output j with them: mbk_quantize with objective 0, preds = dh's column j
  * and labels of 0. */
 enum { MBK_F32 = 0, MBK_BF16 = 1 };

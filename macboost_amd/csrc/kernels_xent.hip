@@ -10,16 +10,17 @@
 // its G, and two products turn that into dh and dW before the next piece overwrites
 // it.
 //
-// Operands.  The matrix instructions take 16-bit operands and add in f32.  bf16
-// inputs go in as they are, and G is rounded to bf16 (half a step, 2^-8 of each
-// element at most, random in sign: what the outputs' own rounding to bf16 costs).  f32
-// inputs go in as two f16 terms, x 2^s = hi + lo, which hold 22 bits of it, and
-// three products hi hi + hi lo + lo hi: what is dropped, lo lo and the bits behind
-// lo, is at most 2^-21 of an element's product and random in sign, the size of
-// what an f32 sum over the same length rounds away.  (f32 operands have an
-// instruction of 1/16 of the bf16 rate; three of these cost 3/16.)  s is a power of
-// two that puts the largest element of h's row, or of all of W, below 2^14, so that
-// elements down to 2^-38 of it keep a step of their own.
+// Operands.  The matrix instructions take 16-bit operands and add in f32.  All operands go
+// in as f16 terms of x 2^s, s a power of two that puts the largest element of h's row, or
+// of all of W, below 2^14, so that elements down to 2^-38 of it keep a step of their own.
+//   bf16 inputs: one term, which holds their 8 bits as they are (exactly, down to 2^-31 of the
+//   largest).  G is rounded to one f16 term, too, 11 bits: as bf16 terms it would add as
+//   much error again to dh and dW as their own rounding to bf16 (measured 2.8e-3 in place
+//   of 1.7e-3 of their norm), at the same rate.
+//   f32 inputs: two terms, hi + lo, 22 bits, and three products hi hi + hi lo + lo hi: what is
+//   dropped, lo lo and the bits behind lo, is at most 2^-21 of an element's product and
+//   random in sign, the size of what an f32 sum over the same length rounds away.  (f32
+//   operands have an instruction of 1/16 of the rate; three of these cost 3/16.)
 //
 // Classes not offered (bias -inf) are packed as zeros, and so are rows that are out
 // (label outside [0, V), weight 0, or no class offered) and hold NaN, infinities or values
@@ -35,8 +36,10 @@ namespace mbk {
 
 namespace {
 
+typedef __attribute__((ext_vector_type(8))) unsigned short u16x8;
+
 constexpr int LD_PAD = 128;              // operands' rows are padded to it
-constexpr float G_SCALE = 32768.0f;      // f32: |G / w| <= 1 as f16 terms
+constexpr float G_SCALE = 32768.0f;      // |G / w| <= 1 as f16 terms
 
 __global__ void k_xent_init(XentCtl *ctl) {
     ctl->w_max = ctl->hg_max = ctl->open = 0;
@@ -46,43 +49,90 @@ template <typename T> __device__ __forceinline__ float load_f32(const void *p, i
     return (float)static_cast<const T *>(p)[i];
 }
 
+// Eight elements of a row from f on, zeros behind its d: 16 bytes at a time where the rows
+// allow.
+template <typename T>
+__device__ __forceinline__ void load8(const void *p, int64_t row, int f, int d, bool aligned,
+                                      float (&x)[8]) {
+    const T *from = static_cast<const T *>(p) + row + f;
+    if (aligned && f + 8 <= d) {
+        u32x4 v[sizeof(T) / 2];
+#pragma unroll
+        for (int q = 0; q < (int)sizeof(T) / 2; ++q) v[q] = reinterpret_cast<const u32x4 *>(from)[q];
+        T y[8];
+        __builtin_memcpy(y, v, sizeof y);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = (float)y[e];
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = f + e < d ? (float)from[e] : 0.0f;
+    }
+}
+template <typename T> __device__ __forceinline__ bool aligned16(const void *p, int64_t stride) {
+    return ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)(stride * sizeof(T))) & 15) == 0;
+}
+// Eight elements times 2^s into the planes.
+template <typename T>
+__device__ __forceinline__ void pack8(const float (&x)[8], int s, u16 *to, int64_t plane) {
+    u16x8 hi, lo;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        u16 a, b;
+        split_f16(ldexpf(x[e], s), a, b);
+        hi[e] = a;
+        lo[e] = b;
+    }
+    *reinterpret_cast<u16x8 *>(to) = hi;
+    if (sizeof(T) == 4) *reinterpret_cast<u16x8 *>(to + plane) = lo;
+}
+// The workgroup's largest goes to *max: few atomics on one word.
+__device__ __forceinline__ void raise_by_block(uint32_t *max, uint32_t v) {
+    __shared__ uint32_t most[4];
+    v = wave_max(v);
+    if ((threadIdx.x & 63) == 0) most[threadIdx.x >> 6] = v;
+    __syncthreads();
+    if (threadIdx.x == 0) raise(max, ::max(::max(most[0], most[1]), ::max(most[2], most[3])));
+}
+
+// The kernels that prepare take a wavefront a row, over the rows in turns.
 // Classes: the padded bias, whether any is offered, the largest |W|.
 template <typename T>
 __global__ __launch_bounds__(256) void k_xent_classes(XentPack k, const void *w, int64_t stride,
                                                       const float *__restrict__ bias) {
     const int lane = threadIdx.x & 63;
-    const int64_t v = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (v >= k.v_pad) return;
-    const float b = v < k.v ? (bias ? bias[v] : 0.0f) : -INFINITY;
-    const bool open = b != -INFINITY;
-    if (lane == 0) {
-        k.bias[v] = b * LOG2E;
-        if (open && !k.ctl->open) k.ctl->open = 1u;
-    }
-    if (sizeof(T) == 2 || !open) return;
+    const bool aligned = aligned16<T>(w, stride);
     uint32_t m = 0;
-    for (int32_t f = lane; f < k.d; f += 64) m = max(m, finite_bits(load_f32<T>(w, v * stride + f)));
-    m = wave_max(m);
-    if (lane == 0) raise(&k.ctl->w_max, m);
+    bool any = false;
+    for (int64_t v = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); v < k.v_pad;
+         v += (int64_t)gridDim.x * 4) {
+        const float b = v < k.v ? (bias ? bias[v] : 0.0f) : -INFINITY;
+        const bool open = b != -INFINITY;
+        any = any || open;
+        if (lane == 0) k.bias[v] = b * LOG2E;
+        if (!open) continue;
+        for (int32_t f = lane * 8; f < k.d; f += 512) {
+            float x[8];
+            load8<T>(w, v * stride, f, k.d, aligned, x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) m = max(m, finite_bits(x[e]));
+        }
+    }
+    if (any && !k.ctl->open) k.ctl->open = 1u;
+    raise_by_block(&k.ctl->w_max, m);
 }
 
 template <typename T>
 __global__ __launch_bounds__(256) void k_xent_pack_w(XentPack k, const void *w, int64_t stride) {
     const int lane = threadIdx.x & 63;
-    const int64_t v = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (v >= k.v_pad) return;
-    const bool open = k.bias[v] != -INFINITY;
-    const int s = sizeof(T) == 4 ? scale_exp(k.ctl->w_max) : 0;
-    u16 *row = k.w + v * k.ld;
-    for (int32_t f = lane; f < k.ld; f += 64) {
-        const bool in = open && f < k.d;
-        if (sizeof(T) == 2) {
-            row[f] = in ? static_cast<const u16 *>(w)[v * stride + f] : 0;
-        } else {
-            u16 hi, lo;
-            split_f16(in ? ldexpf(load_f32<T>(w, v * stride + f), s) : 0.0f, hi, lo);
-            row[f] = hi;
-            row[k.v_pad * k.ld + f] = lo;
+    const bool aligned = aligned16<T>(w, stride);
+    const int s = scale_exp(k.ctl->w_max);
+    for (int64_t v = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); v < k.v_pad;
+         v += (int64_t)gridDim.x * 4) {
+        const int32_t d = k.bias[v] != -INFINITY ? k.d : 0;
+        for (int32_t f = lane * 8; f < k.ld; f += 512) {
+            float x[8];
+            load8<T>(w, v * stride, f, d, aligned, x);
+            pack8<T>(x, s, k.w + v * k.ld + f, k.v_pad * k.ld);
         }
     }
 }
@@ -94,68 +144,68 @@ __global__ __launch_bounds__(256) void k_xent_rows(XentPack k, const void *h, in
                                                    const int32_t *__restrict__ labels,
                                                    const float *__restrict__ weights) {
     const int lane = threadIdx.x & 63;
-    const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (i >= k.n_pad) return;
-    int32_t y = i < k.n ? labels[i] : -1;
-    float wt = i < k.n ? (weights ? weights[i] : 1.0f) : 0.0f;
-    const bool out = y < 0 || y >= k.v || wt == 0.0f || !k.ctl->open;
-    int s = 0;
-    bool zeros = i >= k.n;
-    if (out) {
-        y = -1;
-        wt = 0.0f;
-    }
-    if ((out || sizeof(T) == 4) && i < k.n) {
+    const bool aligned = aligned16<T>(h, stride), any = k.ctl->open;
+    const int sw = scale_exp(k.ctl->w_max);
+    uint32_t hg = 0;
+    for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < k.n_pad;
+         i += (int64_t)gridDim.x * 4) {
+        int32_t y = i < k.n ? labels[i] : -1, d = i < k.n ? k.d : 0;
+        float wt = i < k.n ? (weights ? weights[i] : 1.0f) : 0.0f;
+        const bool out = y < 0 || y >= k.v || wt == 0.0f || !any;
         uint32_t m = 0, most = 0;
-        for (int32_t f = lane; f < k.d; f += 64) {
-            const float x = load_f32<T>(h, i * stride + f);
-            m = max(m, finite_bits(x));
-            most = max(most, __float_as_uint(fabsf(x)));
+        for (int32_t f = lane * 8; f < d; f += 512) {
+            float x[8];
+            load8<T>(h, i * stride, f, d, aligned, x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                m = max(m, finite_bits(x[e]));
+                most = max(most, __float_as_uint(fabsf(x[e])));
+            }
         }
         m = wave_max(m);
-        if (out && wave_max(most) >= XENT_HUGE) {
-            y = -2;
-            m = 0;
-            zeros = true;
+        if (out) {
+            y = -1;
+            wt = 0.0f;
+            if (wave_max(most) >= XENT_HUGE) {
+                y = -2;
+                m = 0;
+                d = 0;
+            }
         }
-        if (sizeof(T) == 4) s = scale_exp(m);
-        if (sizeof(T) == 4 && lane == 0 && wt != 0.0f)
-            raise(&k.ctl->hg_max, finite_bits(wt * __uint_as_float(m)));
-    }
-    if (lane == 0) {
-        if (sizeof(T) == 4) k.row_scale[i] = ldexpf(LOG2E, -(s + scale_exp(k.ctl->w_max)));
-        k.label[i] = y;
-        k.weight[i] = wt;
-    }
-    u16 *row = k.h + i * k.ld;
-    for (int32_t f = lane; f < k.ld; f += 64) {
-        const bool in = !zeros && f < k.d;
-        if (sizeof(T) == 2) {
-            row[f] = in ? static_cast<const u16 *>(h)[i * stride + f] : 0;
-        } else {
-            u16 hi, lo;
-            split_f16(in ? ldexpf(load_f32<T>(h, i * stride + f), s) : 0.0f, hi, lo);
-            row[f] = hi;
-            row[k.n_pad * k.ld + f] = lo;
+        const int s = scale_exp(m);
+        if (wt != 0.0f) hg = max(hg, finite_bits(wt * __uint_as_float(m)));
+        if (lane == 0) {
+            k.row_scale[i] = ldexpf(LOG2E, -(s + sw));
+            k.label[i] = y;
+            k.weight[i] = wt;
+        }
+        for (int32_t f = lane * 8; f < k.ld; f += 512) {
+            float x[8];
+            load8<T>(h, i * stride, f, d, aligned, x);
+            pack8<T>(x, s, k.h + i * k.ld + f, k.n_pad * k.ld);
         }
     }
+    raise_by_block(&k.ctl->hg_max, hg);
 }
 
-// f32: h as dW's product takes it, times the row's weight and with one scale for all
-// rows (they are summed over).
-__global__ __launch_bounds__(256) void k_xent_pack_hg(XentPack k, const float *h, int64_t stride) {
+// h as dW's product takes it, times the row's weight and with one scale for all rows
+// (they are summed over).
+template <typename T>
+__global__ __launch_bounds__(256) void k_xent_pack_hg(XentPack k, const void *h, int64_t stride) {
     const int lane = threadIdx.x & 63;
-    const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (i >= k.n_pad) return;
-    const bool live = k.label[i] >= 0;
-    const float wt = k.weight[i];
+    const bool aligned = aligned16<T>(h, stride);
     const int s = scale_exp(k.ctl->hg_max);
-    u16 *row = k.hg + i * k.ld;
-    for (int32_t f = lane; f < k.ld; f += 64) {
-        u16 hi, lo;
-        split_f16(live && f < k.d ? ldexpf(wt * h[i * stride + f], s) : 0.0f, hi, lo);
-        row[f] = hi;
-        row[k.n_pad * k.ld + f] = lo;
+    for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < k.n_pad;
+         i += (int64_t)gridDim.x * 4) {
+        const int32_t d = k.label[i] >= 0 ? k.d : 0;
+        const float wt = k.weight[i];
+        for (int32_t f = lane * 8; f < k.ld; f += 512) {
+            float x[8];
+            load8<T>(h, i * stride, f, d, aligned, x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] *= wt;
+            pack8<T>(x, s, k.hg + i * k.ld + f, k.n_pad * k.ld);
+        }
     }
 }
 
@@ -163,11 +213,11 @@ __global__ __launch_bounds__(256) void k_xent_pack_hg(XentPack k, const float *h
 // C[m][n] = sum_k A[m][k] B[n][k].  An operand lies with k contiguous (KC: element (m, k)
 // at m * ld + k) or with m contiguous (k * ld + m); the second kind is turned by the LDS
 // reads (ds_read_tr16_b64: 16 lanes read 4 rows of 16 elements, lane i gets column i).
-// P == 1: bf16; P == 2: f16 in two planes, three products.
+// P planes of f16 terms.
 //
 // A workgroup has a tile of 256 x 256 in eight wavefronts (Wide: 128 x 64 each) or of
 // 128 x 128 in four (Narrow: 64 x 64 each).  Steps of k are copied into LDS directly, one
-// step ahead, 64 of bf16 or 32 of the planes.
+// step ahead, 64 of one plane or 32 of two.
 template <int WM_, int WN_, int MT_, int NT_> struct Tiling {
     static constexpr int WM = WM_, WN = WN_, MT = MT_, NT = NT_;     // wavefronts, blocks of 32
     static constexpr int WAVES = WM * WN, T = WM * MT * 32;
@@ -377,7 +427,7 @@ __global__ __launch_bounds__(C::WAVES * 64, 2) void k_xent_stats(XentPack k, int
         row[y] = i0 + wave % C::WN * C::NT * 32 + y * 32 + (lane & 31);
         m[y] = -INFINITY;
         s[y] = 0.0f;
-        sc[y] = P == 2 ? k.row_scale[row[y]] : LOG2E;
+        sc[y] = k.row_scale[row[y]];
     }
     Acc<C> acc;
     const auto next = [&](int64_t i, int64_t &m0, int64_t &n0) {
@@ -460,17 +510,18 @@ __global__ __launch_bounds__(256) void k_xent_join(XentPack k, XentCall c, int32
         top = now;
         dot += __shfl_xor(dot, o, 64);
     }
-    const float l2 = (top == -INFINITY ? 0.0f : top) + log2f(sum);
     if (lane != 0) return;
-    lse2[i] = l2;
+    const LogSum l = log_sum(top, sum);
+    lse2[i] = l.base2;
     if (i >= k.n) return;
-    const float lse = y == -2 ? NAN : l2 * LN2, z = open ? dot + (c.bias ? c.bias[y] : 0.0f) : -INFINITY;
+    const float lse = y == -2 ? NAN : l.natural, z = open ? dot + (c.bias ? c.bias[y] : 0.0f) : -INFINITY;
     c.lse[i] = lse;
     c.loss[i] = y < 0 ? 0.0f : k.weight[i] * (lse - z);
 }
 
 // ---- pass 2: G of a piece ------------------------------------------------------------
-// g[v - v0][i - r0], rows of rows_pad; f32: G / w in two f16 terms times 2^15.
+// g[v - v0][i - r0], rows of rows_pad: G / w times 2^15.  part_db[part of the rows][v]: sums
+// of G itself.
 // A workgroup has a tile of rows and every splits-th tile of classes.
 template <int P, class C>
 __global__ __launch_bounds__(C::WAVES * 64, 2) void k_xent_g(XentPack k, int64_t v0, int64_t r0,
@@ -478,7 +529,8 @@ __global__ __launch_bounds__(C::WAVES * 64, 2) void k_xent_g(XentPack k, int64_t
                                                              int32_t row_tiles,
                                                              int32_t class_tiles, int32_t splits,
                                                              const float *__restrict__ lse2,
-                                                             u16 *__restrict__ g) {
+                                                             u16 *__restrict__ g,
+                                                             float *__restrict__ part_db) {
     extern __shared__ char lds[];
     const int lane = threadIdx.x & 63, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -492,10 +544,10 @@ __global__ __launch_bounds__(C::WAVES * 64, 2) void k_xent_g(XentPack k, int64_t
 #pragma unroll
     for (int y = 0; y < C::NT; ++y) {
         const int64_t i = iw + y * 32 + (lane & 31);
-        sc[y] = P == 2 ? k.row_scale[i] : LOG2E;
+        sc[y] = k.row_scale[i];
         label[y] = k.label[i];
         l[y] = label[y] < 0 ? INFINITY : lse2[i];        // a row that is out: 2^-inf
-        wt[y] = P == 2 ? G_SCALE : k.weight[i];
+        wt[y] = k.weight[i];
     }
     const uint32_t mine = half * 4 * (uint32_t)rows_pad + (lane & 31);
     Acc<C> acc;
@@ -506,10 +558,11 @@ __global__ __launch_bounds__(C::WAVES * 64, 2) void k_xent_g(XentPack k, int64_t
     const auto done = [&](int64_t i) {
         const int64_t c0 = v0 + (split + i * splits) * C::T + wave / C::WN * C::MT * 32;
 #pragma unroll
-        for (int x = 0; x < C::MT; ++x)
+        for (int x = 0; x < C::MT; ++x) {
+            const int64_t c = c0 + x * 32;
+            float db[16];
 #pragma unroll
             for (int y = 0; y < C::NT; ++y) {
-                const int64_t c = c0 + x * 32;
                 const int64_t at = label[y] - c - half * 4;      // 8 q + e if the label is here
                 const bool hot = __any(at >= 0 && at < 32);
                 u16 *to = g + (c - v0) * rows_pad + (iw - r0) + y * 32;
@@ -522,19 +575,35 @@ __global__ __launch_bounds__(C::WAVES * 64, 2) void k_xent_g(XentPack k, int64_t
                         float p = __builtin_amdgcn_exp2f(
                             __builtin_fmaf(acc[x][y][q * 4 + e], sc[y], b2[e] - l[y]));
                         if (hot && at == q * 8 + e) p -= 1.0f;
-                        p *= wt[y];
-                        if constexpr (P == 1) {
-                            to[mine] = bits_of((__bf16)p);
-                        } else {
-                            u16 hi, lo;
-                            split_f16(p, hi, lo);
-                            to[mine] = hi;
-                            to[plane + mine] = lo;
-                        }
+                        db[q * 4 + e] = y == 0 ? p * wt[y]
+                                               : __builtin_fmaf(p, wt[y], db[q * 4 + e]);
+                        u16 hi, lo;
+                        split_f16(p * G_SCALE, hi, lo);
+                        to[mine] = hi;
+                        if constexpr (P == 2) to[plane + mine] = lo;
                         to += e < 3 ? rows_pad : 5 * rows_pad;
                     }
                 }
             }
+            // The sums over the rows: each exchange halves the classes a lane holds, and
+            // lane l % 32 ends with the class of register l >> 1 & 15.
+            if (part_db) {
+#pragma unroll
+                for (int n = 8, o = 16; n > 0; n >>= 1, o >>= 1) {
+                    const bool upper = lane & o;
+#pragma unroll
+                    for (int r = 0; r < n; ++r) {
+                        const float keep = upper ? db[r + n] : db[r];
+                        db[r] = keep + __shfl_xor(upper ? db[r] : db[r + n], o, 64);
+                    }
+                }
+                db[0] += __shfl_xor(db[0], 1, 64);
+                const int r = lane >> 1 & 15;
+                if (!(lane & 1))
+                    part_db[((int64_t)row_tile * C::WN + wave % C::WN) * k.v_pad + c +
+                            (r >> 2) * 8 + half * 4 + (r & 3)] = db[0];
+            }
+        }
     };
     const int64_t tiles = (class_tiles - (int64_t)split + splits - 1) / splits;
     products<P, true, true, C>(a, b, tiles, 0, (k.d + BK<P> - 1) / BK<P>, lds, acc, next, done);
@@ -549,10 +618,9 @@ struct Out {
     int32_t splits;
     void *out;
     int64_t rows, stride;        // of the output; its columns are k.d
-    bool classes;                // dW: rows whose bias is -inf are 0; dh: f32, times weight
+    bool classes;                // dW: rows whose bias is -inf are 0; dh: times weight
 };
-template <int P> __device__ __forceinline__ float out_scale(const XentPack &k, bool classes) {
-    if (P == 1) return 1.0f;
+__device__ __forceinline__ float out_scale(const XentPack &k, bool classes) {
     return ldexpf(1.0f, -scale_exp(classes ? k.ctl->hg_max : k.ctl->w_max)) / G_SCALE;
 }
 template <int P>
@@ -561,10 +629,10 @@ __device__ __forceinline__ void put(const XentPack &k, const Out &o, int64_t m, 
     if (m >= o.rows || n >= k.d) return;
     if (o.classes) {
         if (k.bias[m] == -INFINITY) v = 0.0f;
-    } else if (P == 2) {
+    } else {
         scale *= k.weight[m];
     }
-    if constexpr (P == 1) static_cast<__bf16 *>(o.out)[m * o.stride + n] = (__bf16)v;
+    if constexpr (P == 1) static_cast<__bf16 *>(o.out)[m * o.stride + n] = (__bf16)(v * scale);
     else static_cast<float *>(o.out)[m * o.stride + n] = v * scale;
 }
 
@@ -588,7 +656,7 @@ __global__ __launch_bounds__(C::WAVES * 64, 2) void k_xent_product(XentPack k, O
     };
     products<P, AK, false, C>(a, b, 1, steps * split / o.splits, steps * (split + 1) / o.splits,
                               lds, acc, next, [](int64_t) {});
-    const float scale = out_scale<P>(k, o.classes);
+    const float scale = out_scale(k, o.classes);
     float *sums = o.acc + split * o.m_pad * k.ld;
 #pragma unroll
     for (int x = 0; x < C::MT; ++x)
@@ -616,7 +684,7 @@ __global__ __launch_bounds__(C::WAVES * 64, 2) void k_xent_product(XentPack k, O
 template <int P>
 __global__ __launch_bounds__(256) void k_xent_join_splits(XentPack k, int64_t m_first, Out o) {
     const int64_t m = m_first + blockIdx.x;
-    const float scale = out_scale<P>(k, o.classes);
+    const float scale = out_scale(k, o.classes);
     for (int32_t n = threadIdx.x; n < k.d; n += 256) {
         float v = 0.0f;
 #pragma unroll 4
@@ -625,33 +693,18 @@ __global__ __launch_bounds__(256) void k_xent_join_splits(XentPack k, int64_t m_
     }
 }
 
-// db[v] += sum over the rows of G, one wavefront a class.
-template <int P>
-__global__ __launch_bounds__(256) void k_xent_db(XentPack k, int64_t v0, int64_t classes, int64_t r0,
-                                                 int64_t rows_pad, int64_t plane,
-                                                 const u16 *__restrict__ g, bool first,
-                                                 float *__restrict__ db) {
-    const int lane = threadIdx.x & 63;
-    const int64_t c = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+// db[v] += the parts' sums, in order.
+__global__ __launch_bounds__(256) void k_xent_join_db(XentPack k, int64_t v0, int64_t classes,
+                                                      int32_t parts,
+                                                      const float *__restrict__ part_db,
+                                                      bool first, float *__restrict__ db) {
+    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (c >= classes) return;
-    float sum = 0.0f;
-    for (int64_t i = lane; i < rows_pad; i += 64) {
-        const u16 *at = g + c * rows_pad + i;
-        if constexpr (P == 1) {
-            sum += (float)__builtin_bit_cast(__bf16, *at);
-        } else {
-            const float p = (float)__builtin_bit_cast(_Float16, at[0]) +
-                            (float)__builtin_bit_cast(_Float16, at[plane]);
-            if (k.label[r0 + i] >= 0) sum += p * k.weight[r0 + i];
-        }
-    }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-    if (lane == 0) {
-        if (P == 2) sum *= 1.0f / G_SCALE;
-        if (k.bias[v0 + c] == -INFINITY) sum = 0.0f;
-        db[v0 + c] = first ? sum : db[v0 + c] + sum;
-    }
+    double sum = 0.0;
+#pragma unroll 8
+    for (int p = 0; p < parts; ++p) sum += part_db[p * k.v_pad + v0 + c];
+    if (k.bias[v0 + c] == -INFINITY) sum = 0.0;
+    db[v0 + c] = first ? (float)sum : (float)(db[v0 + c] + sum);
 }
 
 // Zeros where there is no row to sum over.
@@ -707,7 +760,7 @@ struct Plan {
     int64_t n_pad, v_pad, ld, piece_rows, piece_classes;
     int32_t splits;
     Cut dh, dw;                  // of whole pieces
-    size_t ctl, h, hg, w, bias, scale, label, weight, lse, part, g, dh_acc, dw_acc, end;
+    size_t ctl, h, hg, w, bias, scale, label, weight, lse, part, g, db, dh_acc, dw_acc, end;
 };
 
 Plan plan_of(const XentCall &c) {
@@ -742,7 +795,8 @@ Plan plan_of(const XentCall &c) {
     p.lse = take((size_t)4 * p.n_pad);
     p.part = take((size_t)16 * p.splits * p.n_pad);
     if (c.grad) {
-        p.hg = c.bf16 ? p.h : take((size_t)2 * p.P * p.n_pad * p.ld + past);
+        p.hg = take((size_t)2 * p.P * p.n_pad * p.ld + past);
+        if (c.dbias) p.db = take((size_t)4 * (p.piece_rows / 64) * p.v_pad);
         p.g = take((size_t)2 * p.P * p.piece_rows * p.piece_classes);
         p.dh = cut_of(p.wide, p.piece_rows, c.dim, p.piece_classes / step, c.num_cus);
         p.dw = cut_of(p.wide, p.piece_classes, c.dim, p.piece_rows / step, c.num_cus);
@@ -780,11 +834,11 @@ void launch_stats(hipStream_t s, const XentPack &k, int32_t splits, float2 *part
 }
 template <int P, class C>
 void launch_g(hipStream_t s, const XentPack &k, int64_t v0, int64_t nv, int64_t r0, int64_t nr,
-              int64_t plane, int num_cus, const float *lse2, u16 *g) {
+              int64_t plane, int num_cus, const float *lse2, u16 *g, float *part_db) {
     const int32_t rt = (int32_t)(nr / C::T), vt = (int32_t)(nv / C::T);
     const int32_t splits = splits_of<C>(rt, vt, num_cus);
     hipLaunchKernelGGL((k_xent_g<P, C>), dim3((uint32_t)rt * splits), dim3(C::WAVES * 64),
-                       (LDS_TILES<P, C>), s, k, v0, r0, nr, plane, rt, vt, splits, lse2, g);
+                       (LDS_TILES<P, C>), s, k, v0, r0, nr, plane, rt, vt, splits, lse2, g, part_db);
 }
 
 template <int P, typename T>
@@ -820,27 +874,28 @@ hipError_t run(hipStream_t s, const XentCall &c, const Plan &p, char *m) {
         if (e != hipSuccess) return e;
     }
     hipLaunchKernelGGL(k_xent_init, dim3(1), dim3(1), 0, s, k.ctl);
-    hipLaunchKernelGGL((k_xent_classes<T>), dim3(blocks(k.v_pad, 4)), b, 0, s, k, c.w, c.w_stride,
-                       c.bias);
-    hipLaunchKernelGGL((k_xent_pack_w<T>), dim3(blocks(k.v_pad, 4)), b, 0, s, k, c.w, c.w_stride);
-    hipLaunchKernelGGL((k_xent_rows<T>), dim3(blocks(k.n_pad, 4)), b, 0, s, k, c.h, c.h_stride,
-                       c.labels, c.weights);
+    const auto grid = [&](int64_t rows) {
+        return dim3(std::min<uint32_t>(blocks(rows, 4), 8 * (uint32_t)c.num_cus));
+    };
+    hipLaunchKernelGGL((k_xent_classes<T>), grid(k.v_pad), b, 0, s, k, c.w, c.w_stride, c.bias);
+    hipLaunchKernelGGL((k_xent_pack_w<T>), grid(k.v_pad), b, 0, s, k, c.w, c.w_stride);
+    hipLaunchKernelGGL((k_xent_rows<T>), grid(k.n_pad), b, 0, s, k, c.h, c.h_stride, c.labels,
+                       c.weights);
     if (p.wide) launch_stats<P, Wide>(s, k, p.splits, part);
     else launch_stats<P, Narrow>(s, k, p.splits, part);
     hipLaunchKernelGGL((k_xent_join<T>), dim3(blocks(k.n_pad, 4)), b, 0, s, k, c, 2 * p.splits,
                        part, lse2);
     if (!c.grad) return hipGetLastError();
-    if constexpr (P == 2)
-        hipLaunchKernelGGL(k_xent_pack_hg, dim3(blocks(k.n_pad, 4)), b, 0, s, k,
-                           static_cast<const float *>(c.h), c.h_stride);
+    hipLaunchKernelGGL((k_xent_pack_hg<T>), grid(k.n_pad), b, 0, s, k, c.h, c.h_stride);
     u16 *g = reinterpret_cast<u16 *>(m + p.g);
+    float *part_db = c.dbias ? reinterpret_cast<float *>(m + p.db) : nullptr;
     const int64_t plane = p.piece_rows * p.piece_classes, step = BK<P>;
     for (int64_t v0 = 0; v0 < k.v_pad; v0 += p.piece_classes)
         for (int64_t r0 = 0; r0 < k.n_pad; r0 += p.piece_rows) {
             const int64_t nv = std::min(p.piece_classes, k.v_pad - v0);
             const int64_t nr = std::min(p.piece_rows, k.n_pad - r0);
-            if (p.wide) launch_g<P, Wide>(s, k, v0, nv, r0, nr, plane, c.num_cus, lse2, g);
-            else launch_g<P, Narrow>(s, k, v0, nv, r0, nr, plane, c.num_cus, lse2, g);
+            if (p.wide) launch_g<P, Wide>(s, k, v0, nv, r0, nr, plane, c.num_cus, lse2, g, part_db);
+            else launch_g<P, Narrow>(s, k, v0, nv, r0, nr, plane, c.num_cus, lse2, g, part_db);
             const Operand ag{g, plane, nr};
             if (c.dh)
                 launch_product<P, false>(
@@ -854,8 +909,9 @@ hipError_t run(hipStream_t s, const XentCall &c, const Plan &p, char *m) {
                         r0 + nr == k.n_pad, 1, c.dw, k.v, c.w_stride, true});
             if (c.dbias) {
                 const int64_t live = std::min(nv, k.v - v0);
-                hipLaunchKernelGGL((k_xent_db<P>), dim3(blocks(live, 4)), b, 0, s, k, v0, live, r0,
-                                   nr, plane, g, r0 == 0, c.dbias);
+                // a part is 64 rows, of either tiling
+                hipLaunchKernelGGL(k_xent_join_db, dim3(blocks(live, 256)), b, 0, s, k, v0, live,
+                                   (int32_t)(nr / 64), part_db, r0 == 0, c.dbias);
             }
         }
     return hipGetLastError();

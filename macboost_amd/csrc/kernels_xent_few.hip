@@ -163,7 +163,7 @@ __global__ __launch_bounds__(64) void k_few_join(XentCall c, int32_t parts,
     }
     if (lane != 0) return;
     const bool none = top == -INFINITY && sum == 0.0f;
-    const float lse = ((top == -INFINITY ? 0.0f : top) + log2f(sum)) * LN2;
+    const float lse = log_sum(top, sum).natural;
     c.lse[i] = lse;
     const bool out = y < 0 || y >= c.classes || wt == 0.0f || none;
     c.loss[i] = out ? 0.0f : wt * (lse - (dot + by));

@@ -16,8 +16,8 @@
 // lane's own registers, rounded, are its operand, and the read across picks Y's
 // rows in that order: no value moves between lanes.
 //
-// f32 operands are two f16 terms (kernels_xent.hip says why); exponents are of 2, with
-// log2 e in the scale of S.
+// Operands are one f16 term (bf16) or two (f32), as kernels_xent.hip says; exponents are
+// of 2, with log2 e in the scale of S.
 #include <algorithm>
 
 #include "mbk.h"
@@ -46,7 +46,7 @@ struct Fused {
     float *bias2;                        // [v_pad] bias log2 e, -inf: not offered
     // of the rows, [n_pad]:
     float *sc;                           // log2 e times the scale of a score
-    int32_t *exp;                        // f32: h is packed times 2^exp
+    int32_t *exp;                        // h is packed times 2^exp
     int32_t *label;                      // -1: out, -2: out and not finite
     float *weight;                       // 0: out
     float *c2;                           // lse log2 e, +inf: out
@@ -99,13 +99,13 @@ __global__ __launch_bounds__(256) void k_fused_classes(Fused k, const void *w, i
         const bool open = b != -INFINITY;
         any = any || open;
         if (f == 0) k.bias2[v] = b * LOG2E;
-        if (sizeof(T) == 2 || !open) continue;
+        if (!open) continue;
         float x[4];
         load4<T>(w, v * stride, f, k.d, x);
         m = max(m, finite_max(x));
     }
     if (any && !k.ctl->open) k.ctl->open = 1u;
-    if (sizeof(T) == 4) raise_by_block(&k.ctl->w_max, m);
+    raise_by_block(&k.ctl->w_max, m);
 }
 
 // The packed rows of W and then of h.
@@ -116,7 +116,7 @@ __global__ __launch_bounds__(256) void k_fused_pack(Fused k, const void *w, int6
                                                     const float *__restrict__ weights) {
     constexpr int LANES = LD / 4, ROWS = 256 / LANES;
     const int f = threadIdx.x % LANES * 4;
-    const int sw = sizeof(T) == 4 ? scale_exp(k.ctl->w_max) : 0;
+    const int sw = scale_exp(k.ctl->w_max);
     const bool any = k.ctl->open;
     uint32_t hg = 0;
     for (int64_t at = (int64_t)blockIdx.x * ROWS + threadIdx.x / LANES; at < k.v_pad + k.n_pad;
@@ -149,28 +149,25 @@ __global__ __launch_bounds__(256) void k_fused_pack(Fused k, const void *w, int6
                     x[0] = x[1] = x[2] = x[3] = 0.0f;
                 }
             }
-            if (sizeof(T) == 4) s = scale_exp(m);
+            s = scale_exp(m);
             if (f == 0) {
                 k.label[i] = y;
                 k.weight[i] = wt;
                 k.exp[i] = s;
-                k.sc[i] = sizeof(T) == 4 ? ldexpf(LOG2E, -(s + sw)) : LOG2E;
+                k.sc[i] = ldexpf(LOG2E, -(s + sw));
                 if (wt != 0.0f) hg = max(hg, finite_bits(wt * __uint_as_float(m)));
             }
         }
         u16 *row = (of_w ? k.w : k.h) + i * LD + f;
         u16 hi[4], lo[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            if (sizeof(T) == 2) hi[e] = bits_of((__bf16)x[e]);
-            else split_f16(ldexpf(x[e], s), hi[e], lo[e]);
-        }
+        for (int e = 0; e < 4; ++e) split_f16(ldexpf(x[e], s), hi[e], lo[e]);
         *reinterpret_cast<u16x4 *>(row) = u16x4{hi[0], hi[1], hi[2], hi[3]};
         if (sizeof(T) == 4)
             *reinterpret_cast<u16x4 *>(row + (of_w ? k.v_pad : k.n_pad) * LD) =
                 u16x4{lo[0], lo[1], lo[2], lo[3]};
     }
-    if (sizeof(T) == 4) raise_by_block(&k.ctl->hg_max, hg);
+    raise_by_block(&k.ctl->hg_max, hg);
 }
 
 // ---- a tile in LDS -----------------------------------------------------------------
@@ -217,22 +214,17 @@ typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
 
 // Eight values as the second product's operand.
 template <int P> __device__ __forceinline__ void pack8(const float (&x)[8], u32x4 (&f)[P]) {
-    if constexpr (P == 1) {
-        bf16x8 v;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = (__bf16)x[e];
-        f[0] = __builtin_bit_cast(u32x4, v);
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-            const f16x2 hi = {(_Float16)x[e], (_Float16)x[e + 1]};
-            const uint32_t h = __builtin_bit_cast(uint32_t, hi);
+    for (int e = 0; e < 8; e += 2) {
+        const f16x2 hi = {(_Float16)x[e], (_Float16)x[e + 1]};
+        const uint32_t h = __builtin_bit_cast(uint32_t, hi);
+        f[0][e / 2] = h;
+        if constexpr (P == 2) {
             float r0, r1;                // x - hi in one instruction each
             asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r0) : "v"(h), "v"(x[e]));
             asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
                 : "=v"(r1) : "v"(h), "v"(x[e + 1]));
             const f16x2 lo = {(_Float16)r0, (_Float16)r1};
-            f[0][e / 2] = h;
             f[1][e / 2] = __builtin_bit_cast(uint32_t, lo);
         }
     }
@@ -373,7 +365,7 @@ __global__ __launch_bounds__(256, 2) void k_fused_rows(Fused k, int32_t splits,
         for (int p = 0; p < P; ++p)
             x[s][p] = *reinterpret_cast<const u32x4 *>(k.h + p * k.n_pad * LD + row * LD + s * 16 +
                                                        half * 8);
-    const float sc = P == 1 ? LOG2E : k.sc[row];
+    const float sc = k.sc[row];
     float ref = 0.0f, top = -INFINITY, sum = 0.0f;
     f32x16 o[GRAD ? JT : 1];
 #pragma unroll
@@ -488,30 +480,25 @@ __global__ __launch_bounds__(256) void k_fused_join_rows(Fused k, XentCall c, in
             o[3] += p.w * scale;
         }
     }
-    // a sum that is not a number is one with no reference, too
-    const float l2 = none && sum == 0.0f ? -INFINITY : (none ? 0.0f : ref) + log2f(sum);
+    const LogSum l = log_sum(ref, sum);
     const float wt = k.weight[i];
     if (f == 0) {
         if (i < k.n) {
-            const float lse = y == -2 ? NAN : l2 * LN2;
+            const float lse = y == -2 ? NAN : l.natural;
             const float z = open ? dot + (c.bias ? c.bias[y] : 0.0f) : -INFINITY;
             c.lse[i] = lse;
             c.loss[i] = y < 0 ? 0.0f : wt * (lse - z);
         }
         if constexpr (GRAD) {
-            k.c2[i] = y < 0 ? INFINITY : l2;
-            if (sizeof(T) == 2) {
-                k.wq[i] = wt;
-            } else {
-                // weight 2^-exp and the power of two that brings the largest below 2^15
-                const float q = ldexpf(wt, wq_exp(k.ctl->hg_max) - k.exp[i]);
-                k.wq[i] = fminf(fmaxf(q, -60000.0f), 60000.0f);
-            }
+            k.c2[i] = y < 0 ? INFINITY : l.base2;
+            // weight 2^-exp and the power of two that brings the largest below 2^15
+            const float q = ldexpf(wt, wq_exp(k.ctl->hg_max) - k.exp[i]);
+            k.wq[i] = fminf(fmaxf(q, -60000.0f), 60000.0f);
         }
     }
     if constexpr (GRAD) {
         if (!c.dh || i >= k.n) return;
-        const float scale = sizeof(T) == 4 ? ldexpf(1.0f, -scale_exp(k.ctl->w_max)) : 1.0f;
+        const float scale = ldexpf(1.0f, -scale_exp(k.ctl->w_max));
 #pragma unroll
         for (int e = 0; e < 4; ++e)
             if (f + e < k.d) {
@@ -546,7 +533,7 @@ __global__ __launch_bounds__(256, 2) void k_fused_classes_pass(Fused k, int32_t 
             x[s][p] = *reinterpret_cast<const u32x4 *>(k.w + p * k.v_pad * LD + v * LD + s * 16 +
                                                        half * 8);
     const float b2 = k.bias2[v];
-    float db = 0.0f;
+    double db = 0.0;                     // of sums over 32 rows
     f32x16 o[JT];
 #pragma unroll
     for (int j = 0; j < JT; ++j)
@@ -583,11 +570,11 @@ __global__ __launch_bounds__(256, 2) void k_fused_classes_pass(Fused k, int32_t 
             f32x16 s = first_product<P, KS>(tile, y, x);
             float p[2][8], of[16], of2[16];
             of_rows(c2, y, of);
-            if (P == 2) of_rows(sc, y, of2);
+            of_rows(sc, y, of2);
 #pragma unroll
             for (int r = 0; r < 16; ++r)
                 p[r >> 3][r & 7] = __builtin_amdgcn_exp2f(
-                    __builtin_fmaf(s[r], P == 1 ? LOG2E : of2[r], b2 - of[r]));
+                    __builtin_fmaf(s[r], of2[r], b2 - of[r]));
             if (hot) {
                 int32_t l[16];
                 of_rows(label, y, l);
@@ -596,9 +583,11 @@ __global__ __launch_bounds__(256, 2) void k_fused_classes_pass(Fused k, int32_t 
                     if (l[r] == v) p[r >> 3][r & 7] -= 1.0f;
             }
             if (part_db) {
+                float sum = 0.0f;
                 of_rows(weight, y, of);
 #pragma unroll
-                for (int r = 0; r < 16; ++r) db = __builtin_fmaf(p[r >> 3][r & 7], of[r], db);
+                for (int r = 0; r < 16; ++r) sum = __builtin_fmaf(p[r >> 3][r & 7], of[r], sum);
+                db += sum;
             }
             of_rows(wq, y, of);
 #pragma unroll
@@ -610,8 +599,8 @@ __global__ __launch_bounds__(256, 2) void k_fused_classes_pass(Fused k, int32_t 
     }
     const int64_t at = split * k.v_pad + v;
     if (part_db) {
-        db += other_half(db);
-        if (half == 0) part_db[at] = db;
+        db += __shfl_xor(db, 32, 64);
+        if (half == 0) part_db[at] = (float)db;
     }
     float *out = part + at * LD;
 #pragma unroll
@@ -631,12 +620,12 @@ __global__ __launch_bounds__(256) void k_fused_join_classes(Fused k, XentCall c,
                                                             const float *__restrict__ part_db) {
     constexpr int LANES = LD / 4, G = GROUPS ? SPLIT_GROUPS : 1, CLASSES = 256 / LANES / G;
     __shared__ float4 sums[GROUPS ? 256 : 1];
-    __shared__ float dbs[GROUPS ? 256 : 1];
+    __shared__ double dbs[GROUPS ? 256 : 1];
     const int l = threadIdx.x % LANES, f = l * 4;
     const int g = threadIdx.x / LANES % G;
     const int64_t v = (int64_t)blockIdx.x * CLASSES + threadIdx.x / (LANES * G);
     float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    float db = 0.0f;
+    double db = 0.0;
     if (v < k.v) {
 #pragma unroll 4
         for (int s = g; s < splits; s += G) {
@@ -664,14 +653,14 @@ __global__ __launch_bounds__(256) void k_fused_join_classes(Fused k, XentCall c,
     }
     if (v >= k.v) return;
     const bool open = k.bias2[v] != -INFINITY;
-    const float scale = sizeof(T) == 4 ? ldexpf(1.0f, -wq_exp(k.ctl->hg_max)) : 1.0f;
+    const float scale = ldexpf(1.0f, -wq_exp(k.ctl->hg_max));
     const float x[4] = {sum.x, sum.y, sum.z, sum.w};
     if (c.dw)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
             if (f + e < k.d)
                 static_cast<T *>(c.dw)[v * c.w_stride + f + e] = (T)(open ? x[e] * scale : 0.0f);
-    if (c.dbias && l == 0) c.dbias[v] = open ? db : 0.0f;
+    if (c.dbias && l == 0) c.dbias[v] = open ? (float)db : 0.0f;
 }
 
 // ---- the call ---------------------------------------------------------------------------

@@ -18,7 +18,6 @@ typedef __attribute__((ext_vector_type(16))) float f32x16;
 typedef unsigned short u16;
 
 constexpr float LOG2E = 1.44269504088896341f;
-constexpr float LN2 = 0.69314718055994531f;
 // Values beyond this (2^60) in a row that is out count as not finite: times a finite W they
 // could still overflow.
 constexpr uint32_t XENT_HUGE = 0x5D800000u;
@@ -50,10 +49,9 @@ __device__ __forceinline__ void raise(uint32_t *max, uint32_t v) {
     if (v > __atomic_load_n(max, __ATOMIC_RELAXED)) atomicMax(max, v);
 }
 
-__device__ __forceinline__ u16 bits_of(__bf16 v) { return __builtin_bit_cast(u16, v); }
 __device__ __forceinline__ u16 bits_of(_Float16 v) { return __builtin_bit_cast(u16, v); }
 
-// x 2^s in two f16 terms.
+// x in two f16 terms.
 __device__ __forceinline__ void split_f16(float x, u16 &hi, u16 &lo) {
     const _Float16 h = (_Float16)x;
     hi = bits_of(h);
@@ -68,24 +66,35 @@ struct XentPack {
     XentCtl *ctl;
     u16 *h, *hg, *w;                     // planes of n_pad * ld, v_pad * ld
     float *bias;                         // [v_pad] bias log2 e, -inf: not offered
-    float *row_scale;                    // [n_pad], f32: log2 e times the scale of a score
+    float *row_scale;                    // [n_pad] log2 e times the scale of a score
     int32_t *label;                      // [n_pad], -1: out, -2: out and not finite
     float *weight;                       // [n_pad], 0: out
 };
 
 template <int P>
 __device__ __forceinline__ f32x16 mma(const u32x4 (&a)[P], const u32x4 (&b)[P], f32x16 c) {
-    if constexpr (P == 1) {
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a[0]),
-                                                       __builtin_bit_cast(bf16x8, b[0]), c, 0, 0,
-                                                       0);
-    } else {
-        const f16x8 a0 = __builtin_bit_cast(f16x8, a[0]), a1 = __builtin_bit_cast(f16x8, a[1]);
-        const f16x8 b0 = __builtin_bit_cast(f16x8, b[0]), b1 = __builtin_bit_cast(f16x8, b[1]);
-        c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a1, b0, c, 0, 0, 0);
-        c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a0, b1, c, 0, 0, 0);
-        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a0, b0, c, 0, 0, 0);
+    const f16x8 a0 = __builtin_bit_cast(f16x8, a[0]), b0 = __builtin_bit_cast(f16x8, b[0]);
+    if constexpr (P == 2) {
+        c = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a[1]), b0, c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a0, __builtin_bit_cast(f16x8, b[1]), c, 0, 0, 0);
     }
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a0, b0, c, 0, 0, 0);
+}
+
+// The logarithm of 2^ref times sum, base 2 and base e: the exponent apart, since the
+// logarithm instruction rounds down, by up to a step of a result of 2^4.  Scores carry
+// LOG2E as f32 holds it, which the second undoes.
+struct LogSum {
+    float base2, natural;
+};
+__device__ __forceinline__ LogSum log_sum(float ref, float sum) {
+    if (!(sum > 0.0f && sum < INFINITY)) {
+        const float l = (ref == -INFINITY ? 0.0f : ref) + log2f(sum);
+        return {l, l};
+    }
+    const int e = __builtin_amdgcn_frexp_expf(sum);
+    const double l = (double)ref + e + log2f(__builtin_amdgcn_frexp_mantf(sum));
+    return {(float)l, (float)(l / (double)LOG2E)};
 }
 
 // ---- copies from memory to LDS

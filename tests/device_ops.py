@@ -97,9 +97,10 @@ class Xent:
 def xent_reference(h, w, labels, kind, bias=None, weights=None):
     """The loss and its gradients in 64 bits, and how far each may be off.
 
-    Half a step of the operands' splitting (two f16 terms hold 22 bits, and what the
-    three products drop is as much again) and of f32 sums of as many terms as there are
-    is carried through the formulas, worst case in every term."""
+    Half a step of the operands' splitting (f32: two f16 terms hold 22 bits, and what the
+    three products drop is as much again; bf16: one term holds it, G has 11 bits) and of
+    f32 sums of as many terms as there are is carried through the formulas, worst case
+    in every term."""
     h, w = rounded(h, kind).astype(np.float64), rounded(w, kind).astype(np.float64)
     n, d = h.shape
     v = w.shape[0]
@@ -139,11 +140,11 @@ def xent_reference(h, w, labels, kind, bias=None, weights=None):
         # the exponent's and exp2's own errors, and G's rounding
         dist = np.where(closed, 0, np.abs(z - lse[:, None]))
         rel = np.where(closed, 0, ez) + elz[:, None] + (3 * dist + 8) * u
-        half = HALF["bf16"] if kind == "bf16" else 2.0 ** -22
+        half = 2.0 ** -11 if kind == "bf16" else 2.0 ** -22     # G in one f16 term or two
         eg = np.abs(wl)[:, None] * (p * rel + np.abs(p - hot) * half + 2.0 ** -38)
         # f16 terms of G times the row's weight share one scale, that of the largest row
         rows = np.abs(hl).max(1) if d else np.zeros(n)
-        with_scale = 0.0 if kind == "bf16" else 2.0 ** -37 * (np.abs(wl) * rows).max(initial=0)
+        with_scale = 2.0 ** -37 * (np.abs(wl) * rows).max(initial=0)
         ew = eg + np.where(rows > 0, with_scale / np.where(rows > 0, rows, 1), 0)[:, None]
         for e in (eg, ew, g):
             e[~live] = 0
@@ -153,10 +154,11 @@ def xent_reference(h, w, labels, kind, bias=None, weights=None):
             return (e_left @ np.abs(right) + np.abs(left) @ e_right
                     + (np.abs(left) @ np.abs(right)) * (split + (products * terms + 16) * u))
 
-        none_w, none_h = np.zeros_like(w), np.zeros_like(hl)
+        # bf16: the row's weight goes into h's f16 term, or into G's
+        none_w, off_h = np.zeros_like(w), np.abs(hl) * (2.0 ** -11 if kind == "bf16" else 0.0)
         for name, value, err in (
                 ("dh", g @ w, product(g, w, eg, none_w, v)),
-                ("dw", g.T @ hl, product(g.T, hl, ew.T, none_h, n)),
+                ("dw", g.T @ hl, product(g.T, hl, ew.T, off_h, n)),
                 ("db", g.sum(0), eg.sum(0) + np.abs(g).sum(0) * (n + 4) * u)):
             step = HALF[kind] if name != "db" else u
             out[name] = (value, err + (np.abs(value) + err) * step + 1e-37)
