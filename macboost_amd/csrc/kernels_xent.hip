@@ -289,38 +289,68 @@ template <class C> __device__ __forceinline__ uint32_t across_at(int m0) {
     return row * (C::T * 2) + ((m >> 3) ^ ((row & 3) * 4)) * 16 + (m & 7) * 2;
 }
 #define TR(dst, addr, off) "ds_read_b64_tr_b16 " dst ", " addr " offset:" off "\n\t"
-template <int P, class C, int SLAB, int N>
-__device__ __forceinline__ void across(uint32_t at, u32x4 (&f)[N][P]) {
-    constexpr int ROW = C::T * 2, O = SLAB * 16 * ROW, O4 = O + 4 * ROW, PLANE = C::T * BK<P> * 2;
+#define TR2(d0, d1, addr, o0, o1) TR(d0, addr, o0) TR(d1, addr, o1)
+template <int N, int P> struct AcrossReads {
     u32x2 x[N][P][2];
-    const uint32_t a1 = at ^ 64, a2 = at ^ 128, a3 = at ^ 192;
+    __device__ __forceinline__ void get(u32x4 (&f)[N][P]) const {
+#pragma unroll
+        for (int t = 0; t < N; ++t)
+#pragma unroll
+            for (int p = 0; p < P; ++p)
+                f[t][p] = u32x4{x[t][p][0][0], x[t][p][0][1], x[t][p][1][0], x[t][p][1][1]};
+    }
+};
+template <int P, class C, int SLAB>
+__device__ __forceinline__ void across(uint32_t at, u32x4 (&f)[2][P]) {
+    constexpr int ROW = C::T * 2, O = SLAB * 16 * ROW, O4 = O + 4 * ROW, PLANE = C::T * BK<P> * 2;
+    AcrossReads<2, P> r;
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+        asm volatile(TR2("%0", "%1", "%4", "%6", "%7") TR2("%2", "%3", "%5", "%6", "%7")
+                     "s_waitcnt lgkmcnt(0)"
+                     : "=&v"(r.x[0][p][0]), "=&v"(r.x[0][p][1]), "=&v"(r.x[1][p][0]),
+                       "=&v"(r.x[1][p][1])
+                     : "v"(at + p * PLANE), "v"((at ^ 64) + p * PLANE), "n"(O), "n"(O4)
+                     : "memory");
+    r.get(f);
+}
+// Both operands across: one wait for all reads of a plane.
+template <int P, class C, int SLAB>
+__device__ __forceinline__ void across_both(uint32_t a, uint32_t b, u32x4 (&fa)[C::MT][P],
+                                            u32x4 (&fb)[C::NT][P]) {
+    constexpr int ROW = C::T * 2, O = SLAB * 16 * ROW, O4 = O + 4 * ROW, PLANE = C::T * BK<P> * 2;
+    AcrossReads<C::MT, P> ra;
+    AcrossReads<C::NT, P> rb;
+    static_assert(C::NT == 2 && (C::MT == 2 || C::MT == 4), "reads of 2 or 4 and 2 blocks");
 #pragma unroll
     for (int p = 0; p < P; ++p) {
-        if constexpr (N == 2) {
-            asm volatile(TR("%0", "%4", "%6") TR("%1", "%4", "%7") TR("%2", "%5", "%6")
-                         TR("%3", "%5", "%7") "s_waitcnt lgkmcnt(0)"
-                         : "=&v"(x[0][p][0]), "=&v"(x[0][p][1]), "=&v"(x[1][p][0]),
-                           "=&v"(x[1][p][1])
-                         : "v"(at + p * PLANE), "v"(a1 + p * PLANE), "n"(O), "n"(O4)
+        const uint32_t ap = a + p * PLANE, bp = b + p * PLANE;
+        if constexpr (C::MT == 4)
+            asm volatile(TR2("%0", "%1", "%12", "%18", "%19") TR2("%2", "%3", "%13", "%18", "%19")
+                         TR2("%4", "%5", "%14", "%18", "%19") TR2("%6", "%7", "%15", "%18", "%19")
+                         TR2("%8", "%9", "%16", "%18", "%19")
+                         TR2("%10", "%11", "%17", "%18", "%19") "s_waitcnt lgkmcnt(0)"
+                         : "=&v"(ra.x[0][p][0]), "=&v"(ra.x[0][p][1]), "=&v"(ra.x[1][p][0]),
+                           "=&v"(ra.x[1][p][1]), "=&v"(ra.x[2][p][0]), "=&v"(ra.x[2][p][1]),
+                           "=&v"(ra.x[3][p][0]), "=&v"(ra.x[3][p][1]), "=&v"(rb.x[0][p][0]),
+                           "=&v"(rb.x[0][p][1]), "=&v"(rb.x[1][p][0]), "=&v"(rb.x[1][p][1])
+                         : "v"(ap), "v"(ap ^ 64), "v"(ap ^ 128), "v"(ap ^ 192), "v"(bp),
+                           "v"(bp ^ 64), "n"(O), "n"(O4)
                          : "memory");
-        } else {
-            asm volatile(TR("%0", "%8", "%12") TR("%1", "%8", "%13") TR("%2", "%9", "%12")
-                         TR("%3", "%9", "%13") TR("%4", "%10", "%12") TR("%5", "%10", "%13")
-                         TR("%6", "%11", "%12") TR("%7", "%11", "%13") "s_waitcnt lgkmcnt(0)"
-                         : "=&v"(x[0][p][0]), "=&v"(x[0][p][1]), "=&v"(x[1][p][0]),
-                           "=&v"(x[1][p][1]), "=&v"(x[2][p][0]), "=&v"(x[2][p][1]),
-                           "=&v"(x[3][p][0]), "=&v"(x[3][p][1])
-                         : "v"(at + p * PLANE), "v"(a1 + p * PLANE), "v"(a2 + p * PLANE),
-                           "v"(a3 + p * PLANE), "n"(O), "n"(O4)
+        else
+            asm volatile(TR2("%0", "%1", "%8", "%12", "%13") TR2("%2", "%3", "%9", "%12", "%13")
+                         TR2("%4", "%5", "%10", "%12", "%13") TR2("%6", "%7", "%11", "%12", "%13")
+                         "s_waitcnt lgkmcnt(0)"
+                         : "=&v"(ra.x[0][p][0]), "=&v"(ra.x[0][p][1]), "=&v"(ra.x[1][p][0]),
+                           "=&v"(ra.x[1][p][1]), "=&v"(rb.x[0][p][0]), "=&v"(rb.x[0][p][1]),
+                           "=&v"(rb.x[1][p][0]), "=&v"(rb.x[1][p][1])
+                         : "v"(ap), "v"(ap ^ 64), "v"(bp), "v"(bp ^ 64), "n"(O), "n"(O4)
                          : "memory");
-        }
     }
-#pragma unroll
-    for (int t = 0; t < N; ++t)
-#pragma unroll
-        for (int p = 0; p < P; ++p)
-            f[t][p] = u32x4{x[t][p][0][0], x[t][p][0][1], x[t][p][1][0], x[t][p][1][1]};
+    ra.get(fa);
+    rb.get(fb);
 }
+#undef TR2
 #undef TR
 
 template <class C> using Acc = f32x16[C::MT][C::NT];
@@ -371,10 +401,15 @@ __device__ __forceinline__ void products(const Operand &a, const Operand &b, int
             const auto slab = [&](auto which) {
                 constexpr int S = decltype(which)::value;
                 u32x4 fa[C::MT][P], fb[C::NT][P];
-                if constexpr (AK) along<P, C, S>(lds + cur, wm, fa);
-                else across<P, C, S>(base + cur + a_at, fa);
-                if constexpr (BKC) along<P, C, S>(lds + cur + OP_BYTES<P, C>, wn, fb);
-                else across<P, C, S>(base + cur + OP_BYTES<P, C> + b_at, fb);
+                if constexpr (!AK && !BKC) {
+                    across_both<P, C, S>(base + cur + a_at, base + cur + OP_BYTES<P, C> + b_at, fa,
+                                         fb);
+                } else {
+                    static_assert(AK, "A across goes with B across");
+                    along<P, C, S>(lds + cur, wm, fa);
+                    if constexpr (BKC) along<P, C, S>(lds + cur + OP_BYTES<P, C>, wn, fb);
+                    else across<P, C, S>(base + cur + OP_BYTES<P, C> + b_at, fb);
+                }
 #pragma unroll
                 for (int x = 0; x < C::MT; ++x)
 #pragma unroll
