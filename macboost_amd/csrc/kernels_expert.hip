@@ -194,6 +194,181 @@ __global__ __launch_bounds__(64 * SORT_WAVES) void k_expert_place(
     no_source(a, b, offsets[experts], source);
 }
 
+// Up to CHUNK_EXPERTS experts: a workgroup takes chunks of assignments, orders each in
+// LDS by (expert, assignment) and writes source from there, in runs.  (10M assignments to
+// 1000 experts: with a wavefront a unit and single writes 88 us, 304 MB written for 80:
+// the part of source that an XCD writes at once does not fit its L2.)
+// R times 64 assignments a wavefront: 16, or 4 where that would leave most CUs idle (131k
+// assignments to 64 experts: 18 us by 16 workgroups, 10 by 64).
+constexpr int CHUNK_WAVES = 8;
+template <int R> constexpr int CHUNK = R * CHUNK_WAVES * 64;
+constexpr int64_t FEW_SLOTS = (int64_t)1 << 19;
+constexpr int32_t CHUNK_EXPERTS = 2048;
+// Counters a place kernel sums up by itself, without the kernels that scan them.
+constexpr int64_t DIRECT_COUNTERS = 8192;
+
+// table[e * units + u]: assignments of workgroup u to expert e.
+template <int R>
+__global__ __launch_bounds__(64 * CHUNK_WAVES) void k_expert_count_chunks(
+    const int32_t *__restrict__ expert, int64_t slots, int32_t experts, int64_t per, int32_t units,
+    uint32_t *__restrict__ table) {
+    extern __shared__ uint32_t count[];
+    const int32_t u = run_of(blockIdx.x, gridDim.x);
+    for (int e = threadIdx.x; e < experts; e += 64 * CHUNK_WAVES) count[e] = 0;
+    __syncthreads();
+    const int64_t b = min(slots, (u + 1) * per);
+    for (int64_t a = u * per; a < b; a += CHUNK<R>) {
+        const int64_t w = a + (threadIdx.x >> 6) * (64 * R);
+        int32_t key[R];
+#pragma unroll
+        for (int q = 0; q < R; ++q) {
+            const int64_t i = w + q * 64 + (threadIdx.x & 63);
+            key[q] = i < b ? expert[i] : -1;
+        }
+#pragma unroll
+        for (int q = 0; q < R; ++q)
+            if ((uint32_t)key[q] < (uint32_t)experts) atomicAdd(&count[key[q]], 1u);
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < experts; e += 64 * CHUNK_WAVES)
+        table[(int64_t)e * units + u] = count[e];
+}
+
+// DIRECT: the table holds counts, and workgroup 0 writes the offsets; else sums over the
+// workgroups before, and the offsets are there.
+template <int R, bool DIRECT>
+__global__ __launch_bounds__(64 * CHUNK_WAVES) void k_expert_place_chunks(
+    const int32_t *__restrict__ expert, int64_t slots, int32_t experts, int32_t key_bits,
+    int64_t per, int32_t units, const uint32_t *__restrict__ table,
+    int32_t *__restrict__ offsets, int32_t *__restrict__ source, int32_t *__restrict__ slot) {
+    extern __shared__ uint32_t lds[];
+    constexpr int THREADS = 64 * CHUNK_WAVES;
+    uint32_t *wave_sum = lds;                        // CHUNK_WAVES
+    uint32_t *next = wave_sum + CHUNK_WAVES;         // [expert] its next slot
+    uint32_t *first = next + experts;                // [expert] its first place in the chunk
+    uint32_t *staged = first + experts;              // [place] expert << 13 | assignment
+    uint32_t *count = staged + CHUNK<R>;                // [wave][expert]
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int32_t u = run_of(blockIdx.x, gridDim.x);
+    uint32_t kept_all, all;
+    if constexpr (DIRECT) {
+        // first: all of an expert's assignments; next: those before this workgroup's
+        for (int e = wave; e < experts; e += CHUNK_WAVES) {
+            uint32_t before = 0, sum = 0;
+            for (int v = lane; v < units; v += 64) {
+                const uint32_t c = table[(int64_t)e * units + v];
+                sum += c;
+                if (v < u) before += c;
+            }
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1) {
+                sum += __shfl_xor(sum, o, 64);
+                before += __shfl_xor(before, o, 64);
+            }
+            if (lane == 0) {
+                first[e] = sum;
+                next[e] = before;
+            }
+        }
+        __syncthreads();
+        uint32_t below = 0;
+        for (int e0 = 0; e0 < experts; e0 += THREADS) {
+            const int e = e0 + threadIdx.x;
+            const uint32_t at =
+                below + sum_before<CHUNK_WAVES>(e < experts ? first[e] : 0, wave_sum, all);
+            if (e < experts) {
+                next[e] += at;
+                if (u == 0) offsets[e] = (int32_t)at;
+            }
+            below += all;
+        }
+        if (u == 0 && threadIdx.x == 0) offsets[experts] = (int32_t)below;
+        kept_all = below;
+    } else {
+        for (int e = threadIdx.x; e < experts; e += THREADS)
+            next[e] = (uint32_t)offsets[e] + table[(int64_t)e * units + u];
+        kept_all = (uint32_t)offsets[experts];
+    }
+    const int64_t b = min(slots, (u + 1) * per);
+    for (int64_t a = u * per; a < b; a += CHUNK<R>) {
+        const int64_t w = a + wave * (64 * R);
+        int32_t key[R];
+        uint32_t rank[R];
+#pragma unroll
+        for (int q = 0; q < R; ++q) {
+            const int64_t i = w + q * 64 + lane;
+            key[q] = i < b ? expert[i] : -1;
+        }
+        for (int e = threadIdx.x; e < CHUNK_WAVES * experts; e += THREADS) count[e] = 0;
+        __syncthreads();
+        uint32_t *mine = count + wave * experts;
+#pragma unroll
+        for (int q = 0; q < R; ++q) {
+            const uint32_t e = (uint32_t)key[q];
+            const bool kept = e < (uint32_t)experts;
+            uint64_t same = __ballot(kept);          // lanes with this lane's expert
+            for (int k = 0; k < key_bits; ++k) {
+                const uint64_t ones = __ballot((e >> k) & 1u);
+                same &= (e >> k) & 1u ? ones : ~ones;
+            }
+            const uint32_t r = lanes_below(same);
+            rank[q] = kept ? mine[e] + r : 0;
+            __builtin_amdgcn_wave_barrier();
+            if (kept && r == 0) mine[e] = rank[q] + (uint32_t)__popcll(same);
+            __builtin_amdgcn_wave_barrier();
+        }
+        __syncthreads();
+        // counts become sums over the wavefronts before, first the place of each expert,
+        // next the slot that goes with place 0
+        uint32_t taken = 0;
+        for (int e0 = 0; e0 < experts; e0 += THREADS) {
+            const int e = e0 + threadIdx.x;
+            uint32_t sum = 0;
+            if (e < experts)
+#pragma unroll
+                for (int v = 0; v < CHUNK_WAVES; ++v) {
+                    const uint32_t c = count[v * experts + e];
+                    count[v * experts + e] = sum;
+                    sum += c;
+                }
+            const uint32_t at = taken + sum_before<CHUNK_WAVES>(sum, wave_sum, all);
+            if (e < experts) {
+                first[e] = at;
+                next[e] -= at;
+            }
+            taken += all;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < R; ++q) {
+            const int64_t i = w + q * 64 + lane;
+            if (i >= b) continue;
+            const uint32_t e = (uint32_t)key[q];
+            int32_t s = -1;
+            if (e < (uint32_t)experts) {
+                const uint32_t at = first[e] + mine[e] + rank[q];
+                staged[at] = e << 13 | (uint32_t)(i - a);
+                s = (int32_t)(next[e] + at);
+            }
+            slot[i] = s;
+        }
+        __syncthreads();
+        for (uint32_t l = threadIdx.x; l < taken; l += THREADS) {
+            const uint32_t v = staged[l];
+            source[next[v >> 13] + l] = (int32_t)(a + (v & (CHUNK<R> - 1)));
+        }
+        __syncthreads();
+        // the chunk's assignments are behind
+        for (int e0 = 0; e0 < experts; e0 += THREADS) {
+            const int e = e0 + threadIdx.x;
+            if (e < experts) next[e] += e + 1 < experts ? first[e + 1] : taken;
+        }
+        __syncthreads();
+    }
+    for (int64_t i = max(u * per, (int64_t)kept_all) + threadIdx.x; i < b; i += THREADS)
+        source[i] = -1;                              // behind the last slot taken
+}
+
 // Few assignments: the whole sort by one workgroup (1000 to 4 experts 13 us less than by
 // the four kernels above, whose launches are all there is).
 constexpr int SMALL_WAVES = 16;
@@ -502,7 +677,7 @@ template <typename T, bool XCOLS, bool SCOLS>
 __global__ __launch_bounds__(256) void k_expert_gather(ExpertPlan p, ExpertMatrix x,
                                                        T *__restrict__ sorted) {
     __shared__ T tile[TILE][TILE + 1];
-    const int64_t i0 = (int64_t)blockIdx.x * TILE;
+    const int64_t i0 = (int64_t)run_of(blockIdx.x, gridDim.x) * TILE;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const T *data = static_cast<const T *>(x.data);
     for (int32_t f0 = blockIdx.y * TILE; f0 < x.cols; f0 += gridDim.y * TILE) {
@@ -542,7 +717,7 @@ __global__ __launch_bounds__(256) void k_expert_combine(ExpertPlan p, const T *_
                                                         ExpertMatrix out) {
     constexpr int Q = TILE / 4;
     __shared__ float tile[TILE][TILE + 1];
-    const int64_t i0 = (int64_t)blockIdx.x * TILE;
+    const int64_t i0 = (int64_t)run_of(blockIdx.x, gridDim.x) * TILE;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     T *data = static_cast<T *>(out.data);
     for (int32_t f0 = blockIdx.y * TILE; f0 < out.cols; f0 += gridDim.y * TILE) {
@@ -564,15 +739,25 @@ __global__ __launch_bounds__(256) void k_expert_combine(ExpertPlan p, const T *_
             float sum[Q];
 #pragma unroll
             for (int q = 0; q < Q; ++q) sum[q] = 0.0f;
-            for (int j = 0; j < p.k; ++j) {
-                const int64_t a = (i0 + lane) * p.k + j;
-                const Place at = place_of(p, a, out.cols, out.blocked);
-                if (at.base < 0) continue;
-                const float w = weights ? weights[a] : 1.0f;
-                const T *from = sorted + at.base + (f0 + wave) * at.step;
+            // two assignments' values are asked for at once
+            for (int j = 0; j < p.k; j += 2) {
+                float v[2][Q], w[2];
 #pragma unroll
-                for (int q = 0; q < Q; ++q)
-                    if (f0 + wave + 4 * q < out.cols) sum[q] += w * to_f32(from[4 * q * at.step]);
+                for (int h = 0; h < 2; ++h) {
+                    const int64_t a = (i0 + lane) * p.k + min(j + h, p.k - 1);
+                    const Place at = place_of(p, a, out.cols, out.blocked);
+                    const bool take = at.base >= 0 && j + h < p.k;
+                    w[h] = take && weights ? weights[a] : 1.0f;
+                    const T *from = sorted + at.base + (f0 + wave) * at.step;
+#pragma unroll
+                    for (int q = 0; q < Q; ++q)
+                        v[h][q] = take && f0 + wave + 4 * q < out.cols
+                                      ? to_f32(from[4 * q * at.step]) : 0.0f;
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int q = 0; q < Q; ++q) sum[q] += w[h] * v[h][q];
             }
 #pragma unroll
             for (int q = 0; q < Q; ++q) tile[lane][wave + 4 * q] = sum[q];
@@ -596,7 +781,7 @@ __global__ __launch_bounds__(256) void k_expert_combine_grad(
     const float *__restrict__ weights, T *__restrict__ d_sorted, float *__restrict__ d_weights) {
     __shared__ T tile[TILE][TILE + 1];
     __shared__ float sums[TILE][5];
-    const int64_t i0 = (int64_t)blockIdx.x * TILE;
+    const int64_t i0 = (int64_t)run_of(blockIdx.x, gridDim.x) * TILE;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const T *data = static_cast<const T *>(dout.data);
     for (int j = 0; j < p.k; ++j) {
@@ -760,15 +945,55 @@ hipError_t combine_grad(hipStream_t s, const ExpertPlan &p, const ExpertMatrix &
 #undef BY_BYTES
 #undef BY_LAYOUT
 
+// Chunks of up to 2048 workgroups (a thread of the scan takes eight).
+SortShape chunk_shape(const ExpertPlan &p, int64_t chunk) {
+    const int64_t slots = p.rows * p.k, chunks = (slots + chunk - 1) / chunk;
+    const int64_t per = std::max<int64_t>(1, (chunks + SCAN * SCAN_EACH - 1) / (SCAN * SCAN_EACH));
+    return {per * chunk, (int32_t)std::max<int64_t>(1, (chunks + per - 1) / per)};
+}
+bool by_chunks(const ExpertPlan &p) { return p.experts <= CHUNK_EXPERTS; }
+SortShape shape_of(const ExpertPlan &p, int num_cus) {
+    if (!by_chunks(p)) return sort_shape(p, num_cus);
+    return chunk_shape(p, p.rows * p.k <= FEW_SLOTS ? CHUNK<4> : CHUNK<16>);
+}
+
+template <int R>
+hipError_t sort_chunks(hipStream_t s, const ExpertPlan &p, const SortShape &sh, int bits,
+                       uint32_t *table, uint32_t *total) {
+    for (const void *f : {reinterpret_cast<const void *>(k_expert_place_chunks<R, true>),
+                          reinterpret_cast<const void *>(k_expert_place_chunks<R, false>)}) {
+        const hipError_t e = allow_all_lds(f);
+        if (e != hipSuccess) return e;
+    }
+    const int64_t slots = p.rows * p.k;
+    const dim3 g((uint32_t)sh.units), b(64 * CHUNK_WAVES);
+    const size_t lds = sizeof(uint32_t) *
+                       (CHUNK_WAVES + CHUNK<R> + (size_t)(CHUNK_WAVES + 2) * p.experts);
+    hipLaunchKernelGGL((k_expert_count_chunks<R>), g, b, sizeof(uint32_t) * p.experts, s, p.expert,
+                       slots, p.experts, sh.per, sh.units, table);
+    if ((int64_t)p.experts * sh.units <= DIRECT_COUNTERS) {
+        hipLaunchKernelGGL((k_expert_place_chunks<R, true>), g, b, lds, s, p.expert, slots,
+                           p.experts, bits, sh.per, sh.units, table, p.offsets, p.source, p.slot);
+    } else {
+        hipLaunchKernelGGL(k_expert_scan, dim3((uint32_t)p.experts), dim3(SCAN), 0, s, table,
+                           sh.units, total);
+        hipLaunchKernelGGL(k_expert_offsets, dim3(1), dim3(1024), 0, s, total, p.experts,
+                           p.offsets);
+        hipLaunchKernelGGL((k_expert_place_chunks<R, false>), g, b, lds, s, p.expert, slots,
+                           p.experts, bits, sh.per, sh.units, table, p.offsets, p.source, p.slot);
+    }
+    return hipGetLastError();
+}
+
 }  // namespace
 
 size_t expert_scratch(const ExpertPlan &p, int num_cus) {
-    const SortShape sh = sort_shape(p, num_cus);
+    const SortShape sh = shape_of(p, num_cus);
     return ((size_t)p.experts * sh.units + p.experts + 1) * sizeof(uint32_t);
 }
 
 hipError_t launch_expert_sort(hipStream_t s, const ExpertPlan &p, int num_cus, char *scratch) {
-    const SortShape sh = sort_shape(p, num_cus);
+    const SortShape sh = shape_of(p, num_cus);
     const int64_t slots = p.rows * p.k;
     uint32_t *table = reinterpret_cast<uint32_t *>(scratch);
     uint32_t *total = table + (size_t)p.experts * sh.units;
@@ -788,6 +1013,9 @@ hipError_t launch_expert_sort(hipStream_t s, const ExpertPlan &p, int num_cus, c
                            slots, p.experts, bits, per, p.offsets, p.source, p.slot, trash);
         return hipGetLastError();
     }
+    if (by_chunks(p))
+        return slots <= FEW_SLOTS ? sort_chunks<4>(s, p, sh, bits, table, total)
+                                  : sort_chunks<16>(s, p, sh, bits, table, total);
     const dim3 g((uint32_t)((sh.units + SORT_WAVES - 1) / SORT_WAVES)), b(64 * SORT_WAVES);
     const size_t lds = (size_t)SORT_WAVES * p.experts * sizeof(uint32_t);
     hipLaunchKernelGGL(k_expert_count, g, b, lds, s, p.expert, slots, p.experts, sh.per, sh.units,

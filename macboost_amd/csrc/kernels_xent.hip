@@ -49,27 +49,33 @@ template <typename T> __device__ __forceinline__ float load_f32(const void *p, i
     return (float)static_cast<const T *>(p)[i];
 }
 
-// Eight elements of a row from f on, zeros behind its d: 16 bytes at a time where the rows
-// allow.
+// What the rows of a matrix are aligned to: 16, 4, or an element.
+template <typename T> __device__ __forceinline__ int alignment(const void *p, int64_t stride) {
+    const uintptr_t all = reinterpret_cast<uintptr_t>(p) | (uintptr_t)(stride * sizeof(T));
+    return all & 15 ? (all & 3 ? 2 : 4) : 16;
+}
+// Eight elements of a row from f on, zeros behind its d.
 template <typename T>
-__device__ __forceinline__ void load8(const void *p, int64_t row, int f, int d, bool aligned,
+__device__ __forceinline__ void load8(const void *p, int64_t row, int f, int d, int align,
                                       float (&x)[8]) {
     const T *from = static_cast<const T *>(p) + row + f;
-    if (aligned && f + 8 <= d) {
+    T y[8];
+    if (align == 16 && f + 8 <= d) {
         u32x4 v[sizeof(T) / 2];
 #pragma unroll
         for (int q = 0; q < (int)sizeof(T) / 2; ++q) v[q] = reinterpret_cast<const u32x4 *>(from)[q];
-        T y[8];
         __builtin_memcpy(y, v, sizeof y);
+    } else if (sizeof(T) == 2 && align != 2 && f + 8 <= d) {
+        uint32_t v[4];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = (float)y[e];
+        for (int q = 0; q < 4; ++q) v[q] = reinterpret_cast<const uint32_t *>(from)[q];
+        __builtin_memcpy(y, v, sizeof v);
     } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = f + e < d ? (float)from[e] : 0.0f;
+        for (int e = 0; e < 8; ++e) y[e] = f + e < d ? from[e] : (T)0.0f;
     }
-}
-template <typename T> __device__ __forceinline__ bool aligned16(const void *p, int64_t stride) {
-    return ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)(stride * sizeof(T))) & 15) == 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = (float)y[e];
 }
 // Eight elements times 2^s into the planes.
 template <typename T>
@@ -100,21 +106,31 @@ template <typename T>
 __global__ __launch_bounds__(256) void k_xent_classes(XentPack k, const void *w, int64_t stride,
                                                       const float *__restrict__ bias) {
     const int lane = threadIdx.x & 63;
-    const bool aligned = aligned16<T>(w, stride);
+    const int align = alignment<T>(w, stride);
     uint32_t m = 0;
     bool any = false;
-    for (int64_t v = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); v < k.v_pad;
-         v += (int64_t)gridDim.x * 4) {
-        const float b = v < k.v ? (bias ? bias[v] : 0.0f) : -INFINITY;
-        const bool open = b != -INFINITY;
-        any = any || open;
-        if (lane == 0) k.bias[v] = b * LOG2E;
-        if (!open) continue;
-        for (int32_t f = lane * 8; f < k.d; f += 512) {
-            float x[8];
-            load8<T>(w, v * stride, f, k.d, aligned, x);
+    // four rows at a time, so that as many loads are on the way
+    constexpr int ROWS = 4;
+    const int64_t hop = (int64_t)gridDim.x * 4;
+    for (int64_t v0 = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); v0 < k.v_pad; v0 += ROWS * hop) {
+        int32_t d[ROWS];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) m = max(m, finite_bits(x[e]));
+        for (int q = 0; q < ROWS; ++q) {
+            const int64_t v = v0 + q * hop;
+            const float b = v < k.v ? (bias ? bias[v] : 0.0f) : -INFINITY;
+            d[q] = b != -INFINITY ? k.d : 0;
+            any = any || d[q] > 0;
+            if (lane == 0 && v < k.v_pad) k.bias[v] = b * LOG2E;
+        }
+        for (int32_t f = lane * 8; f < k.d; f += 512) {
+            float x[ROWS][8];
+#pragma unroll
+            for (int q = 0; q < ROWS; ++q)
+                load8<T>(w, (d[q] ? v0 + q * hop : 0) * stride, f, d[q], align, x[q]);
+#pragma unroll
+            for (int q = 0; q < ROWS; ++q)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) m = max(m, finite_bits(x[q][e]));
         }
     }
     if (any && !k.ctl->open) k.ctl->open = 1u;
@@ -124,15 +140,24 @@ __global__ __launch_bounds__(256) void k_xent_classes(XentPack k, const void *w,
 template <typename T>
 __global__ __launch_bounds__(256) void k_xent_pack_w(XentPack k, const void *w, int64_t stride) {
     const int lane = threadIdx.x & 63;
-    const bool aligned = aligned16<T>(w, stride);
+    const int align = alignment<T>(w, stride);
     const int s = scale_exp(k.ctl->w_max);
-    for (int64_t v = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); v < k.v_pad;
-         v += (int64_t)gridDim.x * 4) {
-        const int32_t d = k.bias[v] != -INFINITY ? k.d : 0;
+    constexpr int ROWS = 2;
+    const int64_t hop = (int64_t)gridDim.x * 4;
+    for (int64_t v0 = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); v0 < k.v_pad; v0 += ROWS * hop) {
+        int32_t d[ROWS];
+#pragma unroll
+        for (int q = 0; q < ROWS; ++q)
+            d[q] = v0 + q * hop < k.v && k.bias[v0 + q * hop] != -INFINITY ? k.d : 0;
         for (int32_t f = lane * 8; f < k.ld; f += 512) {
-            float x[8];
-            load8<T>(w, v * stride, f, d, aligned, x);
-            pack8<T>(x, s, k.w + v * k.ld + f, k.v_pad * k.ld);
+            float x[ROWS][8];
+#pragma unroll
+            for (int q = 0; q < ROWS; ++q)
+                load8<T>(w, (d[q] ? v0 + q * hop : 0) * stride, f, d[q], align, x[q]);
+#pragma unroll
+            for (int q = 0; q < ROWS; ++q)
+                if (v0 + q * hop < k.v_pad)
+                    pack8<T>(x[q], s, k.w + (v0 + q * hop) * k.ld + f, k.v_pad * k.ld);
         }
     }
 }
@@ -144,7 +169,8 @@ __global__ __launch_bounds__(256) void k_xent_rows(XentPack k, const void *h, in
                                                    const int32_t *__restrict__ labels,
                                                    const float *__restrict__ weights) {
     const int lane = threadIdx.x & 63;
-    const bool aligned = aligned16<T>(h, stride), any = k.ctl->open;
+    const int align = alignment<T>(h, stride);
+    const bool any = k.ctl->open;
     const int sw = scale_exp(k.ctl->w_max);
     uint32_t hg = 0;
     for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < k.n_pad;
@@ -155,7 +181,7 @@ __global__ __launch_bounds__(256) void k_xent_rows(XentPack k, const void *h, in
         uint32_t m = 0, most = 0;
         for (int32_t f = lane * 8; f < d; f += 512) {
             float x[8];
-            load8<T>(h, i * stride, f, d, aligned, x);
+            load8<T>(h, i * stride, f, d, align, x);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 m = max(m, finite_bits(x[e]));
@@ -181,7 +207,7 @@ __global__ __launch_bounds__(256) void k_xent_rows(XentPack k, const void *h, in
         }
         for (int32_t f = lane * 8; f < k.ld; f += 512) {
             float x[8];
-            load8<T>(h, i * stride, f, d, aligned, x);
+            load8<T>(h, i * stride, f, d, align, x);
             pack8<T>(x, s, k.h + i * k.ld + f, k.n_pad * k.ld);
         }
     }
@@ -193,7 +219,7 @@ __global__ __launch_bounds__(256) void k_xent_rows(XentPack k, const void *h, in
 template <typename T>
 __global__ __launch_bounds__(256) void k_xent_pack_hg(XentPack k, const void *h, int64_t stride) {
     const int lane = threadIdx.x & 63;
-    const bool aligned = aligned16<T>(h, stride);
+    const int align = alignment<T>(h, stride);
     const int s = scale_exp(k.ctl->hg_max);
     for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < k.n_pad;
          i += (int64_t)gridDim.x * 4) {
@@ -201,7 +227,7 @@ __global__ __launch_bounds__(256) void k_xent_pack_hg(XentPack k, const void *h,
         const float wt = k.weight[i];
         for (int32_t f = lane * 8; f < k.ld; f += 512) {
             float x[8];
-            load8<T>(h, i * stride, f, d, aligned, x);
+            load8<T>(h, i * stride, f, d, align, x);
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[e] *= wt;
             pack8<T>(x, s, k.hg + i * k.ld + f, k.n_pad * k.ld);

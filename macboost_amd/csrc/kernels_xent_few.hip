@@ -4,7 +4,8 @@
 // h lies in LDS whole, as operands of the matrix instruction.  Each wavefront takes tiles
 // of 32 classes by itself: their rows are copied straight into its own LDS buffers, 128
 // bytes of each at a time and two steps ahead, so that eight wavefronts keep 64 KB
-// of a CU on the way and no barrier holds them.  The product is W h' (classes down,
+// of a CU on the way and no barrier holds them.  (Rows of odd bf16 elements go through
+// registers, one step ahead.)  The product is W h' (classes down,
 // rows across): a lane has scores of one row, and keeps its maximum and sum over all
 // tiles.  f32 operands go into the f32 matrix instruction as they are: at 1/16 of
 // the bf16 rate it still takes less time than W's bytes.
@@ -29,7 +30,8 @@ __device__ __forceinline__ void join2(float &top, float &sum, float t2, float s2
 }
 
 // part[workgroup][row]: the maximum of z log2 e and the sum of its powers of 2.
-template <typename T>
+// B: bytes of W a lane copies at a time, what its rows' alignment allows (2: by registers).
+template <typename T, int B>
 __global__ __launch_bounds__(64 * WAVES, 2) void k_few_stats(XentCall c, int64_t tiles, int32_t steps,
                                                              float2 *__restrict__ part) {
     constexpr int PER = 16 / sizeof(T);              // elements of a chunk of 16 bytes
@@ -48,31 +50,51 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_few_stats(XentCall c, int64_t
         *reinterpret_cast<u32x4 *>(h + q * 16) = *reinterpret_cast<const u32x4 *>(x);
     }
     __syncthreads();
-    // this lane's part of a step's copies: rows lane / 8 + 8 j, the chunk permuted by the
-    // row so that 16 rows x 1 chunk fall on all banks
-    const int lrow = lane >> 3;
+    // The chunks of a row are permuted by the row so that 16 rows x 1 chunk fall on all
+    // banks.
     const auto permute = [](int row) { return ((row >> 1) & 1) * 4 + ((row >> 2) & 3); };
     const int64_t first = (int64_t)blockIdx.x * WAVES + wave, hop = (int64_t)gridDim.x * WAVES;
     const int64_t mine = first < tiles ? (tiles - first + hop - 1) / hop : 0;
     const int64_t total = mine * steps;
     int64_t tile = first;                            // of the next copy
     int32_t step = 0;
-    const auto copy = [&](int to) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int row = lrow + 8 * j;
-            const int64_t v = min(tile * 32 + row, c.classes - 1);
-            int k = (step * 8 + ((lane & 7) ^ permute(row))) * PER;
-            if (k >= c.dim) k = 0;                   // times zeros of h
-            __builtin_amdgcn_global_load_lds(
-                (global_void *)(static_cast<const T *>(c.w) + v * c.w_stride + k),
-                (lds_void *)(buf + to * STEP + j * 1024), 16, 0, 0);
-        }
+    const T *w_all = static_cast<const T *>(c.w);
+    const auto next_step = [&] {
         if (++step == steps) {
             step = 0;
             tile += hop;
         }
     };
+    // Where row `row` of the next step has its element k; behind the row, an element that
+    // zeros of h go with.
+    const auto element = [&](int row, int k) {
+        const int64_t v = min(tile * 32 + row, c.classes - 1);
+        return w_all + v * c.w_stride + (k < c.dim ? k : 0);
+    };
+    constexpr int COPIES = B == 2 ? 0 : 4096 / (64 * B);
+    const auto copy = [&](int to) {
+        if constexpr (B != 2) {
+#pragma unroll
+            for (int j = 0; j < COPIES; ++j) {
+                const int at = j * 64 * B + lane * B, row = at / 128, in = at % 128;
+                const int k = (step * 8 + ((in / 16) ^ permute(row))) * PER + in % 16 / (int)sizeof(T);
+                global_void *from = (global_void *)element(row, k);
+                lds_void *dst = (lds_void *)(buf + to * STEP + j * 64 * B);
+                if constexpr (B == 16) __builtin_amdgcn_global_load_lds(from, dst, 16, 0, 0);
+                else __builtin_amdgcn_global_load_lds(from, dst, 4, 0, 0);
+            }
+            next_step();
+        }
+    };
+    T ahead[B == 2 ? 32 : 1];
+    const auto load = [&] {
+        if constexpr (B == 2) {
+#pragma unroll
+            for (int row = 0; row < 32; ++row) ahead[row] = *element(row, step * 64 + lane);
+            next_step();
+        }
+    };
+    if (B == 2 && total > 0) load();
     if (total > 0) copy(0);
     if (total > 1) copy(1);
     float top = -INFINITY, sum = 0.0f;
@@ -82,11 +104,23 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_few_stats(XentCall c, int64_t
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = 0.0f;
         for (int32_t k = 0; k < steps; ++k, ++t) {
-            // this step's four copies are there when at most the next step's are not
-            if (t + 1 < total) __builtin_amdgcn_s_waitcnt(0x0F74);
-            else __builtin_amdgcn_s_waitcnt(0x0F70);
-            __builtin_amdgcn_sched_barrier(0);
-            if (t + 2 < total) copy(at >= 1 ? at - 1 : BUFS - 1);
+            if constexpr (B == 2) {
+#pragma unroll
+                for (int row = 0; row < 32; ++row)
+                    *reinterpret_cast<T *>(buf + at * STEP + row * 128 +
+                                           ((lane >> 3) ^ permute(row)) * 16 + (lane & 7) * 2) =
+                        ahead[row];
+                if (t + 1 < total) load();
+            } else {
+                // this step's copies are there when at most the next step's are not
+                if (t + 1 < total) {
+                    if constexpr (COPIES == 4) __builtin_amdgcn_s_waitcnt(0x0F74);
+                    else __builtin_amdgcn_s_waitcnt(0x4F70);
+                }
+                else __builtin_amdgcn_s_waitcnt(0x0F70);
+                __builtin_amdgcn_sched_barrier(0);
+                if (t + 2 < total) copy(at >= 1 ? at - 1 : BUFS - 1);
+            }
             const char *w = buf + at * STEP;
             at = at == BUFS - 1 ? 0 : at + 1;
             const int row = lane & 31;
@@ -169,14 +203,14 @@ __global__ __launch_bounds__(64) void k_few_join(XentCall c, int32_t parts,
     c.loss[i] = out ? 0.0f : wt * (lse - (dot + by));
 }
 
-template <typename T> hipError_t run(hipStream_t s, const XentCall &c, char *scratch) {
-    const hipError_t e = allow_all_lds(reinterpret_cast<const void *>(k_few_stats<T>));
+template <typename T, int B> hipError_t run(hipStream_t s, const XentCall &c, char *scratch) {
+    const hipError_t e = allow_all_lds(reinterpret_cast<const void *>(k_few_stats<T, B>));
     if (e != hipSuccess) return e;
     const int64_t tiles = (c.classes + 31) / 32;
     const int32_t steps = (int32_t)((c.dim * sizeof(T) + 127) / 128);
     const uint32_t groups = (uint32_t)std::min<int64_t>(c.num_cus, (tiles + WAVES - 1) / WAVES);
     float2 *part = reinterpret_cast<float2 *>(scratch);
-    hipLaunchKernelGGL((k_few_stats<T>), dim3(groups), dim3(64 * WAVES), LDS_BYTES, s, c, tiles,
+    hipLaunchKernelGGL((k_few_stats<T, B>), dim3(groups), dim3(64 * WAVES), LDS_BYTES, s, c, tiles,
                        steps, part);
     hipLaunchKernelGGL((k_few_join<T>), dim3((uint32_t)c.rows), dim3(64), 0, s, c, (int32_t)groups,
                        part);
@@ -185,18 +219,22 @@ template <typename T> hipError_t run(hipStream_t s, const XentCall &c, char *scr
 
 }  // namespace
 
-// W's rows are copied 16 bytes at a time, and h must fit the LDS beside the buffers.
+// h must fit the LDS beside the buffers.
 bool xent_few(const XentCall &c) {
     const int64_t size = c.bf16 ? 2 : 4;
-    return !c.grad && c.rows <= ROWS && (c.dim * size + 127) / 128 * 128 * ROWS <= H_BYTES &&
-           c.dim * size % 16 == 0 && c.w_stride * size % 16 == 0 &&
-           reinterpret_cast<uintptr_t>(c.w) % 16 == 0;
+    return !c.grad && c.rows <= ROWS && (c.dim * size + 127) / 128 * 128 * ROWS <= H_BYTES;
 }
 
 size_t xent_few_scratch(const XentCall &c) { return (size_t)c.num_cus * ROWS * sizeof(float2); }
 
 hipError_t launch_xent_few(hipStream_t s, const XentCall &c, char *scratch) {
-    return c.bf16 ? run<__bf16>(s, c, scratch) : run<float>(s, c, scratch);
+    const int64_t size = c.bf16 ? 2 : 4;
+    const uint64_t all = (uint64_t)(c.dim * size) | (uint64_t)(c.w_stride * size) |
+                         reinterpret_cast<uintptr_t>(c.w);
+    if (all % 16 == 0)
+        return c.bf16 ? run<__bf16, 16>(s, c, scratch) : run<float, 16>(s, c, scratch);
+    if (all % 4 == 0) return c.bf16 ? run<__bf16, 4>(s, c, scratch) : run<float, 4>(s, c, scratch);
+    return run<__bf16, 2>(s, c, scratch);
 }
 
 }  // namespace mbk

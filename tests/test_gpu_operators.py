@@ -64,9 +64,10 @@ def test_xent_many_rows_or_classes(ctx, kind, n, d, v):
     D.check(x.results(), D.xent_reference(h, w, y, kind, bias, weights))
 
 
-@pytest.mark.parametrize("kind,d", [("f32", 4), ("f32", 64), ("f32", 100), ("f32", 512),
-                                    ("bf16", 8), ("bf16", 64), ("bf16", 200), ("bf16", 1024)])
-@pytest.mark.parametrize("n,v", [(1, 1), (1, 1000), (3, 33), (16, 5000), (32, 70000), (32, 300)])
+@pytest.mark.parametrize("kind,d", [("f32", 1), ("f32", 4), ("f32", 64), ("f32", 99), ("f32", 512),
+                                    ("bf16", 1), ("bf16", 8), ("bf16", 66), ("bf16", 199),
+                                    ("bf16", 200), ("bf16", 1024)])
+@pytest.mark.parametrize("n,v", [(1, 1), (1, 1000), (3, 33), (16, 5000), (32, 30000), (32, 300)])
 def test_xent_loss_of_few_rows(ctx, kind, d, n, v):
     rng, h, w, y = _problem(n + v + d, n, d, v)
     bias = rng.standard_normal(v).astype(np.float32)
@@ -318,7 +319,10 @@ def _experts(seed, rows, k, experts, dropped=0.1, skew=True):
 
 @pytest.mark.parametrize("rows,k,experts", [(0, 2, 4), (1, 1, 1), (1, 3, 8192), (63, 1, 2),
                                             (64, 2, 64), (1000, 1, 4), (4097, 3, 65),
-                                            (70001, 2, 1000), (300000, 1, 8192), (50000, 8, 3)])
+                                            (70001, 2, 1000), (300000, 1, 8192), (50000, 8, 3),
+                                            (16385, 1, 2048), (16385, 1, 2049), (9000, 2, 2100),
+                                            (600001, 1, 5), (1100000, 1, 1500), (263000, 2, 70),
+                                            (17000000, 1, 40)])
 def test_sort_by_expert(ctx, rows, k, experts):
     _, e = _experts(rows + k, rows, k, experts)
     x = D.Experts(ctx, e, experts)
