@@ -1,5 +1,5 @@
-// kernels_xent_few.hip — the many-class loss of up to 32 rows without gradients, as in
-// serving: what bounds it is reading W once, so W is not packed first.
+// kernels_xent_few.hip — the many-class loss of up to 32 rows, as in serving or small
+// batches: what bounds it is reading W (and writing dW), so W is not packed first.
 //
 // h lies in LDS whole, as operands of the matrix instruction.  Each wavefront takes tiles
 // of 32 classes by itself: their rows are copied straight into its own LDS buffers, 128
@@ -9,6 +9,11 @@
 // rows across): a lane has scores of one row, and keeps its maximum and sum over all
 // tiles.  f32 operands go into the f32 matrix instruction as they are: at 1/16 of
 // the bf16 rate it still takes less time than W's bytes.
+//
+// The gradients take a second kernel, with a tile of 32 classes of W in LDS at a time: its
+// scores again, G (32 x 32, f32), dW = G' h written at once, and dh += G W kept in
+// registers over the tiles and summed over the workgroups at the end.  All of its
+// products are of the f32 instruction, so nothing is rounded before the outputs.
 #include <algorithm>
 
 #include "mbk.h"
@@ -174,10 +179,12 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_few_stats(XentCall c, int64_t
     }
 }
 
-// One wavefront a row: the parts joined, and the label's score from h and W.
+// One wavefront a row: the parts joined, and the label's score from h and W.  lse2: the
+// logarithm in base 2, +inf for a row that is out (NULL: not wanted).
 template <typename T>
 __global__ __launch_bounds__(64) void k_few_join(XentCall c, int32_t parts,
-                                                 const float2 *__restrict__ part) {
+                                                 const float2 *__restrict__ part,
+                                                 float *__restrict__ lse2) {
     const int lane = threadIdx.x;
     const int64_t i = blockIdx.x;
     const int32_t y = c.labels[i];
@@ -197,23 +204,217 @@ __global__ __launch_bounds__(64) void k_few_join(XentCall c, int32_t parts,
     }
     if (lane != 0) return;
     const bool none = top == -INFINITY && sum == 0.0f;
-    const float lse = log_sum(top, sum).natural;
+    const LogSum l = log_sum(top, sum);
+    const float lse = l.natural;
     c.lse[i] = lse;
     const bool out = y < 0 || y >= c.classes || wt == 0.0f || none;
     c.loss[i] = out ? 0.0f : wt * (lse - (dot + by));
+    if (lse2) lse2[i] = out ? INFINITY : l.base2;
 }
 
+// ---- gradients -------------------------------------------------------------------------
+// Element (x, k) of h or of a tile of W in LDS: chunks of 16 bytes of k, each with its 32
+// rows; the chunks 528 bytes apart, so that reads along x and along k fall on all banks.
+constexpr int CHUNK_BYTES = ROWS * 16 + 16;
+constexpr int GRAD_WAVES = 8, GRAD_BLOCKS = 4;       // blocks of 32 columns a wavefront keeps
+constexpr int G_STRIDE = 33;
+template <typename T>
+__device__ __forceinline__ float element_of(const char *m, int x, int k) {
+    constexpr int PER = 16 / sizeof(T);
+    return (float)*reinterpret_cast<const T *>(m + k / PER * CHUNK_BYTES + x * 16 +
+                                               k % PER * (int)sizeof(T));
+}
+// Rows [0, 32) of a matrix into LDS: row(x) gives row x, or NULL for zeros.
+template <typename T, class Row>
+__device__ __forceinline__ void stage(char *m, int chunks, int dim, bool aligned, Row row) {
+    constexpr int PER = 16 / sizeof(T);
+    for (int q = threadIdx.x; q < chunks * ROWS; q += 64 * GRAD_WAVES) {
+        const int x = q / chunks, c = q % chunks;
+        const T *from = row(x);
+        u32x4 v = {0, 0, 0, 0};
+        if (from && aligned) {
+            v = *reinterpret_cast<const u32x4 *>(from + c * PER);
+        } else if (from) {
+            T e[PER];
+#pragma unroll
+            for (int i = 0; i < PER; ++i)
+                e[i] = c * PER + i < dim ? from[c * PER + i] : (T)0.0f;
+            __builtin_memcpy(&v, e, sizeof v);
+        }
+        *reinterpret_cast<u32x4 *>(m + c * CHUNK_BYTES + x * 16) = v;
+    }
+}
+
+// part_dh[workgroup][row][dim].
+template <typename T>
+__global__ __launch_bounds__(64 * GRAD_WAVES, 2) void k_few_grad(XentCall c, int64_t tiles,
+                                                                 int32_t chunks, bool aligned,
+                                                                 const float *__restrict__ lse2,
+                                                                 float *__restrict__ part_dh) {
+    constexpr int PER = 16 / sizeof(T);
+    extern __shared__ char lds[];
+    char *h = lds, *w = lds + chunks * CHUNK_BYTES;
+    float *sums = reinterpret_cast<float *>(w + chunks * CHUNK_BYTES);   // [4][16][64]
+    float *g = sums + 4 * 16 * 64;                                       // [row][class]
+    const int lane = threadIdx.x & 63, half = lane >> 5, l = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int blocks = (c.dim + 31) / 32;
+    // a row that is out is zeros here: what it holds reaches nothing
+    stage<T>(h, chunks, c.dim, false, [&](int i) -> const T * {
+        return i < c.rows && lse2[i] != INFINITY
+                   ? static_cast<const T *>(c.h) + i * c.h_stride : nullptr;
+    });
+    const float l2 = l < c.rows ? lse2[l] : INFINITY;
+    const int32_t label = l < c.rows ? c.labels[l] : -1;
+    const float wt = l2 == INFINITY ? 0.0f : c.weights ? c.weights[l] : 1.0f;
+    f32x16 dh[GRAD_BLOCKS];
+#pragma unroll
+    for (int b = 0; b < GRAD_BLOCKS; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) dh[b][r] = 0.0f;
+    for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
+        const int64_t v0 = t * 32;
+        __syncthreads();                             // the last tile's reads
+        stage<T>(w, chunks, c.dim, aligned, [&](int x) -> const T * {
+            return v0 + x < c.classes && !(c.bias && c.bias[v0 + x] == -INFINITY)
+                       ? static_cast<const T *>(c.w) + (v0 + x) * c.w_stride : nullptr;
+        });
+        __syncthreads();
+        // scores, classes down and rows across, k in parts of the wavefronts
+        f32x16 s;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = 0.0f;
+        for (int q = wave; q < (chunks + 1) / 2; q += GRAD_WAVES) {
+            const int at = 2 * q + half;
+            u32x4 a = {0, 0, 0, 0}, b = {0, 0, 0, 0};
+            if (at < chunks) {
+                a = *reinterpret_cast<const u32x4 *>(w + at * CHUNK_BYTES + l * 16);
+                b = *reinterpret_cast<const u32x4 *>(h + at * CHUNK_BYTES + l * 16);
+            }
+            T x[PER], y[PER];
+            __builtin_memcpy(x, &a, 16);
+            __builtin_memcpy(y, &b, 16);
+#pragma unroll
+            for (int e = 0; e < PER; ++e)
+                s = __builtin_amdgcn_mfma_f32_32x32x2f32((float)x[e], (float)y[e], s, 0, 0, 0);
+        }
+        // their sum over the wavefronts, in three rounds of halves, in the first one
+#pragma unroll
+        for (int n = GRAD_WAVES / 2; n > 0; n >>= 1) {
+            if (wave >= n && wave < 2 * n)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) sums[((wave - n) * 16 + r) * 64 + lane] = s[r];
+            __syncthreads();
+            if (wave < n)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[r] += sums[(wave * 16 + r) * 64 + lane];
+            __syncthreads();
+        }
+        if (wave == 0)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int x = (r >> 2) * 8 + half * 4 + (r & 3);
+                const int64_t v = v0 + x;
+                float b = -INFINITY;
+                if (v < c.classes) b = c.bias ? c.bias[v] : 0.0f;
+                float p = 0.0f;
+                if (l2 != INFINITY && b != -INFINITY) {
+                    p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], LOG2E, b * LOG2E - l2));
+                    if (v == label) p -= 1.0f;
+                    p *= wt;
+                }
+                g[l * G_STRIDE + x] = p;
+            }
+        __syncthreads();
+        if (c.dbias && threadIdx.x < 32 && v0 + threadIdx.x < c.classes) {
+            float sum = 0.0f;
+            for (int i = 0; i < ROWS; ++i) sum += g[i * G_STRIDE + threadIdx.x];
+            c.dbias[v0 + threadIdx.x] = sum;
+        }
+        // dW and dh, blocks of 32 columns in turn
+        if (c.dw)
+            for (int b = wave; b < blocks; b += GRAD_WAVES) {
+                const int j = min(b * 32 + l, chunks * PER - 1);
+                f32x16 o;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[r] = 0.0f;
+#pragma unroll
+                for (int k = 0; k < ROWS; k += 2)
+                    o = __builtin_amdgcn_mfma_f32_32x32x2f32(g[(k + half) * G_STRIDE + l],
+                                                             element_of<T>(h, k + half, j), o, 0, 0,
+                                                             0);
+                if (b * 32 + l < c.dim)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int64_t v = v0 + (r >> 2) * 8 + half * 4 + (r & 3);
+                        if (v < c.classes)
+                            static_cast<T *>(c.dw)[v * c.w_stride + b * 32 + l] = (T)o[r];
+                    }
+            }
+        if (c.dh)
+#pragma unroll
+            for (int n = 0; n < GRAD_BLOCKS; ++n) {
+                const int b = wave + n * GRAD_WAVES;
+                if (b >= blocks) break;
+                const int j = min(b * 32 + l, chunks * PER - 1);
+#pragma unroll
+                for (int k = 0; k < 32; k += 2)
+                    dh[n] = __builtin_amdgcn_mfma_f32_32x32x2f32(g[l * G_STRIDE + k + half],
+                                                                 element_of<T>(w, k + half, j),
+                                                                 dh[n], 0, 0, 0);
+            }
+    }
+    if (!c.dh) return;
+#pragma unroll
+    for (int n = 0; n < GRAD_BLOCKS; ++n) {
+        const int j = (wave + n * GRAD_WAVES) * 32 + l;
+        if (j >= c.dim) continue;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int i = (r >> 2) * 8 + half * 4 + (r & 3);
+            if (i < c.rows) part_dh[((int64_t)blockIdx.x * c.rows + i) * c.dim + j] = dh[n][r];
+        }
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void k_few_join_dh(XentCall c, int32_t parts,
+                                                     const float *__restrict__ part) {
+    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, all = c.rows * c.dim;
+    if (at >= all) return;
+    float sum = 0.0f;
+#pragma unroll 8
+    for (int p = 0; p < parts; ++p) sum += part[p * all + at];
+    static_cast<T *>(c.dh)[at / c.dim * c.h_stride + at % c.dim] = (T)sum;
+}
+
+// Scratch: the parts of the rows, lse2, the parts of dh.
+size_t part_bytes(const XentCall &c) { return (size_t)c.num_cus * ROWS * sizeof(float2); }
+
 template <typename T, int B> hipError_t run(hipStream_t s, const XentCall &c, char *scratch) {
-    const hipError_t e = allow_all_lds(reinterpret_cast<const void *>(k_few_stats<T, B>));
+    hipError_t e = allow_all_lds(reinterpret_cast<const void *>(k_few_stats<T, B>));
+    if (e == hipSuccess) e = allow_all_lds(reinterpret_cast<const void *>(k_few_grad<T>));
     if (e != hipSuccess) return e;
     const int64_t tiles = (c.classes + 31) / 32;
     const int32_t steps = (int32_t)((c.dim * sizeof(T) + 127) / 128);
-    const uint32_t groups = (uint32_t)std::min<int64_t>(c.num_cus, (tiles + WAVES - 1) / WAVES);
+    uint32_t groups = (uint32_t)std::min<int64_t>(c.num_cus, (tiles + WAVES - 1) / WAVES);
     float2 *part = reinterpret_cast<float2 *>(scratch);
+    float *lse2 = reinterpret_cast<float *>(scratch + part_bytes(c));
     hipLaunchKernelGGL((k_few_stats<T, B>), dim3(groups), dim3(64 * WAVES), LDS_BYTES, s, c, tiles,
                        steps, part);
     hipLaunchKernelGGL((k_few_join<T>), dim3((uint32_t)c.rows), dim3(64), 0, s, c, (int32_t)groups,
-                       part);
+                       part, c.grad ? lse2 : nullptr);
+    if (!c.grad) return hipGetLastError();
+    constexpr int PER = 16 / sizeof(T);
+    const int32_t chunks = (c.dim + PER - 1) / PER;
+    float *part_dh = lse2 + ROWS;
+    groups = (uint32_t)std::min<int64_t>(c.num_cus, tiles);
+    const size_t lds = (size_t)2 * chunks * CHUNK_BYTES + 4 * (4 * 16 * 64 + ROWS * G_STRIDE);
+    hipLaunchKernelGGL((k_few_grad<T>), dim3(groups), dim3(64 * GRAD_WAVES), lds, s, c, tiles,
+                       chunks, B == 16, lse2, part_dh);
+    if (c.dh)
+        hipLaunchKernelGGL((k_few_join_dh<T>), dim3((uint32_t)((c.rows * c.dim + 255) / 256)),
+                           dim3(256), 0, s, c, (int32_t)groups, part_dh);
     return hipGetLastError();
 }
 
@@ -222,10 +423,12 @@ template <typename T, int B> hipError_t run(hipStream_t s, const XentCall &c, ch
 // h must fit the LDS beside the buffers.
 bool xent_few(const XentCall &c) {
     const int64_t size = c.bf16 ? 2 : 4;
-    return !c.grad && c.rows <= ROWS && (c.dim * size + 127) / 128 * 128 * ROWS <= H_BYTES;
+    return c.rows <= ROWS && (c.dim * size + 127) / 128 * 128 * ROWS <= H_BYTES;
 }
 
-size_t xent_few_scratch(const XentCall &c) { return (size_t)c.num_cus * ROWS * sizeof(float2); }
+size_t xent_few_scratch(const XentCall &c) {
+    return part_bytes(c) + 4 * ROWS + (c.grad ? (size_t)4 * c.num_cus * c.rows * c.dim : 0);
+}
 
 hipError_t launch_xent_few(hipStream_t s, const XentCall &c, char *scratch) {
     const int64_t size = c.bf16 ? 2 : 4;

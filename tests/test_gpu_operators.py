@@ -95,6 +95,49 @@ def test_xent_loss_of_few_rows(ctx, kind, d, n, v):
     D.check(x.results(False), D.xent_reference(h, w, y, kind), ("loss", "lse"))
 
 
+@pytest.mark.parametrize("kind,d", [("f32", 1), ("f32", 31), ("f32", 96), ("f32", 130), ("f32", 512),
+                                    ("bf16", 1), ("bf16", 40), ("bf16", 66), ("bf16", 199),
+                                    ("bf16", 1024)])
+@pytest.mark.parametrize("n,v", [(1, 1), (1, 1000), (7, 33), (32, 9000), (31, 300)])
+def test_xent_gradient_of_few_rows(ctx, kind, d, n, v):
+    rng, h, w, y = _problem(n + 3 * v + d, n, d, v)
+    bias = rng.standard_normal(v).astype(np.float32)
+    weights = (rng.random(n) + 0.5).astype(np.float32)
+    closed = rng.random(v) < 0.2
+    closed[0] = False
+    open_classes = np.flatnonzero(~closed)
+    y = open_classes[rng.integers(0, open_classes.size, n)].astype(np.int32)
+    bias[closed] = -np.inf
+    out = n // 2
+    if n > 1:
+        y[out] = -1
+        weights[n // 3] = 0
+    want = D.xent_reference(h, w, y, kind, bias, weights)
+    w[closed] = np.nan                   # not read
+    if n > 1:
+        h[out] = np.inf
+    x = D.Xent(ctx, h, w, y, kind, bias, weights, h_pad=3, w_pad=8)
+    x.grad()
+    got = x.results()
+    first = {key: np.array(value) for key, value in got.items()}
+    if n > 1:
+        keep = np.arange(n) != out
+        got["lse"], want["lse"] = got["lse"][keep], tuple(t[keep] for t in want["lse"])
+        assert not got["dh"][out].any() and not got["dh"][n // 3].any()
+    D.check(got, want)
+    assert not got["dw"][closed].any() and not got["db"][closed].any()
+    x.grad()
+    for key, value in x.results().items():
+        assert np.array_equal(np.array(value), first[key], equal_nan=True)
+    # one gradient alone, without bias and weights
+    _, h, w, y = _problem(n + 3 * v + d, n, d, v)
+    want = D.xent_reference(h, w, y, kind)
+    for alone in ("dh", "dw", "db"):
+        x = D.Xent(ctx, h, w, y, kind)
+        x.grad(**{key: key == alone for key in ("dh", "dw", "db")})
+        D.check(x.results(), want, ("loss", "lse", alone))
+
+
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
 @pytest.mark.parametrize("h_pad,w_pad", [(0, 0), (8, 0), (0, 8), (1, 2)])
 def test_xent_strides_and_no_bias(ctx, kind, h_pad, w_pad):
