@@ -202,10 +202,14 @@ __global__ __launch_bounds__(64 * SORT_WAVES) void k_expert_place(
 // assignments to 64 experts: 18 us by 16 workgroups, 10 by 64).
 constexpr int CHUNK_WAVES = 8;
 template <int R> constexpr int CHUNK = R * CHUNK_WAVES * 64;
-constexpr int64_t FEW_SLOTS = (int64_t)1 << 19;
+// (1M assignments to 64 experts: 24 us by 16, 18 by 4; 4M to 1000: 41 and 61.)
+constexpr int64_t FEW_SLOTS = (int64_t)1 << 20;
 constexpr int32_t CHUNK_EXPERTS = 2048;
-// Counters a place kernel sums up by itself, without the kernels that scan them.
+// Counters a place kernel sums up by itself, without the two kernels that scan them, and the
+// experts whose sums its wavefronts can take one after another (131k assignments: 4 experts
+// 14 us, 20 with the scan, 128 18 and 20; 256 27 and 20; 20k to 512 46 and 20).
 constexpr int64_t DIRECT_COUNTERS = 8192;
+constexpr int32_t DIRECT_EXPERTS = 128;
 
 // table[e * units + u]: assignments of workgroup u to expert e.
 template <int R>
@@ -971,7 +975,7 @@ hipError_t sort_chunks(hipStream_t s, const ExpertPlan &p, const SortShape &sh, 
                        (CHUNK_WAVES + CHUNK<R> + (size_t)(CHUNK_WAVES + 2) * p.experts);
     hipLaunchKernelGGL((k_expert_count_chunks<R>), g, b, sizeof(uint32_t) * p.experts, s, p.expert,
                        slots, p.experts, sh.per, sh.units, table);
-    if ((int64_t)p.experts * sh.units <= DIRECT_COUNTERS) {
+    if (p.experts <= DIRECT_EXPERTS && (int64_t)p.experts * sh.units <= DIRECT_COUNTERS) {
         hipLaunchKernelGGL((k_expert_place_chunks<R, true>), g, b, lds, s, p.expert, slots,
                            p.experts, bits, sh.per, sh.units, table, p.offsets, p.source, p.slot);
     } else {

@@ -787,9 +787,32 @@ uint32_t blocks(int64_t x, int64_t per) { return (uint32_t)((x + per - 1) / per)
 constexpr int64_t PIECE_ROWS = 32768;
 constexpr int64_t PIECE_BYTES = (int64_t)512 << 20;
 
-// Wide tiles where they fill the chip.
-bool wide_tiles(int64_t m, int64_t n, int64_t splits, int num_cus) {
-    return up(m, 256) / 256 * (up(n, 256) / 256) * splits >= num_cus;
+// What a k step of a workgroup of 256 x 256 takes, in us, at the rate that the large products
+// reach (1.1 PFLOP/s), and one of 128 x 128 with another beside it on its CU: half of a
+// quarter of the CU's work each, at 0.85 of the rate (8191 x 768 x 50000 bf16: 0.62 ms by wide
+// tiles, 0.70 by narrow ones; 16384 x 1024 x 65536 with gradients 8.7 and 10.4).
+double step_us(bool wide, int P) { return (P == 1 ? 1.95 : 2.9) * (wide ? 1.0 : 0.5 / 0.85); }
+int64_t slots_of(bool wide, int num_cus) { return (wide ? 1 : 2) * (int64_t)num_cus; }
+
+// Workgroups that share a tile of rows: one wide workgroup a CU or two narrow ones.
+int32_t splits_of(bool wide, int64_t row_tiles, int64_t class_tiles, int num_cus) {
+    return (int32_t)std::max<int64_t>(1, std::min(class_tiles, slots_of(wide, num_cus) / row_tiles));
+}
+
+// Wide tiles where the tiles that a workgroup gets then take less time: padding and the last
+// round, in which few have one, count (f32, loss: 1024 x 512 x 16384 117 us wide, 124
+// narrow; 300 x 512 x 33000 148 and 127; 400 x 1024 x 33000 250 and 217).
+bool wide_tiles(int64_t rows, int64_t classes, int num_cus) {
+    double us[2];
+    for (const bool wide : {false, true}) {
+        const int64_t t = wide ? 256 : 128;
+        const int64_t row_tiles = up(rows, t) / t, class_tiles = up(classes, t) / t;
+        const int64_t splits = splits_of(wide, row_tiles, class_tiles, num_cus);
+        const int64_t slots = slots_of(wide, num_cus);
+        us[wide] = step_us(wide, 1) * (double)((class_tiles + splits - 1) / splits) *
+                   (double)((row_tiles * splits + slots - 1) / slots);
+    }
+    return us[1] <= us[0];
 }
 
 // How a product over k of m x n is cut.
@@ -797,27 +820,34 @@ struct Cut {
     bool wide;
     int32_t tiles_m, tiles_n, splits;
 };
-Cut cut_of(bool wide, int64_t m, int64_t n, int64_t steps, int num_cus) {
-    // not with many columns of wide tiles wasted
-    wide = wide && up(n, 256) * 5 <= up(n, 128) * 6 &&
-           wide_tiles(m, n, std::max<int64_t>(1, steps / 16), num_cus);
-    const int64_t t = wide ? 256 : 128;
-    Cut c{wide, (int32_t)(m / t), (int32_t)(up(n, t) / t), 1};
-    const int64_t tiles = (int64_t)c.tiles_m * c.tiles_n, slots = (wide ? 1 : 2) * (int64_t)num_cus;
-    // too few tiles: k is split, 8 steps a workgroup at least
-    c.splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>({slots / tiles, steps / 8, 64}));
-    return c;
-}
-
-// Workgroups that share a tile of rows: one wide workgroup a CU or two narrow ones.
-template <class C> int32_t splits_of(int64_t row_tiles, int64_t class_tiles, int num_cus) {
-    const int64_t slots = (C::T == 256 ? 1 : 2) * (int64_t)num_cus;
-    return (int32_t)std::max<int64_t>(1, std::min(class_tiles, slots / row_tiles));
+// The least time by the steps of the workgroups' rounds, 3 us for a workgroup's start and
+// end, and what the parts of a split k take to be written, read and joined.  (f32, with
+// gradients: 256 x 512 x 40000 360 us, 1115 without splits.)
+Cut cut_of(bool wide_allowed, int P, int64_t m, int64_t n, int64_t steps, int num_cus) {
+    Cut best{};
+    double least = 1e300;
+    for (const bool wide : {true, false}) {
+        if (wide && !wide_allowed) continue;
+        const int64_t t = wide ? 256 : 128, slots = slots_of(wide, num_cus);
+        const int64_t tiles_m = m / t, tiles_n = up(n, t) / t, tiles = tiles_m * tiles_n;
+        const int64_t most = std::max<int64_t>(
+            1, std::min<int64_t>({steps / 8, 64, 2 * slots / tiles}));
+        for (int64_t s = 1; s <= most; ++s) {
+            const double join = s == 1 ? 0.0 : 4.0 + (double)(s * m) * (double)n * 8.0 / 4.5e6;
+            const double us = (double)((tiles * s + slots - 1) / slots) *
+                                  ((double)((steps + s - 1) / s) * step_us(wide, P) + 3.0) + join;
+            if (us < least) {
+                least = us;
+                best = {wide, (int32_t)tiles_m, (int32_t)tiles_n, (int32_t)s};
+            }
+        }
+    }
+    return best;
 }
 
 struct Plan {
     int P;
-    bool wide;
+    bool wide, wide_g;           // tiles of the statistics (and padding), of G
     int64_t n_pad, v_pad, ld, piece_rows, piece_classes;
     int32_t splits;
     Cut dh, dw;                  // of whole pieces
@@ -827,14 +857,13 @@ struct Plan {
 Plan plan_of(const XentCall &c) {
     Plan p{};
     p.P = c.bf16 ? 1 : 2;
-    p.wide = c.rows > 128 && wide_tiles(c.rows, c.classes, 1, c.num_cus);
+    p.wide = wide_tiles(c.rows, c.classes, c.num_cus);
     const int64_t t = p.wide ? 256 : 128, step = 64 / p.P;
     p.n_pad = up(c.rows, t);
     p.v_pad = up(c.classes, t);
     p.ld = up(c.dim, LD_PAD);
     const int64_t row_tiles = p.n_pad / t, class_tiles = p.v_pad / t;
-    p.splits = p.wide ? splits_of<Wide>(row_tiles, class_tiles, c.num_cus)
-                      : splits_of<Narrow>(row_tiles, class_tiles, c.num_cus);
+    p.splits = splits_of(p.wide, row_tiles, class_tiles, c.num_cus);
     p.piece_rows = std::min(p.n_pad, PIECE_ROWS);
     p.piece_classes = std::min(
         p.v_pad, std::max<int64_t>(t, PIECE_BYTES / (2 * p.P * p.piece_rows) / t * t));
@@ -856,11 +885,12 @@ Plan plan_of(const XentCall &c) {
     p.lse = take((size_t)4 * p.n_pad);
     p.part = take((size_t)16 * p.splits * p.n_pad);
     if (c.grad) {
+        p.wide_g = p.wide && wide_tiles(p.piece_rows, p.piece_classes, c.num_cus);
         p.hg = take((size_t)2 * p.P * p.n_pad * p.ld + past);
         if (c.dbias) p.db = take((size_t)4 * (p.piece_rows / 64) * p.v_pad);
         p.g = take((size_t)2 * p.P * p.piece_rows * p.piece_classes);
-        p.dh = cut_of(p.wide, p.piece_rows, c.dim, p.piece_classes / step, c.num_cus);
-        p.dw = cut_of(p.wide, p.piece_classes, c.dim, p.piece_rows / step, c.num_cus);
+        p.dh = cut_of(p.wide, p.P, p.piece_rows, c.dim, p.piece_classes / step, c.num_cus);
+        p.dw = cut_of(p.wide, p.P, p.piece_classes, c.dim, p.piece_rows / step, c.num_cus);
         if (p.dh.splits > 1 || p.piece_classes < p.v_pad)
             p.dh_acc = take((size_t)4 * p.dh.splits * p.n_pad * p.ld);
         if (p.dw.splits > 1 || p.piece_rows < p.n_pad)
@@ -897,7 +927,7 @@ template <int P, class C>
 void launch_g(hipStream_t s, const XentPack &k, int64_t v0, int64_t nv, int64_t r0, int64_t nr,
               int64_t plane, int num_cus, const float *lse2, u16 *g, float *part_db) {
     const int32_t rt = (int32_t)(nr / C::T), vt = (int32_t)(nv / C::T);
-    const int32_t splits = splits_of<C>(rt, vt, num_cus);
+    const int32_t splits = splits_of(C::T == 256, rt, vt, num_cus);
     hipLaunchKernelGGL((k_xent_g<P, C>), dim3((uint32_t)rt * splits), dim3(C::WAVES * 64),
                        (LDS_TILES<P, C>), s, k, v0, r0, nr, plane, rt, vt, splits, lse2, g, part_db);
 }
@@ -955,7 +985,7 @@ hipError_t run(hipStream_t s, const XentCall &c, const Plan &p, char *m) {
         for (int64_t r0 = 0; r0 < k.n_pad; r0 += p.piece_rows) {
             const int64_t nv = std::min(p.piece_classes, k.v_pad - v0);
             const int64_t nr = std::min(p.piece_rows, k.n_pad - r0);
-            if (p.wide) launch_g<P, Wide>(s, k, v0, nv, r0, nr, plane, c.num_cus, lse2, g, part_db);
+            if (p.wide_g) launch_g<P, Wide>(s, k, v0, nv, r0, nr, plane, c.num_cus, lse2, g, part_db);
             else launch_g<P, Narrow>(s, k, v0, nv, r0, nr, plane, c.num_cus, lse2, g, part_db);
             const Operand ag{g, plane, nr};
             if (c.dh)

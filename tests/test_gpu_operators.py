@@ -95,6 +95,19 @@ def test_xent_loss_of_few_rows(ctx, kind, d, n, v):
     D.check(x.results(False), D.xent_reference(h, w, y, kind), ("loss", "lse"))
 
 
+# tiles of 256 x 256 in the scores, and in dh or in dW
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("n,v", [(16300, 1000), (1000, 16300)])
+def test_xent_wide_tiles(ctx, kind, n, v):
+    rng, h, w, y = _problem(n + 5 * v, n, 1000, v)
+    bias = rng.standard_normal(v).astype(np.float32)
+    bias[1::5] = -np.inf
+    y[::17] = -1
+    x = D.Xent(ctx, h, w, y, kind, bias)
+    x.grad()
+    D.check(x.results(), D.xent_reference(h, w, y, kind, bias))
+
+
 @pytest.mark.parametrize("kind,d", [("f32", 1), ("f32", 31), ("f32", 96), ("f32", 130), ("f32", 512),
                                     ("bf16", 1), ("bf16", 40), ("bf16", 66), ("bf16", 199),
                                     ("bf16", 1024)])
