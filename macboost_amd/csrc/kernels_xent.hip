@@ -42,7 +42,7 @@ constexpr int LD_PAD = 128;              // operands' rows are padded to it
 constexpr float G_SCALE = 32768.0f;      // |G / w| <= 1 as f16 terms
 
 __global__ void k_xent_init(XentCtl *ctl) {
-    ctl->w_max = ctl->hg_max = ctl->open = 0;
+    clear(ctl);
 }
 
 template <typename T> __device__ __forceinline__ float load_f32(const void *p, int64_t i) {
@@ -91,19 +91,11 @@ __device__ __forceinline__ void pack8(const float (&x)[8], int s, u16 *to, int64
     *reinterpret_cast<u16x8 *>(to) = hi;
     if (sizeof(T) == 4) *reinterpret_cast<u16x8 *>(to + plane) = lo;
 }
-// The workgroup's largest goes to *max: few atomics on one word.
-__device__ __forceinline__ void raise_by_block(uint32_t *max, uint32_t v) {
-    __shared__ uint32_t most[4];
-    v = wave_max(v);
-    if ((threadIdx.x & 63) == 0) most[threadIdx.x >> 6] = v;
-    __syncthreads();
-    if (threadIdx.x == 0) raise(max, ::max(::max(most[0], most[1]), ::max(most[2], most[3])));
-}
-
+constexpr int MAX_WAVES = 8;              // of the kernels that find a maximum
 // The kernels that prepare take a wavefront a row, over the rows in turns.
 // Classes: the padded bias, whether any is offered, the largest |W|.
 template <typename T>
-__global__ __launch_bounds__(256) void k_xent_classes(XentPack k, const void *w, int64_t stride,
+__global__ __launch_bounds__(64 * MAX_WAVES) void k_xent_classes(XentPack k, const void *w, int64_t stride,
                                                       const float *__restrict__ bias) {
     const int lane = threadIdx.x & 63;
     const int align = alignment<T>(w, stride);
@@ -111,8 +103,8 @@ __global__ __launch_bounds__(256) void k_xent_classes(XentPack k, const void *w,
     bool any = false;
     // four rows at a time, so that as many loads are on the way
     constexpr int ROWS = 4;
-    const int64_t hop = (int64_t)gridDim.x * 4;
-    for (int64_t v0 = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); v0 < k.v_pad; v0 += ROWS * hop) {
+    const int64_t hop = (int64_t)gridDim.x * MAX_WAVES;
+    for (int64_t v0 = (int64_t)blockIdx.x * MAX_WAVES + (threadIdx.x >> 6); v0 < k.v_pad; v0 += ROWS * hop) {
         int32_t d[ROWS];
 #pragma unroll
         for (int q = 0; q < ROWS; ++q) {
@@ -134,14 +126,14 @@ __global__ __launch_bounds__(256) void k_xent_classes(XentPack k, const void *w,
         }
     }
     if (any && !k.ctl->open) k.ctl->open = 1u;
-    raise_by_block(&k.ctl->w_max, m);
+    raise_by_block<MAX_WAVES>(k.ctl->w_max, m);
 }
 
 template <typename T>
 __global__ __launch_bounds__(256) void k_xent_pack_w(XentPack k, const void *w, int64_t stride) {
     const int lane = threadIdx.x & 63;
     const int align = alignment<T>(w, stride);
-    const int s = scale_exp(k.ctl->w_max);
+    const int s = scale_exp(largest(k.ctl->w_max));
     constexpr int ROWS = 2;
     const int64_t hop = (int64_t)gridDim.x * 4;
     for (int64_t v0 = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); v0 < k.v_pad; v0 += ROWS * hop) {
@@ -165,16 +157,16 @@ __global__ __launch_bounds__(256) void k_xent_pack_w(XentPack k, const void *w, 
 // Rows: label and weight (-1 and 0 where the row is out), h scaled by row.  A row that
 // is out and not finite is packed as zeros, its label -2.
 template <typename T>
-__global__ __launch_bounds__(256) void k_xent_rows(XentPack k, const void *h, int64_t stride,
+__global__ __launch_bounds__(64 * MAX_WAVES) void k_xent_rows(XentPack k, const void *h, int64_t stride,
                                                    const int32_t *__restrict__ labels,
                                                    const float *__restrict__ weights) {
     const int lane = threadIdx.x & 63;
     const int align = alignment<T>(h, stride);
     const bool any = k.ctl->open;
-    const int sw = scale_exp(k.ctl->w_max);
+    const int sw = scale_exp(largest(k.ctl->w_max));
     uint32_t hg = 0;
-    for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < k.n_pad;
-         i += (int64_t)gridDim.x * 4) {
+    for (int64_t i = (int64_t)blockIdx.x * MAX_WAVES + (threadIdx.x >> 6); i < k.n_pad;
+         i += (int64_t)gridDim.x * MAX_WAVES) {
         int32_t y = i < k.n ? labels[i] : -1, d = i < k.n ? k.d : 0;
         float wt = i < k.n ? (weights ? weights[i] : 1.0f) : 0.0f;
         const bool out = y < 0 || y >= k.v || wt == 0.0f || !any;
@@ -211,7 +203,7 @@ __global__ __launch_bounds__(256) void k_xent_rows(XentPack k, const void *h, in
             pack8<T>(x, s, k.h + i * k.ld + f, k.n_pad * k.ld);
         }
     }
-    raise_by_block(&k.ctl->hg_max, hg);
+    raise_by_block<MAX_WAVES>(k.ctl->hg_max, hg);
 }
 
 // h as dW's product takes it, times the row's weight and with one scale for all rows
@@ -220,7 +212,7 @@ template <typename T>
 __global__ __launch_bounds__(256) void k_xent_pack_hg(XentPack k, const void *h, int64_t stride) {
     const int lane = threadIdx.x & 63;
     const int align = alignment<T>(h, stride);
-    const int s = scale_exp(k.ctl->hg_max);
+    const int s = scale_exp(largest(k.ctl->hg_max));
     for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < k.n_pad;
          i += (int64_t)gridDim.x * 4) {
         const int32_t d = k.label[i] >= 0 ? k.d : 0;
@@ -682,7 +674,7 @@ struct Out {
     bool classes;                // dW: rows whose bias is -inf are 0; dh: times weight
 };
 __device__ __forceinline__ float out_scale(const XentPack &k, bool classes) {
-    return ldexpf(1.0f, -scale_exp(classes ? k.ctl->hg_max : k.ctl->w_max)) / G_SCALE;
+    return ldexpf(1.0f, -scale_exp(largest(classes ? k.ctl->hg_max : k.ctl->w_max))) / G_SCALE;
 }
 template <int P>
 __device__ __forceinline__ void put(const XentPack &k, const Out &o, int64_t m, int64_t n, float v,
@@ -964,14 +956,19 @@ hipError_t run(hipStream_t s, const XentCall &c, const Plan &p, char *m) {
         const hipError_t e = allow_all_lds(f);
         if (e != hipSuccess) return e;
     }
-    hipLaunchKernelGGL(k_xent_init, dim3(1), dim3(1), 0, s, k.ctl);
+    hipLaunchKernelGGL(k_xent_init, dim3(1), dim3(64), 0, s, k.ctl);
     const auto grid = [&](int64_t rows) {
         return dim3(std::min<uint32_t>(blocks(rows, 4), 8 * (uint32_t)c.num_cus));
     };
-    hipLaunchKernelGGL((k_xent_classes<T>), grid(k.v_pad), b, 0, s, k, c.w, c.w_stride, c.bias);
+    const auto max_grid = [&](int64_t rows) {
+        return dim3(std::min<uint32_t>(blocks(rows, MAX_WAVES), 4 * (uint32_t)c.num_cus));
+    };
+    const dim3 max_block(64 * MAX_WAVES);
+    hipLaunchKernelGGL((k_xent_classes<T>), max_grid(k.v_pad), max_block, 0, s, k, c.w, c.w_stride,
+                       c.bias);
     hipLaunchKernelGGL((k_xent_pack_w<T>), grid(k.v_pad), b, 0, s, k, c.w, c.w_stride);
-    hipLaunchKernelGGL((k_xent_rows<T>), grid(k.n_pad), b, 0, s, k, c.h, c.h_stride, c.labels,
-                       c.weights);
+    hipLaunchKernelGGL((k_xent_rows<T>), max_grid(k.n_pad), max_block, 0, s, k, c.h, c.h_stride,
+                       c.labels, c.weights);
     if (p.wide) launch_stats<P, Wide>(s, k, p.splits, part);
     else launch_stats<P, Narrow>(s, k, p.splits, part);
     hipLaunchKernelGGL((k_xent_join<T>), dim3(blocks(k.n_pad, 4)), b, 0, s, k, c, 2 * p.splits,

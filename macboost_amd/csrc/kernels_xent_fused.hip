@@ -59,7 +59,7 @@ __device__ __forceinline__ int wq_exp(uint32_t hg_max) {
 }
 
 __global__ void k_fused_init(XentCtl *ctl) {
-    ctl->w_max = ctl->hg_max = ctl->open = 0;
+    clear(ctl);
 }
 
 template <typename T> __device__ __forceinline__ float load_f32(const void *p, int64_t i) {
@@ -75,15 +75,6 @@ __device__ __forceinline__ void load4(const void *p, int64_t row, int f, int d, 
 __device__ __forceinline__ uint32_t finite_max(const float (&x)[4]) {
     return max(max(finite_bits(x[0]), finite_bits(x[1])), max(finite_bits(x[2]), finite_bits(x[3])));
 }
-// The workgroup's largest goes to *max: few atomics on one word.
-__device__ __forceinline__ void raise_by_block(uint32_t *max, uint32_t v) {
-    __shared__ uint32_t most[4];
-    v = wave_max(v);
-    if ((threadIdx.x & 63) == 0) most[threadIdx.x >> 6] = v;
-    __syncthreads();
-    if (threadIdx.x == 0) raise(max, ::max(::max(most[0], most[1]), ::max(most[2], most[3])));
-}
-
 // LD / 4 lanes a row in the kernels that prepare and join, and a grid that goes over
 // the rows in turns.
 template <typename T, int LD>
@@ -105,7 +96,7 @@ __global__ __launch_bounds__(256) void k_fused_classes(Fused k, const void *w, i
         m = max(m, finite_max(x));
     }
     if (any && !k.ctl->open) k.ctl->open = 1u;
-    raise_by_block(&k.ctl->w_max, m);
+    raise_by_block<4>(k.ctl->w_max, m);
 }
 
 // The packed rows of W and then of h.
@@ -116,7 +107,7 @@ __global__ __launch_bounds__(256) void k_fused_pack(Fused k, const void *w, int6
                                                     const float *__restrict__ weights) {
     constexpr int LANES = LD / 4, ROWS = 256 / LANES;
     const int f = threadIdx.x % LANES * 4;
-    const int sw = scale_exp(k.ctl->w_max);
+    const int sw = scale_exp(largest(k.ctl->w_max));
     const bool any = k.ctl->open;
     uint32_t hg = 0;
     for (int64_t at = (int64_t)blockIdx.x * ROWS + threadIdx.x / LANES; at < k.v_pad + k.n_pad;
@@ -167,7 +158,7 @@ __global__ __launch_bounds__(256) void k_fused_pack(Fused k, const void *w, int6
             *reinterpret_cast<u16x4 *>(row + (of_w ? k.v_pad : k.n_pad) * LD) =
                 u16x4{lo[0], lo[1], lo[2], lo[3]};
     }
-    raise_by_block(&k.ctl->hg_max, hg);
+    raise_by_block<4>(k.ctl->hg_max, hg);
 }
 
 // ---- a tile in LDS -----------------------------------------------------------------
@@ -465,9 +456,11 @@ __global__ __launch_bounds__(256) void k_fused_join_rows(Fused k, XentCall c, in
 #pragma unroll
     for (int m = LANES / 2; m > 0; m >>= 1) dot += __shfl_xor(dot, m, 64);
     float ref = -INFINITY;
+#pragma unroll 8
     for (int s = 0; s < splits; ++s) ref = fmaxf(ref, part_ms[s * k.n_pad + i].x);
     const bool none = ref == -INFINITY;
     float sum = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
     for (int s = 0; s < splits; ++s) {
         const float2 ms = part_ms[s * k.n_pad + i];
         const float scale = none ? 1.0f : __builtin_amdgcn_exp2f(ms.x - ref);
@@ -492,13 +485,13 @@ __global__ __launch_bounds__(256) void k_fused_join_rows(Fused k, XentCall c, in
         if constexpr (GRAD) {
             k.c2[i] = y < 0 ? INFINITY : l.base2;
             // weight 2^-exp and the power of two that brings the largest below 2^15
-            const float q = ldexpf(wt, wq_exp(k.ctl->hg_max) - k.exp[i]);
+            const float q = ldexpf(wt, wq_exp(largest(k.ctl->hg_max)) - k.exp[i]);
             k.wq[i] = fminf(fmaxf(q, -60000.0f), 60000.0f);
         }
     }
     if constexpr (GRAD) {
         if (!c.dh || i >= k.n) return;
-        const float scale = ldexpf(1.0f, -scale_exp(k.ctl->w_max));
+        const float scale = ldexpf(1.0f, -scale_exp(largest(k.ctl->w_max)));
 #pragma unroll
         for (int e = 0; e < 4; ++e)
             if (f + e < k.d) {
@@ -653,7 +646,7 @@ __global__ __launch_bounds__(256) void k_fused_join_classes(Fused k, XentCall c,
     }
     if (v >= k.v) return;
     const bool open = k.bias2[v] != -INFINITY;
-    const float scale = ldexpf(1.0f, -wq_exp(k.ctl->hg_max));
+    const float scale = ldexpf(1.0f, -wq_exp(largest(k.ctl->hg_max)));
     const float x[4] = {sum.x, sum.y, sum.z, sum.w};
     if (c.dw)
 #pragma unroll
@@ -755,7 +748,7 @@ hipError_t run(hipStream_t s, const XentCall &c, const Plan &p, char *m) {
         const hipError_t e = allow_all_lds(f);
         if (e != hipSuccess) return e;
     }
-    hipLaunchKernelGGL(k_fused_init, dim3(1), dim3(1), 0, s, k.ctl);
+    hipLaunchKernelGGL(k_fused_init, dim3(1), dim3(64), 0, s, k.ctl);
     const auto grid = [&](int64_t rows) {
         return dim3(std::min<uint32_t>(blocks(rows, 1024 / LD), 8 * (uint32_t)c.num_cus));
     };

@@ -23,8 +23,14 @@ constexpr float LOG2E = 1.44269504088896341f;
 constexpr uint32_t XENT_HUGE = 0x5D800000u;
 
 // ---- control words -----------------------------------------------------------
+// A maximum over workgroups.  Atomics on one word take 15 to 20 ns each (42 us for the largest
+// of 16300 x 1000 f32 by 2048 workgroups), so the workgroups share MAX_WORDS words, a line each.
+constexpr int MAX_WORDS = 16;
+struct XentMax {
+    uint32_t word[MAX_WORDS][16];
+};
 struct XentCtl {
-    uint32_t w_max, hg_max;              // bits of the largest |W|, |w h| that is finite
+    XentMax w_max, hg_max;               // bits of the largest |W|, |w h| that is finite
     uint32_t open;                       // a class is offered
 };
 
@@ -44,9 +50,28 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
     return v;
 }
 
-// *max = max(*max, v): most calls find it there already, and leave the line alone.
-__device__ __forceinline__ void raise(uint32_t *max, uint32_t v) {
-    if (v > __atomic_load_n(max, __ATOMIC_RELAXED)) atomicMax(max, v);
+__device__ __forceinline__ uint32_t largest(const XentMax &m) {
+    uint32_t v = 0;
+#pragma unroll
+    for (int i = 0; i < MAX_WORDS; ++i) v = max(v, m.word[i][0]);
+    return v;
+}
+// The largest of a workgroup of WAVES wavefronts joins the maximum; where it is there
+// already, the line is left alone.  All threads call it, once.
+template <int WAVES> __device__ __forceinline__ void raise_by_block(XentMax &m, uint32_t v) {
+    __shared__ uint32_t most[WAVES];
+    v = wave_max(v);
+    if ((threadIdx.x & 63) == 0) most[threadIdx.x >> 6] = v;
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+#pragma unroll
+    for (int i = 0; i < WAVES; ++i) v = max(v, most[i]);
+    uint32_t *word = m.word[blockIdx.x % MAX_WORDS];
+    if (v > __atomic_load_n(word, __ATOMIC_RELAXED)) atomicMax(word, v);
+}
+__device__ __forceinline__ void clear(XentCtl *ctl) {
+    if (threadIdx.x < MAX_WORDS) ctl->w_max.word[threadIdx.x][0] = ctl->hg_max.word[threadIdx.x][0] = 0;
+    if (threadIdx.x == 0) ctl->open = 0;
 }
 
 __device__ __forceinline__ u16 bits_of(_Float16 v) { return __builtin_bit_cast(u16, v); }
