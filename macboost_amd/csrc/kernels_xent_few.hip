@@ -216,7 +216,7 @@ __global__ __launch_bounds__(64) void k_few_join(XentCall c, int32_t parts,
 // Element (x, k) of h or of a tile of W in LDS: chunks of 16 bytes of k, each with its 32
 // rows; the chunks 528 bytes apart, so that reads along x and along k fall on all banks.
 constexpr int CHUNK_BYTES = ROWS * 16 + 16;
-constexpr int GRAD_WAVES = 8, GRAD_BLOCKS = 4;       // blocks of 32 columns a wavefront keeps
+constexpr int GRAD_WAVES = 8;
 constexpr int G_STRIDE = 33;
 template <typename T>
 __device__ __forceinline__ float element_of(const char *m, int x, int k) {
@@ -224,31 +224,51 @@ __device__ __forceinline__ float element_of(const char *m, int x, int k) {
     return (float)*reinterpret_cast<const T *>(m + k / PER * CHUNK_BYTES + x * 16 +
                                                k % PER * (int)sizeof(T));
 }
-// Rows [0, 32) of a matrix into LDS: row(x) gives row x, or NULL for zeros.
-template <typename T, class Row>
-__device__ __forceinline__ void stage(char *m, int chunks, int dim, bool aligned, Row row) {
+// 32 rows of a matrix on their way to LDS, 16 lanes a row: element k of the lane's row is
+// row[k], NULL for zeros.  B: bytes that the rows are aligned to.
+template <int N> struct Staged {
+    u32x4 v[N];
+};
+template <typename T, int B, int N>
+__device__ __forceinline__ void load(Staged<N> &s, int chunks, int dim, const T *row) {
     constexpr int PER = 16 / sizeof(T);
-    for (int q = threadIdx.x; q < chunks * ROWS; q += 64 * GRAD_WAVES) {
-        const int x = q / chunks, c = q % chunks;
-        const T *from = row(x);
-        u32x4 v = {0, 0, 0, 0};
-        if (from && aligned) {
-            v = *reinterpret_cast<const u32x4 *>(from + c * PER);
-        } else if (from) {
-            T e[PER];
 #pragma unroll
-            for (int i = 0; i < PER; ++i)
-                e[i] = c * PER + i < dim ? from[c * PER + i] : (T)0.0f;
-            __builtin_memcpy(&v, e, sizeof v);
+    for (int n = 0; n < N; ++n) {
+        const int c = (threadIdx.x & 15) + n * 16, k = c * PER;
+        if (c >= chunks) break;
+        u32x4 v = {0, 0, 0, 0};
+        if (row) {
+            if (B == 16) {
+                v = *reinterpret_cast<const u32x4 *>(row + k);
+            } else if (B == 4 && k + PER <= dim) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = reinterpret_cast<const uint32_t *>(row + k)[i];
+            } else {
+                T e[PER];
+#pragma unroll
+                for (int i = 0; i < PER; ++i) e[i] = k + i < dim ? row[k + i] : (T)0.0f;
+                __builtin_memcpy(&v, e, sizeof v);
+            }
         }
-        *reinterpret_cast<u32x4 *>(m + c * CHUNK_BYTES + x * 16) = v;
+        s.v[n] = v;
+    }
+}
+template <int N>
+__device__ __forceinline__ void store(char *m, const Staged<N> &s, int chunks) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        const int c = (threadIdx.x & 15) + n * 16;
+        if (c >= chunks) break;
+        *reinterpret_cast<u32x4 *>(m + c * CHUNK_BYTES + (threadIdx.x >> 4) * 16) = s.v[n];
     }
 }
 
 // part_dh[workgroup][row][dim].
-template <typename T>
-__global__ __launch_bounds__(64 * GRAD_WAVES, 2) void k_few_grad(XentCall c, int64_t tiles,
-                                                                 int32_t chunks, bool aligned,
+// The next tile of W is asked for while this one is worked on.  NB: blocks of 32 columns
+// that a wavefront keeps of dh; with one, two workgroups fit a CU's registers.
+template <typename T, int B, int NB>
+__global__ __launch_bounds__(64 * GRAD_WAVES, NB == 1 ? 4 : 2) void k_few_grad(XentCall c, int64_t tiles,
+                                                                 int32_t chunks,
                                                                  const float *__restrict__ lse2,
                                                                  float *__restrict__ part_dh) {
     constexpr int PER = 16 / sizeof(T);
@@ -260,26 +280,33 @@ __global__ __launch_bounds__(64 * GRAD_WAVES, 2) void k_few_grad(XentCall c, int
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int blocks = (c.dim + 31) / 32;
     // a row that is out is zeros here: what it holds reaches nothing
-    stage<T>(h, chunks, c.dim, false, [&](int i) -> const T * {
-        return i < c.rows && lse2[i] != INFINITY
-                   ? static_cast<const T *>(c.h) + i * c.h_stride : nullptr;
-    });
+    const int x0 = threadIdx.x >> 4;                 // the row that this lane brings
+    Staged<NB * (int)sizeof(T)> staged;
+    load<T, sizeof(T)>(staged, chunks, c.dim,
+                       x0 < c.rows && lse2[x0] != INFINITY
+                           ? static_cast<const T *>(c.h) + x0 * c.h_stride : nullptr);
+    store(h, staged, chunks);
+    const auto ask = [&](int64_t t) {
+        const int64_t v = t * 32 + x0;
+        load<T, B>(staged, chunks, c.dim,
+                   v < c.classes && !(c.bias && c.bias[v] == -INFINITY)
+                       ? static_cast<const T *>(c.w) + v * c.w_stride : nullptr);
+    };
+    if (blockIdx.x < tiles) ask(blockIdx.x);
     const float l2 = l < c.rows ? lse2[l] : INFINITY;
     const int32_t label = l < c.rows ? c.labels[l] : -1;
     const float wt = l2 == INFINITY ? 0.0f : c.weights ? c.weights[l] : 1.0f;
-    f32x16 dh[GRAD_BLOCKS];
+    f32x16 dh[NB];
 #pragma unroll
-    for (int b = 0; b < GRAD_BLOCKS; ++b)
+    for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int r = 0; r < 16; ++r) dh[b][r] = 0.0f;
     for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
         const int64_t v0 = t * 32;
         __syncthreads();                             // the last tile's reads
-        stage<T>(w, chunks, c.dim, aligned, [&](int x) -> const T * {
-            return v0 + x < c.classes && !(c.bias && c.bias[v0 + x] == -INFINITY)
-                       ? static_cast<const T *>(c.w) + (v0 + x) * c.w_stride : nullptr;
-        });
+        store(w, staged, chunks);
         __syncthreads();
+        if (t + gridDim.x < tiles) ask(t + gridDim.x);
         // scores, classes down and rows across, k in parts of the wavefronts
         f32x16 s;
 #pragma unroll
@@ -338,7 +365,7 @@ __global__ __launch_bounds__(64 * GRAD_WAVES, 2) void k_few_grad(XentCall c, int
                 f32x16 o;
 #pragma unroll
                 for (int r = 0; r < 16; ++r) o[r] = 0.0f;
-#pragma unroll
+#pragma unroll 4
                 for (int k = 0; k < ROWS; k += 2)
                     o = __builtin_amdgcn_mfma_f32_32x32x2f32(g[(k + half) * G_STRIDE + l],
                                                              element_of<T>(h, k + half, j), o, 0, 0,
@@ -353,11 +380,11 @@ __global__ __launch_bounds__(64 * GRAD_WAVES, 2) void k_few_grad(XentCall c, int
             }
         if (c.dh)
 #pragma unroll
-            for (int n = 0; n < GRAD_BLOCKS; ++n) {
+            for (int n = 0; n < NB; ++n) {
                 const int b = wave + n * GRAD_WAVES;
                 if (b >= blocks) break;
                 const int j = min(b * 32 + l, chunks * PER - 1);
-#pragma unroll
+#pragma unroll 4
                 for (int k = 0; k < 32; k += 2)
                     dh[n] = __builtin_amdgcn_mfma_f32_32x32x2f32(g[l * G_STRIDE + k + half],
                                                                  element_of<T>(w, k + half, j),
@@ -366,7 +393,7 @@ __global__ __launch_bounds__(64 * GRAD_WAVES, 2) void k_few_grad(XentCall c, int
     }
     if (!c.dh) return;
 #pragma unroll
-    for (int n = 0; n < GRAD_BLOCKS; ++n) {
+    for (int n = 0; n < NB; ++n) {
         const int j = (wave + n * GRAD_WAVES) * 32 + l;
         if (j >= c.dim) continue;
 #pragma unroll
@@ -377,45 +404,64 @@ __global__ __launch_bounds__(64 * GRAD_WAVES, 2) void k_few_grad(XentCall c, int
     }
 }
 
+// The workgroups' parts of 64 elements of dh added, by four wavefronts.
 template <typename T>
 __global__ __launch_bounds__(256) void k_few_join_dh(XentCall c, int32_t parts,
                                                      const float *__restrict__ part) {
-    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, all = c.rows * c.dim;
-    if (at >= all) return;
+    __shared__ float sums[256];
+    const int64_t at = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63), all = c.rows * c.dim;
     float sum = 0.0f;
+    if (at < all)
 #pragma unroll 8
-    for (int p = 0; p < parts; ++p) sum += part[p * all + at];
+        for (int p = threadIdx.x >> 6; p < parts; p += 4) sum += part[p * all + at];
+    sums[threadIdx.x] = sum;
+    __syncthreads();
+    if (threadIdx.x >= 64 || at >= all) return;
+    for (int w = 1; w < 4; ++w) sum += sums[w * 64 + threadIdx.x];
     static_cast<T *>(c.dh)[at / c.dim * c.h_stride + at % c.dim] = (T)sum;
 }
 
 // Scratch: the parts of the rows, lse2, the parts of dh.
 size_t part_bytes(const XentCall &c) { return (size_t)c.num_cus * ROWS * sizeof(float2); }
 
+// Columns that a workgroup of k_few_grad keeps with one block a wavefront.
+constexpr int ONE_BLOCK = 32 * GRAD_WAVES;
+int grad_groups(const XentCall &c) { return (c.dim <= ONE_BLOCK ? 2 : 1) * c.num_cus; }
+
+template <typename T, int B, int NB>
+hipError_t run_grad(hipStream_t s, const XentCall &c, const float *lse2, float *part_dh) {
+    const hipError_t e = allow_all_lds(reinterpret_cast<const void *>(k_few_grad<T, B, NB>));
+    if (e != hipSuccess) return e;
+    constexpr int PER = 16 / sizeof(T);
+    const int32_t chunks = (c.dim + PER - 1) / PER;
+    const int64_t tiles = (c.classes + 31) / 32;
+    const uint32_t groups = (uint32_t)std::min<int64_t>(grad_groups(c), tiles);
+    const size_t lds = (size_t)2 * chunks * CHUNK_BYTES + 4 * (4 * 16 * 64 + ROWS * G_STRIDE);
+    hipLaunchKernelGGL((k_few_grad<T, B, NB>), dim3(groups), dim3(64 * GRAD_WAVES), lds, s, c,
+                       tiles, chunks, lse2, part_dh);
+    if (c.dh)
+        hipLaunchKernelGGL((k_few_join_dh<T>), dim3((uint32_t)((c.rows * c.dim + 63) / 64)),
+                           dim3(256), 0, s, c, (int32_t)groups, part_dh);
+    return hipGetLastError();
+}
+
 template <typename T, int B> hipError_t run(hipStream_t s, const XentCall &c, char *scratch) {
-    hipError_t e = allow_all_lds(reinterpret_cast<const void *>(k_few_stats<T, B>));
-    if (e == hipSuccess) e = allow_all_lds(reinterpret_cast<const void *>(k_few_grad<T>));
+    const hipError_t e = allow_all_lds(reinterpret_cast<const void *>(k_few_stats<T, B>));
     if (e != hipSuccess) return e;
     const int64_t tiles = (c.classes + 31) / 32;
     const int32_t steps = (int32_t)((c.dim * sizeof(T) + 127) / 128);
-    uint32_t groups = (uint32_t)std::min<int64_t>(c.num_cus, (tiles + WAVES - 1) / WAVES);
+    const uint32_t groups = (uint32_t)std::min<int64_t>(c.num_cus, (tiles + WAVES - 1) / WAVES);
     float2 *part = reinterpret_cast<float2 *>(scratch);
-    float *lse2 = reinterpret_cast<float *>(scratch + part_bytes(c));
+    float *lse2 = reinterpret_cast<float *>(scratch + part_bytes(c)), *part_dh = lse2 + ROWS;
     hipLaunchKernelGGL((k_few_stats<T, B>), dim3(groups), dim3(64 * WAVES), LDS_BYTES, s, c, tiles,
                        steps, part);
     hipLaunchKernelGGL((k_few_join<T>), dim3((uint32_t)c.rows), dim3(64), 0, s, c, (int32_t)groups,
                        part, c.grad ? lse2 : nullptr);
     if (!c.grad) return hipGetLastError();
-    constexpr int PER = 16 / sizeof(T);
-    const int32_t chunks = (c.dim + PER - 1) / PER;
-    float *part_dh = lse2 + ROWS;
-    groups = (uint32_t)std::min<int64_t>(c.num_cus, tiles);
-    const size_t lds = (size_t)2 * chunks * CHUNK_BYTES + 4 * (4 * 16 * 64 + ROWS * G_STRIDE);
-    hipLaunchKernelGGL((k_few_grad<T>), dim3(groups), dim3(64 * GRAD_WAVES), lds, s, c, tiles,
-                       chunks, B == 16, lse2, part_dh);
-    if (c.dh)
-        hipLaunchKernelGGL((k_few_join_dh<T>), dim3((uint32_t)((c.rows * c.dim + 255) / 256)),
-                           dim3(256), 0, s, c, (int32_t)groups, part_dh);
-    return hipGetLastError();
+    if (c.dim <= ONE_BLOCK) return run_grad<T, B, 1>(s, c, lse2, part_dh);
+    if constexpr (sizeof(T) == 2)
+        if (c.dim > 2 * ONE_BLOCK) return run_grad<T, B, 4>(s, c, lse2, part_dh);
+    return run_grad<T, B, 2>(s, c, lse2, part_dh);
 }
 
 }  // namespace
@@ -427,7 +473,7 @@ bool xent_few(const XentCall &c) {
 }
 
 size_t xent_few_scratch(const XentCall &c) {
-    return part_bytes(c) + 4 * ROWS + (c.grad ? (size_t)4 * c.num_cus * c.rows * c.dim : 0);
+    return part_bytes(c) + 4 * ROWS + (c.grad ? (size_t)4 * grad_groups(c) * c.rows * c.dim : 0);
 }
 
 hipError_t launch_xent_few(hipStream_t s, const XentCall &c, char *scratch) {
