@@ -81,7 +81,12 @@ typedef struct mbk_context mbk_context;
 int mbk_context_create(int32_t device, mbk_context **out, char **err);
 /* No counterpart in the reference: a context whose calls queue on the caller's
  * stream (a hipStream_t of `device`; NULL: its default stream), in order with the
- * caller's own work there.  The stream must outlive the context. */
+ * caller's own work there.  The stream must outlive the context.
+ * mbk_xent, mbk_xent_grad and the mbk_expert_ calls may be captured there into a
+ * graph.  Their scratch belongs to the context: it grows outside a capture only (a captured call that needs more is
+ * refused: make one of the same sizes before), what a graph has captured is kept
+ * until the context is destroyed, and graphs of one context must not run at the same time
+ * as each other or as its other calls. */
 int mbk_context_create_on(int32_t device, void *stream, mbk_context **out, char **err);
 void mbk_context_destroy(mbk_context *ctx);
 int mbk_device_alloc(mbk_context *ctx, size_t bytes, void **out, char **err);
@@ -355,7 +360,7 @@ typedef struct {
 typedef struct {
     void *data;
     int64_t row_stride, col_stride;
-    int32_t cols;
+    int32_t cols;                /* 1..2^30 */
     int32_t type;                /* MBK_F32 or MBK_BF16 */
     int32_t blocked;
 } mbk_expert_matrix;

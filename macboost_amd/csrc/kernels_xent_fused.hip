@@ -18,6 +18,12 @@
 //
 // Operands are one f16 term (bf16) or two (f32), as kernels_xent.hip says; exponents are
 // of 2, with log2 e in the scale of S.
+//
+// The matrix instructions bound both passes: 20000 x 100 x 10000 f32 takes 268 and 285 us,
+// 1.09 and 1.03 PFLOP/s of f16 products (112 columns of the first and 128 of the second, three
+// terms), with the matrix cores busy 55 % of the cycles at 1.85 GHz, where the power limit holds
+// the clock.  Without the exponentials the rows pass takes 6 % less, without the split of P
+// into terms 5 %.
 #include <algorithm>
 
 #include "mbk.h"
@@ -441,7 +447,8 @@ __global__ __launch_bounds__(256) void k_fused_join_rows(Fused k, XentCall c, in
                                                          const float *__restrict__ part_o,
                                                          const float2 *__restrict__ part_ms) {
     constexpr int LANES = LD / 4;
-    const int64_t i = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+    const int64_t i = (int64_t)group_id() * (256 / LANES) + threadIdx.x / LANES;
+    if (i >= k.n_pad) return;
     const int f = threadIdx.x % LANES * 4;
     const int32_t y = k.label[i];
     const bool open = y >= 0 && k.bias2[y] != -INFINITY;
@@ -616,7 +623,7 @@ __global__ __launch_bounds__(256) void k_fused_join_classes(Fused k, XentCall c,
     __shared__ double dbs[GROUPS ? 256 : 1];
     const int l = threadIdx.x % LANES, f = l * 4;
     const int g = threadIdx.x / LANES % G;
-    const int64_t v = (int64_t)blockIdx.x * CLASSES + threadIdx.x / (LANES * G);
+    const int64_t v = (int64_t)group_id() * CLASSES + threadIdx.x / (LANES * G);
     float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     double db = 0.0;
     if (v < k.v) {
@@ -755,7 +762,8 @@ hipError_t run(hipStream_t s, const XentCall &c, const Plan &p, char *m) {
     hipLaunchKernelGGL((k_fused_classes<T, LD>), grid(k.v_pad), b, 0, s, k, c.w, c.w_stride, c.bias);
     hipLaunchKernelGGL((k_fused_pack<T, LD>), grid(k.v_pad + k.n_pad), b, 0, s, k, c.w, c.w_stride,
                        c.h, c.h_stride, c.labels, c.weights);
-    const dim3 gr((uint32_t)(k.n_pad / XB * p.row_splits)), gj(blocks(k.n_pad, 1024 / LD));
+    const dim3 gr((uint32_t)(k.n_pad / XB * p.row_splits));
+    const dim3 gj = grid_of(blocks(k.n_pad, 1024 / LD));
     if (!c.grad) {
         hipLaunchKernelGGL((k_fused_rows<P, KS, false>), gr, b, lds_rows, s, k, p.row_splits,
                            static_cast<float *>(nullptr), part_ms);
@@ -773,10 +781,10 @@ hipError_t run(hipStream_t s, const XentCall &c, const Plan &p, char *m) {
                            p.class_splits, part, c.dbias ? part_db : nullptr);
         if (p.class_splits >= 2 * SPLIT_GROUPS)
             hipLaunchKernelGGL((k_fused_join_classes<T, LD, true>),
-                               dim3(blocks(k.v, 1024 / LD / SPLIT_GROUPS)), b, 0, s, k, c,
+                               grid_of(blocks(k.v, 1024 / LD / SPLIT_GROUPS)), b, 0, s, k, c,
                                p.class_splits, part, part_db);
         else
-            hipLaunchKernelGGL((k_fused_join_classes<T, LD, false>), dim3(blocks(k.v, 1024 / LD)),
+            hipLaunchKernelGGL((k_fused_join_classes<T, LD, false>), grid_of(blocks(k.v, 1024 / LD)),
                                b, 0, s, k, c, p.class_splits, part, part_db);
     }
     return hipGetLastError();

@@ -68,6 +68,7 @@ mbk::ExpertPlan expert_plan(const mbk_expert_plan *p) {
 mbk::ExpertMatrix expert_matrix(const mbk_expert_matrix *m, int64_t rows) {
     need(m != nullptr, "null matrix");
     need(m->cols >= 1, "cols must be positive");
+    need(m->cols <= (1 << 30), "cols must be at most 2^30");
     need(m->data || !rows, "null matrix data");
     // no element twice: rows apart by a row's columns, or columns by a column's rows
     constexpr int64_t MOST = (int64_t)1 << 40;

@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "grid.hpp"
 #include "ops.h"
 
 namespace mbk {
@@ -139,7 +140,10 @@ template <int N> struct At {
 };
 
 // The kernels of up to XENT_FUSED_DIM outputs (kernels_xent_fused.hip): scores, their
-// exponentials and the product with them in one pass for dh and one for dW.
+// exponentials and the product with them in one pass for dh and one for dW.  128 is what a
+// wavefront's registers hold of both operands; up to there they win at every size (us, fused
+// and by products: f32 20000 x 128 x 10000 loss 204 and 228, with gradients 611 and 1233, 1000 x
+// 128 x 1000 57 and 87; bf16 20000 x 32 x 10000 180 and 537).
 constexpr int XENT_FUSED_DIM = 128;
 size_t xent_fused_scratch(const XentCall &c);
 hipError_t launch_xent_fused(hipStream_t s, const XentCall &c, char *scratch);

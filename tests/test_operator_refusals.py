@@ -85,6 +85,7 @@ def test_expert_plans(change, msg):
 
 @pytest.mark.parametrize("change,msg", [
     ({"cols": 0}, "cols must be positive"),
+    ({"cols": (1 << 30) + 1}, "cols must be at most 2"),
     ({"data": None}, "null matrix data"),
     ({"row_stride": 0}, "row_stride and col_stride"),
     ({"col_stride": -1}, "row_stride and col_stride"),
