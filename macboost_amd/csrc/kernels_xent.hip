@@ -47,10 +47,6 @@ typedef __attribute__((ext_vector_type(8))) unsigned short u16x8;
 constexpr int LD_PAD = 128;              // operands' rows are padded to it
 constexpr float G_SCALE = 32768.0f;      // |G / w| <= 1 as f16 terms
 
-__global__ void k_xent_init(XentCtl *ctl) {
-    clear(ctl);
-}
-
 template <typename T> __device__ __forceinline__ float load_f32(const void *p, int64_t i) {
     return (float)static_cast<const T *>(p)[i];
 }
@@ -131,18 +127,20 @@ __global__ __launch_bounds__(64 * MAX_WAVES) void k_xent_classes(XentPack k, con
                 for (int e = 0; e < 8; ++e) m = max(m, finite_bits(x[q][e]));
         }
     }
-    if (any && !k.ctl->open) k.ctl->open = 1u;
-    raise_by_block<MAX_WAVES>(k.ctl->w_max, m);
+    __shared__ uint32_t lds[2 * MAX_WAVES];
+    const uint32_t most = largest<MAX_WAVES>(m, any, lds);
+    if (threadIdx.x == 0) k.ctl->w.part[blockIdx.x] = most;
 }
 
+// The rows of W, times 2^s.
 template <typename T>
-__global__ __launch_bounds__(256) void k_xent_pack_w(XentPack k, const void *w, int64_t stride) {
+__device__ __forceinline__ void pack_w(const XentPack &k, const void *w, int64_t stride, int s) {
     const int lane = threadIdx.x & 63;
     const int align = alignment<T>(w, stride);
-    const int s = scale_exp(largest(k.ctl->w_max));
     constexpr int ROWS = 2;
-    const int64_t hop = (int64_t)gridDim.x * 4;
-    for (int64_t v0 = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); v0 < k.v_pad; v0 += ROWS * hop) {
+    const int64_t hop = (int64_t)k.pack_w_groups * MAX_WAVES;
+    for (int64_t v0 = (int64_t)blockIdx.x * MAX_WAVES + (threadIdx.x >> 6); v0 < k.v_pad;
+         v0 += ROWS * hop) {
         int32_t d[ROWS];
 #pragma unroll
         for (int q = 0; q < ROWS; ++q)
@@ -160,26 +158,32 @@ __global__ __launch_bounds__(256) void k_xent_pack_w(XentPack k, const void *w, 
     }
 }
 
-// Rows: label and weight (-1 and 0 where the row is out), h scaled by row.  A row that
-// is out and not finite is packed as zeros, its label -2.
+// W packed, and by the workgroups behind those, the rows: label and weight (-1 and 0 where
+// the row is out), h scaled by row.  A row that is out and not finite is packed as zeros, its
+// label -2.
 template <typename T>
-__global__ __launch_bounds__(64 * MAX_WAVES) void k_xent_rows(XentPack k, const void *h, int64_t stride,
-                                                   const int32_t *__restrict__ labels,
-                                                   const float *__restrict__ weights) {
+__global__ __launch_bounds__(64 * MAX_WAVES) void k_xent_pack(XentPack k, XentCall c) {
+    __shared__ uint32_t lds[2 * MAX_WAVES];
+    const uint32_t most_w = largest_of<MAX_WAVES>(k.ctl->w, k.w_groups, lds);
+    const int sw = scale_exp(most_w & ~FLAG);
+    if (blockIdx.x == 0 && threadIdx.x == 0) k.ctl->w.all = most_w & ~FLAG;
+    if ((int32_t)blockIdx.x < k.pack_w_groups) {
+        pack_w<T>(k, c.w, c.w_stride, sw);
+        return;
+    }
+    const int32_t group = blockIdx.x - k.pack_w_groups;
     const int lane = threadIdx.x & 63;
-    const int align = alignment<T>(h, stride);
-    const bool any = k.ctl->open;
-    const int sw = scale_exp(largest(k.ctl->w_max));
+    const int align = alignment<T>(c.h, c.h_stride);
     uint32_t hg = 0;
-    for (int64_t i = (int64_t)blockIdx.x * MAX_WAVES + (threadIdx.x >> 6); i < k.n_pad;
-         i += (int64_t)gridDim.x * MAX_WAVES) {
-        int32_t y = i < k.n ? labels[i] : -1, d = i < k.n ? k.d : 0;
-        float wt = i < k.n ? (weights ? weights[i] : 1.0f) : 0.0f;
-        const bool out = y < 0 || y >= k.v || wt == 0.0f || !any;
+    for (int64_t i = (int64_t)group * MAX_WAVES + (threadIdx.x >> 6); i < k.n_pad;
+         i += (int64_t)k.hg_groups * MAX_WAVES) {
+        int32_t y = i < k.n ? c.labels[i] : -1, d = i < k.n ? k.d : 0;
+        float wt = i < k.n ? (c.weights ? c.weights[i] : 1.0f) : 0.0f;
+        const bool out = y < 0 || y >= k.v || wt == 0.0f || !(most_w & FLAG);
         uint32_t m = 0, most = 0;
         for (int32_t f = lane * 8; f < d; f += 512) {
             float x[8];
-            load8<T>(h, i * stride, f, d, align, x);
+            load8<T>(c.h, i * c.h_stride, f, d, align, x);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 m = max(m, finite_bits(x[e]));
@@ -205,32 +209,12 @@ __global__ __launch_bounds__(64 * MAX_WAVES) void k_xent_rows(XentPack k, const 
         }
         for (int32_t f = lane * 8; f < k.ld; f += 512) {
             float x[8];
-            load8<T>(h, i * stride, f, d, align, x);
+            load8<T>(c.h, i * c.h_stride, f, d, align, x);
             pack8<T>(x, s, k.h + i * k.ld + f, k.n_pad * k.ld);
         }
     }
-    raise_by_block<MAX_WAVES>(k.ctl->hg_max, hg);
-}
-
-// h as dW's product takes it, times the row's weight and with one scale for all rows
-// (they are summed over).
-template <typename T>
-__global__ __launch_bounds__(256) void k_xent_pack_hg(XentPack k, const void *h, int64_t stride) {
-    const int lane = threadIdx.x & 63;
-    const int align = alignment<T>(h, stride);
-    const int s = scale_exp(largest(k.ctl->hg_max));
-    for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < k.n_pad;
-         i += (int64_t)gridDim.x * 4) {
-        const int32_t d = k.label[i] >= 0 ? k.d : 0;
-        const float wt = k.weight[i];
-        for (int32_t f = lane * 8; f < k.ld; f += 512) {
-            float x[8];
-            load8<T>(h, i * stride, f, d, align, x);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] *= wt;
-            pack8<T>(x, s, k.hg + i * k.ld + f, k.n_pad * k.ld);
-        }
-    }
+    const uint32_t most = largest<MAX_WAVES>(hg, 0, lds);
+    if (threadIdx.x == 0) k.ctl->hg.part[group] = most;
 }
 
 // ---- products --------------------------------------------------------------------
@@ -473,6 +457,11 @@ __global__ __launch_bounds__(C::WAVES * 64, 2) void k_xent_stats(XentPack k, int
                                                                  int32_t splits,
                                                                  float2 *__restrict__ part) {
     extern __shared__ char lds[];
+    if (k.hg && blockIdx.x == 0) {       // for the kernels behind this one
+        const uint32_t most = largest_of<C::WAVES>(k.ctl->hg, k.hg_groups,
+                                                     reinterpret_cast<uint32_t *>(lds));
+        if (threadIdx.x == 0) k.ctl->hg.all = most;
+    }
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     uint32_t row_tile, split;
@@ -540,7 +529,8 @@ __global__ __launch_bounds__(C::WAVES * 64, 2) void k_xent_stats(XentPack k, int
 }
 
 // The parts of a row joined, one wavefront a row: lse and loss.  The label's score is
-// summed in f32 from h and W themselves.
+// summed in f32 from h and W themselves.  For gradients, h is packed once more as dW's product
+// takes it, times the row's weight and with one scale for all rows (they are summed over).
 template <typename T>
 __global__ __launch_bounds__(256) void k_xent_join(XentPack k, XentCall c, int32_t parts,
                                                    const float2 *__restrict__ part,
@@ -568,6 +558,18 @@ __global__ __launch_bounds__(256) void k_xent_join(XentPack k, XentCall c, int32
         sum = sum * __builtin_amdgcn_exp2f(top - ref) + s2 * __builtin_amdgcn_exp2f(t2 - ref);
         top = now;
         dot += __shfl_xor(dot, o, 64);
+    }
+    if (k.hg) {
+        const int s = scale_exp(k.ctl->hg.all), align = alignment<T>(c.h, c.h_stride);
+        const int32_t d = y >= 0 ? k.d : 0;
+        const float wt = k.weight[i];
+        for (int32_t f = lane * 8; f < k.ld; f += 512) {
+            float x[8];
+            load8<T>(c.h, i * c.h_stride, f, d, align, x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] *= wt;
+            pack8<T>(x, s, k.hg + i * k.ld + f, k.n_pad * k.ld);
+        }
     }
     if (lane != 0) return;
     const LogSum l = log_sum(top, sum);
@@ -680,7 +682,7 @@ struct Out {
     bool classes;                // dW: rows whose bias is -inf are 0; dh: times weight
 };
 __device__ __forceinline__ float out_scale(const XentPack &k, bool classes) {
-    return ldexpf(1.0f, -scale_exp(largest(classes ? k.ctl->hg_max : k.ctl->w_max))) / G_SCALE;
+    return ldexpf(1.0f, -scale_exp(classes ? k.ctl->hg.all : k.ctl->w.all)) / G_SCALE;
 }
 template <int P>
 __device__ __forceinline__ void put(const XentPack &k, const Out &o, int64_t m, int64_t n, float v,
@@ -941,7 +943,7 @@ hipError_t run(hipStream_t s, const XentCall &c, const Plan &p, char *m) {
     k.ld = (int32_t)p.ld;
     k.ctl = reinterpret_cast<XentCtl *>(m + p.ctl);
     k.h = reinterpret_cast<u16 *>(m + p.h);
-    k.hg = reinterpret_cast<u16 *>(m + p.hg);
+    k.hg = c.grad ? reinterpret_cast<u16 *>(m + p.hg) : nullptr;
     k.w = reinterpret_cast<u16 *>(m + p.w);
     k.bias = reinterpret_cast<float *>(m + p.bias);
     k.row_scale = reinterpret_cast<float *>(m + p.scale);
@@ -962,25 +964,21 @@ hipError_t run(hipStream_t s, const XentCall &c, const Plan &p, char *m) {
         const hipError_t e = allow_all_lds(f);
         if (e != hipSuccess) return e;
     }
-    hipLaunchKernelGGL(k_xent_init, dim3(1), dim3(64), 0, s, k.ctl);
-    const auto grid = [&](int64_t rows) {
-        return dim3(std::min<uint32_t>(blocks(rows, 4), 8 * (uint32_t)c.num_cus));
+    const auto groups = [&](int64_t rows) {
+        return (int32_t)std::min<int64_t>((rows + MAX_WAVES - 1) / MAX_WAVES,
+                                          std::min(4 * c.num_cus, MOST_GROUPS));
     };
-    const auto max_grid = [&](int64_t rows) {
-        return dim3(std::min<uint32_t>(blocks(rows, MAX_WAVES), 4 * (uint32_t)c.num_cus));
-    };
-    const dim3 max_block(64 * MAX_WAVES);
-    hipLaunchKernelGGL((k_xent_classes<T>), max_grid(k.v_pad), max_block, 0, s, k, c.w, c.w_stride,
-                       c.bias);
-    hipLaunchKernelGGL((k_xent_pack_w<T>), grid(k.v_pad), b, 0, s, k, c.w, c.w_stride);
-    hipLaunchKernelGGL((k_xent_rows<T>), max_grid(k.n_pad), max_block, 0, s, k, c.h, c.h_stride,
-                       c.labels, c.weights);
+    k.w_groups = k.pack_w_groups = groups(k.v_pad);
+    k.hg_groups = groups(k.n_pad);
+    hipLaunchKernelGGL((k_xent_classes<T>), dim3((uint32_t)k.w_groups), dim3(64 * MAX_WAVES), 0, s,
+                       k, c.w, c.w_stride, c.bias);
+    hipLaunchKernelGGL((k_xent_pack<T>), dim3((uint32_t)(k.pack_w_groups + k.hg_groups)),
+                       dim3(64 * MAX_WAVES), 0, s, k, c);
     if (p.wide) launch_stats<P, Wide>(s, k, p.splits, part);
     else launch_stats<P, Narrow>(s, k, p.splits, part);
     hipLaunchKernelGGL((k_xent_join<T>), grid_of(blocks(k.n_pad, 4)), b, 0, s, k, c, 2 * p.splits,
                        part, lse2);
     if (!c.grad) return hipGetLastError();
-    hipLaunchKernelGGL((k_xent_pack_hg<T>), grid(k.n_pad), b, 0, s, k, c.h, c.h_stride);
     u16 *g = reinterpret_cast<u16 *>(m + p.g);
     float *part_db = c.dbias ? reinterpret_cast<float *>(m + p.db) : nullptr;
     const int64_t plane = p.piece_rows * p.piece_classes, step = BK<P>;

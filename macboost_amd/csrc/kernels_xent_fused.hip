@@ -47,6 +47,7 @@ __host__ __device__ constexpr int row_ld(int ks) { return ks <= 2 ? 32 : ks <= 4
 struct Fused {
     int64_t n, v, n_pad, v_pad;
     int32_t d;
+    int32_t w_groups, hg_groups;         // that look at W, pack h
     XentCtl *ctl;
     u16 *h, *w;                          // planes of n_pad * ld, v_pad * ld
     float *bias2;                        // [v_pad] bias log2 e, -inf: not offered
@@ -62,10 +63,6 @@ struct Fused {
 // The exponent of the classes pass's weights, for the largest |w h|.
 __device__ __forceinline__ int wq_exp(uint32_t hg_max) {
     return hg_max ? min(126, max(-126, 27 - ilogbf(__uint_as_float(hg_max)))) : 0;
-}
-
-__global__ void k_fused_init(XentCtl *ctl) {
-    clear(ctl);
 }
 
 template <typename T> __device__ __forceinline__ float load_f32(const void *p, int64_t i) {
@@ -101,8 +98,9 @@ __global__ __launch_bounds__(256) void k_fused_classes(Fused k, const void *w, i
         load4<T>(w, v * stride, f, k.d, x);
         m = max(m, finite_max(x));
     }
-    if (any && !k.ctl->open) k.ctl->open = 1u;
-    raise_by_block<4>(k.ctl->w_max, m);
+    __shared__ uint32_t lds[8];
+    const uint32_t most = largest<4>(m, any, lds);
+    if (threadIdx.x == 0) k.ctl->w.part[blockIdx.x] = most;
 }
 
 // The packed rows of W and then of h.
@@ -113,8 +111,11 @@ __global__ __launch_bounds__(256) void k_fused_pack(Fused k, const void *w, int6
                                                     const float *__restrict__ weights) {
     constexpr int LANES = LD / 4, ROWS = 256 / LANES;
     const int f = threadIdx.x % LANES * 4;
-    const int sw = scale_exp(largest(k.ctl->w_max));
-    const bool any = k.ctl->open;
+    __shared__ uint32_t lds[8];
+    const uint32_t most_w = largest_of<4>(k.ctl->w, k.w_groups, lds);
+    const int sw = scale_exp(most_w & ~FLAG);
+    const bool any = most_w & FLAG;
+    if (blockIdx.x == 0 && threadIdx.x == 0) k.ctl->w.all = most_w & ~FLAG;
     uint32_t hg = 0;
     for (int64_t at = (int64_t)blockIdx.x * ROWS + threadIdx.x / LANES; at < k.v_pad + k.n_pad;
          at += (int64_t)gridDim.x * ROWS) {
@@ -164,7 +165,8 @@ __global__ __launch_bounds__(256) void k_fused_pack(Fused k, const void *w, int6
             *reinterpret_cast<u16x4 *>(row + (of_w ? k.v_pad : k.n_pad) * LD) =
                 u16x4{lo[0], lo[1], lo[2], lo[3]};
     }
-    raise_by_block<4>(k.ctl->hg_max, hg);
+    const uint32_t most = largest<4>(hg, 0, lds);
+    if (threadIdx.x == 0) k.ctl->hg.part[blockIdx.x] = most;
 }
 
 // ---- a tile in LDS -----------------------------------------------------------------
@@ -348,6 +350,11 @@ __global__ __launch_bounds__(256, 2) void k_fused_rows(Fused k, int32_t splits,
     constexpr int LD = row_ld(KS), JT = (KS + 1) / 2;
     constexpr int BUF = TILE_BYTES<P, LD> + TY * 4;      // a multiple of 256: see across
     extern __shared__ char lds[];
+    if (GRAD && blockIdx.x == 0) {       // for the kernels behind this one
+        const uint32_t most = largest_of<4>(k.ctl->hg, k.hg_groups,
+                                            reinterpret_cast<uint32_t *>(lds));
+        if (threadIdx.x == 0) k.ctl->hg.all = most;
+    }
     const int lane = threadIdx.x & 63, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t x0 = (int64_t)(blockIdx.x / splits) * XB;
@@ -492,13 +499,13 @@ __global__ __launch_bounds__(256) void k_fused_join_rows(Fused k, XentCall c, in
         if constexpr (GRAD) {
             k.c2[i] = y < 0 ? INFINITY : l.base2;
             // weight 2^-exp and the power of two that brings the largest below 2^15
-            const float q = ldexpf(wt, wq_exp(largest(k.ctl->hg_max)) - k.exp[i]);
+            const float q = ldexpf(wt, wq_exp(k.ctl->hg.all) - k.exp[i]);
             k.wq[i] = fminf(fmaxf(q, -60000.0f), 60000.0f);
         }
     }
     if constexpr (GRAD) {
         if (!c.dh || i >= k.n) return;
-        const float scale = ldexpf(1.0f, -scale_exp(largest(k.ctl->w_max)));
+        const float scale = ldexpf(1.0f, -scale_exp(k.ctl->w.all));
 #pragma unroll
         for (int e = 0; e < 4; ++e)
             if (f + e < k.d) {
@@ -653,7 +660,7 @@ __global__ __launch_bounds__(256) void k_fused_join_classes(Fused k, XentCall c,
     }
     if (v >= k.v) return;
     const bool open = k.bias2[v] != -INFINITY;
-    const float scale = ldexpf(1.0f, -wq_exp(largest(k.ctl->hg_max)));
+    const float scale = ldexpf(1.0f, -wq_exp(k.ctl->hg.all));
     const float x[4] = {sum.x, sum.y, sum.z, sum.w};
     if (c.dw)
 #pragma unroll
@@ -755,13 +762,16 @@ hipError_t run(hipStream_t s, const XentCall &c, const Plan &p, char *m) {
         const hipError_t e = allow_all_lds(f);
         if (e != hipSuccess) return e;
     }
-    hipLaunchKernelGGL(k_fused_init, dim3(1), dim3(64), 0, s, k.ctl);
-    const auto grid = [&](int64_t rows) {
-        return dim3(std::min<uint32_t>(blocks(rows, 1024 / LD), 8 * (uint32_t)c.num_cus));
+    const auto groups = [&](int64_t rows) {
+        return (int32_t)std::min<int64_t>((rows * LD + 1023) / 1024,
+                                          std::min(8 * c.num_cus, MOST_GROUPS));
     };
-    hipLaunchKernelGGL((k_fused_classes<T, LD>), grid(k.v_pad), b, 0, s, k, c.w, c.w_stride, c.bias);
-    hipLaunchKernelGGL((k_fused_pack<T, LD>), grid(k.v_pad + k.n_pad), b, 0, s, k, c.w, c.w_stride,
-                       c.h, c.h_stride, c.labels, c.weights);
+    k.w_groups = groups(k.v_pad);
+    k.hg_groups = groups(k.v_pad + k.n_pad);
+    hipLaunchKernelGGL((k_fused_classes<T, LD>), dim3((uint32_t)k.w_groups), b, 0, s, k, c.w,
+                       c.w_stride, c.bias);
+    hipLaunchKernelGGL((k_fused_pack<T, LD>), dim3((uint32_t)k.hg_groups), b, 0, s, k, c.w,
+                       c.w_stride, c.h, c.h_stride, c.labels, c.weights);
     const dim3 gr((uint32_t)(k.n_pad / XB * p.row_splits));
     const dim3 gj = grid_of(blocks(k.n_pad, 1024 / LD));
     if (!c.grad) {

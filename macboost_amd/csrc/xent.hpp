@@ -24,15 +24,19 @@ constexpr float LOG2E = 1.44269504088896341f;
 constexpr uint32_t XENT_HUGE = 0x5D800000u;
 
 // ---- control words -----------------------------------------------------------
-// A maximum over workgroups.  Atomics on one word take 15 to 20 ns each (42 us for the largest
-// of 16300 x 1000 f32 by 2048 workgroups), so the workgroups share MAX_WORDS words, a line each.
-constexpr int MAX_WORDS = 16;
+// A maximum over the workgroups of a kernel: each leaves its own, and those of a later one
+// look them all over.  (Atomics on one word took 15 to 20 ns each, 42 us for the largest of
+// 16300 x 1000 f32 by 2048 workgroups, and a launch to clear it.)
+constexpr int MOST_GROUPS = 1024;
+constexpr uint32_t FLAG = 0x80000000u;   // beside a maximum of bits without a sign: an or
 struct XentMax {
-    uint32_t word[MAX_WORDS][16];
+    uint32_t part[MOST_GROUPS];
+    uint32_t all;                        // a later kernel's first workgroup leaves it here
 };
 struct XentCtl {
-    XentMax w_max, hg_max;               // bits of the largest |W|, |w h| that is finite
-    uint32_t open;                       // a class is offered
+    XentMax w;                           // bits of the largest |W| that is finite; FLAG: a class
+                                         // is offered
+    XentMax hg;                          // of |w h|
 };
 
 __device__ __forceinline__ uint32_t finite_bits(float x) {
@@ -51,28 +55,34 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
     return v;
 }
 
-__device__ __forceinline__ uint32_t largest(const XentMax &m) {
-    uint32_t v = 0;
-#pragma unroll
-    for (int i = 0; i < MAX_WORDS; ++i) v = max(v, m.word[i][0]);
-    return v;
-}
-// The largest of a workgroup of WAVES wavefronts joins the maximum; where it is there
-// already, the line is left alone.  All threads call it, once.
-template <int WAVES> __device__ __forceinline__ void raise_by_block(XentMax &m, uint32_t v) {
-    __shared__ uint32_t most[WAVES];
+// Of a workgroup of WAVES wavefronts; all of its threads call it.  lds: 2 WAVES words, free
+// again at the end.
+template <int WAVES>
+__device__ __forceinline__ uint32_t largest(uint32_t v, uint32_t flag, uint32_t *lds) {
     v = wave_max(v);
-    if ((threadIdx.x & 63) == 0) most[threadIdx.x >> 6] = v;
+    flag = __any(flag != 0) ? FLAG : 0u;
+    if ((threadIdx.x & 63) == 0) {
+        lds[threadIdx.x >> 6] = v;
+        lds[WAVES + (threadIdx.x >> 6)] = flag;
+    }
     __syncthreads();
-    if (threadIdx.x != 0) return;
 #pragma unroll
-    for (int i = 0; i < WAVES; ++i) v = max(v, most[i]);
-    uint32_t *word = m.word[blockIdx.x % MAX_WORDS];
-    if (v > __atomic_load_n(word, __ATOMIC_RELAXED)) atomicMax(word, v);
+    for (int i = 0; i < WAVES; ++i) {
+        v = max(v, lds[i]);
+        flag |= lds[WAVES + i];
+    }
+    __syncthreads();
+    return v | flag;
 }
-__device__ __forceinline__ void clear(XentCtl *ctl) {
-    if (threadIdx.x < MAX_WORDS) ctl->w_max.word[threadIdx.x][0] = ctl->hg_max.word[threadIdx.x][0] = 0;
-    if (threadIdx.x == 0) ctl->open = 0;
+template <int WAVES>
+__device__ __forceinline__ uint32_t largest_of(const XentMax &m, int32_t groups, uint32_t *lds) {
+    uint32_t v = 0, flag = 0;
+    for (int g = threadIdx.x; g < groups; g += 64 * WAVES) {
+        const uint32_t p = m.part[g];
+        v = max(v, p & ~FLAG);
+        flag |= p & FLAG;
+    }
+    return largest<WAVES>(v, flag, lds);
 }
 
 __device__ __forceinline__ u16 bits_of(_Float16 v) { return __builtin_bit_cast(u16, v); }
@@ -89,8 +99,9 @@ __device__ __forceinline__ void split_f16(float x, u16 &hi, u16 &lo) {
 struct XentPack {
     int64_t n, v, n_pad, v_pad;
     int32_t d, ld;
+    int32_t w_groups, pack_w_groups, hg_groups;      // that look at W, pack W, pack h
     XentCtl *ctl;
-    u16 *h, *hg, *w;                     // planes of n_pad * ld, v_pad * ld
+    u16 *h, *hg, *w;                     // planes of n_pad * ld, v_pad * ld; hg: gradients only
     float *bias;                         // [v_pad] bias log2 e, -inf: not offered
     float *row_scale;                    // [n_pad] log2 e times the scale of a score
     int32_t *label;                      // [n_pad], -1: out, -2: out and not finite
