@@ -697,33 +697,35 @@ __device__ __forceinline__ void put(const XentPack &k, const Out &o, int64_t m, 
     else static_cast<float *>(o.out)[m * o.stride + n] = v * scale;
 }
 
-// The products with G: dh (A = G across, m the rows) and dW (A = G along, m the classes),
-// B = W or h across.  C's first row is m_first of the output.
+// A product with G: its first row is m_first of the output.
+struct Product {
+    Operand a, b;
+    int32_t tiles_m, tiles_n;
+    int64_t steps, m_first;
+    Out o;
+};
 template <int P, bool AK, class C>
-__global__ __launch_bounds__(C::WAVES * 64, 2) void k_xent_product(XentPack k, Operand a,
-                                                                   Operand b, int32_t tiles_m,
-                                                                   int32_t tiles_n, int64_t steps,
-                                                                   int64_t m_first, Out o) {
-    extern __shared__ char lds[];
+__device__ __forceinline__ void product(const XentPack &k, const Product &q, uint32_t id, char *lds) {
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t per = tiles_m * tiles_n, split = blockIdx.x / per;
+    const Out &o = q.o;
+    const uint32_t per = q.tiles_m * q.tiles_n, split = id / per;
     uint32_t tm, tn;
-    tile_of(blockIdx.x % per, per, tiles_m, tiles_n, tm, tn);
+    tile_of(id % per, per, q.tiles_m, q.tiles_n, tm, tn);
     Acc<C> acc;
     const auto next = [&](int64_t, int64_t &m0, int64_t &n0) {
         m0 = (int64_t)tm * C::T;
         n0 = (int64_t)tn * C::T;
     };
-    products<P, AK, false, C>(a, b, 1, steps * split / o.splits, steps * (split + 1) / o.splits,
-                              lds, acc, next, [](int64_t) {});
+    products<P, AK, false, C>(q.a, q.b, 1, q.steps * split / o.splits,
+                              q.steps * (split + 1) / o.splits, lds, acc, next, [](int64_t) {});
     const float scale = out_scale(k, o.classes);
     float *sums = o.acc + split * o.m_pad * k.ld;
 #pragma unroll
     for (int x = 0; x < C::MT; ++x)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            const int64_t m = m_first + (int64_t)tm * C::T + wave / C::WN * C::MT * 32 + x * 32 +
+            const int64_t m = q.m_first + (int64_t)tm * C::T + wave / C::WN * C::MT * 32 + x * 32 +
                               (r >> 2) * 8 + (lane >> 5) * 4 + (r & 3);
 #pragma unroll
             for (int y = 0; y < C::NT; ++y) {
@@ -741,10 +743,20 @@ __global__ __launch_bounds__(C::WAVES * 64, 2) void k_xent_product(XentPack k, O
         }
 }
 
-// The splits of a product added, in order, from row m_first of the output on.
+// Both products, dh (A = G across, m the rows) by the first workgroups and dW (A = G along, m
+// the classes), B = W or h across: where neither fills the chip they run side by side (bf16
+// 194 x 216 x 835 with gradients: 50 us, 69 with a launch for each and for each sum).
+template <int P, class C>
+__global__ __launch_bounds__(C::WAVES * 64, 2) void k_xent_products(XentPack k, Product dh,
+                                                                    uint32_t dh_groups, Product dw) {
+    extern __shared__ char lds[];
+    if (blockIdx.x < dh_groups) product<P, false, C>(k, dh, blockIdx.x, lds);
+    else product<P, true, C>(k, dw, blockIdx.x - dh_groups, lds);
+}
+
+// The splits of a product's row added, in order.
 template <int P>
-__global__ __launch_bounds__(256) void k_xent_join_splits(XentPack k, int64_t m_first, Out o) {
-    const int64_t m = m_first + blockIdx.x;
+__device__ __forceinline__ void join_splits(const XentPack &k, int64_t m, const Out &o) {
     const float scale = out_scale(k, o.classes);
     for (int32_t n = threadIdx.x; n < k.d; n += 256) {
         float v = 0.0f;
@@ -753,13 +765,24 @@ __global__ __launch_bounds__(256) void k_xent_join_splits(XentPack k, int64_t m_
         put<P>(k, o, m, n, v, scale);
     }
 }
-
-// db[v] += the parts' sums, in order.
-__global__ __launch_bounds__(256) void k_xent_join_db(XentPack k, int64_t v0, int64_t classes,
-                                                      int32_t parts,
-                                                      const float *__restrict__ part_db,
-                                                      bool first, float *__restrict__ db) {
-    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+// A workgroup a row of dh_rows and of dw_rows, whose splits it adds, and then one for 256 classes
+// from v0 on: db[v] += the parts' sums, in order.
+template <int P>
+__global__ __launch_bounds__(256) void k_xent_finish(XentPack k, uint32_t dh_rows, int64_t dh_first,
+                                                     Out dh, uint32_t dw_rows, int64_t dw_first,
+                                                     Out dw, int64_t v0, int64_t classes,
+                                                     int32_t parts,
+                                                     const float *__restrict__ part_db, bool first,
+                                                     float *__restrict__ db) {
+    if (blockIdx.x < dh_rows) {
+        join_splits<P>(k, dh_first + blockIdx.x, dh);
+        return;
+    }
+    if (blockIdx.x < dh_rows + dw_rows) {
+        join_splits<P>(k, dw_first + (blockIdx.x - dh_rows), dw);
+        return;
+    }
+    const int64_t c = (int64_t)(blockIdx.x - dh_rows - dw_rows) * 256 + threadIdx.x;
     if (c >= classes) return;
     double sum = 0.0;
 #pragma unroll 8
@@ -818,7 +841,7 @@ bool wide_tiles(int64_t rows, int64_t classes, int num_cus) {
 // How a product over k of m x n is cut.
 struct Cut {
     bool wide;
-    int32_t tiles_m, tiles_n, splits;
+    int32_t tiles_n, splits;
 };
 // The least time by the steps of the workgroups' rounds, 3 us for a workgroup's start and
 // end, and what the parts of a split k take to be written, read and joined.  (f32, with
@@ -831,14 +854,14 @@ Cut cut_of(bool wide_allowed, int P, int64_t m, int64_t n, int64_t steps, int nu
         const int64_t t = wide ? 256 : 128, slots = slots_of(wide, num_cus);
         const int64_t tiles_m = m / t, tiles_n = up(n, t) / t, tiles = tiles_m * tiles_n;
         const int64_t most = std::max<int64_t>(
-            1, std::min<int64_t>({steps / 8, 64, 2 * slots / tiles}));
+            1, std::min<int64_t>({steps / 4, 64, 2 * slots / tiles}));
         for (int64_t s = 1; s <= most; ++s) {
             const double join = s == 1 ? 0.0 : 4.0 + (double)(s * m) * (double)n * 8.0 / 4.5e6;
             const double us = (double)((tiles * s + slots - 1) / slots) *
                                   ((double)((steps + s - 1) / s) * step_us(wide, P) + 3.0) + join;
             if (us < least) {
                 least = us;
-                best = {wide, (int32_t)tiles_m, (int32_t)tiles_n, (int32_t)s};
+                best = {wide, (int32_t)tiles_n, (int32_t)s};
             }
         }
     }
@@ -900,21 +923,30 @@ Plan plan_of(const XentCall &c) {
     return p;
 }
 
-template <int P, bool AK>
-void launch_product(hipStream_t s, const XentPack &k, const Operand &a, const Operand &b, Cut cut,
-                    int64_t m, int64_t steps, int64_t m_first, Out o) {
-    cut.tiles_m = (int32_t)(m / (cut.wide ? 256 : 128));
-    o.splits = cut.splits;
-    const dim3 g((uint32_t)cut.tiles_m * cut.tiles_n * cut.splits);
-    if (cut.wide)
-        hipLaunchKernelGGL((k_xent_product<P, AK, Wide>), g, dim3(512), (LDS_TILES<P, Wide>), s, k,
-                           a, b, cut.tiles_m, cut.tiles_n, steps, m_first, o);
+// Workgroups of a product of m rows.
+uint32_t product_groups(const Cut &c, int64_t m) {
+    return (uint32_t)(m / (c.wide ? 256 : 128)) * c.tiles_n * c.splits;
+}
+Product product_of(const Operand &a, const Operand &b, const Cut &c, int64_t m, int64_t steps,
+                   int64_t m_first, Out o) {
+    o.splits = c.splits;
+    return {a, b, (int32_t)(m / (c.wide ? 256 : 128)), c.tiles_n, steps, m_first, o};
+}
+// Rows of it that a later kernel joins.
+uint32_t rows_to_join(const Product &q, int64_t m) {
+    return q.o.last && q.o.splits > 1 && q.m_first < q.o.rows
+               ? (uint32_t)std::min(m, q.o.rows - q.m_first) : 0;
+}
+template <int P>
+void launch_products(hipStream_t s, const XentPack &k, bool wide, const Product &dh,
+                     uint32_t dh_groups, const Product &dw, uint32_t dw_groups) {
+    const dim3 g(dh_groups + dw_groups);
+    if (wide)
+        hipLaunchKernelGGL((k_xent_products<P, Wide>), g, dim3(512), (LDS_TILES<P, Wide>), s, k, dh,
+                           dh_groups, dw);
     else
-        hipLaunchKernelGGL((k_xent_product<P, AK, Narrow>), g, dim3(256), (LDS_TILES<P, Narrow>), s,
-                           k, a, b, cut.tiles_m, cut.tiles_n, steps, m_first, o);
-    if (o.last && o.splits > 1 && m_first < o.rows)
-        hipLaunchKernelGGL((k_xent_join_splits<P>), dim3((uint32_t)std::min(m, o.rows - m_first)),
-                           dim3(256), 0, s, k, m_first, o);
+        hipLaunchKernelGGL((k_xent_products<P, Narrow>), g, dim3(256), (LDS_TILES<P, Narrow>), s, k,
+                           dh, dh_groups, dw);
 }
 
 template <int P, class C>
@@ -956,10 +988,8 @@ hipError_t run(hipStream_t s, const XentCall &c, const Plan &p, char *m) {
                          reinterpret_cast<const void *>(k_xent_stats<P, Narrow>),
                          reinterpret_cast<const void *>(k_xent_g<P, Wide>),
                          reinterpret_cast<const void *>(k_xent_g<P, Narrow>),
-                         reinterpret_cast<const void *>(k_xent_product<P, true, Wide>),
-                         reinterpret_cast<const void *>(k_xent_product<P, true, Narrow>),
-                         reinterpret_cast<const void *>(k_xent_product<P, false, Wide>),
-                         reinterpret_cast<const void *>(k_xent_product<P, false, Narrow>)};
+                         reinterpret_cast<const void *>(k_xent_products<P, Wide>),
+                         reinterpret_cast<const void *>(k_xent_products<P, Narrow>)};
     for (const void *f : big) {
         const hipError_t e = allow_all_lds(f);
         if (e != hipSuccess) return e;
@@ -989,22 +1019,31 @@ hipError_t run(hipStream_t s, const XentCall &c, const Plan &p, char *m) {
             if (p.wide_g) launch_g<P, Wide>(s, k, v0, nv, r0, nr, plane, c.num_cus, lse2, g, part_db);
             else launch_g<P, Narrow>(s, k, v0, nv, r0, nr, plane, c.num_cus, lse2, g, part_db);
             const Operand ag{g, plane, nr};
-            if (c.dh)
-                launch_product<P, false>(
-                    s, k, ag, {k.w + v0 * k.ld, k.v_pad * k.ld, k.ld}, p.dh, nr, nv / step, r0,
-                    Out{reinterpret_cast<float *>(m + p.dh_acc), k.n_pad, v0 == 0,
-                        v0 + nv == k.v_pad, 1, c.dh, k.n, c.h_stride, false});
-            if (c.dw)
-                launch_product<P, true>(
-                    s, k, ag, {k.hg + r0 * k.ld, k.n_pad * k.ld, k.ld}, p.dw, nv, nr / step, v0,
-                    Out{reinterpret_cast<float *>(m + p.dw_acc), k.v_pad, r0 == 0,
-                        r0 + nr == k.n_pad, 1, c.dw, k.v, c.w_stride, true});
-            if (c.dbias) {
-                const int64_t live = std::min(nv, k.v - v0);
-                // a part is 64 rows, of either tiling
-                hipLaunchKernelGGL(k_xent_join_db, dim3(blocks(live, 256)), b, 0, s, k, v0, live,
-                                   (int32_t)(nr / 64), part_db, r0 == 0, c.dbias);
+            const Product dh = product_of(
+                ag, {k.w + v0 * k.ld, k.v_pad * k.ld, k.ld}, p.dh, nr, nv / step, r0,
+                Out{reinterpret_cast<float *>(m + p.dh_acc), k.n_pad, v0 == 0, v0 + nv == k.v_pad, 1,
+                    c.dh, k.n, c.h_stride, false});
+            const Product dw = product_of(
+                ag, {k.hg + r0 * k.ld, k.n_pad * k.ld, k.ld}, p.dw, nv, nr / step, v0,
+                Out{reinterpret_cast<float *>(m + p.dw_acc), k.v_pad, r0 == 0, r0 + nr == k.n_pad, 1,
+                    c.dw, k.v, c.w_stride, true});
+            const uint32_t dh_groups = c.dh ? product_groups(p.dh, nr) : 0;
+            const uint32_t dw_groups = c.dw ? product_groups(p.dw, nv) : 0;
+            if (p.dh.wide == p.dw.wide && dh_groups && dw_groups) {
+                launch_products<P>(s, k, p.dh.wide, dh, dh_groups, dw, dw_groups);
+            } else {
+                if (dh_groups) launch_products<P>(s, k, p.dh.wide, dh, dh_groups, dw, 0);
+                if (dw_groups) launch_products<P>(s, k, p.dw.wide, dh, 0, dw, dw_groups);
             }
+            const uint32_t dh_rows = c.dh ? rows_to_join(dh, nr) : 0;
+            const uint32_t dw_rows = c.dw ? rows_to_join(dw, nv) : 0;
+            const int64_t live = std::min(nv, k.v - v0);
+            const uint32_t db_groups = c.dbias ? blocks(live, 256) : 0;
+            // a part of db is 64 rows, of either tiling
+            if (dh_rows + dw_rows + db_groups)
+                hipLaunchKernelGGL((k_xent_finish<P>), dim3(dh_rows + dw_rows + db_groups), b, 0, s,
+                                   k, dh_rows, r0, dh.o, dw_rows, v0, dw.o, v0, live,
+                                   (int32_t)(nr / 64), part_db, r0 == 0, c.dbias);
         }
     return hipGetLastError();
 }
