@@ -86,7 +86,7 @@ int mbk_context_create(int32_t device, mbk_context **out, char **err);
  * graph.  Their scratch belongs to the context: it grows outside a capture only (a captured call that needs more is
  * refused: make one of the same sizes before), what a graph has captured is kept
  * until the context is destroyed, and graphs of one context must not run at the same time
- * as each other or as its other calls. */
+ * as each other or as its other calls.  Calls on one context must not overlap. */
 int mbk_context_create_on(int32_t device, void *stream, mbk_context **out, char **err);
 void mbk_context_destroy(mbk_context *ctx);
 int mbk_device_alloc(mbk_context *ctx, size_t bytes, void **out, char **err);
@@ -303,7 +303,8 @@ int mbk_treeshap(mbk_context *ctx, const int32_t *feature, const float *threshol
  * loss and dh are 0, and what its h holds reaches nothing but its own lse (which may be
  * NaN where h holds NaN, infinities or values beyond 2^60).  A class
  * whose bias is -INFINITY is not offered: what its w holds reaches nothing, its dw
- * and dbias are 0.  With no class offered every lse is -INFINITY and every row is out.
+ * and dbias are 0; a row whose label it is has a loss of +INFINITY, and its gradients have no
+ * term of the label.  With no class offered every lse is -INFINITY and every row is out.
  * Other h, w and bias must be finite for finite results.  Sums are f32; bf16 operands
  * are multiplied as they are and g with 11 bits, f32 operands and g with 22 bits, where
  * elements below 2^-38 of the largest of their row (h) or of all (w) count as 0.  The
