@@ -734,18 +734,32 @@ __global__ __launch_bounds__(256) void k_expert_combine(ExpertPlan p, const T *_
     T *data = static_cast<T *>(out.data);
     for (int32_t f0 = blockIdx.y * TILE; f0 < out.cols; f0 += gridDim.y * TILE) {
         if (SCOLS) {
-#pragma unroll 2
-            for (int q = wave; q < TILE; q += 4) {
-                if (i0 + q >= p.rows || f0 + lane >= out.cols) continue;
-                float sum = 0.0f;
+            // eight of the wavefront's rows at once, so that their loads are on the way together
+            constexpr int H = Q / 2;
+#pragma unroll 1
+            for (int q0 = wave; q0 < TILE; q0 += 4 * H) {
+                float sum[H];
+#pragma unroll
+                for (int q = 0; q < H; ++q) sum[q] = 0.0f;
                 for (int j = 0; j < p.k; ++j) {
-                    const int64_t a = (i0 + q) * p.k + j;
-                    const Place at = place_of(p, a, out.cols, out.blocked);
-                    if (at.base < 0) continue;
-                    const float v = to_f32(sorted[at.base + (f0 + lane) * at.step]);
-                    sum += weights ? weights[a] * v : v;
+                    int32_t s[H];
+                    float v[H], w[H];
+#pragma unroll
+                    for (int q = 0; q < H; ++q) {
+                        const int64_t i = i0 + q0 + 4 * q, a = i * p.k + j;
+                        s[q] = i < p.rows ? p.slot[a] : -1;
+                        w[q] = weights && i < p.rows ? weights[a] : 1.0f;
+                    }
+#pragma unroll
+                    for (int q = 0; q < H; ++q)
+                        v[q] = s[q] >= 0 && f0 + lane < out.cols
+                                   ? to_f32(sorted[(int64_t)s[q] * out.cols + f0 + lane]) : 0.0f;
+#pragma unroll
+                    for (int q = 0; q < H; ++q)
+                        if (s[q] >= 0) sum[q] += w[q] * v[q];
                 }
-                tile[q][lane] = sum;
+#pragma unroll
+                for (int q = 0; q < H; ++q) tile[q0 + 4 * q][lane] = sum[q];
             }
         } else if (i0 + lane < p.rows) {
             float sum[Q];
