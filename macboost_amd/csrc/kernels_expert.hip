@@ -703,12 +703,18 @@ __global__ __launch_bounds__(256) void k_expert_gather(ExpertPlan p, ExpertMatri
         }
         __syncthreads();
         if (SCOLS) {
-            for (int q = wave; q < TILE; q += 4) {
-                if (i0 + q >= p.rows || f0 + lane >= x.cols) continue;
-                for (int j = 0; j < p.k; ++j) {
-                    const Place at = place_of(p, (i0 + q) * p.k + j, x.cols, x.blocked);
-                    if (at.base >= 0) sorted[at.base + (f0 + lane) * at.step] = tile[q][lane];
+            constexpr int Q = TILE / 4;
+            for (int j = 0; j < p.k; ++j) {
+                int32_t s[Q];
+#pragma unroll
+                for (int q = 0; q < Q; ++q) {
+                    const int64_t i = i0 + wave + 4 * q;
+                    s[q] = i < p.rows && f0 + lane < x.cols ? p.slot[i * p.k + j] : -1;
                 }
+#pragma unroll
+                for (int q = 0; q < Q; ++q)
+                    if (s[q] >= 0)
+                        sorted[(int64_t)s[q] * x.cols + f0 + lane] = tile[wave + 4 * q][lane];
             }
         } else if (i0 + lane < p.rows) {
             for (int j = 0; j < p.k; ++j) {
@@ -803,7 +809,7 @@ __global__ __launch_bounds__(256) void k_expert_combine(ExpertPlan p, const T *_
 // own columns in f32, and the threads of a row are added in a fixed order.  With few rows their
 // k go to workgroups of their own (1775 x 8 rows of 2 bf16 77 us by 28 workgroups).
 template <typename T, bool XCOLS, bool SCOLS>
-__global__ __launch_bounds__(256) void k_expert_combine_grad(
+__global__ __launch_bounds__(256, 4) void k_expert_combine_grad(
     ExpertPlan p, ExpertMatrix dout, const T *__restrict__ sorted,
     const float *__restrict__ weights, T *__restrict__ d_sorted, float *__restrict__ d_weights) {
     __shared__ T tile[TILE][TILE + 1];
@@ -816,6 +822,15 @@ __global__ __launch_bounds__(256) void k_expert_combine_grad(
         float dot[SCOLS ? TILE / 4 : 1];
 #pragma unroll
         for (int q = 0; q < (SCOLS ? TILE / 4 : 1); ++q) dot[q] = 0.0f;
+        int32_t s[SCOLS ? TILE / 4 : 1];
+        float wt[SCOLS ? TILE / 4 : 1];
+        if constexpr (SCOLS)
+#pragma unroll
+            for (int q = 0; q < TILE / 4; ++q) {
+                const int64_t i = i0 + wave + 4 * q, a = i * p.k + j;
+                s[q] = i < p.rows ? p.slot[a] : -1;
+                wt[q] = weights && i < p.rows ? weights[a] : 1.0f;
+            }
         Place mine{-1, 0};
         float w = 1.0f;
         if (!SCOLS && i0 + lane < p.rows) {
@@ -832,17 +847,26 @@ __global__ __launch_bounds__(256) void k_expert_combine_grad(
             }
             __syncthreads();
             if constexpr (SCOLS) {
+                // eight rows at once, so that their loads are on the way together
+                constexpr int H = TILE / 8;
 #pragma unroll
-                for (int q = 0; q < TILE / 4; ++q) {
-                    const int r = wave + 4 * q;
-                    if (i0 + r >= p.rows || f0 + lane >= dout.cols) continue;
-                    const int64_t a = (i0 + r) * p.k + j;
-                    const Place at = place_of(p, a, dout.cols, dout.blocked);
-                    if (at.base < 0) continue;
-                    const float g = to_f32(tile[r][lane]);
-                    const int64_t k = at.base + (f0 + lane) * at.step;
-                    dot[q] += g * to_f32(sorted[k]);
-                    d_sorted[k] = (T)((weights ? weights[a] : 1.0f) * g);
+                for (int q0 = 0; q0 < TILE / 4; q0 += H) {
+                    int64_t at[H];
+                    float v[H];
+#pragma unroll
+                    for (int q = 0; q < H; ++q) {
+                        int32_t slot = f0 + lane < dout.cols ? s[q0 + q] : -1;
+                        asm volatile("" : "+v"(slot));   // places are not kept over f0: registers
+                        at[q] = slot < 0 ? -1 : (int64_t)slot * dout.cols + f0 + lane;
+                        v[q] = slot < 0 ? 0.0f : to_f32(sorted[at[q]]);
+                    }
+#pragma unroll
+                    for (int q = 0; q < H; ++q) {
+                        if (at[q] < 0) continue;
+                        const float g = to_f32(tile[wave + 4 * (q0 + q)][lane]);
+                        dot[q0 + q] += g * v[q];
+                        d_sorted[at[q]] = (T)(wt[q0 + q] * g);
+                    }
                 }
             } else if (mine.base >= 0) {
 #pragma unroll 4
@@ -856,13 +880,20 @@ __global__ __launch_bounds__(256) void k_expert_combine_grad(
             }
         }
         if constexpr (SCOLS) {
+            // each exchange halves the rows a lane holds
 #pragma unroll
-            for (int q = 0; q < TILE / 4; ++q) {
-                float s = dot[q];
-                for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-                if (lane == 0 && i0 + wave + 4 * q < p.rows)
-                    d_weights[(i0 + wave + 4 * q) * p.k + j] = s;
-            }
+            for (int n = TILE / 8, o = 32; n > 0; n >>= 1, o >>= 1)
+#pragma unroll
+                for (int q = 0; q < n; ++q) {
+                    const bool upper = lane & o;
+                    const float keep = upper ? dot[q + n] : dot[q], give = upper ? dot[q] : dot[q + n];
+                    dot[q] = keep + __shfl_xor(give, o, 64);
+                }
+            dot[0] += __shfl_xor(dot[0], 2, 64);
+            dot[0] += __shfl_xor(dot[0], 1, 64);
+            const int64_t i = i0 + wave + 4 * ((lane >> 5 & 1) * 8 + (lane >> 4 & 1) * 4 +
+                                               (lane >> 3 & 1) * 2 + (lane >> 2 & 1));
+            if ((lane & 3) == 0 && i < p.rows) d_weights[i * p.k + j] = dot[0];
         } else {
             sums[lane][wave] = dot[0];
             __syncthreads();

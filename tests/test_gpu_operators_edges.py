@@ -8,6 +8,7 @@ import pytest
 
 import device_ops as D
 import macboost_amd as mb
+from macboost_amd import _core
 from test_gpu_operators import Hip, _experts, _problem, ctx      # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -131,7 +132,7 @@ def test_captured_calls_of_each_form(kind, n, d, v):
         other.grad()                                # the same scratch, in between
         err, clear = ctypes.c_char_p(), np.zeros(n, np.float32)
         for p in (x.loss, x.lse):
-            assert D._core.lib().mbk_copy_to_device(c.ptr, p, clear.ctypes.data, clear.nbytes,
+            assert _core.lib().mbk_copy_to_device(c.ptr, p, clear.ctypes.data, clear.nbytes,
                                                     ctypes.byref(err)) == 0
         hip("hipGraphLaunch", run, stream)
         got = x.results()
@@ -208,3 +209,59 @@ def test_many_choices_and_experts(ctx, kind, major, blocked, rows, cols, k, expe
     copies = (slot >= 0).sum(1)[:, None]
     exact = a.astype(np.float64) * copies
     assert np.all(np.abs(got - exact) <= np.abs(exact) * ((k + 1) * 2.0 ** -24 + D.HALF[kind]) + 1e-37)
+
+
+@KINDS
+@pytest.mark.parametrize("blocked", [False, True])
+@pytest.mark.parametrize("order", ["columns", "rows"])
+def test_elements_apart(ctx, kind, blocked, order):
+    """Rows' matrices whose elements are three apart in either direction."""
+    rows, cols, k, experts = 150, 70, 2, 6
+    rng, e = _experts(3, rows, k, experts)
+    x = D.Experts(ctx, e, experts)
+    x.sort()
+    offsets, source, slot = D.sort_reference(e, experts)
+    kept, slots = int(offsets[-1]), rows * k
+    dtype = np.uint16 if kind == "bf16" else np.float32
+    stride = (3 * cols + 4, 3) if order == "columns" else (3, 3 * rows + 4)
+    at = np.arange(rows)[:, None] * stride[0] + np.arange(cols)[None, :] * stride[1]
+    size = int(at.max()) + 1
+
+    def matrix(values, fill):
+        flat = np.full(size, fill, np.float32)
+        flat[at] = values
+        p = ctx.upload(D.encode(flat, kind))
+        return p, _core.MbkExpertMatrix(p, *stride, cols, _core.BF16 if kind == "bf16" else _core.F32,
+                                        int(blocked))
+
+    a = D.rounded(rng.standard_normal((rows, cols)).astype(np.float32), kind)
+    y = D.rounded(rng.standard_normal((slots, cols)).astype(np.float32), kind)
+    weights = rng.standard_normal((rows, k)).astype(np.float32)
+    plan, wdev = ctypes.byref(x.plan), ctx.upload(weights)
+    out, dy = (ctx.upload(D.encode(np.full(slots * cols, 7.0, np.float32), kind)) for _ in range(2))
+    ydev, dw = ctx.upload(D.encode(D.to_sorted(y, offsets, blocked), kind)), ctx.alloc(slots * 4)
+    _, m = matrix(a, np.nan)
+    back, mback = matrix(np.zeros((rows, cols), np.float32), 7.0)
+    ctx.call("mbk_expert_gather", plan, ctypes.byref(m), out)
+    ctx.call("mbk_expert_combine", plan, ydev, wdev, ctypes.byref(mback))
+    ctx.call("mbk_expert_combine_grad", plan, ctypes.byref(m), ydev, wdev, dy, dw)
+    ctx.sync()
+    row_of = source[:kept] // k
+    for p, rows_of in ((out, a[row_of]),
+                       (dy, D.rounded(weights.reshape(-1)[source[:kept], None] * a[row_of], kind))):
+        want = np.full((slots, cols), 7.0, np.float32)
+        want[:kept] = rows_of
+        got = D.decode(ctx.download(p, slots * cols, dtype), kind)
+        assert np.array_equal(got, D.to_sorted(want, offsets, blocked))
+    flat = D.decode(ctx.download(back, size, dtype), kind)
+    terms = np.where(slot[..., None] >= 0, y[slot].astype(np.float64), 0.0)
+    exact = (terms * weights[..., None]).sum(1)
+    tol = (np.abs(terms) * np.abs(weights)[..., None]).sum(1) * (k + 1) * 2.0 ** -24
+    tol += (np.abs(exact) + tol) * D.HALF[kind]
+    assert np.all(np.abs(flat[at] - exact) <= tol)
+    between = np.ones(size, bool)
+    between[at] = False
+    assert np.all(flat[between] == 7.0)
+    prod = a[:, None, :].astype(np.float64) * terms
+    got = ctx.download(dw, (rows, k), np.float32)
+    assert np.all(np.abs(got - prod.sum(2)) <= np.abs(prod).sum(2) * (cols + 2) * 2.0 ** -24)
