@@ -83,10 +83,11 @@ int mbk_context_create(int32_t device, mbk_context **out, char **err);
  * stream (a hipStream_t of `device`; NULL: its default stream), in order with the
  * caller's own work there.  The stream must outlive the context.
  * mbk_xent, mbk_xent_grad and the mbk_expert_ calls may be captured there into a
- * graph.  Their scratch belongs to the context: it grows outside a capture only (a captured call that needs more is
- * refused: make one of the same sizes before), what a graph has captured is kept
- * until the context is destroyed, and graphs of one context must not run at the same time
- * as each other or as its other calls.  Calls on one context must not overlap. */
+ * graph.  Their scratch belongs to the context: it grows outside a capture only (a
+ * captured call that needs more is refused: make one of the same sizes before), what a
+ * graph has captured is kept until the context is destroyed, and graphs of one context
+ * must not run at the same time as each other or as its other calls.  These calls may come
+ * from several threads at once: they share the stream. */
 int mbk_context_create_on(int32_t device, void *stream, mbk_context **out, char **err);
 void mbk_context_destroy(mbk_context *ctx);
 int mbk_device_alloc(mbk_context *ctx, size_t bytes, void **out, char **err);

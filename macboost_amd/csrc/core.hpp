@@ -29,6 +29,7 @@ int context_cus(const mbk_context *ctx);
 // current: one block that grows.  A block that a captured graph may replay on is kept
 // until the context ends, and growing under capture is refused.
 char *context_scratch(mbk_context *ctx, size_t bytes);
+std::mutex &context_scratch_mutex(mbk_context *ctx);     // held while a call queues its work
 
 // A named range on the ROCm tracer's marker timeline (rocprofv3
 // --marker-trace) around one phase of host work; free when no tool listens.

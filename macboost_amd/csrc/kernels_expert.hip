@@ -196,8 +196,9 @@ __global__ __launch_bounds__(64 * SORT_WAVES) void k_expert_place(
 }
 
 // Up to CHUNK_EXPERTS experts (their counters of eight wavefronts fit LDS beside the chunk;
-// 10M assignments to 2048 145 us, 188 by wavefronts; to 1024 83 and 164): a workgroup takes chunks of assignments, orders each in
-// LDS by (expert, assignment) and writes source from there, in runs.  (10M assignments to
+// 10M assignments to 2048 145 us, 188 by wavefronts; to 1024 83 and 164): a workgroup takes
+// chunks of assignments, orders each in LDS by (expert, assignment) and writes source from
+// there, in runs.  (10M assignments to
 // 1000 experts: with a wavefront a unit and single writes 88 us, 304 MB written for 80:
 // the part of source that an XCD writes at once does not fit its L2.)
 // R times 64 assignments a wavefront: 16, or 4 where that would leave most CUs idle (131k

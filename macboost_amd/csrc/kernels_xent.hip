@@ -97,8 +97,9 @@ constexpr int MAX_WAVES = 8;              // of the kernels that find a maximum
 // The kernels that prepare take a wavefront a row, over the rows in turns.
 // Classes: the padded bias, whether any is offered, the largest |W|.
 template <typename T>
-__global__ __launch_bounds__(64 * MAX_WAVES) void k_xent_classes(XentPack k, const void *w, int64_t stride,
-                                                      const float *__restrict__ bias) {
+__global__ __launch_bounds__(64 * MAX_WAVES) void k_xent_classes(XentPack k, const void *w,
+                                                                 int64_t stride,
+                                                                 const float *__restrict__ bias) {
     const int lane = threadIdx.x & 63;
     const int align = alignment<T>(w, stride);
     uint32_t m = 0;
@@ -106,7 +107,8 @@ __global__ __launch_bounds__(64 * MAX_WAVES) void k_xent_classes(XentPack k, con
     // four rows at a time, so that as many loads are on the way
     constexpr int ROWS = 4;
     const int64_t hop = (int64_t)gridDim.x * MAX_WAVES;
-    for (int64_t v0 = (int64_t)blockIdx.x * MAX_WAVES + (threadIdx.x >> 6); v0 < k.v_pad; v0 += ROWS * hop) {
+    for (int64_t v0 = (int64_t)blockIdx.x * MAX_WAVES + (threadIdx.x >> 6); v0 < k.v_pad;
+         v0 += ROWS * hop) {
         int32_t d[ROWS];
 #pragma unroll
         for (int q = 0; q < ROWS; ++q) {
@@ -843,7 +845,7 @@ struct Cut {
     bool wide;
     int32_t tiles_n, splits;
 };
-// The least time by the steps of the workgroups' rounds, 3 us for a workgroup's start and
+// The least time, four steps a workgroup at least, by the steps of the workgroups' rounds, 3 us for a workgroup's start and
 // end, and what the parts of a split k take to be written, read and joined.  (f32, with
 // gradients: 256 x 512 x 40000 360 us, 1115 without splits.)
 Cut cut_of(bool wide_allowed, int P, int64_t m, int64_t n, int64_t steps, int num_cus) {

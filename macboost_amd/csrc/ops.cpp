@@ -1,7 +1,8 @@
 // ops.cpp — the seam's operators beside the tree build: the loss over many classes
 // (mbk_xent, mbk_xent_grad) and rows sorted by expert (mbk_expert_*).  Each call
-// checks its arguments (the context last), queues its kernels on the context's stream and returns; it
-// allocates only when it needs more scratch than the context holds.
+// checks its arguments (the context last), queues its kernels on the context's stream and
+// returns; it allocates only when it needs more scratch than the context holds.  Calls that
+// use scratch are queued whole, one after another, whichever threads make them.
 #include "../../include/macboost.h"
 #include "abi.hpp"
 #include "core.hpp"
@@ -52,6 +53,7 @@ void run_xent(mbk_context *ctx, mbk::XentCall c) {
     need(ctx != nullptr, "null kernel-seam context");
     c.num_cus = mb::context_cus(ctx);
     mb::OnDevice here(mb::context_device(ctx));
+    std::lock_guard<std::mutex> lock(mb::context_scratch_mutex(ctx));
     char *scratch = mb::context_scratch(ctx, mbk::xent_scratch(c));
     MB_HIP(mbk::launch_xent(mb::context_stream(ctx), c, scratch));
 }
@@ -112,6 +114,7 @@ int mbk_expert_sort(mbk_context *ctx, const mbk_expert_plan *plan, char **err) {
         need(ctx != nullptr, "null kernel-seam context");
         mb::OnDevice here(mb::context_device(ctx));
         const int cus = mb::context_cus(ctx);
+        std::lock_guard<std::mutex> lock(mb::context_scratch_mutex(ctx));
         char *scratch = mb::context_scratch(ctx, mbk::expert_scratch(p, cus));
         MB_HIP(mbk::launch_expert_sort(mb::context_stream(ctx), p, cus, scratch));
         return 0;

@@ -73,6 +73,7 @@ struct Scratch {
     DevBuf<char> ops;
     std::vector<DevBuf<char>> ops_before;            // outgrown, but in a captured graph
     bool ops_captured = false;
+    std::mutex ops_mu;
 };
 
 }  // namespace
@@ -243,6 +244,8 @@ namespace mb {
 int context_device(const mbk_context *ctx) { return ctx->dev->id; }
 hipStream_t context_stream(const mbk_context *ctx) { return ctx->dev->stream; }
 int context_cus(const mbk_context *ctx) { return ctx->dev->num_cus; }
+
+std::mutex &context_scratch_mutex(mbk_context *ctx) { return ctx->scratch.ops_mu; }
 
 char *context_scratch(mbk_context *ctx, size_t bytes) {
     Scratch &sc = ctx->scratch;

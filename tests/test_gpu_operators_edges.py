@@ -178,6 +178,32 @@ def test_two_contexts_at_once():
                 assert np.array_equal(r[name], want[i][name]), name
 
 
+def test_one_context_from_two_threads():
+    c = mb.Context(0)
+    calls = []
+    for s, n, d, v in ((1, 300, 60, 900), (2, 700, 250, 3000)):          # the second outgrows the first
+        _, h, w, y = _problem(s, n, d, v)
+        calls.append((D.Xent(c, h, w, y, "f32"), D.xent_reference(h, w, y, "f32")))
+    failed = []
+
+    def work(x):
+        try:
+            for _ in range(30):
+                x.grad()
+        except Exception as e:                      # noqa: BLE001
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(x,)) for x, _ in calls]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+    for x, want in calls:
+        D.check(x.results(), want)
+    c.close()
+
+
 @KINDS
 @pytest.mark.parametrize("major", ["row", "feature"])
 @pytest.mark.parametrize("blocked", [False, True])
