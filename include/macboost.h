@@ -306,7 +306,8 @@ int mbk_treeshap(mbk_context *ctx, const int32_t *feature, const float *threshol
  * whose bias is -INFINITY is not offered: what its w holds reaches nothing, its dw
  * and dbias are 0; a row whose label it is has a loss of +INFINITY, and its gradients have no
  * term of the label.  With no class offered every lse is -INFINITY and every row is out.
- * Other h, w and bias must be finite for finite results.  Sums are f32; bf16 operands
+ * Other h, w and bias must be finite for finite results.  A score is rounded to f32 with its
+ * bias, which may have any finite value.  Sums are f32; bf16 operands
  * are multiplied as they are and g with 11 bits, f32 operands and g with 22 bits, where
  * elements below 2^-38 of the largest of their row (h) or of all (w) count as 0.  The
  * results do not depend on the call, bit for bit.

@@ -116,7 +116,7 @@ __global__ __launch_bounds__(64 * MAX_WAVES) void k_xent_classes(XentPack k, con
             const float b = v < k.v ? (bias ? bias[v] : 0.0f) : -INFINITY;
             d[q] = b != -INFINITY ? k.d : 0;
             any = any || d[q] > 0;
-            if (lane == 0 && v < k.v_pad) k.bias[v] = b * LOG2E;
+            if (lane == 0 && v < k.v_pad) k.bias[v] = b;
         }
         for (int32_t f = lane * 8; f < k.d; f += 512) {
             float x[ROWS][8];
@@ -205,7 +205,7 @@ __global__ __launch_bounds__(64 * MAX_WAVES) void k_xent_pack(XentPack k, XentCa
         const int s = scale_exp(m);
         if (wt != 0.0f) hg = max(hg, finite_bits(wt * __uint_as_float(m)));
         if (lane == 0) {
-            k.row_scale[i] = ldexpf(LOG2E, -(s + sw));
+            k.row_scale[i] = ldexpf(1.0f, -(s + sw));
             k.label[i] = y;
             k.weight[i] = wt;
         }
@@ -452,7 +452,7 @@ __device__ __forceinline__ void tile_of(uint32_t id, uint32_t total, uint32_t ti
 // The product is W h' (classes down, rows across), so that a lane has scores of one
 // row: the maximum and sum stay in registers over the classes of a split, and only
 // two lanes and two wavefronts have parts of a row.  part[2 * split + half][row]: the
-// maximum of z log2 e, and the sum of its powers of 2.
+// maximum of z, and the sum of exp(z - it).
 template <int P, class C>
 __global__ __launch_bounds__(C::WAVES * 64, 2) void k_xent_stats(XentPack k, int32_t row_tiles,
                                                                  int32_t class_tiles,
@@ -494,12 +494,12 @@ __global__ __launch_bounds__(C::WAVES * 64, 2) void k_xent_stats(XentPack k, int
         for (int x = 0; x < C::MT; ++x)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                const f32x4 b2 = *reinterpret_cast<const f32x4 *>(bias + x * 32 + q * 8);
+                const f32x4 b = *reinterpret_cast<const f32x4 *>(bias + x * 32 + q * 8);
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
 #pragma unroll
                     for (int y = 0; y < C::NT; ++y) {
-                        const float z = __builtin_fmaf(acc[x][y][q * 4 + e], sc[y], b2[e]);
+                        const float z = __builtin_fmaf(acc[x][y][q * 4 + e], sc[y], b[e]);
                         acc[x][y][q * 4 + e] = z;
                         top[y] = fmaxf(top[y], z);
                     }
@@ -507,12 +507,12 @@ __global__ __launch_bounds__(C::WAVES * 64, 2) void k_xent_stats(XentPack k, int
 #pragma unroll
         for (int y = 0; y < C::NT; ++y) {
             const float ref = top[y] == -INFINITY ? 0.0f : top[y];
-            float sum[2] = {s[y] * __builtin_amdgcn_exp2f(m[y] - ref), 0.0f};
+            float sum[2] = {s[y] * exp_of(m[y] - ref), 0.0f};
 #pragma unroll
             for (int x = 0; x < C::MT; ++x)
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
-                    sum[r & 1] += __builtin_amdgcn_exp2f(acc[x][y][r] - ref);
+                    sum[r & 1] += exp_of(acc[x][y][r] - ref);
             m[y] = top[y];
             s[y] = sum[0] + sum[1];
         }
@@ -523,20 +523,19 @@ __global__ __launch_bounds__(C::WAVES * 64, 2) void k_xent_stats(XentPack k, int
     for (int y = 0; y < C::NT; ++y) {
         const float m2 = __shfl_xor(m[y], 32, 64), s2 = __shfl_xor(s[y], 32, 64);
         const float top = fmaxf(m[y], m2), ref = top == -INFINITY ? 0.0f : top;
-        const float sum = s[y] * __builtin_amdgcn_exp2f(m[y] - ref) +
-                          s2 * __builtin_amdgcn_exp2f(m2 - ref);
+        const float sum = s[y] * exp_of(m[y] - ref) + s2 * exp_of(m2 - ref);
         if (lane < 32)
             part[(2 * split + wave / C::WN) * k.n_pad + row[y]] = make_float2(top, sum);
     }
 }
 
-// The parts of a row joined, one wavefront a row: lse and loss.  The label's score is
-// summed in f32 from h and W themselves.  For gradients, h is packed once more as dW's product
+// The parts of a row joined, one wavefront a row: lse, as reference and log2 of the sum for
+// the gradients, and loss.  The label's score is summed in f32 from h and W themselves.  For gradients, h is packed once more as dW's product
 // takes it, times the row's weight and with one scale for all rows (they are summed over).
 template <typename T>
 __global__ __launch_bounds__(256) void k_xent_join(XentPack k, XentCall c, int32_t parts,
                                                    const float2 *__restrict__ part,
-                                                   float *__restrict__ lse2) {
+                                                   float2 *__restrict__ lse2) {
     const int lane = threadIdx.x & 63;
     const int64_t i = (int64_t)group_id() * 4 + (threadIdx.x >> 6);
     if (i >= k.n_pad) return;
@@ -544,7 +543,7 @@ __global__ __launch_bounds__(256) void k_xent_join(XentPack k, XentCall c, int32
     for (int p = lane; p < parts; p += 64) {
         const float2 q = part[p * k.n_pad + i];
         const float now = fmaxf(top, q.x), ref = now == -INFINITY ? 0.0f : now;
-        sum = sum * __builtin_amdgcn_exp2f(top - ref) + q.y * __builtin_amdgcn_exp2f(q.x - ref);
+        sum = sum * exp_of(top - ref) + q.y * exp_of(q.x - ref);
         top = now;
     }
     const int32_t y = k.label[i];
@@ -557,7 +556,7 @@ __global__ __launch_bounds__(256) void k_xent_join(XentPack k, XentCall c, int32
     for (int o = 32; o > 0; o >>= 1) {
         const float t2 = __shfl_xor(top, o, 64), s2 = __shfl_xor(sum, o, 64);
         const float now = fmaxf(top, t2), ref = now == -INFINITY ? 0.0f : now;
-        sum = sum * __builtin_amdgcn_exp2f(top - ref) + s2 * __builtin_amdgcn_exp2f(t2 - ref);
+        sum = sum * exp_of(top - ref) + s2 * exp_of(t2 - ref);
         top = now;
         dot += __shfl_xor(dot, o, 64);
     }
@@ -574,12 +573,12 @@ __global__ __launch_bounds__(256) void k_xent_join(XentPack k, XentCall c, int32
         }
     }
     if (lane != 0) return;
-    const LogSum l = log_sum(top, sum);
-    lse2[i] = l.base2;
+    const LogSum l = log_sum(sum);
+    lse2[i] = make_float2(top, l.base2);
     if (i >= k.n) return;
-    const float lse = y == -2 ? NAN : l.natural, z = open ? dot + (c.bias ? c.bias[y] : 0.0f) : -INFINITY;
-    c.lse[i] = lse;
-    c.loss[i] = y < 0 ? 0.0f : k.weight[i] * (lse - z);
+    const float z = open ? dot + (c.bias ? c.bias[y] : 0.0f) : -INFINITY;
+    c.lse[i] = y == -2 ? NAN : lse_of(top, l);
+    c.loss[i] = y < 0 ? 0.0f : k.weight[i] * loss_of(top, l, z);
 }
 
 // ---- pass 2: G of a piece ------------------------------------------------------------
@@ -591,7 +590,7 @@ __global__ __launch_bounds__(C::WAVES * 64, 2) void k_xent_g(XentPack k, int64_t
                                                              int64_t rows_pad, int64_t plane,
                                                              int32_t row_tiles,
                                                              int32_t class_tiles, int32_t splits,
-                                                             const float *__restrict__ lse2,
+                                                             const float2 *__restrict__ lse2,
                                                              u16 *__restrict__ g,
                                                              float *__restrict__ part_db) {
     extern __shared__ char lds[];
@@ -602,14 +601,16 @@ __global__ __launch_bounds__(C::WAVES * 64, 2) void k_xent_g(XentPack k, int64_t
     const int64_t i0 = r0 + (int64_t)row_tile * C::T;
     const Operand a{k.w, k.v_pad * k.ld, k.ld}, b{k.h, k.n_pad * k.ld, k.ld};
     const int64_t iw = i0 + wave % C::WN * C::NT * 32;
-    float sc[C::NT], l[C::NT], wt[C::NT];
+    float sc[C::NT], ref[C::NT], l[C::NT], wt[C::NT];
     int32_t label[C::NT];
 #pragma unroll
     for (int y = 0; y < C::NT; ++y) {
         const int64_t i = iw + y * 32 + (lane & 31);
         sc[y] = k.row_scale[i];
         label[y] = k.label[i];
-        l[y] = label[y] < 0 ? INFINITY : lse2[i];        // a row that is out: 2^-inf
+        const float2 lse = lse2[i];
+        ref[y] = label[y] < 0 ? 0.0f : lse.x;
+        l[y] = label[y] < 0 ? INFINITY : lse.y;          // a row that is out: 2^-inf
         wt[y] = k.weight[i];
     }
     const uint32_t mine = half * 4 * (uint32_t)rows_pad + (lane & 31);
@@ -631,12 +632,13 @@ __global__ __launch_bounds__(C::WAVES * 64, 2) void k_xent_g(XentPack k, int64_t
                 u16 *to = g + (c - v0) * rows_pad + (iw - r0) + y * 32;
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                    const f32x4 b2 =
+                    const f32x4 b =
                         *reinterpret_cast<const f32x4 *>(k.bias + c + half * 4 + q * 8);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
+                        const float z = __builtin_fmaf(acc[x][y][q * 4 + e], sc[y], b[e]);
                         float p = __builtin_amdgcn_exp2f(
-                            __builtin_fmaf(acc[x][y][q * 4 + e], sc[y], b2[e] - l[y]));
+                            __builtin_fmaf(z - ref[y], LOG2E, -l[y]));
                         if (hot && at == q * 8 + e) p -= 1.0f;
                         db[q * 4 + e] = y == 0 ? p * wt[y]
                                                : __builtin_fmaf(p, wt[y], db[q * 4 + e]);
@@ -907,7 +909,7 @@ Plan plan_of(const XentCall &c) {
     p.scale = take((size_t)4 * p.n_pad);
     p.label = take((size_t)4 * p.n_pad);
     p.weight = take((size_t)4 * p.n_pad);
-    p.lse = take((size_t)4 * p.n_pad);
+    p.lse = take((size_t)8 * p.n_pad);
     p.part = take((size_t)16 * p.splits * p.n_pad);
     if (c.grad) {
         p.wide_g = p.wide && wide_tiles(p.piece_rows, p.piece_classes, c.num_cus);
@@ -959,7 +961,7 @@ void launch_stats(hipStream_t s, const XentPack &k, int32_t splits, float2 *part
 }
 template <int P, class C>
 void launch_g(hipStream_t s, const XentPack &k, int64_t v0, int64_t nv, int64_t r0, int64_t nr,
-              int64_t plane, int num_cus, const float *lse2, u16 *g, float *part_db) {
+              int64_t plane, int num_cus, const float2 *lse2, u16 *g, float *part_db) {
     const int32_t rt = (int32_t)(nr / C::T), vt = (int32_t)(nv / C::T);
     const int32_t splits = splits_of(C::T == 256, rt, vt, num_cus);
     hipLaunchKernelGGL((k_xent_g<P, C>), dim3((uint32_t)rt * splits), dim3(C::WAVES * 64),
@@ -983,7 +985,7 @@ hipError_t run(hipStream_t s, const XentCall &c, const Plan &p, char *m) {
     k.row_scale = reinterpret_cast<float *>(m + p.scale);
     k.label = reinterpret_cast<int32_t *>(m + p.label);
     k.weight = reinterpret_cast<float *>(m + p.weight);
-    float *lse2 = reinterpret_cast<float *>(m + p.lse);
+    float2 *lse2 = reinterpret_cast<float2 *>(m + p.lse);
     float2 *part = reinterpret_cast<float2 *>(m + p.part);
     const dim3 b(256);
     const void *big[] = {reinterpret_cast<const void *>(k_xent_stats<P, Wide>),

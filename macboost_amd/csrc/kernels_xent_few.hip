@@ -34,11 +34,11 @@ constexpr int ROWS = 32;
 
 __device__ __forceinline__ void join2(float &top, float &sum, float t2, float s2) {
     const float now = fmaxf(top, t2), ref = now == -INFINITY ? 0.0f : now;
-    sum = sum * __builtin_amdgcn_exp2f(top - ref) + s2 * __builtin_amdgcn_exp2f(t2 - ref);
+    sum = sum * exp_of(top - ref) + s2 * exp_of(t2 - ref);
     top = now;
 }
 
-// part[workgroup][row]: the maximum of z log2 e and the sum of its powers of 2.
+// part[workgroup][row]: the maximum of z and the sum of exp(z - it).
 // B: bytes of W a lane copies at a time, what its rows' alignment allows (2: by registers).
 template <typename T, int B>
 __global__ __launch_bounds__(64 * WAVES, 2) void k_few_stats(XentCall c, int64_t tiles, int32_t steps,
@@ -160,13 +160,13 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_few_stats(XentCall c, int64_t
             if (v >= c.classes) b = -INFINITY;
             else if (c.bias) b = c.bias[v];
             // a class that is not offered, whatever its w gave
-            s[r] = b == -INFINITY ? -INFINITY : __builtin_fmaf(s[r], LOG2E, b * LOG2E);
+            s[r] = b == -INFINITY ? -INFINITY : s[r] + b;
             m = fmaxf(m, s[r]);
         }
         const float ref = m == -INFINITY ? 0.0f : m;
-        sum *= __builtin_amdgcn_exp2f(top - ref);
+        sum *= exp_of(top - ref);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) sum += __builtin_amdgcn_exp2f(s[r] - ref);
+        for (int r = 0; r < 16; ++r) sum += exp_of(s[r] - ref);
         top = m;
     }
     join2(top, sum, __shfl_xor(top, 32, 64), __shfl_xor(sum, 32, 64));
@@ -184,11 +184,11 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_few_stats(XentCall c, int64_t
 }
 
 // One wavefront a row: the parts joined, and the label's score from h and W.  lse2: the
-// logarithm in base 2, +inf for a row that is out (NULL: not wanted).
+// reference and log2 of the sum, +inf for a row that is out (NULL: not wanted).
 template <typename T>
 __global__ __launch_bounds__(64) void k_few_join(XentCall c, int32_t parts,
                                                  const float2 *__restrict__ part,
-                                                 float *__restrict__ lse2) {
+                                                 float2 *__restrict__ lse2) {
     const int lane = threadIdx.x;
     const int64_t i = blockIdx.x;
     const int32_t y = c.labels[i];
@@ -208,12 +208,11 @@ __global__ __launch_bounds__(64) void k_few_join(XentCall c, int32_t parts,
     }
     if (lane != 0) return;
     const bool none = top == -INFINITY && sum == 0.0f;
-    const LogSum l = log_sum(top, sum);
-    const float lse = l.natural;
-    c.lse[i] = lse;
+    const LogSum l = log_sum(sum);
+    c.lse[i] = lse_of(top, l);
     const bool out = y < 0 || y >= c.classes || wt == 0.0f || none;
-    c.loss[i] = out ? 0.0f : wt * (lse - (dot + by));
-    if (lse2) lse2[i] = out ? INFINITY : l.base2;
+    c.loss[i] = out ? 0.0f : wt * loss_of(top, l, dot + by);
+    if (lse2) lse2[i] = out ? make_float2(0.0f, INFINITY) : make_float2(top, l.base2);
 }
 
 // ---- gradients -------------------------------------------------------------------------
@@ -273,7 +272,7 @@ __device__ __forceinline__ void store(char *m, const Staged<N> &s, int chunks) {
 template <typename T, int B, int NB>
 __global__ __launch_bounds__(64 * GRAD_WAVES, NB == 1 ? 4 : 2) void k_few_grad(XentCall c, int64_t tiles,
                                                                  int32_t chunks,
-                                                                 const float *__restrict__ lse2,
+                                                                 const float2 *__restrict__ lse2,
                                                                  float *__restrict__ part_dh) {
     constexpr int PER = 16 / sizeof(T);
     extern __shared__ char lds[];
@@ -287,7 +286,7 @@ __global__ __launch_bounds__(64 * GRAD_WAVES, NB == 1 ? 4 : 2) void k_few_grad(X
     const int x0 = threadIdx.x >> 4;                 // the row that this lane brings
     Staged<NB * (int)sizeof(T)> staged;
     load<T, sizeof(T)>(staged, chunks, c.dim,
-                       x0 < c.rows && lse2[x0] != INFINITY
+                       x0 < c.rows && lse2[x0].y != INFINITY
                            ? static_cast<const T *>(c.h) + x0 * c.h_stride : nullptr);
     store(h, staged, chunks);
     const auto ask = [&](int64_t t) {
@@ -297,7 +296,7 @@ __global__ __launch_bounds__(64 * GRAD_WAVES, NB == 1 ? 4 : 2) void k_few_grad(X
                        ? static_cast<const T *>(c.w) + v * c.w_stride : nullptr);
     };
     if (blockIdx.x < tiles) ask(blockIdx.x);
-    const float l2 = l < c.rows ? lse2[l] : INFINITY;
+    const float ref = l < c.rows ? lse2[l].x : 0.0f, l2 = l < c.rows ? lse2[l].y : INFINITY;
     const int32_t label = l < c.rows ? c.labels[l] : -1;
     const float wt = l2 == INFINITY ? 0.0f : c.weights ? c.weights[l] : 1.0f;
     f32x16 dh[NB];
@@ -350,7 +349,7 @@ __global__ __launch_bounds__(64 * GRAD_WAVES, NB == 1 ? 4 : 2) void k_few_grad(X
                 if (v < c.classes) b = c.bias ? c.bias[v] : 0.0f;
                 float p = 0.0f;
                 if (l2 != INFINITY && b != -INFINITY) {
-                    p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], LOG2E, b * LOG2E - l2));
+                    p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r] + b - ref, LOG2E, -l2));
                     if (v == label) p -= 1.0f;
                     p *= wt;
                 }
@@ -433,7 +432,7 @@ constexpr int ONE_BLOCK = 32 * GRAD_WAVES;
 int grad_groups(const XentCall &c) { return (c.dim <= ONE_BLOCK ? 2 : 1) * c.num_cus; }
 
 template <typename T, int B, int NB>
-hipError_t run_grad(hipStream_t s, const XentCall &c, const float *lse2, float *part_dh) {
+hipError_t run_grad(hipStream_t s, const XentCall &c, const float2 *lse2, float *part_dh) {
     const hipError_t e = allow_all_lds(reinterpret_cast<const void *>(k_few_grad<T, B, NB>));
     if (e != hipSuccess) return e;
     constexpr int PER = 16 / sizeof(T);
@@ -456,7 +455,8 @@ template <typename T, int B> hipError_t run(hipStream_t s, const XentCall &c, ch
     const int32_t steps = (int32_t)((c.dim * sizeof(T) + 127) / 128);
     const uint32_t groups = (uint32_t)std::min<int64_t>(c.num_cus, (tiles + WAVES - 1) / WAVES);
     float2 *part = reinterpret_cast<float2 *>(scratch);
-    float *lse2 = reinterpret_cast<float *>(scratch + part_bytes(c)), *part_dh = lse2 + ROWS;
+    float2 *lse2 = reinterpret_cast<float2 *>(scratch + part_bytes(c));
+    float *part_dh = reinterpret_cast<float *>(lse2 + ROWS);
     hipLaunchKernelGGL((k_few_stats<T, B>), dim3(groups), dim3(64 * WAVES), LDS_BYTES, s, c, tiles,
                        steps, part);
     hipLaunchKernelGGL((k_few_join<T>), dim3((uint32_t)c.rows), dim3(64), 0, s, c, (int32_t)groups,
@@ -477,7 +477,7 @@ bool xent_few(const XentCall &c) {
 }
 
 size_t xent_few_scratch(const XentCall &c) {
-    return part_bytes(c) + 4 * ROWS + (c.grad ? (size_t)4 * grad_groups(c) * c.rows * c.dim : 0);
+    return part_bytes(c) + 8 * ROWS + (c.grad ? (size_t)4 * grad_groups(c) * c.rows * c.dim : 0);
 }
 
 hipError_t launch_xent_few(hipStream_t s, const XentCall &c, char *scratch) {

@@ -16,8 +16,7 @@
 // lane's own registers, rounded, are its operand, and the read across picks Y's
 // rows in that order: no value moves between lanes.
 //
-// Operands are one f16 term (bf16) or two (f32), as kernels_xent.hip says; exponents are
-// of 2, with log2 e in the scale of S.
+// Operands are one f16 term (bf16) or two (f32), as kernels_xent.hip says.
 //
 // The matrix instructions bound both passes: 20000 x 100 x 10000 f32 takes 268 and 285 us,
 // 1.09 and 1.03 PFLOP/s of f16 products (112 columns of the first and 128 of the second, three
@@ -37,9 +36,10 @@ typedef __attribute__((ext_vector_type(4))) unsigned short u16x4;
 
 constexpr int XB = 128;                  // X rows of a workgroup, 32 a wavefront
 constexpr int TY = 64;                   // Y rows of a tile
-// p = 2^(z - maximum) is kept times 2^13, and the maximum may lag by 2^2, so that p as
+// p = exp(z - maximum) is kept times 2^13, and the maximum may lag by 2 log 2, so that p as
 // f16 terms is at most 2^15 and keeps steps of 2^-38.
-constexpr float P_EXP = 13.0f, LAG = 2.0f;
+constexpr int P_EXP = 13;
+constexpr float LAG = 1.38f;
 
 // Elements of a packed row for KS slabs of 16.
 __host__ __device__ constexpr int row_ld(int ks) { return ks <= 2 ? 32 : ks <= 4 ? 64 : 128; }
@@ -50,13 +50,13 @@ struct Fused {
     int32_t w_groups, hg_groups;         // that look at W, pack h
     XentCtl *ctl;
     u16 *h, *w;                          // planes of n_pad * ld, v_pad * ld
-    float *bias2;                        // [v_pad] bias log2 e, -inf: not offered
+    float *bias;                         // [v_pad] the bias, -inf: not offered
     // of the rows, [n_pad]:
-    float *sc;                           // log2 e times the scale of a score
+    float *sc;                           // the scale of a score
     int32_t *exp;                        // h is packed times 2^exp
     int32_t *label;                      // -1: out, -2: out and not finite
     float *weight;                       // 0: out
-    float *c2;                           // lse log2 e, +inf: out
+    float *ref, *l2;                     // lse as a score and log2 of the sum, +inf: out
     float *wq;                           // weight as the classes pass multiplies with it
 };
 
@@ -92,7 +92,7 @@ __global__ __launch_bounds__(256) void k_fused_classes(Fused k, const void *w, i
         const float b = v < k.v ? (bias ? bias[v] : 0.0f) : -INFINITY;
         const bool open = b != -INFINITY;
         any = any || open;
-        if (f == 0) k.bias2[v] = b * LOG2E;
+        if (f == 0) k.bias[v] = b;
         if (!open) continue;
         float x[4];
         load4<T>(w, v * stride, f, k.d, x);
@@ -124,7 +124,7 @@ __global__ __launch_bounds__(256) void k_fused_pack(Fused k, const void *w, int6
         float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         int s = sw;
         if (of_w) {
-            if (k.bias2[i] != -INFINITY) load4<T>(w, i * w_stride, f, k.d, x);
+            if (k.bias[i] != -INFINITY) load4<T>(w, i * w_stride, f, k.d, x);
         } else {
             if (i < k.n) load4<T>(h, i * h_stride, f, k.d, x);
             int32_t y = i < k.n ? labels[i] : -1;
@@ -152,7 +152,7 @@ __global__ __launch_bounds__(256) void k_fused_pack(Fused k, const void *w, int6
                 k.label[i] = y;
                 k.weight[i] = wt;
                 k.exp[i] = s;
-                k.sc[i] = ldexpf(LOG2E, -(s + sw));
+                k.sc[i] = ldexpf(1.0f, -(s + sw));
                 if (wt != 0.0f) hg = max(hg, finite_bits(wt * __uint_as_float(m)));
             }
         }
@@ -342,7 +342,7 @@ __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 
 
 // ---- rows pass ----------------------------------------------------------------------
 // part_o[split][row][ld], part_ms[split][row] = (reference, sum): sum and O are of
-// 2^(z - reference).
+// 2^13 exp(z - reference).
 template <int P, int KS, bool GRAD>
 __global__ __launch_bounds__(256, 2) void k_fused_rows(Fused k, int32_t splits,
                                                        float *__restrict__ part_o,
@@ -381,7 +381,7 @@ __global__ __launch_bounds__(256, 2) void k_fused_rows(Fused k, int32_t splits,
         char *to = lds + buf * BUF;
         load_tile<P, LD>(k.w + t * TY * LD, k.v_pad * LD, to, wave);
         if (wave == 0)
-            __builtin_amdgcn_global_load_lds((global_void *)(k.bias2 + t * TY + lane),
+            __builtin_amdgcn_global_load_lds((global_void *)(k.bias + t * TY + lane),
                                              (lds_void *)(to + TILE_BYTES<P, LD>), 4, 0, 0);
     };
     if (first < last) load(first, 0);
@@ -396,35 +396,34 @@ __global__ __launch_bounds__(256, 2) void k_fused_rows(Fused k, int32_t splits,
         static_assert(BUF % 256 == 0, "reads across xor the low bits of the address");
         auto block = [&](auto where) {
             constexpr int y = decltype(where)::value;
-            float b2[16];
-            of_rows(bias, y, b2);
+            float b[16];
+            of_rows(bias, y, b);
             f32x16 s = first_product<P, KS>(tile, y, x);
             float m = -INFINITY;
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                s[r] = __builtin_fmaf(s[r], sc, b2[r]);
+                s[r] = __builtin_fmaf(s[r], sc, b[r]);
                 m = fmaxf(m, s[r]);
             }
             // a new maximum: what was summed so far is brought to it
             if (__any(m > top + LAG)) {
                 const float now = fmaxf(top, fmaxf(m, other_half(m)));
                 if (now > top) {
-                    const float to = now - P_EXP;
-                    const float scale = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ref - to);
+                    const float scale = top == -INFINITY ? 0.0f : exp_of(top - now);
                     sum *= scale;
                     if constexpr (GRAD)
 #pragma unroll
                         for (int j = 0; j < JT; ++j)
 #pragma unroll
                             for (int r = 0; r < 16; ++r) o[j][r] *= scale;
-                    ref = to;
-                    top = now;
+                    ref = top = now;
                 }
             }
             float p[2][8], part[2] = {0.0f, 0.0f};
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                p[r >> 3][r & 7] = __builtin_amdgcn_exp2f(s[r] - ref);
+                p[r >> 3][r & 7] =
+                    __builtin_amdgcn_exp2f(__builtin_fmaf(s[r] - ref, LOG2E, (float)P_EXP));
                 part[r & 1] += p[r >> 3][r & 7];
             }
             sum += part[0] + part[1];
@@ -435,7 +434,7 @@ __global__ __launch_bounds__(256, 2) void k_fused_rows(Fused k, int32_t splits,
     }
     sum += other_half(sum);
     const int64_t at = split * k.n_pad + row;
-    if (half == 0) part_ms[at] = make_float2(top == -INFINITY ? -INFINITY : ref, sum);
+    if (half == 0) part_ms[at] = make_float2(top, sum);
     if constexpr (GRAD) {
         float *out = part_o + at * LD;
 #pragma unroll
@@ -458,7 +457,7 @@ __global__ __launch_bounds__(256) void k_fused_join_rows(Fused k, XentCall c, in
     if (i >= k.n_pad) return;
     const int f = threadIdx.x % LANES * 4;
     const int32_t y = k.label[i];
-    const bool open = y >= 0 && k.bias2[y] != -INFINITY;
+    const bool open = y >= 0 && k.bias[y] != -INFINITY;
     float wy[4] = {0.0f, 0.0f, 0.0f, 0.0f}, dot = 0.0f;
     if (open)
 #pragma unroll
@@ -477,7 +476,7 @@ __global__ __launch_bounds__(256) void k_fused_join_rows(Fused k, XentCall c, in
 #pragma unroll 4
     for (int s = 0; s < splits; ++s) {
         const float2 ms = part_ms[s * k.n_pad + i];
-        const float scale = none ? 1.0f : __builtin_amdgcn_exp2f(ms.x - ref);
+        const float scale = none ? 1.0f : exp_of(ms.x - ref);
         sum += ms.y * scale;
         if constexpr (GRAD) {
             const float4 p = *reinterpret_cast<const float4 *>(part_o + (s * k.n_pad + i) * LD + f);
@@ -487,17 +486,17 @@ __global__ __launch_bounds__(256) void k_fused_join_rows(Fused k, XentCall c, in
             o[3] += p.w * scale;
         }
     }
-    const LogSum l = log_sum(ref, sum);
+    const LogSum l = log_sum(sum, P_EXP);
     const float wt = k.weight[i];
     if (f == 0) {
         if (i < k.n) {
-            const float lse = y == -2 ? NAN : l.natural;
             const float z = open ? dot + (c.bias ? c.bias[y] : 0.0f) : -INFINITY;
-            c.lse[i] = lse;
-            c.loss[i] = y < 0 ? 0.0f : wt * (lse - z);
+            c.lse[i] = y == -2 ? NAN : lse_of(ref, l);
+            c.loss[i] = y < 0 ? 0.0f : wt * loss_of(ref, l, z);
         }
         if constexpr (GRAD) {
-            k.c2[i] = y < 0 ? INFINITY : l.base2;
+            k.ref[i] = y < 0 ? 0.0f : ref;
+            k.l2[i] = y < 0 ? INFINITY : l.base2;
             // weight 2^-exp and the power of two that brings the largest below 2^15
             const float q = ldexpf(wt, wq_exp(k.ctl->hg.all) - k.exp[i]);
             k.wq[i] = fminf(fmaxf(q, -60000.0f), 60000.0f);
@@ -517,13 +516,14 @@ __global__ __launch_bounds__(256) void k_fused_join_rows(Fused k, XentCall c, in
 
 // ---- classes pass ---------------------------------------------------------------------
 // part[split][class][ld] of dW, part_db[split][class]
+constexpr int ROW_ARRAYS = 6;            // of a tile's rows: sc, ref, wq, label, weight, l2
 template <int P, int KS>
 __global__ __launch_bounds__(256, 2) void k_fused_classes_pass(Fused k, int32_t splits,
                                                                float *__restrict__ part,
                                                                float *__restrict__ part_db) {
     constexpr int LD = row_ld(KS), JT = (KS + 1) / 2;
-    constexpr int ROWS_AT = TILE_BYTES<P, LD>;           // sc, c2, wq, label, weight
-    constexpr int BUF = ROWS_AT + 5 * TY * 4;
+    constexpr int ROWS_AT = TILE_BYTES<P, LD>;           // ROW_ARRAYS of them
+    constexpr int BUF = ROWS_AT + ROW_ARRAYS * TY * 4;
     extern __shared__ char lds[];
     const int lane = threadIdx.x & 63, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -539,7 +539,7 @@ __global__ __launch_bounds__(256, 2) void k_fused_classes_pass(Fused k, int32_t 
         for (int p = 0; p < P; ++p)
             x[s][p] = *reinterpret_cast<const u32x4 *>(k.w + p * k.v_pad * LD + v * LD + s * 16 +
                                                        half * 8);
-    const float b2 = k.bias2[v];
+    const float b = k.bias[v];
     double db = 0.0;                     // of sums over 32 rows
     f32x16 o[JT];
 #pragma unroll
@@ -550,9 +550,9 @@ __global__ __launch_bounds__(256, 2) void k_fused_classes_pass(Fused k, int32_t 
     auto load = [&](int64_t t, int buf) {
         char *to = lds + buf * BUF;
         load_tile<P, LD>(k.h + t * TY * LD, k.n_pad * LD, to, wave);
-        const void *rows[5] = {k.sc, k.c2, k.wq, k.label, k.weight};
+        const void *rows[ROW_ARRAYS] = {k.sc, k.ref, k.wq, k.label, k.weight, k.l2};
 #pragma unroll
-        for (int q = 0; q < 5; ++q)
+        for (int q = 0; q < ROW_ARRAYS; ++q)
             if (wave == (q & 3))
                 __builtin_amdgcn_global_load_lds(
                     (global_void *)(static_cast<const float *>(rows[q]) + t * TY + lane),
@@ -565,8 +565,8 @@ __global__ __launch_bounds__(256, 2) void k_fused_classes_pass(Fused k, int32_t 
         __syncthreads();
         if (t + 1 < last) load(t + 1, buf ^ 1);
         const char *tile = lds + buf * BUF;
-        const float *sc = reinterpret_cast<const float *>(tile + ROWS_AT), *c2 = sc + TY,
-                    *wq = sc + 2 * TY, *weight = sc + 4 * TY;
+        const float *sc = reinterpret_cast<const float *>(tile + ROWS_AT), *ref = sc + TY,
+                    *wq = sc + 2 * TY, *weight = sc + 4 * TY, *l2 = sc + 5 * TY;
         const int32_t *label = reinterpret_cast<const int32_t *>(sc + 3 * TY);
         const uint32_t at = lds_address(tile) + across_at<LD>();
         static_assert(BUF % 256 == 0, "reads across xor the low bits of the address");
@@ -576,12 +576,15 @@ __global__ __launch_bounds__(256, 2) void k_fused_classes_pass(Fused k, int32_t 
             const bool hot = __any(mine >= 0 && mine < 32);
             f32x16 s = first_product<P, KS>(tile, y, x);
             float p[2][8], of[16], of2[16];
-            of_rows(c2, y, of);
-            of_rows(sc, y, of2);
+            of_rows(sc, y, of);
+            of_rows(ref, y, of2);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], of[r], b) - of2[r];
+            of_rows(l2, y, of);
 #pragma unroll
             for (int r = 0; r < 16; ++r)
-                p[r >> 3][r & 7] = __builtin_amdgcn_exp2f(
-                    __builtin_fmaf(s[r], of2[r], b2 - of[r]));
+                p[r >> 3][r & 7] =
+                    __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], LOG2E, -of[r]));
             if (hot) {
                 int32_t l[16];
                 of_rows(label, y, l);
@@ -659,7 +662,7 @@ __global__ __launch_bounds__(256) void k_fused_join_classes(Fused k, XentCall c,
         }
     }
     if (v >= k.v) return;
-    const bool open = k.bias2[v] != -INFINITY;
+    const bool open = k.bias[v] != -INFINITY;
     const float scale = ldexpf(1.0f, -wq_exp(k.ctl->hg.all));
     const float x[4] = {sum.x, sum.y, sum.z, sum.w};
     if (c.dw)
@@ -697,7 +700,7 @@ struct Plan {
     int P, ks;
     int64_t n_pad, v_pad, ld;
     int32_t row_splits, class_splits;
-    size_t ctl, h, w, bias2, rows, part_ms, part, part_db, end;
+    size_t ctl, h, w, bias, rows, part_ms, part, part_db, end;
 };
 
 Plan plan_of(const XentCall &c) {
@@ -718,8 +721,8 @@ Plan plan_of(const XentCall &c) {
     p.ctl = take(sizeof(XentCtl));
     p.h = take((size_t)2 * p.P * p.n_pad * p.ld);
     p.w = take((size_t)2 * p.P * p.v_pad * p.ld);
-    p.bias2 = take((size_t)4 * p.v_pad);
-    p.rows = take((size_t)6 * 4 * p.n_pad);
+    p.bias = take((size_t)4 * p.v_pad);
+    p.rows = take((size_t)7 * 4 * p.n_pad);
     p.part_ms = take((size_t)8 * p.row_splits * p.n_pad);
     if (c.grad) {
         p.part = take((size_t)4 * p.ld * std::max(p.row_splits * p.n_pad, p.class_splits * p.v_pad));
@@ -741,20 +744,21 @@ hipError_t run(hipStream_t s, const XentCall &c, const Plan &p, char *m) {
     k.ctl = reinterpret_cast<XentCtl *>(m + p.ctl);
     k.h = reinterpret_cast<u16 *>(m + p.h);
     k.w = reinterpret_cast<u16 *>(m + p.w);
-    k.bias2 = reinterpret_cast<float *>(m + p.bias2);
+    k.bias = reinterpret_cast<float *>(m + p.bias);
     float *rows = reinterpret_cast<float *>(m + p.rows);
     k.sc = rows;
     k.exp = reinterpret_cast<int32_t *>(rows + p.n_pad);
     k.label = reinterpret_cast<int32_t *>(rows + 2 * p.n_pad);
     k.weight = rows + 3 * p.n_pad;
-    k.c2 = rows + 4 * p.n_pad;
-    k.wq = rows + 5 * p.n_pad;
+    k.ref = rows + 4 * p.n_pad;
+    k.l2 = rows + 5 * p.n_pad;
+    k.wq = rows + 6 * p.n_pad;
     float2 *part_ms = reinterpret_cast<float2 *>(m + p.part_ms);
     float *part = reinterpret_cast<float *>(m + p.part);
     float *part_db = reinterpret_cast<float *>(m + p.part_db);
     const dim3 b(256);
     const size_t lds_rows = 2 * (TILE_BYTES<P, LD> + TY * 4);
-    const size_t lds_classes = 2 * (TILE_BYTES<P, LD> + 5 * TY * 4);
+    const size_t lds_classes = 2 * (TILE_BYTES<P, LD> + ROW_ARRAYS * TY * 4);
     const void *big[] = {reinterpret_cast<const void *>(k_fused_rows<P, KS, true>),
                          reinterpret_cast<const void *>(k_fused_rows<P, KS, false>),
                          reinterpret_cast<const void *>(k_fused_classes_pass<P, KS>)};

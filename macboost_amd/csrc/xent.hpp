@@ -102,8 +102,8 @@ struct XentPack {
     int32_t w_groups, pack_w_groups, hg_groups;      // that look at W, pack W, pack h
     XentCtl *ctl;
     u16 *h, *hg, *w;                     // planes of n_pad * ld, v_pad * ld; hg: gradients only
-    float *bias;                         // [v_pad] bias log2 e, -inf: not offered
-    float *row_scale;                    // [n_pad] log2 e times the scale of a score
+    float *bias;                         // [v_pad] the bias, -inf: not offered
+    float *row_scale;                    // [n_pad] the scale of a score
     int32_t *label;                      // [n_pad], -1: out, -2: out and not finite
     float *weight;                       // [n_pad], 0: out
 };
@@ -118,20 +118,34 @@ __device__ __forceinline__ f32x16 mma(const u32x4 (&a)[P], const u32x4 (&b)[P], 
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a0, b0, c, 0, 0, 0);
 }
 
-// The logarithm of 2^ref times sum, base 2 and base e: the exponent apart, since the
-// logarithm instruction rounds down, by up to a step of a result of 2^4.  Scores carry
-// LOG2E as f32 holds it, which the second undoes.
+// Scores are kept as they are, base e: times log2 e a finite bias below -2.4e38 would become
+// the -inf of a class that is not offered.  What is left of a score behind its row's
+// maximum takes the factor.
+__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * LOG2E); }
+
+// A row's sum of exp(z - reference), as its logarithm apart from the reference: together in one
+// f32 a reference of 2^24 would leave nothing of it.
 struct LogSum {
-    float base2, natural;
+    float base2;
+    double natural;
 };
-__device__ __forceinline__ LogSum log_sum(float ref, float sum) {
+// Of sum / 2^shift.  The exponent apart, since the logarithm instruction rounds down, by up to
+// a step of a result of 2^4.
+__device__ __forceinline__ LogSum log_sum(float sum, int shift = 0) {
     if (!(sum > 0.0f && sum < INFINITY)) {
-        const float l = (ref == -INFINITY ? 0.0f : ref) + log2f(sum);
+        const float l = log2f(sum);
         return {l, l};
     }
-    const int e = __builtin_amdgcn_frexp_expf(sum);
-    const double l = (double)ref + e + log2f(__builtin_amdgcn_frexp_mantf(sum));
-    return {(float)l, (float)(l / (double)LOG2E)};
+    const int e = __builtin_amdgcn_frexp_expf(sum) - shift;
+    const double l = (double)e + log2f(__builtin_amdgcn_frexp_mantf(sum));
+    return {(float)l, l * 0.693147180559945309};
+}
+// lse and, of a score z, lse - z.
+__device__ __forceinline__ float lse_of(float ref, const LogSum &l) {
+    return (float)((ref == -INFINITY ? 0.0 : (double)ref) + l.natural);
+}
+__device__ __forceinline__ float loss_of(float ref, const LogSum &l, float z) {
+    return (float)(((double)ref - z) + l.natural);
 }
 
 // ---- copies from memory to LDS

@@ -1,0 +1,110 @@
+"""Numbers at the ends of their range in the many-class loss, on either side of 32 rows and of
+128 outputs."""
+import numpy as np
+import pytest
+
+import device_ops as D
+from test_gpu_operators import _problem, ctx      # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+KINDS = pytest.mark.parametrize("kind", ["f32", "bf16"])
+FORMS = pytest.mark.parametrize("n,d", [(11, 24), (32, 300), (33, 24), (60, 128), (60, 200)])
+LOWEST = np.finfo(np.float32).min
+U = 2.0 ** -24
+
+
+def _biased_reference(h, w, y, kind, bias):
+    """The loss and its gradients in 64 bits of scores that are rounded to f32 with their
+    bias, and how far each may be off.  A class's score is off by its operands' and its
+    sum's half steps and by a step of the rounding with the bias, but where a rounding that
+    large goes one way for all classes of a probability, as here, by the dot product's alone:
+    a bias beyond 2^60 leaves nothing of a dot product of this size."""
+    h, w = D.rounded(h, kind).astype(np.float64), D.rounded(w, kind).astype(np.float64)
+    n, d = h.shape
+    v = w.shape[0]
+    b = np.asarray(bias, np.float32).astype(np.float64)
+    huge = np.abs(b) > 2.0 ** 60
+    split = 0.0 if kind == "bf16" else 3 * 2.0 ** -22
+    products = 1 if kind == "bf16" else 3
+    dot = h @ w.T
+    z = np.where(huge, b, dot + b)
+    ez = (np.abs(h) @ np.abs(w).T) * (split + (products * d + 16) * U) + np.abs(z) * 2 * U
+    ez[:, huge] = 0.0
+    top = z.max(1, keepdims=True)
+    e = np.exp(z - top)
+    total = e.sum(1, keepdims=True)
+    p = e / total
+    rows = np.arange(n)
+    # log's sum is off by the mean of its terms' errors and its own f32 sum of v terms
+    esum = (p * ez).sum(1) * 1.01 + (v + 32) * U
+    lse = top[:, 0] + np.log(total[:, 0])
+    elz = esum + 4 * U * np.maximum(1, np.abs(lse))
+    loss = (top[:, 0] - z[rows, y]) + np.log(total[:, 0])
+    eloss = esum + ez[rows, y] + 4 * U * np.abs(loss) + 4 * U * np.log(v)
+    g = p.copy()
+    g[rows, y] -= 1
+    half = 2.0 ** -11 if kind == "bf16" else 2.0 ** -22
+    dist = np.where(p > 0, np.minimum(top - z, 200.0), 0)
+    eg = p * (ez + esum[:, None] + (3 * dist + 16) * U) + np.abs(g) * half + 2.0 ** -37
+    out = {"lse": (lse, elz), "loss": (loss, eloss)}
+    off_h = 2.0 ** -11 if kind == "bf16" else 0.0
+
+    def product(left, right, e_left, terms, off):
+        return (e_left @ np.abs(right)
+                + (np.abs(left) @ np.abs(right)) * (split + off + (products * terms + 16) * U))
+
+    for name, value, err in (("dh", g @ w, product(g, w, eg, v, 0.0)),
+                             ("dw", g.T @ h, product(g.T, h, eg.T, n, off_h)),
+                             ("db", g.sum(0), eg.sum(0) + np.abs(g).sum(0) * (n + 4) * U)):
+        step = D.HALF[kind] if name != "db" else U
+        out[name] = (value, err + (np.abs(value) + err) * step)
+    # tolerances that could not pass anything else
+    for name in ("dh", "dw"):
+        value, tol = out[name]
+        assert tol.sum() < 0.1 * np.abs(value).sum(), name
+    return out
+
+
+BIASES = {
+    "labels_masked": lambda v: np.where(np.arange(v) % 3 == 0, LOWEST, 0.0),
+    "all_lowest": lambda v: np.full(v, LOWEST),
+    "one_kept_of_low": lambda v: np.where(np.arange(v) == 4, -2.5e38, LOWEST),
+    "all_low_two_kinds": lambda v: np.where(np.arange(v) % 2 == 0, -2.5e38, LOWEST),
+    "high": lambda v: np.where(np.arange(v) % 2 == 0, 3e38, 0.0),
+    "both_ends": lambda v: np.where(np.arange(v) % 2 == 0, -LOWEST, LOWEST),
+}
+
+
+@KINDS
+@FORMS
+@pytest.mark.parametrize("what", ["labels_masked", "all_lowest", "one_kept_of_low",
+                                  "all_low_two_kinds", "high"])
+def test_finite_biases(ctx, kind, n, d, what):
+    """A class is not offered if its bias is -inf, and only then."""
+    _, h, w, y = _problem(n + d + 40, n, d, 90)
+    bias = BIASES[what](90).astype(np.float32)
+    y[::2] = y[::2] // 3 * 3                          # every second label on a masked class
+    x = D.Xent(ctx, h, w, y, kind, bias)
+    x.grad()
+    got, want = x.results(), _biased_reference(h, w, y, kind, bias)
+    D.check(got, want)
+    x.forward()
+    again = x.results(False)
+    for name in ("loss", "lse"):
+        assert np.array_equal(got[name], again[name])
+
+
+@KINDS
+@FORMS
+def test_biases_of_both_ends(ctx, kind, n, d):
+    """A loss beyond f32 is infinite; lse and the gradients are not."""
+    _, h, w, y = _problem(n + d + 41, n, d, 90)
+    bias = BIASES["both_ends"](90).astype(np.float32)
+    x = D.Xent(ctx, h, w, y, kind, bias)
+    x.grad()
+    got, want = x.results(), _biased_reference(h, w, y, kind, bias)
+    beyond = y % 2 == 1
+    assert np.all(got["loss"][beyond] == np.inf)
+    got["loss"], want["loss"] = got["loss"][~beyond], tuple(t[~beyond] for t in want["loss"])
+    D.check(got, want)
