@@ -508,7 +508,8 @@ __global__ __launch_bounds__(256) void k_fused_join_rows(Fused k, XentCall c, in
 #pragma unroll
         for (int e = 0; e < 4; ++e)
             if (f + e < k.d) {
-                const float g = y < 0 ? 0.0f : wt * (o[e] * scale / sum - wy[e]);
+                // divided first: the sum of 2^13 p W is beyond f32 for W that is not
+                const float g = y < 0 ? 0.0f : wt * (o[e] / sum * scale - wy[e]);
                 static_cast<T *>(c.dh)[i * c.h_stride + f + e] = (T)g;
             }
     }

@@ -108,3 +108,18 @@ def test_biases_of_both_ends(ctx, kind, n, d):
     assert np.all(got["loss"][beyond] == np.inf)
     got["loss"], want["loss"] = got["loss"][~beyond], tuple(t[~beyond] for t in want["loss"])
     D.check(got, want)
+
+
+@KINDS
+@FORMS
+@pytest.mark.parametrize("big", [1e35, 2e36])
+def test_large_class_vectors(ctx, kind, n, d, big):
+    """h and w of reciprocal magnitudes: sums of 90 such w still fit f32."""
+    _, h, w, y = _problem(n + d + 42, n, d, 90)
+    h = (h / np.float32(big)).astype(np.float32)
+    w = (w * np.float32(big)).astype(np.float32)
+    x = D.Xent(ctx, h, w, y, kind)
+    x.grad()
+    want = D.xent_reference(h, w, y, kind)
+    assert np.abs(want["dh"][0]).max() < 1e38
+    D.check(x.results(), want)
