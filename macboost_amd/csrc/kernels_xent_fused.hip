@@ -499,7 +499,8 @@ __global__ __launch_bounds__(256) void k_fused_join_rows(Fused k, XentCall c, in
             k.l2[i] = y < 0 ? INFINITY : l.base2;
             // weight 2^-exp and the power of two that brings the largest below 2^15
             const float q = ldexpf(wt, wq_exp(k.ctl->hg.all) - k.exp[i]);
-            k.wq[i] = fminf(fmaxf(q, -60000.0f), 60000.0f);
+            // a row of zeros has no exponent of its own; a weight that is not finite stays so
+            k.wq[i] = fabsf(wt) < INFINITY ? fminf(fmaxf(q, -60000.0f), 60000.0f) : wt;
         }
     }
     if constexpr (GRAD) {

@@ -123,3 +123,27 @@ def test_large_class_vectors(ctx, kind, n, d, big):
     want = D.xent_reference(h, w, y, kind)
     assert np.abs(want["dh"][0]).max() < 1e38
     D.check(x.results(), want)
+
+
+@KINDS
+@FORMS
+def test_weights_that_are_not_finite(ctx, kind, n, d):
+    _, h, w, y = _problem(n + d + 43, n, d, 70)
+    weights = np.ones(n, np.float32)
+    weights[7] = np.nan
+    x = D.Xent(ctx, h, w, y, kind, weights=weights)
+    x.grad()
+    r = x.results()
+    assert np.isnan(r["loss"][7]) and np.isnan(r["dh"][7]).all()
+    assert np.isnan(r["dw"]).all() and np.isnan(r["db"]).all()
+    keep = np.arange(n) != 7
+    want = D.xent_reference(h, w, y, kind)
+    for name in ("loss", "lse", "dh"):
+        r[name], want[name] = r[name][keep], tuple(t[keep] for t in want[name])
+    D.check(r, want, ("loss", "lse", "dh"))
+    for value in (np.inf, -np.inf):
+        weights[7] = value
+        x = D.Xent(ctx, h, w, y, kind, weights=weights)
+        x.grad()
+        r = x.results()
+        assert not np.isfinite(r["loss"][7]) and not np.isfinite(r["dw"][y[7]]).any()
