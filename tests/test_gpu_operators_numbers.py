@@ -147,3 +147,20 @@ def test_weights_that_are_not_finite(ctx, kind, n, d):
         x.grad()
         r = x.results()
         assert not np.isfinite(r["loss"][7]) and not np.isfinite(r["dw"][y[7]]).any()
+
+
+@KINDS
+@FORMS
+@pytest.mark.parametrize("value", [np.nan, np.inf])
+def test_classes_not_offered_beside_a_row_not_finite(ctx, kind, n, d, value):
+    """What is not offered has gradients of 0, whatever the rows hold."""
+    _, h, w, y = _problem(n + d + 44, n, d, 70)
+    bias = np.zeros(70, np.float32)
+    bias[::7] = -np.inf
+    y = (y // 7 * 7 + 1).astype(np.int32)
+    h[3, 5] = value
+    x = D.Xent(ctx, h, w, y, kind, bias)
+    x.grad()
+    r = x.results()
+    assert np.all(r["dw"][::7] == 0) and np.all(r["db"][::7] == 0)
+    assert not np.isfinite(r["dw"][y[3]]).all()
