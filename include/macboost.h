@@ -302,15 +302,23 @@ int mbk_treeshap(mbk_context *ctx, const int32_t *feature, const float *threshol
  * NULL.  Outputs must not overlap inputs.
  * A row whose label is outside [0, classes) or whose weight is 0 is left out: its
  * loss and dh are 0, and what its h holds reaches nothing but its own lse (which may be
- * NaN where h holds NaN, infinities or values beyond 2^60).  A class
+ * NaN where h holds NaN, infinities or values beyond 2^60, or scores pass 2^100).  A class
  * whose bias is -INFINITY is not offered: what its w holds reaches nothing, its dw
  * and dbias are 0; a row whose label it is has a loss of +INFINITY, and its gradients have no
  * term of the label.  With no class offered every lse is -INFINITY and every row is out.
  * Other h, w and bias must be finite for finite results.  A score is rounded to f32 with its
- * bias, which may have any finite value.  Sums are f32; bf16 operands
- * are multiplied as they are and g with 11 bits, f32 operands and g with 22 bits, where
- * elements below 2^-38 of the largest of their row (h) or of all (w) count as 0.  The
- * results do not depend on the call, bit for bit.
+ * bias, which may have any finite value.  Sums are f32.
+ * Up to 32 rows (of up to 512 outputs in f32, 1024 in bf16) operands are multiplied as they
+ * are and g as f32.  Otherwise f32 operands and g go in with 22 bits, bf16 operands as they
+ * are and beside them g and weight h with 11, and what is far smaller than others beside it is
+ * off by up to
+ *   2^-38 of the largest of its column for w, and for weight h in dw,
+ *   2^-38 of the row's largest |h[j]| max_v |w[v][j]| for h in the scores,
+ *   2^-40 of the weight for g.
+ * Up to 128 outputs, where dw takes the h of the scores, that is 2^(k-38) of the largest of its
+ * column for w and h (of rows brought to one size), if the column's |h| |w| is 2^-2k of the
+ * largest column's, and for a row's share of dw 2^-38 of the largest weight times row.
+ * The results do not depend on the call, bit for bit.
  * To boost output j with them: mbk_quantize with objective 0, preds = dh's column j
  * and labels of 0. */
 enum { MBK_F32 = 0, MBK_BF16 = 1 };

@@ -11,16 +11,23 @@
 // it.
 //
 // Operands.  The matrix instructions take 16-bit operands and add in f32.  All operands go
-// in as f16 terms of x 2^s, s a power of two that puts the largest element of h's row, or
-// of all of W, below 2^14, so that elements down to 2^-38 of it keep a step of their own.
-//   bf16 inputs: one term, which holds their 8 bits as they are (exactly, down to 2^-31 of the
-//   largest).  G is rounded to one f16 term, too, 11 bits: as bf16 terms it would add as
-//   much error again to dh and dW as their own rounding to bf16 (measured 2.8e-3 in place
-//   of 1.7e-3 of their norm), at the same rate.
+// in as f16 terms of x 2^s:
+//   W: s is its column's, and puts the column's largest element below 2^14.
+//   h, for the scores: the columns' powers of W are taken back, and one of the row puts the
+//   largest h_ij max_v |W_vj| below 2^14.
+//   w h, for dW: s is its column's.
+// So columns may be of very different sizes.
+//   bf16 inputs: one term, which holds their 8 bits as they are down to 2^-30 of that
+//   largest.  G is rounded to one f16 term, too, 11 bits, and w h again where there are weights: as
+//   bf16 terms they would add as much error again to dh and dW as their own rounding to bf16
+//   (measured 2.8e-3 in place of 1.7e-3 of their norm), at the same rate.
 //   f32 inputs: two terms, hi + lo, 22 bits, and three products hi hi + hi lo + lo hi: what is
 //   dropped, lo lo and the bits behind lo, is at most 2^-21 of an element's product and
 //   random in sign, the size of what an f32 sum over the same length rounds away.  (f32
 //   operands have an instruction of 1/16 of the rate; three of these cost 3/16.)
+// That holds for elements from 2^-16 of the largest on (f16 has no smaller exponents); below,
+// they are off by up to 2^-38 of it, so that a score is by 2^-21 sum_j |h_ij W_vj| + 2^-37 d
+// max_j (|h_ij| max_v |W_vj|) at most.  G / w is off by up to 2^-40 where that is more.
 //
 // Classes not offered (bias -inf) are packed as zeros, and so are rows that are out
 // (label outside [0, V), weight 0, or no class offered) and hold NaN, infinities or values
@@ -45,8 +52,18 @@ namespace {
 typedef __attribute__((ext_vector_type(8))) unsigned short u16x8;
 
 constexpr int LD_PAD = 128;              // operands' rows are padded to it
-constexpr float G_SCALE = 32768.0f;      // |G / w| <= 1 as f16 terms
+constexpr int G_EXP = 15;                // |G / w| <= 1 goes in times 2^this
 
+// Eight of an array whose length is padded.
+template <typename V> __device__ __forceinline__ void load8(const V *p, int f, V (&x)[8]) {
+    typedef __attribute__((ext_vector_type(4))) V V4;
+    const V4 a = *reinterpret_cast<const V4 *>(p + f), b = *reinterpret_cast<const V4 *>(p + f + 4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        x[e] = a[e];
+        x[e + 4] = b[e];
+    }
+}
 template <typename T> __device__ __forceinline__ float load_f32(const void *p, int64_t i) {
     return (float)static_cast<const T *>(p)[i];
 }
@@ -81,62 +98,141 @@ __device__ __forceinline__ void load8(const void *p, int64_t row, int f, int d, 
 }
 // Eight elements times 2^s into the planes.
 template <typename T>
-__device__ __forceinline__ void pack8(const float (&x)[8], int s, u16 *to, int64_t plane) {
+__device__ __forceinline__ void pack8(const float (&x)[8], const int (&s)[8], u16 *to,
+                                      int64_t plane) {
     u16x8 hi, lo;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         u16 a, b;
-        split_f16(ldexpf(x[e], s), a, b);
+        split_f16(ldexpf(x[e], s[e]), a, b);
         hi[e] = a;
         lo[e] = b;
     }
     *reinterpret_cast<u16x8 *>(to) = hi;
     if (sizeof(T) == 4) *reinterpret_cast<u16x8 *>(to + plane) = lo;
 }
-constexpr int MAX_WAVES = 8;              // of the kernels that find a maximum
-// The kernels that prepare take a wavefront a row, over the rows in turns.
-// Classes: the padded bias, whether any is offered, the largest |W|.
-template <typename T>
-__global__ __launch_bounds__(64 * MAX_WAVES) void k_xent_classes(XentPack k, const void *w,
-                                                                 int64_t stride,
-                                                                 const float *__restrict__ bias) {
-    const int lane = threadIdx.x & 63;
-    const int align = alignment<T>(w, stride);
-    uint32_t m = 0;
-    bool any = false;
-    // four rows at a time, so that as many loads are on the way
-    constexpr int ROWS = 4;
-    const int64_t hop = (int64_t)gridDim.x * MAX_WAVES;
-    for (int64_t v0 = (int64_t)blockIdx.x * MAX_WAVES + (threadIdx.x >> 6); v0 < k.v_pad;
-         v0 += ROWS * hop) {
-        int32_t d[ROWS];
-#pragma unroll
-        for (int q = 0; q < ROWS; ++q) {
-            const int64_t v = v0 + q * hop;
-            const float b = v < k.v ? (bias ? bias[v] : 0.0f) : -INFINITY;
-            d[q] = b != -INFINITY ? k.d : 0;
-            any = any || d[q] > 0;
-            if (lane == 0 && v < k.v_pad) k.bias[v] = b;
-        }
-        for (int32_t f = lane * 8; f < k.d; f += 512) {
-            float x[ROWS][8];
-#pragma unroll
-            for (int q = 0; q < ROWS; ++q)
-                load8<T>(w, (d[q] ? v0 + q * hop : 0) * stride, f, d[q], align, x[q]);
-#pragma unroll
-            for (int q = 0; q < ROWS; ++q)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) m = max(m, finite_bits(x[q][e]));
-        }
-    }
-    __shared__ uint32_t lds[2 * MAX_WAVES];
-    const uint32_t most = largest<MAX_WAVES>(m, any, lds);
-    if (threadIdx.x == 0) k.ctl->w.part[blockIdx.x] = most;
+constexpr int MAX_WAVES = 8;              // of the kernels that prepare
+// Whether row i counts.  A class offered is looked for elsewhere.
+__device__ __forceinline__ bool row_in(const XentPack &k, const XentCall &c, int64_t i, float &wt) {
+    const int32_t y = c.labels[i];
+    wt = c.weights ? c.weights[i] : 1.0f;
+    return y >= 0 && y < k.v && wt != 0.0f;
 }
 
-// The rows of W, times 2^s.
+// The columns' largest: workgroups of W, then (gradients) of the rows' w h, 256 columns
+// each, eight a lane, and two rows a wavefront, in turns.  Those of W also leave the padded bias
+// and whether a class is offered.
+constexpr int COLUMNS = 256, COLUMN_ROWS = 2 * MAX_WAVES, ROWS_AHEAD = 4;
 template <typename T>
-__device__ __forceinline__ void pack_w(const XentPack &k, const void *w, int64_t stride, int s) {
+__global__ __launch_bounds__(64 * MAX_WAVES) void k_xent_columns(XentPack k, XentCall c) {
+    __shared__ uint32_t most[COLUMN_ROWS][COLUMNS];
+    const int lane = threadIdx.x & 31, r = threadIdx.x >> 5;
+    const bool of_w = (int32_t)blockIdx.x < k.w_groups;
+    const int32_t group = of_w ? blockIdx.x : blockIdx.x - k.w_groups;
+    const int64_t stride = of_w ? c.w_stride : c.h_stride, rows = of_w ? k.v_pad : k.n;
+    const void *from = of_w ? c.w : c.h;
+    const int align = alignment<T>(from, stride);
+    const int32_t f = blockIdx.y * COLUMNS + lane * 8;
+    uint32_t m[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    bool any = false;
+    // four rows at a time, so that as many loads are on the way
+    const int64_t hop = (int64_t)(of_w ? k.w_groups : k.hg_groups) * COLUMN_ROWS;
+    for (int64_t v0 = (int64_t)group * COLUMN_ROWS + r; v0 < rows; v0 += ROWS_AHEAD * hop) {
+        float wt[ROWS_AHEAD], x[ROWS_AHEAD][8];
+#pragma unroll
+        for (int q = 0; q < ROWS_AHEAD; ++q) {
+            const int64_t v = v0 + q * hop;
+            const bool here = v < (of_w ? k.v : k.n);
+            load8<T>(from, (here ? v : 0) * stride, f, here ? k.d : 0, align, x[q]);
+            wt[q] = 0.0f;
+            if (of_w) {
+                const float b = here ? (c.bias ? c.bias[v] : 0.0f) : -INFINITY;
+                if (b != -INFINITY) wt[q] = 1.0f;
+                if (lane == 0 && blockIdx.y == 0 && v < k.v_pad) k.bias[v] = b;
+            } else if (here && !row_in(k, c, v, wt[q])) {
+                wt[q] = 0.0f;
+            }
+            any = any || wt[q] != 0.0f;
+        }
+        // times 0 a value that is not finite is none either
+#pragma unroll
+        for (int q = 0; q < ROWS_AHEAD; ++q)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) m[e] = max(m[e], finite_bits(x[q][e] * wt[q]));
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) most[r][lane * 8 + e] = m[e];
+    const bool offered = __syncthreads_or(any);
+    if (of_w && blockIdx.y == 0 && threadIdx.x == 0) k.ctl->offered.part[group] = offered;
+    const int64_t col = (int64_t)blockIdx.y * COLUMNS + threadIdx.x;
+    if (threadIdx.x >= COLUMNS || col >= k.ld) return;
+    uint32_t v = 0;
+#pragma unroll
+    for (int q = 0; q < COLUMN_ROWS; ++q) v = max(v, most[q][threadIdx.x]);
+    (of_w ? k.w_part : k.hg_part)[group * (int64_t)k.ld + col] = v;
+}
+
+// A column's power of two, of the bits of its largest.  A column of W that is all zeros has one
+// that keeps h's column from its rows' scales.
+constexpr int ZERO_COLUMN = 1000;
+__device__ __forceinline__ int32_t column_exp(uint32_t most, bool of_w) {
+    const int e = exponent_of(__uint_as_float(most));
+    return e != NO_EXP ? TOP_EXP - e : of_w ? ZERO_COLUMN : 0;
+}
+// All of them: 64 columns a workgroup, whose wavefronts go over the groups in turns.
+constexpr int SCALE_WAVES = 16;
+__global__ __launch_bounds__(64 * SCALE_WAVES) void k_xent_scales(XentPack k) {
+    __shared__ uint32_t most[SCALE_WAVES][64], words[SCALE_WAVES];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int32_t cols = k.ld / 64;
+    const bool of_w = (int32_t)blockIdx.x < cols;
+    const int64_t col = (int64_t)(of_w ? blockIdx.x : blockIdx.x - cols) * 64 + lane;
+    const uint32_t *part = of_w ? k.w_part : k.hg_part;
+    const int32_t groups = of_w ? k.w_groups : k.hg_groups;
+    uint32_t m = 0;
+#pragma unroll 8
+    for (int g = wave; g < groups; g += SCALE_WAVES) m = max(m, part[(int64_t)g * k.ld + col]);
+    most[wave][lane] = m;
+    if (blockIdx.x == 0) {
+        const uint32_t any = largest_of<SCALE_WAVES>(k.ctl->offered, k.w_groups, words);
+        if (threadIdx.x == 0) k.ctl->offered.all = any;
+    }
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int w = 1; w < SCALE_WAVES; ++w) m = max(m, most[w][lane]);
+    (of_w ? k.w_exp : k.hg_exp)[col] = column_exp(m, of_w);
+}
+// Of few groups and columns, by each workgroup of the next kernel, without a launch (4.5 us):
+// W's in LDS, and both in memory by the first one.
+constexpr int FEW_GROUPS = 32, FEW_COLUMNS = 64 * MAX_WAVES;
+__device__ __forceinline__ bool few_scales(const XentPack &k, int32_t *exps, uint32_t *words) {
+    const int32_t col = threadIdx.x;
+    if (col < k.ld) {
+        uint32_t w = 0, h = 0;
+#pragma unroll 8
+        for (int g = 0; g < k.w_groups; ++g) w = max(w, k.w_part[g * k.ld + col]);
+        exps[col] = column_exp(w, true);
+        if (blockIdx.x == 0) {
+#pragma unroll 8
+            for (int g = 0; g < k.hg_groups; ++g) h = max(h, k.hg_part[g * k.ld + col]);
+            k.w_exp[col] = exps[col];
+            k.hg_exp[col] = column_exp(h, false);
+        }
+    }
+    return largest_of<MAX_WAVES>(k.ctl->offered, k.w_groups, words);
+}
+// Eight columns' powers of W.
+__device__ __forceinline__ void load_exps(const XentPack &k, const int32_t *few, int f,
+                                          int (&s)[8]) {
+    if (k.few) load8<int32_t>(few, f, s);
+    else load8<int32_t>(k.w_exp, f, s);
+}
+
+// The kernels that pack take a wavefront a row, over the rows in turns.
+template <typename T>
+__device__ __forceinline__ void pack_w(const XentPack &k, const void *w, int64_t stride,
+                                       const int32_t *exps) {
     const int lane = threadIdx.x & 63;
     const int align = alignment<T>(w, stride);
     constexpr int ROWS = 2;
@@ -149,9 +245,11 @@ __device__ __forceinline__ void pack_w(const XentPack &k, const void *w, int64_t
             d[q] = v0 + q * hop < k.v && k.bias[v0 + q * hop] != -INFINITY ? k.d : 0;
         for (int32_t f = lane * 8; f < k.ld; f += 512) {
             float x[ROWS][8];
+            int s[8];
 #pragma unroll
             for (int q = 0; q < ROWS; ++q)
                 load8<T>(w, (d[q] ? v0 + q * hop : 0) * stride, f, d[q], align, x[q]);
+            load_exps(k, exps, f, s);
 #pragma unroll
             for (int q = 0; q < ROWS; ++q)
                 if (v0 + q * hop < k.v_pad)
@@ -161,62 +259,67 @@ __device__ __forceinline__ void pack_w(const XentPack &k, const void *w, int64_t
 }
 
 // W packed, and by the workgroups behind those, the rows: label and weight (-1 and 0 where
-// the row is out), h scaled by row.  A row that is out and not finite is packed as zeros, its
-// label -2.
+// the row is out) and h.  A row that is out and whose scores may not be finite is packed as
+// zeros, its label -2.
+constexpr int FAR_ROW = -100;            // scores of up to 2^(13 - this)
 template <typename T>
 __global__ __launch_bounds__(64 * MAX_WAVES) void k_xent_pack(XentPack k, XentCall c) {
-    __shared__ uint32_t lds[2 * MAX_WAVES];
-    const uint32_t most_w = largest_of<MAX_WAVES>(k.ctl->w, k.w_groups, lds);
-    const int sw = scale_exp(most_w & ~FLAG);
-    if (blockIdx.x == 0 && threadIdx.x == 0) k.ctl->w.all = most_w & ~FLAG;
+    __shared__ int32_t exps[FEW_COLUMNS];
+    __shared__ uint32_t words[MAX_WAVES];
+    const bool offered = k.few ? few_scales(k, exps, words) : k.ctl->offered.all != 0;
     if ((int32_t)blockIdx.x < k.pack_w_groups) {
-        pack_w<T>(k, c.w, c.w_stride, sw);
+        pack_w<T>(k, c.w, c.w_stride, exps);
         return;
     }
     const int32_t group = blockIdx.x - k.pack_w_groups;
     const int lane = threadIdx.x & 63;
     const int align = alignment<T>(c.h, c.h_stride);
-    uint32_t hg = 0;
     for (int64_t i = (int64_t)group * MAX_WAVES + (threadIdx.x >> 6); i < k.n_pad;
-         i += (int64_t)k.hg_groups * MAX_WAVES) {
-        int32_t y = i < k.n ? c.labels[i] : -1, d = i < k.n ? k.d : 0;
-        float wt = i < k.n ? (c.weights ? c.weights[i] : 1.0f) : 0.0f;
-        const bool out = y < 0 || y >= k.v || wt == 0.0f || !(most_w & FLAG);
-        uint32_t m = 0, most = 0;
+         i += (int64_t)k.pack_h_groups * MAX_WAVES) {
+        int32_t d = i < k.n ? k.d : 0;
+        float wt = 0.0f;
+        const bool in = i < k.n && row_in(k, c, i, wt) && offered;
+        int m = NO_EXP;
+        uint32_t most = 0;
         for (int32_t f = lane * 8; f < d; f += 512) {
             float x[8];
+            int s[8];
             load8<T>(c.h, i * c.h_stride, f, d, align, x);
+            load_exps(k, exps, f, s);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                m = max(m, finite_bits(x[e]));
+                m = max(m, exponent_of(x[e]) - s[e]);
                 most = max(most, __float_as_uint(fabsf(x[e])));
             }
         }
         m = wave_max(m);
-        if (out) {
-            y = -1;
+        int s = m > NO_EXP / 2 ? TOP_EXP - m : 0;
+        int32_t y = -1;
+        if (in) {
+            y = c.labels[i];
+        } else {
             wt = 0.0f;
-            if (wave_max(most) >= XENT_HUGE) {
+            if (wave_max(most) >= XENT_HUGE || s < FAR_ROW) {
                 y = -2;
-                m = 0;
+                s = 0;
                 d = 0;
             }
         }
-        const int s = scale_exp(m);
-        if (wt != 0.0f) hg = max(hg, finite_bits(wt * __uint_as_float(m)));
         if (lane == 0) {
-            k.row_scale[i] = ldexpf(1.0f, -(s + sw));
+            k.row_scale[i] = power_of_2(-s);
             k.label[i] = y;
             k.weight[i] = wt;
         }
         for (int32_t f = lane * 8; f < k.ld; f += 512) {
             float x[8];
+            int e[8];
             load8<T>(c.h, i * c.h_stride, f, d, align, x);
-            pack8<T>(x, s, k.h + i * k.ld + f, k.n_pad * k.ld);
+            load_exps(k, exps, f, e);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) e[q] = s - e[q];
+            pack8<T>(x, e, k.h + i * k.ld + f, k.n_pad * k.ld);
         }
     }
-    const uint32_t most = largest<MAX_WAVES>(hg, 0, lds);
-    if (threadIdx.x == 0) k.ctl->hg.part[group] = most;
 }
 
 // ---- products --------------------------------------------------------------------
@@ -459,11 +562,6 @@ __global__ __launch_bounds__(C::WAVES * 64, 2) void k_xent_stats(XentPack k, int
                                                                  int32_t splits,
                                                                  float2 *__restrict__ part) {
     extern __shared__ char lds[];
-    if (k.hg && blockIdx.x == 0) {       // for the kernels behind this one
-        const uint32_t most = largest_of<C::WAVES>(k.ctl->hg, k.hg_groups,
-                                                     reinterpret_cast<uint32_t *>(lds));
-        if (threadIdx.x == 0) k.ctl->hg.all = most;
-    }
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     uint32_t row_tile, split;
@@ -531,7 +629,7 @@ __global__ __launch_bounds__(C::WAVES * 64, 2) void k_xent_stats(XentPack k, int
 
 // The parts of a row joined, one wavefront a row: lse, as reference and log2 of the sum for
 // the gradients, and loss.  The label's score is summed in f32 from h and W themselves.  For gradients, h is packed once more as dW's product
-// takes it, times the row's weight and with one scale for all rows (they are summed over).
+// takes it, times the row's weight and with its columns' scales (the rows are summed over).
 template <typename T>
 __global__ __launch_bounds__(256) void k_xent_join(XentPack k, XentCall c, int32_t parts,
                                                    const float2 *__restrict__ part,
@@ -561,12 +659,14 @@ __global__ __launch_bounds__(256) void k_xent_join(XentPack k, XentCall c, int32
         dot += __shfl_xor(dot, o, 64);
     }
     if (k.hg) {
-        const int s = scale_exp(k.ctl->hg.all), align = alignment<T>(c.h, c.h_stride);
+        const int align = alignment<T>(c.h, c.h_stride);
         const int32_t d = y >= 0 ? k.d : 0;
         const float wt = k.weight[i];
         for (int32_t f = lane * 8; f < k.ld; f += 512) {
             float x[8];
+            int s[8];
             load8<T>(c.h, i * c.h_stride, f, d, align, x);
+            load8<int32_t>(k.hg_exp, f, s);
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[e] *= wt;
             pack8<T>(x, s, k.hg + i * k.ld + f, k.n_pad * k.ld);
@@ -643,7 +743,7 @@ __global__ __launch_bounds__(C::WAVES * 64, 2) void k_xent_g(XentPack k, int64_t
                         db[q * 4 + e] = y == 0 ? p * wt[y]
                                                : __builtin_fmaf(p, wt[y], db[q * 4 + e]);
                         u16 hi, lo;
-                        split_f16(p * G_SCALE, hi, lo);
+                        split_f16(p * (float)(1 << G_EXP), hi, lo);
                         to[mine] = hi;
                         if constexpr (P == 2) to[plane + mine] = lo;
                         to += e < 3 ? rows_pad : 5 * rows_pad;
@@ -685,20 +785,19 @@ struct Out {
     int64_t rows, stride;        // of the output; its columns are k.d
     bool classes;                // dW: rows whose bias is -inf are 0; dh: times weight
 };
-__device__ __forceinline__ float out_scale(const XentPack &k, bool classes) {
-    return ldexpf(1.0f, -scale_exp(classes ? k.ctl->hg.all : k.ctl->w.all)) / G_SCALE;
+// The power of two of column n of a product with G.
+__device__ __forceinline__ int out_exp(const XentPack &k, bool classes, int64_t n) {
+    return n < k.d ? -G_EXP - (classes ? k.hg_exp : k.w_exp)[n] : 0;
 }
 template <int P>
 __device__ __forceinline__ void put(const XentPack &k, const Out &o, int64_t m, int64_t n, float v,
-                                    float scale) {
+                                    int exp) {
     if (m >= o.rows || n >= k.d) return;
-    if (o.classes) {
-        if (k.bias[m] == -INFINITY) v = 0.0f;
-    } else {
-        scale *= k.weight[m];
-    }
-    if constexpr (P == 1) static_cast<__bf16 *>(o.out)[m * o.stride + n] = (__bf16)(v * scale);
-    else static_cast<float *>(o.out)[m * o.stride + n] = v * scale;
+    v = ldexpf(v, exp);
+    if (!o.classes) v *= k.weight[m];
+    else if (k.bias[m] == -INFINITY) v = 0.0f;
+    if constexpr (P == 1) static_cast<__bf16 *>(o.out)[m * o.stride + n] = (__bf16)v;
+    else static_cast<float *>(o.out)[m * o.stride + n] = v;
 }
 
 // A product with G: its first row is m_first of the output.
@@ -723,7 +822,11 @@ __device__ __forceinline__ void product(const XentPack &k, const Product &q, uin
     };
     products<P, AK, false, C>(q.a, q.b, 1, q.steps * split / o.splits,
                               q.steps * (split + 1) / o.splits, lds, acc, next, [](int64_t) {});
-    const float scale = out_scale(k, o.classes);
+    int exp[C::NT];
+#pragma unroll
+    for (int y = 0; y < C::NT; ++y)
+        exp[y] = out_exp(k, o.classes,
+                         (int64_t)tn * C::T + wave % C::WN * C::NT * 32 + y * 32 + (lane & 31));
     float *sums = o.acc + split * o.m_pad * k.ld;
 #pragma unroll
     for (int x = 0; x < C::MT; ++x)
@@ -737,10 +840,10 @@ __device__ __forceinline__ void product(const XentPack &k, const Product &q, uin
                                   (lane & 31);
                 float v = acc[x][y][r];
                 if (o.first && o.last && o.splits == 1) {
-                    put<P>(k, o, m, n, v, scale);
+                    put<P>(k, o, m, n, v, exp[y]);
                 } else if (n < k.ld) {
                     if (!o.first) v += sums[m * k.ld + n];
-                    if (o.last && o.splits == 1) put<P>(k, o, m, n, v, scale);
+                    if (o.last && o.splits == 1) put<P>(k, o, m, n, v, exp[y]);
                     else sums[m * k.ld + n] = v;
                 }
             }
@@ -761,12 +864,11 @@ __global__ __launch_bounds__(C::WAVES * 64, 2) void k_xent_products(XentPack k, 
 // The splits of a product's row added, in order.
 template <int P>
 __device__ __forceinline__ void join_splits(const XentPack &k, int64_t m, const Out &o) {
-    const float scale = out_scale(k, o.classes);
     for (int32_t n = threadIdx.x; n < k.d; n += 256) {
         float v = 0.0f;
 #pragma unroll 4
         for (int s = 0; s < o.splits; ++s) v += o.acc[(s * o.m_pad + m) * k.ld + n];
-        put<P>(k, o, m, n, v, scale);
+        put<P>(k, o, m, n, v, out_exp(k, o.classes, n));
     }
 }
 // A workgroup a row of dh_rows and of dw_rows, whose splits it adds, and then one for 256 classes
@@ -878,7 +980,9 @@ struct Plan {
     int64_t n_pad, v_pad, ld, piece_rows, piece_classes;
     int32_t splits;
     Cut dh, dw;                  // of whole pieces
-    size_t ctl, h, hg, w, bias, scale, label, weight, lse, part, g, db, dh_acc, dw_acc, end;
+    int32_t w_groups, hg_groups;
+    size_t ctl, w_part, hg_part, w_exp, hg_exp, h, hg, w, bias, scale, label, weight, lse, part, g,
+        db, dh_acc, dw_acc, end;
 };
 
 Plan plan_of(const XentCall &c) {
@@ -902,7 +1006,19 @@ Plan plan_of(const XentCall &c) {
     };
     // a wide tile may read 128 elements past the last packed row
     const size_t past = 512;
+    // workgroups of k_xent_columns: four a CU over all columns
+    const int64_t most = std::max<int64_t>(
+        1, std::min(4 * c.num_cus, MOST_GROUPS) / (up(c.dim, COLUMNS) / COLUMNS));
+    const auto groups = [&](int64_t rows) {
+        return (int32_t)std::min(blocks(rows, COLUMN_ROWS * ROWS_AHEAD), (uint32_t)most);
+    };
+    p.w_groups = groups(p.v_pad);
+    p.hg_groups = c.grad ? groups(p.n_pad) : 0;
     p.ctl = take(sizeof(XentCtl));
+    p.w_part = take((size_t)4 * p.w_groups * p.ld);
+    p.hg_part = take((size_t)4 * p.hg_groups * p.ld);
+    p.w_exp = take((size_t)4 * p.ld);
+    p.hg_exp = take((size_t)4 * p.ld);
     p.h = take((size_t)2 * p.P * p.n_pad * p.ld + past);
     p.w = take((size_t)2 * p.P * p.v_pad * p.ld + past);
     p.bias = take((size_t)4 * p.v_pad);
@@ -978,6 +1094,13 @@ hipError_t run(hipStream_t s, const XentCall &c, const Plan &p, char *m) {
     k.d = c.dim;
     k.ld = (int32_t)p.ld;
     k.ctl = reinterpret_cast<XentCtl *>(m + p.ctl);
+    k.w_groups = p.w_groups;
+    k.hg_groups = p.hg_groups;
+    k.few = p.w_groups <= FEW_GROUPS && p.hg_groups <= FEW_GROUPS && p.ld <= FEW_COLUMNS;
+    k.w_part = reinterpret_cast<uint32_t *>(m + p.w_part);
+    k.hg_part = reinterpret_cast<uint32_t *>(m + p.hg_part);
+    k.w_exp = reinterpret_cast<int32_t *>(m + p.w_exp);
+    k.hg_exp = reinterpret_cast<int32_t *>(m + p.hg_exp);
     k.h = reinterpret_cast<u16 *>(m + p.h);
     k.hg = c.grad ? reinterpret_cast<u16 *>(m + p.hg) : nullptr;
     k.w = reinterpret_cast<u16 *>(m + p.w);
@@ -999,14 +1122,17 @@ hipError_t run(hipStream_t s, const XentCall &c, const Plan &p, char *m) {
         if (e != hipSuccess) return e;
     }
     const auto groups = [&](int64_t rows) {
-        return (int32_t)std::min<int64_t>((rows + MAX_WAVES - 1) / MAX_WAVES,
-                                          std::min(4 * c.num_cus, MOST_GROUPS));
+        return (int32_t)std::min<int64_t>((rows + MAX_WAVES - 1) / MAX_WAVES, 4 * c.num_cus);
     };
-    k.w_groups = k.pack_w_groups = groups(k.v_pad);
-    k.hg_groups = groups(k.n_pad);
-    hipLaunchKernelGGL((k_xent_classes<T>), dim3((uint32_t)k.w_groups), dim3(64 * MAX_WAVES), 0, s,
-                       k, c.w, c.w_stride, c.bias);
-    hipLaunchKernelGGL((k_xent_pack<T>), dim3((uint32_t)(k.pack_w_groups + k.hg_groups)),
+    k.pack_w_groups = groups(k.v_pad);
+    k.pack_h_groups = groups(k.n_pad);
+    hipLaunchKernelGGL((k_xent_columns<T>),
+                       dim3((uint32_t)(k.w_groups + k.hg_groups), blocks(c.dim, COLUMNS)),
+                       dim3(64 * MAX_WAVES), 0, s, k, c);
+    if (!k.few)
+        hipLaunchKernelGGL(k_xent_scales, dim3((uint32_t)(k.ld / 64 * (c.grad ? 2 : 1))),
+                           dim3(64 * SCALE_WAVES), 0, s, k);
+    hipLaunchKernelGGL((k_xent_pack<T>), dim3((uint32_t)(k.pack_w_groups + k.pack_h_groups)),
                        dim3(64 * MAX_WAVES), 0, s, k, c);
     if (p.wide) launch_stats<P, Wide>(s, k, p.splits, part);
     else launch_stats<P, Narrow>(s, k, p.splits, part);

@@ -16,7 +16,12 @@
 // lane's own registers, rounded, are its operand, and the read across picks Y's
 // rows in that order: no value moves between lanes.
 //
-// Operands are one f16 term (bf16) or two (f32), as kernels_xent.hip says.
+// Operands are one f16 term (bf16) or two (f32), as kernels_xent.hip says, but one packed h
+// serves the scores and dW.  So a column of W is packed times 2^c and h's times 2^-c, half the
+// difference of their sizes (h's over the rows, each brought to the size 1): both columns'
+// largest are then 2^-k of the largest of all if their product is 2^-2k of the largest product,
+// and are held with 22 bits up to k = 16, with 38 - k from there on.  P carries the rows' weights
+// over their powers of two into dW, off by 2^-40 of the largest.
 //
 // The matrix instructions bound both passes: 20000 x 100 x 10000 f32 takes 268 and 285 us,
 // 1.09 and 1.03 PFLOP/s of f16 products (112 columns of the first and 128 of the second, three
@@ -47,22 +52,27 @@ __host__ __device__ constexpr int row_ld(int ks) { return ks <= 2 ? 32 : ks <= 4
 struct Fused {
     int64_t n, v, n_pad, v_pad;
     int32_t d;
-    int32_t w_groups, hg_groups;         // that look at W, pack h
+    int32_t w_groups, h_groups, pack_groups;     // that look at W's and h's columns, pack
+    bool few;                            // of the first two: those that pack sum them up
     XentCtl *ctl;
+    int32_t *part, *col;                 // [group][ld] and [W, h][ld] largest exponents of columns
+    int32_t *exp2;                       // [ld] a column of W is packed times 2^this
     u16 *h, *w;                          // planes of n_pad * ld, v_pad * ld
     float *bias;                         // [v_pad] the bias, -inf: not offered
     // of the rows, [n_pad]:
     float *sc;                           // the scale of a score
-    int32_t *exp;                        // h is packed times 2^exp
+    int32_t *exp;                        // h is packed times 2^(exp - its column's exp2)
     int32_t *label;                      // -1: out, -2: out and not finite
     float *weight;                       // 0: out
     float *ref, *l2;                     // lse as a score and log2 of the sum, +inf: out
     float *wq;                           // weight as the classes pass multiplies with it
 };
 
-// The exponent of the classes pass's weights, for the largest |w h|.
-__device__ __forceinline__ int wq_exp(uint32_t hg_max) {
-    return hg_max ? min(126, max(-126, 27 - ilogbf(__uint_as_float(hg_max)))) : 0;
+// The classes pass multiplies P with a row's weight over its power of two; E, of the largest
+// of them, puts that below 2^15.  Words of XentMax hold E + ROW_BIAS, 0 for no row.
+constexpr int ROW_BIAS = 1 << 14;
+__device__ __forceinline__ int wq_exp(uint32_t row_max) {
+    return row_max ? 15 - ((int)row_max - ROW_BIAS) : 0;
 }
 
 template <typename T> __device__ __forceinline__ float load_f32(const void *p, int64_t i) {
@@ -75,98 +85,222 @@ __device__ __forceinline__ void load4(const void *p, int64_t row, int f, int d, 
 #pragma unroll
     for (int e = 0; e < 4; ++e) x[e] = f + e < d ? load_f32<T>(p, row + f + e) : 0.0f;
 }
-__device__ __forceinline__ uint32_t finite_max(const float (&x)[4]) {
-    return max(max(finite_bits(x[0]), finite_bits(x[1])), max(finite_bits(x[2]), finite_bits(x[3])));
-}
 // LD / 4 lanes a row in the kernels that prepare and join, and a grid that goes over
 // the rows in turns.
+template <int LANES> __device__ __forceinline__ int row_max(int m) {
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) m = max(m, __shfl_xor(m, o, 64));
+    return m;
+}
+// The largest exponents of the columns: of W by the first workgroups, which also leave the
+// padded bias and whether a class is offered, and of h, less the row's largest, by those behind.
 template <typename T, int LD>
-__global__ __launch_bounds__(256) void k_fused_classes(Fused k, const void *w, int64_t stride,
-                                                       const float *__restrict__ bias) {
+__global__ __launch_bounds__(256) void k_fused_columns(Fused k, XentCall c) {
     constexpr int LANES = LD / 4, ROWS = 256 / LANES;
-    const int f = threadIdx.x % LANES * 4;
-    uint32_t m = 0;
+    __shared__ int32_t most[ROWS][LD];
+    const int f = threadIdx.x % LANES * 4, r = threadIdx.x / LANES;
+    int m[4] = {NO_EXP, NO_EXP, NO_EXP, NO_EXP};
     bool any = false;
-    for (int64_t v = (int64_t)blockIdx.x * ROWS + threadIdx.x / LANES; v < k.v_pad;
-         v += (int64_t)gridDim.x * ROWS) {
-        const float b = v < k.v ? (bias ? bias[v] : 0.0f) : -INFINITY;
-        const bool open = b != -INFINITY;
-        any = any || open;
-        if (f == 0) k.bias[v] = b;
-        if (!open) continue;
-        float x[4];
-        load4<T>(w, v * stride, f, k.d, x);
-        m = max(m, finite_max(x));
+    // four rows at a time, so that as many loads are on the way
+    constexpr int AHEAD = 4;
+    float x[AHEAD][4];
+    bool in[AHEAD];
+    if ((int32_t)blockIdx.x < k.w_groups) {
+        const int64_t hop = (int64_t)k.w_groups * ROWS;
+        for (int64_t v0 = (int64_t)blockIdx.x * ROWS + r; v0 < k.v_pad; v0 += AHEAD * hop) {
+#pragma unroll
+            for (int q = 0; q < AHEAD; ++q) {
+                const int64_t v = v0 + q * hop;
+                const float b = v < k.v ? (c.bias ? c.bias[v] : 0.0f) : -INFINITY;
+                if (f == 0 && v < k.v_pad) k.bias[v] = b;
+                in[q] = b != -INFINITY;
+                any = any || in[q];
+                load4<T>(c.w, (v < k.v ? v : 0) * c.w_stride, f, v < k.v ? k.d : 0, x[q]);
+            }
+#pragma unroll
+            for (int q = 0; q < AHEAD; ++q)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (in[q]) m[e] = max(m[e], exponent_of(x[q][e]));
+        }
+    } else {
+        const int64_t hop = (int64_t)k.h_groups * ROWS;
+        for (int64_t i0 = (int64_t)(blockIdx.x - k.w_groups) * ROWS + r; i0 < k.n;
+             i0 += AHEAD * hop) {
+#pragma unroll
+            for (int q = 0; q < AHEAD; ++q) {
+                const int64_t i = i0 + q * hop;
+                const int32_t y = i < k.n ? c.labels[i] : -1;
+                in[q] = y >= 0 && y < k.v && !(c.weights && c.weights[i] == 0.0f);
+                load4<T>(c.h, (i < k.n ? i : 0) * c.h_stride, f, i < k.n ? k.d : 0, x[q]);
+            }
+#pragma unroll
+            for (int q = 0; q < AHEAD; ++q) {
+                int at[4], top = NO_EXP;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    at[e] = exponent_of(x[q][e]);
+                    top = max(top, at[e]);
+                }
+                top = row_max<LANES>(top);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (in[q] && at[e] != NO_EXP) m[e] = max(m[e], at[e] - top);
+            }
+        }
     }
-    __shared__ uint32_t lds[8];
-    const uint32_t most = largest<4>(m, any, lds);
-    if (threadIdx.x == 0) k.ctl->w.part[blockIdx.x] = most;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) most[r][f + e] = m[e];
+    const bool offered = __syncthreads_or(any);
+    if ((int32_t)blockIdx.x < k.w_groups && threadIdx.x == 0)
+        k.ctl->offered.part[blockIdx.x] = offered;
+    if (threadIdx.x >= LD) return;
+    int all = NO_EXP;
+#pragma unroll
+    for (int q = 0; q < ROWS; ++q) all = max(all, most[q][threadIdx.x]);
+    k.part[(int64_t)blockIdx.x * LD + threadIdx.x] = all;
 }
 
-// The packed rows of W and then of h.
+// Over the groups: 32 columns a workgroup, and 32 threads a column in turns.
+__global__ __launch_bounds__(1024) void k_fused_scales(Fused k, int32_t ld) {
+    __shared__ int32_t most[32][32];
+    __shared__ uint32_t words[16];
+    const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
+    const bool of_w = (int32_t)blockIdx.x < ld / 32;
+    const int32_t col = (of_w ? blockIdx.x : blockIdx.x - ld / 32) * 32 + lane;
+    const int32_t first = of_w ? 0 : k.w_groups, groups = of_w ? k.w_groups : k.h_groups;
+    int m = NO_EXP;
+#pragma unroll 8
+    for (int g = slice; g < groups; g += 32) m = max(m, k.part[(int64_t)(first + g) * ld + col]);
+    most[slice][lane] = m;
+    if (blockIdx.x == 0) {
+        const uint32_t any = largest_of<16>(k.ctl->offered, k.w_groups, words);
+        if (threadIdx.x == 0) k.ctl->offered.all = any;
+    }
+    __syncthreads();
+    if (slice != 0) return;
+#pragma unroll
+    for (int q = 1; q < 32; ++q) m = max(m, most[q][lane]);
+    k.col[(of_w ? 0 : ld) + col] = m;
+}
+
+// The same of few groups, by each workgroup of the next kernel, without a launch (4.5 us).
+constexpr int FEW_GROUPS = 64;
+template <int LD>
+__device__ __forceinline__ void few_columns(const Fused &k, int32_t *col, int32_t (&part)[256]) {
+    const int32_t c = threadIdx.x % LD, slice = threadIdx.x / LD;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int32_t first = h ? k.w_groups : 0, groups = h ? k.h_groups : k.w_groups;
+        int m = NO_EXP;
+#pragma unroll 8
+        for (int g = slice; g < groups; g += 256 / LD) m = max(m, k.part[(first + g) * LD + c]);
+        part[threadIdx.x] = m;
+        __syncthreads();
+        if (threadIdx.x < LD) {
+#pragma unroll
+            for (int q = 1; q < 256 / LD; ++q) m = max(m, part[threadIdx.x + q * LD]);
+            col[h * LD + threadIdx.x] = m;
+        }
+        __syncthreads();
+    }
+}
+
+// Column threadIdx.x's power of two, by the first LD threads: a, b are the largest exponents
+// of W's and h's column; 2^c for W and 2^-c for h leave both at level (a + b) / 2, and the
+// largest level goes to TOP_EXP.  A column that only one of them has goes to that level.
+template <int LD>
+__device__ __forceinline__ int column_exp(const int32_t *col, int32_t *words) {
+    int a = NO_EXP, b = NO_EXP;
+    if (threadIdx.x < LD) {
+        a = col[threadIdx.x];
+        b = col[LD + threadIdx.x];
+    }
+    const bool both = a != NO_EXP && b != NO_EXP;
+    const int c = (b - a) >> 1;
+    int level = largest<4>(both ? a + c : NO_EXP, words);
+    if (level == NO_EXP) level = 0;
+    return both ? c + TOP_EXP - level : a != NO_EXP ? TOP_EXP - a
+                                      : b != NO_EXP ? b + TOP_EXP - 2 * level : 0;
+}
+
+// The packed rows of W and then of h.  A row that is out and whose scores may not be finite
+// is packed as zeros, its label -2.
+constexpr int FAR_ROW = -100;            // scores of up to 2^(13 - this)
+constexpr int ZERO_ROW = 1 << 20;        // of exp: nothing but zeros
 template <typename T, int LD>
-__global__ __launch_bounds__(256) void k_fused_pack(Fused k, const void *w, int64_t w_stride,
-                                                    const void *h, int64_t h_stride,
-                                                    const int32_t *__restrict__ labels,
-                                                    const float *__restrict__ weights) {
+__global__ __launch_bounds__(256) void k_fused_pack(Fused k, XentCall c) {
     constexpr int LANES = LD / 4, ROWS = 256 / LANES;
     const int f = threadIdx.x % LANES * 4;
-    __shared__ uint32_t lds[8];
-    const uint32_t most_w = largest_of<4>(k.ctl->w, k.w_groups, lds);
-    const int sw = scale_exp(most_w & ~FLAG);
-    const bool any = most_w & FLAG;
-    if (blockIdx.x == 0 && threadIdx.x == 0) k.ctl->w.all = most_w & ~FLAG;
-    uint32_t hg = 0;
+    __shared__ int32_t words[4], exps[LD], cols[2 * LD], part[256];
+    if (k.few) few_columns<LD>(k, cols, part);
+    const int mine = column_exp<LD>(k.few ? cols : k.col, words);
+    if (threadIdx.x < LD) {
+        exps[threadIdx.x] = mine;
+        if (blockIdx.x == 0) k.exp2[threadIdx.x] = mine;
+    }
+    __syncthreads();
+    int ex[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) ex[e] = exps[f + e];
+    const bool any = k.few ? largest_of<4>(k.ctl->offered, k.w_groups,
+                                           reinterpret_cast<uint32_t *>(words)) != 0
+                           : k.ctl->offered.all != 0;
+    uint32_t row = 0;
     for (int64_t at = (int64_t)blockIdx.x * ROWS + threadIdx.x / LANES; at < k.v_pad + k.n_pad;
-         at += (int64_t)gridDim.x * ROWS) {
+         at += (int64_t)k.pack_groups * ROWS) {
         const bool of_w = at < k.v_pad;
         const int64_t i = of_w ? at : at - k.v_pad;
         float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        int s = sw;
+        int s[4] = {ex[0], ex[1], ex[2], ex[3]};
         if (of_w) {
-            if (k.bias[i] != -INFINITY) load4<T>(w, i * w_stride, f, k.d, x);
+            if (k.bias[i] != -INFINITY) load4<T>(c.w, i * c.w_stride, f, k.d, x);
         } else {
-            if (i < k.n) load4<T>(h, i * h_stride, f, k.d, x);
-            int32_t y = i < k.n ? labels[i] : -1;
-            float wt = i < k.n ? (weights ? weights[i] : 1.0f) : 0.0f;
-            uint32_t m = finite_max(x);
-            uint32_t most = m;                   // of all values, finite or not
+            if (i < k.n) load4<T>(c.h, i * c.h_stride, f, k.d, x);
+            int32_t y = i < k.n ? c.labels[i] : -1;
+            float wt = i < k.n ? (c.weights ? c.weights[i] : 1.0f) : 0.0f;
+            int m = NO_EXP;
+            bool huge = false;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) most = max(most, __float_as_uint(fabsf(x[e])));
-#pragma unroll
-            for (int o = LANES / 2; o > 0; o >>= 1) {
-                m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
-                most = max(most, (uint32_t)__shfl_xor((int)most, o, 64));
+            for (int e = 0; e < 4; ++e) {
+                m = max(m, exponent_of(x[e]) - ex[e]);
+                huge = huge || __float_as_uint(fabsf(x[e])) >= XENT_HUGE;
             }
+            m = row_max<LANES>(m);
+            huge = row_max<LANES>(huge);
+            const bool zeros = m < NO_EXP / 2;
+            int exp = zeros ? 0 : TOP_EXP - m;
             if (y < 0 || y >= k.v || wt == 0.0f || !any) {
                 wt = 0.0f;
                 y = -1;
-                if (most >= XENT_HUGE) {
+                if (huge || exp < FAR_ROW) {
                     y = -2;
-                    m = 0;
+                    exp = 0;
                     x[0] = x[1] = x[2] = x[3] = 0.0f;
                 }
             }
-            s = scale_exp(m);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[e] = exp - ex[e];
             if (f == 0) {
                 k.label[i] = y;
                 k.weight[i] = wt;
-                k.exp[i] = s;
-                k.sc[i] = ldexpf(1.0f, -(s + sw));
-                if (wt != 0.0f) hg = max(hg, finite_bits(wt * __uint_as_float(m)));
+                k.exp[i] = zeros ? ZERO_ROW : exp;
+                k.sc[i] = power_of_2(-exp);
+                const int e = exponent_of(wt);
+                if (!zeros && e != NO_EXP) row = max(row, (uint32_t)(e - exp + ROW_BIAS));
             }
         }
-        u16 *row = (of_w ? k.w : k.h) + i * LD + f;
+        u16 *to = (of_w ? k.w : k.h) + i * LD + f;
         u16 hi[4], lo[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) split_f16(ldexpf(x[e], s), hi[e], lo[e]);
-        *reinterpret_cast<u16x4 *>(row) = u16x4{hi[0], hi[1], hi[2], hi[3]};
+        for (int e = 0; e < 4; ++e) split_f16(ldexpf(x[e], s[e]), hi[e], lo[e]);
+        *reinterpret_cast<u16x4 *>(to) = u16x4{hi[0], hi[1], hi[2], hi[3]};
         if (sizeof(T) == 4)
-            *reinterpret_cast<u16x4 *>(row + (of_w ? k.v_pad : k.n_pad) * LD) =
+            *reinterpret_cast<u16x4 *>(to + (of_w ? k.v_pad : k.n_pad) * LD) =
                 u16x4{lo[0], lo[1], lo[2], lo[3]};
     }
-    const uint32_t most = largest<4>(hg, 0, lds);
-    if (threadIdx.x == 0) k.ctl->hg.part[blockIdx.x] = most;
+    const uint32_t most = largest<4>(row, reinterpret_cast<uint32_t *>(words));
+    if (threadIdx.x == 0) k.ctl->row.part[blockIdx.x] = most;
 }
 
 // ---- a tile in LDS -----------------------------------------------------------------
@@ -351,9 +485,9 @@ __global__ __launch_bounds__(256, 2) void k_fused_rows(Fused k, int32_t splits,
     constexpr int BUF = TILE_BYTES<P, LD> + TY * 4;      // a multiple of 256: see across
     extern __shared__ char lds[];
     if (GRAD && blockIdx.x == 0) {       // for the kernels behind this one
-        const uint32_t most = largest_of<4>(k.ctl->hg, k.hg_groups,
+        const uint32_t most = largest_of<4>(k.ctl->row, k.pack_groups,
                                             reinterpret_cast<uint32_t *>(lds));
-        if (threadIdx.x == 0) k.ctl->hg.all = most;
+        if (threadIdx.x == 0) k.ctl->row.all = most;
     }
     const int lane = threadIdx.x & 63, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -497,20 +631,19 @@ __global__ __launch_bounds__(256) void k_fused_join_rows(Fused k, XentCall c, in
         if constexpr (GRAD) {
             k.ref[i] = y < 0 ? 0.0f : ref;
             k.l2[i] = y < 0 ? INFINITY : l.base2;
-            // weight 2^-exp and the power of two that brings the largest below 2^15
-            const float q = ldexpf(wt, wq_exp(k.ctl->hg.all) - k.exp[i]);
-            // a row of zeros has no exponent of its own; a weight that is not finite stays so
-            k.wq[i] = fabsf(wt) < INFINITY ? fminf(fmaxf(q, -60000.0f), 60000.0f) : wt;
+            // a row of zeros has no power of two; a weight that is not finite stays so
+            const int e = k.exp[i];
+            k.wq[i] = e != ZERO_ROW ? ldexpf(wt, wq_exp(k.ctl->row.all) - e)
+                                    : fabsf(wt) < INFINITY ? 0.0f : wt;
         }
     }
     if constexpr (GRAD) {
         if (!c.dh || i >= k.n) return;
-        const float scale = ldexpf(1.0f, -scale_exp(k.ctl->w.all));
 #pragma unroll
         for (int e = 0; e < 4; ++e)
             if (f + e < k.d) {
                 // divided first: the sum of 2^13 p W is beyond f32 for W that is not
-                const float g = y < 0 ? 0.0f : wt * (o[e] / sum * scale - wy[e]);
+                const float g = y < 0 ? 0.0f : wt * (ldexpf(o[e] / sum, -k.exp2[f + e]) - wy[e]);
                 static_cast<T *>(c.dh)[i * c.h_stride + f + e] = (T)g;
             }
     }
@@ -665,13 +798,14 @@ __global__ __launch_bounds__(256) void k_fused_join_classes(Fused k, XentCall c,
     }
     if (v >= k.v) return;
     const bool open = k.bias[v] != -INFINITY;
-    const float scale = ldexpf(1.0f, -wq_exp(k.ctl->hg.all));
+    const int exp = wq_exp(k.ctl->row.all);
     const float x[4] = {sum.x, sum.y, sum.z, sum.w};
     if (c.dw)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
             if (f + e < k.d)
-                static_cast<T *>(c.dw)[v * c.w_stride + f + e] = (T)(open ? x[e] * scale : 0.0f);
+                static_cast<T *>(c.dw)[v * c.w_stride + f + e] =
+                    (T)(open ? ldexpf(x[e], k.exp2[f + e] - exp) : 0.0f);
     if (c.dbias && l == 0) c.dbias[v] = open ? (float)db : 0.0f;
 }
 
@@ -702,7 +836,8 @@ struct Plan {
     int P, ks;
     int64_t n_pad, v_pad, ld;
     int32_t row_splits, class_splits;
-    size_t ctl, h, w, bias, rows, part_ms, part, part_db, end;
+    int32_t w_groups, h_groups;
+    size_t ctl, col_part, col, exp2, h, w, bias, rows, part_ms, part, part_db, end;
 };
 
 Plan plan_of(const XentCall &c) {
@@ -720,7 +855,17 @@ Plan plan_of(const XentCall &c) {
         at += (bytes + 255) / 256 * 256;
         return here;
     };
+    // workgroups of k_fused_columns: eight a CU, four rows a thread or more
+    const auto groups = [&](int64_t rows) {
+        return (int32_t)std::max<int64_t>(
+            1, std::min<int64_t>((rows * p.ld + 4095) / 4096, std::min(4 * c.num_cus, MOST_GROUPS)));
+    };
+    p.w_groups = groups(p.v_pad);
+    p.h_groups = groups(p.n_pad);
     p.ctl = take(sizeof(XentCtl));
+    p.col_part = take((size_t)4 * (p.w_groups + p.h_groups) * p.ld);
+    p.col = take((size_t)8 * p.ld);
+    p.exp2 = take((size_t)4 * p.ld);
     p.h = take((size_t)2 * p.P * p.n_pad * p.ld);
     p.w = take((size_t)2 * p.P * p.v_pad * p.ld);
     p.bias = take((size_t)4 * p.v_pad);
@@ -744,6 +889,12 @@ hipError_t run(hipStream_t s, const XentCall &c, const Plan &p, char *m) {
     k.v_pad = p.v_pad;
     k.d = c.dim;
     k.ctl = reinterpret_cast<XentCtl *>(m + p.ctl);
+    k.w_groups = p.w_groups;
+    k.h_groups = p.h_groups;
+    k.few = k.w_groups + k.h_groups <= FEW_GROUPS;
+    k.part = reinterpret_cast<int32_t *>(m + p.col_part);
+    k.col = reinterpret_cast<int32_t *>(m + p.col);
+    k.exp2 = reinterpret_cast<int32_t *>(m + p.exp2);
     k.h = reinterpret_cast<u16 *>(m + p.h);
     k.w = reinterpret_cast<u16 *>(m + p.w);
     k.bias = reinterpret_cast<float *>(m + p.bias);
@@ -768,16 +919,13 @@ hipError_t run(hipStream_t s, const XentCall &c, const Plan &p, char *m) {
         const hipError_t e = allow_all_lds(f);
         if (e != hipSuccess) return e;
     }
-    const auto groups = [&](int64_t rows) {
-        return (int32_t)std::min<int64_t>((rows * LD + 1023) / 1024,
-                                          std::min(8 * c.num_cus, MOST_GROUPS));
-    };
-    k.w_groups = groups(k.v_pad);
-    k.hg_groups = groups(k.v_pad + k.n_pad);
-    hipLaunchKernelGGL((k_fused_classes<T, LD>), dim3((uint32_t)k.w_groups), b, 0, s, k, c.w,
-                       c.w_stride, c.bias);
-    hipLaunchKernelGGL((k_fused_pack<T, LD>), dim3((uint32_t)k.hg_groups), b, 0, s, k, c.w,
-                       c.w_stride, c.h, c.h_stride, c.labels, c.weights);
+    k.pack_groups = (int32_t)std::min<int64_t>(((k.v_pad + k.n_pad) * LD + 1023) / 1024,
+                                               std::min(8 * c.num_cus, MOST_GROUPS));
+    hipLaunchKernelGGL((k_fused_columns<T, LD>), dim3((uint32_t)(k.w_groups + k.h_groups)), b, 0, s,
+                       k, c);
+    if (!k.few)
+        hipLaunchKernelGGL(k_fused_scales, dim3(2 * LD / 32), dim3(1024), 0, s, k, LD);
+    hipLaunchKernelGGL((k_fused_pack<T, LD>), dim3((uint32_t)k.pack_groups), b, 0, s, k, c);
     const dim3 gr((uint32_t)(k.n_pad / XB * p.row_splits));
     const dim3 gj = grid_of(blocks(k.n_pad, 1024 / LD));
     if (!c.grad) {

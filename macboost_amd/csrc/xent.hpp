@@ -28,61 +28,50 @@ constexpr uint32_t XENT_HUGE = 0x5D800000u;
 // look them all over.  (Atomics on one word took 15 to 20 ns each, 42 us for the largest of
 // 16300 x 1000 f32 by 2048 workgroups, and a launch to clear it.)
 constexpr int MOST_GROUPS = 1024;
-constexpr uint32_t FLAG = 0x80000000u;   // beside a maximum of bits without a sign: an or
 struct XentMax {
     uint32_t part[MOST_GROUPS];
     uint32_t all;                        // a later kernel's first workgroup leaves it here
 };
 struct XentCtl {
-    XentMax w;                           // bits of the largest |W| that is finite; FLAG: a class
-                                         // is offered
-    XentMax hg;                          // of |w h|
+    XentMax offered;                     // 1: a class is
+    XentMax row;                         // see kernels_xent_fused.hip
 };
 
 __device__ __forceinline__ uint32_t finite_bits(float x) {
     const uint32_t b = __float_as_uint(fabsf(x));
     return b < 0x7F800000u ? b : 0u;
 }
-// The exponent that brings a maximum below 2^14 (0 for a maximum of 0).
-__device__ __forceinline__ int scale_exp(uint32_t max_bits) {
-    if (!max_bits) return 0;
-    const int s = 13 - ilogbf(__uint_as_float(max_bits));
-    return min(126, max(-126, s));
+// Packed operands lie below 2^TOP_EXP.
+constexpr int TOP_EXP = 14;
+// e, where |x| is in [2^(e-1), 2^e); NO_EXP for 0 and what is not finite.
+constexpr int NO_EXP = -(1 << 20);
+__device__ __forceinline__ int exponent_of(float x) {
+    return finite_bits(x) ? __builtin_amdgcn_frexp_expf(x) : NO_EXP;
 }
-__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+// 2^e, at most 2^127: 0 times it is 0.
+__device__ __forceinline__ float power_of_2(int e) { return ldexpf(1.0f, min(e, 127)); }
+
+template <typename V> __device__ __forceinline__ V wave_max(V v) {
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o, 64));
+    for (int o = 32; o > 0; o >>= 1) v = max(v, (V)__shfl_xor((int)v, o, 64));
     return v;
 }
-
-// Of a workgroup of WAVES wavefronts; all of its threads call it.  lds: 2 WAVES words, free
+// Of a workgroup of WAVES wavefronts; all of its threads call it.  lds: WAVES words, free
 // again at the end.
-template <int WAVES>
-__device__ __forceinline__ uint32_t largest(uint32_t v, uint32_t flag, uint32_t *lds) {
+template <int WAVES, typename V> __device__ __forceinline__ V largest(V v, V *lds) {
     v = wave_max(v);
-    flag = __any(flag != 0) ? FLAG : 0u;
-    if ((threadIdx.x & 63) == 0) {
-        lds[threadIdx.x >> 6] = v;
-        lds[WAVES + (threadIdx.x >> 6)] = flag;
-    }
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < WAVES; ++i) {
-        v = max(v, lds[i]);
-        flag |= lds[WAVES + i];
-    }
+    for (int i = 0; i < WAVES; ++i) v = max(v, lds[i]);
     __syncthreads();
-    return v | flag;
+    return v;
 }
 template <int WAVES>
 __device__ __forceinline__ uint32_t largest_of(const XentMax &m, int32_t groups, uint32_t *lds) {
-    uint32_t v = 0, flag = 0;
-    for (int g = threadIdx.x; g < groups; g += 64 * WAVES) {
-        const uint32_t p = m.part[g];
-        v = max(v, p & ~FLAG);
-        flag |= p & FLAG;
-    }
-    return largest<WAVES>(v, flag, lds);
+    uint32_t v = 0;
+    for (int g = threadIdx.x; g < groups; g += 64 * WAVES) v = max(v, m.part[g]);
+    return largest<WAVES>(v, lds);
 }
 
 __device__ __forceinline__ u16 bits_of(_Float16 v) { return __builtin_bit_cast(u16, v); }
@@ -99,8 +88,12 @@ __device__ __forceinline__ void split_f16(float x, u16 &hi, u16 &lo) {
 struct XentPack {
     int64_t n, v, n_pad, v_pad;
     int32_t d, ld;
-    int32_t w_groups, pack_w_groups, hg_groups;      // that look at W, pack W, pack h
+    int32_t w_groups, hg_groups;         // that look at W's and w h's columns
+    int32_t pack_w_groups, pack_h_groups;
+    bool few;                            // groups: those that pack sum them up
     XentCtl *ctl;
+    uint32_t *w_part, *hg_part;          // [group][ld] bits of the largest of a column
+    int32_t *w_exp, *hg_exp;             // [ld] a column is packed times 2^this
     u16 *h, *hg, *w;                     // planes of n_pad * ld, v_pad * ld; hg: gradients only
     float *bias;                         // [v_pad] the bias, -inf: not offered
     float *row_scale;                    // [n_pad] the scale of a score

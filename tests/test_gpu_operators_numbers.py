@@ -164,3 +164,63 @@ def test_classes_not_offered_beside_a_row_not_finite(ctx, kind, n, d, value):
     r = x.results()
     assert np.all(r["dw"][::7] == 0) and np.all(r["db"][::7] == 0)
     assert not np.isfinite(r["dw"][y[3]]).all()
+
+
+@KINDS
+@FORMS
+@pytest.mark.parametrize("k", [16, 24, 32, 40])
+@pytest.mark.parametrize("side", ["both", "h", "w"])
+def test_columns_of_different_sizes(ctx, kind, n, d, k, side):
+    """Every eighth column of h 2^k smaller, of w 2^k larger or smaller, or both, where the
+    scores stay as they are: f32 sums of products do not mind."""
+    _, h, w, y = _problem(n + d + 45, n, d, 150)
+    if side in ("both", "h"):
+        h[:, ::8] *= np.float32(2.0 ** -k)
+    if side in ("both", "w"):
+        w[:, ::8] *= np.float32(2.0 ** (k if side == "both" else -k))
+    weights = (np.random.default_rng(k).random(n) + 0.5).astype(np.float32)
+    x = D.Xent(ctx, h, w, y, kind, weights=weights)
+    x.grad()
+    want = D.xent_reference(h, w, y, kind, weights=weights)
+    if n > 32 and d <= 128:
+        # Columns of w and h are packed times 2^-r and 2^r, r half the difference of their largest
+        # exponents, to within 1.  f16 terms of operands below 2^14 are off by 2^-25 where
+        # that is more than their 22 bits: at least 2^13 is reached by the largest element of all
+        # of w and of each row of h.  What that gives from here on k of 2^33 in f32.
+        h64, w64 = (D.rounded(a, kind).astype(np.float64) for a in (h, w))
+        a = np.log2(np.abs(w64).max(0))
+        b = np.log2((np.abs(h64) / np.abs(h64).max(1, keepdims=True)).max(0))
+        r = (a - b) / 2
+        off_w = 2.0 ** -36 * 2.0 ** r * (np.abs(w64) * 2.0 ** -r).max()
+        off_h = 2.0 ** -36 * 2.0 ** -r * (np.abs(h64) * 2.0 ** r).max(1, keepdims=True)
+        z = h64 @ w64.T
+        g = np.exp(z - z.max(1, keepdims=True))
+        g /= g.sum(1, keepdims=True)
+        g[np.arange(n), y] -= 1
+        g = np.abs(g) * weights.astype(np.float64)[:, None]
+        for name, off in (("dh", g.sum(1, keepdims=True) * off_w), ("dw", g.T @ off_h)):
+            want[name] = (want[name][0], want[name][1] + off)
+    D.check(x.results(), want)
+
+
+@KINDS
+@FORMS
+def test_columns_of_zeros_and_of_one_side(ctx, kind, n, d):
+    """A column of w that is all zeros beside large values of h, and the other way round."""
+    _, h, w, y = _problem(n + d + 46, n, d, 150)
+    h[:, 2] *= np.float32(2.0 ** 60)
+    w[:, 2] = 0
+    w[:, 9] *= np.float32(2.0 ** 60)
+    h[:, 9] = 0
+    h[:, 11] = w[:, 11] = 0
+    h[4] = 0
+    x = D.Xent(ctx, h, w, y, kind)
+    x.grad()
+    r, want = x.results(), D.xent_reference(h, w, y, kind)
+    D.check(r, want)
+    x = D.Xent(ctx, np.zeros_like(h), w, y, kind)
+    x.grad()
+    D.check(x.results(), D.xent_reference(np.zeros_like(h), w, y, kind))
+    x = D.Xent(ctx, h, np.zeros_like(w), y, kind)
+    x.grad()
+    D.check(x.results(), D.xent_reference(h, np.zeros_like(w), y, kind))
