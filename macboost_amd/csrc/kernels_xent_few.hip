@@ -278,16 +278,16 @@ __global__ __launch_bounds__(64 * GRAD_WAVES, NB == 1 ? 4 : 2) void k_few_grad(X
     extern __shared__ char lds[];
     char *h = lds, *w = lds + chunks * CHUNK_BYTES;
     float *sums = reinterpret_cast<float *>(w + chunks * CHUNK_BYTES);   // [4][16][64]
-    // [row][class], and behind a row the bias of the class of its number
-    float *g = sums + 4 * 16 * 64;
+    float *g = sums + 4 * 16 * 64;                                       // [row][class]
     const int lane = threadIdx.x & 63, half = lane >> 5, l = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int blocks = (c.dim + 31) / 32;
-    // a row that is out is zeros here: what it holds reaches nothing
+    // A row that is out is zeros here: what it holds reaches nothing.  So is one whose lse is not
+    // finite: its G is NaN where a class is offered, and 0 times what it holds where none is.
     const int x0 = threadIdx.x >> 4;                 // the row that this lane brings
     Staged<NB * (int)sizeof(T)> staged;
     load<T, sizeof(T)>(staged, chunks, c.dim,
-                       x0 < c.rows && lse2[x0].y != INFINITY
+                       x0 < c.rows && fabsf(lse2[x0].y) < INFINITY
                            ? static_cast<const T *>(c.h) + x0 * c.h_stride : nullptr);
     store(h, staged, chunks);
     const auto ask = [&](int64_t t) {
@@ -355,7 +355,6 @@ __global__ __launch_bounds__(64 * GRAD_WAVES, NB == 1 ? 4 : 2) void k_few_grad(X
                     p *= wt;
                 }
                 g[l * G_STRIDE + x] = p;
-                if (l == 0) g[x * G_STRIDE + ROWS] = b;
             }
         __syncthreads();
         if (c.dbias && threadIdx.x < 32 && v0 + threadIdx.x < c.classes) {
@@ -378,11 +377,9 @@ __global__ __launch_bounds__(64 * GRAD_WAVES, NB == 1 ? 4 : 2) void k_few_grad(X
                 if (b * 32 + l < c.dim)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
-                        const int x = (r >> 2) * 8 + half * 4 + (r & 3);
-                        // not offered: 0, also beside a row that is not finite
-                        const float value = g[x * G_STRIDE + ROWS] == -INFINITY ? 0.0f : o[r];
-                        if (v0 + x < c.classes)
-                            static_cast<T *>(c.dw)[(v0 + x) * c.w_stride + b * 32 + l] = (T)value;
+                        const int64_t v = v0 + (r >> 2) * 8 + half * 4 + (r & 3);
+                        if (v < c.classes)
+                            static_cast<T *>(c.dw)[v * c.w_stride + b * 32 + l] = (T)o[r];
                     }
             }
         if (c.dh)
