@@ -34,7 +34,8 @@ struct XentMax {
 };
 struct XentCtl {
     XentMax offered;                     // 1: a class is
-    XentMax row;                         // see kernels_xent_fused.hip
+    XentMax row;                         // see kernels_xent_fused.hip, and this
+    uint32_t far;
 };
 
 __device__ __forceinline__ uint32_t finite_bits(float x) {
