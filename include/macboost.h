@@ -81,7 +81,9 @@ typedef struct mbk_context mbk_context;
 int mbk_context_create(int32_t device, mbk_context **out, char **err);
 /* No counterpart in the reference: a context whose calls queue on the caller's
  * stream (a hipStream_t of `device`; NULL: its default stream), in order with the
- * caller's own work there.  The stream must outlive the context.
+ * caller's own work there.  The stream must outlive the context; mbk_context_destroy waits for it.
+ * While it is captured no context is made on it, and mbk_context_destroy leaves the context as
+ * it is: call it again after the capture.
  * mbk_xent, mbk_xent_grad and the mbk_expert_ calls may be captured there into a
  * graph.  Their scratch belongs to the context: it grows outside a capture only (a
  * captured call that needs more is refused: make one of the same sizes before), what a

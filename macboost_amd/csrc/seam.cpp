@@ -221,6 +221,12 @@ mbk_context *make_context(std::unique_ptr<mb::Device> dev) {
     return c.release();
 }
 
+bool being_captured(hipStream_t s) {
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    MB_HIP(hipStreamIsCapturing(s, &st));
+    return st != hipStreamCaptureStatusNone;
+}
+
 // `device`, if there is one.
 int device_or_throw(int device) {
     int n = 0;
@@ -249,9 +255,7 @@ std::mutex &context_scratch_mutex(mbk_context *ctx) { return ctx->scratch.ops_mu
 
 char *context_scratch(mbk_context *ctx, size_t bytes) {
     Scratch &sc = ctx->scratch;
-    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-    MB_HIP(hipStreamIsCapturing(ctx->dev->stream, &st));
-    const bool capturing = st != hipStreamCaptureStatusNone;
+    const bool capturing = being_captured(ctx->dev->stream);
     if (sc.ops.n < bytes) {
         need(!capturing, "the context's scratch must grow, which a captured call cannot do: "
                          "make a call of the same sizes before the capture");
@@ -284,13 +288,21 @@ int mbk_context_create_on(int32_t device, void *stream, mbk_context **out, char 
             MB_HIP(hipStreamGetDevice(s, &of));
             need(of == device, "the stream belongs to another device");
         }
+        need(!being_captured(s), "the stream is being captured");
         *out = make_context(std::make_unique<mb::Device>(device, s));
         return 0;
     }, -1);
 }
 
 void mbk_context_destroy(mbk_context *ctx) {
-    if (ctx && ctx->dev) (void)hipStreamSynchronize(ctx->dev->stream);
+    if (ctx && ctx->dev) {
+        // what the graph has captured must stay, and a wait would end the capture
+        hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+        if (ctx->dev->borrowed && hipStreamIsCapturing(ctx->dev->stream, &st) == hipSuccess &&
+            st != hipStreamCaptureStatusNone)
+            return;
+        (void)hipStreamSynchronize(ctx->dev->stream);
+    }
     delete ctx;
 }
 
