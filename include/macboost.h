@@ -329,7 +329,7 @@ typedef struct {
     int64_t classes;             /* 1..2^31-256 */
     int32_t dim;                 /* 1..2^20 */
     int32_t type;                /* of h, w, dh, dw: MBK_F32 or MBK_BF16 */
-    int64_t h_stride, w_stride;  /* elements from row to row, >= dim */
+    int64_t h_stride, w_stride;  /* elements from row to row, dim..2^40 */
 } mbk_xent_shape;
 int mbk_xent(mbk_context *ctx, const mbk_xent_shape *shape, const void *h, const void *w,
              const float *bias, const int32_t *labels, const float *weights, float *loss,

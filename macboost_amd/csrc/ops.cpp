@@ -16,6 +16,7 @@ void need(bool ok, const char *what) {
 
 constexpr int64_t MOST_ROWS = 0x7FFFFF00;
 constexpr int32_t MOST_EXPERTS = 8192;       // counters of four wavefronts in LDS
+constexpr int64_t MOST_STRIDE = (int64_t)1 << 40;
 
 bool is_bf16(int32_t type) {
     need(type == MBK_F32 || type == MBK_BF16, "type must be MBK_F32 or MBK_BF16");
@@ -31,6 +32,8 @@ mbk::XentCall xent_call(const mbk_xent_shape *sh, const void *h,
     need(sh->dim >= 1 && sh->dim <= (1 << 20), "dim must be in 1..2^20");
     need(sh->h_stride >= sh->dim && sh->w_stride >= sh->dim,
          "h_stride and w_stride must be at least dim");
+    need(sh->h_stride <= MOST_STRIDE && sh->w_stride <= MOST_STRIDE,
+         "h_stride and w_stride must be at most 2^40");
     need(w && (!sh->rows || (h && labels && loss && lse)), "null argument");
     mbk::XentCall c{};
     c.rows = sh->rows;
@@ -73,9 +76,8 @@ mbk::ExpertMatrix expert_matrix(const mbk_expert_matrix *m, int64_t rows) {
     need(m->cols <= (1 << 30), "cols must be at most 2^30");
     need(m->data || !rows, "null matrix data");
     // no element twice: rows apart by a row's columns, or columns by a column's rows
-    constexpr int64_t MOST = (int64_t)1 << 40;
     const int64_t rs = m->row_stride, cs = m->col_stride;
-    need(rs >= 1 && cs >= 1 && rs <= MOST && cs <= MOST &&
+    need(rs >= 1 && cs >= 1 && rs <= MOST_STRIDE && cs <= MOST_STRIDE &&
              ((m->cols - 1) <= (rs - 1) / cs || rows - 1 <= (cs - 1) / rs),
          "row_stride and col_stride must be in 1..2^40 and keep the elements apart");
     return {m->data, m->row_stride, m->col_stride, m->cols, is_bf16(m->type), m->blocked != 0};
