@@ -321,8 +321,10 @@ int mbk_treeshap(mbk_context *ctx, const int32_t *feature, const float *threshol
  * column for w and h (of rows brought to one size), if the column's |h| |w| is 2^-2k of the
  * largest column's, and for a row's share of dw 2^-38 of the largest weight times row.
  * The results do not depend on the call, bit for bit.
- * To boost output j with them: mbk_quantize with objective 0, preds = dh's column j
- * and labels of 0. */
+ * To boost output j with them: mbk_quantize with objective 0, labels of 0 and preds = dh's
+ * column j, which it takes as rows values one after another.  Forests' outputs lie like that, too,
+ * [dim][rows].  With every row's expert 0 (below), mbk_expert_combine brings those into h, and
+ * mbk_expert_gather dh into [dim][rows], blocked both. */
 enum { MBK_F32 = 0, MBK_BF16 = 1 };
 typedef struct {
     int64_t rows;                /* 0..2^31-256 */
