@@ -837,10 +837,14 @@ int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 uint32_t blocks(int64_t x, int64_t per) { return (uint32_t)((x + per - 1) / per); }
 
 // Workgroups for `blocks` X blocks over `tiles` Y tiles: two run on a CU at once, and
-// the last round of them should be full.  At least 4 tiles a split.
-int32_t pick_splits(int64_t x_blocks, int64_t tiles, int num_cus) {
+// the last round of them should be full.  At least 4 tiles a split, and at most 512 MB of
+// parts, unless one takes more: past that a fuller last round is a few percent of many (1M x 128
+// x 1M f32: 11 splits and 5.6 GB for 4 %).
+constexpr int64_t PART_BYTES = (int64_t)512 << 20;
+int32_t pick_splits(int64_t x_blocks, int64_t tiles, int64_t part_bytes, int num_cus) {
     const int64_t slots = 2 * (int64_t)num_cus;
-    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(tiles / 4, 64));
+    const int64_t most =
+        std::max<int64_t>(1, std::min<int64_t>({tiles / 4, 64, PART_BYTES / part_bytes}));
     int64_t best = 1;
     double cost = 1e30;
     for (int64_t s = 1; s <= most; ++s) {
@@ -870,8 +874,9 @@ Plan plan_of(const XentCall &c) {
     p.ld = row_ld(p.ks);
     p.n_pad = up(c.rows, XB);
     p.v_pad = up(c.classes, XB);
-    p.row_splits = pick_splits(p.n_pad / XB, p.v_pad / TY, c.num_cus);
-    p.class_splits = pick_splits(p.v_pad / XB, p.n_pad / TY, c.num_cus);
+    const int64_t part_row = c.grad ? 4 * p.ld : 8;
+    p.row_splits = pick_splits(p.n_pad / XB, p.v_pad / TY, part_row * p.n_pad, c.num_cus);
+    p.class_splits = pick_splits(p.v_pad / XB, p.n_pad / TY, part_row * p.v_pad, c.num_cus);
     size_t at = 0;
     auto take = [&](size_t bytes) {
         const size_t here = at;
