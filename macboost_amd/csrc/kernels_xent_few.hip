@@ -268,7 +268,7 @@ __device__ __forceinline__ void store(char *m, const Staged<N> &s, int chunks) {
 
 // part_dh[workgroup][row][dim].
 // The next tile of W is asked for while this one is worked on.  NB: blocks of 32 columns
-// that a wavefront keeps of dh; with one, two workgroups fit a CU's registers.
+// that a wavefront keeps of dh; with one, two workgroups fit a CU's registers (grad_groups).
 template <typename T, int B, int NB>
 __global__ __launch_bounds__(64 * GRAD_WAVES, NB == 1 ? 4 : 2) void k_few_grad(XentCall c, int64_t tiles,
                                                                  int32_t chunks,
@@ -430,18 +430,23 @@ size_t part_bytes(const XentCall &c) { return (size_t)c.num_cus * ROWS * sizeof(
 
 // Columns that a workgroup of k_few_grad keeps with one block a wavefront.
 constexpr int ONE_BLOCK = 32 * GRAD_WAVES;
-int grad_groups(const XentCall &c) { return (c.dim <= ONE_BLOCK ? 2 : 1) * c.num_cus; }
+int32_t grad_chunks(const XentCall &c) { return (c.dim * (c.bf16 ? 2 : 4) + 15) / 16; }
+size_t grad_lds(const XentCall &c) {
+    return (size_t)2 * grad_chunks(c) * CHUNK_BYTES + 4 * (4 * 16 * 64 + ROWS * G_STRIDE);
+}
+// Two workgroups a CU where they fit its LDS, too (f32: up to 232 outputs).
+int grad_groups(const XentCall &c) {
+    return (c.dim <= ONE_BLOCK && 2 * grad_lds(c) <= LDS_BYTES ? 2 : 1) * c.num_cus;
+}
 
 template <typename T, int B, int NB>
 hipError_t run_grad(hipStream_t s, const XentCall &c, const float2 *lse2, float *part_dh) {
     const hipError_t e = allow_all_lds(reinterpret_cast<const void *>(k_few_grad<T, B, NB>));
     if (e != hipSuccess) return e;
-    constexpr int PER = 16 / sizeof(T);
-    const int32_t chunks = (c.dim + PER - 1) / PER;
+    const int32_t chunks = grad_chunks(c);
     const int64_t tiles = (c.classes + 31) / 32;
     const uint32_t groups = (uint32_t)std::min<int64_t>(grad_groups(c), tiles);
-    const size_t lds = (size_t)2 * chunks * CHUNK_BYTES + 4 * (4 * 16 * 64 + ROWS * G_STRIDE);
-    hipLaunchKernelGGL((k_few_grad<T, B, NB>), dim3(groups), dim3(64 * GRAD_WAVES), lds, s, c,
+    hipLaunchKernelGGL((k_few_grad<T, B, NB>), dim3(groups), dim3(64 * GRAD_WAVES), grad_lds(c), s, c,
                        tiles, chunks, lse2, part_dh);
     if (c.dh)
         hipLaunchKernelGGL((k_few_join_dh<T>), dim3((uint32_t)((c.rows * c.dim + 63) / 64)),
