@@ -628,8 +628,9 @@ __global__ __launch_bounds__(C::WAVES * 64, 2) void k_xent_stats(XentPack k, int
 }
 
 // The parts of a row joined, one wavefront a row: lse, as reference and log2 of the sum for
-// the gradients, and loss.  The label's score is summed in f32 from h and W themselves.  For gradients, h is packed once more as dW's product
-// takes it, times the row's weight and with its columns' scales (the rows are summed over).
+// the gradients, and loss.  The label's score is summed in f32 from h and W themselves.  For
+// gradients, h is packed once more as dW's product takes it, times the row's weight and with
+// powers of two of its columns (the rows are summed over).
 template <typename T>
 __global__ __launch_bounds__(256) void k_xent_join(XentPack k, XentCall c, int32_t parts,
                                                    const float2 *__restrict__ part,
