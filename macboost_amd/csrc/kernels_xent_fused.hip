@@ -606,6 +606,14 @@ __global__ __launch_bounds__(256) void k_fused_join_rows(Fused k, XentCall c, in
     const int f = threadIdx.x % LANES * 4;
     const int32_t y = k.label[i];
     const bool open = y >= 0 && k.bias[y] != -INFINITY;
+    const float wt = k.weight[i];
+    const int32_t exp = k.exp[i];
+    int32_t ex[4] = {0, 0, 0, 0}, row_exp = 0;       // asked for ahead of the stores
+    if constexpr (GRAD) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ex[e] = k.exp2[f + e];
+        row_exp = wq_exp(k.ctl->row.all);
+    }
     float wy[4] = {0.0f, 0.0f, 0.0f, 0.0f}, dot = 0.0f;
     if (open)
 #pragma unroll
@@ -635,7 +643,6 @@ __global__ __launch_bounds__(256) void k_fused_join_rows(Fused k, XentCall c, in
         }
     }
     const LogSum l = log_sum(sum, P_EXP);
-    const float wt = k.weight[i];
     if (f == 0) {
         if (i < k.n) {
             const float z = open ? dot + (c.bias ? c.bias[y] : 0.0f) : -INFINITY;
@@ -648,9 +655,8 @@ __global__ __launch_bounds__(256) void k_fused_join_rows(Fused k, XentCall c, in
             k.c2[i] = y < 0 ? -INFINITY : -__builtin_fmaf(ref, LOG2E, l.base2);
             if (y >= 0 && fabsf(ref) >= FAR) k.ctl->far = 1;
             // a row of zeros has no power of two; a weight that is not finite stays so
-            const int e = k.exp[i];
-            k.wq[i] = e != ZERO_ROW ? ldexpf(wt, wq_exp(k.ctl->row.all) - e)
-                                    : fabsf(wt) < INFINITY ? 0.0f : wt;
+            k.wq[i] = exp != ZERO_ROW ? ldexpf(wt, row_exp - exp)
+                                      : fabsf(wt) < INFINITY ? 0.0f : wt;
         }
     }
     if constexpr (GRAD) {
@@ -659,7 +665,7 @@ __global__ __launch_bounds__(256) void k_fused_join_rows(Fused k, XentCall c, in
         for (int e = 0; e < 4; ++e)
             if (f + e < k.d) {
                 // divided first: the sum of 2^13 p W is beyond f32 for W that is not
-                const float g = y < 0 ? 0.0f : wt * (ldexpf(o[e] / sum, -k.exp2[f + e]) - wy[e]);
+                const float g = y < 0 ? 0.0f : wt * (ldexpf(o[e] / sum, -ex[e]) - wy[e]);
                 static_cast<T *>(c.dh)[i * c.h_stride + f + e] = (T)g;
             }
     }
@@ -822,13 +828,16 @@ __global__ __launch_bounds__(256) void k_fused_join_classes(Fused k, XentCall c,
     if (v >= k.v) return;
     const bool open = k.bias[v] != -INFINITY;
     const int exp = wq_exp(k.ctl->row.all);
+    int32_t ex[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) ex[e] = k.exp2[f + e];
     const float x[4] = {sum.x, sum.y, sum.z, sum.w};
     if (c.dw)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
             if (f + e < k.d)
                 static_cast<T *>(c.dw)[v * c.w_stride + f + e] =
-                    (T)(open ? ldexpf(x[e], k.exp2[f + e] - exp) : 0.0f);
+                    (T)(open ? ldexpf(x[e], ex[e] - exp) : 0.0f);
     if (c.dbias && l == 0) c.dbias[v] = open ? (float)db : 0.0f;
 }
 
