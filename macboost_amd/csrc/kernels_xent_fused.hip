@@ -188,26 +188,32 @@ __global__ __launch_bounds__(1024) void k_fused_scales(Fused k, int32_t ld) {
     k.col[(of_w ? 0 : ld) + col] = m;
 }
 
-// The same of few groups, by each workgroup of the next kernel, without a launch (4.5 us).
+// The same of few groups, by each workgroup of the next kernel, without a launch (4.5 us):
+// whether a class is offered.
 constexpr int FEW_GROUPS = 64;
 template <int LD>
-__device__ __forceinline__ void few_columns(const Fused &k, int32_t *col, int32_t (&part)[256]) {
+__device__ __forceinline__ bool few_columns(const Fused &k, int32_t *col, int32_t (&part)[2][256]) {
     const int32_t c = threadIdx.x % LD, slice = threadIdx.x / LD;
+    const int32_t *from = k.part + c;
+    int w = NO_EXP, h = NO_EXP;
+#pragma unroll 4
+    for (int g = slice; g < k.w_groups; g += 256 / LD) w = max(w, from[g * LD]);
+    from += k.w_groups * LD;
+#pragma unroll 4
+    for (int g = slice; g < k.h_groups; g += 256 / LD) h = max(h, from[g * LD]);
+    const bool any = (int32_t)threadIdx.x < k.w_groups && k.ctl->offered.part[threadIdx.x];
+    part[0][threadIdx.x] = w;
+    part[1][threadIdx.x] = h;
+    const bool offered = __syncthreads_or(any);
+    if (threadIdx.x < 2 * LD) {
+        const int32_t *p = part[threadIdx.x / LD] + c;
+        int m = p[0];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int32_t first = h ? k.w_groups : 0, groups = h ? k.h_groups : k.w_groups;
-        int m = NO_EXP;
-#pragma unroll 8
-        for (int g = slice; g < groups; g += 256 / LD) m = max(m, k.part[(first + g) * LD + c]);
-        part[threadIdx.x] = m;
-        __syncthreads();
-        if (threadIdx.x < LD) {
-#pragma unroll
-            for (int q = 1; q < 256 / LD; ++q) m = max(m, part[threadIdx.x + q * LD]);
-            col[h * LD + threadIdx.x] = m;
-        }
-        __syncthreads();
+        for (int q = 1; q < 256 / LD; ++q) m = max(m, p[q * LD]);
+        col[threadIdx.x] = m;
     }
+    __syncthreads();
+    return offered;
 }
 
 // Column threadIdx.x's power of two, by the first LD threads: a, b are the largest exponents
@@ -236,8 +242,8 @@ template <typename T, int LD>
 __global__ __launch_bounds__(256) void k_fused_pack(Fused k, XentCall c) {
     constexpr int LANES = LD / 4, ROWS = 256 / LANES;
     const int f = threadIdx.x % LANES * 4;
-    __shared__ int32_t words[4], exps[LD], cols[2 * LD], part[256];
-    if (k.few) few_columns<LD>(k, cols, part);
+    __shared__ int32_t words[4], exps[LD], cols[2 * LD], part[2][256];
+    const bool any = k.few ? few_columns<LD>(k, cols, part) : k.ctl->offered.all != 0;
     const int mine = column_exp<LD>(k.few ? cols : k.col, words);
     if (threadIdx.x < LD) {
         exps[threadIdx.x] = mine;
@@ -248,9 +254,6 @@ __global__ __launch_bounds__(256) void k_fused_pack(Fused k, XentCall c) {
     int ex[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) ex[e] = exps[f + e];
-    const bool any = k.few ? largest_of<4>(k.ctl->offered, k.w_groups,
-                                           reinterpret_cast<uint32_t *>(words)) != 0
-                           : k.ctl->offered.all != 0;
     uint32_t row = 0;
     for (int64_t at = (int64_t)blockIdx.x * ROWS + threadIdx.x / LANES; at < k.v_pad + k.n_pad;
          at += (int64_t)k.pack_groups * ROWS) {
