@@ -34,11 +34,11 @@
 // that could overflow: what they hold reaches nothing, and a finite row that is out is
 // multiplied by zeros.
 //
-// The matrix instructions bound all four: 16384 x 1024 x 65536 bf16 takes 2.03 ms for the
-// statistics (1.08 PFLOP/s), 2.67 for G (0.82; it writes 2.1 GB), 2.22 for dh (0.99) and 2.10
-// for dW (1.05), with the matrix cores busy 50 to 55 % of the cycles at 1.85 GHz, where the
-// power limit holds the clock; a library product of bf16 reaches 1.23 to 1.56.  Without
-// their copies the products take 17 % less.
+// 16384 x 1024 x 65536 bf16 takes 2.1 ms for the statistics (1.05 PFLOP/s), 2.55 for G (0.86; it
+// writes 2.1 GB) and 4.27 for dh and dW (1.03); a library product of bf16 reaches 1.23 to 1.56.
+// The matrix cores are busy 50 to 53 % of the cycles (G 41 %), at 1.85 to 1.9 GHz, where the
+// kernels that pack run at 2.4; the wavefronts wait for 38 to 47 % of theirs, at the ends of steps
+// of copies and of LDS reads.  Without their copies the products take 17 % less.
 #include <algorithm>
 
 #include "mbk.h"
@@ -203,8 +203,9 @@ __global__ __launch_bounds__(64 * SCALE_WAVES) void k_xent_scales(XentPack k) {
     for (int w = 1; w < SCALE_WAVES; ++w) m = max(m, most[w][lane]);
     (of_w ? k.w_exp : k.hg_exp)[col] = column_exp(m, of_w);
 }
-// Of few groups and columns, by each workgroup of the next kernel, without a launch (4.5 us):
-// W's in LDS, and both in memory by the first one.
+// Of few groups and columns, by each workgroup of the next kernel, without a launch: W's in LDS,
+// and both in memory by the first one (2000 x 256 x 2000 f32, 32 groups, 29 us and 30.5 with
+// the launch, 4000 x 256 x 4000, 63 groups, 52.5 and 51).
 constexpr int FEW_GROUPS = 32, FEW_COLUMNS = 64 * MAX_WAVES;
 __device__ __forceinline__ bool few_scales(const XentPack &k, int32_t *exps, uint32_t *words) {
     const int32_t col = threadIdx.x;

@@ -9,7 +9,7 @@
 // rows across): a lane has scores of one row, and keeps its maximum and sum over all
 // tiles.  f32 operands go into the f32 matrix instruction as they are: at 1/16 of
 // the bf16 rate it still takes less time than W's bytes.  16 x 1024 x 100000 bf16: 55 us, W at
-// 4.6 TB/s by the first kernel.  (32 rows are one operand of the instruction: with gradients,
+// 4.9 TB/s by the first kernel.  (32 rows are one operand of the instruction: with gradients,
 // 32 x 512 x 100000 f32 239 us here and 494 by the kernels for more rows, 32 x 64 x 1000 22 and 37.)
 // Copies of 16 bytes a lane where W's rows are aligned to them, else of 4, or by registers:
 // 16 x 512 x 100000 f32 63 us by 16 bytes, 84 by 4.

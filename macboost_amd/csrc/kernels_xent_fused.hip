@@ -23,11 +23,11 @@
 // and are held with 22 bits up to k = 16, with 38 - k from there on.  P carries the rows' weights
 // over their powers of two into dW, off by 2^-40 of the largest.
 //
-// The matrix instructions bound both passes: 20000 x 100 x 10000 f32 takes 268 and 285 us,
-// 1.09 and 1.03 PFLOP/s of f16 products (112 columns of the first and 128 of the second, three
-// terms), with the matrix cores busy 55 % of the cycles at 1.85 GHz, where the power limit holds
-// the clock.  Without the exponentials the rows pass takes 6 % less, without the split of P
-// into terms 5 %.
+// 20000 x 100 x 10000 f32 takes 262 and 275 us, 1.12 and 1.06 PFLOP/s of f16 products (112 columns
+// of the first and 128 of the second, three terms), with the matrix cores busy 51 to 54 % of the
+// cycles at 1.92 to 1.96 GHz.  Without the exponentials the rows pass takes 6 % less, without the
+// split of P into terms 5 %.  bf16, with a third of the products and as many exponentials, takes
+// 128 and 146 us: matrix cores busy 34 and 29 %, vector instructions 41 and 37 %.
 #include <algorithm>
 
 #include "mbk.h"
@@ -46,7 +46,7 @@ constexpr int TY = 64;                   // Y rows of a tile
 constexpr int P_EXP = 13;
 constexpr float LAG = 1.38f;
 // exp(z - ref) is 2^(z log2 e + c), c = -ref log2 e, in two instructions where that fits f32 by
-// far, else in three (bf16 20000 x 32 x 10000 188 and 173 us with gradients).
+// far, else in three (bf16 20000 x 32 x 10000 with gradients 187 us, by three always 195).
 constexpr float FAR = 0x1p100f;
 
 // Elements of a packed row for KS slabs of 16.
@@ -188,8 +188,9 @@ __global__ __launch_bounds__(1024) void k_fused_scales(Fused k, int32_t ld) {
     k.col[(of_w ? 0 : ld) + col] = m;
 }
 
-// The same of few groups, by each workgroup of the next kernel, without a launch (4.5 us):
-// whether a class is offered.
+// The same of few groups, by each workgroup of the next kernel, without a launch (2000 x 64 x
+// 2000 f32, 64 groups, 24.4 us and 25.1 with the launch, 3500 x 128 x 4000, 235 groups, 45 and
+// 40): whether a class is offered.
 constexpr int FEW_GROUPS = 64;
 template <int LD>
 __device__ __forceinline__ bool few_columns(const Fused &k, int32_t *col, int32_t (&part)[2][256]) {
