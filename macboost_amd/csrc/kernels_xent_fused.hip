@@ -45,9 +45,10 @@ constexpr int TY = 64;                   // Y rows of a tile
 // f16 terms is at most 2^15 and keeps steps of 2^-38.
 constexpr int P_EXP = 13;
 constexpr float LAG = 1.38f;
-// exp(z - ref) is 2^(z log2 e + c), c = -ref log2 e, in two instructions where that fits f32 by
-// far, else in three (bf16 20000 x 32 x 10000 with gradients 187 us, by three always 195).
-constexpr float FAR = 0x1p100f;
+// exp(z - ref) is 2^(z log2 e + c), c = -ref log2 e, in two instructions, else in three (bf16 20000
+// x 32 x 10000 with gradients 187 us, by three always 195).  c's rounding is a relative error of
+// |ref| 2^-24, no more than z's own: up to here 2^-16.
+constexpr float FAR = 256.0f;
 
 // Elements of a packed row for KS slabs of 16.
 __host__ __device__ constexpr int row_ld(int ks) { return ks <= 2 ? 32 : ks <= 4 ? 64 : 128; }

@@ -19,12 +19,12 @@ def _biased_reference(h, w, y, kind, bias):
     bias, and how far each may be off.  A class's score is off by its operands' and its
     sum's half steps and by a step of the rounding with the bias, but where a rounding that
     large goes one way for all classes of a probability, as here, by the dot product's alone:
-    a bias beyond 2^60 leaves nothing of a dot product of this size."""
+    a bias beyond 2^31 leaves nothing of a dot product of this size."""
     h, w = D.rounded(h, kind).astype(np.float64), D.rounded(w, kind).astype(np.float64)
     n, d = h.shape
     v = w.shape[0]
     b = np.asarray(bias, np.float32).astype(np.float64)
-    huge = np.abs(b) > 2.0 ** 60
+    huge = np.abs(b) > 2.0 ** 31
     split = 0.0 if kind == "bf16" else 3 * 2.0 ** -22
     products = 1 if kind == "bf16" else 3
     dot = h @ w.T
@@ -73,13 +73,19 @@ BIASES = {
     "all_low_two_kinds": lambda v: np.where(np.arange(v) % 2 == 0, -2.5e38, LOWEST),
     "high": lambda v: np.where(np.arange(v) % 2 == 0, 3e38, 0.0),
     "both_ends": lambda v: np.where(np.arange(v) % 2 == 0, -LOWEST, LOWEST),
+    "all_1000": lambda v: np.full(v, 1000.0),
+    "all_1e10": lambda v: np.full(v, 1e10),
+    "all_-1e10": lambda v: np.full(v, -1e10),
+    "all_1e20": lambda v: np.full(v, 1e20),
+    "some_-1e5": lambda v: np.where(np.arange(v) % 3 == 0, -1e5, 0.0),
 }
 
 
 @KINDS
 @FORMS
 @pytest.mark.parametrize("what", ["labels_masked", "all_lowest", "one_kept_of_low",
-                                  "all_low_two_kinds", "high"])
+                                  "all_low_two_kinds", "high", "all_1000", "all_1e10", "all_-1e10",
+                                  "all_1e20", "some_-1e5"])
 def test_finite_biases(ctx, kind, n, d, what):
     """A class is not offered if its bias is -inf, and only then."""
     _, h, w, y = _problem(n + d + 40, n, d, 90)
