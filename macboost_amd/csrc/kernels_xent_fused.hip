@@ -888,7 +888,8 @@ Plan plan_of(const XentCall &c) {
     p.ld = row_ld(p.ks);
     p.n_pad = up(c.rows, XB);
     p.v_pad = up(c.classes, XB);
-    const int64_t part_row = c.grad ? 4 * p.ld : 8;
+    // of the loss alone as with gradients, so that its bits are the same
+    const int64_t part_row = 4 * p.ld;
     p.row_splits = pick_splits(p.n_pad / XB, p.v_pad / TY, part_row * p.n_pad, c.num_cus);
     p.class_splits = pick_splits(p.v_pad / XB, p.n_pad / TY, part_row * p.v_pad, c.num_cus);
     size_t at = 0;

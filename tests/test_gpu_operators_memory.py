@@ -35,3 +35,23 @@ def test_parts_of_many_rows():
     assert np.all(np.abs(got - np.log(classes)) <= (classes + 32) * 2.0 ** -24 + 1e-6)
     assert not c.download(dh, (rows, dim), np.float32).any()
     c.close()
+
+
+def test_loss_of_many_rows_with_and_without_gradients():
+    """Bit for bit, also where the parts' size sets their number."""
+    rows, dim, classes = 600_000, 128, 20_000
+    rng = np.random.default_rng(4)
+    c = mb.Context(0)
+    h = c.upload(np.tile(rng.standard_normal((6000, dim)).astype(np.float32), (100, 1)))
+    w = c.upload((rng.standard_normal((classes, dim)) / 8).astype(np.float32))
+    labels = c.upload(np.tile(rng.integers(0, classes, 6000).astype(np.int32), 100))
+    loss, lse, dh = c.alloc(rows * 4), c.alloc(rows * 4), c.alloc(rows * dim * 4)
+    shape = _core.MbkXentShape(rows, classes, dim, _core.F32, dim, dim)
+    got = []
+    for name, more in (("mbk_xent_grad", (dh, None, None)), ("mbk_xent", ())):
+        c.call(name, ctypes.byref(shape), h, w, None, labels, None, loss, lse, *more)
+        c.sync()
+        got.append((c.download(loss, rows, np.float32), c.download(lse, rows, np.float32)))
+    assert np.array_equal(got[0][0], got[1][0]) and np.array_equal(got[0][1], got[1][1])
+    assert np.isfinite(got[0][0]).all()
+    c.close()
