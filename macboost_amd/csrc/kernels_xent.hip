@@ -112,6 +112,15 @@ __device__ __forceinline__ void pack8(const float (&x)[8], const int (&s)[8], u1
     if (sizeof(T) == 4) *reinterpret_cast<u16x8 *>(to + plane) = lo;
 }
 constexpr int MAX_WAVES = 8;              // of the kernels that prepare
+// A weight, its exponent apart: times h it may pass f32, where G is small.
+struct Apart {
+    float mantissa;
+    int exp;
+};
+__device__ __forceinline__ Apart apart(float w) {
+    const int e = exponent_of(w);
+    return e != NO_EXP ? Apart{__builtin_amdgcn_frexp_mantf(w), e} : Apart{w, 0};
+}
 // Whether row i counts.  A class offered is looked for elsewhere.
 __device__ __forceinline__ bool row_in(const XentPack &k, const XentCall &c, int64_t i, float &wt) {
     const int32_t y = c.labels[i];
@@ -125,7 +134,7 @@ __device__ __forceinline__ bool row_in(const XentPack &k, const XentCall &c, int
 constexpr int COLUMNS = 256, COLUMN_ROWS = 2 * MAX_WAVES, ROWS_AHEAD = 4;
 template <typename T>
 __global__ __launch_bounds__(64 * MAX_WAVES) void k_xent_columns(XentPack k, XentCall c) {
-    __shared__ uint32_t most[COLUMN_ROWS][COLUMNS];
+    __shared__ int32_t most[COLUMN_ROWS][COLUMNS];
     const int lane = threadIdx.x & 31, r = threadIdx.x >> 5;
     const bool of_w = (int32_t)blockIdx.x < k.w_groups;
     const int32_t group = of_w ? blockIdx.x : blockIdx.x - k.w_groups;
@@ -133,7 +142,7 @@ __global__ __launch_bounds__(64 * MAX_WAVES) void k_xent_columns(XentPack k, Xen
     const void *from = of_w ? c.w : c.h;
     const int align = alignment<T>(from, stride);
     const int32_t f = blockIdx.y * COLUMNS + lane * 8;
-    uint32_t m[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    int m[8] = {NO_EXP, NO_EXP, NO_EXP, NO_EXP, NO_EXP, NO_EXP, NO_EXP, NO_EXP};
     bool any = false;
     // four rows at a time, so that as many loads are on the way
     const int64_t hop = (int64_t)(of_w ? k.w_groups : k.hg_groups) * COLUMN_ROWS;
@@ -156,9 +165,12 @@ __global__ __launch_bounds__(64 * MAX_WAVES) void k_xent_columns(XentPack k, Xen
         }
         // times 0 a value that is not finite is none either
 #pragma unroll
-        for (int q = 0; q < ROWS_AHEAD; ++q)
+        for (int q = 0; q < ROWS_AHEAD; ++q) {
+            const Apart w = apart(wt[q]);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) m[e] = max(m[e], finite_bits(x[q][e] * wt[q]));
+            for (int e = 0; e < 8; ++e)
+                m[e] = max(m[e], exponent_of(x[q][e] * w.mantissa) + w.exp);
+        }
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) most[r][lane * 8 + e] = m[e];
@@ -166,30 +178,30 @@ __global__ __launch_bounds__(64 * MAX_WAVES) void k_xent_columns(XentPack k, Xen
     if (of_w && blockIdx.y == 0 && threadIdx.x == 0) k.ctl->offered.part[group] = offered;
     const int64_t col = (int64_t)blockIdx.y * COLUMNS + threadIdx.x;
     if (threadIdx.x >= COLUMNS || col >= k.ld) return;
-    uint32_t v = 0;
+    int v = NO_EXP;
 #pragma unroll
     for (int q = 0; q < COLUMN_ROWS; ++q) v = max(v, most[q][threadIdx.x]);
     (of_w ? k.w_part : k.hg_part)[group * (int64_t)k.ld + col] = v;
 }
 
-// A column's power of two, of the bits of its largest.  A column of W that is all zeros has one
+// A column's power of two, of its largest exponent.  A column of W that is all zeros has one
 // that keeps h's column from its rows' scales.
 constexpr int ZERO_COLUMN = 1000;
-__device__ __forceinline__ int32_t column_exp(uint32_t most, bool of_w) {
-    const int e = exponent_of(__uint_as_float(most));
-    return e != NO_EXP ? TOP_EXP - e : of_w ? ZERO_COLUMN : 0;
+__device__ __forceinline__ int32_t column_exp(int e, bool of_w) {
+    return e > NO_EXP / 2 ? TOP_EXP - e : of_w ? ZERO_COLUMN : 0;
 }
 // All of them: 64 columns a workgroup, whose wavefronts go over the groups in turns.
 constexpr int SCALE_WAVES = 16;
 __global__ __launch_bounds__(64 * SCALE_WAVES) void k_xent_scales(XentPack k) {
-    __shared__ uint32_t most[SCALE_WAVES][64], words[SCALE_WAVES];
+    __shared__ int32_t most[SCALE_WAVES][64];
+    __shared__ uint32_t words[SCALE_WAVES];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int32_t cols = k.ld / 64;
     const bool of_w = (int32_t)blockIdx.x < cols;
     const int64_t col = (int64_t)(of_w ? blockIdx.x : blockIdx.x - cols) * 64 + lane;
-    const uint32_t *part = of_w ? k.w_part : k.hg_part;
+    const int32_t *part = of_w ? k.w_part : k.hg_part;
     const int32_t groups = of_w ? k.w_groups : k.hg_groups;
-    uint32_t m = 0;
+    int m = NO_EXP;
 #pragma unroll 8
     for (int g = wave; g < groups; g += SCALE_WAVES) m = max(m, part[(int64_t)g * k.ld + col]);
     most[wave][lane] = m;
@@ -210,7 +222,7 @@ constexpr int FEW_GROUPS = 32, FEW_COLUMNS = 64 * MAX_WAVES;
 __device__ __forceinline__ bool few_scales(const XentPack &k, int32_t *exps, uint32_t *words) {
     const int32_t col = threadIdx.x;
     if (col < k.ld) {
-        uint32_t w = 0, h = 0;
+        int w = NO_EXP, h = NO_EXP;
 #pragma unroll 8
         for (int g = 0; g < k.w_groups; ++g) w = max(w, k.w_part[g * k.ld + col]);
         exps[col] = column_exp(w, true);
@@ -663,14 +675,17 @@ __global__ __launch_bounds__(256) void k_xent_join(XentPack k, XentCall c, int32
     if (k.hg) {
         const int align = alignment<T>(c.h, c.h_stride);
         const int32_t d = y >= 0 ? k.d : 0;
-        const float wt = k.weight[i];
+        const Apart wt = apart(k.weight[i]);
         for (int32_t f = lane * 8; f < k.ld; f += 512) {
             float x[8];
             int s[8];
             load8<T>(c.h, i * c.h_stride, f, d, align, x);
             load8<int32_t>(k.hg_exp, f, s);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] *= wt;
+            for (int e = 0; e < 8; ++e) {
+                x[e] *= wt.mantissa;
+                s[e] += wt.exp;
+            }
             pack8<T>(x, s, k.hg + i * k.ld + f, k.n_pad * k.ld);
         }
     }
@@ -1099,8 +1114,8 @@ hipError_t run(hipStream_t s, const XentCall &c, const Plan &p, char *m) {
     k.w_groups = p.w_groups;
     k.hg_groups = p.hg_groups;
     k.few = p.w_groups <= FEW_GROUPS && p.hg_groups <= FEW_GROUPS && p.ld <= FEW_COLUMNS;
-    k.w_part = reinterpret_cast<uint32_t *>(m + p.w_part);
-    k.hg_part = reinterpret_cast<uint32_t *>(m + p.hg_part);
+    k.w_part = reinterpret_cast<int32_t *>(m + p.w_part);
+    k.hg_part = reinterpret_cast<int32_t *>(m + p.hg_part);
     k.w_exp = reinterpret_cast<int32_t *>(m + p.w_exp);
     k.hg_exp = reinterpret_cast<int32_t *>(m + p.hg_exp);
     k.h = reinterpret_cast<u16 *>(m + p.h);

@@ -93,7 +93,7 @@ struct XentPack {
     int32_t pack_w_groups, pack_h_groups;
     bool few;                            // groups: those that pack sum them up
     XentCtl *ctl;
-    uint32_t *w_part, *hg_part;          // [group][ld] bits of the largest of a column
+    int32_t *w_part, *hg_part;           // [group][ld] a column's largest exponent
     int32_t *w_exp, *hg_exp;             // [ld] a column is packed times 2^this
     u16 *h, *hg, *w;                     // planes of n_pad * ld, v_pad * ld; hg: gradients only
     float *bias;                         // [v_pad] the bias, -inf: not offered

@@ -230,3 +230,26 @@ def test_columns_of_zeros_and_of_one_side(ctx, kind, n, d):
     x = D.Xent(ctx, h, np.zeros_like(w), y, kind)
     x.grad()
     D.check(x.results(), D.xent_reference(h, np.zeros_like(w), y, kind))
+
+
+@KINDS
+@FORMS
+def test_weight_times_h_past_f32(ctx, kind, n, d):
+    """Where the gradient is small the product with h is not: rows that are nearly certain."""
+    _, h, w, y = _problem(n + d + 47, n, d, 80)
+    y = np.argmax(h @ w.T, 1).astype(np.int32)
+    big = np.arange(n) % 4 == 0
+    h[big] *= np.float32(16)
+    h = (h * np.float32(2.0 ** 60)).astype(np.float32)
+    w = (w * np.float32(2.0 ** -60)).astype(np.float32)
+    weights = np.where(big, 1e20, 1e10).astype(np.float32)
+    assert (np.abs(h.astype(np.float64)).max(1) * weights)[big].max() > 1e39
+    x = D.Xent(ctx, h, w, y, kind, weights=weights)
+    x.grad()
+    got, want = x.results(), D.xent_reference(h, w, y, kind, weights=weights)
+    for name in ("dh", "dw", "db"):
+        value, tol = want[name]
+        fits = np.abs(value) + tol < 3e38
+        assert fits.mean() > 0.9
+        off = np.abs(got[name].astype(np.float64) - value)
+        assert np.all(off[fits] <= tol[fits]), name
