@@ -274,7 +274,6 @@ __device__ __forceinline__ void pack_w(const XentPack &k, const void *w, int64_t
 // W packed, and by the workgroups behind those, the rows: label and weight (-1 and 0 where
 // the row is out) and h.  A row that is out and whose scores may not be finite is packed as
 // zeros, its label -2.
-constexpr int FAR_ROW = -100;            // scores of up to 2^(13 - this)
 template <typename T>
 __global__ __launch_bounds__(64 * MAX_WAVES) void k_xent_pack(XentPack k, XentCall c) {
     __shared__ int32_t exps[FEW_COLUMNS];

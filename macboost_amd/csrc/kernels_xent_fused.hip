@@ -238,7 +238,6 @@ __device__ __forceinline__ int column_exp(const int32_t *col, int32_t *words) {
 
 // The packed rows of W and then of h.  A row that is out and whose scores may not be finite
 // is packed as zeros, its label -2.
-constexpr int FAR_ROW = -100;            // scores of up to 2^(13 - this)
 constexpr int ZERO_ROW = 1 << 20;        // of exp: nothing but zeros
 template <typename T, int LD>
 __global__ __launch_bounds__(256) void k_fused_pack(Fused k, XentCall c) {
@@ -550,10 +549,11 @@ __global__ __launch_bounds__(256, 2) void k_fused_rows(Fused k, int32_t splits,
                 s[r] = __builtin_fmaf(s[r], sc, b[r]);
                 m = fmaxf(m, s[r]);
             }
-            // a new maximum: what was summed so far is brought to it
+            // a new maximum: what was summed so far is brought to it, of the rows that have
+            // one, so that no row's bits depend on another's
             if (__any(m > top + LAG)) {
-                const float now = fmaxf(top, fmaxf(m, other_half(m)));
-                if (now > top) {
+                const float now = fmaxf(m, other_half(m));
+                if (now > top + LAG) {
                     const float scale = top == -INFINITY ? 0.0f : exp_of(top - now);
                     sum *= scale;
                     if constexpr (GRAD)
@@ -567,13 +567,16 @@ __global__ __launch_bounds__(256, 2) void k_fused_rows(Fused k, int32_t splits,
                 far = __any(fabsf(ref) >= FAR);
             }
             float p[2][8], part[2] = {0.0f, 0.0f};
-            if (far)
+            if (far) {
+                const bool mine = fabsf(ref) >= FAR;
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
-                    s[r] = __builtin_fmaf(s[r] - ref, LOG2E, (float)P_EXP);
-            else
+                    s[r] = mine ? __builtin_fmaf(s[r] - ref, LOG2E, (float)P_EXP)
+                                : __builtin_fmaf(s[r], LOG2E, c2);
+            } else {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], LOG2E, c2);
+            }
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 p[r >> 3][r & 7] = __builtin_amdgcn_exp2f(s[r]);
@@ -744,10 +747,13 @@ __global__ __launch_bounds__(256, 2) void k_fused_classes_pass(Fused k, int32_t 
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], of2[r], b);
             if (far) {
-                of_rows(k.ref + t * TY, y, of);
+                float ref[16];
+                of_rows(k.ref + t * TY, y, ref);
                 of_rows(k.l2 + t * TY, y, of2);
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r] - of[r], LOG2E, -of2[r]);
+                for (int r = 0; r < 16; ++r)
+                    s[r] = fabsf(ref[r]) >= FAR ? __builtin_fmaf(s[r] - ref[r], LOG2E, -of2[r])
+                                                : __builtin_fmaf(s[r], LOG2E, of[r]);
             } else {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], LOG2E, of[r]);

@@ -22,6 +22,8 @@ constexpr float LOG2E = 1.44269504088896341f;
 // Values beyond this (2^60) in a row that is out count as not finite: times a finite W they
 // could still overflow.
 constexpr uint32_t XENT_HUGE = 0x5D800000u;
+// So does the whole row where its power of two is below 2^this: its scores may pass 2^100.
+constexpr int FAR_ROW = -100;
 
 // ---- control words -----------------------------------------------------------
 // A maximum over the workgroups of a kernel: each leaves its own, and those of a later one

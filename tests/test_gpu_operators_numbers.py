@@ -253,3 +253,27 @@ def test_weight_times_h_past_f32(ctx, kind, n, d):
         assert fits.mean() > 0.9
         off = np.abs(got[name].astype(np.float64) - value)
         assert np.all(off[fits] <= tol[fits]), name
+
+
+@KINDS
+@FORMS
+def test_what_is_out_changes_no_bit(ctx, kind, n, d):
+    """Neither its values nor its size: no other row, class or column notices."""
+    _, h, w, y = _problem(n + d + 48, n, d, 90)
+    bias = np.zeros(90, np.float32)
+    closed = np.arange(90) % 6 == 0
+    bias[closed] = -np.inf
+    y = (y // 6 * 6 + 1).astype(np.int32)
+    weights = np.ones(n, np.float32)
+    y[3], y[4], weights[5] = -1, 90, 0
+    out = np.isin(np.arange(n), (3, 4, 5))
+    runs = []
+    for rows, classes in ((0.0, 0.0), (1e-6, 1e6), (1e15, 1e-20), (3e38, 3e38), (np.nan, np.inf)):
+        h[out], w[closed] = rows, classes
+        x = D.Xent(ctx, h, w, y, kind, bias, weights)
+        x.grad()
+        runs.append(x.results())
+    for r in runs:
+        assert np.array_equal(r["lse"][~out], runs[0]["lse"][~out])
+        for name in ("loss", "dh", "dw", "db"):
+            assert np.array_equal(r[name], runs[0][name]), name
