@@ -684,7 +684,7 @@ __global__ __launch_bounds__(256) void k_expert_gather_runs(ExpertPlan p, Expert
 // ---- other layouts: a tile of 64 rows x 64 columns at a time, 256 threads ----
 // XCOLS / SCOLS: the lanes of a wavefront run along the columns of the rows' matrix / of
 // the sorted matrix, else along the rows; LDS turns the tile where the two differ.  Sums of
-// 99991 x 2 blocks' rows of 37 f32: 14 us, 3.1 TB/s of its 43 MB, much of them in the L2s.
+// 99991 x 2 blocks' rows of 37 f32: 14.4 us, 3.0 TB/s of its 43 MB, much of them in the L2s.
 constexpr int TILE = 64;
 template <typename T, bool XCOLS, bool SCOLS>
 __global__ __launch_bounds__(256) void k_expert_gather(ExpertPlan p, ExpertMatrix x,
