@@ -9,7 +9,7 @@ Kinds of case:
 - ``clip``: the norm of many gradients together, and each of them scaled so that it is at most
   ``max_norm`` (``mbk_grad_clip``).
 - ``scores``: the classes' scores ``h W' + b`` with W in 4 bits and a scale for each group of
-  ``group`` elements of a class (``mbk_q4_scores``).
+  ``group`` elements of a class (``mbk_fourbit_scores``).
 - ``adjust``: scores with penalties for the classes that a row's history holds, biases, and -inf for
   classes that are not allowed (``mbk_adjust``).
 
@@ -408,10 +408,10 @@ def _describe(s):
                                   _core.F32 if g.dtype == torch.float32 else _core.BF16)
                                  for g, o in zip(s["grads"], outs)])
     elif kind == "scores":
-        s["shape"] = _core.MbkQ4Shape(case["classes"], case["dim"], case["group"])
+        s["shape"] = _core.MbkFourbitShape(case["classes"], case["dim"], case["group"])
         w = s.pop("w")
-        s["packed"] = torch.empty(_core.q4_bytes(s["shape"]), dtype=torch.uint8, device="cuda")
-        ctx.call("mbk_q4_pack", ctypes.byref(s["shape"]), _CODES[case["type"]], _ptr(w),
+        s["packed"] = torch.empty(_core.fourbit_bytes(s["shape"]), dtype=torch.uint8, device="cuda")
+        ctx.call("mbk_fourbit_pack", ctypes.byref(s["shape"]), _CODES[case["type"]], _ptr(w),
                  w.stride(0), _ptr(s["packed"]))
     else:
         mask_stride = s["allowed"].stride(0) if case["mask"] == "row" else 0
@@ -434,7 +434,7 @@ def _own_run(s):
         ctx.call("mbk_grad_clip", s["list"].ptr, s["max_norm"], _ptr(s["norm"]))
         return [s["norm"]] + list((s["buffers"] or {}).values())
     elif kind == "scores":
-        ctx.call("mbk_q4_scores", ref(s["shape"]), case["rows"], _CODES[case["type"]],
+        ctx.call("mbk_fourbit_scores", ref(s["shape"]), case["rows"], _CODES[case["type"]],
                  _ptr(s["h"]), s["h"].stride(0), _ptr(s["packed"]), _ptr(s["bias"]),
                  _ptr(s["scores"]), s["scores"].stride(0))
         return s["scores"]
