@@ -388,6 +388,105 @@ int mbk_expert_combine_grad(mbk_context *ctx, const mbk_expert_plan *plan,
                             const mbk_expert_matrix *dout, const void *sorted,
                             const float *weights, void *d_sorted, float *d_weights, char **err);
 
+/* ---- category vectors.  No counterpart in the reference.  A column of many categories gives
+ * each row's outputs a vector of its category's, trained by gradient beside the forests.  All
+ * arrays are device memory.
+ * mbk_embed: out[row] = base[row] + scale * table[ids[row]]; an id outside [0, entries) adds
+ * nothing.  base (NULL: 0) lies as out does and may be out itself.
+ * mbk_embed_grad: dtable[v] = base[v] + scale * the sum of dout[row] over the rows with
+ * ids[row] = v.  base (NULL: 0) lies as dtable does.  If it is dtable itself, entries without
+ * rows are neither read nor written; else every entry is written.  What dout holds of rows whose
+ * id is outside reaches nothing.
+ * Sums are f32, in runs of at most 128 rows and then over the runs, rounded once with
+ * base; their order is fixed by the shape, the ids and the number of compute units.  What lies
+ * between rows of out and dtable stays as it is; outputs overlap no input but base. */
+typedef struct {
+    int64_t rows;                /* 0..2^31-256 */
+    int64_t entries;             /* 1..2^31-256 */
+    int32_t dim;                 /* 1..2^20 */
+    int32_t type;                /* of table, base, out, dout, dtable: MBK_F32 or MBK_BF16 */
+    int64_t row_stride;          /* elements from row to row of out (base) or dout, dim..2^40 */
+    int64_t table_stride;        /* of table or dtable (base) */
+    float scale;                 /* finite */
+} mbk_embed_shape;
+int mbk_embed(mbk_context *ctx, const mbk_embed_shape *shape, const void *table,
+              const int32_t *ids, const void *base, void *out, char **err);
+int mbk_embed_grad(mbk_context *ctx, const mbk_embed_shape *shape, const int32_t *ids,
+                   const void *dout, const void *base, void *dtable, char **err);
+
+/* ---- the norm of many gradients together.  No counterpart in the reference.
+ * mbk_tensors_create lists the gradients (device memory; the list itself is host memory, read
+ * within the call, which waits for the context's stream).  The list belongs to the context:
+ * mbk_tensors_destroy gives it back (after the stream's work; while the stream is captured, and
+ * for a list that a captured call has used, its memory stays until the context is destroyed), and
+ * so does mbk_context_destroy.
+ * mbk_grad_clip: norm[0] (device) = the root of the sum of all squares, and every out = grad *
+ * min(1, max_norm / norm).  A sum of squares that is not finite leaves out = grad: the norm
+ * tells.  A norm beyond f32 is +INFINITY, but clips.  max_norm may be INFINITY (outs are
+ * copies then).  Sums of squares and the factor are f64, an element's product is rounded to f32
+ * and from there to its type; the order of the sums is fixed by the list and the number of
+ * compute units. */
+typedef struct {
+    const void *grad;            /* rows rows of cols elements, stride elements apart */
+    void *out;                   /* lies as grad does and may be grad itself; NULL: none */
+    int64_t rows, cols;          /* >= 0; all together at most 2^38 elements */
+    int64_t stride;              /* cols..2^40 */
+    int32_t type;                /* MBK_F32 or MBK_BF16 */
+} mbk_tensor;
+typedef struct mbk_tensors mbk_tensors;
+int mbk_tensors_create(mbk_context *ctx, const mbk_tensor *list, int32_t count, mbk_tensors **out,
+                       char **err);
+void mbk_tensors_destroy(mbk_context *ctx, mbk_tensors *list);
+int mbk_grad_clip(mbk_context *ctx, mbk_tensors *list, float max_norm, float *norm, char **err);
+
+/* ---- scores of many classes with class vectors in 4 bits.  No counterpart in the reference.
+ * A group of `group` elements of a class (the last may be shorter) has the scale
+ * bf16(max |w| * f32(1/7)), and an element the code nearest to w / scale (f32 division, ties to
+ * even) in -8..7, 0 where the scale is 0; the element is code * scale.
+ * mbk_fourbit_pack lays w (device, [classes] rows of dim elements, stride apart) out so, in
+ * mbk_fourbit_bytes(shape) bytes at an address that is a multiple of 16 (device; the layout is the
+ * library's own).  mbk_fourbit_bytes is -1 for a shape that the calls refuse.
+ * mbk_fourbit_scores: scores[row][v] = h[row] . w[v] + bias[v] (bias NULL: 0), f32; a class whose bias
+ * is -INFINITY has that score whatever its w and h hold.
+ * Elements of w are taken as they are, but for what is below 2^-28 of its class's largest scale,
+ * off by up to 2^-36 of that scale; bf16 h as it is, but for what is below 2^-29 of its row's
+ * largest, off by up to 2^-39 of that; f32 h with 22 bits, and beside the row's largest off by up
+ * to 2^-49 of it.  Sums are f32, rounded with the bias once more.  A class whose w is not finite
+ * has scores that are NaN, a row whose h is not finite has scores that are not finite. */
+typedef struct {
+    int64_t classes;             /* 1..2^31-256 */
+    int32_t dim;                 /* 1..2^20 */
+    int32_t group;               /* 32, 64 or 128 */
+} mbk_fourbit_shape;
+int64_t mbk_fourbit_bytes(const mbk_fourbit_shape *shape);
+int mbk_fourbit_pack(mbk_context *ctx, const mbk_fourbit_shape *shape, int32_t type, const void *w,
+                int64_t w_stride, void *packed, char **err);
+int mbk_fourbit_scores(mbk_context *ctx, const mbk_fourbit_shape *shape, int64_t rows, int32_t type,
+                  const void *h, int64_t h_stride, const void *packed, const float *bias,
+                  float *scores, int64_t score_stride, char **err);
+
+/* ---- penalties, biases and masks of scores.  No counterpart in the reference.  All arrays are
+ * device memory.  With c the times that class v is among the row's first lengths[row] ids of
+ * history (lengths NULL: all; less than 0 counts as 0, more than history as history; ids outside
+ * [0, classes) count nowhere):
+ *   z = scores[row][v]
+ *   c > 0:  z = (z > 0 ? z / repetition : z * repetition) - (presence + frequency * c)
+ *   out[row][v] = z + bias[v], or -INFINITY if bit v % 32 of the row's mask word v / 32 is 0,
+ * whatever z is.  ids (history 0), bias and allowed may be NULL: none of it.  out may be
+ * scores itself, with the same stride; what lies between its rows stays as it is. */
+typedef struct {
+    int64_t rows, classes;       /* rows 0..2^31-256, classes 1..2^31-256, together below 2^40 */
+    int64_t score_stride, out_stride;    /* elements from row to row, classes..2^40 */
+    int32_t history;             /* ids a row: 0..2^24 */
+    int64_t history_stride;      /* history..2^40 */
+    int64_t mask_stride;         /* 32-bit words from row to row of allowed, 0: one mask for all */
+    float repetition;            /* positive and finite */
+    float presence, frequency;   /* finite */
+} mbk_adjust_shape;
+int mbk_adjust(mbk_context *ctx, const mbk_adjust_shape *shape, const float *scores,
+               const int32_t *ids, const int32_t *lengths, const float *bias,
+               const uint32_t *allowed, float *out, char **err);
+
 /* fitImpl (Booster.swift:445-1701) over raw features already in device
  * memory: x is read as x[i*cols + f] when row_major != 0, else x[f*rows + i];
  * y, w (nullable) and the feature-major validation set (nullable) are host

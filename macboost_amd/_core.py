@@ -85,7 +85,38 @@ class MbkExpertMatrix(ctypes.Structure):
                 ("cols", ctypes.c_int32), ("type", ctypes.c_int32), ("blocked", ctypes.c_int32)]
 
 
+class MbkEmbedShape(ctypes.Structure):
+    """mbk_embed_shape (include/macboost.h)."""
+    _fields_ = [("rows", ctypes.c_int64), ("entries", ctypes.c_int64), ("dim", ctypes.c_int32),
+                ("type", ctypes.c_int32), ("row_stride", ctypes.c_int64),
+                ("table_stride", ctypes.c_int64), ("scale", ctypes.c_float)]
+
+
+class MbkTensor(ctypes.Structure):
+    """mbk_tensor: a gradient in device memory and where its scaled form goes."""
+    _fields_ = [("grad", _P), ("out", _P), ("rows", ctypes.c_int64), ("cols", ctypes.c_int64),
+                ("stride", ctypes.c_int64), ("type", ctypes.c_int32)]
+
+
+class MbkFourbitShape(ctypes.Structure):
+    """mbk_fourbit_shape (include/macboost.h)."""
+    _fields_ = [("classes", ctypes.c_int64), ("dim", ctypes.c_int32), ("group", ctypes.c_int32)]
+
+
+class MbkAdjustShape(ctypes.Structure):
+    """mbk_adjust_shape (include/macboost.h)."""
+    _fields_ = [("rows", ctypes.c_int64), ("classes", ctypes.c_int64),
+                ("score_stride", ctypes.c_int64), ("out_stride", ctypes.c_int64),
+                ("history", ctypes.c_int32), ("history_stride", ctypes.c_int64),
+                ("mask_stride", ctypes.c_int64), ("repetition", ctypes.c_float),
+                ("presence", ctypes.c_float), ("frequency", ctypes.c_float)]
+
+
 F32, BF16 = 0, 1         # MBK_F32, MBK_BF16
+_EMBED_P = ctypes.POINTER(MbkEmbedShape)
+_TENSOR_P = ctypes.POINTER(MbkTensor)
+_FOURBIT_P = ctypes.POINTER(MbkFourbitShape)
+_ADJUST_P = ctypes.POINTER(MbkAdjustShape)
 _XENT_P = ctypes.POINTER(MbkXentShape)
 _PLAN_P = ctypes.POINTER(MbkExpertPlan)
 _MATRIX_P = ctypes.POINTER(MbkExpertMatrix)
@@ -180,9 +211,22 @@ def _configure(l):
             ("mbk_expert_sort", [_P, _PLAN_P, _c_char_pp]),
             ("mbk_expert_gather", [_P, _PLAN_P, _MATRIX_P, _P, _c_char_pp]),
             ("mbk_expert_combine", [_P, _PLAN_P, _P, _P, _MATRIX_P, _c_char_pp]),
-            ("mbk_expert_combine_grad", [_P, _PLAN_P, _MATRIX_P, _P, _P, _P, _P, _c_char_pp])):
+            ("mbk_expert_combine_grad", [_P, _PLAN_P, _MATRIX_P, _P, _P, _P, _P, _c_char_pp]),
+            ("mbk_embed", [_P, _EMBED_P, _P, _P, _P, _P, _c_char_pp]),
+            ("mbk_embed_grad", [_P, _EMBED_P, _P, _P, _P, _P, _c_char_pp]),
+            ("mbk_tensors_create", [_P, _TENSOR_P, ctypes.c_int32, ctypes.POINTER(_P),
+                                    _c_char_pp]),
+            ("mbk_grad_clip", [_P, _P, ctypes.c_float, _P, _c_char_pp]),
+            ("mbk_fourbit_pack", [_P, _FOURBIT_P, ctypes.c_int32, _P, ctypes.c_int64, _P, _c_char_pp]),
+            ("mbk_fourbit_scores", [_P, _FOURBIT_P, ctypes.c_int64, ctypes.c_int32, _P, ctypes.c_int64, _P,
+                               _P, _P, ctypes.c_int64, _c_char_pp]),
+            ("mbk_adjust", [_P, _ADJUST_P, _P, _P, _P, _P, _P, _P, _c_char_pp])):
         getattr(l, name).restype = ctypes.c_int
         getattr(l, name).argtypes = args
+    l.mbk_tensors_destroy.restype = None
+    l.mbk_tensors_destroy.argtypes = [_P, _P]
+    l.mbk_fourbit_bytes.restype = ctypes.c_int64
+    l.mbk_fourbit_bytes.argtypes = [_FOURBIT_P]
     l.mbk_fit.restype = ctypes.c_void_p
     l.mbk_fit.argtypes = [_P, ctypes.c_char_p, _P, ctypes.c_int64, ctypes.c_int64,
                           ctypes.c_int32, _f32_p, _f32_p, _f32_p, ctypes.c_int64, _f32_p,
@@ -263,7 +307,9 @@ EXPORTED = (
     "mbk_node_hist_split", "mbk_predict_forest", "mbk_fit", "mbk_tree_begin", "mbk_hist_build",
     "mbk_hist_subtract", "mbk_find_splits", "mbk_decide_level", "mbk_route", "mbk_final_leaves",
     "mbk_xent", "mbk_xent_grad", "mbk_expert_sort", "mbk_expert_gather", "mbk_expert_combine",
-    "mbk_expert_combine_grad", "mbk_grow_tree", "mbk_treeshap", "mbk_node_hist_split_noalloc",
+    "mbk_expert_combine_grad", "mbk_embed", "mbk_embed_grad", "mbk_tensors_create",
+    "mbk_tensors_destroy", "mbk_grad_clip", "mbk_fourbit_bytes", "mbk_fourbit_pack", "mbk_fourbit_scores",
+    "mbk_adjust", "mbk_grow_tree", "mbk_treeshap", "mbk_node_hist_split_noalloc",
     "mbx_trainer_create", "mbx_trainer_grow", "mbx_trainer_profile", "mbx_trainer_hist_stats",
     "mbx_trainer_level_stats", "mbx_trainer_setup_seconds", "mbx_trainer_booster", "mbx_trainer_free", "mbx_friedman",
     "mbx_version", "mbx_dataset_make", "mbx_dataset_save", "mbx_dataset_load",
@@ -638,6 +684,11 @@ class Context:
         err = ctypes.c_char_p()
         self._check(getattr(lib(), name)(self.ptr, *args, ctypes.byref(err)), err)
 
+    def tensors(self, gradients) -> "Tensors":
+        """The list of gradients that mbk_grad_clip takes as one (mbk_tensors_create): tuples
+        (gradient, output or None, rows, cols, stride, F32 or BF16) with device pointers."""
+        return Tensors(self, gradients)
+
     def profile(self, enable: bool = True, every: int = 1) -> None:
         """HIP-event timing of the histogram launches of every every-th tree
         of later fits (enable=False stops it)."""
@@ -672,6 +723,32 @@ class Context:
 
     def __del__(self):
         self.close()
+
+
+class Tensors:
+    """A list of gradients of a context (mbk_tensors): .ptr goes to mbk_grad_clip."""
+
+    def __init__(self, ctx: Context, gradients):
+        self.ctx, self.ptr = ctx, _P()
+        items = [MbkTensor(*g) for g in gradients]
+        ctx.call("mbk_tensors_create", (MbkTensor * max(1, len(items)))(*items), len(items),
+                 ctypes.byref(self.ptr))
+
+    def close(self):
+        if self.ptr.value and self.ctx.ptr.value and _lib_instance is not None:
+            _lib_instance.mbk_tensors_destroy(self.ctx.ptr, self.ptr)
+        self.ptr = _P()
+
+    def __del__(self):
+        self.close()
+
+
+def fourbit_bytes(shape: MbkFourbitShape) -> int:
+    """Bytes of W in 4 bits (mbk_fourbit_bytes)."""
+    n = lib().mbk_fourbit_bytes(ctypes.byref(shape))
+    if n < 0:
+        raise MacBoostError("Invalid input: mbk_fourbit_shape")
+    return n
 
 
 class Dataset:

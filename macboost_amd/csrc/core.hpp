@@ -16,8 +16,10 @@
 #include <rocprofiler-sdk-roctx/roctx.h>
 
 #include "mbk.h"
+#include "ops.h"
 
 struct mbk_context;
+struct mbk_tensors;
 
 namespace mb {
 
@@ -30,6 +32,9 @@ int context_cus(const mbk_context *ctx);
 // until the context ends, and growing under capture is refused.
 char *context_scratch(mbk_context *ctx, size_t bytes);
 std::mutex &context_scratch_mutex(mbk_context *ctx);     // held while a call queues its work
+bool context_captured(const mbk_context *ctx);           // its stream is being captured
+// The context's lists of gradients (mbk_tensors), which end with it.
+std::vector<std::unique_ptr<mbk_tensors>> &context_lists(mbk_context *ctx);
 
 // A named range on the ROCm tracer's marker timeline (rocprofv3
 // --marker-trace) around one phase of host work; free when no tool listens.
@@ -405,3 +410,12 @@ std::string swift_float(float v);
 int host_threads();
 
 }  // namespace mb
+
+// A list of gradients (mbk_tensors_create) in pieces.
+struct mbk_tensors {
+    mb::DevBuf<mbk::ClipPiece> piece;
+    int64_t pieces = 0;
+    bool outputs = false;
+    bool captured = false;           // a captured graph may use it
+    bool gone = false;               // given back, but captured
+};

@@ -1,8 +1,14 @@
 // ops.cpp — the seam's operators beside the tree build: the loss over many classes
-// (mbk_xent, mbk_xent_grad) and rows sorted by expert (mbk_expert_*).  Each call
+// (mbk_xent, mbk_xent_grad), rows sorted by expert (mbk_expert_*), category vectors
+// (mbk_embed*), the norm of gradients (mbk_tensors_*, mbk_grad_clip), scores from class vectors
+// in 4 bits (mbk_fourbit_*) and their penalties (mbk_adjust).  Each call
 // checks its arguments (the context last), queues its kernels on the context's stream and
 // returns; it allocates only when it needs more scratch than the context holds.  Calls that
 // use scratch are queued whole, one after another, whichever threads make them.
+#include <algorithm>
+#include <cmath>
+#include <vector>
+
 #include "../../include/macboost.h"
 #include "abi.hpp"
 #include "core.hpp"
@@ -17,6 +23,7 @@ void need(bool ok, const char *what) {
 constexpr int64_t MOST_ROWS = 0x7FFFFF00;
 constexpr int32_t MOST_EXPERTS = 8192;       // counters of four wavefronts in LDS
 constexpr int64_t MOST_STRIDE = (int64_t)1 << 40;
+constexpr int64_t MOST_ELEMENTS = (int64_t)1 << 38;
 
 bool is_bf16(int32_t type) {
     need(type == MBK_F32 || type == MBK_BF16, "type must be MBK_F32 or MBK_BF16");
@@ -81,6 +88,67 @@ mbk::ExpertMatrix expert_matrix(const mbk_expert_matrix *m, int64_t rows) {
              ((m->cols - 1) <= (rs - 1) / cs || rows - 1 <= (cs - 1) / rs),
          "row_stride and col_stride must be in 1..2^40 and keep the elements apart");
     return {m->data, m->row_stride, m->col_stride, m->cols, is_bf16(m->type), m->blocked != 0};
+}
+
+mbk::EmbedCall embed_call(const mbk_embed_shape *sh, const int32_t *ids, const void *base) {
+    need(sh != nullptr, "null shape");
+    need(sh->rows >= 0 && sh->rows <= MOST_ROWS, "rows must be in 0..2^31-256");
+    need(sh->entries >= 1 && sh->entries <= MOST_ROWS, "entries must be in 1..2^31-256");
+    need(sh->dim >= 1 && sh->dim <= (1 << 20), "dim must be in 1..2^20");
+    need(sh->row_stride >= sh->dim && sh->table_stride >= sh->dim &&
+             sh->row_stride <= MOST_STRIDE && sh->table_stride <= MOST_STRIDE,
+         "row_stride and table_stride must be in dim..2^40");
+    need(std::isfinite(sh->scale), "scale must be finite");
+    mbk::EmbedCall c{};
+    c.rows = sh->rows;
+    c.entries = sh->entries;
+    c.dim = sh->dim;
+    c.bf16 = is_bf16(sh->type);
+    c.row_stride = sh->row_stride;
+    c.table_stride = sh->table_stride;
+    c.scale = sh->scale;
+    c.ids = ids;
+    c.base = base;
+    return c;
+}
+
+// The pieces of one gradient of the list: short rows together, long ones and gradients without
+// gaps in runs.
+void add_pieces(const mbk_tensor &t, std::vector<mbk::ClipPiece> &out) {
+    const bool bf16 = t.type == MBK_BF16;
+    const int64_t size = bf16 ? 2 : 4, most = mbk::CLIP_PIECE;
+    const auto add = [&](int64_t at, int64_t rows, int64_t cols) {
+        const char *g = static_cast<const char *>(t.grad) + at * size;
+        char *o = t.out ? static_cast<char *>(t.out) + at * size : nullptr;
+        const bool wide = reinterpret_cast<uintptr_t>(g) % 16 == 0 &&
+                          reinterpret_cast<uintptr_t>(o) % 16 == 0 &&
+                          (rows == 1 || t.stride * size % 16 == 0);
+        out.push_back({g, o, t.stride, (int32_t)rows, (int32_t)cols, bf16, wide});
+    };
+    if (!t.rows || !t.cols) return;
+    const bool whole = t.rows == 1 || t.stride == t.cols;
+    const int64_t rows = whole ? 1 : t.rows, cols = whole ? t.rows * t.cols : t.cols;
+    if (cols >= most || whole) {
+        for (int64_t r = 0; r < rows; ++r)
+            for (int64_t c = 0; c < cols; c += most)
+                add(r * t.stride + c, 1, std::min(most, cols - c));
+        return;
+    }
+    const int64_t each = most / cols;
+    for (int64_t r = 0; r < rows; r += each) add(r * t.stride, std::min(each, rows - r), cols);
+}
+
+mbk::FourbitShape fourbit_shape(const mbk_fourbit_shape *sh) {
+    need(sh != nullptr, "null shape");
+    need(sh->classes >= 1 && sh->classes <= MOST_ROWS, "classes must be in 1..2^31-256");
+    need(sh->dim >= 1 && sh->dim <= (1 << 20), "dim must be in 1..2^20");
+    need(sh->group == 32 || sh->group == 64 || sh->group == 128, "group must be 32, 64 or 128");
+    return mbk::fourbit_shape(sh->classes, sh->dim, sh->group);
+}
+
+void need_packed(const void *packed) {
+    need(packed != nullptr, "null argument");
+    need(reinterpret_cast<uintptr_t>(packed) % 16 == 0, "packed must be a multiple of 16 bytes");
 }
 
 }  // namespace
@@ -163,6 +231,229 @@ int mbk_expert_combine_grad(mbk_context *ctx, const mbk_expert_plan *plan,
         mb::OnDevice here(mb::context_device(ctx));
         MB_HIP(mbk::launch_expert_combine_grad(mb::context_stream(ctx), p, m, sorted, weights,
                                                d_sorted, d_weights));
+        return 0;
+    }, -1);
+}
+
+int mbk_embed(mbk_context *ctx, const mbk_embed_shape *shape, const void *table,
+              const int32_t *ids, const void *base, void *out, char **err) {
+    return mb::guarded(err, [&]() -> int {
+        mbk::EmbedCall c = embed_call(shape, ids, base);
+        need(table && (!c.rows || (ids && out)), "null argument");
+        need(ctx != nullptr, "null kernel-seam context");
+        if (!c.rows) return 0;
+        c.table = table;
+        c.out = out;
+        mb::OnDevice here(mb::context_device(ctx));
+        MB_HIP(mbk::launch_embed(mb::context_stream(ctx), c));
+        return 0;
+    }, -1);
+}
+
+int mbk_embed_grad(mbk_context *ctx, const mbk_embed_shape *shape, const int32_t *ids,
+                   const void *dout, const void *base, void *dtable, char **err) {
+    return mb::guarded(err, [&]() -> int {
+        mbk::EmbedCall c = embed_call(shape, ids, base);
+        need(dtable && (!c.rows || (ids && dout)), "null argument");
+        need(ctx != nullptr, "null kernel-seam context");
+        if (!c.rows && base == dtable) return 0;
+        c.dout = dout;
+        c.dtable = dtable;
+        c.num_cus = mb::context_cus(ctx);
+        mb::OnDevice here(mb::context_device(ctx));
+        std::lock_guard<std::mutex> lock(mb::context_scratch_mutex(ctx));
+        char *scratch = mb::context_scratch(ctx, mbk::embed_grad_scratch(c));
+        MB_HIP(mbk::launch_embed_grad(mb::context_stream(ctx), c, scratch));
+        return 0;
+    }, -1);
+}
+
+int mbk_tensors_create(mbk_context *ctx, const mbk_tensor *list, int32_t count, mbk_tensors **out,
+                       char **err) {
+    return mb::guarded(err, [&]() -> int {
+        need(count >= 0 && count <= (1 << 24), "count must be in 0..2^24");
+        need(out && (!count || list), "null argument");
+        int64_t elements = 0;
+        for (int32_t i = 0; i < count; ++i) {
+            const mbk_tensor &t = list[i];
+            (void)is_bf16(t.type);
+            need(t.rows >= 0 && t.cols >= 0 && t.rows <= MOST_ELEMENTS && t.cols <= MOST_ELEMENTS,
+                 "rows and cols must be in 0..2^38");
+            need(t.stride >= t.cols && t.stride <= MOST_STRIDE, "stride must be in cols..2^40");
+            need(!t.cols || t.rows <= (MOST_ELEMENTS - elements) / t.cols,
+                 "gradients must have at most 2^38 elements together");
+            elements += t.rows * t.cols;
+            need(t.grad || !t.rows || !t.cols, "null gradient");
+        }
+        std::vector<mbk::ClipPiece> pieces;
+        auto made = std::make_unique<mbk_tensors>();
+        for (int32_t i = 0; i < count; ++i) {
+            add_pieces(list[i], pieces);
+            made->outputs |= list[i].out != nullptr;
+        }
+        need(ctx != nullptr, "null kernel-seam context");
+        need(!mb::context_captured(ctx), "the context's stream is being captured");
+        mb::OnDevice here(mb::context_device(ctx));
+        made->pieces = (int64_t)pieces.size();
+        made->piece.alloc(pieces.size());
+        hipStream_t s = mb::context_stream(ctx);
+        if (!pieces.empty())
+            MB_HIP(hipMemcpyAsync(made->piece.ptr, pieces.data(),
+                                  pieces.size() * sizeof(mbk::ClipPiece), hipMemcpyHostToDevice, s));
+        MB_HIP(hipStreamSynchronize(s));
+        std::lock_guard<std::mutex> lock(mb::context_scratch_mutex(ctx));
+        mb::context_lists(ctx).push_back(std::move(made));
+        *out = mb::context_lists(ctx).back().get();
+        return 0;
+    }, -1);
+}
+
+void mbk_tensors_destroy(mbk_context *ctx, mbk_tensors *list) {
+    (void)mb::guarded(nullptr, [&]() -> int {
+        if (!ctx || !list) return 0;
+        mb::OnDevice here(mb::context_device(ctx));
+        std::lock_guard<std::mutex> lock(mb::context_scratch_mutex(ctx));
+        auto &lists = mb::context_lists(ctx);
+        const auto at = std::find_if(lists.begin(), lists.end(),
+                                     [&](const auto &l) { return l.get() == list; });
+        if (at == lists.end()) return 0;
+        // what a graph has captured must stay, and a wait would end the capture
+        list->gone = true;
+        if (list->captured || mb::context_captured(ctx)) return 0;
+        (void)hipStreamSynchronize(mb::context_stream(ctx));
+        lists.erase(at);
+        return 0;
+    }, -1);
+}
+
+int mbk_grad_clip(mbk_context *ctx, mbk_tensors *list, float max_norm, float *norm, char **err) {
+    return mb::guarded(err, [&]() -> int {
+        need(max_norm >= 0.0f, "max_norm must be >= 0");
+        need(list && norm, "null argument");
+        need(ctx != nullptr, "null kernel-seam context");
+        std::lock_guard<std::mutex> lock(mb::context_scratch_mutex(ctx));
+        const auto &lists = mb::context_lists(ctx);
+        need(std::any_of(lists.begin(), lists.end(),
+                         [&](const auto &l) { return l.get() == list && !l->gone; }),
+             "the list is not one of the context's");
+        mb::OnDevice here(mb::context_device(ctx));
+        const int cus = mb::context_cus(ctx);
+        char *scratch = mb::context_scratch(ctx, mbk::clip_scratch(list->pieces, cus));
+        list->captured |= mb::context_captured(ctx);
+        MB_HIP(mbk::launch_clip(mb::context_stream(ctx),
+                                {list->piece.ptr, list->pieces, list->outputs, max_norm, norm, cus},
+                                scratch));
+        return 0;
+    }, -1);
+}
+
+int64_t mbk_fourbit_bytes(const mbk_fourbit_shape *shape) {
+    return mb::guarded(nullptr, [&]() -> int64_t { return (int64_t)mbk::fourbit_bytes(fourbit_shape(shape)); },
+                       -1);
+}
+
+int mbk_fourbit_pack(mbk_context *ctx, const mbk_fourbit_shape *shape, int32_t type, const void *w,
+                int64_t w_stride, void *packed, char **err) {
+    return mb::guarded(err, [&]() -> int {
+        const mbk::FourbitShape s = fourbit_shape(shape);
+        need(w_stride >= s.dim && w_stride <= MOST_STRIDE, "w_stride must be in dim..2^40");
+        const bool bf16 = is_bf16(type);
+        need(w != nullptr, "null argument");
+        need_packed(packed);
+        need(ctx != nullptr, "null kernel-seam context");
+        mb::OnDevice here(mb::context_device(ctx));
+        MB_HIP(mbk::launch_fourbit_pack(mb::context_stream(ctx), s, bf16, w, w_stride,
+                                   static_cast<char *>(packed)));
+        return 0;
+    }, -1);
+}
+
+int mbk_fourbit_scores(mbk_context *ctx, const mbk_fourbit_shape *shape, int64_t rows, int32_t type,
+                  const void *h, int64_t h_stride, const void *packed, const float *bias,
+                  float *scores, int64_t score_stride, char **err) {
+    return mb::guarded(err, [&]() -> int {
+        mbk::FourbitCall c{};
+        c.shape = fourbit_shape(shape);
+        need(rows >= 0 && rows <= MOST_ROWS, "rows must be in 0..2^31-256");
+        need(h_stride >= c.shape.dim && h_stride <= MOST_STRIDE, "h_stride must be in dim..2^40");
+        need(score_stride >= c.shape.classes && score_stride <= MOST_STRIDE,
+             "score_stride must be in classes..2^40");
+        c.bf16 = is_bf16(type);
+        need(!rows || (h && scores), "null argument");
+        need_packed(packed);
+        need(ctx != nullptr, "null kernel-seam context");
+        if (!rows) return 0;
+        uint32_t *codes;
+        _Float16 *scales;
+        int32_t *exponents;
+        mbk::fourbit_parts(c.shape, static_cast<char *>(const_cast<void *>(packed)), &codes, &scales,
+                      &exponents);
+        c.rows = rows;
+        c.h = h;
+        c.h_stride = h_stride;
+        c.codes = codes;
+        c.scales = scales;
+        c.exponents = exponents;
+        c.bias = bias;
+        c.scores = scores;
+        c.score_stride = score_stride;
+        c.num_cus = mb::context_cus(ctx);
+        mb::OnDevice here(mb::context_device(ctx));
+        std::lock_guard<std::mutex> lock(mb::context_scratch_mutex(ctx));
+        char *scratch = mb::context_scratch(ctx, mbk::fourbit_scratch(c));
+        MB_HIP(mbk::launch_fourbit_scores(mb::context_stream(ctx), c, scratch));
+        return 0;
+    }, -1);
+}
+
+int mbk_adjust(mbk_context *ctx, const mbk_adjust_shape *shape, const float *scores,
+               const int32_t *ids, const int32_t *lengths, const float *bias,
+               const uint32_t *allowed, float *out, char **err) {
+    return mb::guarded(err, [&]() -> int {
+        const mbk_adjust_shape *sh = shape;
+        need(sh != nullptr, "null shape");
+        need(sh->rows >= 0 && sh->rows <= MOST_ROWS, "rows must be in 0..2^31-256");
+        need(sh->classes >= 1 && sh->classes <= MOST_ROWS, "classes must be in 1..2^31-256");
+        need(sh->rows <= MOST_STRIDE / sh->classes, "rows * classes must be at most 2^40");
+        need(sh->score_stride >= sh->classes && sh->out_stride >= sh->classes &&
+                 sh->score_stride <= MOST_STRIDE && sh->out_stride <= MOST_STRIDE,
+             "score_stride and out_stride must be in classes..2^40");
+        need(sh->history >= 0 && sh->history <= (1 << 24), "history must be in 0..2^24");
+        need(sh->history_stride >= sh->history && sh->history_stride <= MOST_STRIDE,
+             "history_stride must be in history..2^40");
+        need(sh->mask_stride == 0 || (sh->mask_stride >= (sh->classes + 31) / 32 &&
+                                      sh->mask_stride <= MOST_STRIDE),
+             "mask_stride must be 0 or in classes / 32..2^40");
+        need(sh->repetition > 0.0f && std::isfinite(sh->repetition),
+             "repetition must be positive and finite");
+        need(std::isfinite(sh->presence) && std::isfinite(sh->frequency),
+             "presence and frequency must be finite");
+        need(!sh->rows || (scores && out && (!sh->history || ids)), "null argument");
+        need(scores != out || sh->score_stride == sh->out_stride,
+             "scores that are out must have its stride");
+        need(ctx != nullptr, "null kernel-seam context");
+        if (!sh->rows) return 0;
+        mbk::AdjustCall c{};
+        c.rows = sh->rows;
+        c.classes = sh->classes;
+        c.score_stride = sh->score_stride;
+        c.out_stride = sh->out_stride;
+        c.history = sh->history;
+        c.history_stride = sh->history_stride;
+        c.mask_stride = sh->mask_stride;
+        c.repetition = sh->repetition;
+        c.presence = sh->presence;
+        c.frequency = sh->frequency;
+        c.penalties = sh->history > 0 && (sh->repetition != 1.0f || sh->presence != 0.0f ||
+                                          sh->frequency != 0.0f);
+        c.scores = scores;
+        c.ids = ids;
+        c.lengths = lengths;
+        c.bias = bias;
+        c.allowed = allowed;
+        c.out = out;
+        mb::OnDevice here(mb::context_device(ctx));
+        MB_HIP(mbk::launch_adjust(mb::context_stream(ctx), c));
         return 0;
     }, -1);
 }

@@ -1,5 +1,7 @@
-// ops.h — kernel launchers of the seam's many-class loss (kernels_xent.hip) and
-// of rows sorted by expert (kernels_expert.hip); ops.cpp checks the arguments.
+// ops.h — kernel launchers of the seam's many-class loss (kernels_xent.hip), of
+// rows sorted by expert (kernels_expert.hip), of category vectors (kernels_embed.hip), of the
+// norm of gradients (kernels_clip.hip) and of scores from class vectors in 4 bits and their
+// penalties (kernels_fourbit.hip, kernels_adjust.hip); ops.cpp checks the arguments.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -52,5 +54,91 @@ hipError_t launch_expert_combine(hipStream_t s, const ExpertPlan &p, const void 
 hipError_t launch_expert_combine_grad(hipStream_t s, const ExpertPlan &p,
                                       const ExpertMatrix &dout, const void *sorted,
                                       const float *weights, void *d_sorted, float *d_weights);
+
+// ---- category vectors ---------------------------------------------------------
+
+struct EmbedCall {
+    int64_t rows, entries;
+    int32_t dim;
+    bool bf16;                       // table, base, out, dout, dtable: bf16, else f32
+    int64_t row_stride, table_stride;
+    float scale;
+    const int32_t *ids;
+    const void *table, *base;        // base NULL: 0
+    void *out;
+    const void *dout;                // of the gradient
+    void *dtable;
+    int num_cus;
+};
+hipError_t launch_embed(hipStream_t s, const EmbedCall &c);
+size_t embed_grad_scratch(const EmbedCall &c);
+hipError_t launch_embed_grad(hipStream_t s, const EmbedCall &c, char *scratch);
+
+// ---- the norm of many gradients -------------------------------------------------
+
+// A part of a gradient: rows of cols elements; one row, or short ones.
+struct ClipPiece {
+    const void *grad;
+    void *out;                       // NULL: none
+    int64_t stride;
+    int32_t rows, cols;
+    bool bf16;
+    bool wide;                       // addresses and stride are multiples of 16 bytes
+};
+constexpr int64_t CLIP_PIECE = 8192;     // elements
+struct ClipCall {
+    const ClipPiece *piece;
+    int64_t pieces;
+    bool outputs;
+    float max_norm;
+    float *norm;
+    int num_cus;
+};
+size_t clip_scratch(int64_t pieces, int num_cus);
+hipError_t launch_clip(hipStream_t s, const ClipCall &c, char *scratch);
+
+// ---- scores from class vectors in 4 bits, and their penalties -----------------------
+
+struct FourbitShape {
+    int64_t classes;
+    int32_t dim, group;
+    int32_t blocks;                  // of 128 elements
+};
+FourbitShape fourbit_shape(int64_t classes, int32_t dim, int32_t group);
+size_t fourbit_bytes(const FourbitShape &s);
+void fourbit_parts(const FourbitShape &s, char *packed, uint32_t **codes, _Float16 **scales,
+              int32_t **exponents);
+hipError_t launch_fourbit_pack(hipStream_t st, const FourbitShape &s, bool bf16, const void *w,
+                          int64_t stride, char *packed);
+struct FourbitCall {
+    FourbitShape shape;
+    int64_t rows;
+    bool bf16;                       // h: bf16, else f32
+    const void *h;
+    int64_t h_stride;
+    const uint32_t *codes;
+    const _Float16 *scales;
+    const int32_t *exponents;
+    const float *bias;               // NULL: none
+    float *scores;
+    int64_t score_stride;
+    int num_cus;
+};
+size_t fourbit_scratch(const FourbitCall &c);
+hipError_t launch_fourbit_scores(hipStream_t st, const FourbitCall &c, char *scratch);
+
+struct AdjustCall {
+    int64_t rows, classes, score_stride, out_stride;
+    int32_t history;                 // ids a row, at most
+    int64_t history_stride, mask_stride;
+    float repetition, presence, frequency;
+    bool penalties;                  // there are a history and a penalty
+    const float *scores;
+    const int32_t *ids, *lengths;    // lengths NULL: history
+    const float *bias;               // NULL: none
+    const uint32_t *allowed;         // NULL: all
+    float *out;
+};
+hipError_t launch_adjust(hipStream_t s, const AdjustCall &c);
 
 }  // namespace mbk

@@ -74,6 +74,7 @@ struct Scratch {
     std::vector<DevBuf<char>> ops_before;            // outgrown, but in a captured graph
     bool ops_captured = false;
     std::mutex ops_mu;
+    std::vector<std::unique_ptr<mbk_tensors>> lists;
 };
 
 }  // namespace
@@ -252,6 +253,10 @@ hipStream_t context_stream(const mbk_context *ctx) { return ctx->dev->stream; }
 int context_cus(const mbk_context *ctx) { return ctx->dev->num_cus; }
 
 std::mutex &context_scratch_mutex(mbk_context *ctx) { return ctx->scratch.ops_mu; }
+bool context_captured(const mbk_context *ctx) { return being_captured(ctx->dev->stream); }
+std::vector<std::unique_ptr<mbk_tensors>> &context_lists(mbk_context *ctx) {
+    return ctx->scratch.lists;
+}
 
 char *context_scratch(mbk_context *ctx, size_t bytes) {
     Scratch &sc = ctx->scratch;
