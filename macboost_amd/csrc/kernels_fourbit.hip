@@ -10,8 +10,9 @@
 // Layout of W in 4 bits, tiles of 16 classes by blocks of 128 elements, as the matrix
 // instruction's lanes take them: lane q * 16 + c of a block holds 16 bytes of class c, its word j
 // the elements 32 j + 8 q + i, i = 0..7, in nibble (i >> 1) + 4 (i & 1), a code plus 8.
-// Behind them the scales as f16, [tile][block][class][groups of the block], and behind those each
-// class's exponent as int32, [tile][class].
+// Behind them the scales as f16, [tile][four blocks][class][groups of the four blocks], so that a
+// lane loads those of four blocks at once, and behind those each class's exponent as int32,
+// [tile][class].
 #include <algorithm>
 
 #include "grid.hpp"
@@ -58,7 +59,8 @@ __global__ __launch_bounds__(256) void k_fourbit_pack(FourbitShape s, const T *_
     const int64_t cls = tile * TILE + c;
     const bool real = cls < s.classes;
     const T *row = w + (real ? cls : 0) * stride;
-    const int blocks = s.blocks, per = BLOCK / s.group, groups = blocks * per;
+    const int blocks = s.blocks, quads = (blocks + 3) / 4, per = BLOCK / s.group;
+    const int groups = quads * 4 * per;
     const auto scale_of = [&](int g) {
         float m = 0.0f;
         bool finite = true;
@@ -80,8 +82,9 @@ __global__ __launch_bounds__(256) void k_fourbit_pack(FourbitShape s, const T *_
     if (part == 0) exponents[cls] = e;
     for (int g = part; g < groups; g += 16) {
         const float scale = scale_of(g);
-        scales[((tile * blocks + g / per) * TILE + c) * per + g % per] =
+        scales[((tile * quads + g / (4 * per)) * TILE + c) * 4 * per + g % (4 * per)] =
             (_Float16)ldexpf(scale, -e);
+        if (g >= blocks * per) continue;
         for (int k0 = g * s.group; k0 < (g + 1) * s.group; k0 += 8) {
             uint32_t word = 0;
             for (int i = 0; i < 8; ++i) {
@@ -100,46 +103,106 @@ __global__ __launch_bounds__(256) void k_fourbit_pack(FourbitShape s, const T *_
 // h as columns of f16 terms: column r of bf16 rows, columns 2 r and 2 r + 1 of f32 rows (the row
 // and 2^11 times what its f16 leaves, 22 bits together), a power of two apart that brings the row's
 // largest near the top of f16's range.  As the matrix instruction takes them: [column tile][32
-// elements][lane][8], lane q * 16 + column.  A workgroup a row.
+// elements][lane][8], lane q * 16 + column with the elements 8 q + i.
+template <typename T> constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;
+
+// Eight elements of a row from k on, 0 behind its end.
 template <typename T>
-__global__ __launch_bounds__(256) void k_fourbit_columns(const T *__restrict__ h, int64_t stride,
-                                                    int64_t rows, int32_t dim, int32_t steps,
-                                                    _Float16 *__restrict__ columns,
-                                                    int32_t *__restrict__ exponents) {
-    constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;
-    __shared__ float most[4];
-    const int64_t r = group_id();                    // rows of whole tiles of columns
-    if (r * TERMS >= (rows * TERMS + 15) / 16 * 16) return;
-    const T *row = h + (r < rows ? r : 0) * stride;
-    const int n = r < rows ? dim : 0;
+__device__ __forceinline__ void eight(const T *row, int k, int dim, bool wide, float (&v)[8]) {
+    if (wide && k + 8 <= dim) {
+        constexpr int N = 16 / sizeof(T);
+        typedef T V __attribute__((ext_vector_type(N)));
+#pragma unroll
+        for (int x = 0; x < 8 / N; ++x) {
+            const V part = reinterpret_cast<const V *>(row + k)[x];
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[x * N + i] = to_f32(part[i]);
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = k + i < dim ? to_f32(row[k + i]) : 0.0f;
+}
+
+// A wavefront's part of a tile of columns: the steps first, first + each, ... of the largest |h|
+// of the lane's row, over all of its lanes.
+template <typename T>
+__device__ __forceinline__ float largest(const T *row, int dim, bool wide, int steps, int first,
+                                         int each) {
+    const int q = (threadIdx.x & 63) >> 4;
     float m = 0.0f;
-    for (int k = threadIdx.x; k < n; k += 256) m = fmaxf(m, fabsf(to_f32(row[k])));
-    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-    if ((threadIdx.x & 63) == 0) most[threadIdx.x >> 6] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
-    const int e = exponent(m) - H_TOP;
-    if (threadIdx.x == 0 && r < rows) exponents[r] = e;
-    for (int k = threadIdx.x; k < steps * 32; k += 256) {
-        const float v = k < n ? ldexpf(to_f32(row[k]), -e) : 0.0f;
-        const int64_t col = r * TERMS;
-        _Float16 *to = columns + (((col / 16) * steps + k / 32) * 64 + k % 32 / 8 * 16 + col % 16) * 8 +
-                       k % 8;
-        const _Float16 t = (_Float16)v;
-        to[0] = t;
-        if constexpr (TERMS == 2) to[8] = (_Float16)((v - (float)t) * 2048.0f);
+    for (int s = first; s < steps; s += each) {
+        float v[8];
+        eight(row, s * 32 + q * 8, dim, wide, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(v[i]));
+    }
+    m = fmaxf(m, __shfl_xor(m, 16, 64));
+    return fmaxf(m, __shfl_xor(m, 32, 64));
+}
+
+// The same steps as terms, a KB a step.
+template <typename T>
+__device__ __forceinline__ void terms(const T *row, int dim, bool wide, int steps, int first,
+                                      int each, int e, half8 *to) {
+    const int lane = threadIdx.x & 63;
+    for (int s = first; s < steps; s += each) {
+        float v[8];
+        eight(row, s * 32 + (lane >> 4) * 8, dim, wide, v);
+        half8 out;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float x = ldexpf(v[i], -e);
+            const _Float16 t = (_Float16)x;
+            out[i] = TERMS<T> == 2 && (lane & 1) ? (_Float16)((x - (float)t) * 2048.0f) : t;
+        }
+        to[s * 64 + lane] = out;
     }
 }
 
+// Where many columns are made for all workgroups: a workgroup a tile of columns.
+constexpr int COLUMN_WAVES = 8;
+template <typename T>
+__global__ __launch_bounds__(64 * COLUMN_WAVES) void k_fourbit_columns(
+    const T *__restrict__ h, int64_t stride, int64_t rows, int32_t dim, bool wide, int32_t steps,
+    half8 *__restrict__ columns, int32_t *__restrict__ exponents) {
+    __shared__ float most[COLUMN_WAVES][16];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int64_t tile = group_id(), r = (tile * 16 + (lane & 15)) / TERMS<T>;
+    if (tile * 16 >= rows * TERMS<T>) return;
+    const T *row = h + (r < rows ? r : 0) * stride;
+    const int n = r < rows ? dim : 0;
+    const float m = largest(row, n, wide, steps, wave, COLUMN_WAVES);
+    if (lane < 16) most[wave][lane] = m;
+    __syncthreads();
+    float all = 0.0f;
+#pragma unroll
+    for (int w = 0; w < COLUMN_WAVES; ++w) all = fmaxf(all, most[w][lane & 15]);
+    const int e = exponent(all) - H_TOP;
+    if (wave == 0 && lane < 16 && r < rows) exponents[r] = e;
+    terms(row, n, wide, steps, wave, COLUMN_WAVES, e, columns + tile * steps * 64);
+}
+
+// Constants of weights() in registers, so that a mask and the exponent's bits are one instruction
+// (which takes no literals).
+struct Unpack {
+    uint32_t low, high;              // masks of the nibbles
+    uint32_t exponent;               // f16's 1024
+    __device__ __forceinline__ Unpack() {
+        asm("s_mov_b32 %0, 0x000F000F" : "=s"(low));
+        asm("s_mov_b32 %0, 0x00F000F0" : "=s"(high));
+        asm("v_mov_b32 %0, 0x64006400" : "=v"(exponent));
+    }
+};
+
 // Eight codes of a word times the scale, exact.
-__device__ __forceinline__ half8 weights(uint32_t word, _Float16 scale) {
+__device__ __forceinline__ half8 weights(const Unpack &u, uint32_t word, _Float16 scale) {
     const half2 s = {scale, scale};
     half8 out;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         // 1024 + n or 1024 + 16 n in the low bits of an f16
-        const uint32_t w = i < 2 ? word : word >> 8;
-        const uint32_t bits = (w & (i & 1 ? 0x00F000F0u : 0x000F000Fu)) | 0x64006400u;
+        const uint32_t bits = ((i < 2 ? word : word >> 8) & (i & 1 ? u.high : u.low)) | u.exponent;
         half2 v = __builtin_bit_cast(half2, bits);
         if (i & 1) {
             const half2 by = {(_Float16)0.0625f, (_Float16)0.0625f};
@@ -156,79 +219,312 @@ __device__ __forceinline__ half8 weights(uint32_t word, _Float16 scale) {
     return out;
 }
 
-// A wavefront two tiles of classes by CT tiles of columns.
-template <int TERMS, int CT>
-__global__ __launch_bounds__(256) void k_fourbit_scores(FourbitCall c, const _Float16 *__restrict__ columns,
-                                                   const int32_t *__restrict__ row_exponents) {
-    constexpr int TC = 2;
+// Words and scales of a class tile's blocks.
+template <int PER> struct Scales {
+    half8 x[PER < 2 ? 1 : PER / 2];                  // of four blocks; PER 1: half of it
+};
+template <int PER>
+__device__ __forceinline__ Scales<PER> scales_of(const _Float16 *scales, int64_t quad) {
+    const _Float16 *s = scales + (quad * TILE + (threadIdx.x & 15)) * 4 * PER;
+    Scales<PER> out;
+    if constexpr (PER == 1) {
+        typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+        const half4 v = *reinterpret_cast<const half4 *>(s);
+        out.x[0] = half8{v[0], v[1], v[2], v[3], 0, 0, 0, 0};
+    } else {
+#pragma unroll
+        for (int i = 0; i < PER / 2; ++i) out.x[i] = reinterpret_cast<const half8 *>(s)[i];
+    }
+    return out;
+}
+// Of word j of block i.
+template <int PER>
+__device__ __forceinline__ _Float16 scale_at(const Scales<PER> &s, int i, int j) {
+    const int at = i * PER + j * PER / 4;
+    return s.x[at / 8][at % 8];
+}
+
+__device__ __forceinline__ float other_term(float v) {       // the neighbouring column's
+    return __builtin_bit_cast(
+        float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0xB1, 0xF, 0xF, true));
+}
+
+// What the scores of a tile of classes end with: a lane's classes, their exponents and biases.  N
+// terms a row: with two a column's lanes have two of its four classes each.  Loaded before the
+// first scores are written, since loads between the stores wait one by one.
+template <int N> struct Ends {
+    static constexpr int EACH = 4 / N;
+    int64_t cls;
+    int e[EACH];
+    float b[EACH];
+};
+template <int N>
+__device__ __forceinline__ Ends<N> ends_of(const FourbitCall &c, int64_t tile) {
     const int lane = threadIdx.x & 63;
+    Ends<N> out;
+    out.cls = tile * TILE + (lane >> 4) * 4 + (N == 2 && (lane & 1) ? 2 : 0);
+#pragma unroll
+    for (int i = 0; i < Ends<N>::EACH; ++i) {
+        const bool real = out.cls + i < c.shape.classes;
+        out.e[i] = real ? c.exponents[out.cls + i] : 0;
+        out.b[i] = real && c.bias ? c.bias[out.cls + i] : 0.0f;
+    }
+    return out;
+}
+
+template <int N>
+__device__ __forceinline__ void write_scores(const FourbitCall &c, const float4v &z,
+                                             const Ends<N> &end, int64_t column,
+                                             int row_exponent) {
+    constexpr int EACH = Ends<N>::EACH;
+    float v[EACH];
+    if constexpr (N == 2) {
+        const bool odd = threadIdx.x & 1;
+        const float a = other_term(odd ? z[0] : z[2]), b = other_term(odd ? z[1] : z[3]);
+        v[0] = odd ? __builtin_fmaf(z[2], 0x1p-11f, a) : __builtin_fmaf(a, 0x1p-11f, z[0]);
+        v[1] = odd ? __builtin_fmaf(z[3], 0x1p-11f, b) : __builtin_fmaf(b, 0x1p-11f, z[1]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = z[i];
+    }
+    const int64_t row = column / N;
+    if (row >= c.rows) return;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+        v[i] = ldexpf(v[i], end.e[i] + row_exponent);
+        if (c.bias) v[i] = end.b[i] == -__builtin_inff() ? end.b[i] : v[i] + end.b[i];
+    }
+    float *to = c.scores + row * c.score_stride + end.cls;
+    typedef float V __attribute__((ext_vector_type(EACH)));
+    if (c.wide_scores && end.cls + EACH <= c.shape.classes) {
+        V out;
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) out[i] = v[i];
+        *reinterpret_cast<V *>(to) = out;
+    } else {
+#pragma unroll
+        for (int i = 0; i < EACH; ++i)
+            if (end.cls + i < c.shape.classes) to[i] = v[i];
+    }
+}
+
+// ---- few columns: reading W is the work ------------------------------------------------
+// All columns lie in LDS, made there by each workgroup.  A wavefront streams its tiles of classes,
+// four blocks at a time and two such reads ahead; `ks` wavefronts share a tile's blocks where
+// there are few tiles.  Tiles go to the workgroups in turn, so that no CU has two more than another.
+constexpr int FEW_WAVES = 8;
+template <typename T, int CT, int PER>
+__global__ __launch_bounds__(64 * FEW_WAVES, 4) void k_fourbit_few(FourbitCall c, int32_t ks) {
+    extern __shared__ half8 lds[];
+    float *most = reinterpret_cast<float *>(lds);    // [wave][column]
+    half8 *columns = lds + FEW_WAVES * CT * 4;       // [column tile][step][lane]
+    constexpr int N = TERMS<T>;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int64_t tiles = (c.shape.classes + TILE - 1) / TILE;
-    const int64_t tile0 = ((int64_t)group_id() * 4 + (threadIdx.x >> 6)) * TC;
-    if (tile0 >= tiles) return;
-    const int blocks = c.shape.blocks, per = BLOCK / c.shape.group;
-    const int64_t col_tiles = (c.rows * TERMS + 15) / 16;
-    for (int64_t ct0 = (int64_t)blockIdx.y * CT; ct0 < col_tiles; ct0 += (int64_t)gridDim.y * CT) {
-        float4v acc[TC][CT];
+    const int blocks = c.shape.blocks, quads = (blocks + 3) / 4, steps = blocks * 4;
+    const int part = wave % ks;
+    const int first = part * quads / ks, last = (part + 1) * quads / ks;
+    const int64_t turn = (int64_t)gridDim.x * (FEW_WAVES / ks);
+    const Unpack unpack;
+
+    struct Place {
+        int64_t tile;
+        int quad;
+    };
+    struct Buffer {
+        uint4v word[4];
+        Scales<PER> scale;
+    };
+    const auto after = [&](Place p) {
+        return p.quad + 1 < last ? Place{p.tile, p.quad + 1} : Place{p.tile + turn, first};
+    };
+    const auto fetch = [&](Buffer &b, const Place &p) {
+        if (p.tile >= tiles) return;
+        const uint4v *from =
+            reinterpret_cast<const uint4v *>(c.codes) + (p.tile * blocks + p.quad * 4) * 64;
 #pragma unroll
-        for (int t = 0; t < TC; ++t)
+        for (int i = 0; i < 4; ++i)
+            if (p.quad * 4 + i < blocks) b.word[i] = from[i * 64 + lane];
+        b.scale = scales_of<PER>(c.scales, p.tile * quads + p.quad);
+    };
+    Place at{(int64_t)(wave / ks) * gridDim.x + blockIdx.x, first};
+    Place ahead = after(at);
+    Buffer x0, x1, x2;
+    fetch(x0, at);
+    fetch(x1, ahead);
+
+    const T *h = static_cast<const T *>(c.h);
+    int64_t rows_at[CT];
 #pragma unroll
-            for (int x = 0; x < CT; ++x) acc[t][x] = float4v{0, 0, 0, 0};
-        for (int b = 0; b < blocks; ++b) {
-            uint4v word[TC];
-            _Float16 scale[TC][4];
+    for (int x = 0; x < CT; ++x) {
+        const int64_t r = (x * 16 + (lane & 15)) / N;
+        rows_at[x] = r < c.rows ? r : -1;
+        const float m = largest(h + (rows_at[x] < 0 ? 0 : r) * c.h_stride,
+                                rows_at[x] < 0 ? 0 : c.shape.dim, c.wide_h, steps, wave, FEW_WAVES);
+        if (lane < 16) most[(wave * CT + x) * 16 + lane] = m;
+    }
+    __syncthreads();
+    int re[CT];
 #pragma unroll
-            for (int t = 0; t < TC; ++t) {
-                const int64_t at = min(tile0 + t, tiles - 1) * blocks + b;
-                word[t] = reinterpret_cast<const uint4v *>(c.codes)[at * 64 + lane];
-                const _Float16 *s = c.scales + (at * TILE + (lane & 15)) * per;
+    for (int x = 0; x < CT; ++x) {
+        float m = 0.0f;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) scale[t][j] = s[j * per / 4];
-            }
+        for (int w = 0; w < FEW_WAVES; ++w) m = fmaxf(m, most[(w * CT + x) * 16 + (lane & 15)]);
+        re[x] = exponent(m) - H_TOP;
+        terms(h + (rows_at[x] < 0 ? 0 : rows_at[x]) * c.h_stride, rows_at[x] < 0 ? 0 : c.shape.dim,
+              c.wide_h, steps, wave, FEW_WAVES, re[x], columns + x * steps * 64);
+    }
+    __syncthreads();
+
+    float4v acc[CT];
+#pragma unroll
+    for (int x = 0; x < CT; ++x) acc[x] = float4v{0, 0, 0, 0};
+    Ends<N> end;
+    // One read's blocks; false behind the last one.
+    const auto step = [&](const Buffer &b, Buffer &next) {
+        if (at.tile >= tiles) return false;
+        const Place then = after(ahead);
+        fetch(next, then);
+        if (at.quad == first) end = ends_of<N>(c, at.tile);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (at.quad * 4 + i >= blocks) break;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                half8 a[TC];
+                const half8 a = weights(unpack, b.word[i][j], scale_at<PER>(b.scale, i, j));
 #pragma unroll
-                for (int t = 0; t < TC; ++t) a[t] = weights(word[t][j], scale[t][j]);
-#pragma unroll
-                for (int x = 0; x < CT; ++x) {
-                    const int64_t ct = min(ct0 + x, col_tiles - 1);
-                    const half8 h = reinterpret_cast<const half8 *>(
-                        columns)[(ct * blocks * 4 + b * 4 + j) * 64 + lane];
-#pragma unroll
-                    for (int t = 0; t < TC; ++t)
-                        acc[t][x] =
-                            __builtin_amdgcn_mfma_f32_16x16x32_f16(a[t], h, acc[t][x], 0, 0, 0);
-                }
+                for (int x = 0; x < CT; ++x)
+                    acc[x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                        a, columns[(x * steps + (at.quad * 4 + i) * 4 + j) * 64 + lane], acc[x], 0,
+                        0, 0);
             }
         }
-#pragma unroll
-        for (int t = 0; t < TC; ++t) {
-            const int64_t cls = (tile0 + t) * TILE + (lane >> 4) * 4;
+        if (at.quad + 1 == last && ks == 1) {
 #pragma unroll
             for (int x = 0; x < CT; ++x) {
-                float4v z = acc[t][x];
-                if constexpr (TERMS == 2)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        z[i] = __builtin_fmaf(__shfl_xor(z[i], 1, 64), 0x1p-11f, z[i]);
-                const int64_t row = ((ct0 + x) * 16 + (lane & 15)) / TERMS;
-                const bool mine = (TERMS == 1 || !(lane & 1)) && row < c.rows;
-                if (mine && tile0 + t < tiles) {
-                    const int re = row_exponents[row];
-                    float *to = c.scores + row * c.score_stride + cls;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (cls + i < c.shape.classes) {
-                            float v = ldexpf(z[i], c.exponents[cls + i] + re);
-                            if (c.bias) {
-                                const float b = c.bias[cls + i];
-                                v = b == -__builtin_inff() ? b : v + b;
-                            }
-                            to[i] = v;
-                        }
-                }
+                write_scores<N>(c, acc[x], end, x * 16 + (lane & 15), re[x]);
+                acc[x] = float4v{0, 0, 0, 0};
             }
         }
+        at = ahead;
+        ahead = then;
+        return true;
+    };
+    while (step(x0, x2) && step(x1, x0) && step(x2, x1)) {}
+    if (ks == 1) return;
+    // a tile a group of wavefronts: their sums meet in LDS, in the order of the blocks
+    __syncthreads();                                 // the columns are read
+    float4v *sums = reinterpret_cast<float4v *>(columns);
+#pragma unroll
+    for (int x = 0; x < CT; ++x) sums[(wave * CT + x) * 64 + lane] = acc[x];
+    __syncthreads();
+    const int64_t tile = (int64_t)(wave / ks) * gridDim.x + blockIdx.x;
+    if (part != 0 || tile >= tiles) return;
+#pragma unroll
+    for (int x = 0; x < CT; ++x) {
+        float4v z = acc[x];
+        for (int p = 1; p < ks; ++p) {
+            const float4v y = sums[((wave + p) * CT + x) * 64 + lane];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) z[i] += y[i];
+        }
+        write_scores<N>(c, z, end, x * 16 + (lane & 15), re[x]);
+    }
+}
+
+// ---- more columns: tiles of 256 classes by CT * 16 columns --------------------------------
+// A wavefront four tiles of classes, whose codes it turns into f16 in registers; the four share the
+// columns of a block of W, copied to LDS while the block before is worked on.
+typedef __attribute__((address_space(1))) void global_void;
+typedef __attribute__((address_space(3))) void lds_void;
+constexpr int WIDE_WAVES = 4, WIDE_TILES = 4;
+template <int N, int CT, int PER>
+__global__ __launch_bounds__(64 * WIDE_WAVES, 2) void k_fourbit_tiles(
+    FourbitCall c, const half8 *__restrict__ columns, const int32_t *__restrict__ row_exponents,
+    int64_t column_tiles, int32_t turns) {
+    extern __shared__ half8 lds[];                   // [buffer][column tile][step of the block][lane]
+    constexpr int BUFFER = CT * 4 * 64;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int64_t tiles = (c.shape.classes + TILE - 1) / TILE;
+    const int blocks = c.shape.blocks, quads = (blocks + 3) / 4;
+    const int64_t id = group_id();
+    const int64_t tile0 = (id / turns * WIDE_WAVES + wave) * WIDE_TILES;
+    const int64_t column0 = id % turns * CT;
+    if (id / turns * WIDE_WAVES * WIDE_TILES >= tiles) return;
+    const auto copy = [&](int b) {
+#pragma unroll
+        for (int x = 0; x < CT; ++x) {
+            const int64_t t = min(column0 + x, column_tiles - 1);
+            __builtin_amdgcn_global_load_lds(
+                (global_void *)(columns + ((t * blocks + b) * 4 + wave) * 64 + lane),
+                (lds_void *)(lds + (b & 1) * BUFFER + (x * 4 + wave) * 64), 16, 0, 0);
+        }
+    };
+    const Unpack unpack;
+    int64_t at[WIDE_TILES];
+#pragma unroll
+    for (int t = 0; t < WIDE_TILES; ++t) at[t] = min(tile0 + t, tiles - 1);
+    uint4v word[WIDE_TILES], ahead[WIDE_TILES];
+    const auto fetch = [&](int b) {
+#pragma unroll
+        for (int t = 0; t < WIDE_TILES; ++t)
+            ahead[t] = reinterpret_cast<const uint4v *>(c.codes)[(at[t] * blocks + b) * 64 + lane];
+    };
+    typedef _Float16 halves __attribute__((ext_vector_type(PER)));
+    halves scale[WIDE_TILES], scale_ahead[WIDE_TILES];
+    const auto fetch_scales = [&](int b) {
+#pragma unroll
+        for (int t = 0; t < WIDE_TILES; ++t)
+            scale_ahead[t] = reinterpret_cast<const halves *>(
+                c.scales)[((at[t] * quads + b / 4) * TILE + (lane & 15)) * 4 + b % 4];
+    };
+    float4v acc[WIDE_TILES][CT];
+#pragma unroll
+    for (int t = 0; t < WIDE_TILES; ++t)
+#pragma unroll
+        for (int x = 0; x < CT; ++x) acc[t][x] = float4v{0, 0, 0, 0};
+    copy(0);
+    fetch(0);
+    fetch_scales(0);
+    for (int b = 0; b < blocks; ++b) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();                             // the block is there; the other buffer is read
+#pragma unroll
+        for (int t = 0; t < WIDE_TILES; ++t) {
+            word[t] = ahead[t];
+            scale[t] = scale_ahead[t];
+        }
+        if (b + 1 < blocks) {
+            copy(b + 1);
+            fetch(b + 1);
+            fetch_scales(b + 1);
+        }
+        const half8 *here = lds + (b & 1) * BUFFER + lane;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            half8 a[WIDE_TILES];
+#pragma unroll
+            for (int t = 0; t < WIDE_TILES; ++t) a[t] = weights(unpack, word[t][j], scale[t][j * PER / 4]);
+#pragma unroll
+            for (int x = 0; x < CT; ++x) {
+                const half8 h = here[(x * 4 + j) * 64];
+#pragma unroll
+                for (int t = 0; t < WIDE_TILES; ++t)
+                    acc[t][x] =
+                        __builtin_amdgcn_mfma_f32_16x16x32_f16(a[t], h, acc[t][x], 0, 0, 0);
+            }
+        }
+    }
+    int e[CT];
+#pragma unroll
+    for (int x = 0; x < CT; ++x)
+        e[x] = row_exponents[min(((column0 + x) * 16 + (lane & 15)) / N, c.rows - 1)];
+#pragma unroll
+    for (int t = 0; t < WIDE_TILES; ++t) {
+        const Ends<N> end = ends_of<N>(c, tile0 + t);
+#pragma unroll
+        for (int x = 0; x < CT; ++x)
+            write_scores<N>(c, acc[t][x], end, (column0 + x) * 16 + (lane & 15), e[x]);
     }
 }
 
@@ -238,7 +534,8 @@ size_t code_bytes(const FourbitShape &s) {
     return (size_t)((s.classes + TILE - 1) / TILE) * s.blocks * 1024;
 }
 size_t scale_bytes(const FourbitShape &s) {
-    return (size_t)((s.classes + TILE - 1) / TILE) * s.blocks * TILE * (BLOCK / s.group) * 2;
+    return (size_t)((s.classes + TILE - 1) / TILE) * ((s.blocks + 3) / 4) * 4 * TILE *
+           (BLOCK / s.group) * 2;
 }
 
 // Columns of h that are held: 64 MB of them, or 16 rows.
@@ -250,29 +547,80 @@ size_t column_bytes(const FourbitCall &c, size_t rows) {
     return (rows * (c.bf16 ? 1 : 2) + 15) / 16 * c.shape.blocks * 4096;
 }
 
-template <int TERMS, int CT>
-hipError_t scores(hipStream_t st, const FourbitCall &c, const _Float16 *columns, const int32_t *e) {
+// The columns that fit LDS beside the wavefronts' maxima.
+constexpr size_t FEW_LDS = 150 << 10;
+template <typename T> int64_t column_tiles(const FourbitCall &c) {
+    return (c.rows * TERMS<T> + 15) / 16;
+}
+bool few(const FourbitCall &c) {
+    const int64_t tiles = c.bf16 ? column_tiles<__bf16>(c) : column_tiles<float>(c);
+    return tiles <= 4 && (size_t)(tiles == 3 ? 4 : tiles) * c.shape.blocks * 4096 <= FEW_LDS;
+}
+
+template <typename T, int CT, int PER> hipError_t run_few(hipStream_t st, const FourbitCall &c) {
+    const void *f = reinterpret_cast<const void *>(k_fourbit_few<T, CT, PER>);
+    const hipError_t e = allow_all_lds(f);
+    if (e != hipSuccess) return e;
     const int64_t tiles = (c.shape.classes + TILE - 1) / TILE;
-    const int64_t col_tiles = (c.rows * TERMS + 15) / 16;
-    const int64_t turns = (col_tiles + CT - 1) / CT;
-    hipLaunchKernelGGL((k_fourbit_scores<TERMS, CT>), grid_of((tiles + 7) / 8, (uint32_t)std::min<int64_t>(turns, 32768)),
-                       dim3(256), 0, st, c, columns, e);
+    const int quads = (c.shape.blocks + 3) / 4;
+    // wavefronts a tile: as many as leave each CU a workgroup
+    int ks = 1;
+    while (ks < FEW_WAVES && 2 * ks <= quads && tiles * ks < (int64_t)FEW_WAVES * c.num_cus) ks *= 2;
+    const int64_t groups = (tiles * ks + FEW_WAVES - 1) / FEW_WAVES;
+    const size_t columns = (size_t)CT * c.shape.blocks * 4096;
+    const size_t lds = (size_t)FEW_WAVES * CT * 64 +
+                       std::max<size_t>(columns, ks > 1 ? (size_t)FEW_WAVES * CT * 1024 : 0);
+    const int64_t most = (int64_t)c.num_cus * (lds <= (80 << 10) ? 2 : 1);
+    hipLaunchKernelGGL((k_fourbit_few<T, CT, PER>),
+                       dim3((uint32_t)(ks > 1 ? groups : std::min(groups, most))),
+                       dim3(64 * FEW_WAVES), lds, st, c, ks);
     return hipGetLastError();
 }
 
-template <typename T>
-hipError_t run(hipStream_t st, const FourbitCall &c, char *scratch) {
-    constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;
-    _Float16 *columns = reinterpret_cast<_Float16 *>(scratch);
-    const int64_t col_tiles = (c.rows * TERMS + 15) / 16;
+template <typename T, int CT, int PER>
+hipError_t run_tiles(hipStream_t st, const FourbitCall &c, const half8 *columns, const int32_t *e,
+                     int64_t column_tiles, int turns) {
+    const hipError_t bad =
+        allow_all_lds(reinterpret_cast<const void *>(k_fourbit_tiles<TERMS<T>, CT, PER>));
+    if (bad != hipSuccess) return bad;
+    const int64_t tiles = (c.shape.classes + TILE - 1) / TILE;
+    const int64_t groups = (tiles + WIDE_WAVES * WIDE_TILES - 1) / (WIDE_WAVES * WIDE_TILES) * turns;
+    hipLaunchKernelGGL((k_fourbit_tiles<TERMS<T>, CT, PER>), grid_of(groups), dim3(64 * WIDE_WAVES),
+                       (size_t)CT * 8192, st, c, columns, e, column_tiles, turns);
+    return hipGetLastError();
+}
+
+template <typename T, int PER> hipError_t run(hipStream_t st, const FourbitCall &c, char *scratch) {
+    const int64_t tiles = column_tiles<T>(c);
+    if (few(c))
+        return tiles <= 1 ? run_few<T, 1, PER>(st, c)
+                          : tiles <= 2 ? run_few<T, 2, PER>(st, c) : run_few<T, 4, PER>(st, c);
+    half8 *columns = reinterpret_cast<half8 *>(scratch);
     const int steps = c.shape.blocks * 4;
     int32_t *e = reinterpret_cast<int32_t *>(scratch + column_bytes(c, (size_t)c.rows));
-    hipLaunchKernelGGL((k_fourbit_columns<T>), grid_of(col_tiles * 16 / TERMS), dim3(256), 0, st,
-                       static_cast<const T *>(c.h), c.h_stride, c.rows, c.shape.dim, steps, columns,
-                       e);
-    if (col_tiles <= 1) return scores<TERMS, 1>(st, c, columns, e);
-    if (col_tiles <= 2) return scores<TERMS, 2>(st, c, columns, e);
-    return scores<TERMS, 4>(st, c, columns, e);
+    hipLaunchKernelGGL((k_fourbit_columns<T>), grid_of(tiles), dim3(64 * COLUMN_WAVES), 0, st,
+                       static_cast<const T *>(c.h), c.h_stride, c.rows, c.shape.dim, c.wide_h, steps,
+                       columns, e);
+    // up to 8 tiles of columns a turn, turns of one size
+    const int64_t turns = (tiles + 7) / 8;
+    switch ((tiles + turns - 1) / turns) {
+    case 1: return run_tiles<T, 1, PER>(st, c, columns, e, tiles, (int)turns);
+    case 2: return run_tiles<T, 2, PER>(st, c, columns, e, tiles, (int)turns);
+    case 3: return run_tiles<T, 3, PER>(st, c, columns, e, tiles, (int)turns);
+    case 4: return run_tiles<T, 4, PER>(st, c, columns, e, tiles, (int)turns);
+    case 5: return run_tiles<T, 5, PER>(st, c, columns, e, tiles, (int)turns);
+    case 6: return run_tiles<T, 6, PER>(st, c, columns, e, tiles, (int)turns);
+    case 7: return run_tiles<T, 7, PER>(st, c, columns, e, tiles, (int)turns);
+    default: return run_tiles<T, 8, PER>(st, c, columns, e, tiles, (int)turns);
+    }
+}
+
+template <typename T> hipError_t run(hipStream_t st, const FourbitCall &c, char *scratch) {
+    switch (c.shape.group) {
+    case 32: return run<T, 4>(st, c, scratch);
+    case 64: return run<T, 2>(st, c, scratch);
+    default: return run<T, 1>(st, c, scratch);
+    }
 }
 
 }  // namespace
@@ -310,6 +658,7 @@ hipError_t launch_fourbit_pack(hipStream_t st, const FourbitShape &s, bool bf16,
 }
 
 size_t fourbit_scratch(const FourbitCall &c) {
+    if (few(c)) return 0;
     const size_t rows = (size_t)std::min(c.rows, rows_a_turn(c));
     return column_bytes(c, rows) + 4 * rows;
 }
@@ -317,9 +666,13 @@ size_t fourbit_scratch(const FourbitCall &c) {
 hipError_t launch_fourbit_scores(hipStream_t st, const FourbitCall &c, char *scratch) {
     const int64_t each = rows_a_turn(c);
     const int64_t row = c.h_stride * (c.bf16 ? 2 : 4);
+    const bool wide_h = reinterpret_cast<uintptr_t>(c.h) % 16 == 0 && row % 16 == 0;
+    const bool wide_scores = reinterpret_cast<uintptr_t>(c.scores) % 16 == 0 && c.score_stride % 4 == 0;
     for (int64_t r = 0; r < c.rows; r += each) {
         FourbitCall part = c;
         part.rows = std::min(each, c.rows - r);
+        part.wide_h = wide_h;
+        part.wide_scores = wide_scores;
         part.h = static_cast<const char *>(c.h) + r * row;
         part.scores = c.scores + r * c.score_stride;
         const hipError_t e = c.bf16 ? run<__bf16>(st, part, scratch) : run<float>(st, part, scratch);

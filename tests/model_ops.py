@@ -129,11 +129,12 @@ class Fourbit:
         # element 32 j + 8 q + i
         code = code.transpose(0, 3, 1, 4, 2, 5).reshape(tiles * 16, blocks * 128)
         at = tiles * blocks * 1024
-        size = tiles * blocks * 16 * per * 2
-        half = raw[at:at + size].view(np.float16).reshape(tiles, blocks, 16, per)
+        quads = -(-blocks // 4)
+        size = tiles * quads * 16 * 4 * per * 2
+        half = raw[at:at + size].view(np.float16).reshape(tiles, quads, 16, 4 * per)
         at += -(-size // 256) * 256
         exponent = raw[at:at + tiles * 64].view(np.int32)
-        scale = half.astype(np.float64).transpose(0, 2, 1, 3).reshape(tiles * 16, blocks * per)
+        scale = half.astype(np.float64).transpose(0, 2, 1, 3).reshape(tiles * 16, quads * 4 * per)
         return code, np.ldexp(scale, exponent[:, None])
 
     def scores(self, h, bias=None, pad=0, score_pad=0, shift=0, out=None):

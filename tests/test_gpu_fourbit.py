@@ -58,6 +58,7 @@ SHAPES = [
     (1, 1, 1), (1, 64, 1000), (2, 37, 100), (3, 128, 16), (8, 200, 31), (9, 129, 333), (15, 96, 47),
     (16, 1024, 500), (17, 1000, 129), (31, 300, 65), (33, 260, 1003), (64, 512, 200), (65, 130, 77),
     (130, 777, 300), (201, 100, 2100), (500, 33, 40), (4, 4000, 50), (1, 8200, 18),
+    (40, 1300, 70), (16, 2600, 300), (20, 2600, 33), (96, 140, 600), (5, 1024, 2000), (7, 600, 5000),
 ]
 
 
