@@ -309,23 +309,40 @@ __device__ __forceinline__ void write_scores(const FourbitCall &c, const float4v
 }
 
 // ---- few columns: reading W is the work ------------------------------------------------
-// All columns lie in LDS, made there by each workgroup.  A wavefront streams its tiles of classes,
-// four blocks at a time and two such reads ahead; `ks` wavefronts share a tile's blocks where
-// there are few tiles.  Tiles go to the workgroups in turn, so that no CU has two more than another.
-constexpr int FEW_WAVES = 8;
+// All columns lie in LDS, made there by each workgroup: [step][q][column], without the columns
+// that no row has, in whose place the matrix instruction gets the last one's.  A wavefront streams
+// its tiles of classes, four blocks at a time and two such reads ahead; `ks` wavefronts share a
+// tile's blocks where there are few tiles.  Tiles go to the workgroups in turn, so that no CU has
+// two more than another.
+constexpr int FEW_WAVES = 8, FEW_THREADS = 64 * FEW_WAVES;
+constexpr int FEW_HEAD = 1024;       // bytes of LDS before the columns: exponents of up to 64 rows
+constexpr int KEPT = 4;              // eights of h that a thread keeps from the maximum on
 template <typename T, int CT, int PER>
-__global__ __launch_bounds__(64 * FEW_WAVES, 4) void k_fourbit_few(FourbitCall c, int32_t ks) {
+__global__ __launch_bounds__(FEW_THREADS, 4) void k_fourbit_few(FourbitCall c, int32_t ks,
+                                                                int32_t log2_rows) {
     extern __shared__ half8 lds[];
-    float *most = reinterpret_cast<float *>(lds);    // [wave][column]
-    half8 *columns = lds + FEW_WAVES * CT * 4;       // [column tile][step][lane]
+    int *exponents = reinterpret_cast<int *>(lds);   // [row]
+    half8 *columns = lds + FEW_HEAD / 16;
     constexpr int N = TERMS<T>;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int64_t tiles = (c.shape.classes + TILE - 1) / TILE;
-    const int blocks = c.shape.blocks, quads = (blocks + 3) / 4, steps = blocks * 4;
+    const int blocks = c.shape.blocks, quads = (blocks + 3) / 4;
     const int part = wave % ks;
     const int first = part * quads / ks, last = (part + 1) * quads / ks;
     const int64_t turn = (int64_t)gridDim.x * (FEW_WAVES / ks);
+    const int width = (int)c.rows * N;               // columns
     const Unpack unpack;
+
+    // a thread's row of h, and its eights of it: the first ones stay in registers
+    const int my_row = threadIdx.x & ((1 << log2_rows) - 1);
+    const int eights = blocks * (BLOCK / 8), each = FEW_THREADS >> log2_rows;
+    const int first_eight = threadIdx.x >> log2_rows;
+    const bool has_row = my_row < c.rows;
+    const T *row = static_cast<const T *>(c.h) + (has_row ? my_row : 0) * c.h_stride;
+    const int n = has_row ? c.shape.dim : 0;
+    float kept[KEPT][8], most = 0.0f;
+#pragma unroll
+    for (int i = 0; i < KEPT; ++i) eight(row, (first_eight + i * each) * 8, n, c.wide_h, kept[i]);
 
     struct Place {
         int64_t tile;
@@ -353,28 +370,56 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 4) void k_fourbit_few(FourbitCall c
     fetch(x0, at);
     fetch(x1, ahead);
 
-    const T *h = static_cast<const T *>(c.h);
-    int64_t rows_at[CT];
 #pragma unroll
-    for (int x = 0; x < CT; ++x) {
-        const int64_t r = (x * 16 + (lane & 15)) / N;
-        rows_at[x] = r < c.rows ? r : -1;
-        const float m = largest(h + (rows_at[x] < 0 ? 0 : r) * c.h_stride,
-                                rows_at[x] < 0 ? 0 : c.shape.dim, c.wide_h, steps, wave, FEW_WAVES);
-        if (lane < 16) most[(wave * CT + x) * 16 + lane] = m;
+    for (int i = 0; i < KEPT; ++i)
+#pragma unroll
+        for (int x = 0; x < 8; ++x) most = fmaxf(most, fabsf(kept[i][x]));
+    for (int g = first_eight + KEPT * each; g < eights; g += each) {
+        float v[8];
+        eight(row, g * 8, n, c.wide_h, v);
+#pragma unroll
+        for (int x = 0; x < 8; ++x) most = fmaxf(most, fabsf(v[x]));
+    }
+    for (int o = 1 << log2_rows; o < 64; o <<= 1) most = fmaxf(most, __shfl_xor(most, o, 64));
+    // [wave][row] where the columns come
+    float *meet = reinterpret_cast<float *>(columns);
+    if (lane < 1 << log2_rows) meet[(wave << log2_rows) + lane] = most;
+    __syncthreads();
+    for (int w = 0; w < FEW_WAVES; ++w) most = fmaxf(most, meet[(w << log2_rows) + my_row]);
+    __syncthreads();
+    const int e = exponent(most) - H_TOP;
+    if (threadIdx.x < c.rows) exponents[threadIdx.x] = e;
+    const auto put = [&](int g, const float (&v)[8]) {
+        half8 t, rest;
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+            const float y = ldexpf(v[x], -e);
+            t[x] = (_Float16)y;
+            rest[x] = (_Float16)((y - (float)t[x]) * 2048.0f);
+        }
+        half8 *to = columns + g * width + my_row * N;
+        to[0] = t;
+        if constexpr (N == 2) to[1] = rest;
+    };
+    if (has_row) {
+#pragma unroll
+        for (int i = 0; i < KEPT; ++i)
+            if (first_eight + i * each < eights) put(first_eight + i * each, kept[i]);
+        for (int g = first_eight + KEPT * each; g < eights; g += each) {
+            float v[8];
+            eight(row, g * 8, n, c.wide_h, v);
+            put(g, v);
+        }
     }
     __syncthreads();
+    const half8 *mine[CT];                           // the lane's column of step 0
     int re[CT];
 #pragma unroll
     for (int x = 0; x < CT; ++x) {
-        float m = 0.0f;
-#pragma unroll
-        for (int w = 0; w < FEW_WAVES; ++w) m = fmaxf(m, most[(w * CT + x) * 16 + (lane & 15)]);
-        re[x] = exponent(m) - H_TOP;
-        terms(h + (rows_at[x] < 0 ? 0 : rows_at[x]) * c.h_stride, rows_at[x] < 0 ? 0 : c.shape.dim,
-              c.wide_h, steps, wave, FEW_WAVES, re[x], columns + x * steps * 64);
+        const int column = min(x * 16 + (lane & 15), width - 1);
+        mine[x] = columns + (lane >> 4) * width + column;
+        re[x] = exponents[column / N];
     }
-    __syncthreads();
 
     float4v acc[CT];
 #pragma unroll
@@ -395,8 +440,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 4) void k_fourbit_few(FourbitCall c
 #pragma unroll
                 for (int x = 0; x < CT; ++x)
                     acc[x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                        a, columns[(x * steps + (at.quad * 4 + i) * 4 + j) * 64 + lane], acc[x], 0,
-                        0, 0);
+                        a, mine[x][((at.quad * 4 + i) * 4 + j) * 4 * width], acc[x], 0, 0, 0);
             }
         }
         if (at.quad + 1 == last && ks == 1) {
@@ -547,14 +591,20 @@ size_t column_bytes(const FourbitCall &c, size_t rows) {
     return (rows * (c.bf16 ? 1 : 2) + 15) / 16 * c.shape.blocks * 4096;
 }
 
-// The columns that fit LDS beside the wavefronts' maxima.
-constexpr size_t FEW_LDS = 150 << 10;
 template <typename T> int64_t column_tiles(const FourbitCall &c) {
     return (c.rows * TERMS<T> + 15) / 16;
 }
+// LDS of the columns, or of the wavefronts' sums or maxima in their place.
+constexpr size_t FEW_LDS = 159 << 10;
+size_t few_lds(const FourbitCall &c) {
+    const size_t width = (size_t)c.rows * (c.bf16 ? 1 : 2);
+    return FEW_HEAD + std::max(width * c.shape.blocks * (BLOCK * 2),
+                               (size_t)FEW_WAVES * ((width + 15) / 16 == 1 ? 1 : 2) * 1024);
+}
+constexpr int FEW_TILES = 2;
 bool few(const FourbitCall &c) {
-    const int64_t tiles = c.bf16 ? column_tiles<__bf16>(c) : column_tiles<float>(c);
-    return tiles <= 4 && (size_t)(tiles == 3 ? 4 : tiles) * c.shape.blocks * 4096 <= FEW_LDS;
+    return (c.bf16 ? column_tiles<__bf16>(c) : column_tiles<float>(c)) <= FEW_TILES &&
+           few_lds(c) <= FEW_LDS;
 }
 
 template <typename T, int CT, int PER> hipError_t run_few(hipStream_t st, const FourbitCall &c) {
@@ -563,17 +613,16 @@ template <typename T, int CT, int PER> hipError_t run_few(hipStream_t st, const 
     if (e != hipSuccess) return e;
     const int64_t tiles = (c.shape.classes + TILE - 1) / TILE;
     const int quads = (c.shape.blocks + 3) / 4;
-    // wavefronts a tile: as many as leave each CU a workgroup
+    const size_t lds = few_lds(c);
+    const int64_t most = (int64_t)c.num_cus * (lds <= (80 << 10) ? 2 : 1);      // workgroups at once
+    // wavefronts a tile: as many as fill them
     int ks = 1;
-    while (ks < FEW_WAVES && 2 * ks <= quads && tiles * ks < (int64_t)FEW_WAVES * c.num_cus) ks *= 2;
+    while (ks < FEW_WAVES && 2 * ks <= quads && 2 * ks * tiles <= most * FEW_WAVES) ks *= 2;
     const int64_t groups = (tiles * ks + FEW_WAVES - 1) / FEW_WAVES;
-    const size_t columns = (size_t)CT * c.shape.blocks * 4096;
-    const size_t lds = (size_t)FEW_WAVES * CT * 64 +
-                       std::max<size_t>(columns, ks > 1 ? (size_t)FEW_WAVES * CT * 1024 : 0);
-    const int64_t most = (int64_t)c.num_cus * (lds <= (80 << 10) ? 2 : 1);
-    hipLaunchKernelGGL((k_fourbit_few<T, CT, PER>),
-                       dim3((uint32_t)(ks > 1 ? groups : std::min(groups, most))),
-                       dim3(64 * FEW_WAVES), lds, st, c, ks);
+    int log2_rows = 0;
+    while ((1 << log2_rows) < c.rows) ++log2_rows;
+    hipLaunchKernelGGL((k_fourbit_few<T, CT, PER>), dim3((uint32_t)std::min(groups, most)),
+                       dim3(FEW_THREADS), lds, st, c, ks, log2_rows);
     return hipGetLastError();
 }
 
@@ -593,8 +642,7 @@ hipError_t run_tiles(hipStream_t st, const FourbitCall &c, const half8 *columns,
 template <typename T, int PER> hipError_t run(hipStream_t st, const FourbitCall &c, char *scratch) {
     const int64_t tiles = column_tiles<T>(c);
     if (few(c))
-        return tiles <= 1 ? run_few<T, 1, PER>(st, c)
-                          : tiles <= 2 ? run_few<T, 2, PER>(st, c) : run_few<T, 4, PER>(st, c);
+        return tiles <= 1 ? run_few<T, 1, PER>(st, c) : run_few<T, 2, PER>(st, c);
     half8 *columns = reinterpret_cast<half8 *>(scratch);
     const int steps = c.shape.blocks * 4;
     int32_t *e = reinterpret_cast<int32_t *>(scratch + column_bytes(c, (size_t)c.rows));
