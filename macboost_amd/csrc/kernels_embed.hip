@@ -99,7 +99,8 @@ __global__ __launch_bounds__(256) void k_embed(EmbedCall c, int32_t chunks) {
 //
 // A pass of the sort by up to 10 bits takes two launches: counts a workgroup, and the
 // placement, in which each workgroup sums up the counts before its own (at most 256
-// workgroups' of 1024, from L2) and writes runs of 2 to 16 pairs that it has ordered in LDS.
+// workgroups' of 1024, from L2, 16 bytes a lane) and writes runs of 2 to 16 pairs that it has
+// ordered in LDS.
 // ---------------------------------------------------------------------------
 constexpr int SORT_THREADS = 512, SORT_WAVES = SORT_THREADS / 64;
 constexpr int MOST_UNITS = 256;
@@ -156,7 +157,7 @@ struct Pass {
     uint32_t *key_out, *row_out;
     int64_t rows, per;               // rows a workgroup
     int32_t units, shift, bits;
-    uint32_t *table;                 // [workgroup][digit]
+    void *table;                     // [workgroup][digit], of the kernels' type of count
     uint32_t *zero;                  // a word that the placement clears
 };
 
@@ -164,7 +165,8 @@ __device__ __forceinline__ uint32_t key_at(const Pass &p, int64_t i) {
     return p.ids ? key_of(p.ids, p.entries, i) : p.key_in[i];
 }
 
-template <int R>
+// C: 16 bits where a workgroup has fewer than 2^16 rows.
+template <int R, typename C>
 __global__ __launch_bounds__(SORT_THREADS) void k_embed_count(Pass p) {
     __shared__ uint32_t count[1 << MOST_BITS];
     const int bins = 1 << p.bits;
@@ -184,11 +186,59 @@ __global__ __launch_bounds__(SORT_THREADS) void k_embed_count(Pass p) {
                 atomicAdd(&count[(key[q] >> p.shift) & (bins - 1)], 1u);
     }
     __syncthreads();
-    for (int d = threadIdx.x; d < bins; d += SORT_THREADS)
-        p.table[(int64_t)blockIdx.x * bins + d] = count[d];
+    C *to = static_cast<C *>(p.table) + (int64_t)blockIdx.x * bins;
+    for (int d = threadIdx.x; d < bins; d += SORT_THREADS) to[d] = (C)count[d];
 }
 
-template <int R>
+// next[d]: the place of this workgroup's first row of digit d.
+template <typename C>
+__device__ __forceinline__ void first_places(const Pass &p, int bins, uint32_t *next,
+                                             uint32_t *total, uint32_t *wave_sum) {
+    constexpr int E = 16 / sizeof(C);
+    typedef C V __attribute__((ext_vector_type(E)));
+    for (int d = threadIdx.x; d < bins; d += SORT_THREADS) next[d] = total[d] = 0;
+    __syncthreads();
+    const int wide = bins / E, col = threadIdx.x & (wide - 1);
+    const int group = threadIdx.x / wide, groups = SORT_THREADS / wide;
+    const V *table = static_cast<const V *>(p.table) + col;
+    uint32_t before[E], all[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) before[e] = all[e] = 0;
+    for (int u0 = group; u0 < p.units; u0 += 8 * groups) {
+        V c[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            const int u = u0 + q * groups;
+            c[q] = table[(int64_t)min(u, p.units - 1) * wide];
+        }
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            const int u = u0 + q * groups;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                all[e] += u < p.units ? c[q][e] : 0;
+                before[e] += u < (int)blockIdx.x ? c[q][e] : 0;
+            }
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        atomicAdd(&next[col * E + e], before[e]);
+        atomicAdd(&total[col * E + e], all[e]);
+    }
+    __syncthreads();
+    uint32_t sum, below = 0;
+    for (int d0 = 0; d0 < bins; d0 += SORT_THREADS) {
+        const int d = d0 + threadIdx.x;
+        const uint32_t at =
+            below + sum_before<SORT_WAVES>(d < bins ? total[d] : 0, wave_sum, sum);
+        if (d < bins) next[d] += at;
+        below += sum;
+    }
+    __syncthreads();
+}
+
+template <int R, typename C>
 __global__ __launch_bounds__(SORT_THREADS) void k_embed_place(Pass p) {
     extern __shared__ uint32_t lds[];
     const int bins = 1 << p.bits;
@@ -200,26 +250,8 @@ __global__ __launch_bounds__(SORT_THREADS) void k_embed_place(Pass p) {
     uint32_t *count = row_staged + CHUNK<R>;         // [wave][digit]
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     if (blockIdx.x == 0 && threadIdx.x == 0) *p.zero = 0;
-    uint32_t all, below = 0;
-    for (int d0 = 0; d0 < bins; d0 += SORT_THREADS) {
-        const int d = d0 + threadIdx.x;
-        uint32_t before = 0, total = 0;
-        if (d < bins)
-            for (int u0 = 0; u0 < p.units; u0 += 8) {
-                uint32_t c[8];
-#pragma unroll
-                for (int q = 0; q < 8; ++q)
-                    c[q] = u0 + q < p.units ? p.table[(int64_t)(u0 + q) * bins + d] : 0;
-#pragma unroll
-                for (int q = 0; q < 8; ++q) {
-                    total += c[q];
-                    if (u0 + q < (int)blockIdx.x) before += c[q];
-                }
-            }
-        const uint32_t at = below + sum_before<SORT_WAVES>(total, wave_sum, all);
-        if (d < bins) next[d] = at + before;
-        below += all;
-    }
+    uint32_t all;
+    first_places<C>(p, bins, next, first, wave_sum);
     const int64_t a = blockIdx.x * p.per, b = min(p.rows, a + p.per);
     for (int64_t c = a; c < b; c += CHUNK<R>) {
         // wavefront by wavefront, so that equal digits keep their order
@@ -288,7 +320,8 @@ __global__ __launch_bounds__(SORT_THREADS) void k_embed_place(Pass p) {
 }
 
 // Few rows: the whole sort by one workgroup in one launch.
-constexpr int SMALL_WAVES = 16, SMALL_THREADS = 64 * SMALL_WAVES, SMALL_EACH = 16;
+// (16384 rows of 17 bits take 46 us so, 20 by the kernels above.)
+constexpr int SMALL_WAVES = 16, SMALL_THREADS = 64 * SMALL_WAVES, SMALL_EACH = 4;
 constexpr int64_t SMALL_ROWS = SMALL_THREADS * SMALL_EACH;
 constexpr int SMALL_BITS = 8;
 __global__ __launch_bounds__(SMALL_THREADS) void k_embed_sort_small(Pass p, int32_t passes) {
@@ -367,10 +400,11 @@ __global__ __launch_bounds__(SMALL_THREADS) void k_embed_sort_small(Pass p, int3
 
 // ---------------------------------------------------------------------------
 // The sums.  The sorted rows and the table's entries are merged: entry e comes behind the
-// rows of key e.  A worker, `lanes` lanes that hold E columns each, takes `per` items of that
-// list: it adds the rows and writes the entries, zeros for those without rows, so that rows and
-// entries weigh the same whatever the ids.  (Without entries, where dtable is its own base, the
-// list is the rows.)
+// rows of key e, so that row i of key k lies at i + k.  A worker, `lanes` lanes that hold E columns
+// each, takes `per` items of that list: it adds the rows and writes the entries, zeros for those
+// without rows, so that rows and entries weigh the same whatever the ids, and what both read
+// (an entry its base) is on the way AHEAD items at a time.  Where dtable is its own base, entries
+// without rows are not on the list, and a worker takes `per` rows.
 //
 // A worker's end that falls into an entry's rows is put behind them if they are at most SHORT;
 // else the entry is longer than a worker: each of its workers leaves its sum in parts, and the
@@ -380,7 +414,9 @@ __global__ __launch_bounds__(SMALL_THREADS) void k_embed_sort_small(Pass p, int3
 constexpr int SUM_WAVES = 4, SUM_THREADS = 64 * SUM_WAVES;
 constexpr int SHORT = 64;            // rows
 constexpr int MOST_ITEMS = 4096;     // of a workgroup
-constexpr int AHEAD = 8;             // rows on the way
+constexpr int AHEAD = 8;             // items on the way
+constexpr uint32_t ENTRY = 0x80000000u;      // an item that is an entry: which, if not all are there
+constexpr uint32_t NOTHING = 0xFFFFFFFFu;
 
 struct Sums {
     int64_t rows, workers;
@@ -388,18 +424,21 @@ struct Sums {
     int32_t dim, chunks;             // pieces of E columns
     int32_t lanes, groups;           // of a worker; workers a wavefront
     int32_t per;
-    bool dense;                      // entries without rows are written
+    bool dense;                      // entries without rows are on the list
     int64_t row_stride, table_stride;
     float scale;
     const uint32_t *key, *row;
     const void *dout, *base;
     void *dtable;
-    float *parts;                    // [worker][head, tail][dim]
+    int32_t part_stride;             // dim in whole fours
+    float *parts;                    // [worker][head, tail][part_stride]
+    uint32_t *open;                  // [worker] the entry that it leaves open, or NOTHING
     uint32_t *found;                 // [0]: how many; then (worker, entry)
 };
+// Rows that a workgroup of `items` items may look at.
+__host__ __device__ constexpr int held_rows(int items) { return items + 2 * SHORT + 2; }
 
-// Rows of the sorted list and entries before an item of the merged one, in which row i of key
-// k lies at i + k.  i counts from the first row that the workgroup holds in LDS.
+// Rows and entries before an item.  i counts from the first row that the workgroup holds in LDS.
 struct Cut {
     int i;
     uint32_t e;
@@ -444,182 +483,236 @@ __device__ __forceinline__ Cut cut_at(const Sums &s, const uint32_t *key, int64_
     return c;
 }
 
+// 256-ary search: the number of rows i with i + key[i] below d[0] and d[1], of [lo, hi] both.
+__device__ __forceinline__ void both_ends(const Sums &s, const int64_t (&d)[2], int64_t *found) {
+    int64_t lo[2], hi[2];
+    for (int x = 0; x < 2; ++x) {
+        lo[x] = max((int64_t)0, d[x] - (int64_t)s.entries);
+        hi[x] = min(s.rows, d[x]);
+    }
+    while (hi[0] > lo[0] || hi[1] > lo[1]) {
+        uint32_t k[2];
+        int64_t m[2], step[2];
+        bool in[2];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            step[x] = (hi[x] - lo[x] + SUM_THREADS - 1) / SUM_THREADS;
+            m[x] = lo[x] + threadIdx.x * step[x];
+            in[x] = m[x] < hi[x];
+            k[x] = in[x] ? s.key[m[x]] : 0;
+        }
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const int n = __syncthreads_count(in[x] && m[x] + (int64_t)k[x] < d[x]);
+            if (n == 0) {
+                hi[x] = lo[x];
+                continue;
+            }
+            const int64_t last = lo[x] + (n - 1) * step[x];
+            hi[x] = min(hi[x], last + step[x]);
+            lo[x] = last + 1;
+        }
+    }
+    found[0] = lo[0];
+    found[1] = lo[1];
+}
+
+// E elements as they lie in memory; those behind the n-th are 0.
+template <typename T, int E> using Raw = T __attribute__((ext_vector_type(E)));
+template <typename T, int E>
+__device__ __forceinline__ Raw<T, E> load_raw(const T *p, int n) {
+    if (n >= E) return *reinterpret_cast<const Raw<T, E> *>(p);
+    Raw<T, E> v;
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = e < n ? p[e] : (T)0.0f;
+    return v;
+}
+
 template <typename T, int E>
 __global__ __launch_bounds__(SUM_THREADS) void k_embed_sum(Sums s) {
     extern __shared__ uint32_t lds[];
-    __shared__ int64_t ends[2];
+    __shared__ uint32_t wave_sum[SUM_WAVES];
+    const int items = SUM_WAVES * s.groups * s.per, most = held_rows(items);
+    uint32_t *key = lds;                             // [row]
+    uint32_t *item = key + most;                     // [item]: a row, or an entry
+    uint32_t *place = item + 2 * most;               // [row] its item, where it is not i + key
     const int64_t first = (int64_t)group_id() * (SUM_WAVES * s.groups);
     if (first >= s.workers) return;
-    // the rows of the workgroup's items: 256-ary search for both ends
-    const int64_t d0 = first * s.per;
-    const int64_t d1 = min(min(first + SUM_WAVES * s.groups, s.workers) * s.per,
-                           s.rows + (s.dense ? (int64_t)s.entries : 0));
-    if (!s.dense) {
-        if (threadIdx.x < 2) ends[threadIdx.x] = threadIdx.x ? d1 : d0;
-    } else {
-        for (int side = 0; side < 2; ++side) {
-            const int64_t d = side ? d1 : d0;
-            int64_t lo = max((int64_t)0, d - (int64_t)s.entries), hi = min(s.rows, d);
-            while (hi > lo) {                            // the answer is in [lo, hi]
-                const int64_t step = (hi - lo + SUM_THREADS - 1) / SUM_THREADS;
-                const int64_t m = lo + threadIdx.x * step;
-                const bool under = m < hi && m + (int64_t)s.key[m] < d;
-                const int n = __syncthreads_count(under);
-                if (n == 0) {
-                    hi = lo;
-                    break;
-                }
-                const int64_t last = lo + (n - 1) * step;
-                lo = last + 1;
-                hi = min(hi, last + step);
-            }
-            if (threadIdx.x == 0) ends[side] = lo;
+    const int64_t d[2] = {first * s.per, min(min(first + SUM_WAVES * s.groups, s.workers) * s.per,
+                                             s.rows + (s.dense ? (int64_t)s.entries : 0))};
+    int64_t ends[2] = {d[0], d[1]};
+    if (s.dense) both_ends(s, d, ends);
+    const int64_t begin = max((int64_t)0, ends[0] - SHORT - 1);
+    const int held = (int)(min(s.rows, ends[1] + SHORT + 1) - begin);
+    const int lo = (int)(ends[0] - begin), hi = (int)(ends[1] - begin);
+    if (s.dense) {
+        for (int i = threadIdx.x; i < items + SHORT + 2; i += SUM_THREADS) item[i] = ENTRY;
+        __syncthreads();
+        for (int i = threadIdx.x; i < held; i += SUM_THREADS) {
+            const uint32_t k = s.key[begin + i], r = s.row[begin + i];
+            key[i] = k;
+            const int64_t at = begin + i + (int64_t)k - d[0];
+            if (at >= 0 && at < items + SHORT + 2 && k < s.entries) item[at] = r;
         }
-    }
-    __syncthreads();
-    const int64_t lo = ends[0], hi = ends[1];
-    const int64_t begin = max((int64_t)0, lo - SHORT - 1), end = min(s.rows, hi + SHORT + 1);
-    uint32_t *key = lds;
-    uint32_t *row = lds + (SUM_WAVES * s.groups * s.per + 2 * SHORT + 2);
-    for (int64_t i = begin + threadIdx.x; i < end; i += SUM_THREADS) {
-        key[i - begin] = s.key[i];
-        row[i - begin] = s.row[i];
+    } else {
+        for (int i = threadIdx.x; i < held; i += SUM_THREADS) key[i] = s.key[begin + i];
+        __syncthreads();
+        // a row's item lies behind as many entries as end before it
+        uint32_t before = 0, all;
+        for (int i0 = 0; i0 < held; i0 += SUM_THREADS) {
+            const int i = i0 + threadIdx.x;
+            const uint32_t k = i < held ? key[i] : NOTHING;
+            const bool ends_here = k < s.entries && (begin + i + 1 >= s.rows ||
+                                                     (i + 1 < held && key[i + 1] != k));
+            const uint32_t at = i + before + sum_before<SUM_WAVES>(ends_here, wave_sum, all);
+            if (i < held) {
+                place[i] = at;
+                item[at] = k < s.entries ? s.row[begin + i] : NOTHING;
+                if (ends_here) item[at + 1] = ENTRY | k;
+            }
+            before += all;
+        }
+        if (threadIdx.x == 0) place[held] = held + before;
     }
     __syncthreads();
     const int lane = threadIdx.x & 63, group = lane / s.lanes;
     const int64_t worker = first + (threadIdx.x >> 6) * s.groups + group;
     const int32_t chunk = blockIdx.y * 64 + lane - group * s.lanes;
     if (group >= s.groups || worker >= s.workers || chunk >= s.chunks) return;
-    const int held = (int)(end - begin), from_lo = (int)(lo - begin), to_hi = (int)(hi - begin);
-    const Cut from = cut_at(s, key, begin, held, from_lo, to_hi, worker * s.per);
-    const Cut to = cut_at(s, key, begin, held, from_lo, to_hi, (worker + 1) * s.per);
+    const Cut from = cut_at(s, key, begin, held, lo, hi, worker * s.per);
+    const Cut to = cut_at(s, key, begin, held, lo, hi, (worker + 1) * s.per);
     const int col = chunk * E, n = s.dim - col;
     const T *dout = static_cast<const T *>(s.dout) + col;
-    const T *base = static_cast<const T *>(s.base);
+    const T *base = s.base ? static_cast<const T *>(s.base) + col : nullptr;
     T *dtable = static_cast<T *>(s.dtable) + col;
-    if (base) base += col;
 
     float acc[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = 0.0f;
-    uint32_t next = from.e;          // the next entry to write
-    bool has = from.open, head = from.open;
-    // Writes entry e = base + scale * acc.
-    const auto write = [&](uint32_t e) {
-        float v[E], b[E];
-#pragma unroll
-        for (int x = 0; x < E; ++x) b[x] = 0.0f;
-        if (base) load<T, E>(base + (int64_t)e * s.table_stride, n, b);
-#pragma unroll
-        for (int x = 0; x < E; ++x) v[x] = __builtin_fmaf(s.scale, acc[x], b[x]);
-        store<T, E>(dtable + (int64_t)e * s.table_stride, n, v);
-    };
+    bool head = from.open;
     const auto leave = [&](int side) {
-        float *p = s.parts + (worker * 2 + side) * s.dim + col;
+        float *p = s.parts + (worker * 2 + side) * s.part_stride + col;
 #pragma unroll
         for (int e = 0; e < E; ++e)
             if (e < n) p[e] = acc[e];
     };
-    // The entry `next`, whose rows are all added.
-    const auto finish = [&]() {
-        if (head) {
-            leave(0);
-            if (chunk == 0) {
-                const uint32_t at = atomicAdd(&s.found[0], 1u);
-                s.found[2 + 2 * at] = (uint32_t)worker;
-                s.found[3 + 2 * at] = next;
-            }
-            head = false;
-        } else {
-            write(next);
-        }
-#pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] = 0.0f;
-        has = false;
-        ++next;
-    };
-    for (int i = from.i; i < to.i; i += AHEAD) {
-        float v[AHEAD][E];
+    uint32_t next = from.e;          // the next entry, where all are on the list
+    int p = s.dense ? (int)(begin + from.i + (int64_t)from.e - d[0]) : (int)place[from.i];
+    const int end = s.dense ? (int)(begin + to.i + (int64_t)to.e - d[0]) : (int)place[to.i];
+    for (; p < end; p += AHEAD) {
+        uint32_t what[AHEAD];
+        Raw<T, E> v[AHEAD];
+        uint32_t e = next;
 #pragma unroll
         for (int q = 0; q < AHEAD; ++q) {
-            const bool here = i + q < to.i && key[i + q] < s.entries;
-            load<T, E>(dout + (here ? row[i + q] * s.row_stride : 0), here ? n : 0, v[q]);
+            what[q] = p + q < end ? item[p + q] : NOTHING;
+            if (s.dense && what[q] == ENTRY) {
+                what[q] = e < s.entries ? ENTRY | e : NOTHING;       // behind all: left out
+                ++e;
+            }
         }
 #pragma unroll
         for (int q = 0; q < AHEAD; ++q) {
-            if (i + q >= to.i) break;
-            const uint32_t k = key[i + q];
-            if (k >= s.entries) break;                   // left out, as are all behind
-            if (k != next || !has) {
-                if (has) finish();
-                if (s.dense)
-                    while (next < k) finish();
-                next = k;
-                has = true;
+            const bool is_row = what[q] < ENTRY;
+            const int64_t at = is_row ? what[q] * s.row_stride
+                                      : (int64_t)(what[q] & ~ENTRY) * s.table_stride;
+            const bool read = is_row || (what[q] != NOTHING && base);
+            v[q] = load_raw<T, E>((is_row ? dout : base) + (read ? at : 0), read ? n : 0);
+        }
+#pragma unroll
+        for (int q = 0; q < AHEAD; ++q) {
+            if (what[q] == NOTHING) continue;
+            if (what[q] < ENTRY) {
+#pragma unroll
+                for (int x = 0; x < E; ++x) acc[x] += to_f32(v[q][x]);
+                continue;
+            }
+            const uint32_t entry = what[q] & ~ENTRY;
+            if (head) {
+                leave(0);
+                if (chunk == 0) {
+                    const uint32_t at = atomicAdd(&s.found[0], 1u);
+                    s.found[2 + 2 * at] = (uint32_t)worker;
+                    s.found[3 + 2 * at] = entry;
+                }
+                head = false;
+            } else {
+                float out[E];
+#pragma unroll
+                for (int x = 0; x < E; ++x)
+                    out[x] = __builtin_fmaf(s.scale, acc[x], base ? to_f32(v[q][x]) : 0.0f);
+                store<T, E>(dtable + entry * s.table_stride, n, out);
             }
 #pragma unroll
-            for (int e = 0; e < E; ++e) acc[e] += v[q][e];
+            for (int x = 0; x < E; ++x) acc[x] = 0.0f;
         }
+        next = e;
     }
-    if (to.open && (has ? next : from.e) == to.e) {
-        leave(1);
-        return;
-    }
-    if (has) finish();
-    if (s.dense)
-        while (next < to.e) finish();
+    if (to.open) leave(1);
+    if (chunk == 0) s.open[worker] = to.open ? to.e : NOTHING;
 }
 
-// The entries on the list: heads and tails of their workers.  A workgroup an entry; slices of
-// its workers are summed side by side, and the slices' sums in their order.
-constexpr int JOIN_WAVES = 8, JOIN_THREADS = 64 * JOIN_WAVES;
+// The entries on the list: heads and tails of their workers, from the first that left the entry
+// open to the one in which it ends.  A workgroup an entry; slices of its workers are summed side
+// by side, and the slices' sums in their order.
+constexpr int JOIN_WAVES = 4, JOIN_THREADS = 64 * JOIN_WAVES;
 template <typename T>
 __global__ __launch_bounds__(JOIN_THREADS) void k_embed_join(Sums s) {
-    __shared__ float sums[JOIN_THREADS];
+    typedef float V __attribute__((ext_vector_type(4)));
+    __shared__ V sums[JOIN_THREADS];
     const uint32_t count = s.found[0];
-    const int wide = min(s.dim, 64), groups = 64 / wide, slices = JOIN_WAVES * groups;
+    const int fours = s.part_stride / 4, wide = min(fours, 64), groups = 64 / wide;
+    const int slices = JOIN_WAVES * groups;
     const int lane = threadIdx.x & 63, group = lane / wide;
     const int slice = (threadIdx.x >> 6) * groups + group, col0 = lane - group * wide;
     for (uint32_t f = blockIdx.x; f < count; f += gridDim.x) {
         const int64_t last = s.found[2 + 2 * f];
         const uint32_t entry = s.found[3 + 2 * f];
-        int64_t lo = 0, hi = s.rows;                     // the entry's first row
-        while (hi > lo) {
-            const int64_t step = (hi - lo + JOIN_THREADS - 1) / JOIN_THREADS;
-            const int64_t m = lo + threadIdx.x * step;
-            const int n = __syncthreads_count(m < hi && s.key[m] < entry);
-            if (n == 0) break;
-            const int64_t at = lo + (n - 1) * step;
-            lo = at + 1;
-            hi = min(hi, at + step);
+        int64_t start = last;
+        for (;;) {
+            const int64_t w = start - 1 - threadIdx.x;
+            const bool same = w >= 0 && s.open[w] == entry;
+            // workers that left the entry open lie side by side
+            const int n = __syncthreads_count(same);
+            start -= n;
+            if (n < JOIN_THREADS) break;
         }
-        const int64_t start = (lo + (s.dense ? (int64_t)entry : 0)) / s.per;
         const int64_t each = (last - start + slices) / slices;      // of last - start + 1 parts
         const int64_t a = start + slice * each, b = min(a + each, last + 1);
-        for (int c0 = 0; c0 < s.dim; c0 += wide) {
-            const int col = c0 + col0;
-            float sum = 0.0f;
-            if (group < groups && col < s.dim)
+        for (int c0 = 0; c0 < fours; c0 += wide) {
+            const int col = (c0 + col0) * 4;
+            V sum = {0, 0, 0, 0};
+            if (group < groups && c0 + col0 < fours)
                 for (int64_t w = a; w < b; w += AHEAD) {
-                    float v[AHEAD];
+                    V v[AHEAD];
+#pragma unroll
+                    for (int q = 0; q < AHEAD; ++q) {
+                        const int64_t x = min(w + q, b - 1);
+                        v[q] = *reinterpret_cast<const V *>(
+                            s.parts + (x * 2 + (x < last)) * s.part_stride + col);
+                    }
 #pragma unroll
                     for (int q = 0; q < AHEAD; ++q)
-                        v[q] = w + q < b
-                                   ? s.parts[((w + q) * 2 + (w + q < last)) * s.dim + col] : 0.0f;
 #pragma unroll
-                    for (int q = 0; q < AHEAD; ++q) sum += v[q];
+                        for (int e = 0; e < 4; ++e) sum[e] += w + q < b ? v[q][e] : 0.0f;
                 }
             sums[threadIdx.x] = sum;
             __syncthreads();
-            if (threadIdx.x < (unsigned)wide && col < s.dim) {
-                float total = 0.0f;
-                for (int v = 0; v < slices; ++v)
-                    total += sums[(v / groups) * 64 + (v % groups) * wide + col0];
-                T *to = static_cast<T *>(s.dtable) + (int64_t)entry * s.table_stride + col;
-                const float b0 = s.base ? to_f32(static_cast<const T *>(
-                                              s.base)[(int64_t)entry * s.table_stride + col])
-                                        : 0.0f;
-                *to = (T)__builtin_fmaf(s.scale, total, b0);
+            if (threadIdx.x < (unsigned)wide && c0 + col0 < fours) {
+                V total = {0, 0, 0, 0};
+                for (int v = 0; v < slices; ++v) {
+                    const V part = sums[(v / groups) * 64 + (v % groups) * wide + col0];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) total[e] += part[e];
+                }
+                const int64_t at = (int64_t)entry * s.table_stride + col;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (col + e < s.dim) {
+                        const float b0 = s.base ? to_f32(static_cast<const T *>(s.base)[at + e]) : 0.0f;
+                        static_cast<T *>(s.dtable)[at + e] =
+                            (T)__builtin_fmaf(s.scale, total[e], b0);
+                    }
             }
             __syncthreads();
         }
@@ -641,6 +734,7 @@ struct GradShape {
     bool small;
     int64_t per;                     // rows a workgroup of the sort, or a wavefront
     int each;                        // R
+    bool narrow;                     // counts of 16 bits
     int lanes, groups, cols, items, chunks;
     int elements;                    // E
     bool dense;
@@ -653,7 +747,7 @@ GradShape grad_shape(const EmbedCall &c) {
     g.small = c.rows <= SMALL_ROWS;
     const int most = g.small ? SMALL_BITS : MOST_BITS;
     g.passes = (bits + most - 1) / most;
-    g.bits = (bits + g.passes - 1) / g.passes;
+    g.bits = std::max(3, (bits + g.passes - 1) / g.passes);      // 16 bytes of counts
     if (g.small) {
         g.per = ((c.rows + SMALL_WAVES - 1) / SMALL_WAVES + 63) / 64 * 64;
         g.units = 1;
@@ -663,6 +757,7 @@ GradShape grad_shape(const EmbedCall &c) {
         const int64_t chunks = (c.rows + chunk - 1) / chunk;
         g.per = (chunks + MOST_UNITS - 1) / MOST_UNITS * chunk;
         g.units = (int)((c.rows + g.per - 1) / g.per);
+        g.narrow = g.per < (1 << 16);
     }
     const size_t size = c.bf16 ? 2 : 4;
     const bool wide = aligned(c.dout, c.row_stride, size) && aligned(c.dtable, c.table_stride, size) &&
@@ -684,14 +779,29 @@ GradShape grad_shape(const EmbedCall &c) {
 }
 
 size_t rounded(size_t bytes) { return (bytes + 255) / 256 * 256; }
+size_t table_bytes(const GradShape &g) {
+    return rounded(g.small ? 0 : ((size_t)g.units << g.bits) * (g.narrow ? 2 : 4));
+}
+int32_t part_stride(const EmbedCall &c) { return (c.dim + 3) / 4 * 4; }
+
+template <int R, typename C>
+hipError_t sort_pass(hipStream_t st, const Pass &p) {
+    const hipError_t e = allow_all_lds(reinterpret_cast<const void *>(k_embed_place<R, C>));
+    if (e != hipSuccess) return e;
+    const dim3 grid((uint32_t)p.units), block(SORT_THREADS);
+    const size_t lds = 4 * (SORT_WAVES + ((size_t)(2 + SORT_WAVES) << p.bits) + 2 * CHUNK<R>);
+    hipLaunchKernelGGL((k_embed_count<R, C>), grid, block, 0, st, p);
+    hipLaunchKernelGGL((k_embed_place<R, C>), grid, block, lds, st, p);
+    return hipGetLastError();
+}
 
 template <typename T, int E>
 hipError_t sums(hipStream_t st, const Sums &s, int cols, int num_cus) {
     const int64_t each = SUM_WAVES * s.groups;
     dim3 g = grid_of((s.workers + each - 1) / each, (uint32_t)cols);
-    const size_t lds = 2 * sizeof(uint32_t) * (each * s.per + 2 * SHORT + 2);
+    const size_t lds = sizeof(uint32_t) * (4 * (size_t)held_rows((int)each * s.per) + 1);
     hipLaunchKernelGGL((k_embed_sum<T, E>), g, dim3(SUM_THREADS), lds, st, s);
-    hipLaunchKernelGGL((k_embed_join<T>), dim3((uint32_t)(2 * num_cus)), dim3(JOIN_THREADS), 0, st,
+    hipLaunchKernelGGL((k_embed_join<T>), dim3((uint32_t)(4 * num_cus)), dim3(JOIN_THREADS), 0, st,
                        s);
     return hipGetLastError();
 }
@@ -718,9 +828,9 @@ hipError_t launch_embed(hipStream_t s, const EmbedCall &c) {
 size_t embed_grad_scratch(const EmbedCall &c) {
     const GradShape g = grad_shape(c);
     const size_t rows = rounded((size_t)c.rows * 4);
-    return (g.small || g.passes < 2 ? 2 : 4) * rows +
-           rounded(g.small ? 0 : ((size_t)g.units << g.bits) * 4) + rounded(8 + 8 * (size_t)g.workers) +
-           rounded(8 * (size_t)g.workers * c.dim);
+    return (g.small || g.passes < 2 ? 2 : 4) * rows + table_bytes(g) +
+           rounded(4 * (size_t)g.workers) + rounded(8 + 8 * (size_t)g.workers) +
+           rounded(8 * (size_t)g.workers * part_stride(c));
 }
 
 hipError_t launch_embed_grad(hipStream_t st, const EmbedCall &c, char *scratch) {
@@ -733,11 +843,14 @@ hipError_t launch_embed_grad(hipStream_t st, const EmbedCall &c, char *scratch) 
         row[i] = reinterpret_cast<uint32_t *>(scratch + rows);
         scratch += 2 * rows;
     }
-    uint32_t *table = reinterpret_cast<uint32_t *>(scratch);
-    scratch += rounded(g.small ? 0 : ((size_t)g.units << g.bits) * 4);
+    void *table = scratch;
+    scratch += table_bytes(g);
     Sums s{};
+    s.open = reinterpret_cast<uint32_t *>(scratch);
+    scratch += rounded(4 * (size_t)g.workers);
     s.found = reinterpret_cast<uint32_t *>(scratch);
     s.parts = reinterpret_cast<float *>(scratch + rounded(8 + 8 * (size_t)g.workers));
+    s.part_stride = part_stride(c);
     Pass p{};
     p.entries = (uint32_t)c.entries;
     p.rows = c.rows;
@@ -756,14 +869,6 @@ hipError_t launch_embed_grad(hipStream_t st, const EmbedCall &c, char *scratch) 
         const size_t lds = 4 * (SMALL_WAVES + ((size_t)SMALL_WAVES << g.bits) + c.rows) + 2 * c.rows;
         hipLaunchKernelGGL(k_embed_sort_small, dim3(1), dim3(SMALL_THREADS), lds, st, p, g.passes);
     } else {
-        for (const void *f : {reinterpret_cast<const void *>(k_embed_place<4>),
-                              reinterpret_cast<const void *>(k_embed_place<8>)}) {
-            const hipError_t e = allow_all_lds(f);
-            if (e != hipSuccess) return e;
-        }
-        const dim3 grid((uint32_t)g.units), block(SORT_THREADS);
-        const size_t lds = 4 * (SORT_WAVES + ((size_t)(2 + SORT_WAVES) << g.bits) +
-                                2 * (size_t)SORT_THREADS * g.each);
         for (int i = 0; i < g.passes; ++i) {
             to = i & 1;
             p.ids = i == 0 ? c.ids : nullptr;
@@ -774,13 +879,10 @@ hipError_t launch_embed_grad(hipStream_t st, const EmbedCall &c, char *scratch) 
             p.key_out = key[to];
             p.row_out = row[to];
             p.shift = i * g.bits;
-            if (g.each == 4) {
-                hipLaunchKernelGGL(k_embed_count<4>, grid, block, 0, st, p);
-                hipLaunchKernelGGL(k_embed_place<4>, grid, block, lds, st, p);
-            } else {
-                hipLaunchKernelGGL(k_embed_count<8>, grid, block, 0, st, p);
-                hipLaunchKernelGGL(k_embed_place<8>, grid, block, lds, st, p);
-            }
+            const hipError_t e = g.each == 4 ? sort_pass<4, uint16_t>(st, p)
+                                 : g.narrow  ? sort_pass<8, uint16_t>(st, p)
+                                             : sort_pass<8, uint32_t>(st, p);
+            if (e != hipSuccess) return e;
         }
     }
     s.rows = c.rows;
