@@ -153,8 +153,8 @@ __device__ __forceinline__ uint32_t key_of(const int32_t *ids, uint32_t entries,
 struct Pass {
     const int32_t *ids;              // the first pass's keys, else NULL
     uint32_t entries;
-    const uint32_t *key_in, *row_in;
-    uint32_t *key_out, *row_out;
+    const uint2 *in;                 // key and row
+    uint2 *out;
     int64_t rows, per;               // rows a workgroup
     int32_t units, shift, bits;
     void *table;                     // [workgroup][digit], of the kernels' type of count
@@ -162,10 +162,10 @@ struct Pass {
 };
 
 __device__ __forceinline__ uint32_t key_at(const Pass &p, int64_t i) {
-    return p.ids ? key_of(p.ids, p.entries, i) : p.key_in[i];
+    return p.ids ? key_of(p.ids, p.entries, i) : p.in[i].x;
 }
 
-// C: 16 bits where a workgroup has fewer than 2^16 rows.
+// C: 16 bits where a workgroup has fewer than 2^13 rows.
 template <int R, typename C>
 __global__ __launch_bounds__(SORT_THREADS) void k_embed_count(Pass p) {
     __shared__ uint32_t count[1 << MOST_BITS];
@@ -201,31 +201,32 @@ __device__ __forceinline__ void first_places(const Pass &p, int bins, uint32_t *
     const int wide = bins / E, col = threadIdx.x & (wide - 1);
     const int group = threadIdx.x / wide, groups = SORT_THREADS / wide;
     const V *table = static_cast<const V *>(p.table) + col;
-    uint32_t before[E], all[E];
+    uint32_t all[E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) before[e] = all[e] = 0;
-    for (int u0 = group; u0 < p.units; u0 += 8 * groups) {
-        V c[8];
+    for (int e = 0; e < E; ++e) all[e] = 0;
+    const auto add = [&](int u, int end) {
+        for (; u < end; u += 8) {
+            V c[8], sum = 0;
 #pragma unroll
-        for (int q = 0; q < 8; ++q) {
-            const int u = u0 + q * groups;
-            c[q] = table[(int64_t)min(u, p.units - 1) * wide];
-        }
-#pragma unroll
-        for (int q = 0; q < 8; ++q) {
-            const int u = u0 + q * groups;
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                all[e] += u < p.units ? c[q][e] : 0;
-                before[e] += u < (int)blockIdx.x ? c[q][e] : 0;
+            for (int q = 0; q < 8; ++q) {
+                c[q] = 0;
+                if (u + q < end) c[q] = table[(int64_t)(u + q) * wide];
             }
-        }
-    }
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        atomicAdd(&next[col * E + e], before[e]);
-        atomicAdd(&total[col * E + e], all[e]);
-    }
+            for (int q = 0; q < 8; ++q) sum += c[q];         // 8 counts of 2^13 fit 16 bits
+#pragma unroll
+            for (int e = 0; e < E; ++e) all[e] += sum[e];
+        }
+    };
+    // a run of the workgroups a group of threads: those before this one, and the others
+    const int run = (p.units + groups - 1) / groups, from = group * run;
+    const int to = min(from + run, p.units), mid = max(from, min(to, (int)blockIdx.x));
+    add(from, mid);
+#pragma unroll
+    for (int e = 0; e < E; ++e) atomicAdd(&next[col * E + e], all[e]);
+    add(mid, to);
+#pragma unroll
+    for (int e = 0; e < E; ++e) atomicAdd(&total[col * E + e], all[e]);
     __syncthreads();
     uint32_t sum, below = 0;
     for (int d0 = 0; d0 < bins; d0 += SORT_THREADS) {
@@ -245,30 +246,34 @@ __global__ __launch_bounds__(SORT_THREADS) void k_embed_place(Pass p) {
     uint32_t *wave_sum = lds;                        // SORT_WAVES
     uint32_t *next = wave_sum + SORT_WAVES;          // [digit] its next place
     uint32_t *first = next + bins;                   // [digit] its first place in the chunk
-    uint32_t *key_staged = first + bins;             // [place in the chunk]
-    uint32_t *row_staged = key_staged + CHUNK<R>;
-    uint32_t *count = row_staged + CHUNK<R>;         // [wave][digit]
+    uint2 *staged = reinterpret_cast<uint2 *>(first + bins);        // [place in the chunk]
+    uint32_t *count = reinterpret_cast<uint32_t *>(staged + CHUNK<R>);      // [wave][digit]
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     if (blockIdx.x == 0 && threadIdx.x == 0) *p.zero = 0;
-    uint32_t all;
-    first_places<C>(p, bins, next, first, wave_sum);
     const int64_t a = blockIdx.x * p.per, b = min(p.rows, a + p.per);
-    for (int64_t c = a; c < b; c += CHUNK<R>) {
-        // wavefront by wavefront, so that equal digits keep their order
-        const int64_t w = c + wave * (64 * R);
-        uint32_t key[R], row[R], rank[R];
+    uint2 pair[R];
+    // wavefront by wavefront, so that equal digits keep their order
+    const auto load_chunk = [&](int64_t c) {
 #pragma unroll
         for (int q = 0; q < R; ++q) {
-            const int64_t i = w + q * 64 + lane;
-            key[q] = i < b ? key_at(p, i) : 0;
-            row[q] = i < b ? (p.ids ? (uint32_t)i : p.row_in[i]) : 0;
+            const int64_t i = c + wave * (64 * R) + q * 64 + lane;
+            pair[q] = uint2{0, 0};
+            if (i < b) pair[q] = p.ids ? uint2{key_of(p.ids, p.entries, i), (uint32_t)i} : p.in[i];
         }
+    };
+    load_chunk(a);                                   // on the way while the counts are
+    uint32_t all;
+    first_places<C>(p, bins, next, first, wave_sum);
+    for (int64_t c = a; c < b; c += CHUNK<R>) {
+        const int64_t w = c + wave * (64 * R);
+        uint32_t rank[R];
+        if (c > a) load_chunk(c);
         for (int d = threadIdx.x; d < SORT_WAVES * bins; d += SORT_THREADS) count[d] = 0;
         __syncthreads();
         uint32_t *mine = count + wave * bins;
 #pragma unroll
         for (int q = 0; q < R; ++q) {
-            const uint32_t d = (key[q] >> p.shift) & (bins - 1);
+            const uint32_t d = (pair[q].x >> p.shift) & (bins - 1);
             const bool here = w + q * 64 + lane < b;
             const uint64_t same = same_digit(d, here, p.bits);
             const uint32_t r = lanes_below(same);
@@ -300,17 +305,13 @@ __global__ __launch_bounds__(SORT_THREADS) void k_embed_place(Pass p) {
 #pragma unroll
         for (int q = 0; q < R; ++q) {
             if (w + q * 64 + lane >= b) continue;
-            const uint32_t d = (key[q] >> p.shift) & (bins - 1);
-            const uint32_t at = first[d] + mine[d] + rank[q];
-            key_staged[at] = key[q];
-            row_staged[at] = row[q];
+            const uint32_t d = (pair[q].x >> p.shift) & (bins - 1);
+            staged[first[d] + mine[d] + rank[q]] = pair[q];
         }
         __syncthreads();
         for (uint32_t l = threadIdx.x; l < taken; l += SORT_THREADS) {
-            const uint32_t k = key_staged[l];
-            const uint32_t to = next[(k >> p.shift) & (bins - 1)] + l;
-            p.key_out[to] = k;
-            p.row_out[to] = row_staged[l];
+            const uint2 v = staged[l];
+            p.out[next[(v.x >> p.shift) & (bins - 1)] + l] = v;
         }
         __syncthreads();
         for (int d = threadIdx.x; d < bins; d += SORT_THREADS)       // the chunk is behind
@@ -393,8 +394,7 @@ __global__ __launch_bounds__(SMALL_THREADS) void k_embed_sort_small(Pass p, int3
     for (int q = 0; q < SMALL_EACH; ++q) {
         const int i = a + q * 64 + lane;
         if (i >= b) continue;
-        p.key_out[i] = key[q];
-        p.row_out[i] = row[q];
+        p.out[i] = uint2{key[q], row[q]};
     }
 }
 
@@ -406,13 +406,12 @@ __global__ __launch_bounds__(SMALL_THREADS) void k_embed_sort_small(Pass p, int3
 // (an entry its base) is on the way AHEAD items at a time.  Where dtable is its own base, entries
 // without rows are not on the list, and a worker takes `per` rows.
 //
-// A worker's end that falls into an entry's rows is put behind them if they are at most SHORT;
+// A worker's end that falls into an entry's rows is put behind them if they are at most `per`;
 // else the entry is longer than a worker: each of its workers leaves its sum in parts, and the
 // one in which it ends puts it on the list that k_embed_join works off.  Sums of a worker are
 // in the rows' order, those of parts in a fixed order too: the same bits in every run.
 // ---------------------------------------------------------------------------
 constexpr int SUM_WAVES = 4, SUM_THREADS = 64 * SUM_WAVES;
-constexpr int SHORT = 64;            // rows
 constexpr int MOST_ITEMS = 4096;     // of a workgroup
 constexpr int AHEAD = 8;             // items on the way
 constexpr uint32_t ENTRY = 0x80000000u;      // an item that is an entry: which, if not all are there
@@ -427,7 +426,7 @@ struct Sums {
     bool dense;                      // entries without rows are on the list
     int64_t row_stride, table_stride;
     float scale;
-    const uint32_t *key, *row;
+    const uint2 *sorted;             // key and row
     const void *dout, *base;
     void *dtable;
     int32_t part_stride;             // dim in whole fours
@@ -436,13 +435,13 @@ struct Sums {
     uint32_t *found;                 // [0]: how many; then (worker, entry)
 };
 // Rows that a workgroup of `items` items may look at.
-__host__ __device__ constexpr int held_rows(int items) { return items + 2 * SHORT + 2; }
+__host__ __device__ constexpr int held_rows(int items, int per) { return items + 2 * per + 2; }
 
 // Rows and entries before an item.  i counts from the first row that the workgroup holds in LDS.
 struct Cut {
     int i;
     uint32_t e;
-    bool open;                       // e's rows begin before i, and there are more than SHORT
+    bool open;                       // e's rows begin before i, and there are more than `per`
 };
 
 // The first of [lo, hi) for which under() does not hold, which does for all before.
@@ -472,10 +471,10 @@ __device__ __forceinline__ Cut cut_at(const Sums &s, const uint32_t *key, int64_
         c.open = d > 0 && d < s.rows && c.e < s.entries && key[c.i] == c.e;
     }
     if (!c.open) return c;
-    const int a = first_not(max(0, c.i - SHORT - 1), c.i, [&](int m) { return key[m] < c.e; });
-    const int b = first_not(c.i, min(held, c.i + SHORT + 1),
+    const int a = first_not(max(0, c.i - s.per - 1), c.i, [&](int m) { return key[m] < c.e; });
+    const int b = first_not(c.i, min(held, c.i + s.per + 1),
                             [&](int m) { return key[m] <= c.e; });
-    if (b - a <= SHORT) {
+    if (b - a <= s.per) {
         c.i = b;
         c.e += 1;
         c.open = false;
@@ -499,7 +498,7 @@ __device__ __forceinline__ void both_ends(const Sums &s, const int64_t (&d)[2], 
             step[x] = (hi[x] - lo[x] + SUM_THREADS - 1) / SUM_THREADS;
             m[x] = lo[x] + threadIdx.x * step[x];
             in[x] = m[x] < hi[x];
-            k[x] = in[x] ? s.key[m[x]] : 0;
+            k[x] = in[x] ? s.sorted[m[x]].x : 0;
         }
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
@@ -517,22 +516,18 @@ __device__ __forceinline__ void both_ends(const Sums &s, const int64_t (&d)[2], 
     found[1] = lo[1];
 }
 
-// E elements as they lie in memory; those behind the n-th are 0.
-template <typename T, int E> using Raw = T __attribute__((ext_vector_type(E)));
+// E elements in a row, at any address that holds one.
 template <typename T, int E>
-__device__ __forceinline__ Raw<T, E> load_raw(const T *p, int n) {
-    if (n >= E) return *reinterpret_cast<const Raw<T, E> *>(p);
-    Raw<T, E> v;
-#pragma unroll
-    for (int e = 0; e < E; ++e) v[e] = e < n ? p[e] : (T)0.0f;
-    return v;
-}
+using Run = T __attribute__((ext_vector_type(E), aligned(sizeof(T))));
 
-template <typename T, int E>
+// E > 1: the last piece of a row that is no multiple of E long is its last E columns, some of which
+// the piece before has too: both lanes write the same.
+// BASE: dtable has a base.  ONE: one worker a wavefront, whose items are the same in all lanes.
+template <typename T, int E, bool BASE, bool ONE>
 __global__ __launch_bounds__(SUM_THREADS) void k_embed_sum(Sums s) {
     extern __shared__ uint32_t lds[];
     __shared__ uint32_t wave_sum[SUM_WAVES];
-    const int items = SUM_WAVES * s.groups * s.per, most = held_rows(items);
+    const int items = SUM_WAVES * s.groups * s.per, most = held_rows(items, s.per);
     uint32_t *key = lds;                             // [row]
     uint32_t *item = key + most;                     // [item]: a row, or an entry
     uint32_t *place = item + 2 * most;               // [row] its item, where it is not i + key
@@ -542,20 +537,20 @@ __global__ __launch_bounds__(SUM_THREADS) void k_embed_sum(Sums s) {
                                              s.rows + (s.dense ? (int64_t)s.entries : 0))};
     int64_t ends[2] = {d[0], d[1]};
     if (s.dense) both_ends(s, d, ends);
-    const int64_t begin = max((int64_t)0, ends[0] - SHORT - 1);
-    const int held = (int)(min(s.rows, ends[1] + SHORT + 1) - begin);
+    const int64_t begin = max((int64_t)0, ends[0] - s.per - 1);
+    const int held = (int)(min(s.rows, ends[1] + s.per + 1) - begin);
     const int lo = (int)(ends[0] - begin), hi = (int)(ends[1] - begin);
     if (s.dense) {
-        for (int i = threadIdx.x; i < items + SHORT + 2; i += SUM_THREADS) item[i] = ENTRY;
+        for (int i = threadIdx.x; i < items + s.per + 2; i += SUM_THREADS) item[i] = ENTRY;
         __syncthreads();
         for (int i = threadIdx.x; i < held; i += SUM_THREADS) {
-            const uint32_t k = s.key[begin + i], r = s.row[begin + i];
-            key[i] = k;
-            const int64_t at = begin + i + (int64_t)k - d[0];
-            if (at >= 0 && at < items + SHORT + 2 && k < s.entries) item[at] = r;
+            const uint2 x = s.sorted[begin + i];
+            key[i] = x.x;
+            const int64_t at = begin + i + (int64_t)x.x - d[0];
+            if (at >= 0 && at < items + s.per + 2 && x.x < s.entries) item[at] = x.y;
         }
     } else {
-        for (int i = threadIdx.x; i < held; i += SUM_THREADS) key[i] = s.key[begin + i];
+        for (int i = threadIdx.x; i < held; i += SUM_THREADS) key[i] = s.sorted[begin + i].x;
         __syncthreads();
         // a row's item lies behind as many entries as end before it
         uint32_t before = 0, all;
@@ -567,7 +562,7 @@ __global__ __launch_bounds__(SUM_THREADS) void k_embed_sum(Sums s) {
             const uint32_t at = i + before + sum_before<SUM_WAVES>(ends_here, wave_sum, all);
             if (i < held) {
                 place[i] = at;
-                item[at] = k < s.entries ? s.row[begin + i] : NOTHING;
+                item[at] = s.sorted[begin + i].y;
                 if (ends_here) item[at + 1] = ENTRY | k;
             }
             before += all;
@@ -580,53 +575,65 @@ __global__ __launch_bounds__(SUM_THREADS) void k_embed_sum(Sums s) {
     const int32_t chunk = blockIdx.y * 64 + lane - group * s.lanes;
     if (group >= s.groups || worker >= s.workers || chunk >= s.chunks) return;
     const Cut from = cut_at(s, key, begin, held, lo, hi, worker * s.per);
-    const Cut to = cut_at(s, key, begin, held, lo, hi, (worker + 1) * s.per);
-    const int col = chunk * E, n = s.dim - col;
+    Cut to = cut_at(s, key, begin, held, lo, hi, (worker + 1) * s.per);
+    if (to.i > from.i && key[to.i - 1] >= s.entries)         // rows that are left out, behind all
+        to.i = first_not(from.i, to.i, [&](int m) { return key[m] < s.entries; });
+    uint32_t next = from.e;          // the next entry, where all are on the list
+    int p = s.dense ? (int)(begin + from.i + (int64_t)from.e - d[0]) : (int)place[from.i];
+    int end = s.dense ? (int)(begin + to.i + (int64_t)to.e - d[0]) : (int)place[to.i];
+    if constexpr (ONE) {
+        next = __builtin_amdgcn_readfirstlane(next);
+        p = __builtin_amdgcn_readfirstlane(p);
+        end = __builtin_amdgcn_readfirstlane(end);
+    }
+    const int col = min(chunk * E, s.dim - E);
     const T *dout = static_cast<const T *>(s.dout) + col;
-    const T *base = s.base ? static_cast<const T *>(s.base) + col : nullptr;
+    const T *base = BASE ? static_cast<const T *>(s.base) + col : nullptr;
     T *dtable = static_cast<T *>(s.dtable) + col;
+    float *parts = s.parts + worker * 2 * s.part_stride + col;
 
     float acc[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = 0.0f;
     bool head = from.open;
     const auto leave = [&](int side) {
-        float *p = s.parts + (worker * 2 + side) * s.part_stride + col;
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-            if (e < n) p[e] = acc[e];
+        for (int e = 0; e < E; ++e) parts[side * s.part_stride + e] = acc[e];
     };
-    uint32_t next = from.e;          // the next entry, where all are on the list
-    int p = s.dense ? (int)(begin + from.i + (int64_t)from.e - d[0]) : (int)place[from.i];
-    const int end = s.dense ? (int)(begin + to.i + (int64_t)to.e - d[0]) : (int)place[to.i];
     for (; p < end; p += AHEAD) {
         uint32_t what[AHEAD];
-        Raw<T, E> v[AHEAD];
-        uint32_t e = next;
+        Run<T, E> v[AHEAD];
 #pragma unroll
         for (int q = 0; q < AHEAD; ++q) {
-            what[q] = p + q < end ? item[p + q] : NOTHING;
-            if (s.dense && what[q] == ENTRY) {
-                what[q] = e < s.entries ? ENTRY | e : NOTHING;       // behind all: left out
-                ++e;
+            what[q] = item[p + q];
+            if constexpr (ONE) what[q] = __builtin_amdgcn_readfirstlane(what[q]);
+            if (s.dense) {
+                const bool entry = what[q] == ENTRY;
+                what[q] |= entry ? next : 0;
+                next += entry;
             }
+            if (p + q >= end) what[q] = NOTHING;
+        }
+#pragma unroll
+        for (int q = 0; q < AHEAD; ++q) {
+            if (what[q] < ENTRY)
+                v[q] = *reinterpret_cast<const Run<T, E> *>(dout + what[q] * s.row_stride);
+            else if (BASE && what[q] != NOTHING)
+                v[q] = *reinterpret_cast<const Run<T, E> *>(
+                    base + (int64_t)(what[q] & ~ENTRY) * s.table_stride);
         }
 #pragma unroll
         for (int q = 0; q < AHEAD; ++q) {
             const bool is_row = what[q] < ENTRY;
-            const int64_t at = is_row ? what[q] * s.row_stride
-                                      : (int64_t)(what[q] & ~ENTRY) * s.table_stride;
-            const bool read = is_row || (what[q] != NOTHING && base);
-            v[q] = load_raw<T, E>((is_row ? dout : base) + (read ? at : 0), read ? n : 0);
-        }
+            if constexpr (ONE) {
+                if (is_row)
 #pragma unroll
-        for (int q = 0; q < AHEAD; ++q) {
-            if (what[q] == NOTHING) continue;
-            if (what[q] < ENTRY) {
+                    for (int e = 0; e < E; ++e) acc[e] += to_f32(v[q][e]);
+            } else {
 #pragma unroll
-                for (int x = 0; x < E; ++x) acc[x] += to_f32(v[q][x]);
-                continue;
+                for (int e = 0; e < E; ++e) acc[e] = is_row ? acc[e] + to_f32(v[q][e]) : acc[e];
             }
+            if (is_row || what[q] == NOTHING) continue;
             const uint32_t entry = what[q] & ~ENTRY;
             if (head) {
                 leave(0);
@@ -637,85 +644,115 @@ __global__ __launch_bounds__(SUM_THREADS) void k_embed_sum(Sums s) {
                 }
                 head = false;
             } else {
-                float out[E];
+                Run<T, E> out;
 #pragma unroll
-                for (int x = 0; x < E; ++x)
-                    out[x] = __builtin_fmaf(s.scale, acc[x], base ? to_f32(v[q][x]) : 0.0f);
-                store<T, E>(dtable + entry * s.table_stride, n, out);
+                for (int e = 0; e < E; ++e)
+                    out[e] = (T)__builtin_fmaf(s.scale, acc[e], BASE ? to_f32(v[q][e]) : 0.0f);
+                *reinterpret_cast<Run<T, E> *>(dtable + entry * s.table_stride) = out;
             }
 #pragma unroll
-            for (int x = 0; x < E; ++x) acc[x] = 0.0f;
+            for (int e = 0; e < E; ++e) acc[e] = 0.0f;
         }
-        next = e;
     }
     if (to.open) leave(1);
     if (chunk == 0) s.open[worker] = to.open ? to.e : NOTHING;
 }
 
 // The entries on the list: heads and tails of their workers, from the first that left the entry
-// open to the one in which it ends.  A workgroup an entry; slices of its workers are summed side
-// by side, and the slices' sums in their order.
+// open to the one in which it ends.  A wavefront an entry, or all of a workgroup's an entry of
+// more than WAVE_PARTS parts: slices of the parts are summed side by side, and the slices' sums
+// in their order.
 constexpr int JOIN_WAVES = 4, JOIN_THREADS = 64 * JOIN_WAVES;
+constexpr int WAVE_PARTS = 64;
+constexpr int PARTS = 8;             // parts on the way
 template <typename T>
 __global__ __launch_bounds__(JOIN_THREADS) void k_embed_join(Sums s) {
     typedef float V __attribute__((ext_vector_type(4)));
     __shared__ V sums[JOIN_THREADS];
+    __shared__ int64_t firsts[JOIN_WAVES];
     const uint32_t count = s.found[0];
     const int fours = s.part_stride / 4, wide = min(fours, 64), groups = 64 / wide;
-    const int slices = JOIN_WAVES * groups;
-    const int lane = threadIdx.x & 63, group = lane / wide;
-    const int slice = (threadIdx.x >> 6) * groups + group, col0 = lane - group * wide;
-    for (uint32_t f = blockIdx.x; f < count; f += gridDim.x) {
-        const int64_t last = s.found[2 + 2 * f];
-        const uint32_t entry = s.found[3 + 2 * f];
-        int64_t start = last;
-        for (;;) {
-            const int64_t w = start - 1 - threadIdx.x;
-            const bool same = w >= 0 && s.open[w] == entry;
-            // workers that left the entry open lie side by side
-            const int n = __syncthreads_count(same);
-            start -= n;
-            if (n < JOIN_THREADS) break;
-        }
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, group = lane / wide;
+    const int col0 = lane - group * wide;
+    // Slice `slice` of `slices` of the parts [start, last] of four columns, met in sums[at ...].
+    const auto part_sum = [&](int64_t start, int64_t last, int slice, int slices, int four) {
         const int64_t each = (last - start + slices) / slices;      // of last - start + 1 parts
         const int64_t a = start + slice * each, b = min(a + each, last + 1);
-        for (int c0 = 0; c0 < fours; c0 += wide) {
-            const int col = (c0 + col0) * 4;
-            V sum = {0, 0, 0, 0};
-            if (group < groups && c0 + col0 < fours)
-                for (int64_t w = a; w < b; w += AHEAD) {
-                    V v[AHEAD];
+        V sum = {0, 0, 0, 0};
+        if (group < groups && four < fours)
+            for (int64_t w = a; w < b; w += PARTS) {
+                V v[PARTS];
 #pragma unroll
-                    for (int q = 0; q < AHEAD; ++q) {
-                        const int64_t x = min(w + q, b - 1);
-                        v[q] = *reinterpret_cast<const V *>(
-                            s.parts + (x * 2 + (x < last)) * s.part_stride + col);
-                    }
-#pragma unroll
-                    for (int q = 0; q < AHEAD; ++q)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) sum[e] += w + q < b ? v[q][e] : 0.0f;
+                for (int q = 0; q < PARTS; ++q) {
+                    const int64_t x = min(w + q, b - 1);
+                    v[q] = *reinterpret_cast<const V *>(
+                        s.parts + (x * 2 + (x < last)) * s.part_stride + four * 4);
                 }
-            sums[threadIdx.x] = sum;
-            __syncthreads();
-            if (threadIdx.x < (unsigned)wide && c0 + col0 < fours) {
-                V total = {0, 0, 0, 0};
-                for (int v = 0; v < slices; ++v) {
-                    const V part = sums[(v / groups) * 64 + (v % groups) * wide + col0];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) total[e] += part[e];
-                }
-                const int64_t at = (int64_t)entry * s.table_stride + col;
+                for (int q = 0; q < PARTS; ++q)
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (col + e < s.dim) {
-                        const float b0 = s.base ? to_f32(static_cast<const T *>(s.base)[at + e]) : 0.0f;
-                        static_cast<T *>(s.dtable)[at + e] =
-                            (T)__builtin_fmaf(s.scale, total[e], b0);
-                    }
+                    for (int e = 0; e < 4; ++e) sum[e] += w + q < b ? v[q][e] : 0.0f;
             }
-            __syncthreads();
+        sums[threadIdx.x] = sum;
+    };
+    // The slices' sums of a wavefront, or of all.
+    const auto finish = [&](uint32_t entry, int first_wave, int slices, int four) {
+        if (group != 0 || four >= fours) return;
+        V total = {0, 0, 0, 0};
+        for (int v = 0; v < slices; ++v) {
+            const V part = sums[(first_wave + v / groups) * 64 + (v % groups) * wide + col0];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) total[e] += part[e];
         }
+        const int col = four * 4;
+        const int64_t at = (int64_t)entry * s.table_stride + col;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (col + e < s.dim) {
+                const float b0 = s.base ? to_f32(static_cast<const T *>(s.base)[at + e]) : 0.0f;
+                static_cast<T *>(s.dtable)[at + e] = (T)__builtin_fmaf(s.scale, total[e], b0);
+            }
+    };
+    for (uint32_t f0 = blockIdx.x * JOIN_WAVES; f0 < count; f0 += gridDim.x * JOIN_WAVES) {
+        const uint32_t mine = f0 + wave;
+        int64_t last = 0, start = 0;
+        uint32_t entry = NOTHING;
+        if (mine < count) {
+            last = start = s.found[2 + 2 * mine];
+            entry = s.found[3 + 2 * mine];
+            // the entry's workers lie side by side: the 64 before, or 64-ary search
+            const int64_t w = start - 1 - lane;
+            const int n = __popcll(__ballot(w >= 0 && s.open[w] == entry));
+            start -= n;
+            int64_t lo = 0;
+            while (n == 64 && start > lo) {          // the first one is in [lo, start]
+                const int64_t step = (start - lo + 63) / 64, m = start - step * (lane + 1);
+                const int more = __popcll(__ballot(m >= lo && s.open[max(m, lo)] == entry));
+                lo = max(lo, start - step * (more + 1) + 1);
+                start -= step * more;
+            }
+        }
+        if (lane == 0) firsts[wave] = start;
+        __syncthreads();
+        for (int four0 = blockIdx.y * wide; four0 < fours; four0 += gridDim.y * wide) {
+            const int four = four0 + col0;
+            if (mine < count && last - start < WAVE_PARTS) {
+                part_sum(start, last, group, groups, four);
+                __builtin_amdgcn_wave_barrier();
+                finish(entry, wave, groups, four);
+                __builtin_amdgcn_wave_barrier();
+            }
+            for (uint32_t x = 0; x < JOIN_WAVES && f0 + x < count; ++x) {
+                const int64_t of = s.found[2 + 2 * (f0 + x)];
+                if (of - firsts[x] < WAVE_PARTS) continue;
+                __syncthreads();
+                part_sum(firsts[x], of, wave * groups + group, JOIN_WAVES * groups, four);
+                __syncthreads();
+                if (wave == 0) finish(s.found[3 + 2 * (f0 + x)], 0, JOIN_WAVES * groups, four);
+                __syncthreads();
+            }
+        }
+        __syncthreads();
     }
 }
 
@@ -757,12 +794,13 @@ GradShape grad_shape(const EmbedCall &c) {
         const int64_t chunks = (c.rows + chunk - 1) / chunk;
         g.per = (chunks + MOST_UNITS - 1) / MOST_UNITS * chunk;
         g.units = (int)((c.rows + g.per - 1) / g.per);
-        g.narrow = g.per < (1 << 16);
+        g.narrow = g.per < (1 << 13);
     }
-    const size_t size = c.bf16 ? 2 : 4;
-    const bool wide = aligned(c.dout, c.row_stride, size) && aligned(c.dtable, c.table_stride, size) &&
-                      (!c.base || aligned(c.base, c.table_stride, size));
-    g.elements = wide ? (c.bf16 ? 8 : 4) : 1;
+    // 16 bytes a lane, unless the last piece of a row shares columns with one of another
+    // wavefront that may have written them to the base
+    const int elements = c.bf16 ? 8 : 4;
+    const bool apart = c.dim % elements == 0 || c.dim <= 64 * elements || c.base != c.dtable;
+    g.elements = c.dim >= elements && apart ? elements : 1;
     g.chunks = (c.dim + g.elements - 1) / g.elements;
     g.lanes = std::min(g.chunks, 64);
     g.groups = 64 / g.lanes;
@@ -795,14 +833,28 @@ hipError_t sort_pass(hipStream_t st, const Pass &p) {
     return hipGetLastError();
 }
 
-template <typename T, int E>
-hipError_t sums(hipStream_t st, const Sums &s, int cols, int num_cus) {
+template <typename T, int E, bool BASE, bool ONE>
+void sums(hipStream_t st, const Sums &s, int cols) {
     const int64_t each = SUM_WAVES * s.groups;
-    dim3 g = grid_of((s.workers + each - 1) / each, (uint32_t)cols);
-    const size_t lds = sizeof(uint32_t) * (4 * (size_t)held_rows((int)each * s.per) + 1);
-    hipLaunchKernelGGL((k_embed_sum<T, E>), g, dim3(SUM_THREADS), lds, st, s);
-    hipLaunchKernelGGL((k_embed_join<T>), dim3((uint32_t)(4 * num_cus)), dim3(JOIN_THREADS), 0, st,
-                       s);
+    const size_t lds = sizeof(uint32_t) * (4 * (size_t)held_rows((int)each * s.per, s.per) + 1);
+    hipLaunchKernelGGL((k_embed_sum<T, E, BASE, ONE>),
+                       grid_of((s.workers + each - 1) / each, (uint32_t)cols), dim3(SUM_THREADS), lds,
+                       st, s);
+}
+template <typename T, int E> void sums(hipStream_t st, const Sums &s, int cols) {
+    if (s.groups == 1)
+        s.base ? sums<T, E, true, true>(st, s, cols) : sums<T, E, false, true>(st, s, cols);
+    else
+        s.base ? sums<T, E, true, false>(st, s, cols) : sums<T, E, false, false>(st, s, cols);
+}
+template <typename T>
+hipError_t sums(hipStream_t st, const Sums &s, const GradShape &g, int num_cus) {
+    constexpr int E = 16 / sizeof(T);
+    g.elements > 1 ? sums<T, E>(st, s, g.cols) : sums<T, 1>(st, s, g.cols);
+    const int turns = (s.part_stride / 4 + 63) / 64;
+    hipLaunchKernelGGL((k_embed_join<T>),
+                       dim3((uint32_t)(4 * num_cus), (uint32_t)std::min(turns, 16)),
+                       dim3(JOIN_THREADS), 0, st, s);
     return hipGetLastError();
 }
 
@@ -827,21 +879,19 @@ hipError_t launch_embed(hipStream_t s, const EmbedCall &c) {
 
 size_t embed_grad_scratch(const EmbedCall &c) {
     const GradShape g = grad_shape(c);
-    const size_t rows = rounded((size_t)c.rows * 4);
-    return (g.small || g.passes < 2 ? 2 : 4) * rows + table_bytes(g) +
+    const size_t rows = rounded((size_t)c.rows * sizeof(uint2));
+    return (g.small || g.passes < 2 ? 1 : 2) * rows + table_bytes(g) +
            rounded(4 * (size_t)g.workers) + rounded(8 + 8 * (size_t)g.workers) +
            rounded(8 * (size_t)g.workers * part_stride(c));
 }
 
 hipError_t launch_embed_grad(hipStream_t st, const EmbedCall &c, char *scratch) {
     const GradShape g = grad_shape(c);
-    const size_t rows = rounded((size_t)c.rows * 4);
-    uint32_t *key[2], *row[2];
-    const int sides = g.small || g.passes < 2 ? 1 : 2;
-    for (int i = 0; i < sides; ++i) {
-        key[i] = reinterpret_cast<uint32_t *>(scratch);
-        row[i] = reinterpret_cast<uint32_t *>(scratch + rows);
-        scratch += 2 * rows;
+    const size_t rows = rounded((size_t)c.rows * sizeof(uint2));
+    uint2 *pairs[2];
+    for (int i = 0; i < (g.small || g.passes < 2 ? 1 : 2); ++i) {
+        pairs[i] = reinterpret_cast<uint2 *>(scratch);
+        scratch += rows;
     }
     void *table = scratch;
     scratch += table_bytes(g);
@@ -864,20 +914,15 @@ hipError_t launch_embed_grad(hipStream_t st, const EmbedCall &c, char *scratch) 
         const hipError_t e = allow_all_lds(reinterpret_cast<const void *>(k_embed_sort_small));
         if (e != hipSuccess) return e;
         p.ids = c.ids;
-        p.key_out = key[0];
-        p.row_out = row[0];
+        p.out = pairs[0];
         const size_t lds = 4 * (SMALL_WAVES + ((size_t)SMALL_WAVES << g.bits) + c.rows) + 2 * c.rows;
         hipLaunchKernelGGL(k_embed_sort_small, dim3(1), dim3(SMALL_THREADS), lds, st, p, g.passes);
     } else {
         for (int i = 0; i < g.passes; ++i) {
             to = i & 1;
             p.ids = i == 0 ? c.ids : nullptr;
-            if (i > 0) {
-                p.key_in = key[to ^ 1];
-                p.row_in = row[to ^ 1];
-            }
-            p.key_out = key[to];
-            p.row_out = row[to];
+            if (i > 0) p.in = pairs[to ^ 1];
+            p.out = pairs[to];
             p.shift = i * g.bits;
             const hipError_t e = g.each == 4 ? sort_pass<4, uint16_t>(st, p)
                                  : g.narrow  ? sort_pass<8, uint16_t>(st, p)
@@ -897,16 +942,11 @@ hipError_t launch_embed_grad(hipStream_t st, const EmbedCall &c, char *scratch) 
     s.row_stride = c.row_stride;
     s.table_stride = c.table_stride;
     s.scale = c.scale;
-    s.key = key[to];
-    s.row = row[to];
+    s.sorted = pairs[to];
     s.dout = c.dout;
     s.base = c.base;
     s.dtable = c.dtable;
-    if (c.bf16)
-        return g.elements > 1 ? sums<__bf16, 8>(st, s, g.cols, c.num_cus)
-                              : sums<__bf16, 1>(st, s, g.cols, c.num_cus);
-    return g.elements > 1 ? sums<float, 4>(st, s, g.cols, c.num_cus)
-                          : sums<float, 1>(st, s, g.cols, c.num_cus);
+    return c.bf16 ? sums<__bf16>(st, s, g, c.num_cus) : sums<float>(st, s, g, c.num_cus);
 }
 
 }  // namespace mbk
