@@ -591,6 +591,7 @@ __global__ __launch_bounds__(SUM_THREADS) void k_embed_sum(Sums s) {
     const T *base = BASE ? static_cast<const T *>(s.base) + col : nullptr;
     T *dtable = static_cast<T *>(s.dtable) + col;
     float *parts = s.parts + worker * 2 * s.part_stride + col;
+    const T *some_row = s.rows ? dout : dtable;
 
     float acc[E];
 #pragma unroll
@@ -616,11 +617,17 @@ __global__ __launch_bounds__(SUM_THREADS) void k_embed_sum(Sums s) {
         }
 #pragma unroll
         for (int q = 0; q < AHEAD; ++q) {
-            if (what[q] < ENTRY)
-                v[q] = *reinterpret_cast<const Run<T, E> *>(dout + what[q] * s.row_stride);
-            else if (BASE && what[q] != NOTHING)
+            const bool is_row = what[q] < ENTRY;
+            // without branches: what has nothing to read takes a row or an entry that is there
+            if constexpr (BASE) {
+                const T *at = is_row ? dout : what[q] == NOTHING ? dtable : base;
+                const uint32_t which = what[q] == NOTHING ? 0 : what[q] & ~ENTRY;
                 v[q] = *reinterpret_cast<const Run<T, E> *>(
-                    base + (int64_t)(what[q] & ~ENTRY) * s.table_stride);
+                    at + which * (is_row ? s.row_stride : s.table_stride));
+            } else {
+                v[q] = *reinterpret_cast<const Run<T, E> *>(
+                    some_row + (is_row ? what[q] : 0) * s.row_stride);
+            }
         }
 #pragma unroll
         for (int q = 0; q < AHEAD; ++q) {
