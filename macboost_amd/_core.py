@@ -735,9 +735,9 @@ class Tensors:
                  ctypes.byref(self.ptr))
 
     def close(self):
-        if self.ptr.value and self.ctx.ptr.value and _lib_instance is not None:
+        if self.ptr and self.ctx.ptr and _lib_instance is not None:
             _lib_instance.mbk_tensors_destroy(self.ctx.ptr, self.ptr)
-        self.ptr = _P()
+        self.ptr = None
 
     def __del__(self):
         self.close()

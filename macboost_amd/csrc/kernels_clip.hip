@@ -12,56 +12,68 @@ namespace {
 
 constexpr int THREADS = 256, WAVES = THREADS / 64;
 
-// Visits the elements of a piece, E at a time: take(offset of the first, how many of them).
-// E > 1 only where the piece's addresses and stride are multiples of 16 bytes.
-template <int E, class Take>
-__device__ __forceinline__ void each_of(const ClipPiece &p, Take take) {
-    if (p.rows == 1) {
-        for (int i = threadIdx.x * E; i < p.cols; i += THREADS * E) take((int64_t)i, p.cols - i);
-        return;
-    }
+// 16 bytes at any address that holds an element.
+template <typename T, int E> using Run = T __attribute__((ext_vector_type(E), aligned(sizeof(T))));
+
+// Visits a piece 16 bytes at a time, AT_ONCE of them on the way: take(runs, where they are, how
+// many elements of each count).  Where a row ends inside a run only its elements are read.
+constexpr int AT_ONCE = 4;
+template <typename T, int E, class Take>
+__device__ __forceinline__ void each_run(const ClipPiece &p, Take take) {
+    const T *g = static_cast<const T *>(p.grad);
     const uint32_t chunks = (uint32_t)(p.cols + E - 1) / E, all = chunks * (uint32_t)p.rows;
-    for (uint32_t i = threadIdx.x; i < all; i += THREADS) {
-        const uint32_t r = i / chunks, c = (i - r * chunks) * E;
-        take(r * p.stride + c, p.cols - (int)c);
+    for (uint32_t i0 = threadIdx.x; i0 < all; i0 += AT_ONCE * THREADS) {
+        Run<T, E> v[AT_ONCE];
+        int64_t at[AT_ONCE];
+        int n[AT_ONCE];
+#pragma unroll
+        for (int q = 0; q < AT_ONCE; ++q) {
+            const uint32_t i = i0 + q * THREADS;
+            const uint32_t r = p.rows == 1 ? 0 : i / chunks, c = (i - r * chunks) * E;
+            at[q] = r * p.stride + c;
+            n[q] = i < all ? p.cols - (int)c : 0;
+            if (n[q] >= E) v[q] = *reinterpret_cast<const Run<T, E> *>(g + at[q]);
+        }
+#pragma unroll
+        for (int q = 0; q < AT_ONCE; ++q)
+            if (n[q] < E)
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[q][e] = e < n[q] ? g[at[q] + e] : (T)0.0f;
+        take(v, at, n);
     }
 }
 
 template <typename T, int E>
 __device__ __forceinline__ double squares(const ClipPiece &p) {
-    typedef T V __attribute__((ext_vector_type(E)));
-    const T *g = static_cast<const T *>(p.grad);
     double sum = 0.0;
-    each_of<E>(p, [&](int64_t at, int n) {
-        if (n >= E) {
-            const V v = *reinterpret_cast<const V *>(g + at);
+    each_run<T, E>(p, [&](const Run<T, E> (&v)[AT_ONCE], const int64_t (&)[AT_ONCE],
+                          const int (&)[AT_ONCE]) {
 #pragma unroll
-            for (int e = 0; e < E; ++e) sum = __builtin_fma((double)v[e], (double)v[e], sum);
-        } else {
-            for (int e = 0; e < n; ++e) sum = __builtin_fma((double)g[at + e], (double)g[at + e], sum);
-        }
+        for (int q = 0; q < AT_ONCE; ++q)
+#pragma unroll
+            for (int e = 0; e < E; ++e) sum = __builtin_fma((double)v[q][e], (double)v[q][e], sum);
     });
     return sum;
 }
 
-// A product in 64 bits, rounded to f32 and from there to the type.
-template <typename T> __device__ __forceinline__ T scaled(T v, double by) {
-    return (T)(float)((double)v * by);
-}
-
+// Products in 64 bits, rounded to f32 and from there to the type.
 template <typename T, int E>
 __device__ __forceinline__ void scale(const ClipPiece &p, double by) {
-    typedef T V __attribute__((ext_vector_type(E)));
-    const T *g = static_cast<const T *>(p.grad);
     T *o = static_cast<T *>(p.out);
-    each_of<E>(p, [&](int64_t at, int n) {
-        if (n >= E) {
-            V v = *reinterpret_cast<const V *>(g + at);
+    each_run<T, E>(p, [&](const Run<T, E> (&v)[AT_ONCE], const int64_t (&at)[AT_ONCE],
+                          const int (&n)[AT_ONCE]) {
 #pragma unroll
-            for (int e = 0; e < E; ++e) v[e] = scaled<T>(v[e], by);
-            *reinterpret_cast<V *>(o + at) = v;
-        } else {
-            for (int e = 0; e < n; ++e) o[at + e] = scaled<T>(g[at + e], by);
+        for (int q = 0; q < AT_ONCE; ++q) {
+            Run<T, E> x;
+#pragma unroll
+            for (int e = 0; e < E; ++e) x[e] = (T)(float)((double)v[q][e] * by);
+            if (n[q] >= E) {
+                *reinterpret_cast<Run<T, E> *>(o + at[q]) = x;
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    if (e < n[q]) o[at[q] + e] = x[e];
+            }
         }
     });
 }
@@ -86,8 +98,7 @@ __global__ __launch_bounds__(THREADS) void k_clip_norm(const ClipPiece *__restri
     double sum = 0.0;
     for (int64_t i = blockIdx.x; i < count; i += gridDim.x) {
         const ClipPiece p = pieces[i];
-        if (p.bf16) sum += p.wide ? squares<__bf16, 8>(p) : squares<__bf16, 1>(p);
-        else sum += p.wide ? squares<float, 4>(p) : squares<float, 1>(p);
+        sum += p.bf16 ? squares<__bf16, 8>(p) : squares<float, 4>(p);
     }
     sum = sum_all(sum, wave_sum);
     if (threadIdx.x == 0) partial[blockIdx.x] = sum;
@@ -112,13 +123,8 @@ __global__ __launch_bounds__(THREADS) void k_clip_scale(const ClipPiece *__restr
     for (int64_t i = blockIdx.x; i < count; i += gridDim.x) {
         const ClipPiece p = pieces[count - 1 - i];
         if (!p.out || (!clip && p.out == p.grad)) continue;
-        if (p.bf16) {
-            if (p.wide) scale<__bf16, 8>(p, by);
-            else scale<__bf16, 1>(p, by);
-        } else {
-            if (p.wide) scale<float, 4>(p, by);
-            else scale<float, 1>(p, by);
-        }
+        if (p.bf16) scale<__bf16, 8>(p, by);
+        else scale<float, 4>(p, by);
     }
 }
 

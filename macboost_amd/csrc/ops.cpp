@@ -114,16 +114,13 @@ mbk::EmbedCall embed_call(const mbk_embed_shape *sh, const int32_t *ids, const v
 
 // The pieces of one gradient of the list: short rows together, long ones and gradients without
 // gaps in runs.
-void add_pieces(const mbk_tensor &t, std::vector<mbk::ClipPiece> &out) {
+void add_pieces(const mbk_tensor &t, int64_t most, std::vector<mbk::ClipPiece> &out) {
     const bool bf16 = t.type == MBK_BF16;
-    const int64_t size = bf16 ? 2 : 4, most = mbk::CLIP_PIECE;
+    const int64_t size = bf16 ? 2 : 4;
     const auto add = [&](int64_t at, int64_t rows, int64_t cols) {
         const char *g = static_cast<const char *>(t.grad) + at * size;
         char *o = t.out ? static_cast<char *>(t.out) + at * size : nullptr;
-        const bool wide = reinterpret_cast<uintptr_t>(g) % 16 == 0 &&
-                          reinterpret_cast<uintptr_t>(o) % 16 == 0 &&
-                          (rows == 1 || t.stride * size % 16 == 0);
-        out.push_back({g, o, t.stride, (int32_t)rows, (int32_t)cols, bf16, wide});
+        out.push_back({g, o, t.stride, (int32_t)rows, (int32_t)cols, bf16});
     };
     if (!t.rows || !t.cols) return;
     const bool whole = t.rows == 1 || t.stride == t.cols;
@@ -288,7 +285,7 @@ int mbk_tensors_create(mbk_context *ctx, const mbk_tensor *list, int32_t count, 
         std::vector<mbk::ClipPiece> pieces;
         auto made = std::make_unique<mbk_tensors>();
         for (int32_t i = 0; i < count; ++i) {
-            add_pieces(list[i], pieces);
+            add_pieces(list[i], mbk::clip_piece(elements), pieces);
             made->outputs |= list[i].out != nullptr;
         }
         need(ctx != nullptr, "null kernel-seam context");
