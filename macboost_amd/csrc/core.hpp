@@ -416,6 +416,7 @@ struct mbk_tensors {
     mb::DevBuf<mbk::ClipPiece> piece;
     int64_t pieces = 0;
     bool outputs = false;
+    bool streamed = false;           // of outputs beyond the caches
     bool captured = false;           // a captured graph may use it
     bool gone = false;               // given back, but captured
 };

@@ -58,7 +58,7 @@ __device__ __forceinline__ double squares(const ClipPiece &p) {
 
 // Products in 64 bits, rounded to f32 and from there to the type.
 template <typename T, int E>
-__device__ __forceinline__ void scale(const ClipPiece &p, double by) {
+__device__ __forceinline__ void scale(const ClipPiece &p, double by, bool streamed) {
     T *o = static_cast<T *>(p.out);
     each_run<T, E>(p, [&](const Run<T, E> (&v)[AT_ONCE], const int64_t (&at)[AT_ONCE],
                           const int (&n)[AT_ONCE]) {
@@ -68,7 +68,7 @@ __device__ __forceinline__ void scale(const ClipPiece &p, double by) {
 #pragma unroll
             for (int e = 0; e < E; ++e) x[e] = (T)(float)((double)v[q][e] * by);
             if (n[q] >= E) {
-                *reinterpret_cast<Run<T, E> *>(o + at[q]) = x;
+                put(reinterpret_cast<Run<T, E> *>(o + at[q]), x, streamed);
             } else {
 #pragma unroll
                 for (int e = 0; e < E; ++e)
@@ -105,12 +105,14 @@ __global__ __launch_bounds__(THREADS) void k_clip_norm(const ClipPiece *__restri
 }
 
 // Every workgroup sums up the partial sums by itself.  Pieces come in the other order than in the
-// first pass, so that the last ones read are still in a cache.
+// first pass, so that the last ones read are still in a cache (353 MB forwards 120 us, 117 so);
+// stores of many outputs go past it (the next call's first pass: 82 us after ordinary ones, 54).
 __global__ __launch_bounds__(THREADS) void k_clip_scale(const ClipPiece *__restrict__ pieces,
                                                         int64_t count,
                                                         const double *__restrict__ partial,
                                                         int32_t partials, float max_norm,
-                                                        float *__restrict__ norm, bool outputs) {
+                                                        float *__restrict__ norm, bool outputs,
+                                                        bool streamed) {
     __shared__ double wave_sum[WAVES];
     double sum = 0.0;
     for (int i = threadIdx.x; i < partials; i += THREADS) sum += partial[i];
@@ -123,8 +125,8 @@ __global__ __launch_bounds__(THREADS) void k_clip_scale(const ClipPiece *__restr
     for (int64_t i = blockIdx.x; i < count; i += gridDim.x) {
         const ClipPiece p = pieces[count - 1 - i];
         if (!p.out || (!clip && p.out == p.grad)) continue;
-        if (p.bf16) scale<__bf16, 8>(p, by);
-        else scale<float, 4>(p, by);
+        if (p.bf16) scale<__bf16, 8>(p, by, streamed);
+        else scale<float, 4>(p, by, streamed);
     }
 }
 
@@ -143,7 +145,7 @@ hipError_t launch_clip(hipStream_t s, const ClipCall &c, char *scratch) {
     double *partial = reinterpret_cast<double *>(scratch);
     hipLaunchKernelGGL(k_clip_norm, dim3(groups), dim3(THREADS), 0, s, c.piece, c.pieces, partial);
     hipLaunchKernelGGL(k_clip_scale, dim3(c.outputs ? groups : 1), dim3(THREADS), 0, s, c.piece,
-                       c.pieces, partial, groups, c.max_norm, c.norm, c.outputs);
+                       c.pieces, partial, groups, c.max_norm, c.norm, c.outputs, c.streamed);
     return hipGetLastError();
 }
 

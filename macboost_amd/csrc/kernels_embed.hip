@@ -31,14 +31,14 @@ __device__ __forceinline__ void load(const T *p, int n, float (&f)[E]) {
 }
 
 template <typename T, int E>
-__device__ __forceinline__ void store(T *p, int n, const float (&f)[E]) {
+__device__ __forceinline__ void store(T *p, int n, const float (&f)[E], bool streamed) {
     if constexpr (E > 1) {
         typedef T V __attribute__((ext_vector_type(E)));
         if (n >= E) {
             V v;
 #pragma unroll
             for (int e = 0; e < E; ++e) v[e] = (T)f[e];
-            *reinterpret_cast<V *>(p) = v;
+            put(reinterpret_cast<V *>(p), v, streamed);
             return;
         }
     }
@@ -89,7 +89,7 @@ __global__ __launch_bounds__(256) void k_embed(EmbedCall c, int32_t chunks) {
         if (!here[q]) continue;
 #pragma unroll
         for (int e = 0; e < E; ++e) v[q][e] = __builtin_fmaf(c.scale, v[q][e], b[q][e]);
-        store<T, E>(out + row[q] * c.row_stride + col[q], c.dim - col[q], v[q]);
+        store<T, E>(out + row[q] * c.row_stride + col[q], c.dim - col[q], v[q], c.streamed);
     }
 }
 
@@ -424,6 +424,7 @@ struct Sums {
     int32_t lanes, groups;           // of a worker; workers a wavefront
     int32_t per;
     bool dense;                      // entries without rows are on the list
+    bool streamed;                   // dtable is stored past the caches
     int64_t row_stride, table_stride;
     float scale;
     const uint2 *sorted;             // key and row
@@ -655,7 +656,7 @@ __global__ __launch_bounds__(SUM_THREADS) void k_embed_sum(Sums s) {
 #pragma unroll
                 for (int e = 0; e < E; ++e)
                     out[e] = (T)__builtin_fmaf(s.scale, acc[e], BASE ? to_f32(v[q][e]) : 0.0f);
-                *reinterpret_cast<Run<T, E> *>(dtable + entry * s.table_stride) = out;
+                put(reinterpret_cast<Run<T, E> *>(dtable + entry * s.table_stride), out, s.streamed);
             }
 #pragma unroll
             for (int e = 0; e < E; ++e) acc[e] = 0.0f;
@@ -880,7 +881,9 @@ hipError_t lookup(hipStream_t st, const EmbedCall &c) {
 
 }  // namespace
 
-hipError_t launch_embed(hipStream_t s, const EmbedCall &c) {
+hipError_t launch_embed(hipStream_t s, const EmbedCall &call) {
+    EmbedCall c = call;
+    c.streamed = c.rows * c.dim * (c.bf16 ? 2 : 4) > STREAMED;
     return c.bf16 ? lookup<__bf16>(s, c) : lookup<float>(s, c);
 }
 
@@ -946,6 +949,7 @@ hipError_t launch_embed_grad(hipStream_t st, const EmbedCall &c, char *scratch) 
     s.groups = g.groups;
     s.per = g.items;
     s.dense = g.dense;
+    s.streamed = g.dense && c.entries * c.dim * (c.bf16 ? 2 : 4) > STREAMED;
     s.row_stride = c.row_stride;
     s.table_stride = c.table_stride;
     s.scale = c.scale;

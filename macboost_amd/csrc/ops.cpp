@@ -284,7 +284,9 @@ int mbk_tensors_create(mbk_context *ctx, const mbk_tensor *list, int32_t count, 
         }
         std::vector<mbk::ClipPiece> pieces;
         auto made = std::make_unique<mbk_tensors>();
+        int64_t written = 0;
         for (int32_t i = 0; i < count; ++i) {
+            if (list[i].out) written += list[i].rows * list[i].cols * (list[i].type == MBK_BF16 ? 2 : 4);
             add_pieces(list[i], mbk::clip_piece(elements), pieces);
             made->outputs |= list[i].out != nullptr;
         }
@@ -292,6 +294,7 @@ int mbk_tensors_create(mbk_context *ctx, const mbk_tensor *list, int32_t count, 
         need(!mb::context_captured(ctx), "the context's stream is being captured");
         mb::OnDevice here(mb::context_device(ctx));
         made->pieces = (int64_t)pieces.size();
+        made->streamed = written > mbk::STREAMED;
         made->piece.alloc(pieces.size());
         hipStream_t s = mb::context_stream(ctx);
         if (!pieces.empty())
@@ -338,7 +341,8 @@ int mbk_grad_clip(mbk_context *ctx, mbk_tensors *list, float max_norm, float *no
         char *scratch = mb::context_scratch(ctx, mbk::clip_scratch(list->pieces, cus));
         list->captured |= mb::context_captured(ctx);
         MB_HIP(mbk::launch_clip(mb::context_stream(ctx),
-                                {list->piece.ptr, list->pieces, list->outputs, max_norm, norm, cus},
+                                {list->piece.ptr, list->pieces, list->outputs, list->streamed,
+                                 max_norm, norm, cus},
                                 scratch));
         return 0;
     }, -1);

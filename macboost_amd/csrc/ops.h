@@ -55,6 +55,25 @@ hipError_t launch_expert_combine_grad(hipStream_t s, const ExpertPlan &p,
                                       const ExpertMatrix &dout, const void *sorted,
                                       const float *weights, void *d_sorted, float *d_weights);
 
+// Outputs of more bytes than all XCDs' L2 hold are stored past it: they would drive out what is
+// read, and what takes them next finds little of them there (65536 x 1024 bf16 rows looked up and
+// added: 70 us by ordinary stores, 57 so).
+constexpr int64_t STREAMED = (int64_t)32 << 20;
+#ifdef __HIP_DEVICE_COMPILE__
+// The empty statements keep the compiler from making one ordinary store of both.
+template <typename V> __device__ __forceinline__ void put(V *to, const V &v, bool streamed) {
+    if (streamed) {
+        __builtin_nontemporal_store(v, to);
+    } else {
+        asm volatile("" ::: "memory");
+        *to = v;
+        asm volatile("" ::: "memory");
+    }
+}
+#else
+template <typename V> __device__ void put(V *, const V &, bool) {}
+#endif
+
 // ---- category vectors ---------------------------------------------------------
 
 struct EmbedCall {
@@ -69,6 +88,7 @@ struct EmbedCall {
     const void *dout;                // of the gradient
     void *dtable;
     int num_cus;
+    bool streamed;                   // set by the launchers
 };
 hipError_t launch_embed(hipStream_t s, const EmbedCall &c);
 size_t embed_grad_scratch(const EmbedCall &c);
@@ -92,7 +112,7 @@ constexpr int64_t clip_piece(int64_t elements) {
 struct ClipCall {
     const ClipPiece *piece;
     int64_t pieces;
-    bool outputs;
+    bool outputs, streamed;
     float max_norm;
     float *norm;
     int num_cus;
