@@ -272,12 +272,11 @@ __device__ __forceinline__ Ends<N> ends_of(const FourbitCall &c, int64_t tile) {
     return out;
 }
 
+// The scores of a lane's classes and row.
 template <int N>
-__device__ __forceinline__ void write_scores(const FourbitCall &c, const float4v &z,
-                                             const Ends<N> &end, int64_t column,
-                                             int row_exponent) {
-    constexpr int EACH = Ends<N>::EACH;
-    float v[EACH];
+__device__ __forceinline__ void scores_of(const FourbitCall &c, const float4v &z,
+                                          const Ends<N> &end, int row_exponent,
+                                          float (&v)[Ends<N>::EACH]) {
     if constexpr (N == 2) {
         const bool odd = threadIdx.x & 1;
         const float a = other_term(odd ? z[0] : z[2]), b = other_term(odd ? z[1] : z[3]);
@@ -287,25 +286,39 @@ __device__ __forceinline__ void write_scores(const FourbitCall &c, const float4v
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = z[i];
     }
-    const int64_t row = column / N;
-    if (row >= c.rows) return;
 #pragma unroll
-    for (int i = 0; i < EACH; ++i) {
+    for (int i = 0; i < Ends<N>::EACH; ++i) {
         v[i] = ldexpf(v[i], end.e[i] + row_exponent);
         if (c.bias) v[i] = end.b[i] == -__builtin_inff() ? end.b[i] : v[i] + end.b[i];
     }
-    float *to = c.scores + row * c.score_stride + end.cls;
-    typedef float V __attribute__((ext_vector_type(EACH)));
-    if (c.wide_scores && end.cls + EACH <= c.shape.classes) {
+}
+
+// E scores of a row from class cls on, at any address of a float.
+template <int E>
+__device__ __forceinline__ void put_scores(const FourbitCall &c, int64_t row, int64_t cls,
+                                           const float (&v)[E]) {
+    if (row >= c.rows) return;
+    float *to = c.scores + row * c.score_stride + cls;
+    if (cls + E <= c.shape.classes) {
+        typedef float V __attribute__((ext_vector_type(E), aligned(4)));
         V out;
 #pragma unroll
-        for (int i = 0; i < EACH; ++i) out[i] = v[i];
+        for (int i = 0; i < E; ++i) out[i] = v[i];
         *reinterpret_cast<V *>(to) = out;
     } else {
 #pragma unroll
-        for (int i = 0; i < EACH; ++i)
-            if (end.cls + i < c.shape.classes) to[i] = v[i];
+        for (int i = 0; i < E; ++i)
+            if (cls + i < c.shape.classes) to[i] = v[i];
     }
+}
+
+template <int N>
+__device__ __forceinline__ void write_scores(const FourbitCall &c, const float4v &z,
+                                             const Ends<N> &end, int64_t column,
+                                             int row_exponent) {
+    float v[Ends<N>::EACH];
+    scores_of<N>(c, z, end, row_exponent, v);
+    put_scores(c, column / N, end.cls, v);
 }
 
 // ---- few columns: reading W is the work ------------------------------------------------
@@ -436,6 +449,7 @@ __global__ __launch_bounds__(FEW_THREADS, 4) void k_fourbit_few(FourbitCall c, i
             if (at.quad * 4 + i >= blocks) break;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
+                if (j && (at.quad * 4 + i) * BLOCK + j * 32 >= c.shape.dim) break;
                 const half8 a = weights(unpack, b.word[i][j], scale_at<PER>(b.scale, i, j));
 #pragma unroll
                 for (int x = 0; x < CT; ++x)
@@ -546,6 +560,7 @@ __global__ __launch_bounds__(64 * WIDE_WAVES, 2) void k_fourbit_tiles(
         const half8 *here = lds + (b & 1) * BUFFER + lane;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
+            if (b * BLOCK + j * 32 >= c.shape.dim) break;
             half8 a[WIDE_TILES];
 #pragma unroll
             for (int t = 0; t < WIDE_TILES; ++t) a[t] = weights(unpack, word[t][j], scale[t][j * PER / 4]);
@@ -563,12 +578,33 @@ __global__ __launch_bounds__(64 * WIDE_WAVES, 2) void k_fourbit_tiles(
 #pragma unroll
     for (int x = 0; x < CT; ++x)
         e[x] = row_exponents[min(((column0 + x) * 16 + (lane & 15)) / N, c.rows - 1)];
+    Ends<N> end[WIDE_TILES];
 #pragma unroll
-    for (int t = 0; t < WIDE_TILES; ++t) {
-        const Ends<N> end = ends_of<N>(c, tile0 + t);
+    for (int t = 0; t < WIDE_TILES; ++t) end[t] = ends_of<N>(c, tile0 + t);
+    // a wavefront's 64 classes of a tile of columns meet in LDS, so that a row's go out 256 bytes
+    // together: where rows are at odd addresses, 64 at a time leave parts of lines
+    constexpr int ROWS = 16 / N, ROW = WIDE_TILES * TILE + 4;
+    float *meet = reinterpret_cast<float *>(lds) + wave * ROWS * ROW;
+    __syncthreads();                                 // the columns are read
 #pragma unroll
-        for (int x = 0; x < CT; ++x)
-            write_scores<N>(c, acc[t][x], end, (column0 + x) * 16 + (lane & 15), e[x]);
+    for (int x = 0; x < CT; ++x) {
+#pragma unroll
+        for (int t = 0; t < WIDE_TILES; ++t) {
+            float v[Ends<N>::EACH];
+            scores_of<N>(c, acc[t][x], end[t], e[x], v);
+            float *to = meet + (lane & 15) / N * ROW + (int)(end[t].cls - tile0 * TILE);
+#pragma unroll
+            for (int i = 0; i < Ends<N>::EACH; ++i) to[i] = v[i];
+        }
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int i = 0; i < ROWS / 4; ++i) {
+            const int row = i * 4 + (lane >> 4);
+            const float4v z = *reinterpret_cast<const float4v *>(meet + row * ROW + (lane & 15) * 4);
+            const float v[4] = {z[0], z[1], z[2], z[3]};
+            put_scores(c, (column0 + x) * 16 / N + row, tile0 * TILE + (lane & 15) * 4, v);
+        }
+        __builtin_amdgcn_wave_barrier();
     }
 }
 
@@ -635,7 +671,8 @@ hipError_t run_tiles(hipStream_t st, const FourbitCall &c, const half8 *columns,
     const int64_t tiles = (c.shape.classes + TILE - 1) / TILE;
     const int64_t groups = (tiles + WIDE_WAVES * WIDE_TILES - 1) / (WIDE_WAVES * WIDE_TILES) * turns;
     hipLaunchKernelGGL((k_fourbit_tiles<TERMS<T>, CT, PER>), grid_of(groups), dim3(64 * WIDE_WAVES),
-                       (size_t)CT * 8192, st, c, columns, e, column_tiles, turns);
+                       std::max((size_t)CT * 8192, (size_t)WIDE_WAVES * (16 / TERMS<T>) * (WIDE_TILES * TILE + 4) * 4), st,
+                       c, columns, e, column_tiles, turns);
     return hipGetLastError();
 }
 
@@ -649,17 +686,25 @@ template <typename T, int PER> hipError_t run(hipStream_t st, const FourbitCall 
     hipLaunchKernelGGL((k_fourbit_columns<T>), grid_of(tiles), dim3(64 * COLUMN_WAVES), 0, st,
                        static_cast<const T *>(c.h), c.h_stride, c.rows, c.shape.dim, c.wide_h, steps,
                        columns, e);
-    // up to 8 tiles of columns a turn, turns of one size
-    const int64_t turns = (tiles + 7) / 8;
-    switch ((tiles + turns - 1) / turns) {
-    case 1: return run_tiles<T, 1, PER>(st, c, columns, e, tiles, (int)turns);
-    case 2: return run_tiles<T, 2, PER>(st, c, columns, e, tiles, (int)turns);
-    case 3: return run_tiles<T, 3, PER>(st, c, columns, e, tiles, (int)turns);
-    case 4: return run_tiles<T, 4, PER>(st, c, columns, e, tiles, (int)turns);
-    case 5: return run_tiles<T, 5, PER>(st, c, columns, e, tiles, (int)turns);
-    case 6: return run_tiles<T, 6, PER>(st, c, columns, e, tiles, (int)turns);
-    case 7: return run_tiles<T, 7, PER>(st, c, columns, e, tiles, (int)turns);
-    default: return run_tiles<T, 8, PER>(st, c, columns, e, tiles, (int)turns);
+    // tiles of columns a turn: the time is that of the CU with most turns, each its tiles' products
+    // and about two tiles' worth of unpacking, beginning and end
+    const int64_t groups =
+        ((c.shape.classes + TILE - 1) / TILE + WIDE_WAVES * WIDE_TILES - 1) / (WIDE_WAVES * WIDE_TILES);
+    int64_t best = 0, least = 0;
+    for (int64_t ct = 1; ct <= 8; ++ct) {
+        const int64_t each = (groups * ((tiles + ct - 1) / ct) + c.num_cus - 1) / c.num_cus;
+        if (!best || each * (ct + 2) <= least) best = ct, least = each * (ct + 2);
+    }
+    const int turns = (int)((tiles + best - 1) / best);
+    switch (best) {
+    case 1: return run_tiles<T, 1, PER>(st, c, columns, e, tiles, turns);
+    case 2: return run_tiles<T, 2, PER>(st, c, columns, e, tiles, turns);
+    case 3: return run_tiles<T, 3, PER>(st, c, columns, e, tiles, turns);
+    case 4: return run_tiles<T, 4, PER>(st, c, columns, e, tiles, turns);
+    case 5: return run_tiles<T, 5, PER>(st, c, columns, e, tiles, turns);
+    case 6: return run_tiles<T, 6, PER>(st, c, columns, e, tiles, turns);
+    case 7: return run_tiles<T, 7, PER>(st, c, columns, e, tiles, turns);
+    default: return run_tiles<T, 8, PER>(st, c, columns, e, tiles, turns);
     }
 }
 
@@ -715,12 +760,10 @@ hipError_t launch_fourbit_scores(hipStream_t st, const FourbitCall &c, char *scr
     const int64_t each = rows_a_turn(c);
     const int64_t row = c.h_stride * (c.bf16 ? 2 : 4);
     const bool wide_h = reinterpret_cast<uintptr_t>(c.h) % 16 == 0 && row % 16 == 0;
-    const bool wide_scores = reinterpret_cast<uintptr_t>(c.scores) % 16 == 0 && c.score_stride % 4 == 0;
     for (int64_t r = 0; r < c.rows; r += each) {
         FourbitCall part = c;
         part.rows = std::min(each, c.rows - r);
         part.wide_h = wide_h;
-        part.wide_scores = wide_scores;
         part.h = static_cast<const char *>(c.h) + r * row;
         part.scores = c.scores + r * c.score_stride;
         const hipError_t e = c.bf16 ? run<__bf16>(st, part, scratch) : run<float>(st, part, scratch);

@@ -145,7 +145,7 @@ struct FourbitCall {
     const float *bias;               // NULL: none
     float *scores;
     int64_t score_stride;
-    bool wide_h, wide_scores;        // rows at multiples of 16 bytes; set by the launcher
+    bool wide_h;                     // rows at multiples of 16 bytes; set by the launcher
     int num_cus;
 };
 size_t fourbit_scratch(const FourbitCall &c);
