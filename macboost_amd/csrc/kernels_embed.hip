@@ -408,8 +408,9 @@ __global__ __launch_bounds__(SMALL_THREADS) void k_embed_sort_small(Pass p, int3
 //
 // A worker's end that falls into an entry's rows is put behind them if they are at most `per`;
 // else the entry is longer than a worker: each of its workers leaves its sum in parts, and the
-// one in which it ends puts it on the list that k_embed_join works off.  Sums of a worker are
-// in the rows' order, those of parts in a fixed order too: the same bits in every run.
+// one in which it ends puts it on the list that k_embed_join works off.  Where all of a workgroup's
+// workers are inside one entry, they leave one sum, as their first one's.  Sums of a worker are in
+// the rows' order, those of parts in a fixed order too: the same bits in every run.
 // ---------------------------------------------------------------------------
 constexpr int SUM_WAVES = 4, SUM_THREADS = 64 * SUM_WAVES;
 constexpr int MOST_ITEMS = 4096;     // of a workgroup
@@ -572,9 +573,12 @@ __global__ __launch_bounds__(SUM_THREADS) void k_embed_sum(Sums s) {
     }
     __syncthreads();
     const int lane = threadIdx.x & 63, group = lane / s.lanes;
-    const int64_t worker = first + (threadIdx.x >> 6) * s.groups + group;
-    const int32_t chunk = blockIdx.y * 64 + lane - group * s.lanes;
-    if (group >= s.groups || worker >= s.workers || chunk >= s.chunks) return;
+    const int mine = (threadIdx.x >> 6) * s.groups + min(group, s.groups - 1);
+    const int64_t worker = min(first + mine, s.workers - 1);
+    const int32_t chunk = min(blockIdx.y * 64 + lane - group * s.lanes, s.chunks - 1);
+    // lanes without a worker or columns of their own do another's work and write none of it
+    const bool idle = group >= s.groups || first + mine >= s.workers ||
+                      (int)(blockIdx.y * 64) + lane - group * s.lanes >= s.chunks;
     const Cut from = cut_at(s, key, begin, held, lo, hi, worker * s.per);
     Cut to = cut_at(s, key, begin, held, lo, hi, (worker + 1) * s.per);
     if (to.i > from.i && key[to.i - 1] >= s.entries)         // rows that are left out, behind all
@@ -599,6 +603,7 @@ __global__ __launch_bounds__(SUM_THREADS) void k_embed_sum(Sums s) {
     for (int e = 0; e < E; ++e) acc[e] = 0.0f;
     bool head = from.open;
     const auto leave = [&](int side) {
+        if (idle) return;
 #pragma unroll
         for (int e = 0; e < E; ++e) parts[side * s.part_stride + e] = acc[e];
     };
@@ -645,7 +650,7 @@ __global__ __launch_bounds__(SUM_THREADS) void k_embed_sum(Sums s) {
             const uint32_t entry = what[q] & ~ENTRY;
             if (head) {
                 leave(0);
-                if (chunk == 0) {
+                if (!idle && chunk == 0) {
                     const uint32_t at = atomicAdd(&s.found[0], 1u);
                     s.found[2 + 2 * at] = (uint32_t)worker;
                     s.found[3 + 2 * at] = entry;
@@ -656,62 +661,103 @@ __global__ __launch_bounds__(SUM_THREADS) void k_embed_sum(Sums s) {
 #pragma unroll
                 for (int e = 0; e < E; ++e)
                     out[e] = (T)__builtin_fmaf(s.scale, acc[e], BASE ? to_f32(v[q][e]) : 0.0f);
-                put(reinterpret_cast<Run<T, E> *>(dtable + entry * s.table_stride), out, s.streamed);
+                if (!idle)
+                    put(reinterpret_cast<Run<T, E> *>(dtable + entry * s.table_stride), out,
+                        s.streamed);
             }
 #pragma unroll
             for (int e = 0; e < E; ++e) acc[e] = 0.0f;
         }
     }
-    if (to.open) leave(1);
-    if (chunk == 0) s.open[worker] = to.open ? to.e : NOTHING;
+    if (!idle && chunk == 0) s.open[worker] = to.open ? to.e : NOTHING;
+    const bool inside = from.open && to.open && from.e == to.e;
+    const int here = (int)min((int64_t)SUM_WAVES * s.groups, s.workers - first);
+    if (!__syncthreads_and(inside) || here == 1) {
+        if (to.open) leave(1);
+        return;
+    }
+    float *meet = reinterpret_cast<float *>(lds) + threadIdx.x * E;
+    const int stride = s.lanes * E;                  // between the workers of a wavefront
+#pragma unroll
+    for (int e = 0; e < E; ++e) meet[e] = acc[e];
+    for (int o = 128; o > 0; o >>= 1) {              // at most 256 workers
+        __syncthreads();
+        const int other = mine + o;
+        if (!idle && mine < o && other < here) {
+            const float *from_other =
+                meet + ((other / s.groups - (int)(threadIdx.x >> 6)) * 64 * E) +
+                (other % s.groups - group) * stride;
+#pragma unroll
+            for (int e = 0; e < E; ++e) meet[e] += from_other[e];
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = meet[e];
+    if (mine == 0) leave(1);
 }
 
 // The entries on the list: heads and tails of their workers, from the first that left the entry
-// open to the one in which it ends.  A wavefront an entry, or all of a workgroup's an entry of
-// more than WAVE_PARTS parts: slices of the parts are summed side by side, and the slices' sums
-// in their order.
+// open to the one in which it ends; of workgroups all inside it, one tail.  A wavefront an entry,
+// or all of a workgroup's an entry of more than WAVE_PARTS parts: slices of the parts are summed
+// side by side, and the slices' sums by halves.
 constexpr int JOIN_WAVES = 4, JOIN_THREADS = 64 * JOIN_WAVES;
 constexpr int WAVE_PARTS = 64;
 constexpr int PARTS = 8;             // parts on the way
+struct Span {
+    int32_t start, last;             // workers
+    int32_t blocks, behind;          // the first worker of the workgroups all inside, and behind them
+    int32_t inside, each;            // how many workgroups, of how many workers
+    uint32_t entry;
+    __device__ __forceinline__ int32_t parts() const {
+        return last + 1 - start - (behind - blocks) + inside;
+    }
+    // The place in parts of the i-th part.
+    __device__ __forceinline__ int64_t at(int32_t i) const {
+        const int32_t before = blocks - start;
+        const int32_t w = i < before ? start + i
+                          : i < before + inside ? blocks + (i - before) * each
+                                                : behind + (i - before - inside);
+        return (int64_t)w * 2 + (w < last);
+    }
+};
 template <typename T>
 __global__ __launch_bounds__(JOIN_THREADS) void k_embed_join(Sums s) {
     typedef float V __attribute__((ext_vector_type(4)));
     __shared__ V sums[JOIN_THREADS];
-    __shared__ int64_t firsts[JOIN_WAVES];
+    __shared__ Span spans[JOIN_WAVES];
     const uint32_t count = s.found[0];
     const int fours = s.part_stride / 4, wide = min(fours, 64), groups = 64 / wide;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, group = lane / wide;
     const int col0 = lane - group * wide;
-    // Slice `slice` of `slices` of the parts [start, last] of four columns, met in sums[at ...].
-    const auto part_sum = [&](int64_t start, int64_t last, int slice, int slices, int four) {
-        const int64_t each = (last - start + slices) / slices;      // of last - start + 1 parts
-        const int64_t a = start + slice * each, b = min(a + each, last + 1);
+    // Slice `slice` of `slices` of a span's parts, four columns.
+    const auto part_sum = [&](const Span &x, int slice, int slices, int four) {
+        const int32_t n = x.parts(), each = (n + slices - 1) / slices;
+        const int32_t a = slice * each, b = min(a + each, n);
         V sum = {0, 0, 0, 0};
         if (group < groups && four < fours)
-            for (int64_t w = a; w < b; w += PARTS) {
+            for (int32_t i = a; i < b; i += PARTS) {
                 V v[PARTS];
 #pragma unroll
-                for (int q = 0; q < PARTS; ++q) {
-                    const int64_t x = min(w + q, b - 1);
+                for (int q = 0; q < PARTS; ++q)
                     v[q] = *reinterpret_cast<const V *>(
-                        s.parts + (x * 2 + (x < last)) * s.part_stride + four * 4);
-                }
+                        s.parts + x.at(min(i + q, b - 1)) * s.part_stride + four * 4);
 #pragma unroll
                 for (int q = 0; q < PARTS; ++q)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) sum[e] += w + q < b ? v[q][e] : 0.0f;
+                    for (int e = 0; e < 4; ++e) sum[e] += i + q < b ? v[q][e] : 0.0f;
             }
         sums[threadIdx.x] = sum;
     };
-    // The slices' sums of a wavefront, or of all.
-    const auto finish = [&](uint32_t entry, int first_wave, int slices, int four) {
-        if (group != 0 || four >= fours) return;
-        V total = {0, 0, 0, 0};
-        for (int v = 0; v < slices; ++v) {
-            const V part = sums[(first_wave + v / groups) * 64 + (v % groups) * wide + col0];
+    // The sum of slice v and the one o behind.
+    const auto halve = [&](int v, int o, int slices, int first_wave) {
+        if (group >= groups || v >= o || v + o >= slices) return;
+        const V other = sums[(first_wave + (v + o) / groups) * 64 + (v + o) % groups * wide + col0];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) total[e] += part[e];
-        }
+        for (int e = 0; e < 4; ++e) sums[threadIdx.x][e] += other[e];
+    };
+    const auto write = [&](uint32_t entry, int four) {
+        if (group != 0 || four >= fours) return;
+        const V total = sums[threadIdx.x];
         const int col = four * 4;
         const int64_t at = (int64_t)entry * s.table_stride + col;
 #pragma unroll
@@ -721,42 +767,60 @@ __global__ __launch_bounds__(JOIN_THREADS) void k_embed_join(Sums s) {
                 static_cast<T *>(s.dtable)[at + e] = (T)__builtin_fmaf(s.scale, total[e], b0);
             }
     };
-    for (uint32_t f0 = blockIdx.x * JOIN_WAVES; f0 < count; f0 += gridDim.x * JOIN_WAVES) {
-        const uint32_t mine = f0 + wave;
-        int64_t last = 0, start = 0;
-        uint32_t entry = NOTHING;
-        if (mine < count) {
-            last = start = s.found[2 + 2 * mine];
-            entry = s.found[3 + 2 * mine];
+    // few entries: one a workgroup
+    const uint32_t turn = count > gridDim.x ? JOIN_WAVES : 1;
+    for (uint32_t f0 = blockIdx.x * turn; f0 < count; f0 += gridDim.x * turn) {
+        const uint32_t f = f0 + wave;
+        Span x{};
+        x.each = SUM_WAVES * s.groups;
+        x.last = -1;
+        const bool has = (uint32_t)wave < turn && f < count;
+        if (has) {
+            x.last = x.start = (int32_t)s.found[2 + 2 * f];
+            x.entry = s.found[3 + 2 * f];
             // the entry's workers lie side by side: the 64 before, or 64-ary search
-            const int64_t w = start - 1 - lane;
-            const int n = __popcll(__ballot(w >= 0 && s.open[w] == entry));
-            start -= n;
-            int64_t lo = 0;
-            while (n == 64 && start > lo) {          // the first one is in [lo, start]
-                const int64_t step = (start - lo + 63) / 64, m = start - step * (lane + 1);
-                const int more = __popcll(__ballot(m >= lo && s.open[max(m, lo)] == entry));
-                lo = max(lo, start - step * (more + 1) + 1);
-                start -= step * more;
+            const int w = x.start - 1 - lane;
+            const int n = __popcll(__ballot(w >= 0 && s.open[max(w, 0)] == x.entry));
+            x.start -= n;
+            int lo = 0;
+            while (n == 64 && x.start > lo) {        // the first one is in [lo, start]
+                const int step = (x.start - lo + 63) / 64;
+                const int64_t m = x.start - (int64_t)step * (lane + 1);
+                const int more =
+                    __popcll(__ballot(m >= lo && s.open[max(m, (int64_t)lo)] == x.entry));
+                lo = (int)max((int64_t)lo, x.start - (int64_t)step * (more + 1) + 1);
+                x.start -= step * more;
             }
+            x.blocks = (x.start / x.each + 1) * x.each;
+            x.behind = x.last / x.each * x.each;
+            if (x.blocks >= x.behind) x.blocks = x.behind = x.last;
+            x.inside = (x.behind - x.blocks) / x.each;
         }
-        if (lane == 0) firsts[wave] = start;
+        if (lane == 0) spans[wave] = x;
         __syncthreads();
         for (int four0 = blockIdx.y * wide; four0 < fours; four0 += gridDim.y * wide) {
             const int four = four0 + col0;
-            if (mine < count && last - start < WAVE_PARTS) {
-                part_sum(start, last, group, groups, four);
+            if (has && x.parts() <= WAVE_PARTS) {
+                part_sum(x, group, groups, four);
+                for (int o = 32; o > 0; o >>= 1) {
+                    __builtin_amdgcn_wave_barrier();
+                    halve(group, o, groups, wave);
+                }
                 __builtin_amdgcn_wave_barrier();
-                finish(entry, wave, groups, four);
+                write(x.entry, four);
                 __builtin_amdgcn_wave_barrier();
             }
-            for (uint32_t x = 0; x < JOIN_WAVES && f0 + x < count; ++x) {
-                const int64_t of = s.found[2 + 2 * (f0 + x)];
-                if (of - firsts[x] < WAVE_PARTS) continue;
+            for (uint32_t y = 0; y < turn && f0 + y < count; ++y) {
+                if (spans[y].parts() <= WAVE_PARTS) continue;
+                const int slice = wave * groups + group, slices = JOIN_WAVES * groups;
                 __syncthreads();
-                part_sum(firsts[x], of, wave * groups + group, JOIN_WAVES * groups, four);
+                part_sum(spans[y], slice, slices, four);
+                for (int o = 32 * JOIN_WAVES; o > 0; o >>= 1) {
+                    __syncthreads();
+                    halve(slice, o, slices, 0);
+                }
                 __syncthreads();
-                if (wave == 0) finish(s.found[3 + 2 * (f0 + x)], 0, JOIN_WAVES * groups, four);
+                if (wave == 0) write(spans[y].entry, four);
                 __syncthreads();
             }
         }
@@ -844,7 +908,8 @@ hipError_t sort_pass(hipStream_t st, const Pass &p) {
 template <typename T, int E, bool BASE, bool ONE>
 void sums(hipStream_t st, const Sums &s, int cols) {
     const int64_t each = SUM_WAVES * s.groups;
-    const size_t lds = sizeof(uint32_t) * (4 * (size_t)held_rows((int)each * s.per, s.per) + 1);
+    const size_t lds = sizeof(uint32_t) * std::max(4 * (size_t)held_rows((int)each * s.per, s.per) + 1,
+                                                   (size_t)SUM_THREADS * E);
     hipLaunchKernelGGL((k_embed_sum<T, E, BASE, ONE>),
                        grid_of((s.workers + each - 1) / each, (uint32_t)cols), dim3(SUM_THREADS), lds,
                        st, s);
