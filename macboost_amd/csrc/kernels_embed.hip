@@ -324,7 +324,7 @@ __global__ __launch_bounds__(SORT_THREADS) void k_embed_place(Pass p) {
 // (16384 rows of 17 bits take 46 us so, 20 by the kernels above.)
 constexpr int SMALL_WAVES = 16, SMALL_THREADS = 64 * SMALL_WAVES, SMALL_EACH = 4;
 constexpr int64_t SMALL_ROWS = SMALL_THREADS * SMALL_EACH;
-constexpr int SMALL_BITS = 8;
+constexpr int SMALL_BITS = 10;
 __global__ __launch_bounds__(SMALL_THREADS) void k_embed_sort_small(Pass p, int32_t passes) {
     extern __shared__ uint32_t lds[];
     const int bins = 1 << p.bits;
@@ -882,6 +882,7 @@ GradShape grad_shape(const EmbedCall &c) {
     // 16 to 64 items a worker, as many as leave every CU 16 wavefronts
     const int64_t workers = (int64_t)16 * c.num_cus * g.groups / g.cols + 1;
     int64_t per = std::min<int64_t>(64, std::max<int64_t>(16, items / workers));
+    if (c.rows <= 64) per = 64;          // no entry is longer than a worker: nothing to join
     per = std::min<int64_t>(per, MOST_ITEMS / (SUM_WAVES * g.groups));
     g.items = (int)per;
     g.workers = (items + per - 1) / per;
@@ -924,6 +925,7 @@ template <typename T>
 hipError_t sums(hipStream_t st, const Sums &s, const GradShape &g, int num_cus) {
     constexpr int E = 16 / sizeof(T);
     g.elements > 1 ? sums<T, E>(st, s, g.cols) : sums<T, 1>(st, s, g.cols);
+    if (s.rows <= s.per) return hipGetLastError();       // no entry is longer than a worker
     const int turns = (s.part_stride / 4 + 63) / 64;
     hipLaunchKernelGGL((k_embed_join<T>),
                        dim3((uint32_t)(4 * num_cus), (uint32_t)std::min(turns, 16)),

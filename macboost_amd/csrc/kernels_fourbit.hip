@@ -14,6 +14,7 @@
 // lane loads those of four blocks at once, and behind those each class's exponent as int32,
 // [tile][class].
 #include <algorithm>
+#include <type_traits>
 
 #include "grid.hpp"
 #include "mbk.h"
@@ -45,67 +46,6 @@ __device__ __forceinline__ int exponent(float v) {
     return v == 0.0f ? 0 : v < __builtin_inff() ? ilogbf(v) : 127;
 }
 
-// A workgroup a tile and a run of its blocks; a wavefront a block: two passes over W, the
-// first for the largest scale of each class.
-template <typename T>
-__global__ __launch_bounds__(256) void k_fourbit_pack(FourbitShape s, const T *__restrict__ w,
-                                                 int64_t stride, uint32_t *__restrict__ codes,
-                                                 _Float16 *__restrict__ scales,
-                                                 int32_t *__restrict__ exponents) {
-    __shared__ float most[256];
-    const int64_t tile = group_id();
-    if (tile * TILE >= s.classes) return;
-    const int c = threadIdx.x & 15, part = threadIdx.x >> 4;       // 16 parts a class
-    const int64_t cls = tile * TILE + c;
-    const bool real = cls < s.classes;
-    const T *row = w + (real ? cls : 0) * stride;
-    const int blocks = s.blocks, quads = (blocks + 3) / 4, per = BLOCK / s.group;
-    const int groups = quads * 4 * per;
-    const auto scale_of = [&](int g) {
-        float m = 0.0f;
-        bool finite = true;
-        if (real)
-            for (int k = g * s.group; k < min(s.dim, (g + 1) * s.group); ++k) {
-                const float v = fabsf(to_f32(row[k]));
-                finite &= v < __builtin_inff();
-                m = fmaxf(m, v);
-            }
-        // f32(1 / 7); NaN reaches every score of the class
-        return finite ? bf16_rounded(m * 0x1.24924ap-3f) : __builtin_nanf("");
-    };
-    float m = 0.0f;
-    for (int g = part; g < groups; g += 16) m = fmaxf(m, scale_of(g));
-    most[threadIdx.x] = m;
-    __syncthreads();
-    for (int p = 0; p < 16; ++p) m = fmaxf(m, most[p * 16 + c]);
-    const int e = exponent(m) - TOP;
-    if (part == 0) exponents[cls] = e;
-    for (int g = part; g < groups; g += 16) {
-        const float scale = scale_of(g);
-        scales[((tile * quads + g / (4 * per)) * TILE + c) * 4 * per + g % (4 * per)] =
-            (_Float16)ldexpf(scale, -e);
-        if (g >= blocks * per) continue;
-        for (int k0 = g * s.group; k0 < (g + 1) * s.group; k0 += 8) {
-            uint32_t word = 0;
-            for (int i = 0; i < 8; ++i) {
-                float code = 0.0f;
-                if (real && k0 + i < s.dim && scale > 0.0f)
-                    code = rintf(to_f32(row[k0 + i]) / scale);
-                const uint32_t n = (uint32_t)((int)fminf(fmaxf(code, -8.0f), 7.0f) + 8);
-                word |= n << (4 * ((i >> 1) + 4 * (i & 1)));
-            }
-            const int block = k0 / BLOCK, j = k0 % BLOCK / 32, q = k0 % 32 / 8;
-            codes[(((tile * blocks + block) * 64) + q * 16 + c) * 4 + j] = word;
-        }
-    }
-}
-
-// h as columns of f16 terms: column r of bf16 rows, columns 2 r and 2 r + 1 of f32 rows (the row
-// and 2^11 times what its f16 leaves, 22 bits together), a power of two apart that brings the row's
-// largest near the top of f16's range.  As the matrix instruction takes them: [column tile][32
-// elements][lane][8], lane q * 16 + column with the elements 8 q + i.
-template <typename T> constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;
-
 // Eight elements of a row from k on, 0 behind its end.
 template <typename T>
 __device__ __forceinline__ void eight(const T *row, int k, int dim, bool wide, float (&v)[8]) {
@@ -123,6 +63,92 @@ __device__ __forceinline__ void eight(const T *row, int k, int dim, bool wide, f
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = k + i < dim ? to_f32(row[k + i]) : 0.0f;
 }
+
+// A workgroup a tile of classes, a wavefront a block of it at a time, in the lanes that hold its
+// codes: the scales first, for the class's exponent, and then all again.  100000 x 1024 bf16 91
+// us, f32 153, the second reading from L2.
+constexpr int PACK_WAVES = 4;
+template <typename T, int PER>
+__global__ __launch_bounds__(64 * PACK_WAVES) void k_fourbit_pack(
+    FourbitShape s, const T *__restrict__ w, int64_t stride, bool wide, uint4v *__restrict__ codes,
+    _Float16 *__restrict__ scales, int32_t *__restrict__ exponents) {
+    __shared__ float most[PACK_WAVES][TILE];
+    const int64_t tile = group_id();
+    if (tile * TILE >= s.classes) return;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
+    const int64_t cls = tile * TILE + c;
+    const T *row = w + (cls < s.classes ? cls : 0) * stride;
+    const int dim = cls < s.classes ? s.dim : 0;
+    const int quads = (s.blocks + 3) / 4;
+    // The lane's 32 elements of a block and the scales of its groups.
+    const auto block = [&](int b, float (&v)[4][8], float (&scale)[PER]) {
+        float m[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            eight(row, b * BLOCK + j * 32 + q * 8, dim, wide, v[j]);
+            m[j] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float x = fabsf(v[j][i]);
+                m[j] = fmaxf(m[j], x < __builtin_inff() ? x : __builtin_inff());
+            }
+            m[j] = fmaxf(m[j], __shfl_xor(m[j], 16, 64));
+            m[j] = fmaxf(m[j], __shfl_xor(m[j], 32, 64));
+        }
+#pragma unroll
+        for (int g = 0; g < PER; ++g) {
+            float all = 0.0f;
+#pragma unroll
+            for (int j = g * 4 / PER; j < (g + 1) * 4 / PER; ++j) all = fmaxf(all, m[j]);
+            // f32(1 / 7); what is not finite reaches every score of the class
+            scale[g] = all < __builtin_inff() ? bf16_rounded(all * 0x1.24924ap-3f)
+                                              : __builtin_nanf("");
+        }
+    };
+    float v[4][8], scale[PER], m = 0.0f;
+    for (int b = wave; b < s.blocks; b += PACK_WAVES) {
+        block(b, v, scale);
+#pragma unroll
+        for (int g = 0; g < PER; ++g) m = fmaxf(m, scale[g]);
+    }
+    if (q == 0) most[wave][c] = m;
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < PACK_WAVES; ++x) m = fmaxf(m, most[x][c]);
+    const int e = exponent(m) - TOP;
+    if (wave == 0 && q == 0) exponents[cls] = e;
+    for (int b = wave; b < quads * 4; b += PACK_WAVES) {
+#pragma unroll
+        for (int g = 0; g < PER; ++g) scale[g] = 0.0f;
+        if (b < s.blocks) {
+            block(b, v, scale);
+            uint4v words;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float by = scale[j * PER / 4];
+                words[j] = 0;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float code = by > 0.0f ? rintf(v[j][i] / by) : 0.0f;
+                    words[j] |= (uint32_t)((int)fminf(fmaxf(code, -8.0f), 7.0f) + 8)
+                                << (4 * ((i >> 1) + 4 * (i & 1)));
+                }
+            }
+            codes[(tile * s.blocks + b) * 64 + lane] = words;
+        }
+        if (q == 0)
+#pragma unroll
+            for (int g = 0; g < PER; ++g)
+                scales[(((tile * quads + b / 4) * TILE + c) * 4 + b % 4) * PER + g] =
+                    (_Float16)ldexpf(scale[g], -e);
+    }
+}
+
+// h as columns of f16 terms: column r of bf16 rows, columns 2 r and 2 r + 1 of f32 rows (the row
+// and 2^11 times what its f16 leaves, 22 bits together), a power of two apart that brings the row's
+// largest near the top of f16's range.  As the matrix instruction takes them: [column tile][32
+// elements][lane][8], lane q * 16 + column with the elements 8 q + i.
+template <typename T> constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;
 
 // A wavefront's part of a tile of columns: the steps first, first + each, ... of the largest |h|
 // of the lane's row, over all of its lanes.
@@ -740,13 +766,21 @@ hipError_t launch_fourbit_pack(hipStream_t st, const FourbitShape &s, bool bf16,
     _Float16 *scales;
     int32_t *exponents;
     fourbit_parts(s, packed, &codes, &scales, &exponents);
+    const bool wide = reinterpret_cast<uintptr_t>(w) % 16 == 0 && stride * (bf16 ? 2 : 4) % 16 == 0;
     const dim3 g = grid_of((s.classes + TILE - 1) / TILE);
-    if (bf16)
-        hipLaunchKernelGGL((k_fourbit_pack<__bf16>), g, dim3(256), 0, st, s,
-                           static_cast<const __bf16 *>(w), stride, codes, scales, exponents);
-    else
-        hipLaunchKernelGGL((k_fourbit_pack<float>), g, dim3(256), 0, st, s,
-                           static_cast<const float *>(w), stride, codes, scales, exponents);
+    const auto launch = [&](auto type, auto per) {
+        using T = decltype(type);
+        hipLaunchKernelGGL((k_fourbit_pack<T, decltype(per)::value>), g, dim3(64 * PACK_WAVES), 0, st,
+                           s, static_cast<const T *>(w), stride, wide,
+                           reinterpret_cast<uint4v *>(codes), scales, exponents);
+    };
+    const auto typed = [&](auto type) {
+        if (s.group == 32) launch(type, std::integral_constant<int, 4>{});
+        else if (s.group == 64) launch(type, std::integral_constant<int, 2>{});
+        else launch(type, std::integral_constant<int, 1>{});
+    };
+    if (bf16) typed(__bf16{});
+    else typed(float{});
     return hipGetLastError();
 }
 

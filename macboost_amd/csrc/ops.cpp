@@ -281,6 +281,10 @@ int mbk_tensors_create(mbk_context *ctx, const mbk_tensor *list, int32_t count, 
                  "gradients must have at most 2^38 elements together");
             elements += t.rows * t.cols;
             need(t.grad || !t.rows || !t.cols, "null gradient");
+            const uintptr_t size = t.type == MBK_BF16 ? 2 : 4;
+            need(reinterpret_cast<uintptr_t>(t.grad) % size == 0 &&
+                     reinterpret_cast<uintptr_t>(t.out) % size == 0,
+                 "grad and out must be multiples of their elements' size");
         }
         std::vector<mbk::ClipPiece> pieces;
         auto made = std::make_unique<mbk_tensors>();

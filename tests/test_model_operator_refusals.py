@@ -61,6 +61,7 @@ TENSOR = {"grad": P, "out": None, "rows": 2, "cols": 3, "stride": 3, "type": 0}
     ({"stride": 2}, "stride must be in"), ({"stride": 2 ** 40 + 1}, "stride must be in"),
     ({"rows": 2 ** 20, "cols": 2 ** 19, "stride": 2 ** 19}, "at most 2.38 elements together"),
     ({"grad": None}, "null gradient"), ({"type": 3}, "type must be"),
+    ({"grad": P + 2}, "multiples of their"), ({"out": P + 1, "type": 1}, "multiples of their"),
     ({}, "null kernel-seam context"), ({"rows": 0, "grad": None}, "null kernel-seam context"),
 ])
 def test_tensors(change, msg):
