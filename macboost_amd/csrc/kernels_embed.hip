@@ -406,7 +406,7 @@ __global__ __launch_bounds__(SMALL_THREADS) void k_embed_sort_small(Pass p, int3
 // (an entry its base) is on the way AHEAD items at a time.  Where dtable is its own base, entries
 // without rows are not on the list, and a worker takes `per` rows.
 //
-// A worker's end that falls into an entry's rows is put behind them if they are at most `per`;
+// A worker's end that falls into an entry's rows is put behind them if they are at most `whole`;
 // else the entry is longer than a worker: each of its workers leaves its sum in parts, and the
 // one in which it ends puts it on the list that k_embed_join works off.  Where all of a workgroup's
 // workers are inside one entry, they leave one sum, as their first one's.  Sums of a worker are in
@@ -424,6 +424,7 @@ struct Sums {
     int32_t dim, chunks;             // pieces of E columns
     int32_t lanes, groups;           // of a worker; workers a wavefront
     int32_t per;
+    int32_t whole;                   // rows of an entry that are not parted: per, or all rows
     bool dense;                      // entries without rows are on the list
     bool streamed;                   // dtable is stored past the caches
     int64_t row_stride, table_stride;
@@ -437,13 +438,13 @@ struct Sums {
     uint32_t *found;                 // [0]: how many; then (worker, entry)
 };
 // Rows that a workgroup of `items` items may look at.
-__host__ __device__ constexpr int held_rows(int items, int per) { return items + 2 * per + 2; }
+__host__ __device__ constexpr int held_rows(int items, int whole) { return items + 2 * whole + 2; }
 
 // Rows and entries before an item.  i counts from the first row that the workgroup holds in LDS.
 struct Cut {
     int i;
     uint32_t e;
-    bool open;                       // e's rows begin before i, and there are more than `per`
+    bool open;                       // e's rows begin before i, and there are more than `whole`
 };
 
 // The first of [lo, hi) for which under() does not hold, which does for all before.
@@ -473,10 +474,10 @@ __device__ __forceinline__ Cut cut_at(const Sums &s, const uint32_t *key, int64_
         c.open = d > 0 && d < s.rows && c.e < s.entries && key[c.i] == c.e;
     }
     if (!c.open) return c;
-    const int a = first_not(max(0, c.i - s.per - 1), c.i, [&](int m) { return key[m] < c.e; });
-    const int b = first_not(c.i, min(held, c.i + s.per + 1),
+    const int a = first_not(max(0, c.i - s.whole - 1), c.i, [&](int m) { return key[m] < c.e; });
+    const int b = first_not(c.i, min(held, c.i + s.whole + 1),
                             [&](int m) { return key[m] <= c.e; });
-    if (b - a <= s.per) {
+    if (b - a <= s.whole) {
         c.i = b;
         c.e += 1;
         c.open = false;
@@ -529,7 +530,7 @@ template <typename T, int E, bool BASE, bool ONE>
 __global__ __launch_bounds__(SUM_THREADS) void k_embed_sum(Sums s) {
     extern __shared__ uint32_t lds[];
     __shared__ uint32_t wave_sum[SUM_WAVES];
-    const int items = SUM_WAVES * s.groups * s.per, most = held_rows(items, s.per);
+    const int items = SUM_WAVES * s.groups * s.per, most = held_rows(items, s.whole);
     uint32_t *key = lds;                             // [row]
     uint32_t *item = key + most;                     // [item]: a row, or an entry
     uint32_t *place = item + 2 * most;               // [row] its item, where it is not i + key
@@ -539,17 +540,17 @@ __global__ __launch_bounds__(SUM_THREADS) void k_embed_sum(Sums s) {
                                              s.rows + (s.dense ? (int64_t)s.entries : 0))};
     int64_t ends[2] = {d[0], d[1]};
     if (s.dense) both_ends(s, d, ends);
-    const int64_t begin = max((int64_t)0, ends[0] - s.per - 1);
-    const int held = (int)(min(s.rows, ends[1] + s.per + 1) - begin);
+    const int64_t begin = max((int64_t)0, ends[0] - s.whole - 1);
+    const int held = (int)(min(s.rows, ends[1] + s.whole + 1) - begin);
     const int lo = (int)(ends[0] - begin), hi = (int)(ends[1] - begin);
     if (s.dense) {
-        for (int i = threadIdx.x; i < items + s.per + 2; i += SUM_THREADS) item[i] = ENTRY;
+        for (int i = threadIdx.x; i < items + s.whole + 2; i += SUM_THREADS) item[i] = ENTRY;
         __syncthreads();
         for (int i = threadIdx.x; i < held; i += SUM_THREADS) {
             const uint2 x = s.sorted[begin + i];
             key[i] = x.x;
             const int64_t at = begin + i + (int64_t)x.x - d[0];
-            if (at >= 0 && at < items + s.per + 2 && x.x < s.entries) item[at] = x.y;
+            if (at >= 0 && at < items + s.whole + 2 && x.x < s.entries) item[at] = x.y;
         }
     } else {
         for (int i = threadIdx.x; i < held; i += SUM_THREADS) key[i] = s.sorted[begin + i].x;
@@ -844,7 +845,7 @@ struct GradShape {
     int64_t per;                     // rows a workgroup of the sort, or a wavefront
     int each;                        // R
     bool narrow;                     // counts of 16 bits
-    int lanes, groups, cols, items, chunks;
+    int lanes, groups, cols, items, whole, chunks;
     int elements;                    // E
     bool dense;
     int64_t workers;
@@ -882,9 +883,9 @@ GradShape grad_shape(const EmbedCall &c) {
     // 16 to 64 items a worker, as many as leave every CU 16 wavefronts
     const int64_t workers = (int64_t)16 * c.num_cus * g.groups / g.cols + 1;
     int64_t per = std::min<int64_t>(64, std::max<int64_t>(16, items / workers));
-    if (c.rows <= 64) per = 64;          // no entry is longer than a worker: nothing to join
     per = std::min<int64_t>(per, MOST_ITEMS / (SUM_WAVES * g.groups));
     g.items = (int)per;
+    g.whole = c.rows <= 64 ? 64 : g.items;           // few rows: nothing to join
     g.workers = (items + per - 1) / per;
     return g;
 }
@@ -909,7 +910,7 @@ hipError_t sort_pass(hipStream_t st, const Pass &p) {
 template <typename T, int E, bool BASE, bool ONE>
 void sums(hipStream_t st, const Sums &s, int cols) {
     const int64_t each = SUM_WAVES * s.groups;
-    const size_t lds = sizeof(uint32_t) * std::max(4 * (size_t)held_rows((int)each * s.per, s.per) + 1,
+    const size_t lds = sizeof(uint32_t) * std::max(4 * (size_t)held_rows((int)each * s.per, s.whole) + 1,
                                                    (size_t)SUM_THREADS * E);
     hipLaunchKernelGGL((k_embed_sum<T, E, BASE, ONE>),
                        grid_of((s.workers + each - 1) / each, (uint32_t)cols), dim3(SUM_THREADS), lds,
@@ -925,7 +926,7 @@ template <typename T>
 hipError_t sums(hipStream_t st, const Sums &s, const GradShape &g, int num_cus) {
     constexpr int E = 16 / sizeof(T);
     g.elements > 1 ? sums<T, E>(st, s, g.cols) : sums<T, 1>(st, s, g.cols);
-    if (s.rows <= s.per) return hipGetLastError();       // no entry is longer than a worker
+    if (s.rows <= s.whole) return hipGetLastError();     // no entry is parted
     const int turns = (s.part_stride / 4 + 63) / 64;
     hipLaunchKernelGGL((k_embed_join<T>),
                        dim3((uint32_t)(4 * num_cus), (uint32_t)std::min(turns, 16)),
@@ -1015,6 +1016,7 @@ hipError_t launch_embed_grad(hipStream_t st, const EmbedCall &c, char *scratch) 
     s.lanes = g.lanes;
     s.groups = g.groups;
     s.per = g.items;
+    s.whole = g.whole;
     s.dense = g.dense;
     s.streamed = g.dense && c.entries * c.dim * (c.bf16 ? 2 : 4) > STREAMED;
     s.row_stride = c.row_stride;
