@@ -448,10 +448,10 @@ int mbk_grad_clip(mbk_context *ctx, mbk_tensors *list, float max_norm, float *no
  * library's own).  mbk_fourbit_bytes is -1 for a shape that the calls refuse.
  * mbk_fourbit_scores: scores[row][v] = h[row] . w[v] + bias[v] (bias NULL: 0), f32; a class whose bias
  * is -INFINITY has that score whatever its w and h hold.
- * Elements of w are taken as they are, but for what is below 2^-28 of its class's largest scale,
- * off by up to 2^-36 of that scale; bf16 h as it is, but for what is below 2^-29 of its row's
- * largest, off by up to 2^-39 of that; f32 h with 22 bits, and beside the row's largest off by up
- * to 2^-49 of it.  Sums are f32, rounded with the bias once more.  A class whose w is not finite
+ * Elements of w are taken as they are, but for groups whose scale is below 2^-28 of their class's
+ * largest, whose elements are off by up to 2^-33 of that scale; bf16 h as it is, but for what is
+ * below 2^-31 of its row's largest, off by up to 2^-39 of that; f32 h with 22 bits, and beside the
+ * row's largest off by up to 2^-50 of it.  Sums are f32, rounded with the bias once more.  A class whose w is not finite
  * has scores that are NaN, a row whose h is not finite has scores that are not finite. */
 typedef struct {
     int64_t classes;             /* 1..2^31-256 */
