@@ -112,14 +112,21 @@ __device__ __forceinline__ uint32_t lanes_below(uint64_t mask) {
                                      __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0u));
 }
 
-// Lanes with this lane's digit, among those that are here.
-__device__ __forceinline__ uint64_t same_digit(uint32_t digit, bool here, int bits) {
-    uint64_t same = __ballot(here);
-    for (int k = 0; k < bits; ++k) {
-        const uint64_t ones = __ballot((digit >> k) & 1u);
-        same &= (digit >> k) & 1u ? ones : ~ones;
-    }
-    return same;
+// For each of R keys of a lane: the lanes with its digit, among those whose key is here.  A bit of
+// all R at a time, since a chain of one key's bits waits for itself.
+template <int R>
+__device__ __forceinline__ void same_digits(const uint32_t (&digit)[R], const bool (&here)[R],
+                                            int bits, uint64_t (&same)[R]) {
+#pragma unroll
+    for (int q = 0; q < R; ++q) same[q] = __ballot(here[q]);
+    for (int k = 0; k < bits; ++k)
+#pragma unroll
+        for (int q = 0; q < R; ++q) {
+            const uint32_t all = (uint32_t)((int32_t)(digit[q] << (31 - k)) >> 31);
+            const uint64_t ones = __ballot(all != 0);
+            const uint32_t lo = ~((uint32_t)ones ^ all), hi = ~((uint32_t)(ones >> 32) ^ all);
+            same[q] &= (uint64_t)hi << 32 | lo;
+        }
 }
 
 // The sum of v over the threads before, and over all, of a workgroup of W wavefronts.
@@ -271,15 +278,21 @@ __global__ __launch_bounds__(SORT_THREADS) void k_embed_place(Pass p) {
         for (int d = threadIdx.x; d < SORT_WAVES * bins; d += SORT_THREADS) count[d] = 0;
         __syncthreads();
         uint32_t *mine = count + wave * bins;
+        uint32_t digit[R];
+        bool here[R];
+        uint64_t same[R];
 #pragma unroll
         for (int q = 0; q < R; ++q) {
-            const uint32_t d = (pair[q].x >> p.shift) & (bins - 1);
-            const bool here = w + q * 64 + lane < b;
-            const uint64_t same = same_digit(d, here, p.bits);
-            const uint32_t r = lanes_below(same);
-            rank[q] = here ? mine[d] + r : 0;
+            digit[q] = (pair[q].x >> p.shift) & (bins - 1);
+            here[q] = w + q * 64 + lane < b;
+        }
+        same_digits(digit, here, p.bits, same);
+#pragma unroll
+        for (int q = 0; q < R; ++q) {
+            const uint32_t r = lanes_below(same[q]);
+            rank[q] = here[q] ? mine[digit[q]] + r : 0;
             __builtin_amdgcn_wave_barrier();
-            if (here && r == 0) mine[d] = rank[q] + (uint32_t)__popcll(same);
+            if (here[q] && r == 0) mine[digit[q]] = rank[q] + (uint32_t)__popcll(same[q]);
             __builtin_amdgcn_wave_barrier();
         }
         __syncthreads();
@@ -304,9 +317,7 @@ __global__ __launch_bounds__(SORT_THREADS) void k_embed_place(Pass p) {
         __syncthreads();
 #pragma unroll
         for (int q = 0; q < R; ++q) {
-            if (w + q * 64 + lane >= b) continue;
-            const uint32_t d = (pair[q].x >> p.shift) & (bins - 1);
-            staged[first[d] + mine[d] + rank[q]] = pair[q];
+            if (here[q]) staged[first[digit[q]] + mine[digit[q]] + rank[q]] = pair[q];
         }
         __syncthreads();
         for (uint32_t l = threadIdx.x; l < taken; l += SORT_THREADS) {
@@ -348,16 +359,22 @@ __global__ __launch_bounds__(SMALL_THREADS) void k_embed_sort_small(Pass p, int3
         for (int d = threadIdx.x; d < SMALL_WAVES * bins; d += SMALL_THREADS) count[d] = 0;
         __syncthreads();
         uint32_t *mine = count + wave * bins;
+        uint32_t digit[SMALL_EACH];
+        bool here[SMALL_EACH];
+        uint64_t same[SMALL_EACH];
+#pragma unroll
+        for (int q = 0; q < SMALL_EACH; ++q) {
+            digit[q] = (key[q] >> shift) & (bins - 1);
+            here[q] = a + q * 64 + lane < b;
+        }
+        same_digits(digit, here, p.bits, same);
 #pragma unroll
         for (int q = 0; q < SMALL_EACH; ++q) {
             if (a + q * 64 >= b) continue;
-            const uint32_t d = (key[q] >> shift) & (bins - 1);
-            const bool here = a + q * 64 + lane < b;
-            const uint64_t same = same_digit(d, here, p.bits);
-            const uint32_t r = lanes_below(same);
-            rank[q] = here ? mine[d] + r : 0;
+            const uint32_t r = lanes_below(same[q]);
+            rank[q] = here[q] ? mine[digit[q]] + r : 0;
             __builtin_amdgcn_wave_barrier();
-            if (here && r == 0) mine[d] = rank[q] + (uint32_t)__popcll(same);
+            if (here[q] && r == 0) mine[digit[q]] = rank[q] + (uint32_t)__popcll(same[q]);
             __builtin_amdgcn_wave_barrier();
         }
         __syncthreads();
