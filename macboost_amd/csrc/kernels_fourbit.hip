@@ -322,7 +322,7 @@ __device__ __forceinline__ void scores_of(const FourbitCall &c, const float4v &z
 // E scores of a row from class cls on, at any address of a float.
 template <int E>
 __device__ __forceinline__ void put_scores(const FourbitCall &c, int64_t row, int64_t cls,
-                                           const float (&v)[E]) {
+                                           const float (&v)[E], bool streamed) {
     if (row >= c.rows) return;
     float *to = c.scores + row * c.score_stride + cls;
     if (cls + E <= c.shape.classes) {
@@ -330,7 +330,7 @@ __device__ __forceinline__ void put_scores(const FourbitCall &c, int64_t row, in
         V out;
 #pragma unroll
         for (int i = 0; i < E; ++i) out[i] = v[i];
-        *reinterpret_cast<V *>(to) = out;
+        put(reinterpret_cast<V *>(to), out, streamed);
     } else {
 #pragma unroll
         for (int i = 0; i < E; ++i)
@@ -344,7 +344,7 @@ __device__ __forceinline__ void write_scores(const FourbitCall &c, const float4v
                                              int row_exponent) {
     float v[Ends<N>::EACH];
     scores_of<N>(c, z, end, row_exponent, v);
-    put_scores(c, column / N, end.cls, v);
+    put_scores(c, column / N, end.cls, v, false);
 }
 
 // ---- few columns: reading W is the work ------------------------------------------------
@@ -628,7 +628,8 @@ __global__ __launch_bounds__(64 * WIDE_WAVES, 2) void k_fourbit_tiles(
             const int row = i * 4 + (lane >> 4);
             const float4v z = *reinterpret_cast<const float4v *>(meet + row * ROW + (lane & 15) * 4);
             const float v[4] = {z[0], z[1], z[2], z[3]};
-            put_scores(c, (column0 + x) * 16 / N + row, tile0 * TILE + (lane & 15) * 4, v);
+            put_scores(c, (column0 + x) * 16 / N + row, tile0 * TILE + (lane & 15) * 4, v,
+                       c.streamed);
         }
         __builtin_amdgcn_wave_barrier();
     }
@@ -798,6 +799,7 @@ hipError_t launch_fourbit_scores(hipStream_t st, const FourbitCall &c, char *scr
         FourbitCall part = c;
         part.rows = std::min(each, c.rows - r);
         part.wide_h = wide_h;
+        part.streamed = part.rows * c.shape.classes * 4 > STREAMED;
         part.h = static_cast<const char *>(c.h) + r * row;
         part.scores = c.scores + r * c.score_stride;
         const hipError_t e = c.bf16 ? run<__bf16>(st, part, scratch) : run<float>(st, part, scratch);

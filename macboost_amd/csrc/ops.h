@@ -145,7 +145,8 @@ struct FourbitCall {
     const float *bias;               // NULL: none
     float *scores;
     int64_t score_stride;
-    bool wide_h;                     // rows at multiples of 16 bytes; set by the launcher
+    bool wide_h;                     // rows at multiples of 16 bytes; set by the launcher,
+    bool streamed;                   // as this is
     int num_cus;
 };
 size_t fourbit_scratch(const FourbitCall &c);
@@ -162,6 +163,7 @@ struct AdjustCall {
     const float *bias;               // NULL: none
     const uint32_t *allowed;         // NULL: all
     float *out;
+    bool streamed;                   // set by the launcher
 };
 hipError_t launch_adjust(hipStream_t s, const AdjustCall &c);
 
