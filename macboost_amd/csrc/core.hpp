@@ -415,6 +415,7 @@ int host_threads();
 struct mbk_tensors {
     mb::DevBuf<mbk::ClipPiece> piece;
     int64_t pieces = 0;
+    bool one = false;                // for one workgroup
     bool outputs = false;
     bool streamed = false;           // of outputs beyond the caches
     bool captured = false;           // a captured graph may use it

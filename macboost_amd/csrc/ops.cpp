@@ -113,8 +113,8 @@ mbk::EmbedCall embed_call(const mbk_embed_shape *sh, const int32_t *ids, const v
 }
 
 // The pieces of one gradient of the list: short rows together, long ones and gradients without
-// gaps in runs.
-void add_pieces(const mbk_tensor &t, int64_t most, std::vector<mbk::ClipPiece> &out) {
+// gaps in runs of `most` elements.  runs: 16-byte runs of short rows a piece, at most.
+void add_pieces(const mbk_tensor &t, int64_t most, int64_t runs, std::vector<mbk::ClipPiece> &out) {
     const bool bf16 = t.type == MBK_BF16;
     const int64_t size = bf16 ? 2 : 4;
     const auto add = [&](int64_t at, int64_t rows, int64_t cols) {
@@ -131,7 +131,8 @@ void add_pieces(const mbk_tensor &t, int64_t most, std::vector<mbk::ClipPiece> &
                 add(r * t.stride + c, 1, std::min(most, cols - c));
         return;
     }
-    const int64_t each = most / cols;
+    const int64_t chunks = (cols * size + 15) / 16;
+    const int64_t each = std::max<int64_t>(1, std::min(most / cols, runs / chunks));
     for (int64_t r = 0; r < rows; r += each) add(r * t.stride, std::min(each, rows - r), cols);
 }
 
@@ -291,9 +292,17 @@ int mbk_tensors_create(mbk_context *ctx, const mbk_tensor *list, int32_t count, 
         int64_t written = 0;
         for (int32_t i = 0; i < count; ++i) {
             if (list[i].out) written += list[i].rows * list[i].cols * (list[i].type == MBK_BF16 ? 2 : 4);
-            add_pieces(list[i], mbk::clip_piece(elements), pieces);
             made->outputs |= list[i].out != nullptr;
         }
+        const auto cut = [&](int64_t most, int64_t runs) {
+            pieces.clear();
+            for (int32_t i = 0; i < count; ++i) add_pieces(list[i], most, runs, pieces);
+        };
+        if (elements <= 4 * mbk::CLIP_ONE * mbk::CLIP_RUNS) {
+            cut(4 * mbk::CLIP_RUNS, mbk::CLIP_RUNS);
+            made->one = pieces.size() <= (size_t)mbk::CLIP_ONE;
+        }
+        if (!made->one) cut(mbk::clip_piece(elements), INT64_MAX);
         need(ctx != nullptr, "null kernel-seam context");
         need(!mb::context_captured(ctx), "the context's stream is being captured");
         mb::OnDevice here(mb::context_device(ctx));
@@ -345,8 +354,8 @@ int mbk_grad_clip(mbk_context *ctx, mbk_tensors *list, float max_norm, float *no
         char *scratch = mb::context_scratch(ctx, mbk::clip_scratch(list->pieces, cus));
         list->captured |= mb::context_captured(ctx);
         MB_HIP(mbk::launch_clip(mb::context_stream(ctx),
-                                {list->piece.ptr, list->pieces, list->outputs, list->streamed,
-                                 max_norm, norm, cus},
+                                {list->piece.ptr, list->pieces, list->one, list->outputs,
+                                 list->streamed, max_norm, norm, cus},
                                 scratch));
         return 0;
     }, -1);

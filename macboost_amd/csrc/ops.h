@@ -109,9 +109,12 @@ struct ClipPiece {
 constexpr int64_t clip_piece(int64_t elements) {
     return elements < ((int64_t)1 << 18) ? 1024 : elements < ((int64_t)1 << 21) ? 2048 : 8192;
 }
+constexpr int CLIP_ONE = 32;             // pieces of at most 256 runs of 16 bytes that one workgroup takes
+constexpr int CLIP_RUNS = 256;
 struct ClipCall {
     const ClipPiece *piece;
     int64_t pieces;
+    bool one;                        // at most CLIP_ONE such pieces
     bool outputs, streamed;
     float max_norm;
     float *norm;

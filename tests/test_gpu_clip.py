@@ -28,6 +28,11 @@ LISTS = [
     [(2, 20001, "f32", 3, 1), (9000, 1, "bf16", 1, 0), (9000, 1, "f32", 3, 0), (1, 100000, "f32", 0, 3)],
     [(64, 64, "bf16", 0, 0)] * 60 + [(10, 10, "f32", 0, 0)] * 60,
     [(5000, 700, "bf16", 0, 0), (3000, 900, "f32", 0, 0), (1, 70000, "f32", 0, 0)],
+    # one workgroup's, and just more
+    [(1, 32768, "f32", 0, 0)], [(1, 32769, "f32", 0, 0)], [(1, 32768, "bf16", 0, 1)],
+    [(256, 1, "f32", 2, 0)] * 32, [(256, 1, "bf16", 1, 0)] * 16 + [(257, 1, "f32", 1, 0)] * 16,
+    [(100, 37, "f32", 3, 1), (100, 37, "bf16", 0, 0), (1, 5, "f32", 0, 0), (0, 3, "f32", 0, 0)],
+    [(1, 1, "f32", 0, 0)] * 33, [(1, 1, "bf16", 0, 0)] * 32, [(200, 1023, "f32", 1, 0)],
 ]
 
 
