@@ -187,7 +187,7 @@ __device__ __forceinline__ void terms(const T *row, int dim, bool wide, int step
 }
 
 // Where many columns are made for all workgroups: a workgroup a tile of columns.
-constexpr int COLUMN_WAVES = 8;
+constexpr int COLUMN_WAVES = 16;
 template <typename T>
 __global__ __launch_bounds__(64 * COLUMN_WAVES) void k_fourbit_columns(
     const T *__restrict__ h, int64_t stride, int64_t rows, int32_t dim, bool wide, int32_t steps,
