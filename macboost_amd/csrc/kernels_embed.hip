@@ -331,45 +331,38 @@ __global__ __launch_bounds__(SORT_THREADS) void k_embed_place(Pass p) {
     }
 }
 
-// Few rows: the whole sort by one workgroup in one launch.
-// (16384 rows of 17 bits take 46 us so, 20 by the kernels above.)
-constexpr int SMALL_WAVES = 16, SMALL_THREADS = 64 * SMALL_WAVES, SMALL_EACH = 4;
-constexpr int64_t SMALL_ROWS = SMALL_THREADS * SMALL_EACH;
-constexpr int SMALL_BITS = 10;
-__global__ __launch_bounds__(SMALL_THREADS) void k_embed_sort_small(Pass p, int32_t passes) {
-    extern __shared__ uint32_t lds[];
-    const int bins = 1 << p.bits;
-    uint32_t *wave_sum = lds;                            // SMALL_WAVES
-    uint32_t *count = wave_sum + SMALL_WAVES;            // [wave][digit]
-    uint32_t *keys = count + SMALL_WAVES * bins;         // [rows]
-    uint16_t *order = reinterpret_cast<uint16_t *>(keys + p.rows);
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    if (threadIdx.x == 0) *p.zero = 0;
+// Few rows: the whole sort by one workgroup.  Up to 64 * EACH rows a wavefront, p.per of them;
+// keys and order hold the sorted list in the end, key and row a lane's places of it.
+template <int WAVES, int EACH>
+__device__ __forceinline__ void sort_in_lds(const Pass &p, int passes, uint32_t *wave_sum,
+                                            uint32_t *count, uint32_t *keys, uint16_t *order,
+                                            uint32_t (&key)[EACH], uint16_t (&row)[EACH]) {
+    constexpr int N = 64 * WAVES;
+    const int bins = 1 << p.bits, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int a = min((int)p.rows, wave * (int)p.per), b = min((int)p.rows, a + (int)p.per);
-    uint32_t key[SMALL_EACH], rank[SMALL_EACH];
-    uint16_t row[SMALL_EACH];
+    uint32_t rank[EACH];
 #pragma unroll
-    for (int q = 0; q < SMALL_EACH; ++q) {
+    for (int q = 0; q < EACH; ++q) {
         const int i = a + q * 64 + lane;
         key[q] = i < b ? key_of(p.ids, p.entries, i) : 0;
         row[q] = (uint16_t)i;
     }
     for (int s = 0; s < passes; ++s) {
         const int shift = s * p.bits;
-        for (int d = threadIdx.x; d < SMALL_WAVES * bins; d += SMALL_THREADS) count[d] = 0;
+        for (int d = threadIdx.x; d < WAVES * bins; d += N) count[d] = 0;
         __syncthreads();
         uint32_t *mine = count + wave * bins;
-        uint32_t digit[SMALL_EACH];
-        bool here[SMALL_EACH];
-        uint64_t same[SMALL_EACH];
+        uint32_t digit[EACH];
+        bool here[EACH];
+        uint64_t same[EACH];
 #pragma unroll
-        for (int q = 0; q < SMALL_EACH; ++q) {
+        for (int q = 0; q < EACH; ++q) {
             digit[q] = (key[q] >> shift) & (bins - 1);
             here[q] = a + q * 64 + lane < b;
         }
         same_digits(digit, here, p.bits, same);
 #pragma unroll
-        for (int q = 0; q < SMALL_EACH; ++q) {
+        for (int q = 0; q < EACH; ++q) {
             if (a + q * 64 >= b) continue;
             const uint32_t r = lanes_below(same[q]);
             rank[q] = here[q] ? mine[digit[q]] + r : 0;
@@ -378,28 +371,32 @@ __global__ __launch_bounds__(SMALL_THREADS) void k_embed_sort_small(Pass p, int3
             __builtin_amdgcn_wave_barrier();
         }
         __syncthreads();
-        uint32_t sum = 0, all;                           // bins <= SMALL_THREADS
-        const int d = threadIdx.x;
-        if (d < bins)
-            for (int v = 0; v < SMALL_WAVES; ++v) sum += count[v * bins + d];
-        uint32_t at = sum_before<SMALL_WAVES>(sum, wave_sum, all);
-        if (d < bins)
-            for (int v = 0; v < SMALL_WAVES; ++v) {
-                const uint32_t n = count[v * bins + d];
-                count[v * bins + d] = at;
-                at += n;
-            }
+        uint32_t before = 0, all;
+        for (int d0 = 0; d0 < bins; d0 += N) {
+            const int d = d0 + threadIdx.x;
+            uint32_t sum = 0;
+            if (d < bins)
+                for (int v = 0; v < WAVES; ++v) sum += count[v * bins + d];
+            uint32_t at = before + sum_before<WAVES>(sum, wave_sum, all);
+            if (d < bins)
+                for (int v = 0; v < WAVES; ++v) {
+                    const uint32_t n = count[v * bins + d];
+                    count[v * bins + d] = at;
+                    at += n;
+                }
+            before += all;
+        }
         __syncthreads();
 #pragma unroll
-        for (int q = 0; q < SMALL_EACH; ++q) {
-            if (a + q * 64 + lane >= b) continue;
-            const uint32_t to = mine[(key[q] >> shift) & (bins - 1)] + rank[q];
+        for (int q = 0; q < EACH; ++q) {
+            if (!here[q]) continue;
+            const uint32_t to = mine[digit[q]] + rank[q];
             keys[to] = key[q];
             order[to] = row[q];
         }
         __syncthreads();
 #pragma unroll
-        for (int q = 0; q < SMALL_EACH; ++q) {
+        for (int q = 0; q < EACH; ++q) {
             const int i = a + q * 64 + lane;
             if (i >= b) continue;
             key[q] = keys[i];
@@ -407,11 +404,27 @@ __global__ __launch_bounds__(SMALL_THREADS) void k_embed_sort_small(Pass p, int3
         }
         __syncthreads();
     }
+}
+
+// (16384 rows of 17 bits take 46 us so, 20 by the kernels above.)
+constexpr int SMALL_WAVES = 16, SMALL_THREADS = 64 * SMALL_WAVES, SMALL_EACH = 4;
+constexpr int64_t SMALL_ROWS = SMALL_THREADS * SMALL_EACH;
+__global__ __launch_bounds__(SMALL_THREADS) void k_embed_sort_small(Pass p, int32_t passes) {
+    extern __shared__ uint32_t lds[];
+    uint32_t *wave_sum = lds;                            // SMALL_WAVES
+    uint32_t *count = wave_sum + SMALL_WAVES;            // [wave][digit]
+    uint32_t *keys = count + (SMALL_WAVES << p.bits);    // [rows]
+    uint16_t *order = reinterpret_cast<uint16_t *>(keys + p.rows);
+    if (threadIdx.x == 0) *p.zero = 0;
+    uint32_t key[SMALL_EACH];
+    uint16_t row[SMALL_EACH];
+    sort_in_lds<SMALL_WAVES>(p, passes, wave_sum, count, keys, order, key, row);
+    const int a = (threadIdx.x >> 6) * (int)p.per;
+    const int b = min((int)p.rows, a + (int)p.per);
 #pragma unroll
     for (int q = 0; q < SMALL_EACH; ++q) {
-        const int i = a + q * 64 + lane;
-        if (i >= b) continue;
-        p.out[i] = uint2{key[q], row[q]};
+        const int i = a + q * 64 + (threadIdx.x & 63);
+        if (i < b) p.out[i] = uint2{key[q], row[q]};
     }
 }
 
@@ -434,6 +447,7 @@ constexpr int MOST_ITEMS = 4096;     // of a workgroup
 constexpr int AHEAD = 8;             // items on the way
 constexpr uint32_t ENTRY = 0x80000000u;      // an item that is an entry: which, if not all are there
 constexpr uint32_t NOTHING = 0xFFFFFFFFu;
+constexpr uint32_t PASSED = 0xFFFFFFFEu;     // an entry that is summed elsewhere
 
 struct Sums {
     int64_t rows, workers;
@@ -540,6 +554,60 @@ __device__ __forceinline__ void both_ends(const Sums &s, const int64_t (&d)[2], 
 template <typename T, int E>
 using Run = T __attribute__((ext_vector_type(E), aligned(sizeof(T))));
 
+// The items [p, end): rows are added to acc, at_entry(entry, its base) takes it.  next: the next
+// entry, where all are on the list.  SOME: some entries are passed.
+template <typename T, int E, bool BASE, bool ONE, bool SOME, class AtEntry>
+__device__ __forceinline__ void walk(const Sums &s, const uint32_t *item, int p, int end,
+                                     uint32_t next, const T *dout, const T *base, const T *dtable,
+                                     float (&acc)[E], AtEntry at_entry) {
+    const T *some_row = s.rows ? dout : dtable;
+    for (; p < end; p += AHEAD) {
+        uint32_t what[AHEAD];
+        Run<T, E> v[AHEAD];
+#pragma unroll
+        for (int q = 0; q < AHEAD; ++q) {
+            what[q] = item[p + q];
+            if constexpr (ONE) what[q] = __builtin_amdgcn_readfirstlane(what[q]);
+            if (s.dense) {
+                const bool entry = what[q] == ENTRY, passed = SOME && what[q] == PASSED;
+                what[q] |= entry ? next : passed ? NOTHING : 0;
+                next += entry || passed;
+            }
+            if (p + q >= end) what[q] = NOTHING;
+        }
+#pragma unroll
+        for (int q = 0; q < AHEAD; ++q) {
+            const bool is_row = what[q] < ENTRY;
+            // without branches: what has nothing to read takes a row or an entry that is there
+            if constexpr (BASE) {
+                const T *at = is_row ? dout : what[q] == NOTHING ? dtable : base;
+                const uint32_t which = what[q] == NOTHING ? 0 : what[q] & ~ENTRY;
+                v[q] = *reinterpret_cast<const Run<T, E> *>(
+                    at + which * (is_row ? s.row_stride : s.table_stride));
+            } else {
+                v[q] = *reinterpret_cast<const Run<T, E> *>(
+                    some_row + (is_row ? what[q] : 0) * s.row_stride);
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < AHEAD; ++q) {
+            const bool is_row = what[q] < ENTRY;
+            if constexpr (ONE) {
+                if (is_row)
+#pragma unroll
+                    for (int e = 0; e < E; ++e) acc[e] += to_f32(v[q][e]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; ++e) acc[e] = is_row ? acc[e] + to_f32(v[q][e]) : acc[e];
+            }
+            if (is_row || what[q] == NOTHING) continue;
+            at_entry(what[q] & ~ENTRY, v[q]);
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[e] = 0.0f;
+        }
+    }
+}
+
 // E > 1: the last piece of a row that is no multiple of E long is its last E columns, some of which
 // the piece before has too: both lanes write the same.
 // BASE: dtable has a base.  ONE: one worker a wavefront, whose items are the same in all lanes.
@@ -550,7 +618,7 @@ __global__ __launch_bounds__(SUM_THREADS) void k_embed_sum(Sums s) {
     const int items = SUM_WAVES * s.groups * s.per, most = held_rows(items, s.whole);
     uint32_t *key = lds;                             // [row]
     uint32_t *item = key + most;                     // [item]: a row, or an entry
-    uint32_t *place = item + 2 * most;               // [row] its item, where it is not i + key
+    uint32_t *place = item + 2 * most + AHEAD;       // [row] its item, where it is not i + key
     const int64_t first = (int64_t)group_id() * (SUM_WAVES * s.groups);
     if (first >= s.workers) return;
     const int64_t d[2] = {first * s.per, min(min(first + SUM_WAVES * s.groups, s.workers) * s.per,
@@ -614,7 +682,6 @@ __global__ __launch_bounds__(SUM_THREADS) void k_embed_sum(Sums s) {
     const T *base = BASE ? static_cast<const T *>(s.base) + col : nullptr;
     T *dtable = static_cast<T *>(s.dtable) + col;
     float *parts = s.parts + worker * 2 * s.part_stride + col;
-    const T *some_row = s.rows ? dout : dtable;
 
     float acc[E];
 #pragma unroll
@@ -625,68 +692,25 @@ __global__ __launch_bounds__(SUM_THREADS) void k_embed_sum(Sums s) {
 #pragma unroll
         for (int e = 0; e < E; ++e) parts[side * s.part_stride + e] = acc[e];
     };
-    for (; p < end; p += AHEAD) {
-        uint32_t what[AHEAD];
-        Run<T, E> v[AHEAD];
-#pragma unroll
-        for (int q = 0; q < AHEAD; ++q) {
-            what[q] = item[p + q];
-            if constexpr (ONE) what[q] = __builtin_amdgcn_readfirstlane(what[q]);
-            if (s.dense) {
-                const bool entry = what[q] == ENTRY;
-                what[q] |= entry ? next : 0;
-                next += entry;
+    walk<T, E, BASE, ONE, false>(s, item, p, end, next, dout, base, dtable, acc,
+                          [&](uint32_t entry, const Run<T, E> &v) {
+        if (head) {
+            leave(0);
+            if (!idle && chunk == 0) {
+                const uint32_t at = atomicAdd(&s.found[0], 1u);
+                s.found[2 + 2 * at] = (uint32_t)worker;
+                s.found[3 + 2 * at] = entry;
             }
-            if (p + q >= end) what[q] = NOTHING;
+            head = false;
+        } else {
+            Run<T, E> out;
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                out[e] = (T)__builtin_fmaf(s.scale, acc[e], BASE ? to_f32(v[e]) : 0.0f);
+            if (!idle)
+                put(reinterpret_cast<Run<T, E> *>(dtable + entry * s.table_stride), out, s.streamed);
         }
-#pragma unroll
-        for (int q = 0; q < AHEAD; ++q) {
-            const bool is_row = what[q] < ENTRY;
-            // without branches: what has nothing to read takes a row or an entry that is there
-            if constexpr (BASE) {
-                const T *at = is_row ? dout : what[q] == NOTHING ? dtable : base;
-                const uint32_t which = what[q] == NOTHING ? 0 : what[q] & ~ENTRY;
-                v[q] = *reinterpret_cast<const Run<T, E> *>(
-                    at + which * (is_row ? s.row_stride : s.table_stride));
-            } else {
-                v[q] = *reinterpret_cast<const Run<T, E> *>(
-                    some_row + (is_row ? what[q] : 0) * s.row_stride);
-            }
-        }
-#pragma unroll
-        for (int q = 0; q < AHEAD; ++q) {
-            const bool is_row = what[q] < ENTRY;
-            if constexpr (ONE) {
-                if (is_row)
-#pragma unroll
-                    for (int e = 0; e < E; ++e) acc[e] += to_f32(v[q][e]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < E; ++e) acc[e] = is_row ? acc[e] + to_f32(v[q][e]) : acc[e];
-            }
-            if (is_row || what[q] == NOTHING) continue;
-            const uint32_t entry = what[q] & ~ENTRY;
-            if (head) {
-                leave(0);
-                if (!idle && chunk == 0) {
-                    const uint32_t at = atomicAdd(&s.found[0], 1u);
-                    s.found[2 + 2 * at] = (uint32_t)worker;
-                    s.found[3 + 2 * at] = entry;
-                }
-                head = false;
-            } else {
-                Run<T, E> out;
-#pragma unroll
-                for (int e = 0; e < E; ++e)
-                    out[e] = (T)__builtin_fmaf(s.scale, acc[e], BASE ? to_f32(v[q][e]) : 0.0f);
-                if (!idle)
-                    put(reinterpret_cast<Run<T, E> *>(dtable + entry * s.table_stride), out,
-                        s.streamed);
-            }
-#pragma unroll
-            for (int e = 0; e < E; ++e) acc[e] = 0.0f;
-        }
-    }
+    });
     if (!idle && chunk == 0) s.open[worker] = to.open ? to.e : NOTHING;
     const bool inside = from.open && to.open && from.e == to.e;
     const int here = (int)min((int64_t)SUM_WAVES * s.groups, s.workers - first);
@@ -846,6 +870,167 @@ __global__ __launch_bounds__(JOIN_THREADS) void k_embed_join(Sums s) {
     }
 }
 
+// ---------------------------------------------------------------------------
+// Up to FEW_ROWS rows: one launch.  Every workgroup sorts all of them for itself; the first
+// `lists` take the merged list as above, without the entries of more than `whole` rows, and each of the
+// others one of those.
+// ---------------------------------------------------------------------------
+constexpr int FEW_EACH = 4;
+constexpr int64_t FEW_ROWS = 64 * SUM_WAVES * FEW_EACH;
+struct FewLayout {                   // words of LDS, at most 28 KB
+    int count, keys, order, place, item, all;
+};
+__host__ __device__ inline FewLayout few_layout(const Sums &s, int bits, int elements) {
+    FewLayout l{};
+    const int items = SUM_WAVES * s.groups * s.per + s.whole + 2 + AHEAD;
+    const int rows = ((int)s.rows + 63) / 64 * 64;
+    l.keys = SUM_WAVES;              // behind the wavefronts' sums
+    l.order = l.keys + rows;
+    l.place = l.order + rows / 2;
+    l.count = l.item = (l.place + rows + 4) / 4 * 4;     // one behind the other in time
+    int most = SUM_WAVES << bits;
+    most = most > items ? most : items;
+    most = most > 2 * rows + 2 + AHEAD ? most : 2 * rows + 2 + AHEAD;
+    most = most > SUM_THREADS * elements ? most : SUM_THREADS * elements;
+    l.all = l.item + most;
+    return l;
+}
+
+template <typename T, int E, bool BASE>
+__global__ __launch_bounds__(SUM_THREADS) void k_embed_few(Sums s, Pass p, int32_t passes,
+                                                           int32_t lists) {
+    extern __shared__ uint32_t lds[];
+    const FewLayout l = few_layout(s, p.bits, E);
+    uint32_t *wave_sum = lds, *key = lds + l.keys, *item = lds + l.item, *place = lds + l.place;
+    uint16_t *order = reinterpret_cast<uint16_t *>(lds + l.order);
+    {
+        uint32_t k[FEW_EACH];
+        uint16_t r[FEW_EACH];
+        sort_in_lds<SUM_WAVES>(p, passes, wave_sum, lds + l.count, key, order, k, r);
+    }
+    const int rows = (int)s.rows, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int group = lane / s.lanes, chunk0 = blockIdx.y * 64 + lane - group * s.lanes;
+    const int32_t chunk = min(chunk0, s.chunks - 1);
+    const int col = min(chunk * E, s.dim - E);
+    const T *dout = static_cast<const T *>(s.dout) + col;
+    const T *base = BASE ? static_cast<const T *>(s.base) + col : nullptr;
+    T *dtable = static_cast<T *>(s.dtable) + col;
+    float acc[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.0f;
+    const auto write = [&](uint32_t entry, const Run<T, E> &b) {
+        Run<T, E> out;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            out[e] = (T)__builtin_fmaf(s.scale, acc[e], BASE ? to_f32(b[e]) : 0.0f);
+        put(reinterpret_cast<Run<T, E> *>(dtable + entry * s.table_stride), out, s.streamed);
+    };
+
+    if ((int)blockIdx.x >= lists) {
+        // the rows [a, b) of the entry: slices of them side by side, and their sums by halves
+        __shared__ int found;
+        uint32_t before = 0, all;
+        for (int i0 = 0; i0 < rows; i0 += SUM_THREADS) {
+            const int i = i0 + threadIdx.x;
+            const bool starts = i + s.whole < rows && key[i] < s.entries &&
+                                (i == 0 || key[i - 1] != key[i]) && key[i + s.whole] == key[i];
+            const uint32_t at = before + sum_before<SUM_WAVES>(starts, wave_sum, all);
+            if (starts && at == blockIdx.x - lists) found = i;
+            before += all;
+        }
+        __syncthreads();
+        if (blockIdx.x - lists >= before) return;
+        const int a = found;
+        const uint32_t entry = key[a];
+        const int b = first_not(a, rows, [&](int m) { return key[m] == entry; });
+        const int groups = 64 / s.lanes, slices = SUM_WAVES * groups;
+        const int slice = wave * groups + min(group, groups - 1);
+        const bool idle = group >= groups || chunk0 >= s.chunks;
+        const int each = (b - a + slices - 1) / slices;
+        const int to = min(b, a + (slice + 1) * each);
+        for (int i = a + slice * each; i < to; i += AHEAD) {
+            Run<T, E> v[AHEAD];
+#pragma unroll
+            for (int q = 0; q < AHEAD; ++q)
+                v[q] = *reinterpret_cast<const Run<T, E> *>(dout + order[min(i + q, to - 1)] *
+                                                                       s.row_stride);
+#pragma unroll
+            for (int q = 0; q < AHEAD; ++q)
+#pragma unroll
+                for (int e = 0; e < E; ++e) acc[e] += i + q < to ? to_f32(v[q][e]) : 0.0f;
+        }
+        float *meet = reinterpret_cast<float *>(item) + threadIdx.x * E;
+#pragma unroll
+        for (int e = 0; e < E; ++e) meet[e] = acc[e];
+        for (int o = 128; o > 0; o >>= 1) {
+            __syncthreads();
+            const int other = slice + o;
+            if (!idle && slice < o && other < slices) {
+                const float *from = meet + ((other / groups - wave) * 64 +
+                                            (other % groups - group) * s.lanes) * E;
+#pragma unroll
+                for (int e = 0; e < E; ++e) meet[e] += from[e];
+            }
+        }
+        if (idle || slice != 0) return;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = meet[e];
+        Run<T, E> b0{};
+        if constexpr (BASE) b0 = *reinterpret_cast<const Run<T, E> *>(base + entry * s.table_stride);
+        write(entry, b0);
+        return;
+    }
+
+    const int64_t first = (int64_t)blockIdx.x * (SUM_WAVES * s.groups), d0 = first * s.per;
+    const int items = SUM_WAVES * s.groups * s.per + s.whole + 2;
+    // whether the entry of row i has more than `whole` rows
+    const auto is_long = [&](int i) {
+        const uint32_t k = key[i];
+        const int a = first_not(max(0, i - s.whole), i, [&](int m) { return key[m] < k; });
+        return a + s.whole < rows && key[a + s.whole] == k;
+    };
+    if (s.dense) {
+        for (int i = threadIdx.x; i < items; i += SUM_THREADS) item[i] = ENTRY;
+        __syncthreads();
+        for (int i = threadIdx.x; i < rows; i += SUM_THREADS) {
+            const uint32_t k = key[i];
+            const int64_t at = i + (int64_t)k - d0;
+            if (k >= s.entries || at < -1 || at >= items) continue;
+            const bool elsewhere = is_long(i);
+            if (at >= 0) item[at] = elsewhere ? NOTHING : order[i];
+            if (elsewhere && at + 1 < items && (i + 1 == rows || key[i + 1] != k))
+                item[at + 1] = PASSED;
+        }
+    } else {
+        uint32_t before = 0, all;
+        for (int i0 = 0; i0 < rows; i0 += SUM_THREADS) {
+            const int i = i0 + threadIdx.x;
+            const uint32_t k = i < rows ? key[i] : NOTHING;
+            const bool ends_here = k < s.entries && (i + 1 == rows || key[i + 1] != k);
+            const uint32_t at = i + before + sum_before<SUM_WAVES>(ends_here, wave_sum, all);
+            if (i < rows) {
+                const bool elsewhere = k < s.entries && is_long(i);
+                place[i] = at;
+                item[at] = elsewhere ? NOTHING : order[i];
+                if (ends_here) item[at + 1] = elsewhere ? NOTHING : ENTRY | k;
+            }
+            before += all;
+        }
+        if (threadIdx.x == 0) place[rows] = rows + before;
+    }
+    __syncthreads();
+    const int mine = wave * s.groups + group;
+    const int64_t worker = first + mine;
+    if (group >= s.groups || worker >= s.workers || chunk0 >= s.chunks) return;
+    const Cut from = cut_at(s, key, 0, rows, 0, rows, worker * s.per);
+    Cut to = cut_at(s, key, 0, rows, 0, rows, (worker + 1) * s.per);
+    if (to.i > from.i && key[to.i - 1] >= s.entries)         // rows that are left out, behind all
+        to.i = first_not(from.i, to.i, [&](int m) { return key[m] < s.entries; });
+    const int at = s.dense ? (int)(from.i + (int64_t)from.e - d0) : (int)place[from.i];
+    const int end = s.dense ? (int)(to.i + (int64_t)to.e - d0) : (int)place[to.i];
+    walk<T, E, BASE, false, true>(s, item, at, end, from.e, dout, base, dtable, acc, write);
+}
+
 bool aligned(const void *p, int64_t stride, size_t size) {
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * (int64_t)size % 16 == 0;
 }
@@ -866,14 +1051,15 @@ struct GradShape {
     int elements;                    // E
     bool dense;
     int64_t workers;
+    bool few;                        // one launch
+    int64_t lists;                   // its workgroups of the list
 };
 
 GradShape grad_shape(const EmbedCall &c) {
     GradShape g{};
     const int bits = bits_of(c.entries);
     g.small = c.rows <= SMALL_ROWS;
-    const int most = g.small ? SMALL_BITS : MOST_BITS;
-    g.passes = (bits + most - 1) / most;
+    g.passes = (bits + MOST_BITS - 1) / MOST_BITS;
     g.bits = std::max(3, (bits + g.passes - 1) / g.passes);      // 16 bytes of counts
     if (g.small) {
         g.per = ((c.rows + SMALL_WAVES - 1) / SMALL_WAVES + 63) / 64 * 64;
@@ -908,6 +1094,15 @@ GradShape grad_shape(const EmbedCall &c) {
     g.items = (int)per;
     g.whole = c.rows <= 64 ? 64 : g.items;           // few rows: nothing to join
     g.workers = (items + per - 1) / per;
+    // few rows: sorted again by each workgroup, which pays up to where there are very many of them
+    // (1000 x 64 f32 to 60,000 entries 17.9 us, 28.0 by three launches; to 1M 64 and 74; 300 x 37 to 300
+    // 15.9 and 21.8; 1000 x 1000 to one 19.5 and 22.3)
+    g.lists = (g.workers + (int64_t)SUM_WAVES * g.groups - 1) / ((int64_t)SUM_WAVES * g.groups);
+    g.few = c.rows >= 1 && c.rows <= FEW_ROWS && g.lists * g.cols <= 64 * (int64_t)c.num_cus;
+    if (g.few) {
+        g.whole = 64;
+        g.per = ((c.rows + SUM_WAVES - 1) / SUM_WAVES + 63) / 64 * 64;
+    }
     return g;
 }
 
@@ -931,7 +1126,8 @@ hipError_t sort_pass(hipStream_t st, const Pass &p) {
 template <typename T, int E, bool BASE, bool ONE>
 void sums(hipStream_t st, const Sums &s, int cols) {
     const int64_t each = SUM_WAVES * s.groups;
-    const size_t lds = sizeof(uint32_t) * std::max(4 * (size_t)held_rows((int)each * s.per, s.whole) + 1,
+    const size_t most = (size_t)held_rows((int)each * s.per, s.whole);
+    const size_t lds = sizeof(uint32_t) * std::max((s.dense ? 2 : 4) * most + AHEAD + 1,
                                                    (size_t)SUM_THREADS * E);
     hipLaunchKernelGGL((k_embed_sum<T, E, BASE, ONE>),
                        grid_of((s.workers + each - 1) / each, (uint32_t)cols), dim3(SUM_THREADS), lds,
@@ -953,6 +1149,22 @@ hipError_t sums(hipStream_t st, const Sums &s, const GradShape &g, int num_cus) 
                        dim3((uint32_t)(4 * num_cus), (uint32_t)std::min(turns, 16)),
                        dim3(JOIN_THREADS), 0, st, s);
     return hipGetLastError();
+}
+
+template <typename T, int E, bool BASE>
+hipError_t few(hipStream_t st, const Sums &s, const Pass &p, const GradShape &g) {
+    const int64_t longs = s.rows / (s.whole + 1);
+    hipLaunchKernelGGL((k_embed_few<T, E, BASE>),
+                       dim3((uint32_t)(g.lists + longs), (uint32_t)g.cols), dim3(SUM_THREADS),
+                       4 * (size_t)few_layout(s, p.bits, E).all, st, s, p, g.passes,
+                       (int32_t)g.lists);
+    return hipGetLastError();
+}
+template <typename T>
+hipError_t few(hipStream_t st, const Sums &s, const Pass &p, const GradShape &g) {
+    constexpr int E = 16 / sizeof(T);
+    if (g.elements > 1) return s.base ? few<T, E, true>(st, s, p, g) : few<T, E, false>(st, s, p, g);
+    return s.base ? few<T, 1, true>(st, s, p, g) : few<T, 1, false>(st, s, p, g);
 }
 
 template <typename T>
@@ -978,6 +1190,7 @@ hipError_t launch_embed(hipStream_t s, const EmbedCall &call) {
 
 size_t embed_grad_scratch(const EmbedCall &c) {
     const GradShape g = grad_shape(c);
+    if (g.few) return 0;
     const size_t rows = rounded((size_t)c.rows * sizeof(uint2));
     return (g.small || g.passes < 2 ? 1 : 2) * rows + table_bytes(g) +
            rounded(4 * (size_t)g.workers) + rounded(8 + 8 * (size_t)g.workers) +
@@ -1008,6 +1221,30 @@ hipError_t launch_embed_grad(hipStream_t st, const EmbedCall &c, char *scratch) 
     p.bits = g.bits;
     p.table = table;
     p.zero = s.found;
+    s.rows = c.rows;
+    s.workers = g.workers;
+    s.entries = (uint32_t)c.entries;
+    s.dim = c.dim;
+    s.chunks = g.chunks;
+    s.lanes = g.lanes;
+    s.groups = g.groups;
+    s.per = g.items;
+    s.whole = g.whole;
+    s.dense = g.dense;
+    // whole lines only: narrower rows' are made whole by the caches (16M entries of 4 f32 704 us past
+    // them, 134 so; 2M of 32, lines of 128 bytes, 93 past them and 97)
+    s.streamed = g.dense && g.lanes * g.elements * (c.bf16 ? 2 : 4) >= 128 &&
+                 c.entries * c.dim * (c.bf16 ? 2 : 4) > STREAMED;
+    s.row_stride = c.row_stride;
+    s.table_stride = c.table_stride;
+    s.scale = c.scale;
+    s.dout = c.dout;
+    s.base = c.base;
+    s.dtable = c.dtable;
+    if (g.few) {
+        p.ids = c.ids;
+        return c.bf16 ? few<__bf16>(st, s, p, g) : few<float>(st, s, p, g);
+    }
     int to = 0;
     if (g.small) {
         const hipError_t e = allow_all_lds(reinterpret_cast<const void *>(k_embed_sort_small));
@@ -1029,24 +1266,7 @@ hipError_t launch_embed_grad(hipStream_t st, const EmbedCall &c, char *scratch) 
             if (e != hipSuccess) return e;
         }
     }
-    s.rows = c.rows;
-    s.workers = g.workers;
-    s.entries = (uint32_t)c.entries;
-    s.dim = c.dim;
-    s.chunks = g.chunks;
-    s.lanes = g.lanes;
-    s.groups = g.groups;
-    s.per = g.items;
-    s.whole = g.whole;
-    s.dense = g.dense;
-    s.streamed = g.dense && c.entries * c.dim * (c.bf16 ? 2 : 4) > STREAMED;
-    s.row_stride = c.row_stride;
-    s.table_stride = c.table_stride;
-    s.scale = c.scale;
     s.sorted = pairs[to];
-    s.dout = c.dout;
-    s.base = c.base;
-    s.dtable = c.dtable;
     return c.bf16 ? sums<__bf16>(st, s, g, c.num_cus) : sums<float>(st, s, g, c.num_cus);
 }
 
