@@ -13,35 +13,34 @@ namespace {
 __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(__bf16 v) { return (float)v; }
 
-// E elements at p as f32, of which the first n are read; the rest are 0.  E > 1: 16 bytes at an
-// address that is a multiple of 16.
+// E elements in a row, at any address that holds one.
+template <typename T, int E>
+using Run = T __attribute__((ext_vector_type(E), aligned(sizeof(T))));
+
+// E elements at p as f32, of which the first n are read; the rest are 0.
 template <typename T, int E>
 __device__ __forceinline__ void load(const T *p, int n, float (&f)[E]) {
-    if constexpr (E > 1) {
-        typedef T V __attribute__((ext_vector_type(E)));
+    if constexpr (E > 1)
         if (n >= E) {
-            const V v = *reinterpret_cast<const V *>(p);
+            const Run<T, E> v = *reinterpret_cast<const Run<T, E> *>(p);
 #pragma unroll
             for (int e = 0; e < E; ++e) f[e] = to_f32(v[e]);
             return;
         }
-    }
 #pragma unroll
     for (int e = 0; e < E; ++e) f[e] = e < n ? to_f32(p[e]) : 0.0f;
 }
 
 template <typename T, int E>
 __device__ __forceinline__ void store(T *p, int n, const float (&f)[E], bool streamed) {
-    if constexpr (E > 1) {
-        typedef T V __attribute__((ext_vector_type(E)));
+    if constexpr (E > 1)
         if (n >= E) {
-            V v;
+            Run<T, E> v;
 #pragma unroll
             for (int e = 0; e < E; ++e) v[e] = (T)f[e];
-            put(reinterpret_cast<V *>(p), v, streamed);
+            put(reinterpret_cast<Run<T, E> *>(p), v, streamed);
             return;
         }
-    }
 #pragma unroll
     for (int e = 0; e < E; ++e)
         if (e < n) p[e] = (T)f[e];
@@ -62,6 +61,9 @@ __global__ __launch_bounds__(256) void k_embed(EmbedCall c, int32_t chunks) {
     const T *table = static_cast<const T *>(c.table);
     const T *base = static_cast<const T *>(c.base);
     T *out = static_cast<T *>(c.out);
+    // the last piece of a row is its last E columns, some of which the one before writes too, but
+    // where it may have written them to the base
+    const bool last_whole = E > 1 && base != out;
     int64_t row[LOOKUP];
     int col[LOOKUP];
     int32_t id[LOOKUP];
@@ -72,6 +74,7 @@ __global__ __launch_bounds__(256) void k_embed(EmbedCall c, int32_t chunks) {
         const uint32_t r = i / (uint32_t)chunks;
         row[q] = row0 + r;
         col[q] = (int)(i - r * chunks) * E;
+        if (last_whole) col[q] = min(col[q], c.dim - E);
         here[q] = row[q] < c.rows;
         id[q] = here[q] ? c.ids[row[q]] : -1;
     }
@@ -550,10 +553,6 @@ __device__ __forceinline__ void both_ends(const Sums &s, const int64_t (&d)[2], 
     found[1] = lo[1];
 }
 
-// E elements in a row, at any address that holds one.
-template <typename T, int E>
-using Run = T __attribute__((ext_vector_type(E), aligned(sizeof(T))));
-
 // The items [p, end): rows are added to acc, at_entry(entry, its base) takes it.  next: the next
 // entry, where all are on the list.  SOME: some entries are passed.
 template <typename T, int E, bool BASE, bool ONE, bool SOME, class AtEntry>
@@ -1031,10 +1030,6 @@ __global__ __launch_bounds__(SUM_THREADS) void k_embed_few(Sums s, Pass p, int32
     walk<T, E, BASE, false, true>(s, item, at, end, from.e, dout, base, dtable, acc, write);
 }
 
-bool aligned(const void *p, int64_t stride, size_t size) {
-    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * (int64_t)size % 16 == 0;
-}
-
 int bits_of(int64_t most) {          // of keys 0..most
     int bits = 1;
     while (bits < 32 && (most >> bits)) ++bits;
@@ -1170,12 +1165,9 @@ hipError_t few(hipStream_t st, const Sums &s, const Pass &p, const GradShape &g)
 template <typename T>
 hipError_t lookup(hipStream_t st, const EmbedCall &c) {
     constexpr int E = 16 / sizeof(T);
-    const bool wide = aligned(c.table, c.table_stride, sizeof(T)) &&
-                      aligned(c.out, c.row_stride, sizeof(T)) &&
-                      (!c.base || aligned(c.base, c.row_stride, sizeof(T)));
-    const int32_t chunks = wide ? (c.dim + E - 1) / E : c.dim;
+    const int32_t chunks = c.dim >= E ? (c.dim + E - 1) / E : c.dim;
     const dim3 g = grid_of((c.rows * chunks + 256 * LOOKUP - 1) / (256 * LOOKUP));
-    if (wide) hipLaunchKernelGGL((k_embed<T, E>), g, dim3(256), 0, st, c, chunks);
+    if (c.dim >= E) hipLaunchKernelGGL((k_embed<T, E>), g, dim3(256), 0, st, c, chunks);
     else hipLaunchKernelGGL((k_embed<T, 1>), g, dim3(256), 0, st, c, chunks);
     return hipGetLastError();
 }
