@@ -84,7 +84,8 @@ int mbk_context_create(int32_t device, mbk_context **out, char **err);
  * caller's own work there.  The stream must outlive the context; mbk_context_destroy waits for it.
  * While it is captured no context is made on it, and mbk_context_destroy leaves the context as
  * it is: call it again after the capture.
- * mbk_xent, mbk_xent_grad and the mbk_expert_ calls may be captured there into a
+ * mbk_xent, mbk_xent_grad, the mbk_expert_ calls, mbk_embed, mbk_embed_grad, mbk_grad_clip,
+ * mbk_fourbit_pack, mbk_fourbit_scores and mbk_adjust may be captured there into a
  * graph.  Their scratch belongs to the context: it grows outside a capture only (a
  * captured call that needs more is refused: make one of the same sizes before), what a
  * graph has captured is kept until the context is destroyed, and graphs of one context
@@ -419,7 +420,8 @@ int mbk_embed_grad(mbk_context *ctx, const mbk_embed_shape *shape, const int32_t
  * within the call, which waits for the context's stream).  The list belongs to the context:
  * mbk_tensors_destroy gives it back (after the stream's work; while the stream is captured, and
  * for a list that a captured call has used, its memory stays until the context is destroyed), and
- * so does mbk_context_destroy.
+ * so does mbk_context_destroy.  An out overlaps no other out, and of the gradients that have outs
+ * only its own; one that begins where one of those does is refused.
  * mbk_grad_clip: norm[0] (device) = the root of the sum of all squares, and every out = grad *
  * min(1, max_norm / norm).  A sum of squares that is not finite leaves out = grad: the norm
  * tells.  A norm beyond f32 is +INFINITY, but clips.  max_norm may be INFINITY (outs are
@@ -446,13 +448,14 @@ int mbk_grad_clip(mbk_context *ctx, mbk_tensors *list, float max_norm, float *no
  * mbk_fourbit_pack lays w (device, [classes] rows of dim elements, stride apart) out so, in
  * mbk_fourbit_bytes(shape) bytes at an address that is a multiple of 16 (device; the layout is the
  * library's own).  mbk_fourbit_bytes is -1 for a shape that the calls refuse.
- * mbk_fourbit_scores: scores[row][v] = h[row] . w[v] + bias[v] (bias NULL: 0), f32; a class whose bias
- * is -INFINITY has that score whatever its w and h hold.
+ * mbk_fourbit_scores: scores[row][v] = h[row] . w[v] + bias[v] (bias NULL: 0), f32; a class whose
+ * bias is -INFINITY has that score whatever its w and h hold.
  * Elements of w are taken as they are, but for groups whose scale is below 2^-28 of their class's
  * largest, whose elements are off by up to 2^-33 of that scale; bf16 h as it is, but for what is
  * below 2^-31 of its row's largest, off by up to 2^-39 of that; f32 h with 22 bits, and beside the
- * row's largest off by up to 2^-50 of it.  Sums are f32, rounded with the bias once more.  A class whose w is not finite
- * has scores that are NaN, a row whose h is not finite has scores that are not finite. */
+ * row's largest off by up to 2^-50 of it.  Sums are f32, rounded with the bias once more.  A class
+ * whose w is not finite has scores that are NaN, a row whose h is not finite has scores that are not
+ * finite. */
 typedef struct {
     int64_t classes;             /* 1..2^31-256 */
     int32_t dim;                 /* 1..2^20 */
@@ -460,10 +463,10 @@ typedef struct {
 } mbk_fourbit_shape;
 int64_t mbk_fourbit_bytes(const mbk_fourbit_shape *shape);
 int mbk_fourbit_pack(mbk_context *ctx, const mbk_fourbit_shape *shape, int32_t type, const void *w,
-                int64_t w_stride, void *packed, char **err);
+                     int64_t w_stride, void *packed, char **err);
 int mbk_fourbit_scores(mbk_context *ctx, const mbk_fourbit_shape *shape, int64_t rows, int32_t type,
-                  const void *h, int64_t h_stride, const void *packed, const float *bias,
-                  float *scores, int64_t score_stride, char **err);
+                       const void *h, int64_t h_stride, const void *packed, const float *bias,
+                       float *scores, int64_t score_stride, char **err);
 
 /* ---- penalties, biases and masks of scores.  No counterpart in the reference.  All arrays are
  * device memory.  With c the times that class v is among the row's first lengths[row] ids of

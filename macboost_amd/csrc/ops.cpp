@@ -7,6 +7,7 @@
 // use scratch are queued whole, one after another, whichever threads make them.
 #include <algorithm>
 #include <cmath>
+#include <functional>
 #include <vector>
 
 #include "../../include/macboost.h"
@@ -134,6 +135,21 @@ void add_pieces(const mbk_tensor &t, int64_t most, int64_t runs, std::vector<mbk
     const int64_t chunks = (cols * size + 15) / 16;
     const int64_t each = std::max<int64_t>(1, std::min(most / cols, runs / chunks));
     for (int64_t r = 0; r < rows; r += each) add(r * t.stride, std::min(each, rows - r), cols);
+}
+
+// Two outs at one place would be scaled twice, and an out that is another's gradient be read after
+// that.  (A gradient without an out is read before all stores.)
+void need_apart(const mbk_tensor *list, int32_t count) {
+    const auto some = [&](int32_t i) { return list[i].rows && list[i].cols; };
+    std::vector<const void *> outs;
+    for (int32_t i = 0; i < count; ++i)
+        if (list[i].out && some(i)) outs.push_back(list[i].out);
+    std::sort(outs.begin(), outs.end(), std::less<>());
+    bool apart = std::adjacent_find(outs.begin(), outs.end()) == outs.end();
+    for (int32_t i = 0; i < count && apart; ++i)
+        apart = !some(i) || !list[i].out || list[i].out == list[i].grad ||
+                !std::binary_search(outs.begin(), outs.end(), list[i].grad, std::less<>());
+    need(apart, "an out is also another gradient or its out");
 }
 
 mbk::FourbitShape fourbit_shape(const mbk_fourbit_shape *sh) {
@@ -287,6 +303,7 @@ int mbk_tensors_create(mbk_context *ctx, const mbk_tensor *list, int32_t count, 
                      reinterpret_cast<uintptr_t>(t.out) % size == 0,
                  "grad and out must be multiples of their elements' size");
         }
+        need_apart(list, count);
         std::vector<mbk::ClipPiece> pieces;
         auto made = std::make_unique<mbk_tensors>();
         int64_t written = 0;

@@ -72,6 +72,24 @@ def test_tensors(change, msg):
     assert not out.value
 
 
+Q = 0x9000
+
+
+@pytest.mark.parametrize("pairs,apart", [
+    ([(P, P), (P, P)], False), ([(P, Q), (Q, P)], False), ([(P, Q), (P, Q)], False),
+    ([(P, P), (P, Q)], False), ([(P, P), (Q, P)], False), ([(P, P), (P, None)], True),
+    ([(P, None), (P, None)], True), ([(P, P), (Q, Q)], True), ([(P, Q), (P, None)], True),
+])
+def test_a_place_has_one_output(pairs, apart):
+    """A gradient may be listed again without an output: it counts twice in the norm."""
+    out = ctypes.c_void_p()
+    made = [_core.MbkTensor(**{**TENSOR, "grad": g, "out": o}) for g, o in pairs]
+    empty = _core.MbkTensor(**{**TENSOR, "out": P, "rows": 0})
+    msg = "null kernel-seam context" if apart else "also another gradient"
+    with pytest.raises(mb.MacBoostError, match=msg):
+        _call("mbk_tensors_create", (_core.MbkTensor * 3)(*made, empty), 3, ctypes.byref(out))
+
+
 def test_lists_and_norms():
     out = ctypes.c_void_p()
     with pytest.raises(mb.MacBoostError, match="count must be"):
