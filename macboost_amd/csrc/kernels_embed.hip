@@ -1040,6 +1040,142 @@ __global__ __launch_bounds__(SUM_THREADS) void k_embed_few(Sums s, Pass p, int32
     walk<T, E, BASE, false, true>(s, item, at, end, from.e, dout, base, dtable, acc, write);
 }
 
+// ---------------------------------------------------------------------------
+// Few entries: slices of up to FEW_ROWS rows, each sorted and summed by a workgroup, which writes the
+// sums of the entries that it has and a bit for each of them; and those of all slices summed up.
+// ---------------------------------------------------------------------------
+constexpr int SLICE_WORDS = (1 << MOST_BITS) / 32;   // bits of a slice's entries
+
+template <typename T, int E>
+__global__ __launch_bounds__(SUM_THREADS) void k_embed_slice(Sums s, Pass p) {
+    extern __shared__ uint32_t lds[];
+    uint32_t *wave_sum = lds, *bits = lds + SUM_WAVES, *key = bits + SLICE_WORDS;
+    uint16_t *order = reinterpret_cast<uint16_t *>(key + FEW_ROWS);
+    uint32_t *rest = key + FEW_ROWS + FEW_ROWS / 2;
+    const int64_t row0 = (int64_t)blockIdx.x * s.whole;
+    p.ids += row0;
+    p.rows = min(p.rows - row0, (int64_t)s.whole);
+    if (threadIdx.x < SLICE_WORDS) bits[threadIdx.x] = 0;
+    {
+        uint32_t k[FEW_EACH];
+        uint16_t r[FEW_EACH];
+        sort_in_lds<SUM_WAVES>(p, 1, wave_sum, rest, key, order, k, r);
+    }
+    const int kept = first_not(0, (int)p.rows, [&](int m) { return key[m] < s.entries; });
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int group = lane / s.lanes, chunk0 = blockIdx.y * 64 + lane - group * s.lanes;
+    const int32_t chunk = min(chunk0, s.chunks - 1);
+    const int col = min(chunk * E, s.dim - E);
+    const T *dout = static_cast<const T *>(s.dout) + row0 * s.row_stride + col;
+    float *sums = s.parts + (int64_t)blockIdx.x * s.entries * s.part_stride + col;
+    for (int i = threadIdx.x; i < kept; i += SUM_THREADS)
+        if (i == 0 || key[i - 1] != key[i]) atomicOr(&bits[key[i] >> 5], 1u << (key[i] & 31));
+    // a worker takes `each` rows of the sorted list.  What it has of an entry that a worker before
+    // began goes to the LDS, where the worker that began it finds it.
+    const int mine = wave * s.groups + group, workers = SUM_WAVES * s.groups;
+    const bool idle = group >= s.groups || chunk0 >= s.chunks;
+    const int each = (kept + workers - 1) / workers;
+    const int a = idle ? kept : min(kept, mine * each), b = min(kept, a + each);
+    float acc[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.0f;
+    float *head = reinterpret_cast<float *>(rest);
+    const auto write = [&](uint32_t entry) {
+        Run<float, E> out;
+#pragma unroll
+        for (int e = 0; e < E; ++e) out[e] = acc[e];
+        *reinterpret_cast<Run<float, E> *>(sums + (int64_t)entry * s.part_stride) = out;
+    };
+    const auto leave = [&]() {
+#pragma unroll
+        for (int e = 0; e < E; ++e) head[threadIdx.x * E + e] = acc[e];
+    };
+    bool begun = a > 0 && a < b && key[a - 1] == key[a];     // by a worker before
+    for (int i = a; i < b; i += AHEAD) {
+        Run<T, E> v[AHEAD];
+#pragma unroll
+        for (int q = 0; q < AHEAD; ++q)
+            v[q] = *reinterpret_cast<const Run<T, E> *>(dout + order[min(i + q, b - 1)] *
+                                                                   s.row_stride);
+#pragma unroll
+        for (int q = 0; q < AHEAD; ++q) {
+            if (i + q >= b) break;
+            if (i + q > a && key[i + q - 1] != key[i + q]) {
+                if (begun) leave();
+                else write(key[i + q - 1]);
+                begun = false;
+#pragma unroll
+                for (int e = 0; e < E; ++e) acc[e] = 0.0f;
+            }
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[e] += to_f32(v[q][e]);
+        }
+    }
+    if (a < b && begun) leave();
+    __syncthreads();
+    if (blockIdx.y == 0 && threadIdx.x < SLICE_WORDS)
+        s.open[(int64_t)blockIdx.x * SLICE_WORDS + threadIdx.x] = bits[threadIdx.x];
+    if (a >= b || begun) return;
+    const uint32_t entry = key[b - 1];
+    for (int w = mine + 1, at = b; at < kept && key[at] == entry; ++w, at += each) {
+        const int from = (w / s.groups * 64 + w % s.groups * s.lanes + lane - group * s.lanes) * E;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] += head[from + e];
+    }
+    write(entry);
+}
+
+// A workgroup an entry and 256 columns, four a lane; the lanes share the slices.
+template <typename T>
+__global__ __launch_bounds__(SUM_THREADS) void k_embed_total(Sums s, int32_t slices) {
+    typedef float V __attribute__((ext_vector_type(4)));
+    __shared__ V meet[SUM_THREADS];
+    const uint32_t entry = blockIdx.x;
+    const int chunks = s.part_stride / 4 - blockIdx.y * 64, lanes = min(chunks, 64);
+    const int sub = threadIdx.x / lanes, subs = SUM_THREADS / lanes;
+    const int64_t col = (blockIdx.y * 64 + threadIdx.x - sub * lanes) * 4;
+    V acc = {0, 0, 0, 0};
+    bool any = false;
+    if (sub < subs)
+        for (int p0 = sub; p0 < slices; p0 += AHEAD * subs) {
+            uint32_t word[AHEAD];
+            V v[AHEAD];
+#pragma unroll
+            for (int q = 0; q < AHEAD; ++q) {
+                const int64_t p = min(p0 + q * subs, slices - 1);
+                word[q] = s.open[p * SLICE_WORDS + (entry >> 5)];
+                v[q] = *reinterpret_cast<const V *>(s.parts + (p * s.entries + entry) *
+                                                                  s.part_stride + col);
+            }
+#pragma unroll
+            for (int q = 0; q < AHEAD; ++q) {            // what is not there was not written
+                const bool there = p0 + q * subs < slices && ((word[q] >> (entry & 31)) & 1u);
+                any |= there;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[e] = there ? acc[e] + v[q][e] : acc[e];
+            }
+        }
+    meet[threadIdx.x] = acc;
+    if (!__syncthreads_or(any) && s.base == s.dtable) return;
+    for (int o = SUM_THREADS / 2; o > 0; o >>= 1) {
+        if (sub < o && sub + o < subs) {
+            const V other = meet[threadIdx.x + o * lanes];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[e] += other[e];
+            meet[threadIdx.x] = acc;
+        }
+        __syncthreads();
+    }
+    if (sub != 0) return;
+    const int n = (int)min((int64_t)4, s.dim - col);
+    const int64_t at = (int64_t)entry * s.table_stride + col;
+    float b[4] = {0, 0, 0, 0}, out[4];
+    if (s.base) load<T, 4>(static_cast<const T *>(s.base) + at, n, b);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) out[e] = __builtin_fmaf(s.scale, acc[e], b[e]);
+    store<T, 4>(static_cast<T *>(s.dtable) + at, n, out, false);
+}
+
 int bits_of(int64_t most) {          // of keys 0..most
     int bits = 1;
     while (bits < 32 && (most >> bits)) ++bits;
@@ -1058,7 +1194,10 @@ struct GradShape {
     int64_t workers;
     bool few;                        // one launch
     int64_t lists;                   // its workgroups of the list
+    int64_t slices;                  // of few entries, g.whole rows each; 0: none
 };
+
+constexpr int64_t SLICE_LEAST = 256, SLICE_BYTES = (int64_t)128 << 20;
 
 GradShape grad_shape(const EmbedCall &c) {
     GradShape g{};
@@ -1107,6 +1246,18 @@ GradShape grad_shape(const EmbedCall &c) {
     if (g.few) {
         g.whole = 64;
         g.per = ((c.rows + SUM_WAVES - 1) / SUM_WAVES + 63) / 64 * 64;
+    }
+    const int64_t slice = std::min<int64_t>(
+        FEW_ROWS, std::max<int64_t>(SLICE_LEAST, ((c.rows + c.num_cus - 1) / c.num_cus + 63) / 64 * 64));
+    const int64_t slices = (c.rows + slice - 1) / slice;
+    if (c.rows > FEW_ROWS && c.entries < (1 << MOST_BITS) && g.cols <= 4 &&
+        slices * c.entries * c.dim * 4 <= SLICE_BYTES) {
+        g.slices = slices;
+        g.whole = (int)slice;
+        g.bits = std::max(3, bits);
+        g.per = ((slice + SUM_WAVES - 1) / SUM_WAVES + 63) / 64 * 64;
+        // 16 rows a worker at least
+        g.groups = (int)std::min<int64_t>(64 / g.lanes, (slice + 16 * SUM_WAVES - 1) / (16 * SUM_WAVES));
     }
     return g;
 }
@@ -1173,6 +1324,20 @@ hipError_t few(hipStream_t st, const Sums &s, const Pass &p, const GradShape &g)
 }
 
 template <typename T>
+hipError_t slices(hipStream_t st, const Sums &s, const Pass &p, const GradShape &g) {
+    constexpr int E = 16 / sizeof(T);
+    const dim3 grid((uint32_t)g.slices, (uint32_t)g.cols), block(SUM_THREADS);
+    const size_t lds = 4 * (SUM_WAVES + SLICE_WORDS + (size_t)FEW_ROWS / 2 * 3 +
+                            std::max((size_t)SUM_WAVES << p.bits, (size_t)SUM_THREADS * g.elements));
+    if (g.elements > 1) hipLaunchKernelGGL((k_embed_slice<T, E>), grid, block, lds, st, s, p);
+    else hipLaunchKernelGGL((k_embed_slice<T, 1>), grid, block, lds, st, s, p);
+    hipLaunchKernelGGL((k_embed_total<T>),
+                       dim3(s.entries, (uint32_t)((s.part_stride / 4 + 63) / 64)), block, 0, st, s,
+                       (int32_t)g.slices);
+    return hipGetLastError();
+}
+
+template <typename T>
 hipError_t lookup(hipStream_t st, const EmbedCall &c) {
     constexpr int E = 16 / sizeof(T);
     const int32_t chunks = c.dim >= E ? (c.dim + E - 1) / E : c.dim;
@@ -1193,6 +1358,9 @@ hipError_t launch_embed(hipStream_t s, const EmbedCall &call) {
 size_t embed_grad_scratch(const EmbedCall &c) {
     const GradShape g = grad_shape(c);
     if (g.few) return 0;
+    if (g.slices)
+        return rounded(4 * SLICE_WORDS * (size_t)g.slices) +
+               4 * (size_t)(g.slices * c.entries) * part_stride(c);
     const size_t rows = rounded((size_t)c.rows * sizeof(uint2));
     return (g.small || g.passes < 2 ? 1 : 2) * rows + table_bytes(g) +
            rounded(4 * (size_t)g.workers) + rounded(8 + 8 * (size_t)g.workers) +
@@ -1201,6 +1369,7 @@ size_t embed_grad_scratch(const EmbedCall &c) {
 
 hipError_t launch_embed_grad(hipStream_t st, const EmbedCall &c, char *scratch) {
     const GradShape g = grad_shape(c);
+    char *const scratch0 = scratch;
     const size_t rows = rounded((size_t)c.rows * sizeof(uint2));
     uint2 *pairs[2];
     for (int i = 0; i < (g.small || g.passes < 2 ? 1 : 2); ++i) {
@@ -1246,6 +1415,12 @@ hipError_t launch_embed_grad(hipStream_t st, const EmbedCall &c, char *scratch) 
     if (g.few) {
         p.ids = c.ids;
         return c.bf16 ? few<__bf16>(st, s, p, g) : few<float>(st, s, p, g);
+    }
+    if (g.slices) {
+        p.ids = c.ids;
+        s.open = reinterpret_cast<uint32_t *>(scratch0);
+        s.parts = reinterpret_cast<float *>(scratch0 + rounded(4 * SLICE_WORDS * (size_t)g.slices));
+        return c.bf16 ? slices<__bf16>(st, s, p, g) : slices<float>(st, s, p, g);
     }
     int to = 0;
     if (g.small) {
