@@ -1197,7 +1197,7 @@ struct GradShape {
     int64_t slices;                  // of few entries, g.whole rows each; 0: none
 };
 
-constexpr int64_t SLICE_LEAST = 256, SLICE_BYTES = (int64_t)128 << 20;
+constexpr int64_t SLICE_LEAST = 128, SLICE_BYTES = (int64_t)64 << 20;
 
 GradShape grad_shape(const EmbedCall &c) {
     GradShape g{};
@@ -1248,7 +1248,7 @@ GradShape grad_shape(const EmbedCall &c) {
         g.per = ((c.rows + SUM_WAVES - 1) / SUM_WAVES + 63) / 64 * 64;
     }
     const int64_t slice = std::min<int64_t>(
-        FEW_ROWS, std::max<int64_t>(SLICE_LEAST, ((c.rows + c.num_cus - 1) / c.num_cus + 63) / 64 * 64));
+        FEW_ROWS, std::max<int64_t>(SLICE_LEAST, (c.rows * g.cols / c.num_cus + 63) / 64 * 64));
     const int64_t slices = (c.rows + slice - 1) / slice;
     if (c.rows > FEW_ROWS && c.entries < (1 << MOST_BITS) && g.cols <= 4 &&
         slices * c.entries * c.dim * 4 <= SLICE_BYTES) {

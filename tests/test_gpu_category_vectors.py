@@ -110,6 +110,18 @@ def test_gradient(ctx, kind, rows, dim, entries, skew, pad, shift):
     M.close(out.read(), np.where(used[:, None], value, np.nan), tol)
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,dim,entries,skew,pad,shift", [
+    (1025, 3, 1, 0, 0, 0), (1025, 37, 1023, 0, 1, 1), (1025, 37, 1024, 0, 0, 0),
+    (1100, 257, 2, 0, 0, 0), (2000, 513, 9, 1, 3, 0), (1500, 1025, 1000, 0, 0, 0),
+    (33000, 16, 31, 2, 0, 0), (33000, 15, 32, 1, 0, 1), (70000, 4, 33, 3, 0, 0),
+    (70000, 1, 1023, 0, 0, 0), (262145, 8, 5, 0, 0, 0), (300000, 2, 400, 0.5, 1, 0),
+])
+def test_gradient_of_few_entries(ctx, kind, rows, dim, entries, skew, pad, shift):
+    """Up to 1023 entries, in slices of 128 to 1024 rows."""
+    test_gradient(ctx, kind, rows, dim, entries, skew, pad, shift)
+
+
 @pytest.mark.parametrize("rows", [0, 1, 100, 20000])
 @pytest.mark.parametrize("entries", [1, 5000])
 def test_gradient_without_rows_in_any_entry(ctx, rows, entries):
@@ -134,7 +146,7 @@ def test_gradient_without_rows_in_any_entry(ctx, rows, entries):
     assert np.all(out.read() == (0.0 if rows else M.GUARD))
 
 
-@pytest.mark.parametrize("rows,entries", [(3000, 40), (40000, 900)])
+@pytest.mark.parametrize("rows,entries", [(3000, 40), (40000, 900), (100000, 1500)])
 def test_gradient_of_runs_around_the_workers_ends(ctx, rows, entries):
     """Entries of 60 to 70 rows, some of 1 and of hundreds, in the ids' order."""
     rng = np.random.default_rng(rows)
