@@ -178,7 +178,7 @@ __device__ __forceinline__ uint32_t key_at(const Pass &p, int64_t i) {
 }
 
 // C: 16 bits where a workgroup has fewer than 2^13 rows.  Short of rows, not of bandwidth: 1M rows
-// 6.4 us a pass (4 MB of ids), 99991 3.4.
+// 6.4 us a pass (4 MB of ids), 16384 4.6.
 template <int R, typename C>
 __global__ __launch_bounds__(SORT_THREADS) void k_embed_count(Pass p) {
     __shared__ uint32_t count[1 << MOST_BITS];
@@ -253,7 +253,7 @@ __device__ __forceinline__ void first_places(const Pass &p, int bins, uint32_t *
 }
 
 // Bound by the latency of its chain: the counts before its own out of L2, ranks in LDS, and stores
-// to as many places as there are digits: 1M rows 14.6 us a pass, 99991 10.3.
+// to as many places as there are digits: 1M rows 14.6 us a pass, 16384 7.7.
 template <int R, typename C>
 __global__ __launch_bounds__(SORT_THREADS) void k_embed_place(Pass p) {
     extern __shared__ uint32_t lds[];
@@ -768,7 +768,7 @@ struct Span {
         return (int64_t)w * 2 + (w < last);
     }
 };
-// A launch and a chain of three reads for most: 99991 x 37 to 300 entries 6.4 us, 1M x 64 to
+// A launch and a chain of three reads for most: 16384 x 1024 to 65536 entries 6.0 us, 1M x 64 to
 // 100000 8.2.
 template <typename T>
 __global__ __launch_bounds__(JOIN_THREADS) void k_embed_join(Sums s) {
@@ -1043,6 +1043,9 @@ __global__ __launch_bounds__(SUM_THREADS) void k_embed_few(Sums s, Pass p, int32
 // ---------------------------------------------------------------------------
 // Few entries: slices of up to FEW_ROWS rows, each sorted and summed by a workgroup, which writes the
 // sums of the entries that it has and a bit for each of them; and those of all slices summed up.
+// Two launches instead of four or more.  The first is bound by its sort (7 us) and then by reading
+// dout: 99991 x 37 to 300 entries 13.4 us and 6.0 for the sums' sums, 1M x 64 to 5 43.5 (5.9 TB/s)
+// and 8.5.
 // ---------------------------------------------------------------------------
 constexpr int SLICE_WORDS = (1 << MOST_BITS) / 32;   // bits of a slice's entries
 
@@ -1197,6 +1200,10 @@ struct GradShape {
     int64_t slices;                  // of few entries, g.whole rows each; 0: none
 };
 
+// Slices: as many as CUs, down to 128 rows (10000 x 64 to 1000: 15.0 us, 19.5 by 64 rows and 18.5 by
+// 512), while their sums do not outweigh the longer sort (with the host's call, 50000 x 64 to 1000,
+// 50 MB of sums: 22.2 us, 35.6 without slices; 1M x 16 to 1000, 63 MB: 48.4 and 63.0; 300000 x 256 to
+// 300, 105 MB: 115 and 83).
 constexpr int64_t SLICE_LEAST = 128, SLICE_BYTES = (int64_t)64 << 20;
 
 GradShape grad_shape(const EmbedCall &c) {
