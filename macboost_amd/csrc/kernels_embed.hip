@@ -357,7 +357,8 @@ __device__ __forceinline__ void sort_in_lds(const Pass &p, int passes, uint32_t 
     }
     for (int s = 0; s < passes; ++s) {
         const int shift = s * p.bits;
-        for (int d = threadIdx.x; d < WAVES * bins; d += N) count[d] = 0;
+        for (int d = threadIdx.x * 4; d < WAVES * bins; d += N * 4)
+            *reinterpret_cast<uint4 *>(count + d) = make_uint4(0, 0, 0, 0);
         __syncthreads();
         uint32_t *mine = count + wave * bins;
         uint32_t digit[EACH];
@@ -379,20 +380,31 @@ __device__ __forceinline__ void sort_in_lds(const Pass &p, int passes, uint32_t 
             __builtin_amdgcn_wave_barrier();
         }
         __syncthreads();
-        uint32_t before = 0, all;
-        for (int d0 = 0; d0 < bins; d0 += N) {
-            const int d = d0 + threadIdx.x;
-            uint32_t sum = 0;
-            if (d < bins)
-                for (int v = 0; v < WAVES; ++v) sum += count[v * bins + d];
-            uint32_t at = before + sum_before<WAVES>(sum, wave_sum, all);
-            if (d < bins)
-                for (int v = 0; v < WAVES; ++v) {
-                    const uint32_t n = count[v * bins + d];
-                    count[v * bins + d] = at;
-                    at += n;
-                }
-            before += all;
+        // a thread the digits DIGITS t and on
+        constexpr int DIGITS = (1 << MOST_BITS) / N > 1 ? (1 << MOST_BITS) / N : 1;
+        typedef uint32_t D __attribute__((ext_vector_type(DIGITS)));
+        D *counts = reinterpret_cast<D *>(count) + threadIdx.x;
+        D sum = 0;
+        if ((int)threadIdx.x * DIGITS < bins)
+#pragma unroll
+            for (int v = 0; v < WAVES; ++v) sum += counts[v * bins / DIGITS];
+        uint32_t total = 0, all;
+#pragma unroll
+        for (int e = 0; e < DIGITS; ++e) total += sum[e];
+        total = sum_before<WAVES>(total, wave_sum, all);
+        if ((int)threadIdx.x * DIGITS < bins) {
+            D at;
+#pragma unroll
+            for (int e = 0; e < DIGITS; ++e) {
+                at[e] = total;
+                total += sum[e];
+            }
+#pragma unroll
+            for (int v = 0; v < WAVES; ++v) {
+                const D n = counts[v * bins / DIGITS];
+                counts[v * bins / DIGITS] = at;
+                at += n;
+            }
         }
         __syncthreads();
 #pragma unroll
