@@ -891,7 +891,7 @@ __global__ __launch_bounds__(JOIN_THREADS) void k_embed_join(Sums s) {
 }
 
 // ---------------------------------------------------------------------------
-// Up to FEW_ROWS rows: one launch, bound by the chain of the sort (6 us) and the reads behind it
+// Up to FEW_ROWS rows to many entries: one launch, bound by the chain of the sort (6 us) and the reads behind it
 // (1000 x 64 f32 to 60000 entries 17.9 us with the host's call).  Every workgroup sorts all of them for
 // itself; the first `lists` take the merged list as above, without the entries of more than `whole`
 // rows, and each of the others one of those.
@@ -1217,6 +1217,7 @@ struct GradShape {
 // 50 MB of sums: 22.2 us, 35.6 without slices; 1M x 16 to 1000, 63 MB: 48.4 and 63.0; 300000 x 256 to
 // 300, 105 MB: 115 and 83).
 constexpr int64_t SLICE_LEAST = 128, SLICE_BYTES = (int64_t)64 << 20;
+constexpr int64_t SLICED_FEW = 48, SLICED_FEW_ELEMENTS = (int64_t)1 << 18;
 
 GradShape grad_shape(const EmbedCall &c) {
     GradShape g{};
@@ -1258,8 +1259,7 @@ GradShape grad_shape(const EmbedCall &c) {
     g.whole = c.rows <= 64 ? 64 : g.items;           // few rows: nothing to join
     g.workers = (items + per - 1) / per;
     // few rows: sorted again by each workgroup, which pays up to where there are very many of them
-    // (1000 x 64 f32 to 60,000 entries 17.9 us, 28.0 by three launches; to 1M 64 and 74; 300 x 37 to 300
-    // 15.9 and 21.8; 1000 x 1000 to one 19.5 and 22.3)
+    // (1000 x 64 f32 to 60,000 entries 17.9 us, 28.0 by three launches; to 1M 64 and 74)
     g.lists = (g.workers + (int64_t)SUM_WAVES * g.groups - 1) / ((int64_t)SUM_WAVES * g.groups);
     g.few = c.rows >= 1 && c.rows <= FEW_ROWS && g.lists * g.cols <= 64 * (int64_t)c.num_cus;
     if (g.few) {
@@ -1269,8 +1269,14 @@ GradShape grad_shape(const EmbedCall &c) {
     const int64_t slice = std::min<int64_t>(
         FEW_ROWS, std::max<int64_t>(SLICE_LEAST, (c.rows * g.cols / c.num_cus + 63) / 64 * 64));
     const int64_t slices = (c.rows + slice - 1) / slice;
-    if (c.rows > FEW_ROWS && c.entries < (1 << MOST_BITS) && g.cols <= 4 &&
+    // of up to FEW_ROWS rows where one launch takes longer than two: not of the least, nor where many
+    // entries are written twice (300 x 37 to 300 entries 11.5 us, 16.0 by one; 1000 x 1000 to one 12.1
+    // and 19.6; 32 x 1024 to 20 10.9 and 9.1; 200 x 512 to 1000 16.7 and 14.7)
+    const bool sliced =
+        !g.few || (c.rows >= SLICED_FEW && c.entries * c.dim <= SLICED_FEW_ELEMENTS);
+    if (sliced && c.rows >= 1 && c.entries < (1 << MOST_BITS) && g.cols <= 4 &&
         slices * c.entries * c.dim * 4 <= SLICE_BYTES) {
+        g.few = false;
         g.slices = slices;
         g.whole = (int)slice;
         g.bits = std::max(3, bits);

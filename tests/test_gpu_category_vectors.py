@@ -112,6 +112,8 @@ def test_gradient(ctx, kind, rows, dim, entries, skew, pad, shift):
 
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
 @pytest.mark.parametrize("rows,dim,entries,skew,pad,shift", [
+    (47, 8, 30, 0, 0, 0), (48, 8, 30, 0, 0, 0), (129, 37, 7, 1, 3, 1), (1000, 256, 1023, 0, 0, 0),
+    (1000, 1000, 1, 0, 0, 0), (1000, 300, 1023, 1, 0, 0), (1000, 4, 1024, 0, 0, 0),
     (1025, 3, 1, 0, 0, 0), (1025, 37, 1023, 0, 1, 1), (1025, 37, 1024, 0, 0, 0),
     (1100, 257, 2, 0, 0, 0), (2000, 513, 9, 1, 3, 0), (1500, 1025, 1000, 0, 0, 0),
     (33000, 16, 31, 2, 0, 0), (33000, 15, 32, 1, 0, 1), (70000, 4, 33, 3, 0, 0),
