@@ -1219,6 +1219,8 @@ struct GradShape {
 constexpr int64_t SLICE_LEAST = 128, SLICE_BYTES = (int64_t)64 << 20;
 constexpr int64_t SLICED_FEW = 48, SLICED_FEW_ELEMENTS = (int64_t)1 << 18;
 
+int32_t part_stride(const EmbedCall &c) { return (c.dim + 3) / 4 * 4; }
+
 GradShape grad_shape(const EmbedCall &c) {
     GradShape g{};
     const int bits = bits_of(c.entries);
@@ -1275,7 +1277,7 @@ GradShape grad_shape(const EmbedCall &c) {
     const bool sliced =
         !g.few || (c.rows >= SLICED_FEW && c.entries * c.dim <= SLICED_FEW_ELEMENTS);
     if (sliced && c.rows >= 1 && c.entries < (1 << MOST_BITS) && g.cols <= 4 &&
-        slices * c.entries * c.dim * 4 <= SLICE_BYTES) {
+        slices * c.entries * part_stride(c) * 4 <= SLICE_BYTES) {
         g.few = false;
         g.slices = slices;
         g.whole = (int)slice;
@@ -1291,7 +1293,6 @@ size_t rounded(size_t bytes) { return (bytes + 255) / 256 * 256; }
 size_t table_bytes(const GradShape &g) {
     return rounded(g.small ? 0 : ((size_t)g.units << g.bits) * (g.narrow ? 2 : 4));
 }
-int32_t part_stride(const EmbedCall &c) { return (c.dim + 3) / 4 * 4; }
 
 template <int R, typename C>
 hipError_t sort_pass(hipStream_t st, const Pass &p) {
