@@ -1215,7 +1215,7 @@ struct GradShape {
 // Slices: as many as CUs, down to 128 rows (10000 x 64 to 1000: 15.0 us, 19.5 by 64 rows and 18.5 by
 // 512), while their sums do not outweigh the longer sort (with the host's call, 50000 x 64 to 1000,
 // 50 MB of sums: 22.2 us, 35.6 without slices; 1M x 16 to 1000, 63 MB: 48.4 and 63.0; 300000 x 256 to
-// 300, 105 MB: 115 and 83).
+// 300, 90 MB: 115 and 83).
 constexpr int64_t SLICE_LEAST = 128, SLICE_BYTES = (int64_t)64 << 20;
 constexpr int64_t SLICED_FEW = 48, SLICED_FEW_ELEMENTS = (int64_t)1 << 18;
 

@@ -124,6 +124,17 @@ def test_gradient_of_few_entries(ctx, kind, rows, dim, entries, skew, pad, shift
     test_gradient(ctx, kind, rows, dim, entries, skew, pad, shift)
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,dim,entries,skew,pad,shift", [
+    (1000, 37, 20000, 0, 3, 0), (1024, 5, 1024, 2, 0, 1), (1024, 300, 1500, 3, 0, 0),
+    (1025, 8, 2000, 2, 0, 0), (4096, 6, 5000, 1, 1, 0), (4000, 64, 1025, 3, 0, 0),
+    (4097, 70, 1024, 2, 0, 0), (6000, 1030, 40, 1, 0, 0), (9000, 2060, 200, 0, 0, 0),
+])
+def test_gradient_of_many_entries_or_columns(ctx, kind, rows, dim, entries, skew, pad, shift):
+    """From 1024 entries, or 4 times 64 pieces of 16 bytes, on: one sorted list."""
+    test_gradient(ctx, kind, rows, dim, entries, skew, pad, shift)
+
+
 @pytest.mark.parametrize("rows", [0, 1, 100, 20000])
 @pytest.mark.parametrize("entries", [1, 5000])
 def test_gradient_without_rows_in_any_entry(ctx, rows, entries):
