@@ -490,6 +490,15 @@ struct Sums {
 };
 // Rows that a workgroup of `items` items may look at.
 __host__ __device__ constexpr int held_rows(int items, int whole) { return items + 2 * whole + 2; }
+// Bytes of LDS of a workgroup that holds `most` rows: key, item and, of lists of rows only, place
+// (16 bits, since there are at most 2 * most items).  With the kernel's static ones they are at most
+// the 64 KB that a launch may ask for without more ado.
+constexpr size_t sum_lds(bool dense, size_t most) {
+    return dense ? 4 * (2 * most + AHEAD + 1) : 4 * (3 * most + AHEAD) + 2 * (most + 2);
+}
+static_assert(sum_lds(false, held_rows(MOST_ITEMS, 64)) <= (63 << 10) &&
+                  2 * held_rows(MOST_ITEMS, 64) < (1 << 16),
+              "the largest lists' LDS");
 
 // Rows and entries before an item.  i counts from the first row that the workgroup holds in LDS.
 struct Cut {
@@ -636,7 +645,8 @@ __global__ __launch_bounds__(SUM_THREADS) void k_embed_sum(Sums s) {
     const int items = SUM_WAVES * s.groups * s.per, most = held_rows(items, s.whole);
     uint32_t *key = lds;                             // [row]
     uint32_t *item = key + most;                     // [item]: a row, or an entry
-    uint32_t *place = item + 2 * most + AHEAD;       // [row] its item, where it is not i + key
+    // [row]: its item, where that is not i + key
+    uint16_t *place = reinterpret_cast<uint16_t *>(item + 2 * most + AHEAD);
     const int64_t first = (int64_t)group_id() * (SUM_WAVES * s.groups);
     if (first >= s.workers) return;
     const int64_t d[2] = {first * s.per, min(min(first + SUM_WAVES * s.groups, s.workers) * s.per,
@@ -667,13 +677,13 @@ __global__ __launch_bounds__(SUM_THREADS) void k_embed_sum(Sums s) {
                                                      (i + 1 < held && key[i + 1] != k));
             const uint32_t at = i + before + sum_before<SUM_WAVES>(ends_here, wave_sum, all);
             if (i < held) {
-                place[i] = at;
+                place[i] = (uint16_t)at;
                 item[at] = s.sorted[begin + i].y;
                 if (ends_here) item[at + 1] = ENTRY | k;
             }
             before += all;
         }
-        if (threadIdx.x == 0) place[held] = held + before;
+        if (threadIdx.x == 0) place[held] = (uint16_t)(held + before);
     }
     __syncthreads();
     const int lane = threadIdx.x & 63, group = lane / s.lanes;
@@ -1309,8 +1319,7 @@ template <typename T, int E, bool BASE, bool ONE>
 void sums(hipStream_t st, const Sums &s, int cols) {
     const int64_t each = SUM_WAVES * s.groups;
     const size_t most = (size_t)held_rows((int)each * s.per, s.whole);
-    const size_t lds = sizeof(uint32_t) * std::max((s.dense ? 2 : 4) * most + AHEAD + 1,
-                                                   (size_t)SUM_THREADS * E);
+    const size_t lds = std::max(sum_lds(s.dense, most), sizeof(float) * SUM_THREADS * E);
     hipLaunchKernelGGL((k_embed_sum<T, E, BASE, ONE>),
                        grid_of((s.workers + each - 1) / each, (uint32_t)cols), dim3(SUM_THREADS), lds,
                        st, s);

@@ -1,0 +1,58 @@
+"""Gradients of category vectors in whole numbers whose sums f32 holds without rounding, so that a
+row that is lost, or taken twice, shows however long its entry is."""
+import numpy as np
+import pytest
+
+import device_ops as D
+import macboost_amd as mb
+import model_ops as M
+from test_gpu_category_vectors import _ids
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    c = mb.Context(0)
+    yield c
+    c.close()
+
+
+def _whole(rng, rows, cols, most):
+    return rng.integers(-most, most + 1, (rows, cols), dtype=np.int8).astype(np.float32)
+
+
+def _check(ctx, kind, rows, dim, entries, skew, pad=0, most=4):
+    """Without a base, with one, and on top of what is there."""
+    rng = np.random.default_rng(rows + 7 * dim + entries)
+    ids = _ids(rng, rows, entries, skew, 0.01)
+    kept = (ids >= 0) & (ids < entries)
+    count = np.bincount(ids[kept], minlength=entries)
+    dout, base = _whole(rng, rows, dim, most), _whole(rng, entries, dim, 8)
+    # halves of sums below 2^22, and a base of up to 8: 24 bits
+    assert count.max() * most < 2 ** 22
+    total = np.stack([np.bincount(ids[kept], dout[kept, c], entries) for c in range(dim)], 1)
+    dout[~kept] = np.nan
+    idev, g = ctx.upload(ids), M.Matrix(ctx, dout, kind, pad, fill=np.nan)
+    b = M.Matrix(ctx, base, kind, pad, fill=np.nan)
+    shape = M.embed_shape(rows, entries, dim, kind, g.stride, dim + pad, -0.5)
+    for of, bp in ((0.0, None), (base, b.ptr)):
+        out = M.blank(ctx, entries, dim, kind, pad)
+        ctx.call("mbk_embed_grad", shape, idev, g.ptr, bp, out.ptr)
+        ctx.sync()
+        assert np.array_equal(out.read(), D.rounded((total * -0.5 + of).astype(np.float32), kind))
+    start = np.where(count[:, None] > 0, base, np.float32(np.nan))
+    want = np.where(count[:, None] > 0, total * -0.5 + base, np.nan).astype(np.float32)
+    out = M.Matrix(ctx, start, kind, pad)
+    ctx.call("mbk_embed_grad", shape, idev, g.ptr, out.ptr, out.ptr)
+    ctx.sync()
+    assert np.array_equal(out.read(), D.rounded(want, kind), equal_nan=True)
+
+
+@pytest.mark.parametrize("kind,rows,dim,entries,skew", [
+    ("f32", 1048577, 4, 2000, 0), ("f32", 1048576, 1, 1024, 1), ("bf16", 1048580, 2, 70000, 0.5),
+    ("bf16", 1100003, 8, 2000, 0), ("f32", 4300000, 13, 2000, 1),
+])
+def test_the_longest_lists_of_a_workgroup(ctx, kind, rows, dim, entries, skew):
+    """From 2^20 rows of one to four pieces on, and their sort of several chunks a workgroup."""
+    _check(ctx, kind, rows, dim, entries, skew)
