@@ -399,8 +399,9 @@ int mbk_expert_combine_grad(mbk_context *ctx, const mbk_expert_plan *plan,
  * rows are neither read nor written; else every entry is written.  What dout holds of rows whose
  * id is outside reaches nothing.
  * Sums are f32, in runs of at most 256 rows and then over the runs, rounded once with
- * base; their order is fixed by the shape, the ids and the number of compute units.  What lies
- * between rows of out and dtable stays as it is; outputs overlap no input but base. */
+ * base; their order is fixed by the shape, the ids, whether base is dtable and the number of compute
+ * units.  What lies between rows of out and dtable stays as it is; outputs overlap no input but
+ * base. */
 typedef struct {
     int64_t rows;                /* 0..2^31-256 */
     int64_t entries;             /* 1..2^31-256 */

@@ -603,9 +603,10 @@ __device__ __forceinline__ void walk(const Sums &s, const uint32_t *item, int p,
 #pragma unroll
         for (int q = 0; q < AHEAD; ++q) {
             const bool is_row = what[q] < ENTRY;
-            // without branches: what has nothing to read takes a row or an entry that is there
+            // without branches: what has nothing to read takes row 0, or entry 0 where there are no
+            // rows, which is never in place
             if constexpr (BASE) {
-                const T *at = is_row ? dout : what[q] == NOTHING ? dtable : base;
+                const T *at = is_row ? dout : what[q] == NOTHING ? some_row : base;
                 const uint32_t which = what[q] == NOTHING ? 0 : what[q] & ~ENTRY;
                 v[q] = *reinterpret_cast<const Run<T, E> *>(
                     at + which * (is_row ? s.row_stride : s.table_stride));
