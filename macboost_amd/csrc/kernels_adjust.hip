@@ -75,7 +75,7 @@ __global__ __launch_bounds__(THREADS) void k_adjust(AdjustCall c, int32_t parts)
                 if (!((bits >> e) & 1u)) z[x][e] = -__builtin_inff();
         }
         if (i + 4 <= here) {
-            put(reinterpret_cast<Run *>(out + i), z[x], c.streamed);
+            put(out + i, z[x], c.streamed);
         } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e)

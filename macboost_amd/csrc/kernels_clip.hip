@@ -68,7 +68,7 @@ __device__ __forceinline__ void scale(const ClipPiece &p, double by, bool stream
 #pragma unroll
             for (int e = 0; e < E; ++e) x[e] = (T)(float)((double)v[q][e] * by);
             if (n[q] >= E) {
-                put(reinterpret_cast<Run<T, E> *>(o + at[q]), x, streamed);
+                put(o + at[q], x, streamed);
             } else {
 #pragma unroll
                 for (int e = 0; e < E; ++e)

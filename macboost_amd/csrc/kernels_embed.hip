@@ -38,7 +38,7 @@ __device__ __forceinline__ void store(T *p, int n, const float (&f)[E], bool str
             Run<T, E> v;
 #pragma unroll
             for (int e = 0; e < E; ++e) v[e] = (T)f[e];
-            put(reinterpret_cast<Run<T, E> *>(p), v, streamed);
+            put(p, v, streamed);
             return;
         }
 #pragma unroll
@@ -737,7 +737,7 @@ __global__ __launch_bounds__(SUM_THREADS) void k_embed_sum(Sums s) {
             for (int e = 0; e < E; ++e)
                 out[e] = (T)__builtin_fmaf(s.scale, acc[e], BASE ? to_f32(v[e]) : 0.0f);
             if (!idle)
-                put(reinterpret_cast<Run<T, E> *>(dtable + entry * s.table_stride), out, s.streamed);
+                put(dtable + entry * s.table_stride, out, s.streamed);
         }
     });
     if (!idle && chunk == 0) s.open[worker] = to.open ? to.e : NOTHING;
@@ -955,7 +955,7 @@ __global__ __launch_bounds__(SUM_THREADS) void k_embed_few(Sums s, Pass p, int32
 #pragma unroll
         for (int e = 0; e < E; ++e)
             out[e] = (T)__builtin_fmaf(s.scale, acc[e], BASE ? to_f32(b[e]) : 0.0f);
-        put(reinterpret_cast<Run<T, E> *>(dtable + entry * s.table_stride), out, s.streamed);
+        put(dtable + entry * s.table_stride, out, s.streamed);
     };
 
     if ((int)blockIdx.x >= lists) {

@@ -331,7 +331,7 @@ __device__ __forceinline__ void put_scores(const FourbitCall &c, int64_t row, in
         V out;
 #pragma unroll
         for (int i = 0; i < E; ++i) out[i] = v[i];
-        put(reinterpret_cast<V *>(to), out, streamed);
+        put(to, out, streamed);
     } else {
 #pragma unroll
         for (int i = 0; i < E; ++i)

@@ -60,18 +60,22 @@ hipError_t launch_expert_combine_grad(hipStream_t s, const ExpertPlan &p,
 // added: 70 us by ordinary stores, 57 so).
 constexpr int64_t STREAMED = (int64_t)32 << 20;
 #ifdef __HIP_DEVICE_COMPILE__
-// The empty statements keep the compiler from making one ordinary store of both.
-template <typename V> __device__ __forceinline__ void put(V *to, const V &v, bool streamed) {
+// Stores a vector at any address that holds one of its elements.  (A template's argument leaves a
+// type's alignment behind, so that it is given here.)  The empty statements keep the compiler from
+// making one ordinary store of both.
+template <typename V> __device__ __forceinline__ void put(void *to, const V &v, bool streamed) {
+    typedef V Loose __attribute__((aligned(sizeof(v[0]))));
+    Loose *at = static_cast<Loose *>(to);
     if (streamed) {
-        __builtin_nontemporal_store(v, to);
+        __builtin_nontemporal_store(v, at);
     } else {
         asm volatile("" ::: "memory");
-        *to = v;
+        *at = v;
         asm volatile("" ::: "memory");
     }
 }
 #else
-template <typename V> __device__ void put(V *, const V &, bool) {}
+template <typename V> __device__ void put(void *, const V &, bool) {}
 #endif
 
 // ---- category vectors ---------------------------------------------------------
