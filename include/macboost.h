@@ -391,7 +391,8 @@ int mbk_expert_combine_grad(mbk_context *ctx, const mbk_expert_plan *plan,
 
 /* ---- category vectors.  No counterpart in the reference.  A column of many categories gives
  * each row's outputs a vector of its category's, trained by gradient beside the forests.  All
- * arrays are device memory.
+ * arrays are device memory.  Arrays of these calls and of those behind them, to mbk_adjust, lie at
+ * multiples of their elements' size: another address is refused.
  * mbk_embed: out[row] = base[row] + scale * table[ids[row]]; an id outside [0, entries) adds
  * nothing.  base (NULL: 0) lies as out does and may be out itself.
  * mbk_embed_grad: dtable[v] = base[v] + scale * the sum of dout[row] over the rows with

@@ -8,6 +8,7 @@
 #include <algorithm>
 #include <cmath>
 #include <functional>
+#include <initializer_list>
 #include <vector>
 
 #include "../../include/macboost.h"
@@ -30,6 +31,14 @@ bool is_bf16(int32_t type) {
     need(type == MBK_F32 || type == MBK_BF16, "type must be MBK_F32 or MBK_BF16");
     return type == MBK_BF16;
 }
+
+// Every one a multiple of `size` bytes (NULL is).
+void need_multiple(size_t size, std::initializer_list<const void *> arrays) {
+    for (const void *p : arrays)
+        need(reinterpret_cast<uintptr_t>(p) % size == 0,
+             "arrays must be at multiples of their elements' size");
+}
+size_t size_of(bool bf16) { return bf16 ? 2 : 4; }
 
 mbk::XentCall xent_call(const mbk_xent_shape *sh, const void *h,
                         const void *w, const float *bias, const int32_t *labels,
@@ -254,6 +263,8 @@ int mbk_embed(mbk_context *ctx, const mbk_embed_shape *shape, const void *table,
     return mb::guarded(err, [&]() -> int {
         mbk::EmbedCall c = embed_call(shape, ids, base);
         need(table && (!c.rows || (ids && out)), "null argument");
+        need_multiple(size_of(c.bf16), {table, base, out});
+        need_multiple(sizeof *ids, {ids});
         need(ctx != nullptr, "null kernel-seam context");
         if (!c.rows) return 0;
         c.table = table;
@@ -269,6 +280,8 @@ int mbk_embed_grad(mbk_context *ctx, const mbk_embed_shape *shape, const int32_t
     return mb::guarded(err, [&]() -> int {
         mbk::EmbedCall c = embed_call(shape, ids, base);
         need(dtable && (!c.rows || (ids && dout)), "null argument");
+        need_multiple(size_of(c.bf16), {dout, base, dtable});
+        need_multiple(sizeof *ids, {ids});
         need(ctx != nullptr, "null kernel-seam context");
         if (!c.rows && base == dtable) return 0;
         c.dout = dout;
@@ -298,7 +311,7 @@ int mbk_tensors_create(mbk_context *ctx, const mbk_tensor *list, int32_t count, 
                  "gradients must have at most 2^38 elements together");
             elements += t.rows * t.cols;
             need(t.grad || !t.rows || !t.cols, "null gradient");
-            const uintptr_t size = t.type == MBK_BF16 ? 2 : 4;
+            const size_t size = size_of(t.type == MBK_BF16);
             need(reinterpret_cast<uintptr_t>(t.grad) % size == 0 &&
                      reinterpret_cast<uintptr_t>(t.out) % size == 0,
                  "grad and out must be multiples of their elements' size");
@@ -360,6 +373,7 @@ int mbk_grad_clip(mbk_context *ctx, mbk_tensors *list, float max_norm, float *no
     return mb::guarded(err, [&]() -> int {
         need(max_norm >= 0.0f, "max_norm must be >= 0");
         need(list && norm, "null argument");
+        need_multiple(sizeof *norm, {norm});
         need(ctx != nullptr, "null kernel-seam context");
         std::lock_guard<std::mutex> lock(mb::context_scratch_mutex(ctx));
         const auto &lists = mb::context_lists(ctx);
@@ -390,6 +404,7 @@ int mbk_fourbit_pack(mbk_context *ctx, const mbk_fourbit_shape *shape, int32_t t
         need(w_stride >= s.dim && w_stride <= MOST_STRIDE, "w_stride must be in dim..2^40");
         const bool bf16 = is_bf16(type);
         need(w != nullptr, "null argument");
+        need_multiple(size_of(bf16), {w});
         need_packed(packed);
         need(ctx != nullptr, "null kernel-seam context");
         mb::OnDevice here(mb::context_device(ctx));
@@ -411,6 +426,8 @@ int mbk_fourbit_scores(mbk_context *ctx, const mbk_fourbit_shape *shape, int64_t
              "score_stride must be in classes..2^40");
         c.bf16 = is_bf16(type);
         need(!rows || (h && scores), "null argument");
+        need_multiple(size_of(c.bf16), {h});
+        need_multiple(sizeof *scores, {bias, scores});
         need_packed(packed);
         need(ctx != nullptr, "null kernel-seam context");
         if (!rows) return 0;
@@ -460,6 +477,7 @@ int mbk_adjust(mbk_context *ctx, const mbk_adjust_shape *shape, const float *sco
         need(std::isfinite(sh->presence) && std::isfinite(sh->frequency),
              "presence and frequency must be finite");
         need(!sh->rows || (scores && out && (!sh->history || ids)), "null argument");
+        need_multiple(sizeof *scores, {scores, ids, lengths, bias, allowed, out});
         need(scores != out || sh->score_stride == sh->out_stride,
              "scores that are out must have its stride");
         need(ctx != nullptr, "null kernel-seam context");
