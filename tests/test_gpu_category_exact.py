@@ -56,3 +56,32 @@ def _check(ctx, kind, rows, dim, entries, skew, pad=0, most=4):
 def test_the_longest_lists_of_a_workgroup(ctx, kind, rows, dim, entries, skew):
     """From 2^20 rows of one to four pieces on, and their sort of several chunks a workgroup."""
     _check(ctx, kind, rows, dim, entries, skew)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,dim,entries,skew", [
+    # slices, of one entry, of few and of many, narrow and wide
+    (50000, 70, 1, 0), (262145, 8, 5, 0), (1000000, 1, 70, 0.5), (300000, 2, 400, 2),
+    (70001, 36, 1023, 2), (2000, 513, 9, 1), (1100, 257, 2, 0), (6000, 250, 3, 0),
+    # one launch, whose longest entries have workgroups of their own
+    (1024, 300, 1500, 3), (1000, 20, 20000, 2), (1024, 1030, 1, 0),
+    # a sort in one workgroup, and longer ones
+    (4000, 64, 1025, 3), (4096, 2, 5000, 2), (20000, 300, 1100, 2), (100000, 37, 1500, 1.5),
+    (200000, 16, 2000, 2), (600000, 2, 3000, 1.5), (600000, 5, 3000, 3),
+    # rows of several wavefronts
+    (9000, 2064, 30, 1), (6000, 1030, 40, 2), (9000, 2060, 200, 3),
+])
+def test_long_entries(ctx, kind, rows, dim, entries, skew):
+    _check(ctx, kind, rows, dim, entries, skew, pad=rows % 3)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_sums_of_slices_beyond_their_limit(ctx, kind):
+    """300 entries of 256 columns, whose slices' sums would take 90 MB: one sorted list."""
+    _check(ctx, kind, 300000, 256, 300, 1)
+
+
+@pytest.mark.parametrize("entries", [1, 1500])
+def test_one_entry_of_2_to_21_rows(ctx, entries):
+    """All rows but a few to one entry: more than 1,000 sums of slices or of workgroups."""
+    _check(ctx, "f32", (1 << 21) + 1, 5, entries, 40, most=1)
