@@ -31,7 +31,10 @@ def _check(ctx, kind, rows, dim, entries, skew, pad=0, most=4):
     dout, base = _whole(rng, rows, dim, most), _whole(rng, entries, dim, 8)
     # halves of sums below 2^22, and a base of up to 8: 24 bits
     assert count.max() * most < 2 ** 22
-    total = np.stack([np.bincount(ids[kept], dout[kept, c], entries) for c in range(dim)], 1)
+    if dim > entries:
+        total = np.stack([dout[ids == e].sum(0, dtype=np.float64) for e in range(entries)])
+    else:
+        total = np.stack([np.bincount(ids[kept], dout[kept, c], entries) for c in range(dim)], 1)
     dout[~kept] = np.nan
     idev, g = ctx.upload(ids), M.Matrix(ctx, dout, kind, pad, fill=np.nan)
     b = M.Matrix(ctx, base, kind, pad, fill=np.nan)
