@@ -51,7 +51,8 @@ __device__ __forceinline__ void store(T *p, int n, const float (&f)[E], bool str
 // elements; a workgroup takes 256 * LOOKUP pieces of all the rows' in their order, LOOKUP a
 // thread, so that short rows leave no lane idle and each thread has LOOKUP rows on the way.
 // Bound by memory: 65536 x 1024 bf16 with a base take 57 us, 380 MB at 6.7 TB/s with popular
-// vectors out of the caches; 64 x 37 f32 2.8, a launch and two reads one after the other.
+// vectors out of the caches, and 73 in place; 64 x 37 f32 2.8, a launch and two reads one after the
+// other.
 // ---------------------------------------------------------------------------
 constexpr int LOOKUP = 4;
 
@@ -638,7 +639,8 @@ __device__ __forceinline__ void walk(const Sums &s, const uint32_t *item, int p,
 // the piece before has too: both lanes write the same.
 // BASE: dtable has a base.  ONE: one worker a wavefront, whose items are the same in all lanes.
 // Bound by memory: 1M x 64 f32 rows in any order to 100000 entries take 69 us, 282 MB at 4.1 TB/s
-// in pieces of 256 bytes; 16384 x 1024 bf16 on top of 65536 entries 56.
+// in pieces of 256 bytes; 16384 x 1024 bf16 on top of 65536 entries 56.  In place 78 and 21, and 60
+// where 1030 columns leave 2 bytes a lane.
 template <typename T, int E, bool BASE, bool ONE>
 __global__ __launch_bounds__(SUM_THREADS) void k_embed_sum(Sums s) {
     extern __shared__ uint32_t lds[];
@@ -903,7 +905,7 @@ __global__ __launch_bounds__(JOIN_THREADS) void k_embed_join(Sums s) {
 
 // ---------------------------------------------------------------------------
 // Up to FEW_ROWS rows to many entries: one launch, bound by the chain of the sort (6 us) and the reads behind it
-// (1000 x 64 f32 to 60000 entries 17.9 us with the host's call).  Every workgroup sorts all of them for
+// (1000 x 64 f32 to 60000 entries 19.8 us with the host's call).  Every workgroup sorts all of them for
 // itself; the first `lists` take the merged list as above, without the entries of more than `whole`
 // rows, and each of the others one of those.
 // ---------------------------------------------------------------------------
@@ -1223,10 +1225,10 @@ struct GradShape {
     int64_t slices;                  // of few entries, g.whole rows each; 0: none
 };
 
-// Slices: as many as CUs, down to 128 rows (10000 x 64 to 1000: 15.0 us, 19.5 by 64 rows and 18.5 by
+// Slices: as many as CUs, down to 128 rows (10000 x 64 to 1000: 14.3 us, 18.2 by 64 rows and 17.4 by
 // 512), while their sums do not outweigh the longer sort (with the host's call, 50000 x 64 to 1000,
-// 50 MB of sums: 22.2 us, 35.6 without slices; 1M x 16 to 1000, 63 MB: 48.4 and 63.0; 300000 x 256 to
-// 300, 90 MB: 115 and 83).
+// 50 MB of sums: 21.0 us, 36.8 without slices; 1M x 16 to 1000, 63 MB: 49.2 and 63.7; 300000 x 256 to
+// 300, 90 MB: 113 and 93).
 constexpr int64_t SLICE_LEAST = 128, SLICE_BYTES = (int64_t)64 << 20;
 constexpr int64_t SLICED_FEW = 48, SLICED_FEW_ELEMENTS = (int64_t)1 << 18;
 
@@ -1272,7 +1274,7 @@ GradShape grad_shape(const EmbedCall &c) {
     g.whole = c.rows <= 64 ? 64 : g.items;           // few rows: nothing to join
     g.workers = (items + per - 1) / per;
     // few rows: sorted again by each workgroup, which pays up to where there are very many of them
-    // (1000 x 64 f32 to 60,000 entries 17.9 us, 28.0 by three launches; to 1M 64 and 74)
+    // (1000 x 64 f32 to 60,000 entries 19.8 us, 27.3 by three launches; to 1M 70.5 and 73.2)
     g.lists = (g.workers + (int64_t)SUM_WAVES * g.groups - 1) / ((int64_t)SUM_WAVES * g.groups);
     g.few = c.rows >= 1 && c.rows <= FEW_ROWS && g.lists * g.cols <= 64 * (int64_t)c.num_cus;
     if (g.few) {
@@ -1283,8 +1285,8 @@ GradShape grad_shape(const EmbedCall &c) {
         FEW_ROWS, std::max<int64_t>(SLICE_LEAST, (c.rows * g.cols / c.num_cus + 63) / 64 * 64));
     const int64_t slices = (c.rows + slice - 1) / slice;
     // of up to FEW_ROWS rows where one launch takes longer than two: not of the least, nor where many
-    // entries are written twice (300 x 37 to 300 entries 11.5 us, 16.0 by one; 1000 x 1000 to one 12.1
-    // and 19.6; 32 x 1024 to 20 10.9 and 9.1; 200 x 512 to 1000 16.7 and 14.7)
+    // entries are written twice (300 x 37 to 300 entries 12.0 us, 16.0 by one; 1000 x 1000 to one 12.5
+    // and 25.0; 32 x 1024 to 20 10.9 and 9.3; 200 x 512 to 1000 16.4 and 13.6)
     const bool sliced =
         !g.few || (c.rows >= SLICED_FEW && c.entries * c.dim <= SLICED_FEW_ELEMENTS);
     if (sliced && c.rows >= 1 && c.entries < (1 << MOST_BITS) && g.cols <= 4 &&
@@ -1438,8 +1440,8 @@ hipError_t launch_embed_grad(hipStream_t st, const EmbedCall &c, char *scratch) 
     s.per = g.items;
     s.whole = g.whole;
     s.dense = g.dense;
-    // whole lines only: narrower rows' are made whole by the caches (16M entries of 4 f32 704 us past
-    // them, 134 so; 2M of 32, lines of 128 bytes, 93 past them and 97)
+    // whole lines only: narrower rows' are made whole by the caches (1000 rows to 16M entries of 4 f32
+    // 697 us past them, 184 so; 100000 to 2M of 32, lines of 128 bytes, 104 past them and 120)
     s.streamed = g.dense && g.lanes * g.elements * (c.bf16 ? 2 : 4) >= 128 &&
                  c.entries * c.dim * (c.bf16 ? 2 : 4) > STREAMED;
     s.row_stride = c.row_stride;

@@ -65,8 +65,8 @@ __device__ __forceinline__ void eight(const T *row, int k, int dim, bool wide, f
 }
 
 // A workgroup a tile of classes, a wavefront a block of it at a time, in the lanes that hold its
-// codes: the scales first, for the class's exponent, and then all again.  100000 x 1024 bf16 91
-// us, f32 153, the second reading from L2.
+// codes: the scales first, for the class's exponent, and then all again.  100000 x 1024 bf16 90
+// us, f32 149, the second reading from L2.
 constexpr int PACK_WAVES = 4;
 template <typename T, int PER>
 __global__ __launch_bounds__(64 * PACK_WAVES) void k_fourbit_pack(
@@ -358,7 +358,7 @@ __device__ __forceinline__ void write_scores(const FourbitCall &c, const float4v
 // profiler, of which 4 are the columns and about 4 unpacking that does not hide behind the stream;
 // vector units busy 28 %, the matrix cores 5.  1 x 64 by 1000: 5.3 us, latency.
 constexpr int FEW_WAVES = 8, FEW_THREADS = 64 * FEW_WAVES;
-constexpr int FEW_HEAD = 1024;       // bytes of LDS before the columns: exponents of up to 64 rows
+constexpr int FEW_HEAD = 1024;       // bytes of LDS before the columns, for up to 32 rows' exponents
 constexpr int KEPT = 4;              // eights of h that a thread keeps from the maximum on
 template <typename T, int CT, int PER>
 __global__ __launch_bounds__(FEW_THREADS, 4) void k_fourbit_few(FourbitCall c, int32_t ks,
@@ -525,7 +525,8 @@ __global__ __launch_bounds__(FEW_THREADS, 4) void k_fourbit_few(FourbitCall c, i
 // columns of a block of W, copied to LDS while the block before is worked on.
 // Bound by issue: a block's unpacking is shared by CT products only, and a wavefront waits at each
 // block for its columns.  201 x 777 f32 by 50003 classes of groups of 32: 50 us, 0.7 PFLOP/s of padded
-// products of two terms; matrix cores busy 29 %, vector units 38, wavefronts waiting 34.
+// products of two terms; matrix cores busy 29 %, vector units 38, wavefronts waiting 34.  bf16 31,
+// and 512 x 1024 by 32000 40, 0.84 PFLOP/s.
 typedef __attribute__((address_space(1))) void global_void;
 typedef __attribute__((address_space(3))) void lds_void;
 constexpr int WIDE_WAVES = 4, WIDE_TILES = 4;
